@@ -41,7 +41,7 @@ enum {
 enum { SMOE_ST_OK = 0, SMOE_ST_TIMEOUT_PRODUCER = 1, SMOE_ST_TIMEOUT_MMA = 2, SMOE_ST_TIMEOUT_EPILOGUE = 3 };
 
 /* dtype codes for tensors whose type the caller chooses */
-enum { SMOE_F32 = 0, SMOE_BF16 = 1, SMOE_I32 = 2, SMOE_I64 = 3 };
+enum { SMOE_F32 = 0, SMOE_BF16 = 1, SMOE_I32 = 2, SMOE_I64 = 3, SMOE_F16 = 4 };
 
 /* Library version, for the loader to check that it found the right build. */
 int smoe_abi_version(void);
@@ -427,6 +427,39 @@ int smoe_layer_backward_dx(const void* w1, void* meta, const void* scratch, void
                            int H, int I, int N1, int E, int K, int* status, void* stream);
 int smoe_layer_backward_weights(const void* x, const void* dout, void* meta, const void* scratch, void* dw1, void* dw2,
                                 int T, int H, int I, int N1, int E, int K, int* status, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Tokens sorted by expert and back, for experts that are not this library's GEMMs.  No counterpart among the reference's
+ * operators, whose GEMMs gather and scatter (sonicmoe/functional/__init__.py:19-82 makes the index vectors).
+ * ------------------------------------------------------------------------------------------- */
+
+/* Rows that the sorted layout of n pairs needs whatever the load: an expert that has pairs is padded by less than align. */
+long long smoe_token_permutation_rows(long long n, int E, int align);
+size_t smoe_token_permutation_workspace_bytes(long long n, int E);
+/* The stable sort of the T * K (token, slot) pairs by expert, expert_idx (T,K) SMOE_I32 or SMOE_I64; an index outside [0,E)
+ * drops its pair.  expert_frequency (E): pairs of each expert; expert_frequency_offset (E+1): its first row, a multiple of
+ * `align`, and the end of the last; x_gather_idx, s_scatter_idx (smoe_token_permutation_rows): token and flat slot of each row,
+ * -1 for a row without a pair; s_reverse_scatter_idx (T,K): row of each pair, -1 for a dropped one.  E <= 4096, T * K < 2^31 -
+ * 2^16.  workspace: smoe_token_permutation_workspace_bytes(T * K, E) bytes (0: may be null). */
+int smoe_token_permutation(const void* expert_idx, int idx_dtype, int T, int K, int E, int align, int* expert_frequency,
+                           int* expert_frequency_offset, int* x_gather_idx, int* s_scatter_idx,
+                           int* s_reverse_scatter_idx, void* workspace, void* stream);
+
+/* Row movers over R sorted rows of H values (SMOE_F32, SMOE_BF16 or SMOE_F16), fp32 arithmetic, one rounding.  ld: values from
+ * one row of the input to the next (0: the same row for all); outputs are packed.  weights (T,K): SMOE_F32, SMOE_BF16, SMOE_F16
+ * or NULL = 1.  A row index outside [0,R) counts as -1.
+ *   permute_rows:            rows[s_reverse_scatter_idx[t,k]] = weights[t,k] * x[t]; zeros where s_scatter_idx is negative
+ *   unpermute_rows:          out[t] = sum over k of weights[t,k] * rows[s_reverse_scatter_idx[t,k]], in the order of k
+ *   unpermute_rows_backward: drows as permute_rows of dout, dweights[t,k] = <dout[t], rows[s_reverse_scatter_idx[t,k]]> (0 for
+ *                            a dropped pair), of the type of weights */
+int smoe_permute_rows(const void* x, long long ld, void* rows, int dtype, const void* weights, int weights_dtype,
+                      const int* s_reverse_scatter_idx, const int* s_scatter_idx, int T, int K, int H, long long R,
+                      void* stream);
+int smoe_unpermute_rows(const void* rows, long long ld, void* out, int dtype, const void* weights, int weights_dtype,
+                        const int* s_reverse_scatter_idx, int T, int K, int H, long long R, void* stream);
+int smoe_unpermute_rows_backward(const void* dout, long long dout_ld, const void* rows, long long ld, void* drows, int dtype,
+                                 const void* weights, void* dweights, int weights_dtype, const int* s_reverse_scatter_idx,
+                                 const int* s_scatter_idx, int T, int K, int H, long long R, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Expert parallelism over peer memory (one node, NVLink / NVSwitch).  The reference has no distributed

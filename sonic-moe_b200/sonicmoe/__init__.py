@@ -6,6 +6,7 @@ Exports match the reference package (sonicmoe/__init__.py:5-8).
 from .count_cumsum import count_cumsum
 from .enums import ActivationType, KernelBackendMoE
 from .functional import enable_quack_gemm, moe_general_routing_inputs, moe_TC_softmax_topk_layer
+from .functional.permutation import TokenPermutation, permute_tokens, token_permutation, unpermute_tokens
 from .moe import MoE
 from ._lib import SonicMoEError, check_status
 
@@ -20,4 +21,9 @@ __all__ = [
     # beyond the reference's exports: the status check of the bounded-wait GEMM kernels
     "SonicMoEError",
     "check_status",
+    # and tokens sorted by expert and back, for experts of the caller's own
+    "TokenPermutation",
+    "token_permutation",
+    "permute_tokens",
+    "unpermute_tokens",
 ]

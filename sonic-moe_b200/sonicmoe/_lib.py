@@ -16,7 +16,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsonicmoe_b200.so")
 
-SMOE_F32, SMOE_BF16, SMOE_I32, SMOE_I64 = 0, 1, 2, 3
+SMOE_F32, SMOE_BF16, SMOE_I32, SMOE_I64, SMOE_F16 = 0, 1, 2, 3, 4
 
 _ERRORS = {
     -1: "unsupported or inconsistent sizes",
@@ -101,6 +101,12 @@ SIGNATURES: dict[str, tuple] = {
     "smoe_layer_backward_act": (I, [P, P, P, P, P, P, I, I, P, P, P, P, P, P, P, I, I, I, I, I, I, I, P, P]),
     "smoe_layer_backward_dx": (I, [P, P, P, P, P, I, I, I, I, I, I, I, P, P]),
     "smoe_layer_backward_weights": (I, [P, P, P, P, P, P, I, I, I, I, I, I, P, P]),
+    "smoe_token_permutation_rows": (LL, [LL, I, I]),
+    "smoe_token_permutation_workspace_bytes": (c_size_t, [LL, I]),
+    "smoe_token_permutation": (I, [P, I, I, I, I, I, P, P, P, P, P, P, P]),
+    "smoe_permute_rows": (I, [P, LL, P, I, P, I, P, P, I, I, I, LL, P]),
+    "smoe_unpermute_rows": (I, [P, LL, P, I, P, I, P, I, I, I, LL, P]),
+    "smoe_unpermute_rows_backward": (I, [P, LL, P, LL, P, I, P, P, I, P, P, I, I, I, LL, P]),
     "smoe_peer_alloc": (I, [c_size_t, P]),
     "smoe_peer_free": (I, [P]),
     "smoe_peer_export": (I, [P, P]),

@@ -1,0 +1,190 @@
+"""Tokens sorted by expert and back: for experts that are not this library's own GEMMs (other layers, adapters, 8-bit
+products), which take their rows expert by expert.
+
+    p = token_permutation(topk_indices, E)           # stable sort of the (token, slot) pairs by expert
+    rows = permute_tokens(x, p)                      # rows[r] = x[token of row r]
+    y = experts(rows, p.expert_frequency_offset)     # expert e has rows [offset[e], offset[e] + expert_frequency[e])
+    o = unpermute_tokens(y, p, scores)               # o[t] = sum over k of scores[t, k] y[row of pair (t, k)]
+
+Both directions have gradients (the sums over a token's rows, the rows' dot products for the scores).  A pair whose expert is
+outside [0, E) (-1, say: a token beyond an expert's capacity, a padding token) is dropped: it has no row, adds nothing, and its
+score is not read.  ``align`` starts every expert's rows at a multiple of it; rows without a pair are zeros in `permute_tokens`,
+ignored by `unpermute_tokens` whatever they hold, and get zero gradients.
+
+fp32, bf16 and fp16 rows of any width; sums in fp32 in the order of k, rounded once: the same bits every time.  The number of
+rows follows from the shapes alone, so nothing here waits for the device and all of it can be captured in a graph.
+The reference has no such operators: its GEMMs gather and scatter (sonicmoe/functional/__init__.py:19-82 makes the indices).
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _lib
+from .._lib import check, lib, ptr, stream_ptr
+
+_ROW_TYPES = {torch.float32: _lib.SMOE_F32, torch.bfloat16: _lib.SMOE_BF16, torch.float16: _lib.SMOE_F16}
+_MAX_EXPERTS = 4096
+
+
+@dataclass
+class TokenPermutation:
+    """Index vectors of one routing decision (int32, contiguous, on the tokens' device; the names are those of `Route`)."""
+
+    expert_frequency: torch.Tensor         # (E,)   pairs of each expert
+    expert_frequency_offset: torch.Tensor  # (E+1,) first row of each expert, multiples of `align`; [E]: end of the last
+    x_gather_idx: torch.Tensor             # (rows,) token of each row, -1: none
+    s_scatter_idx: torch.Tensor            # (rows,) flat (token, slot) pair of each row, -1: none
+    s_reverse_scatter_idx: torch.Tensor    # (T, K) row of each pair, -1: dropped
+    align: int = 1
+
+    @property
+    def num_rows(self) -> int:
+        return self.s_scatter_idx.numel()
+
+
+def token_permutation(topk_indices: torch.Tensor, E: int, align: int = 1) -> TokenPermutation:
+    """The stable sort by expert of the pairs of ``topk_indices`` (T, K), int32 or int64: pairs of one expert stay in the order
+    of (token, slot).  The number of rows is T K, or with ``align`` > 1 what every load fits into."""
+    if topk_indices.dim() != 2:
+        raise ValueError(f"topk_indices has to be (T, K), got {tuple(topk_indices.shape)}")
+    if topk_indices.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"topk_indices has to be int32 or int64, got {topk_indices.dtype}")
+    T, K = topk_indices.shape
+    n = T * K
+    if not 0 < E <= _MAX_EXPERTS or align <= 0 or K == 0:
+        raise ValueError(f"1 <= E <= {_MAX_EXPERTS}, 1 <= K and 1 <= align are needed, got E {E}, K {K}, align {align}")
+    rows = lib.smoe_token_permutation_rows(n, E, align)
+    if rows + E * align >= 2 ** 31 or n >= 2 ** 31 - 2 ** 16:
+        raise ValueError(f"{n} pairs of {E} experts aligned to {align} do not fit into 32-bit row numbers")
+    _lib.require_cuda(topk_indices, "topk_indices")
+    idx = topk_indices.detach().contiguous()
+    dev = idx.device
+    with _lib.on_device(dev):
+        freq, off, gather, scatter, reverse = torch.empty(2 * E + 1 + 2 * rows + n, dtype=torch.int32, device=dev).split(
+            (E, E + 1, rows, rows, n))
+        ws = lib.smoe_token_permutation_workspace_bytes(n, E)
+        ws = _lib.workspace(ws, dev) if ws else None
+        check(lib.smoe_token_permutation(
+            idx.data_ptr(), _lib.dtype_code(idx.dtype), T, K, E, align, freq.data_ptr(), off.data_ptr(), gather.data_ptr(),
+            scatter.data_ptr(), reverse.data_ptr(), ptr(ws), stream_ptr(dev)), "token_permutation")
+    return TokenPermutation(freq, off, gather, scatter, reverse.view(T, K), align)
+
+
+def _check_permutation(p: TokenPermutation, dev: torch.device) -> None:
+    pair, row = p.s_reverse_scatter_idx, p.s_scatter_idx
+    if pair.dim() != 2 or row.dim() != 1 or pair.shape[1] == 0:
+        raise ValueError("a permutation's s_reverse_scatter_idx is (T, K) and its s_scatter_idx (rows,)")
+    for t in (pair, row):
+        if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"a permutation's index vectors are contiguous int32 tensors on {dev}")
+
+
+def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
+    """A 2D tensor of a known type whose rows are contiguous (their distance may be anything)."""
+    if t.dim() != 2:
+        raise ValueError(f"{name} has to be 2-dimensional, got {tuple(t.shape)}")
+    if t.dtype not in _ROW_TYPES:
+        raise TypeError(f"{name} has to be fp32, bf16 or fp16, got {t.dtype}")
+    if t.shape[1] == 0:
+        raise ValueError(f"{name} has rows of no values")
+    return t if t.stride(1) == 1 and t.stride(0) >= 0 else t.contiguous()
+
+
+def _spread(x, p: TokenPermutation, scores):
+    x = _rows(x, "x")
+    (T, K), R, H, dev = p.s_reverse_scatter_idx.shape, p.num_rows, x.shape[1], x.device
+    with _lib.on_device(dev):
+        rows = torch.empty(R, H, dtype=x.dtype, device=dev)
+        check(lib.smoe_permute_rows(
+            x.data_ptr(), x.stride(0), rows.data_ptr(), _ROW_TYPES[x.dtype], ptr(scores),
+            0 if scores is None else _ROW_TYPES[scores.dtype], p.s_reverse_scatter_idx.data_ptr(), p.s_scatter_idx.data_ptr(),
+            T, K, H, R, stream_ptr(dev)), "permute_rows")
+    return rows
+
+
+def _collect(rows, p: TokenPermutation, scores):
+    rows = _rows(rows, "rows")
+    (T, K), R, H, dev = p.s_reverse_scatter_idx.shape, p.num_rows, rows.shape[1], rows.device
+    with _lib.on_device(dev):
+        out = torch.empty(T, H, dtype=rows.dtype, device=dev)
+        check(lib.smoe_unpermute_rows(
+            rows.data_ptr(), rows.stride(0), out.data_ptr(), _ROW_TYPES[rows.dtype], ptr(scores),
+            0 if scores is None else _ROW_TYPES[scores.dtype], p.s_reverse_scatter_idx.data_ptr(), T, K, H, R,
+            stream_ptr(dev)), "unpermute_rows")
+    return out
+
+
+class _Permute(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p):
+        ctx.save_for_backward(p.s_reverse_scatter_idx, p.s_scatter_idx)
+        ctx.p = p
+        return _spread(x, p, None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, drows):
+        ctx.saved_tensors  # raises where an index vector was written to since
+        return _collect(drows, ctx.p, None), None
+
+
+class _Unpermute(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, p, scores):
+        ctx.save_for_backward(p.s_reverse_scatter_idx, p.s_scatter_idx, scores,
+                              rows if scores is not None and ctx.needs_input_grad[2] else None)
+        ctx.p = p
+        return _collect(rows, p, scores)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        _, _, scores, rows = ctx.saved_tensors
+        p = ctx.p
+        if rows is None:
+            return _spread(dout, p, scores), None, None
+        dout, rows = _rows(dout, "dout"), _rows(rows, "rows")
+        (T, K), R, H, dev = p.s_reverse_scatter_idx.shape, p.num_rows, rows.shape[1], rows.device
+        with _lib.on_device(dev):
+            drows = torch.empty(R, H, dtype=rows.dtype, device=dev)
+            dscores = torch.empty_like(scores)
+            check(lib.smoe_unpermute_rows_backward(
+                dout.data_ptr(), dout.stride(0), rows.data_ptr(), rows.stride(0), drows.data_ptr(), _ROW_TYPES[rows.dtype],
+                scores.data_ptr(), dscores.data_ptr(), _ROW_TYPES[scores.dtype], p.s_reverse_scatter_idx.data_ptr(),
+                p.s_scatter_idx.data_ptr(), T, K, H, R, stream_ptr(dev)), "unpermute_rows_backward")
+        return drows, None, dscores
+
+
+def permute_tokens(x: torch.Tensor, permutation: TokenPermutation) -> torch.Tensor:
+    """rows (permutation.num_rows, H): x[token] of every row's pair, zeros in rows without one.  x (T, H); the gradient of x is
+    the sum of its tokens' rows."""
+    _lib.require_cuda(x, "x")
+    _check_permutation(permutation, x.device)
+    if x.dim() != 2 or x.shape[0] != permutation.s_reverse_scatter_idx.shape[0]:
+        raise ValueError(f"x has to be ({permutation.s_reverse_scatter_idx.shape[0]}, H), got {tuple(x.shape)}")
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _Permute.apply(x, permutation)
+    return _spread(x, permutation, None)
+
+
+def unpermute_tokens(rows: torch.Tensor, permutation: TokenPermutation, scores: torch.Tensor | None = None) -> torch.Tensor:
+    """out (T, H): the sum over each token's pairs of score * row (``scores`` (T, K) fp32, bf16 or fp16; None: 1).  Gradients flow
+    to rows and scores."""
+    _lib.require_cuda(rows, "rows")
+    _check_permutation(permutation, rows.device)
+    if rows.dim() != 2 or rows.shape[0] != permutation.num_rows:
+        raise ValueError(f"rows has to be ({permutation.num_rows}, H), got {tuple(rows.shape)}")
+    if scores is not None:
+        if scores.shape != permutation.s_reverse_scatter_idx.shape or scores.device != rows.device:
+            raise ValueError(f"scores has to be {tuple(permutation.s_reverse_scatter_idx.shape)} on {rows.device}, got "
+                             f"{tuple(scores.shape)} on {scores.device}")
+        if scores.dtype not in _ROW_TYPES:
+            raise TypeError(f"scores has to be fp32, bf16 or fp16, got {scores.dtype}")
+        scores = scores.contiguous()
+    if torch.is_grad_enabled() and (rows.requires_grad or (scores is not None and scores.requires_grad)):
+        return _Unpermute.apply(rows, permutation, scores)
+    return _collect(rows, permutation, scores)
