@@ -41,7 +41,7 @@ enum {
 enum { SMOE_ST_OK = 0, SMOE_ST_TIMEOUT_PRODUCER = 1, SMOE_ST_TIMEOUT_MMA = 2, SMOE_ST_TIMEOUT_EPILOGUE = 3 };
 
 /* dtype codes for tensors whose type the caller chooses */
-enum { SMOE_F32 = 0, SMOE_BF16 = 1, SMOE_I32 = 2, SMOE_I64 = 3, SMOE_F16 = 4 };
+enum { SMOE_F32 = 0, SMOE_BF16 = 1, SMOE_I32 = 2, SMOE_I64 = 3, SMOE_F16 = 4, SMOE_I8 = 5 };
 
 /* Library version, for the loader to check that it found the right build. */
 int smoe_abi_version(void);
@@ -460,6 +460,35 @@ int smoe_unpermute_rows(const void* rows, long long ld, void* out, int dtype, co
 int smoe_unpermute_rows_backward(const void* dout, long long dout_ld, const void* rows, long long ld, void* drows, int dtype,
                                  const void* weights, void* dweights, int weights_dtype, const int* s_reverse_scatter_idx,
                                  const int* s_scatter_idx, int T, int K, int H, long long R, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Products of 8-bit integers with one fp32 scale per row (token) and one per output channel, dense or grouped by expert, for
+ * serving (no gradients).  The reference has no 8-bit path.
+ * ------------------------------------------------------------------------------------------- */
+
+/* x (rows, cols) SMOE_F32, SMOE_BF16 or SMOE_F16, ld values from row to row -> q (rows, cols) int8, q_ld bytes from row to row
+ * (a multiple of 16; columns up to the next multiple of 16 become zeros), scale (rows): amax / 127 in fp32, 1 for a row of
+ * zeros; q = 127 x / amax rounded half to even, exactly.  A row that holds an infinity or a NaN gets it (NaN before infinity)
+ * as its scale, and zeros: all its products are NaN.  cols <= 131071. */
+int smoe_int8_quantize_rows(const void* x, long long ld, int dtype, void* q, long long q_ld, float* scale, long long rows,
+                            int cols, void* stream);
+
+/* y[r, n] = act(x_scale[s] * w_scale[e, n] * sum_k xq[s, k] wq[e, n, k] + bias[e, n]) for the rows r of every expert e.  The sum
+ * is exact; it is rounded to fp32, and the result to out_dtype.
+ * x (x_rows, cols): SMOE_I8 with x_scale (x_rows), rows starting on 16-byte boundaries (ld bytes apart), or SMOE_F32, SMOE_BF16,
+ * SMOE_F16 (ld values apart, x_scale NULL), which is quantised into the workspace first.  wq (E, N, cols) int8, rows w_ld
+ * bytes apart (a multiple of 16, 16-byte aligned base), w_scale (E, N).  bias (E, N) SMOE_F32, SMOE_BF16, SMOE_F16 or NULL.
+ * expert_frequency_offset (E+1): first row of every expert; NULL: E is 1 and has all rows.  expert_frequency (E) or NULL: rows
+ * of every expert where they do not reach up to the next one's.  Rows of the output that no expert has become zeros.
+ * x_gather_idx (rows): the row s of x that r takes (outside [0, x_rows): a row of zeros), or NULL: s = r and x_rows = rows.
+ * activation: -1 for none, or the codes above; gated ones take the channels 2j and 2j + 1 as gate and up.  out (rows, N), or
+ * (rows, N / 2) with a gated activation, packed, SMOE_F32, SMOE_BF16 or SMOE_F16.
+ * cols <= 131071, E <= 1024.  workspace: smoe_int8_linear_workspace_bytes bytes, 256-byte aligned (0: may be NULL). */
+size_t smoe_int8_linear_workspace_bytes(int x_dtype, int x_rows, int cols);
+int smoe_int8_linear(const void* x, long long ld, int x_dtype, const float* x_scale, const void* wq, long long w_ld,
+                     const float* w_scale, const void* bias, int bias_dtype, void* out, int out_dtype,
+                     const int* expert_frequency_offset, const int* expert_frequency, const int* x_gather_idx, int x_rows,
+                     int rows, int N, int cols, int E, int activation, void* workspace, int* status, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Expert parallelism over peer memory (one node, NVLink / NVSwitch).  The reference has no distributed

@@ -1,0 +1,171 @@
+// Products of 8-bit integers with one scale per row and one per output channel:
+//   y[r, n] = act( (sum_k xq[s(r), k] wq[e(r), n, k]) x_scale[s(r)] w_scale[e(r), n] + bias[e(r), n] )
+// What the kernels share: the argument block, which rows there are, and the arithmetic behind the sum.
+//
+// The sum is exact in 32-bit integers (at most 131071 products of at most 2^14), so it does not matter how a kernel orders or
+// splits it: all of them give the same bits.  It is rounded to fp32 once (2^-24), multiplied by the two scales, the bias is
+// added, and the result is rounded to the output's type.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "epilogue.cuh"
+#include "launch.cuh"
+
+namespace smoe {
+namespace i8 {
+
+constexpr int kMaxCols = 131071;     // 131071 * 128 * 128 < 2^31
+constexpr int kMaxExpertRows = 1024; // experts whose offsets the kernels keep in shared memory
+constexpr int kNoActivation = -1;
+
+struct Params {
+  int E, N, K;           // experts, output channels, columns of x
+  int rows;              // rows of the output
+  int x_rows;            // rows of x
+  const int* off;        // (E + 1) first row of each expert, or nullptr: one expert has all rows
+  const int* count;      // (E) rows of each expert, or nullptr: up to the next expert's first
+  const int* gather;     // (rows) row of x, or nullptr: the same row; out of range: a row of zeros
+  const float* x_scale;  // (x_rows)
+  const float* w_scale;  // (E, N)
+  const void* bias;      // (E, N) or nullptr
+  int bias_type;
+  void* out;             // (rows, N), or (rows, N / 2) with a gated activation
+  int out_type;
+  int activation;        // kNoActivation or smoe::Activation
+  int wide_out;          // rows of the output start on 16-byte boundaries
+  int* status;
+};
+
+__device__ __forceinline__ int first_row(const Params& p, int e) { return p.off != nullptr ? min(max(p.off[e], 0), p.rows) : 0; }
+// The row behind the expert's last one.  Offsets that overlap or run past the output are cut, so that no load reaches past it.
+__device__ __forceinline__ int end_row(const Params& p, int e) {
+  if (p.off == nullptr) return p.rows;
+  const int next = min(max(p.off[e + 1], 0), p.rows);
+  return p.count != nullptr ? min(next, p.off[e] + max(p.count[e], 0)) : next;
+}
+
+// Row of x that output row r takes, or -1.
+__device__ __forceinline__ int source_row(const Params& p, int r) {
+  const int s = p.gather != nullptr ? p.gather[r] : r;
+  return static_cast<unsigned>(s) < static_cast<unsigned>(p.x_rows) ? s : -1;
+}
+
+__device__ __forceinline__ float load_typed(const void* v, int dtype, long long i) {
+  if (dtype == SMOE_F32) return static_cast<const float*>(v)[i];
+  if (dtype == SMOE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(v)[i]);
+  return __half2float(static_cast<const __half*>(v)[i]);
+}
+__device__ __forceinline__ void store_typed(void* v, int dtype, long long i, float f) {
+  if (dtype == SMOE_F32) static_cast<float*>(v)[i] = f;
+  else if (dtype == SMOE_BF16) static_cast<__nv_bfloat16*>(v)[i] = __float2bfloat16_rn(f);
+  else static_cast<__half*>(v)[i] = __float2half_rn(f);
+}
+__device__ __forceinline__ uint32_t pack_typed(int dtype, float lo, float hi) {
+  if (dtype == SMOE_BF16) return pack_bf16(lo, hi);
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ float scaled(int acc, float xs, float ws) { return __int2float_rn(acc) * xs * ws; }
+
+// The activations' values by their definitions.  x sigmoid(x) = x / (1 + exp(-x)) with the fast exponential and division: 2^-21
+// of the value, where the hardware tanh that the bf16 epilogues use is off by 2.5e-4 of x, too much of a small result.
+__device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
+__device__ __forceinline__ float activate(int act, float x) {
+  switch (act) {
+    case ACT_SWIGLU: case ACT_SILU: return silu(x);
+    case ACT_GEGLU: case ACT_GELU: return 0.5f * x * erfcf(x * -0.70710678118654752f);
+    case ACT_RELU_SQ: return x < 0.f ? 0.f : x * x;
+    case ACT_REGLU: case ACT_RELU: return x < 0.f ? 0.f : x;  // NaN stays NaN
+  }
+  return x;
+}
+
+// Rows that no expert has (between an expert's rows and the next one's, behind the last) become zeros.  Warp `warp` of `warps`,
+// all its lanes; a row's expert is found by bisection.
+__device__ __forceinline__ void zero_other_rows(const Params& p, int warp, int warps) {
+  if (p.off == nullptr) return;
+  const int lane = threadIdx.x & 31;
+  const int cols = p.activation >= 0 && act_is_gated(p.activation) ? p.N / 2 : p.N;
+  const long long bytes = static_cast<long long>(cols) * (p.out_type == SMOE_F32 ? 4 : 2);
+  for (long long base = 32ll * warp; base < p.rows; base += 32ll * warps) {
+    const int r = static_cast<int>(base) + lane;
+    bool other = false;
+    if (base + lane < p.rows) {
+      int lo = 0, hi = p.E;  // the last expert whose first row is not behind r
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (p.off[mid] <= r) lo = mid; else hi = mid;
+      }
+      other = r < first_row(p, lo) || r >= end_row(p, lo);
+    }
+    for (unsigned todo = __ballot_sync(0xffffffffu, other); todo != 0u; todo &= todo - 1u) {
+      char* dst = static_cast<char*>(p.out) + (base + __ffs(todo) - 1) * bytes;
+      if (p.wide_out) {
+        for (long long c = 16 * lane; c < bytes; c += 512) *reinterpret_cast<uint4*>(dst + c) = make_uint4(0u, 0u, 0u, 0u);
+      } else {
+        for (long long c = 2 * lane; c < bytes; c += 64) *reinterpret_cast<uint16_t*>(dst + c) = 0;
+      }
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------------------------
+// quantisation of a row: scale = amax / 127 (1 for a row of zeros), q = 127 x / amax rounded half to even
+// ----------------------------------------------------------------------------------------------
+// x times 127 / amax in fp32 is within 127 * 2^-23 = 1.5e-5 of the quotient; where that leaves it open on which side of a
+// border it is (and for rows so small that 127 / amax overflows), the quotient is computed in 64 bits, where it is on the right
+// side: 127 x is exact there, and a quotient of two 24-bit numbers that is no half itself is further than 2^-33 from one.
+// Rows that hold an infinity or a NaN get it as their scale, and zeros: every product of theirs is NaN.
+struct RowScale {
+  float amax, scale, inv;
+  bool fine;  // finite
+  bool tiny;  // every quotient in 64 bits
+};
+// bits: the largest |x| as an integer (a NaN's are above infinity's)
+__device__ __forceinline__ RowScale row_scale(uint32_t bits) {
+  RowScale s;
+  s.amax = __uint_as_float(bits);
+  s.fine = bits < 0x7F800000u;
+  s.tiny = bits < (7u << 23);  // 2^-120
+  s.scale = bits == 0u ? 1.f : s.fine ? __fdiv_rn(s.amax, 127.f) : s.amax;
+  s.inv = s.tiny || !s.fine ? 0.f : __fdiv_rn(127.f, s.amax);
+  return s;
+}
+
+constexpr float kRoundMagic = 12582912.f;  // 1.5 * 2^23: adding it leaves the whole number in the low bits
+constexpr float kBorder = 0.5f - 1.f / 32768.f;
+
+// N values -> N bytes in the low bytes of w (four per word)
+template <int N>
+__device__ __forceinline__ void quantize_values(const RowScale& s, const float (&f)[N], uint32_t (&w)[(N + 3) / 4]) {
+  float far = 0.f;
+  int q[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float t = f[i] * s.inv;
+    const float m = t + kRoundMagic;
+    q[i] = __float_as_int(m);
+    far = fmaxf(far, fabsf(t - (m - kRoundMagic)));
+  }
+  if (far >= kBorder || s.tiny) {
+#pragma unroll 1
+    for (int i = 0; i < N; ++i) {
+      float x = 0.f;
+#pragma unroll
+      for (int j = 0; j < N; ++j) x = i == j ? f[j] : x;  // registers have no index
+      const int v = s.amax > 0.f ? static_cast<int>(rint(127.0 * static_cast<double>(x) / static_cast<double>(s.amax))) : 0;
+#pragma unroll
+      for (int j = 0; j < N; ++j) q[j] = i == j ? v : q[j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < (N + 3) / 4; ++j) {
+    w[j] = 0u;
+#pragma unroll
+    for (int i = 0; i < 4 && 4 * j + i < N; ++i) w[j] |= (s.fine ? static_cast<uint32_t>(q[4 * j + i]) & 0xFFu : 0u) << (8 * i);
+  }
+}
+
+}  // namespace i8
+}  // namespace smoe

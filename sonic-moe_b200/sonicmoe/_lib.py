@@ -16,7 +16,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsonicmoe_b200.so")
 
-SMOE_F32, SMOE_BF16, SMOE_I32, SMOE_I64, SMOE_F16 = 0, 1, 2, 3, 4
+SMOE_F32, SMOE_BF16, SMOE_I32, SMOE_I64, SMOE_F16, SMOE_I8 = 0, 1, 2, 3, 4, 5
 
 _ERRORS = {
     -1: "unsupported or inconsistent sizes",
@@ -107,6 +107,9 @@ SIGNATURES: dict[str, tuple] = {
     "smoe_permute_rows": (I, [P, LL, P, I, P, I, P, P, I, I, I, LL, P]),
     "smoe_unpermute_rows": (I, [P, LL, P, I, P, I, P, I, I, I, LL, P]),
     "smoe_unpermute_rows_backward": (I, [P, LL, P, LL, P, I, P, P, I, P, P, I, I, I, LL, P]),
+    "smoe_int8_quantize_rows": (I, [P, LL, I, P, LL, P, LL, I, P]),
+    "smoe_int8_linear_workspace_bytes": (c_size_t, [I, I, I]),
+    "smoe_int8_linear": (I, [P, LL, I, P, P, LL, P, P, I, P, I, P, P, P, I, I, I, I, I, I, P, P, P]),
     "smoe_peer_alloc": (I, [c_size_t, P]),
     "smoe_peer_free": (I, [P]),
     "smoe_peer_export": (I, [P, P]),
