@@ -1,0 +1,876 @@
+// 8-bit integer products on the tensor cores (tcgen05.mma.kind::i8: signed bytes, 32-bit integer accumulators in tensor
+// memory).  A stage holds 128 columns of an operand row, 128 bytes, so staging, swizzle and descriptors are those of the bf16
+// kernels with elements of half the size, and a stage's four MMAs (K 32 each) do twice the work in the same time.
+//
+//   tiles   256 rows x 256 channels per CTA pair: cta_group::2, two accumulators, persistent
+//   units   128 channels (the MMA's rows) x up to 128 rows of x per CTA, for experts or batches with few rows, where the weights
+//           are the work: see gemm_skinny.cuh for why the operands trade places.  SPLIT: the reduction of a unit is shared by
+//           the CTAs of a cluster, where there are too few units to keep the memory busy.
+//
+// Both take their rows from consecutive rows of x or gathered (TMA tile::gather4, a row that is none reads zeros).  The columns
+// past the last are zeros by the tensor maps' extent.  Every wait is bounded (ptx.cuh).
+#pragma once
+#include "int8.cuh"
+#include "ptx.cuh"
+
+namespace smoe {
+namespace i8 {
+
+constexpr int BK = 128;  // columns, and bytes, of a stage's row
+constexpr int UMMA_K = 32;
+
+// What the epilogue is compiled for: the switch over the other activations around an element loop slows the common ones.
+enum Mode : int { MODE_PLAIN = 0, MODE_SWIGLU = 1, MODE_ANY = 2 };
+
+__host__ __device__ constexpr uint32_t make_idesc_i8(int M, int N) {
+  return (2u << 4)                     // D: 32-bit integers
+         | (1u << 7) | (1u << 10)      // A, B: signed bytes, K-major
+         | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+template <int CTAS>
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CTAS == 2)
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
+        "}\n"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
+        "}\n"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void st_shared_word(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t ld_shared_word(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Where a warp's block of outputs goes: row r of it to base + r * pitch, `valid` bytes from the block's first column to the
+// row's end.
+struct Block {
+  char* base;
+  long long pitch;
+  int rows;        // rows that exist
+  long long valid;
+  bool wide;       // 16-byte pieces; otherwise value by value
+  bool half;       // 16-bit values
+};
+
+// A warp's staged rows (STRIDE bytes apart, BYTES of each, ROWS of them; address of a 16-byte piece by `piece`) go out: whole
+// row segments, neighbouring lanes on neighbouring pieces.  All lanes.
+template <int ROWS, int BYTES, class Piece>
+__device__ __forceinline__ void store_staged(int lane, const Block& b, Piece&& piece) {
+  __syncwarp();
+  if (b.wide) {
+    constexpr int PIECES = BYTES / 16, PER = 32 / PIECES;
+#pragma unroll
+    for (int i = 0; i < ROWS / PER; ++i) {
+      const int r = PER * i + lane / PIECES, q = lane % PIECES;
+      const uint4 v = ld_shared_v4(piece(r, q));
+      if (r < b.rows && 16 * q < b.valid) *reinterpret_cast<uint4*>(b.base + r * b.pitch + 16 * q) = v;
+    }
+  } else {
+    constexpr int WORDS = BYTES / 4, PER = 32 / WORDS;
+    for (int i = 0; i < ROWS / PER; ++i) {
+      const int r = PER * i + lane / WORDS, w = lane % WORDS;
+      const uint32_t v = ld_shared_word(piece(r, w / 4) + 4 * (w % 4));
+      if (r >= b.rows) continue;
+      char* dst = b.base + r * b.pitch + 4 * w;
+      if (b.half) {
+        if (4 * w < b.valid) *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(v);
+        if (4 * w + 2 < b.valid) *reinterpret_cast<uint16_t*>(dst + 2) = static_cast<uint16_t>(v >> 16);
+      } else if (4 * w < b.valid) {
+        *reinterpret_cast<uint32_t*>(dst) = v;
+      }
+    }
+  }
+  __syncwarp();
+}
+
+template <int MODE>
+__device__ __forceinline__ bool is_gated(const Params& p) {
+  if constexpr (MODE == MODE_PLAIN) return false;
+  else if constexpr (MODE == MODE_SWIGLU) return true;
+  else return act_is_gated(p.activation);
+}
+template <int MODE>
+__device__ __forceinline__ float activation_of(const Params& p, float x) {
+  if constexpr (MODE == MODE_SWIGLU) return silu(x);
+  else return activate(p.activation, x);
+}
+
+// First rows, ends and the exclusive prefix of the row tiles of all experts, in shared memory.  One warp, all lanes.
+// Experts with rows in (least, most] count.
+template <class Shared>
+__device__ __forceinline__ void list_experts(const Params& p, Shared& ss, int tile_rows, int least, int most, int lane) {
+  int running = 0;
+  for (int base = 0; base < p.E; base += 32) {
+    const int e = base + lane;
+    int first = 0, end = 0;
+    if (e < p.E) { first = first_row(p, e); end = end_row(p, e); }
+    const int rows = end - first;
+    const int v = rows > least && rows <= most ? (rows + tile_rows - 1) / tile_rows : 0;
+    int incl = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += o;
+    }
+    if (e < p.E) {
+      ss.first[e] = first;
+      ss.end[e] = end;
+      ss.tiles_before[e] = running + incl - v;
+    }
+    running += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  if (lane == 0) ss.tiles_before[p.E] = running;
+}
+
+// Whether experts with more than `limit` rows have at least half of all rows: then the tiles take every expert, as in
+// tiles_take_all.  One warp, all lanes; the two kernels of a call come to the same answer.
+__device__ __forceinline__ bool most_rows_in_tiles(const Params& p, int limit, int lane) {
+  int above = 0, all = 0;
+  for (int e = lane; e < p.E; e += 32) {
+    const int rows = max(end_row(p, e) - first_row(p, e), 0);
+    all += rows;
+    if (rows > limit) above += rows;
+  }
+  above = __reduce_add_sync(0xffffffffu, above);
+  all = __reduce_add_sync(0xffffffffu, all);
+  return 2ll * above >= all;
+}
+
+// ----------------------------------------------------------------------------------------------
+// tiles
+// ----------------------------------------------------------------------------------------------
+namespace tiles {
+
+constexpr int BM = 128, BN = 256, BN_CTA = 128, STAGES = 6;
+constexpr int A_STAGE_BYTES = BM * BK, B_STAGE_BYTES = BN_CTA * BK;
+constexpr int THREADS = 512, FIRST_EPI_WARP = 4, EPI_WARPS = 8, FIRST_GATHER_WARP = 12, GATHER_WARPS = 4;
+constexpr int COLS_PER_WARP = BN * 4 / EPI_WARPS;
+
+struct Shared {
+  uint64_t full[STAGES];
+  uint64_t empty[STAGES];
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];
+  uint32_t tmem_base;
+  int abort_flag;
+  int first[kMaxExpertRows];
+  int end[kMaxExpertRows];
+  int tiles_before[kMaxExpertRows + 1];
+};
+constexpr int SMEM_BYTES = 1024 + STAGES * (A_STAGE_BYTES + B_STAGE_BYTES) + ((sizeof(Shared) + 127) & ~127) + EPI_WARPS * STAGE_ROWS_BYTES;
+static_assert(SMEM_BYTES <= 227 * 1024, "shared memory per CTA");
+
+struct Tile {
+  int e, row0, row_end, n0;  // row0: of this CTA's 128 rows
+};
+
+// The tiles of this CTA pair, expert by expert, the channels of a row tile innermost, dealt out round-robin.
+struct Walker {
+  const Params& p;
+  const Shared& ss;
+  const int lane, num_n, total, step_m, step_n;
+  int t, mi, ni, e = 0;
+  __device__ __forceinline__ Walker(const Params& p_, const Shared& ss_, int lane_)
+      : p(p_), ss(ss_), lane(lane_), num_n((p_.N + BN - 1) / BN), total(ss_.tiles_before[p_.E] * num_n),
+        step_m(static_cast<int>(gridDim.x >> 1) / num_n), step_n(static_cast<int>(gridDim.x >> 1) % num_n),
+        t(blockIdx.x >> 1), mi(t / num_n), ni(t % num_n) {}
+  // the MMA issuer counts tiles only
+  __device__ __forceinline__ bool next_uncounted() {
+    const bool more = t < total;
+    t += gridDim.x >> 1;
+    return more;
+  }
+  __device__ __forceinline__ bool next(uint32_t rank, Tile& tile) {
+    if (!next_uncounted()) return false;
+    while (true) {  // the first expert whose tiles end beyond mi, 32 experts at a time
+      const int i = e + 1 + lane;
+      const unsigned before = __ballot_sync(0xffffffffu, i <= p.E && ss.tiles_before[i] <= mi);
+      e += __popc(before);
+      if (before != 0xffffffffu) break;
+    }
+    tile.e = e;
+    tile.row0 = ss.first[e] + (mi - ss.tiles_before[e]) * (2 * BM) + static_cast<int>(rank) * BM;
+    tile.row_end = ss.end[e];
+    tile.n0 = ni * BN;
+    mi += step_m;
+    ni += step_n;
+    if (ni >= num_n) { ni -= num_n; ++mi; }
+    return true;
+  }
+};
+
+// 32 channels of the warp's 32 rows: lane l has row l's sums in v.
+template <int MODE>
+__device__ __forceinline__ void store_columns(const Params& p, uint32_t stage, int lane, int row_base, int row_end, int e, int n,
+                                              const uint32_t (&v)[32], float xs) {
+  float f[32];
+  const long long at = static_cast<long long>(e) * p.N + n;
+  if (n + 32 <= p.N && reinterpret_cast<uintptr_t>(p.w_scale + at) % 16 == 0) {  // every lane reads the same words
+    const float4* w = reinterpret_cast<const float4*>(p.w_scale + at);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float4 s = w[j];
+      f[4 * j] = s.x; f[4 * j + 1] = s.y; f[4 * j + 2] = s.z; f[4 * j + 3] = s.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) f[j] = n + j < p.N ? p.w_scale[at + j] : 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < 32; ++j) f[j] = scaled(static_cast<int>(v[j]), xs, f[j]);
+  if (p.bias != nullptr) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (n + j < p.N) f[j] += load_typed(p.bias, p.bias_type, at + j);
+  }
+  const bool gated = is_gated<MODE>(p);
+  const long long cols = gated ? p.N / 2 : p.N;
+  const int size = p.out_type == SMOE_F32 ? 4 : 2;
+  Block b;
+  b.pitch = cols * size;
+  const long long col = gated ? n / 2 : n;
+  b.base = static_cast<char*>(p.out) + row_base * b.pitch + col * size;
+  b.rows = row_end - row_base;
+  b.valid = (cols - col) * size;
+  b.wide = p.wide_out;
+  b.half = size == 2;
+  const auto piece = [&](int r, int q) { return stage_piece(stage, r, q); };
+  const auto put = [&](int q, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) { st_shared_v4(piece(lane, q), w0, w1, w2, w3); };
+  const auto bits = [&](int j) { return __float_as_uint(f[j]); };
+  const auto two = [&](int j) { return pack_typed(p.out_type, f[j], f[j + 1]); };
+  if (gated) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) f[j] = activation_of<MODE>(p, f[2 * j]) * f[2 * j + 1];
+    if (b.half) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) put(q, two(8 * q), two(8 * q + 2), two(8 * q + 4), two(8 * q + 6));
+      store_staged<32, 32>(lane, b, piece);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) put(q, bits(4 * q), bits(4 * q + 1), bits(4 * q + 2), bits(4 * q + 3));
+      store_staged<32, 64>(lane, b, piece);
+    }
+    return;
+  }
+  if constexpr (MODE == MODE_ANY) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) f[j] = activation_of<MODE>(p, f[j]);
+  }
+  if (b.half) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) put(q, two(8 * q), two(8 * q + 2), two(8 * q + 4), two(8 * q + 6));
+    store_staged<32, 64>(lane, b, piece);
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) put(q, bits(16 * h + 4 * q), bits(16 * h + 4 * q + 1), bits(16 * h + 4 * q + 2), bits(16 * h + 4 * q + 3));
+      store_staged<32, 64>(lane, b, piece);
+      b.base += 64;
+      b.valid -= 64;
+    }
+  }
+}
+
+// least: experts with at most that many rows are the other kernel's.
+template <int MODE>
+__global__ void __launch_bounds__(THREADS, 1)
+int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p, const int least) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + STAGES * A_STAGE_BYTES;
+  Shared& ss = *reinterpret_cast<Shared*>(smem + STAGES * (A_STAGE_BYTES + B_STAGE_BYTES));
+  uint8_t* stage_out = reinterpret_cast<uint8_t*>(&ss) + ((sizeof(Shared) + 127) & ~127);
+  const int warp = warp_index();
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  volatile int* abort_flag = &ss.abort_flag;
+  const int num_kb = (p.K + BK - 1) / BK;
+  const bool gathered = p.gather != nullptr;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(smem_u32(&ss.full[s]), 1);
+      mbar_init(smem_u32(&ss.empty[s]), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(smem_u32(&ss.acc_full[a]), 1);
+      mbar_init(smem_u32(&ss.acc_empty[a]), 2 * EPI_WARPS);
+    }
+    ss.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&ss.tmem_base), 2 * BN);
+    tmem_relinquish();
+  }
+  wait_for_previous();
+  if (warp == 2) {
+    const int skip = least > 0 && !most_rows_in_tiles(p, least, lane) ? least : 0;
+    list_experts(p, ss, 2 * BM, skip, p.rows, lane);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = ss.tmem_base;
+
+  if (warp < FIRST_EPI_WARP) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
+      // ---- TMA producer: the weights, and the rows of x where they are not gathered --------------
+      const bool elected = elect_one();
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      Tile tile;
+      Walker walk(p, ss, lane);
+      while (ok && walk.next(rank, tile)) {
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait_warp(smem_u32(&ss.empty[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
+          if (elected) {
+            const uint32_t bar = map_to_cta(smem_u32(&ss.full[stage]), 0);
+            if (leader) mbar_arrive_expect_tx(smem_u32(&ss.full[stage]), 2 * (A_STAGE_BYTES + B_STAGE_BYTES));
+            // no rows at all in this CTA's half of the tile: read past the tensor's end, which delivers zeros
+            if (!gathered)
+              tma_load_2d_pair(&tmA, bar, smem_u32(sA + stage * A_STAGE_BYTES), kb * BK, tile.row0 < tile.row_end ? tile.row0 : p.x_rows);
+            tma_load_2d_pair(&tmB, bar, smem_u32(sB + stage * B_STAGE_BYTES), kb * BK,
+                             tile.e * p.N + tile.n0 + static_cast<int>(rank) * BN_CTA);
+          }
+          __syncwarp();
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+      }
+      if (!ok && lane == 0 && p.status) atomicCAS(p.status, ST_OK, ST_TIMEOUT_PRODUCER);
+    } else if (warp == 1) {
+      // ---- MMA issuer ------------------------------------------------------------------------
+      if (leader && elect_one()) {
+        constexpr uint32_t idesc = make_idesc_i8(2 * BM, BN);
+        int stage = 0, acc = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        bool ok = true;
+        Walker walk(p, ss, lane);
+        while (ok && walk.next_uncounted()) {
+          if (!mbar_wait(smem_u32(&ss.acc_empty[acc]), acc_phase ^ 1u, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          for (int kb = 0; kb < num_kb; ++kb) {
+            if (!mbar_wait(smem_u32(&ss.full[stage]), phase, abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            const uint64_t a_desc = make_smem_desc(smem_u32(sA + stage * A_STAGE_BYTES), 16, 1024);
+            const uint64_t b_desc = make_smem_desc(smem_u32(sB + stage * B_STAGE_BYTES), 16, 1024);
+#pragma unroll
+            for (int k4 = 0; k4 < BK / UMMA_K; ++k4)
+              umma_i8<2>(tmem_base + acc * BN, a_desc + ((k4 * UMMA_K) >> 4), b_desc + ((k4 * UMMA_K) >> 4), idesc,
+                         (kb > 0 || k4 > 0) ? 1u : 0u);
+            umma_commit_pair(smem_u32(&ss.empty[stage]), 3);
+            if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+          }
+          if (!ok) break;
+          umma_commit_pair(smem_u32(&ss.acc_full[acc]), 3);
+          if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+        }
+        if (!ok && p.status) atomicCAS(p.status, ST_OK, ST_TIMEOUT_MMA);
+      }
+    } else {
+      if (p.zero_others) zero_other_rows(p, 2 * blockIdx.x + (warp - 2), 2 * gridDim.x);
+    }
+  } else if (warp >= FIRST_GATHER_WARP) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    // ---- row gather: one thread of each warp issues for 32 rows -------------------------------
+    if (gathered) {
+      const int gw = warp - FIRST_GATHER_WARP;
+      const bool elected = elect_one();
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      Tile tile;
+      Walker walk(p, ss, lane);
+      while (ok && walk.next(rank, tile)) {
+        const int r = tile.row0 + 32 * gw + lane;
+        int mine = p.x_rows;  // rows that do not exist: zeros
+        if (r < tile.row_end) {
+          const int s = source_row(p, r);
+          if (s >= 0) mine = s;
+        }
+        int rows[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) rows[i] = __shfl_sync(0xffffffffu, mine, i);
+        if (elected) {
+          for (int kb = 0; kb < num_kb; ++kb) {
+            if (!mbar_wait(smem_u32(&ss.empty[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
+            const uint32_t bar = map_to_cta(smem_u32(&ss.full[stage]), 0);
+            const uint32_t dst = smem_u32(sA + stage * A_STAGE_BYTES) + gw * 4096;
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              tma_gather4_pair(&tmA, bar, dst + q * 512, kb * BK, rows[4 * q], rows[4 * q + 1], rows[4 * q + 2], rows[4 * q + 3]);
+            if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+      }
+      if (!ok && lane == 0 && p.status) atomicCAS(p.status, ST_OK, ST_TIMEOUT_PRODUCER);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    // ---- epilogue: a warp has 32 rows x 128 channels -------------------------------------------
+    const int quad = warp & 3;
+    const int col_half = (warp - FIRST_EPI_WARP) >> 2;
+    const uint32_t my_stage = smem_u32(stage_out) + (warp - FIRST_EPI_WARP) * STAGE_ROWS_BYTES;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    Tile tile;
+    Walker walk(p, ss, lane);
+    while (ok && walk.next(rank, tile)) {
+      const int row_base = tile.row0 + quad * 32, r = row_base + lane;
+      const int n_first = tile.n0 + col_half * COLS_PER_WARP;
+      float xs = 0.f;
+      if (r < tile.row_end) {
+        const int s = source_row(p, r);
+        if (s >= 0) xs = p.x_scale[s];
+      }
+      if (!mbar_wait_warp(smem_u32(&ss.acc_full[acc]), acc_phase, abort_flag)) { ok = false; break; }
+      tc_fence_after();
+      const auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&ss.acc_empty[acc]), 0));
+      };
+      const bool works = n_first < p.N && row_base < tile.row_end;
+      if (!works) release();
+      const uint32_t t_addr = tmem_base + acc * BN + col_half * COLS_PER_WARP + (static_cast<uint32_t>(quad * 32) << 16);
+#pragma unroll 1
+      for (int c = 0; works && c < COLS_PER_WARP / 32; ++c) {
+        const int n = n_first + 32 * c;
+        if (n >= p.N) break;
+        uint32_t v[32];
+        tmem_ld32(t_addr + 32 * c, v);
+        tmem_ld_wait();
+        if (c + 1 == COLS_PER_WARP / 32 || n + 32 >= p.N) release();
+        store_columns<MODE>(p, my_stage, lane, row_base, tile.row_end, tile.e, n, v, xs);
+      }
+      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+    }
+    if (!ok && lane == 0 && p.status) atomicCAS(p.status, ST_OK, ST_TIMEOUT_EPILOGUE);
+  }
+
+  if (*abort_flag != 0) {
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+  }
+  // barriers that the lanes of a warp may reach one by one: the MMA role is one lane's
+  tc_fence_before();
+  block_sync_diverged();
+  cluster_sync_diverged();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 2 * BN);
+  }
+}
+
+}  // namespace tiles
+
+// ----------------------------------------------------------------------------------------------
+// units
+// ----------------------------------------------------------------------------------------------
+namespace units {
+
+constexpr int BM = 128;  // channels
+constexpr int W_STAGE_BYTES = BM * BK;
+constexpr int MAX_NT = 128, MAX_STAGES = 10, MAX_SPLIT = 8;
+constexpr int EPI_WARPS = 8, FIRST_EPI_WARP = 2, FIRST_GATHER_WARP = FIRST_EPI_WARP + EPI_WARPS, GATHER_WARPS = 4;
+constexpr int THREADS = 32 * (FIRST_GATHER_WARP + GATHER_WARPS);
+constexpr int BOX_ROWS = 32;  // rows per TMA box of a row tile that is not gathered
+
+struct Shared {
+  uint64_t full[MAX_STAGES];
+  uint64_t empty[MAX_STAGES];
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];
+  uint32_t tmem_base;
+  int abort_flag;
+  int first[kMaxExpertRows];
+  int end[kMaxExpertRows];
+  int tiles_before[kMaxExpertRows + 1];
+};
+__host__ __device__ constexpr int stage_bytes(int nt) { return W_STAGE_BYTES + nt * BK; }
+__host__ __device__ constexpr int smem_bytes(int nt, int stages) {
+  return 1024 + stages * stage_bytes(nt) + EPI_WARPS * STAGE_ROWS_BYTES + static_cast<int>(sizeof(Shared));
+}
+__host__ __device__ constexpr int num_stages(int nt) {
+  const int fit = (227 * 1024 - smem_bytes(nt, 0)) / stage_bytes(nt);
+  return fit < MAX_STAGES ? fit : MAX_STAGES;
+}
+// SPLIT: a CTA's sums of a whole unit, 32-bit integers, take the stages' place
+static_assert(num_stages(MAX_NT) * stage_bytes(MAX_NT) >= MAX_NT * BM * 4 && num_stages(32) * stage_bytes(32) >= 32 * BM * 4, "room for the sums");
+
+struct Unit {
+  int e, row0, rows, f0;
+};
+
+// The units of this CTA (SPLIT: of its cluster), expert by expert, row tiles innermost.
+struct Walker {
+  const Params& p;
+  const Shared& ss;
+  const int lane, nt, blocks, total, step;
+  int unit, e = 0;
+  __device__ __forceinline__ Walker(const Params& p_, const Shared& ss_, int lane_, int nt_, int split)
+      : p(p_), ss(ss_), lane(lane_), nt(nt_), blocks((p_.N + BM - 1) / BM), total(ss_.tiles_before[p_.E] * blocks),
+        step(gridDim.x / split), unit(blockIdx.x / split) {}
+  __device__ __forceinline__ bool next(Unit& u) {
+    if (unit >= total) return false;
+    while (true) {
+      const int i = e + 1 + lane;
+      const unsigned before = __ballot_sync(0xffffffffu, i <= p.E && ss.tiles_before[i] * blocks <= unit);
+      e += __popc(before);
+      if (before != 0xffffffffu) break;
+    }
+    const int tiles = ss.tiles_before[e + 1] - ss.tiles_before[e];
+    const int in_expert = unit - ss.tiles_before[e] * blocks;
+    const int b = in_expert / tiles;
+    u.e = e;
+    u.f0 = b * BM;
+    u.row0 = ss.first[e] + (in_expert - b * tiles) * nt;
+    u.rows = min(nt, ss.end[e] - u.row0);
+    unit += step;
+    return true;
+  }
+};
+
+// 32 channels (lane l: channel f + l) of up to 32 rows (word j: row row0 + j), of which `rows` exist.  Neighbouring lanes exchange
+// half of their values: afterwards word j of an even lane has the channels (l, l + 1) of row 2j and that of an odd one (l - 1, l) of
+// row 2j + 1, a gate and its up value, or two values of one 32-bit store.
+template <int MODE>
+__device__ __forceinline__ void store_rows(const Params& p, uint32_t stage, int lane, int e, int f, int row0, int rows,
+                                           const uint32_t (&v)[32]) {
+  const bool mine = f + lane < p.N;
+  const long long at = static_cast<long long>(e) * p.N + f + lane;
+  const float ws = mine ? p.w_scale[at] : 0.f;
+  const float bias = mine && p.bias != nullptr ? load_typed(p.bias, p.bias_type, at) : 0.f;
+  float xs = 0.f;
+  if (lane < rows) {
+    const int s = source_row(p, row0 + lane);
+    if (s >= 0) xs = p.x_scale[s];
+  }
+  const bool odd = lane & 1;
+  const bool gated = is_gated<MODE>(p);
+  float lo[16], hi[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    float a = scaled(static_cast<int>(v[2 * j]), __shfl_sync(0xffffffffu, xs, 2 * j), ws);
+    float b = scaled(static_cast<int>(v[2 * j + 1]), __shfl_sync(0xffffffffu, xs, 2 * j + 1), ws);
+    if (p.bias != nullptr) { a += bias; b += bias; }
+    if constexpr (MODE == MODE_ANY) {
+      if (!gated) { a = activation_of<MODE>(p, a); b = activation_of<MODE>(p, b); }
+    }
+    const float other = __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
+    lo[j] = odd ? other : a;
+    hi[j] = odd ? b : other;
+  }
+  const long long cols = gated ? p.N / 2 : p.N;
+  const int size = p.out_type == SMOE_F32 ? 4 : 2;
+  Block b;
+  b.pitch = cols * size;
+  const long long col = gated ? f / 2 : f;
+  b.base = static_cast<char*>(p.out) + row0 * b.pitch + col * size;
+  b.rows = rows;
+  b.valid = (cols - col) * size;
+  b.wide = p.wide_out;
+  b.half = size == 2;
+  const int pair = lane >> 1;
+  const auto at_word = [&](int row, int bytes, int byte) { return stage + row * bytes + byte; };
+  if (gated) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) lo[j] = activation_of<MODE>(p, lo[j]) * hi[j];
+    if (b.half) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const uint32_t h = pack_typed(p.out_type, lo[j], 0.f) & 0xFFFFu;
+        asm volatile("st.shared.b16 [%0], %1;" ::"r"(at_word(2 * j + odd, 32, 2 * pair)), "h"(static_cast<unsigned short>(h)) : "memory");
+      }
+      store_staged<32, 32>(lane, b, [&](int r, int q) { return stage + r * 32 + 16 * q; });
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) st_shared_word(at_word(2 * j + odd, 64, 4 * pair), __float_as_uint(lo[j]));
+      store_staged<32, 64>(lane, b, [&](int r, int q) { return stage + r * 64 + 16 * q; });
+    }
+  } else if (b.half) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) st_shared_word(at_word(2 * j + odd, 64, 4 * pair), pack_typed(p.out_type, lo[j], hi[j]));
+    store_staged<32, 64>(lane, b, [&](int r, int q) { return stage + r * 64 + 16 * q; });
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // 16 rows of 128 bytes at a time
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        st_shared_word(at_word(2 * j + odd, 128, 8 * pair), __float_as_uint(lo[8 * h + j]));
+        st_shared_word(at_word(2 * j + odd, 128, 8 * pair + 4), __float_as_uint(hi[8 * h + j]));
+      }
+      store_staged<16, 128>(lane, b, [&](int r, int q) { return stage + r * 128 + 16 * q; });
+      b.base += 16 * b.pitch;
+      b.rows -= 16;
+    }
+  }
+}
+
+// most: experts with more rows are the tiles'.  split: CTAs of a cluster that share a unit's reduction (1: none); with SPLIT
+// there are at least as many clusters as units.
+template <int MODE, bool SPLIT>
+__global__ void __launch_bounds__(THREADS, 1)
+int8_unit_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Params p, const int most,
+                 const int nt, const int stages, const int split) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int stage_size = stage_bytes(nt);
+  uint8_t* stage_out = smem + stages * stage_size;
+  Shared& ss = *reinterpret_cast<Shared*>(stage_out + EPI_WARPS * STAGE_ROWS_BYTES);
+  const int warp = warp_index();
+  const int lane = threadIdx.x & 31;
+  volatile int* abort_flag = &ss.abort_flag;
+  const bool gathered = p.gather != nullptr;
+  const int all_kb = (p.K + BK - 1) / BK;
+  const int slice = SPLIT ? static_cast<int>(cluster_ctarank()) : 0;
+  const int kb_begin = SPLIT ? slice * all_kb / split : 0;
+  const int kb_end = SPLIT ? (slice + 1) * all_kb / split : all_kb;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(smem_u32(&ss.full[s]), 1 + (gathered ? GATHER_WARPS : 0));
+      mbar_init(smem_u32(&ss.empty[s]), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(smem_u32(&ss.acc_full[a]), 1);
+      mbar_init(smem_u32(&ss.acc_empty[a]), EPI_WARPS);
+    }
+    ss.abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmX);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&ss.tmem_base), 2 * MAX_NT);
+    tmem_relinquish();
+  }
+  wait_for_previous();
+  if (warp == 2) {
+    const int limit = most < p.rows && most_rows_in_tiles(p, most, lane) ? 0 : most;
+    list_experts(p, ss, nt, 0, limit, lane);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = ss.tmem_base;
+  bool ok = true;
+  Unit u;
+  Walker walk(p, ss, lane, nt, split);
+
+  if (warp == 0) {
+    // ---- TMA producer -------------------------------------------------------------------------
+    const bool elected = elect_one();
+    int stage = 0;
+    uint32_t phase = 0;
+    while (ok && walk.next(u)) {
+      const int boxes = (u.rows + BOX_ROWS - 1) / BOX_ROWS;
+      const uint32_t bytes = W_STAGE_BYTES + (gathered ? (u.rows + 3) / 4 * 512 : boxes * (BOX_ROWS * BK));
+      for (int kb = kb_begin; kb < kb_end; ++kb) {
+        if (!mbar_wait_warp(smem_u32(&ss.empty[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
+        const uint32_t bar = smem_u32(&ss.full[stage]);
+        const uint32_t dst = smem_u32(smem + stage * stage_size);
+        if (elected) {
+          mbar_arrive_expect_tx(bar, bytes);
+          tma_load_2d(&tmW, bar, dst, kb * BK, u.e * p.N + u.f0);
+          if (!gathered) {
+            for (int b = 0; b < boxes; ++b)
+              tma_load_2d(&tmX, bar, dst + W_STAGE_BYTES + b * (BOX_ROWS * BK), kb * BK, u.row0 + b * BOX_ROWS);
+          }
+        }
+        __syncwarp();
+        if (++stage == stages) { stage = 0; phase ^= 1u; }
+      }
+    }
+    if (!ok && lane == 0 && p.status) atomicCAS(p.status, ST_OK, ST_TIMEOUT_PRODUCER);
+  } else if (warp == 1) {
+    // ---- MMA issuer ---------------------------------------------------------------------------
+    const bool elected = elect_one();
+    int stage = 0, acc = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    while (ok && walk.next(u)) {
+      if (elected) {
+        const uint32_t idesc = make_idesc_i8(BM, (u.rows + 15) & ~15);
+        ok = mbar_wait(smem_u32(&ss.acc_empty[acc]), acc_phase ^ 1u, abort_flag);
+        tc_fence_after();
+        for (int kb = kb_begin; ok && kb < kb_end; ++kb) {
+          if (!mbar_wait(smem_u32(&ss.full[stage]), phase, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t w_addr = smem_u32(smem + stage * stage_size);
+          const uint64_t a_desc = make_smem_desc(w_addr, 16, 1024);
+          const uint64_t b_desc = make_smem_desc(w_addr + W_STAGE_BYTES, 16, 1024);
+#pragma unroll
+          for (int k4 = 0; k4 < BK / UMMA_K; ++k4)
+            umma_i8<1>(tmem_base + acc * MAX_NT, a_desc + ((k4 * UMMA_K) >> 4), b_desc + ((k4 * UMMA_K) >> 4), idesc,
+                       (kb > kb_begin || k4 > 0) ? 1u : 0u);
+          umma_commit(smem_u32(&ss.empty[stage]));
+          if (++stage == stages) { stage = 0; phase ^= 1u; }
+        }
+        if (ok) umma_commit(smem_u32(&ss.acc_full[acc]));
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+    }
+    if (!ok && lane == 0 && p.status) atomicCAS(p.status, ST_OK, ST_TIMEOUT_MMA);
+  } else if (warp >= FIRST_GATHER_WARP) {
+    // ---- row gather; without one, the rows that no expert has ---------------------------------
+    if (gathered) {
+      const int gt = threadIdx.x - 32 * FIRST_GATHER_WARP;
+      const bool issuer = (gt & 3) == 0;
+      const int j = gt >> 2;  // rows 4j .. 4j + 3 of the unit
+      int stage = 0;
+      uint32_t phase = 0;
+      while (ok && walk.next(u)) {
+        const bool mine = issuer && 4 * j < u.rows;
+        int r4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int s = mine && 4 * j + i < u.rows ? source_row(p, u.row0 + 4 * j + i) : -1;
+          r4[i] = s >= 0 ? s : p.x_rows;  // an index out of range delivers zeros
+        }
+        for (int kb = kb_begin; kb < kb_end; ++kb) {
+          if (!mbar_wait_warp(smem_u32(&ss.empty[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
+          if (mine)
+            tma_gather4(&tmX, smem_u32(&ss.full[stage]), smem_u32(smem + stage * stage_size) + W_STAGE_BYTES + j * 512,
+                        kb * BK, r4[0], r4[1], r4[2], r4[3]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&ss.full[stage]));  // also where the warp has no rows: see gemm_skinny.cuh
+          if (++stage == stages) { stage = 0; phase ^= 1u; }
+        }
+      }
+      if (!ok && lane == 0 && p.status) atomicCAS(p.status, ST_OK, ST_TIMEOUT_PRODUCER);
+    }
+    if (p.zero_others) zero_other_rows(p, GATHER_WARPS * blockIdx.x + (warp - FIRST_GATHER_WARP), GATHER_WARPS * gridDim.x);
+  } else if constexpr (!SPLIT) {
+    // ---- epilogue -----------------------------------------------------------------------------
+    const int quad = warp & 3;
+    const int half = (warp - FIRST_EPI_WARP) >> 2;
+    const uint32_t my_stage = smem_u32(stage_out) + (warp - FIRST_EPI_WARP) * STAGE_ROWS_BYTES;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    while (ok && walk.next(u)) {
+      if (!mbar_wait_warp(smem_u32(&ss.acc_full[acc]), acc_phase, abort_flag)) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t t_addr = tmem_base + acc * MAX_NT + (static_cast<uint32_t>(quad * 32) << 16);
+      const int f = u.f0 + quad * 32;
+      const auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ss.acc_empty[acc]));
+      };
+      const bool works = 32 * half < u.rows && f < p.N;
+      if (!works) release();
+      for (int c = half; works && 32 * c < u.rows; c += 2) {
+        uint32_t v[32];
+        tmem_ld32(t_addr + 32 * c, v);
+        tmem_ld_wait();
+        if (32 * (c + 2) >= u.rows) release();
+        store_rows<MODE>(p, my_stage, lane, u.e, f, u.row0 + 32 * c, u.rows - 32 * c, v);
+      }
+      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+    }
+    if (!ok && lane == 0 && p.status) atomicCAS(p.status, ST_OK, ST_TIMEOUT_EPILOGUE);
+  }
+
+  if constexpr (SPLIT) {
+    // The cluster's unit: every CTA lays its sums out in its own shared memory (the stages have been read when they are
+    // complete), row by row; then each adds up an equal share of the rows over all CTAs and stores it.  32-bit integers: the
+    // order does not matter.  All threads of all CTAs meet in both cluster barriers, also after a wait that was abandoned.
+    Walker again(p, ss, lane, nt, split);
+    const bool have = again.next(u);
+    const int quad = warp & 3;
+    const bool epilogue = warp >= FIRST_EPI_WARP && warp < FIRST_GATHER_WARP;
+    const int part = (warp - FIRST_EPI_WARP) >> 2;
+    if (epilogue && have) {
+      ok = mbar_wait_warp(smem_u32(&ss.acc_full[0]), 0, abort_flag);
+      if (ok) {
+        tc_fence_after();
+        const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+        for (int c = part; 32 * c < u.rows; c += 2) {
+          uint32_t v[32];
+          tmem_ld32(t_addr + 32 * c, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) st_shared_word(smem_u32(smem) + ((32 * c + j) * BM + quad * 32 + lane) * 4, v[j]);
+        }
+        tc_fence_before();
+      } else if (lane == 0 && p.status) {
+        atomicCAS(p.status, ST_OK, ST_TIMEOUT_EPILOGUE);
+      }
+    }
+    cluster_sync_diverged();
+    if (epilogue && have && ok) {
+      const uint32_t my_stage = smem_u32(stage_out) + (warp - FIRST_EPI_WARP) * STAGE_ROWS_BYTES;
+      const int share = (u.rows + split - 1) / split;  // rows of this CTA; half of them for each of a quadrant's two warps
+      const int each = (share + 1) / 2;
+      const int begin = min(slice * share + part * each, u.rows), end = min(min(begin + each, (slice + 1) * share), u.rows);
+      const int f = u.f0 + quad * 32;
+      for (int r0 = begin; r0 < end && f < p.N; r0 += 32) {
+        uint32_t v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = 0u;
+        for (int c = 0; c < split; ++c) {
+          const uint32_t src = map_to_cta(smem_u32(smem), c) + (r0 * BM + quad * 32 + lane) * 4;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if (r0 + j < end) {
+              uint32_t w;
+              asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(w) : "r"(src + j * BM * 4) : "memory");
+              v[j] += w;
+            }
+          }
+        }
+        store_rows<MODE>(p, my_stage, lane, u.e, f, u.row0 + r0, end - r0, v);
+      }
+    }
+    cluster_sync_diverged();  // no CTA leaves while another reads its sums
+  }
+
+  // ---- tear-down ----------------------------------------------------------------------------
+  __syncwarp();
+  if (*abort_flag != 0) {
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 2 * MAX_NT);
+  }
+}
+
+}  // namespace units
+}  // namespace i8
+}  // namespace smoe

@@ -158,6 +158,7 @@ static int quantize(const void* x, long long ld, int dtype, void* q, long long q
 // ----------------------------------------------------------------------------------------------
 // A block takes up to 8 rows of one expert and 32 channels: its rows lie in shared memory, 4096 columns at a time; a warp has
 // four channels, whose weights its lanes load 16 bytes each, straight from memory.  The weights are read once for 8 rows.
+constexpr int kDotMaxRows = 8;
 constexpr int kDotRows = 8, kDotChannels = 4, kDotWarps = 8, kDotChunk = 4096;
 
 __global__ void __launch_bounds__(32 * kDotWarps) dot_kernel(const int8_t* xq, long long x_ld, const int8_t* wq, long long w_ld,
@@ -301,6 +302,8 @@ int smoe_int8_linear(const void* x, long long ld, int x_dtype, const float* x_sc
   if (type_bytes(out_dtype) == 0 || (bias != nullptr && type_bytes(bias_dtype) == 0)) return SMOE_ERR_DTYPE;
   if (x_rows < 0 || rows < 0 || N <= 0 || cols <= 0 || cols > kMaxCols || E <= 0 || E > kMaxExpertRows || ld < 0 || w_ld < cols)
     return SMOE_ERR_SHAPE;
+  if (static_cast<long long>(E) * N > 0x7fffff00ll) return SMOE_ERR_SHAPE;
+  if (x_dtype == SMOE_I8 && x_rows > 0 && ld < cols) return SMOE_ERR_SHAPE;
   if (activation < kNoActivation || activation > ACT_SILU || (activation >= 0 && act_is_gated(activation) && N % 2 != 0)) return SMOE_ERR_SHAPE;
   if (expert_frequency_offset == nullptr && (E != 1 || expert_frequency != nullptr)) return SMOE_ERR_SHAPE;
   if (x_gather_idx == nullptr && x_rows != rows) return SMOE_ERR_SHAPE;
@@ -332,9 +335,11 @@ int smoe_int8_linear(const void* x, long long ld, int x_dtype, const float* x_sc
   p.out = out; p.out_type = out_dtype; p.activation = activation;
   p.wide_out = !misaligned(out, 16) && out_cols * type_bytes(out_dtype) % 16 == 0;
   p.status = status;
+  if (rows > kDotMaxRows && x_rows > 0) return tensor_core_product(xq, ld, static_cast<const int8_t*>(wq), w_ld, p, S(stream));
+  p.zero_others = 1;
   const long long chunks = (static_cast<long long>(rows) + kDotRows - 1) / kDotRows + (E > 1 ? (rows < E ? rows : E) : 0);
+  if (chunks > 65535) return SMOE_ERR_SHAPE;  // only without any row of x
   const dim3 grid((N + kDotWarps * kDotChannels - 1) / (kDotWarps * kDotChannels), static_cast<unsigned>(chunks));
-  if (chunks > 65535) return SMOE_ERR_SHAPE;
   return launched(launch_chained(dot_kernel, grid, 32 * kDotWarps, 0, S(stream), 1, xq, ld, static_cast<const int8_t*>(wq), w_ld,
                                  static_cast<long long>(N) * w_ld, p));
 }

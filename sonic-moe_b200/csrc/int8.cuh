@@ -33,6 +33,7 @@ struct Params {
   int out_type;
   int activation;        // kNoActivation or smoe::Activation
   int wide_out;          // rows of the output start on 16-byte boundaries
+  int zero_others;       // this launch zeroes the rows that no expert has
   int* status;
 };
 
@@ -166,6 +167,9 @@ __device__ __forceinline__ void quantize_values(const RowScale& s, const float (
     for (int i = 0; i < 4 && 4 * j + i < N; ++i) w[j] |= (s.fine ? static_cast<uint32_t>(q[4 * j + i]) & 0xFFu : 0u) << (8 * i);
   }
 }
+
+// gemm_int8.cu
+int tensor_core_product(const int8_t* xq, long long ld, const int8_t* wq, long long w_ld, const Params& p, cudaStream_t st);
 
 }  // namespace i8
 }  // namespace smoe
