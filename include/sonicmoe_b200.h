@@ -440,7 +440,7 @@ size_t smoe_token_permutation_workspace_bytes(long long n, int E);
  * drops its pair.  expert_frequency (E): pairs of each expert; expert_frequency_offset (E+1): its first row, a multiple of
  * `align`, and the end of the last; x_gather_idx, s_scatter_idx (smoe_token_permutation_rows): token and flat slot of each row,
  * -1 for a row without a pair; s_reverse_scatter_idx (T,K): row of each pair, -1 for a dropped one.  E <= 4096, T * K < 2^31 -
- * 2^16.  workspace: smoe_token_permutation_workspace_bytes(T * K, E) bytes (0: may be null). */
+ * 2^16.  workspace: smoe_token_permutation_workspace_bytes(T * K, E) bytes, 16-byte aligned (0: may be null). */
 int smoe_token_permutation(const void* expert_idx, int idx_dtype, int T, int K, int E, int align, int* expert_frequency,
                            int* expert_frequency_offset, int* x_gather_idx, int* s_scatter_idx,
                            int* s_reverse_scatter_idx, void* workspace, void* stream);
@@ -481,10 +481,11 @@ int smoe_int8_quantize_rows(const void* x, long long ld, int dtype, void* q, lon
  * expert_frequency_offset (E+1): first row of every expert; NULL: E is 1 and has all rows.  expert_frequency (E) or NULL: rows
  * of every expert where they do not reach up to the next one's.  Rows of the output that no expert has become zeros.
  * x_gather_idx (rows): the row s of x that r takes (outside [0, x_rows): a row of zeros), or NULL: s = r and x_rows = rows.
+ * rows > 0 needs x_rows > 0.
  * activation: -1 for none, or the codes above; gated ones take the channels 2j and 2j + 1 as gate and up.  out (rows, N), or
  * (rows, N / 2) with a gated activation, packed, SMOE_F32, SMOE_BF16 or SMOE_F16.
  * cols <= 131071, E <= 1024.  workspace: smoe_int8_linear_workspace_bytes bytes, 256-byte aligned (0: may be NULL). */
-size_t smoe_int8_linear_workspace_bytes(int x_dtype, int x_rows, int cols);
+size_t smoe_int8_linear_workspace_bytes(int x_dtype, int x_rows, int rows, int cols);
 int smoe_int8_linear(const void* x, long long ld, int x_dtype, const float* x_scale, const void* wq, long long w_ld,
                      const float* w_scale, const void* bias, int bias_dtype, void* out, int out_dtype,
                      const int* expert_frequency_offset, const int* expert_frequency, const int* x_gather_idx, int x_rows,

@@ -72,7 +72,7 @@ static int launch_tiles(const CUtensorMap& tmA, const CUtensorMap& tmB, const Pa
 }
 
 template <int MODE, bool SPLIT>
-static int launch_units(const CUtensorMap& tmW, const CUtensorMap& tmX, const Params& p, int most, int nt, int split, int clusters,
+static int launch_units(const CUtensorMap& tmW, const CUtensorMap& tmX, const Params& p, const int8_t* wq, long long w_ld, int most, int nt, int split, int clusters,
                         cudaStream_t st) {
   static PerDeviceFlag configured;
   const auto kernel = units::int8_unit_kernel<MODE, SPLIT>;
@@ -83,7 +83,7 @@ static int launch_units(const CUtensorMap& tmW, const CUtensorMap& tmX, const Pa
   const int stages = units::num_stages(nt);
   const unsigned grid = SPLIT ? static_cast<unsigned>(clusters * split) : static_cast<unsigned>(sms);
   return launched(launch_chained(kernel, dim3(grid), units::THREADS, units::smem_bytes(nt, stages), st, static_cast<unsigned>(split), tmW,
-                                 tmX, p, most, nt, stages, split));
+                                 tmX, p, wq, w_ld, most, nt, stages, split));
 }
 
 // Which kernels take the rows: units of `unit` rows (0: none) for experts with at most `most`, tiles for the others.
@@ -99,10 +99,10 @@ static Choice choose(const Params& p, int sms) {
   const auto bound = [&](int nt) { return (p.E == 1 ? (p.rows + nt - 1) / nt : p.rows / nt + used) * blocks; };
   const double mean = static_cast<double>(p.rows) / p.E;
   if (p.E == 1) {
-    // one load only: units of 128 rows cost half a tile each; the smaller number of rounds over the device wins
-    const long long u = (p.rows + 127) / 128 * blocks;
-    const long long t = (static_cast<long long>(p.rows) + 255) / 256 * ((p.N + 255) / 256);
-    if ((u + sms - 1) / sms >= 2 * ((t + sms / 2 - 1) / (sms / 2))) return c;
+    // one load only: units where there are at most two per SM and they need fewer rounds than the tiles, which take twice as long
+    const long long u = (p.rows + 127ll) / 128 * blocks;
+    const long long t = (p.rows + 255ll) / 256 * ((p.N + 255) / 256);
+    if (u > 2ll * sms || (u + sms - 1) / sms >= 2 * ((t + sms / 2 - 1) / (sms / 2))) return c;
     c.unit = p.rows <= 32 ? 32 : p.rows <= 64 ? 64 : 128;
     c.most = p.rows;
   } else {
@@ -141,8 +141,8 @@ static int run(const int8_t* xq, long long ld, const int8_t* wq, long long w_ld,
     rc = encode_rows(&tmX, xq, p.x_rows, p.K, ld, p.gather != nullptr ? 1 : units::BOX_ROWS);
     if (rc != SMOE_OK) return rc;
     p.zero_others = 1;
-    rc = c.split > 1 ? launch_units<MODE, true>(tmW, tmX, p, c.most, c.unit, c.split, c.clusters, st)
-                     : launch_units<MODE, false>(tmW, tmX, p, c.most, c.unit, 1, 0, st);
+    rc = c.split > 1 ? launch_units<MODE, true>(tmW, tmX, p, wq, w_ld, c.most, c.unit, c.split, c.clusters, st)
+                     : launch_units<MODE, false>(tmW, tmX, p, wq, w_ld, c.most, c.unit, 1, 0, st);
     if (rc != SMOE_OK || c.most >= p.rows) return rc;
   }
   rc = encode_rows(&tmX, xq, p.x_rows, p.K, ld, p.gather != nullptr ? 1 : tiles::BM);

@@ -217,29 +217,33 @@ struct Walker {
   }
 };
 
-// 32 channels of the warp's 32 rows: lane l has row l's sums in v.
-template <int MODE>
-__device__ __forceinline__ void store_columns(const Params& p, uint32_t stage, int lane, int row_base, int row_end, int e, int n,
-                                              const uint32_t (&v)[32], float xs) {
-  float f[32];
-  const long long at = static_cast<long long>(e) * p.N + n;
-  if (n + 32 <= p.N && reinterpret_cast<uintptr_t>(p.w_scale + at) % 16 == 0) {  // every lane reads the same words
-    const float4* w = reinterpret_cast<const float4*>(p.w_scale + at);
+// 32 values, one per lane, as every lane's f, through the warp's staging rows: with loads of whole words from memory by all lanes,
+// behind the accumulator, a tile of a short reduction waited 2.5 kilocycles for each 32 channels.
+__device__ __forceinline__ void broadcast32(uint32_t stage, int lane, float mine, float (&f)[32]) {
+  st_shared_word(stage + 4 * lane, __float_as_uint(mine));
+  __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float4 s = w[j];
-      f[4 * j] = s.x; f[4 * j + 1] = s.y; f[4 * j + 2] = s.z; f[4 * j + 3] = s.w;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) f[j] = n + j < p.N ? p.w_scale[at + j] : 0.f;
+  for (int j = 0; j < 8; ++j) {
+    const uint4 v = ld_shared_v4(stage + 16 * j);
+    f[4 * j] = __uint_as_float(v.x); f[4 * j + 1] = __uint_as_float(v.y);
+    f[4 * j + 2] = __uint_as_float(v.z); f[4 * j + 3] = __uint_as_float(v.w);
   }
+  __syncwarp();
+}
+
+// 32 channels of the warp's 32 rows: lane l has row l's sums in v, and channel n + l's scale and bias.
+template <int MODE>
+__device__ __forceinline__ void store_columns(const Params& p, uint32_t stage, int lane, int row_base, int row_end, int n,
+                                              const uint32_t (&v)[32], float xs, float ws, float bias) {
+  float f[32];
+  broadcast32(stage, lane, ws, f);
 #pragma unroll
   for (int j = 0; j < 32; ++j) f[j] = scaled(static_cast<int>(v[j]), xs, f[j]);
   if (p.bias != nullptr) {
+    float b[32];
+    broadcast32(stage, lane, bias, b);
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (n + j < p.N) f[j] += load_typed(p.bias, p.bias_type, at + j);
+    for (int j = 0; j < 32; ++j) f[j] += b[j];
   }
   const bool gated = is_gated<MODE>(p);
   const long long cols = gated ? p.N / 2 : p.N;
@@ -453,6 +457,15 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         const int s = source_row(p, r);
         if (s >= 0) xs = p.x_scale[s];
       }
+      const bool works = n_first < p.N && row_base < tile.row_end;
+      float ws[COLS_PER_WARP / 32], bias[COLS_PER_WARP / 32];  // of the channels 32 c + lane
+#pragma unroll
+      for (int c = 0; c < COLS_PER_WARP / 32; ++c) {
+        const int n = n_first + 32 * c + lane;
+        const long long at = static_cast<long long>(tile.e) * p.N + n;
+        ws[c] = works && n < p.N ? p.w_scale[at] : 0.f;
+        bias[c] = works && n < p.N && p.bias != nullptr ? load_typed(p.bias, p.bias_type, at) : 0.f;
+      }
       if (!mbar_wait_warp(smem_u32(&ss.acc_full[acc]), acc_phase, abort_flag)) { ok = false; break; }
       tc_fence_after();
       const auto release = [&] {
@@ -460,7 +473,6 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&ss.acc_empty[acc]), 0));
       };
-      const bool works = n_first < p.N && row_base < tile.row_end;
       if (!works) release();
       const uint32_t t_addr = tmem_base + acc * BN + col_half * COLS_PER_WARP + (static_cast<uint32_t>(quad * 32) << 16);
 #pragma unroll 1
@@ -469,9 +481,11 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         if (n >= p.N) break;
         uint32_t v[32];
         tmem_ld32(t_addr + 32 * c, v);
+        const float w = c < 2 ? c < 1 ? ws[0] : ws[1] : c < 3 ? ws[2] : ws[3];
+        const float b = c < 2 ? c < 1 ? bias[0] : bias[1] : c < 3 ? bias[2] : bias[3];
         tmem_ld_wait();
         if (c + 1 == COLS_PER_WARP / 32 || n + 32 >= p.N) release();
-        store_columns<MODE>(p, my_stage, lane, row_base, tile.row_end, tile.e, n, v, xs);
+        store_columns<MODE>(p, my_stage, lane, row_base, tile.row_end, n, v, xs, w, b);
       }
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
@@ -527,6 +541,7 @@ __host__ __device__ constexpr int num_stages(int nt) {
   return fit < MAX_STAGES ? fit : MAX_STAGES;
 }
 // SPLIT: a CTA's sums of a whole unit, 32-bit integers, take the stages' place
+static_assert(MAX_NT / 2 <= 64, "a share of a unit's rows, by two warps of 32");
 static_assert(num_stages(MAX_NT) * stage_bytes(MAX_NT) >= MAX_NT * BM * 4 && num_stages(32) * stage_bytes(32) >= 32 * BM * 4, "room for the sums");
 
 struct Unit {
@@ -562,21 +577,25 @@ struct Walker {
   }
 };
 
+// Scale and bias of channel f + lane; scale of row row0 + lane.  Loaded before the sums are waited for.
+__device__ __forceinline__ void load_channel(const Params& p, int e, int f, int lane, float& ws, float& bias) {
+  const bool mine = f + lane < p.N;
+  const long long at = static_cast<long long>(e) * p.N + f + lane;
+  ws = mine ? p.w_scale[at] : 0.f;
+  bias = mine && p.bias != nullptr ? load_typed(p.bias, p.bias_type, at) : 0.f;
+}
+__device__ __forceinline__ float load_row_scale(const Params& p, int row0, int rows, int lane) {
+  if (lane >= rows) return 0.f;
+  const int s = source_row(p, row0 + lane);
+  return s >= 0 ? p.x_scale[s] : 0.f;
+}
+
 // 32 channels (lane l: channel f + l) of up to 32 rows (word j: row row0 + j), of which `rows` exist.  Neighbouring lanes exchange
 // half of their values: afterwards word j of an even lane has the channels (l, l + 1) of row 2j and that of an odd one (l - 1, l) of
 // row 2j + 1, a gate and its up value, or two values of one 32-bit store.
 template <int MODE>
-__device__ __forceinline__ void store_rows(const Params& p, uint32_t stage, int lane, int e, int f, int row0, int rows,
-                                           const uint32_t (&v)[32]) {
-  const bool mine = f + lane < p.N;
-  const long long at = static_cast<long long>(e) * p.N + f + lane;
-  const float ws = mine ? p.w_scale[at] : 0.f;
-  const float bias = mine && p.bias != nullptr ? load_typed(p.bias, p.bias_type, at) : 0.f;
-  float xs = 0.f;
-  if (lane < rows) {
-    const int s = source_row(p, row0 + lane);
-    if (s >= 0) xs = p.x_scale[s];
-  }
+__device__ __forceinline__ void store_rows(const Params& p, uint32_t stage, int lane, int f, int row0, int rows,
+                                           const uint32_t (&v)[32], float ws, float bias, float xs) {
   const bool odd = lane & 1;
   const bool gated = is_gated<MODE>(p);
   float lo[16], hi[16];
@@ -642,8 +661,8 @@ __device__ __forceinline__ void store_rows(const Params& p, uint32_t stage, int 
 // there are at least as many clusters as units.
 template <int MODE, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
-int8_unit_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Params p, const int most,
-                 const int nt, const int stages, const int split) {
+int8_unit_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Params p, const int8_t* wq,
+                 const long long w_ld, const int most, const int nt, const int stages, const int split) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int stage_size = stage_bytes(nt);
@@ -675,6 +694,14 @@ int8_unit_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
   if (warp == 1) {
     tmem_alloc(smem_u32(&ss.tmem_base), 2 * MAX_NT);
     tmem_relinquish();
+  }
+  // One expert: this CTA's weights are known before anything else is.  The L2 fetches them while the previous kernel, as a rule
+  // the one that quantises x, still runs; nothing is read into the block, so nothing can be stale.
+  if (SPLIT && p.off == nullptr && warp >= FIRST_EPI_WARP) {
+    const int tiles = (p.rows + nt - 1) / nt, f0 = static_cast<int>(blockIdx.x) / split / tiles * BM;
+    const int lines = kb_end - kb_begin, all = min(BM, p.N - f0) * lines;
+    for (int i = threadIdx.x - 32 * FIRST_EPI_WARP; i < all; i += THREADS - 32 * FIRST_EPI_WARP)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(wq + (f0 + i / lines) * w_ld + static_cast<long long>(kb_begin + i % lines) * BK));
   }
   wait_for_previous();
   if (warp == 2) {
@@ -780,10 +807,15 @@ int8_unit_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     int acc = 0;
     uint32_t acc_phase = 0;
     while (ok && walk.next(u)) {
+      const int f = u.f0 + quad * 32;
+      float ws, bias;
+      load_channel(p, u.e, f, lane, ws, bias);
+      // a warp has the rows 32 half .. and 32 (half + 2) .. of the unit
+      const float xs0 = load_row_scale(p, u.row0 + 32 * half, u.rows - 32 * half, lane);
+      const float xs1 = load_row_scale(p, u.row0 + 32 * half + 64, u.rows - 32 * half - 64, lane);
       if (!mbar_wait_warp(smem_u32(&ss.acc_full[acc]), acc_phase, abort_flag)) { ok = false; break; }
       tc_fence_after();
       const uint32_t t_addr = tmem_base + acc * MAX_NT + (static_cast<uint32_t>(quad * 32) << 16);
-      const int f = u.f0 + quad * 32;
       const auto release = [&] {
         tc_fence_before();
         __syncwarp();
@@ -796,7 +828,7 @@ int8_unit_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
         tmem_ld32(t_addr + 32 * c, v);
         tmem_ld_wait();
         if (32 * (c + 2) >= u.rows) release();
-        store_rows<MODE>(p, my_stage, lane, u.e, f, u.row0 + 32 * c, u.rows - 32 * c, v);
+        store_rows<MODE>(p, my_stage, lane, f, u.row0 + 32 * c, u.rows - 32 * c, v, ws, bias, c == half ? xs0 : xs1);
       }
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
@@ -812,6 +844,17 @@ int8_unit_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     const int quad = warp & 3;
     const bool epilogue = warp >= FIRST_EPI_WARP && warp < FIRST_GATHER_WARP;
     const int part = (warp - FIRST_EPI_WARP) >> 2;
+    const int share = (u.rows + split - 1) / split;  // rows of this CTA; half of them, at most 32, for each of a quadrant's two warps
+    const int each = (share + 1) / 2;
+    const int begin = have ? min(slice * share + part * each, u.rows) : 0;
+    const int count = have ? min(min(begin + each, (slice + 1) * share), u.rows) - begin : 0;
+    const int f = u.f0 + quad * 32;
+    const bool works = epilogue && have && count > 0 && f < p.N;
+    float ws = 0.f, bias = 0.f, xs = 0.f;
+    if (works) {
+      load_channel(p, u.e, f, lane, ws, bias);
+      xs = load_row_scale(p, u.row0 + begin, count, lane);
+    }
     if (epilogue && have) {
       ok = mbar_wait_warp(smem_u32(&ss.acc_full[0]), 0, abort_flag);
       if (ok) {
@@ -830,29 +873,23 @@ int8_unit_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
       }
     }
     cluster_sync_diverged();
-    if (epilogue && have && ok) {
+    if (works && ok) {
       const uint32_t my_stage = smem_u32(stage_out) + (warp - FIRST_EPI_WARP) * STAGE_ROWS_BYTES;
-      const int share = (u.rows + split - 1) / split;  // rows of this CTA; half of them for each of a quadrant's two warps
-      const int each = (share + 1) / 2;
-      const int begin = min(slice * share + part * each, u.rows), end = min(min(begin + each, (slice + 1) * share), u.rows);
-      const int f = u.f0 + quad * 32;
-      for (int r0 = begin; r0 < end && f < p.N; r0 += 32) {
-        uint32_t v[32];
+      uint32_t v[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = 0u;
-        for (int c = 0; c < split; ++c) {
-          const uint32_t src = map_to_cta(smem_u32(smem), c) + (r0 * BM + quad * 32 + lane) * 4;
+      for (int j = 0; j < 32; ++j) v[j] = 0u;
+      for (int c = 0; c < split; ++c) {
+        const uint32_t src = map_to_cta(smem_u32(smem), c) + (begin * BM + quad * 32 + lane) * 4;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            if (r0 + j < end) {
-              uint32_t w;
-              asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(w) : "r"(src + j * BM * 4) : "memory");
-              v[j] += w;
-            }
+        for (int j = 0; j < 32; ++j) {
+          if (j < count) {
+            uint32_t w;
+            asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(w) : "r"(src + j * BM * 4) : "memory");
+            v[j] += w;
           }
         }
-        store_rows<MODE>(p, my_stage, lane, u.e, f, u.row0 + r0, end - r0, v);
       }
+      store_rows<MODE>(p, my_stage, lane, f, u.row0 + begin, count, v, ws, bias, xs);
     }
     cluster_sync_diverged();  // no CTA leaves while another reads its sums
   }

@@ -17,21 +17,29 @@ static inline cudaStream_t S(void* s) { return static_cast<cudaStream_t>(s); }
 // ----------------------------------------------------------------------------------------------
 // quantisation
 // ----------------------------------------------------------------------------------------------
-// A row is read once, PIECES accesses of BYTES bytes per thread, and stays in registers between the maximum and the
-// conversion; `tpr` threads (a power of two) share it, and a block of 256 threads (or one row's) has 256 / tpr rows.  Rows that
-// are longer than 1024 threads hold are read twice.  Bound by memory.
-template <class T, int BYTES>
+// A row is read once and stays in registers between the maximum and the conversion: PIECES pieces of N values per thread, `tpr`
+// threads (a power of two) per row, and a block of 256 threads (or one row's) has 256 / tpr rows.  Rows that are longer than 1024
+// threads hold are read twice.  Bound by memory: what is read is 2 or 4 times what is written.  WIDE: rows that start on 16-byte
+// boundaries and end on them, one load per piece; otherwise a piece's four values are loaded one by one (its neighbours' come from
+// the same lines), and it is still stored in one word.
+template <class T, bool WIDE>
 struct Loaded {
-  static constexpr int N = BYTES / static_cast<int>(sizeof(T));
-  uint32_t w[BYTES >= 4 ? BYTES / 4 : 1];
-  __device__ __forceinline__ void load(const T* p) {
-    if constexpr (BYTES == 16) {
+  static constexpr int N = WIDE ? 16 / static_cast<int>(sizeof(T)) : 4;
+  static constexpr int WORDS = N * static_cast<int>(sizeof(T)) / 4;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void load(const T* p, int values) {
+    if constexpr (WIDE) {
       const uint4 q = __ldcs(reinterpret_cast<const uint4*>(p));
       w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
-    } else if constexpr (BYTES == 4) {
-      w[0] = __ldcs(reinterpret_cast<const unsigned*>(p));
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = i < values ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
     } else {
-      w[0] = __ldcs(reinterpret_cast<const unsigned short*>(p));
+      uint32_t h[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[i] = i < values ? reinterpret_cast<const unsigned short*>(p)[i] : 0u;
+      w[0] = h[0] | (h[1] << 16);
+      w[1] = h[2] | (h[3] << 16);
     }
   }
   __device__ __forceinline__ void zero() {
@@ -40,41 +48,50 @@ struct Loaded {
   }
   __device__ __forceinline__ float value(int i) const {
     if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
-    const unsigned short h = static_cast<unsigned short>(w[i / 2] >> (16 * (i & 1)));
-    if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half(h));
-    return __bfloat162float(__ushort_as_bfloat16(h));
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(w[i / 2] >> (16 * (i & 1)))));
   }
-  __device__ __forceinline__ uint32_t amax_bits() const {
-    uint32_t m = 0u;
+  // the largest magnitude so far, in the type's own bits: magnitudes compare like whole numbers, a NaN above infinity
+  __device__ __forceinline__ uint32_t amax_bits(uint32_t m) const {
 #pragma unroll
-    for (int i = 0; i < N; ++i) m = max(m, __float_as_uint(value(i)) & 0x7FFFFFFFu);
+    for (int i = 0; i < WORDS; ++i) {
+      if constexpr (sizeof(T) == 4) m = max(m, w[i] & 0x7FFFFFFFu);
+      else m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+    }
     return m;
   }
   __device__ __forceinline__ void store(const RowScale& s, int8_t* q) const {
     float f[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) f[i] = value(i);
-    uint32_t o[(N + 3) / 4];
-    quantize_values<N>(s, f, o);
+    uint32_t o[N / 4];
+    quantize_values<(sizeof(T) == 2)>(s, f, o);
     if constexpr (N == 8) *reinterpret_cast<uint2*>(q) = make_uint2(o[0], o[1]);
-    else if constexpr (N == 4) *reinterpret_cast<uint32_t*>(q) = o[0];
-    else if constexpr (N == 2) *reinterpret_cast<uint16_t*>(q) = static_cast<uint16_t>(o[0]);
-    else *q = static_cast<int8_t>(o[0]);
+    else *reinterpret_cast<uint32_t*>(q) = o[0];
   }
 };
 
-template <class T, int BYTES>
+// bits of `amax_bits` (two halves for 16-bit types) -> those of the magnitude as fp32
+template <class T>
+__device__ __forceinline__ uint32_t amax_as_float_bits(uint32_t m) {
+  if constexpr (sizeof(T) == 4) return m;
+  m = max(m & 0xFFFFu, m >> 16);
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return m << 16;
+  return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
+}
+
+template <class T, bool WIDE>
 __global__ void __launch_bounds__(1024) quantize_rows_kernel(const T* x, long long ld, int8_t* q, long long q_ld, float* scale,
                                                              long long rows, int cols, int tpr) {
   release_next();
   wait_for_previous();
-  using L = Loaded<T, BYTES>;
-  constexpr int PIECES = BYTES == 16 ? 4 : 8;
+  using L = Loaded<T, WIDE>;
+  constexpr int PIECES = 4;
   __shared__ uint32_t part[32];
   const int per_block = blockDim.x / tpr, sub = threadIdx.x / tpr, tid = threadIdx.x % tpr;
   const long long row = static_cast<long long>(blockIdx.x) * per_block + sub;
   const bool live = row < rows;
-  const int pieces = (cols + L::N - 1) / L::N;  // cols is a multiple of N
+  const int pieces = (cols + L::N - 1) / L::N;
   const T* src = x + (live ? row : 0) * ld;
   const bool kept = pieces <= PIECES * tpr;
   L v[PIECES];
@@ -83,18 +100,18 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const T* x, long lo
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
       const int c = i * tpr + tid;
-      if (live && c < pieces) v[i].load(src + c * L::N); else v[i].zero();
+      if (live && c < pieces) v[i].load(src + c * L::N, cols - c * L::N); else v[i].zero();
     }
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) bits = max(bits, v[i].amax_bits());
+    for (int i = 0; i < PIECES; ++i) bits = v[i].amax_bits(bits);
   } else if (live) {
     for (int c = tid; c < pieces; c += tpr) {
-      v[0].load(src + c * L::N);
-      bits = max(bits, v[0].amax_bits());
+      v[0].load(src + c * L::N, cols - c * L::N);
+      bits = v[0].amax_bits(bits);
     }
   }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, d));  // tpr >= 32
+  bits = amax_as_float_bits<T>(bits);
+  bits = __reduce_max_sync(0xffffffffu, bits);  // tpr >= 32
   if (tpr > 32) {
     const int warp = threadIdx.x >> 5, of_row = tpr >> 5;
     if ((threadIdx.x & 31) == 0) part[warp] = bits;
@@ -113,126 +130,176 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const T* x, long lo
     }
   } else {
     for (int c = tid; c < pieces; c += tpr) {
-      v[0].load(src + c * L::N);
+      v[0].load(src + c * L::N, cols - c * L::N);
       v[0].store(s, dst + c * L::N);
     }
   }
-  for (int c = cols + tid; c < (cols + 15) / 16 * 16; c += tpr) dst[c] = 0;
+  // columns up to the next multiple of 16 are zeros
+  for (int c = pieces * L::N + 4 * tid; c < (cols + 15) / 16 * 16; c += 4 * tpr) *reinterpret_cast<uint32_t*>(dst + c) = 0u;
 }
 
-template <class T, int BYTES>
+template <class T, bool WIDE>
 static cudaError_t launch_quantize(const void* x, long long ld, void* q, long long q_ld, float* scale, long long rows, int cols,
                                    cudaStream_t st) {
-  constexpr int N = BYTES / static_cast<int>(sizeof(T)), PIECES = BYTES == 16 ? 4 : 8;
+  constexpr int N = Loaded<T, WIDE>::N, PIECES = 4;
   const int pieces = (cols + N - 1) / N;
   int tpr = 32;
   while (tpr < 1024 && tpr * PIECES < pieces) tpr *= 2;
   const int threads = tpr > 256 ? tpr : 256;
   const long long blocks = (rows + threads / tpr - 1) / (threads / tpr);
-  return launch_chained(quantize_rows_kernel<T, BYTES>, dim3(static_cast<unsigned>(blocks)), threads, 0, st, 1, static_cast<const T*>(x), ld,
+  return launch_chained(quantize_rows_kernel<T, WIDE>, dim3(static_cast<unsigned>(blocks)), threads, 0, st, 1, static_cast<const T*>(x), ld,
                         static_cast<int8_t*>(q), q_ld, scale, rows, cols, tpr);
+}
+
+template <class T>
+static cudaError_t launch_quantize(const void* x, long long ld, void* q, long long q_ld, float* scale, long long rows, int cols,
+                                   cudaStream_t st) {
+  const long long size = sizeof(T);
+  const bool wide = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld * size % 16 == 0 && cols * size % 16 == 0;
+  return wide ? launch_quantize<T, true>(x, ld, q, q_ld, scale, rows, cols, st) : launch_quantize<T, false>(x, ld, q, q_ld, scale, rows, cols, st);
 }
 
 static int quantize(const void* x, long long ld, int dtype, void* q, long long q_ld, float* scale, long long rows, int cols,
                     cudaStream_t st) {
-  const int size = dtype == SMOE_F32 ? 4 : 2;
-  const auto fits = [&](int bytes) {
-    return reinterpret_cast<uintptr_t>(x) % bytes == 0 && (ld * size) % bytes == 0 && (static_cast<long long>(cols) * size) % bytes == 0;
-  };
-  cudaError_t rc;
-  if (dtype == SMOE_F32)
-    rc = fits(16) ? launch_quantize<float, 16>(x, ld, q, q_ld, scale, rows, cols, st) : launch_quantize<float, 4>(x, ld, q, q_ld, scale, rows, cols, st);
-  else if (dtype == SMOE_BF16)
-    rc = fits(16)  ? launch_quantize<__nv_bfloat16, 16>(x, ld, q, q_ld, scale, rows, cols, st)
-         : fits(4) ? launch_quantize<__nv_bfloat16, 4>(x, ld, q, q_ld, scale, rows, cols, st)
-                   : launch_quantize<__nv_bfloat16, 2>(x, ld, q, q_ld, scale, rows, cols, st);
-  else
-    rc = fits(16)  ? launch_quantize<__half, 16>(x, ld, q, q_ld, scale, rows, cols, st)
-         : fits(4) ? launch_quantize<__half, 4>(x, ld, q, q_ld, scale, rows, cols, st)
-                   : launch_quantize<__half, 2>(x, ld, q, q_ld, scale, rows, cols, st);
-  return launched(rc);
+  if (dtype == SMOE_F32) return launched(launch_quantize<float>(x, ld, q, q_ld, scale, rows, cols, st));
+  if (dtype == SMOE_BF16) return launched(launch_quantize<__nv_bfloat16>(x, ld, q, q_ld, scale, rows, cols, st));
+  return launched(launch_quantize<__half>(x, ld, q, q_ld, scale, rows, cols, st));
 }
 
 // ----------------------------------------------------------------------------------------------
 // product by 4-way integer dot products
 // ----------------------------------------------------------------------------------------------
-// A block takes up to 8 rows of one expert and 32 channels: its rows lie in shared memory, 4096 columns at a time; a warp has
-// four channels, whose weights its lanes load 16 bytes each, straight from memory.  The weights are read once for 8 rows.
-constexpr int kDotMaxRows = 8;
-constexpr int kDotRows = 8, kDotChannels = 4, kDotWarps = 8, kDotChunk = 4096;
+// For up to 8 rows in all, where the weights are everything.  A block takes the rows of one expert (all of them: 8 at most) and 32
+// channels, a warp four of those, whose weights its lanes load 16 bytes each, straight from memory and eight loads ahead.  The
+// rows lie in shared memory, 4096 columns at a time; rows that are not 8-bit yet are quantised on the way there, by every block
+// for itself, which is a few microseconds less than a launch of its own (one token, 4096 x 4096: 13.8 + 4.1 us -> see below).
+// Bound by latency: the first loads of the weights are on their way before x is looked at.
+constexpr int kDotRows = 8,  // of an expert, and of a call that takes this kernel
+    kDotChannels = 4, kDotWarps = 8, kDotThreads = 32 * kDotWarps, kDotChunk = 4096, kDotAhead = 2;
 
-__global__ void __launch_bounds__(32 * kDotWarps) dot_kernel(const int8_t* xq, long long x_ld, const int8_t* wq, long long w_ld,
-                                                             long long w_expert, const Params p) {
-  release_next();
-  wait_for_previous();
+// TX: int8_t, or the type that x is quantised from.
+template <class TX, bool WIDE>
+__global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long x_ld, const int8_t* wq, long long w_ld,
+                                                          const Params p) {
+  constexpr bool GIVEN = std::is_same<TX, int8_t>::value;
   __shared__ __align__(16) int8_t xs[kDotRows][kDotChunk];
+  __shared__ uint32_t part[kDotRows][kDotWarps];
+  __shared__ float row_scales[kDotRows];
   __shared__ int where[3];  // expert, first row, rows
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (warp == 0) {  // the expert whose chunks of rows contain blockIdx.y
-    int before = 0, e0 = 0, mine = -1;
-    for (e0 = 0; e0 < p.E; e0 += 32) {
+  const int n0 = (blockIdx.x * kDotWarps + warp) * kDotChannels;
+  release_next();
+  if (p.off == nullptr) {  // the weights are known: the L2 fetches them while the previous kernel still runs
+    for (int j = 0; j < kDotChannels && n0 + j < p.N; ++j)
+      for (int c = 128 * lane; c < p.K; c += 4096) asm volatile("prefetch.global.L2 [%0];" ::"l"(wq + (n0 + j) * w_ld + c));
+  }
+  wait_for_previous();
+  if (warp == 0) {  // the blockIdx.y-th expert that has rows
+    if (lane == 0) where[2] = 0;
+    __syncwarp();
+    int before = 0;
+    for (int e0 = 0; e0 < p.E; e0 += 32) {
       const int e = e0 + lane;
-      const int rows = e < p.E ? max(end_row(p, e) - first_row(p, e), 0) : 0;
-      int incl = (rows + kDotRows - 1) / kDotRows;
-      const int own = incl;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += o;
-      }
-      const int at = static_cast<int>(blockIdx.y) - (before + incl - own);
-      if (at >= 0 && at < own) {
+      const int rows = e < p.E ? end_row(p, e) - first_row(p, e) : 0;
+      const unsigned some = __ballot_sync(0xffffffffu, rows > 0);
+      if (rows > 0 && before + __popc(some & ((1u << lane) - 1u)) == static_cast<int>(blockIdx.y)) {
         where[0] = e;
-        where[1] = first_row(p, e) + at * kDotRows;
-        where[2] = min(kDotRows, rows - at * kDotRows);
-        mine = e;
+        where[1] = first_row(p, e);
+        where[2] = min(rows, kDotRows);
       }
-      if (__any_sync(0xffffffffu, mine >= 0)) break;
-      before += __shfl_sync(0xffffffffu, incl, 31);
+      before += __popc(some);
+      if (before > static_cast<int>(blockIdx.y)) break;
     }
-    if (!__any_sync(0xffffffffu, mine >= 0) && lane == 0) where[2] = 0;
   }
   __syncthreads();
   const int e = where[0], row0 = where[1], rows = where[2];
-  const int n0 = (blockIdx.x * kDotWarps + warp) * kDotChannels;
   if (rows > 0) {
+    const int8_t* w0 = wq + static_cast<long long>(e) * p.N * w_ld + static_cast<long long>(n0) * w_ld;
+    uint4 w[kDotAhead][kDotChannels];
+    const auto fetch = [&](uint4 (&v)[kDotChannels], int c) {
+#pragma unroll
+      for (int j = 0; j < kDotChannels; ++j) {
+        v[j] = make_uint4(0u, 0u, 0u, 0u);
+        if (n0 + j < p.N && c < p.K) v[j] = __ldcs(reinterpret_cast<const uint4*>(w0 + j * w_ld + c));
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < kDotAhead; ++i) fetch(w[i], 16 * lane + 512 * i);
+    if constexpr (!GIVEN) {
+      using L = Loaded<TX, WIDE>;
+      for (int r = 0; r < rows; ++r) {
+        const int s = source_row(p, row0 + r);
+        uint32_t bits = 0u;
+        if (s >= 0) {
+          for (int c = threadIdx.x * L::N; c < p.K; c += kDotThreads * L::N) {
+            L v;
+            v.load(x + s * x_ld + c, p.K - c);
+            bits = v.amax_bits(bits);
+          }
+        }
+        bits = __reduce_max_sync(0xffffffffu, amax_as_float_bits<TX>(bits));
+        if (lane == 0) part[r][warp] = bits;
+      }
+    }
     int acc[kDotRows * kDotChannels];
 #pragma unroll
     for (auto& a : acc) a = 0;
     for (int k0 = 0; k0 < p.K; k0 += kDotChunk) {
-      const int kn = min(kDotChunk, (p.K - k0 + 15) / 16 * 16);  // columns up to the next 16 exist, and those of x are zeros
+      const int kn = min(kDotChunk, (p.K - k0 + 15) / 16 * 16);
       __syncthreads();
-      for (int i = threadIdx.x; i < kDotRows * (kn / 16); i += blockDim.x) {
-        const int r = i / (kn / 16), c = i % (kn / 16) * 16;
-        const int s = r < rows ? source_row(p, row0 + r) : -1;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (s >= 0) v = *reinterpret_cast<const uint4*>(xq + s * x_ld + k0 + c);
-        if (k0 + c + 16 > p.K) {  // columns past the last count as zeros, whatever the caller's buffer holds there
-          uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+      if constexpr (GIVEN) {
+        for (int i = threadIdx.x; i < rows * (kn / 16); i += kDotThreads) {
+          const int r = i / (kn / 16), c = i % (kn / 16) * 16;
+          const int s = source_row(p, row0 + r);
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (s >= 0) v = *reinterpret_cast<const uint4*>(x + s * x_ld + k0 + c);
+          if (k0 + c + 16 > p.K) {  // columns past the last count as zeros, whatever the caller's buffer holds there
+            uint32_t* b = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
-          for (int b = 0; b < 16; ++b)
-            if (k0 + c + b >= p.K) w[b / 4] &= ~(0xFFu << (8 * (b % 4)));
+            for (int i2 = 0; i2 < 16; ++i2)
+              if (k0 + c + i2 >= p.K) b[i2 / 4] &= ~(0xFFu << (8 * (i2 % 4)));
+          }
+          *reinterpret_cast<uint4*>(&xs[r][c]) = v;
         }
-        *reinterpret_cast<uint4*>(&xs[r][c]) = v;
+      } else {
+        using L = Loaded<TX, WIDE>;
+        for (int r = 0; r < rows; ++r) {
+          const int s = source_row(p, row0 + r);
+          uint32_t bits = part[r][0];
+#pragma unroll
+          for (int i = 1; i < kDotWarps; ++i) bits = max(bits, part[r][i]);
+          const RowScale sc = row_scale(bits);
+          if (threadIdx.x == 0) row_scales[r] = s >= 0 ? sc.scale : 0.f;
+          for (int c = threadIdx.x * L::N; c < kn; c += kDotThreads * L::N) {
+            L v;
+            v.zero();
+            if (s >= 0 && k0 + c < p.K) v.load(x + s * x_ld + k0 + c, p.K - k0 - c);
+            v.store(sc, &xs[r][c]);
+          }
+        }
       }
       __syncthreads();
-      for (int c = 16 * lane; c < kn; c += 512) {
-        uint4 w[kDotChannels];
+      for (int c0 = 0; c0 < kn; c0 += 512 * kDotAhead) {
 #pragma unroll
-        for (int j = 0; j < kDotChannels; ++j) {
-          w[j] = make_uint4(0u, 0u, 0u, 0u);
-          if (n0 + j < p.N) w[j] = __ldcs(reinterpret_cast<const uint4*>(wq + e * w_expert + (n0 + j) * w_ld + k0 + c));
-        }
+        for (int i = 0; i < kDotAhead; ++i) {
+          const int c = c0 + 512 * i + 16 * lane;
+          uint4 v[kDotChannels];
 #pragma unroll
-        for (int r = 0; r < kDotRows; ++r) {
-          const uint4 v = *reinterpret_cast<const uint4*>(&xs[r][c]);
+          for (int j = 0; j < kDotChannels; ++j) v[j] = w[i][j];
+          fetch(w[i], k0 + c + 512 * kDotAhead);
+          if (c >= kn) continue;
 #pragma unroll
-          for (int j = 0; j < kDotChannels; ++j) {
-            int& a = acc[r * kDotChannels + j];
-            a = __dp4a(static_cast<int>(v.x), static_cast<int>(w[j].x), a);
-            a = __dp4a(static_cast<int>(v.y), static_cast<int>(w[j].y), a);
-            a = __dp4a(static_cast<int>(v.z), static_cast<int>(w[j].z), a);
-            a = __dp4a(static_cast<int>(v.w), static_cast<int>(w[j].w), a);
+          for (int r = 0; r < kDotRows; ++r) {
+            if (r >= rows) break;
+            const uint4 q = *reinterpret_cast<const uint4*>(&xs[r][c]);
+#pragma unroll
+            for (int j = 0; j < kDotChannels; ++j) {
+              int& a = acc[r * kDotChannels + j];
+              a = __dp4a(static_cast<int>(q.x), static_cast<int>(v[j].x), a);
+              a = __dp4a(static_cast<int>(q.y), static_cast<int>(v[j].y), a);
+              a = __dp4a(static_cast<int>(q.z), static_cast<int>(v[j].z), a);
+              a = __dp4a(static_cast<int>(q.w), static_cast<int>(v[j].w), a);
+            }
           }
         }
       }
@@ -251,8 +318,14 @@ __global__ void __launch_bounds__(32 * kDotWarps) dot_kernel(const int8_t* xq, l
     const bool live = r < rows && n < p.N;
     float y = 0.f;
     if (live) {
-      const int s = source_row(p, row0 + r);
-      y = scaled(acc[0], s >= 0 ? p.x_scale[s] : 0.f, p.w_scale[static_cast<long long>(e) * p.N + n]);
+      float scale;
+      if constexpr (GIVEN) {
+        const int s = source_row(p, row0 + r);
+        scale = s >= 0 ? p.x_scale[s] : 0.f;
+      } else {
+        scale = row_scales[r];
+      }
+      y = scaled(acc[0], scale, p.w_scale[static_cast<long long>(e) * p.N + n]);
       if (p.bias != nullptr) y += load_typed(p.bias, p.bias_type, static_cast<long long>(e) * p.N + n);
     }
     const float up = __shfl_down_sync(0xffffffffu, y, 1);
@@ -264,6 +337,21 @@ __global__ void __launch_bounds__(32 * kDotWarps) dot_kernel(const int8_t* xq, l
     }
   }
   zero_other_rows(p, (blockIdx.y * gridDim.x + blockIdx.x) * kDotWarps + warp, gridDim.x * gridDim.y * kDotWarps);
+}
+
+template <class TX, bool WIDE>
+static int launch_dot(const void* x, long long ld, const void* wq, long long w_ld, const Params& p, cudaStream_t st) {
+  constexpr int channels = kDotWarps * kDotChannels;
+  const dim3 grid((p.N + channels - 1) / channels, p.rows < p.E ? p.rows : p.E);  // experts that can have rows
+  return launched(launch_chained(dot_kernel<TX, WIDE>, grid, kDotThreads, 0, st, 1, static_cast<const TX*>(x), ld,
+                                 static_cast<const int8_t*>(wq), w_ld, p));
+}
+
+template <class TX>
+static int launch_dot_of(const void* x, long long ld, const void* wq, long long w_ld, const Params& p, cudaStream_t st) {
+  const long long size = sizeof(TX);
+  const bool wide = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld * size % 16 == 0 && p.K * size % 16 == 0;
+  return wide ? launch_dot<TX, true>(x, ld, wq, w_ld, p, st) : launch_dot<TX, false>(x, ld, wq, w_ld, p, st);
 }
 
 static int type_bytes(int dtype) { return dtype == SMOE_F32 ? 4 : dtype == SMOE_BF16 || dtype == SMOE_F16 ? 2 : 0; }
@@ -289,8 +377,8 @@ int smoe_int8_quantize_rows(const void* x, long long ld, int dtype, void* q, lon
   return quantize(x, ld, dtype, q, q_ld, scale, rows, cols, S(stream));
 }
 
-size_t smoe_int8_linear_workspace_bytes(int x_dtype, int x_rows, int cols) {
-  if (x_rows <= 0 || cols <= 0 || x_dtype == SMOE_I8) return 0;
+size_t smoe_int8_linear_workspace_bytes(int x_dtype, int x_rows, int rows, int cols) {
+  if (x_rows <= 0 || rows <= kDotRows || cols <= 0 || x_dtype == SMOE_I8) return 0;
   return round256(static_cast<size_t>(x_rows) * pitch(cols)) + round256(static_cast<size_t>(x_rows) * 4);
 }
 
@@ -308,6 +396,7 @@ int smoe_int8_linear(const void* x, long long ld, int x_dtype, const float* x_sc
   if (expert_frequency_offset == nullptr && (E != 1 || expert_frequency != nullptr)) return SMOE_ERR_SHAPE;
   if (x_gather_idx == nullptr && x_rows != rows) return SMOE_ERR_SHAPE;
   if (rows == 0) return SMOE_OK;
+  if (x_rows == 0) return SMOE_ERR_SHAPE;
   if (wq == nullptr || w_scale == nullptr || out == nullptr || (x_rows > 0 && x == nullptr)) return SMOE_ERR_SHAPE;
   if (x_dtype == SMOE_I8 ? x_rows > 0 && x_scale == nullptr : x_scale != nullptr) return SMOE_ERR_SHAPE;
   const bool bytes_given = x_dtype == SMOE_I8;
@@ -316,17 +405,9 @@ int smoe_int8_linear(const void* x, long long ld, int x_dtype, const float* x_sc
       (bias != nullptr && misaligned(bias, type_bytes(bias_dtype))) || misaligned(expert_frequency_offset, 4) ||
       misaligned(expert_frequency, 4) || misaligned(x_gather_idx, 4) || misaligned(status, 4))
     return SMOE_ERR_ALIGNMENT;
-  const size_t ws = smoe_int8_linear_workspace_bytes(x_dtype, x_rows, cols);
+  const size_t ws = smoe_int8_linear_workspace_bytes(x_dtype, x_rows, rows, cols);
   if (ws > 0 && workspace == nullptr) return SMOE_ERR_WORKSPACE;
   if (ws > 0 && misaligned(workspace, 256)) return SMOE_ERR_ALIGNMENT;
-  const int8_t* xq = static_cast<const int8_t*>(x);
-  if (ws > 0) {
-    int8_t* q = static_cast<int8_t*>(workspace);
-    float* s = reinterpret_cast<float*>(q + round256(static_cast<size_t>(x_rows) * pitch(cols)));
-    const int rc = quantize(x, ld, x_dtype, q, pitch(cols), s, x_rows, cols, S(stream));
-    if (rc != SMOE_OK) return rc;
-    xq = q; ld = pitch(cols); x_scale = s;
-  }
   const long long out_cols = activation >= 0 && act_is_gated(activation) ? N / 2 : N;
   Params p = {};
   p.E = E; p.N = N; p.K = cols; p.rows = rows; p.x_rows = x_rows;
@@ -335,13 +416,24 @@ int smoe_int8_linear(const void* x, long long ld, int x_dtype, const float* x_sc
   p.out = out; p.out_type = out_dtype; p.activation = activation;
   p.wide_out = !misaligned(out, 16) && out_cols * type_bytes(out_dtype) % 16 == 0;
   p.status = status;
-  if (rows > kDotMaxRows && x_rows > 0) return tensor_core_product(xq, ld, static_cast<const int8_t*>(wq), w_ld, p, S(stream));
-  p.zero_others = 1;
-  const long long chunks = (static_cast<long long>(rows) + kDotRows - 1) / kDotRows + (E > 1 ? (rows < E ? rows : E) : 0);
-  if (chunks > 65535) return SMOE_ERR_SHAPE;  // only without any row of x
-  const dim3 grid((N + kDotWarps * kDotChannels - 1) / (kDotWarps * kDotChannels), static_cast<unsigned>(chunks));
-  return launched(launch_chained(dot_kernel, grid, 32 * kDotWarps, 0, S(stream), 1, xq, ld, static_cast<const int8_t*>(wq), w_ld,
-                                 static_cast<long long>(N) * w_ld, p));
+  if (rows <= kDotRows) {
+    p.zero_others = 1;
+    switch (x_dtype) {
+      case SMOE_I8: return launch_dot<int8_t, true>(x, ld, wq, w_ld, p, S(stream));
+      case SMOE_F32: return launch_dot_of<float>(x, ld, wq, w_ld, p, S(stream));
+      case SMOE_BF16: return launch_dot_of<__nv_bfloat16>(x, ld, wq, w_ld, p, S(stream));
+      default: return launch_dot_of<__half>(x, ld, wq, w_ld, p, S(stream));
+    }
+  }
+  const int8_t* xq = static_cast<const int8_t*>(x);
+  if (ws > 0) {
+    int8_t* q = static_cast<int8_t*>(workspace);
+    float* s = reinterpret_cast<float*>(q + round256(static_cast<size_t>(x_rows) * pitch(cols)));
+    const int rc = quantize(x, ld, x_dtype, q, pitch(cols), s, x_rows, cols, S(stream));
+    if (rc != SMOE_OK) return rc;
+    xq = q; ld = pitch(cols); p.x_scale = s;
+  }
+  return tensor_core_product(xq, ld, static_cast<const int8_t*>(wq), w_ld, p, S(stream));
 }
 
 }  // extern "C"

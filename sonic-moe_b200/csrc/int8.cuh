@@ -114,31 +114,38 @@ __device__ __forceinline__ void zero_other_rows(const Params& p, int warp, int w
 // ----------------------------------------------------------------------------------------------
 // quantisation of a row: scale = amax / 127 (1 for a row of zeros), q = 127 x / amax rounded half to even
 // ----------------------------------------------------------------------------------------------
-// x times 127 / amax in fp32 is within 127 * 2^-23 = 1.5e-5 of the quotient; where that leaves it open on which side of a
-// border it is (and for rows so small that 127 / amax overflows), the quotient is computed in 64 bits, where it is on the right
-// side: 127 x is exact there, and a quotient of two 24-bit numbers that is no half itself is further than 2^-33 from one.
+// x times 127 / amax in fp32 is within 127 * 2^-23 = 1.5e-5 of the quotient, which leaves it open on which side of a border it
+// is only where it is that near to one.  There the remainder decides: with values of at most 11 bits 127 x - q amax is exact in
+// fp32 (every fourth piece of 256 bf16 values has a border, most of them ties such as amax / 2, so this has to be cheap: with 64-bit
+// divisions 8192 rows of 4096 took 59 us); with fp32 values the quotient is computed in 64 bits, where 127 x is exact and a quotient
+// of two 24-bit numbers that is no half itself is further than 2^-33 from one.  Rows whose largest value is below 2^-120 or above
+// 2^120, where 127 / amax or 127 x leaves fp32's range, take the 64-bit quotient throughout.
 // Rows that hold an infinity or a NaN get it as their scale, and zeros: every product of theirs is NaN.
 struct RowScale {
   float amax, scale, inv;
-  bool fine;  // finite
-  bool tiny;  // every quotient in 64 bits
+  bool fine;     // finite
+  bool extreme;  // every quotient in 64 bits
 };
 // bits: the largest |x| as an integer (a NaN's are above infinity's)
 __device__ __forceinline__ RowScale row_scale(uint32_t bits) {
   RowScale s;
   s.amax = __uint_as_float(bits);
   s.fine = bits < 0x7F800000u;
-  s.tiny = bits < (7u << 23);  // 2^-120
+  s.extreme = (bits < (7u << 23) && bits != 0u) || bits >= (247u << 23);
   s.scale = bits == 0u ? 1.f : s.fine ? __fdiv_rn(s.amax, 127.f) : s.amax;
-  s.inv = s.tiny || !s.fine ? 0.f : __fdiv_rn(127.f, s.amax);
+  s.inv = s.extreme || bits == 0u ? 0.f : __fdiv_rn(127.f, s.amax);
   return s;
 }
 
 constexpr float kRoundMagic = 12582912.f;  // 1.5 * 2^23: adding it leaves the whole number in the low bits
 constexpr float kBorder = 0.5f - 1.f / 32768.f;
 
-// N values -> N bytes in the low bytes of w (four per word)
-template <int N>
+static __device__ __noinline__ int quotient64(float x, float amax) {
+  return static_cast<int>(rint(127.0 * static_cast<double>(x) / static_cast<double>(amax)));
+}
+
+// N values -> N bytes in the low bytes of w (four per word).  SHORT: values of at most 11 bits.
+template <bool SHORT, int N>
 __device__ __forceinline__ void quantize_values(const RowScale& s, const float (&f)[N], uint32_t (&w)[(N + 3) / 4]) {
   float far = 0.f;
   int q[N];
@@ -149,22 +156,27 @@ __device__ __forceinline__ void quantize_values(const RowScale& s, const float (
     q[i] = __float_as_int(m);
     far = fmaxf(far, fabsf(t - (m - kRoundMagic)));
   }
-  if (far >= kBorder || s.tiny) {
-#pragma unroll 1
+  if (s.extreme) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) q[i] = s.fine ? quotient64(f[i], s.amax) : 0;
+  } else if (far >= kBorder) {
+#pragma unroll
     for (int i = 0; i < N; ++i) {
-      float x = 0.f;
-#pragma unroll
-      for (int j = 0; j < N; ++j) x = i == j ? f[j] : x;  // registers have no index
-      const int v = s.amax > 0.f ? static_cast<int>(rint(127.0 * static_cast<double>(x) / static_cast<double>(s.amax))) : 0;
-#pragma unroll
-      for (int j = 0; j < N; ++j) q[j] = i == j ? v : q[j];
+      if constexpr (SHORT) {
+        const float whole = __int_as_float(q[i]) - kRoundMagic;
+        const float rest = fmaf(-whole, s.amax, 127.f * f[i]);
+        const float twice = 2.f * fabsf(rest);
+        if (twice > s.amax || (twice == s.amax && (q[i] & 1))) q[i] += rest > 0.f ? 1 : -1;
+      } else {
+        const float t = f[i] * s.inv;
+        if (fabsf(t - (__int_as_float(q[i]) - kRoundMagic)) >= kBorder) q[i] = quotient64(f[i], s.amax);
+      }
     }
   }
 #pragma unroll
   for (int j = 0; j < (N + 3) / 4; ++j) {
-    w[j] = 0u;
-#pragma unroll
-    for (int i = 0; i < 4 && 4 * j + i < N; ++i) w[j] |= (s.fine ? static_cast<uint32_t>(q[4 * j + i]) & 0xFFu : 0u) << (8 * i);
+    const int b0 = q[4 * j], b1 = 4 * j + 1 < N ? q[4 * j + 1] : 0, b2 = 4 * j + 2 < N ? q[4 * j + 2] : 0, b3 = 4 * j + 3 < N ? q[4 * j + 3] : 0;
+    w[j] = __byte_perm(__byte_perm(b0, b1, 0x0040), __byte_perm(b2, b3, 0x0040), 0x5410);
   }
 }
 

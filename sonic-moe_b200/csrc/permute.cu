@@ -44,7 +44,7 @@ struct Plan {
   int* token;        // (rows)
   int* slot;         // (rows)
   int* row;          // (n)
-  int* hist;         // (blocks, E): pairs of each expert in a block's chunk, then the first row of those pairs
+  int* hist;         // (E, kMaxBlocks): pairs of each expert in a block's chunk, then in the chunks before
 };
 
 // expert of pair p, or -1
@@ -167,7 +167,8 @@ __global__ void __launch_bounds__(32 * kOneWarps) permutation_one_block_kernel(c
   mark_rest(a, base, 0, 1);
 }
 
-// Chunk of block b: pairs [b * per_block, (b + 1) * per_block).
+// Chunk of block b: pairs [b * per_block, (b + 1) * per_block).  hist has kMaxBlocks words per expert, so that the scan reads and
+// writes whole lines of one expert's blocks.
 __global__ void __launch_bounds__(32 * kWarps) permutation_count_kernel(const Plan a, int per_block) {
   release_next();
   wait_for_previous();
@@ -175,41 +176,55 @@ __global__ void __launch_bounds__(32 * kWarps) permutation_count_kernel(const Pl
   for (int e = threadIdx.x; e < a.E; e += blockDim.x) smem[e] = 0;
   __syncthreads();
   const int first = blockIdx.x * per_block, end = min(a.n - first, per_block);
+#pragma unroll 8
   for (int i = threadIdx.x; i < end; i += blockDim.x) {
     const int e = expert_of(a, first + i);
     if (e >= 0) atomicAdd(&smem[e], 1);
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < a.E; e += blockDim.x) a.hist[blockIdx.x * a.E + e] = smem[e];
+  for (int e = threadIdx.x; e < a.E; e += blockDim.x) a.hist[e * kMaxBlocks + blockIdx.x] = smem[e];
 }
 
-// hist[b][e] -> first row of the pairs that block b places for expert e; counts and offsets.
+// hist[e][b] -> pairs of expert e in the blocks before b; counts and offsets.  A warp has an expert at a time, a lane four of its
+// blocks (the ones that do not exist count nothing).  With the experts' words `blocks` apart and one thread per expert, 128
+// blocks and 128 experts took 34 us.
 __global__ void __launch_bounds__(1024) permutation_scan_kernel(const Plan a, int blocks) {
   release_next();
   wait_for_previous();
   __shared__ int partial[32];
+  __shared__ int count[kMaxExperts];
+  const int lane = threadIdx.x & 31;
+  static_assert(kMaxBlocks == 128, "a warp's lanes have four blocks each");
+#pragma unroll 4
+  for (int e = threadIdx.x >> 5; e < a.E; e += 32) {
+    int4* words = reinterpret_cast<int4*>(a.hist + e * kMaxBlocks) + lane;
+    int4 v = *words;
+    if (4 * lane >= blocks) v.x = 0;
+    if (4 * lane + 1 >= blocks) v.y = 0;
+    if (4 * lane + 2 >= blocks) v.z = 0;
+    if (4 * lane + 3 >= blocks) v.w = 0;
+    const int own = v.x + v.y + v.z + v.w;
+    int incl = own;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += o;
+    }
+    const int before = incl - own;
+    *words = make_int4(before, before + v.x, before + v.x + v.y, before + v.x + v.y + v.z);
+    if (lane == 31) {
+      count[e] = incl;
+      a.count[e] = incl;
+    }
+  }
+  __syncthreads();
   int before = 0;
   for (int e0 = 0; e0 < a.E; e0 += blockDim.x) {
     const int e = e0 + threadIdx.x;
-    int c = 0;
-    if (e < a.E) {
-#pragma unroll 16
-      for (int b = 0; b < blocks; ++b) c += a.hist[b * a.E + e];
-    }
     int total;
-    const int at = before + block_scan(round_up(c, a.align), partial, &total);
+    const int at = before + block_scan(e < a.E ? round_up(count[e], a.align) : 0, partial, &total);
     before += total;
-    if (e < a.E) {
-      a.count[e] = c;
-      a.offset[e] = at;
-      int run = at;
-#pragma unroll 16
-      for (int b = 0; b < blocks; ++b) {
-        const int v = a.hist[b * a.E + e];
-        a.hist[b * a.E + e] = run;
-        run += v;
-      }
-    }
+    if (e < a.E) a.offset[e] = at;
   }
   if (threadIdx.x == 0) a.offset[a.E] = before;
 }
@@ -221,7 +236,7 @@ __global__ void __launch_bounds__(32 * kWarps) permutation_place_kernel(const Pl
   int* base = smem;                                             // (E) next row of every expert
   uint16_t* cnt = reinterpret_cast<uint16_t*>(smem + a.E);      // (kWarps, E)
   const int warp = threadIdx.x >> 5;
-  for (int e = threadIdx.x; e < a.E; e += blockDim.x) base[e] = a.hist[blockIdx.x * a.E + e];
+  for (int e = threadIdx.x; e < a.E; e += blockDim.x) base[e] = a.offset[e] + a.hist[e * kMaxBlocks + blockIdx.x];
   Plan mine = a;
   const long long end = static_cast<long long>(blockIdx.x + 1) * per_block;
   mine.n = end < a.n ? static_cast<int>(end) : a.n;
@@ -304,6 +319,12 @@ __device__ __forceinline__ void store_piece(char* p, const Piece<VEC>& v) {
 template <class T, int VEC>
 constexpr int kElems = VEC / static_cast<int>(sizeof(T));
 
+template <class T>
+__device__ __forceinline__ float half_value(uint32_t bits) {
+  if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+  else return __uint_as_float(bits << 16);
+}
+
 template <class T, int VEC>
 __device__ __forceinline__ void unpack(const Piece<VEC>& v, float (&f)[kElems<T, VEC>]) {
 #pragma unroll
@@ -311,9 +332,7 @@ __device__ __forceinline__ void unpack(const Piece<VEC>& v, float (&f)[kElems<T,
     if constexpr (sizeof(T) == 4) {
       f[i] = __uint_as_float(v.w[i]);
     } else {
-      const unsigned short h = static_cast<unsigned short>(v.w[i / 2] >> (16 * (i & 1)));
-      if constexpr (std::is_same<T, __half>::value) f[i] = __half2float(__ushort_as_half(h));
-      else f[i] = __bfloat162float(__ushort_as_bfloat16(h));
+      f[i] = half_value<T>((v.w[i / 2] >> (16 * (i & 1))) & 0xFFFFu);
     }
   }
 }
@@ -470,12 +489,26 @@ __global__ void __launch_bounds__(kThreads) collect_kernel(const Rows a) {
 // Four rows of the token are in flight at a time.  A row's dot product is added up piece by piece in a thread, then over the
 // lanes of each warp, then over the warps: always in the same order.
 constexpr int kDotRows = 4, kDotChunk = 32;
+// dot += <f, g> over the one or two values of a word (FULL: both halves of a 16-bit word); returns w g
+template <class T, bool FULL>
+__device__ __forceinline__ uint32_t dot_word(uint32_t f, uint32_t g, float w, float& dot) {
+  if constexpr (sizeof(T) == 4) {
+    dot += __uint_as_float(f) * __uint_as_float(g);
+    return __float_as_uint(w * __uint_as_float(g));
+  } else {
+    const float g0 = half_value<T>(g & 0xFFFFu), g1 = half_value<T>(g >> 16);
+    dot += half_value<T>(f & 0xFFFFu) * g0;
+    if (!FULL) return half_bits<T>(w * g0);
+    dot += half_value<T>(f >> 16) * g1;
+    return half_bits<T>(w * g0) | (half_bits<T>(w * g1) << 16);
+  }
+}
+
 template <class T, int VEC>
-__global__ void __launch_bounds__(kThreads) spread_dot_kernel(const Rows a, int pad_blocks) {
+__global__ void __launch_bounds__(kThreads, 3) spread_dot_kernel(const Rows a, int pad_blocks) {
   release_next();
   wait_for_previous();
   if (blockIdx.x < pad_blocks) return zero_rows<VEC>(a, blockIdx.x);
-  constexpr int N = kElems<T, VEC>;
   __shared__ float part[kDotChunk][kThreads / 32];
   const int t = blockIdx.x - pad_blocks;
   const int per_row = a.bytes / VEC;
@@ -500,19 +533,15 @@ __global__ void __launch_bounds__(kThreads) spread_dot_kernel(const Rows a, int 
 #pragma unroll
         for (int j = 0; j < kDotRows; ++j)
           if (r[j] >= 0) y[j] = load_piece<VEC, true>(a.row_src + r[j] * a.row_ld + at);
-        float g[N];
-        unpack<T, VEC>(load_piece<VEC, false>(src + at), g);
+        const Piece<VEC> g = load_piece<VEC, false>(src + at);
+        // word by word, the row's gradient in the place of its values: four rows of 32 bytes fit into 80 registers, and three
+        // blocks of 256 threads into an SM (with whole rows unpacked, 120 registers, T 24576, H 1536, K 8 took 223 us)
 #pragma unroll
         for (int j = 0; j < kDotRows; ++j) {
           if (r[j] < 0) continue;
-          float f[N];
-          unpack<T, VEC>(y[j], f);
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            dot[j] += f[i] * g[i];
-            f[i] = w[j] * g[i];
-          }
-          store_piece<VEC>(a.out + static_cast<long long>(r[j]) * a.bytes + at, pack<T, VEC>(f));
+          for (int i = 0; i < (VEC >= 4 ? VEC / 4 : 1); ++i) y[j].w[i] = dot_word<T, (VEC >= 4)>(y[j].w[i], g.w[i], w[j], dot[j]);
+          store_piece<VEC>(a.out + static_cast<long long>(r[j]) * a.bytes + at, y[j]);
         }
       }
 #pragma unroll
@@ -641,9 +670,10 @@ int smoe_token_permutation(const void* expert_idx, int idx_dtype, int T, int K, 
   const size_t ws = smoe_token_permutation_workspace_bytes(n, E);
   if (ws > 0 && workspace == nullptr) return SMOE_ERR_WORKSPACE;
   if (address(expert_idx) % (idx_dtype == SMOE_I64 ? 8 : 4) != 0) return SMOE_ERR_ALIGNMENT;
+  if (address(workspace) % 16 != 0) return SMOE_ERR_ALIGNMENT;
   for (const void* p : {static_cast<const void*>(expert_frequency), static_cast<const void*>(expert_frequency_offset),
                         static_cast<const void*>(x_gather_idx), static_cast<const void*>(s_scatter_idx),
-                        static_cast<const void*>(s_reverse_scatter_idx), static_cast<const void*>(workspace)})
+                        static_cast<const void*>(s_reverse_scatter_idx)})
     if (address(p) % 4 != 0) return SMOE_ERR_ALIGNMENT;
   const Plan a = {expert_idx, idx_dtype == SMOE_I64, static_cast<int>(n), K, E, align, static_cast<int>(rows),
                   expert_frequency, expert_frequency_offset, x_gather_idx, s_scatter_idx, s_reverse_scatter_idx,

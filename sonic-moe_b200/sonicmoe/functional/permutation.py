@@ -21,7 +21,6 @@ from __future__ import annotations
 from dataclasses import dataclass
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .._lib import check, lib, ptr, stream_ptr
@@ -78,9 +77,8 @@ def _check_permutation(p: TokenPermutation, dev: torch.device) -> None:
     pair, row = p.s_reverse_scatter_idx, p.s_scatter_idx
     if pair.dim() != 2 or row.dim() != 1 or pair.shape[1] == 0:
         raise ValueError("a permutation's s_reverse_scatter_idx is (T, K) and its s_scatter_idx (rows,)")
-    for t in (pair, row):
-        if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous():
-            raise ValueError(f"a permutation's index vectors are contiguous int32 tensors on {dev}")
+    if not (pair.dtype == row.dtype == torch.int32 and pair.device == row.device == dev and pair.is_contiguous() and row.is_contiguous()):
+        raise ValueError(f"a permutation's index vectors are contiguous int32 tensors on {dev}")
 
 
 def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -118,6 +116,12 @@ def _collect(rows, p: TokenPermutation, scores):
     return out
 
 
+def _refuse_second_derivative():
+    # (the decorator for it costs more than the launch)
+    if torch.is_grad_enabled():
+        raise NotImplementedError("sorted tokens have first derivatives only")
+
+
 class _Permute(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p):
@@ -126,8 +130,8 @@ class _Permute(torch.autograd.Function):
         return _spread(x, p, None)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, drows):
+        _refuse_second_derivative()
         ctx.saved_tensors  # raises where an index vector was written to since
         return _collect(drows, ctx.p, None), None
 
@@ -141,8 +145,8 @@ class _Unpermute(torch.autograd.Function):
         return _collect(rows, p, scores)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
+        _refuse_second_derivative()
         _, _, scores, rows = ctx.saved_tensors
         p = ctx.p
         if rows is None:

@@ -25,7 +25,7 @@ def test_linear_refusals(built_library):
     at = 4096
 
     def call(x=at, ld=64, x_type=1, xs=None, wq=at, w_ld=64, ws=at, bias=None, bias_type=0, out=at, out_type=1, off=at, freq=None,
-             gather=None, T=8, rows=8, N=32, cols=64, E=4, act=-1, work=at, status=at):
+             gather=None, T=16, rows=16, N=32, cols=64, E=4, act=-1, work=at, status=at):
         return lib.smoe_int8_linear(x, ld, x_type, xs, wq, w_ld, ws, bias, bias_type, out, out_type, off, freq, gather, T, rows, N, cols,
                                     E, act, work, status, None)
 
@@ -33,7 +33,7 @@ def test_linear_refusals(built_library):
     assert call(x_type=2) == call(out_type=2) == call(out_type=5) == call(bias=at, bias_type=3) == -6
     for bad in (dict(T=-1), dict(rows=-1), dict(N=0), dict(cols=0), dict(cols=131072, ld=131072, w_ld=131072), dict(E=0), dict(E=1025),
                 dict(w_ld=48), dict(ld=-1), dict(act=-2), dict(act=7), dict(act=0, N=33), dict(off=None), dict(off=None, E=1, freq=at),
-                dict(rows=9), dict(x=None), dict(wq=None), dict(ws=None), dict(out=None), dict(xs=at), dict(x_type=5)):
+                dict(rows=17), dict(rows=9), dict(gather=at, T=0), dict(given, ld=48), dict(x=None), dict(wq=None), dict(ws=None), dict(out=None), dict(xs=at), dict(x_type=5)):
         assert call(**bad) == -1, bad
     assert call(work=None) == -7
     for bad in (dict(x=at + 1), dict(given, x=at + 8), dict(given, ld=72), dict(wq=at + 8), dict(w_ld=72), dict(ws=at + 2),
@@ -42,7 +42,8 @@ def test_linear_refusals(built_library):
         assert call(**bad) == -2, bad
     assert call(T=0, rows=0) == 0
     size = lib.smoe_int8_linear_workspace_bytes
-    assert size(5, 100, 64) == 0 and size(1, 0, 64) == 0 and size(1, 100, 65) == 100 * 80 + 192 + 512
+    assert size(5, 100, 100, 64) == 0 and size(1, 0, 100, 64) == 0 and size(1, 100, 8, 64) == 0
+    assert size(1, 100, 9, 65) == 100 * 80 + 192 + 512
 
 
 def test_python_refusals(built_library):
