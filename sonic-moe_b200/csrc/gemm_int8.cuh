@@ -217,33 +217,42 @@ struct Walker {
   }
 };
 
-// 32 values, one per lane, as every lane's f, through the warp's staging rows: with loads of whole words from memory by all lanes,
-// behind the accumulator, a tile of a short reduction waited 2.5 kilocycles for each 32 channels.
-__device__ __forceinline__ void broadcast32(uint32_t stage, int lane, float mine, float (&f)[32]) {
-  st_shared_word(stage + 4 * lane, __float_as_uint(mine));
-  __syncwarp();
+// f[j] = v[j] of 32 consecutive values, the same for all lanes: whole words where they start on 16 bytes and all exist.
+__device__ __forceinline__ void load_uniform(const float* v, int exist, float (&f)[32]) {
+  if (exist >= 32 && reinterpret_cast<uintptr_t>(v) % 16 == 0) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint4 v = ld_shared_v4(stage + 16 * j);
-    f[4 * j] = __uint_as_float(v.x); f[4 * j + 1] = __uint_as_float(v.y);
-    f[4 * j + 2] = __uint_as_float(v.z); f[4 * j + 3] = __uint_as_float(v.w);
+    for (int j = 0; j < 8; ++j) {
+      const float4 q = reinterpret_cast<const float4*>(v)[j];
+      f[4 * j] = q.x; f[4 * j + 1] = q.y; f[4 * j + 2] = q.z; f[4 * j + 3] = q.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) f[j] = j < exist ? v[j] : 0.f;
   }
-  __syncwarp();
 }
 
-// 32 channels of the warp's 32 rows: lane l has row l's sums in v, and channel n + l's scale and bias.
+// Asks the L1 for `bytes` from v on (at most 512): the lines that load_uniform will read.
+__device__ __forceinline__ void prefetch_l1(const void* v, int bytes, int lane) {
+  if (128 * lane < bytes + 127 && lane < 5) {
+    const char* at = static_cast<const char*>(v) + min(128 * lane, bytes - 1);
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(at));
+  }
+}
+
+// 32 channels of the warp's 32 rows: lane l has row l's sums in v, and (with a bias) channel n + l's bias.  The scales come by loads
+// that every lane makes of the same words: they were asked for before the accumulator was waited for (without that a tile of a
+// short reduction waited 2.5 kilocycles for each 32 channels), and cost the shared memory, which feeds the MMAs, less than
+// broadcasts through the staging rows (up projection of 8192 tokens 413 and 431 us).
 template <int MODE>
-__device__ __forceinline__ void store_columns(const Params& p, uint32_t stage, int lane, int row_base, int row_end, int n,
-                                              const uint32_t (&v)[32], float xs, float ws, float bias) {
+__device__ __forceinline__ void store_columns(const Params& p, uint32_t stage, int lane, int row_base, int row_end, int e, int n,
+                                              const uint32_t (&v)[32], float xs, float bias) {
   float f[32];
-  broadcast32(stage, lane, ws, f);
+  load_uniform(p.w_scale + static_cast<long long>(e) * p.N + n, p.N - n, f);
 #pragma unroll
   for (int j = 0; j < 32; ++j) f[j] = scaled(static_cast<int>(v[j]), xs, f[j]);
   if (p.bias != nullptr) {
-    float b[32];
-    broadcast32(stage, lane, bias, b);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) f[j] += b[j];
+    for (int j = 0; j < 32; ++j) f[j] += __shfl_sync(0xffffffffu, bias, j);
   }
   const bool gated = is_gated<MODE>(p);
   const long long cols = gated ? p.N / 2 : p.N;
@@ -458,14 +467,13 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         if (s >= 0) xs = p.x_scale[s];
       }
       const bool works = n_first < p.N && row_base < tile.row_end;
-      float ws[COLS_PER_WARP / 32], bias[COLS_PER_WARP / 32];  // of the channels 32 c + lane
+      float bias[COLS_PER_WARP / 32];  // of the channels 32 c + lane
 #pragma unroll
       for (int c = 0; c < COLS_PER_WARP / 32; ++c) {
         const int n = n_first + 32 * c + lane;
-        const long long at = static_cast<long long>(tile.e) * p.N + n;
-        ws[c] = works && n < p.N ? p.w_scale[at] : 0.f;
-        bias[c] = works && n < p.N && p.bias != nullptr ? load_typed(p.bias, p.bias_type, at) : 0.f;
+        bias[c] = works && n < p.N && p.bias != nullptr ? load_typed(p.bias, p.bias_type, static_cast<long long>(tile.e) * p.N + n) : 0.f;
       }
+      if (works) prefetch_l1(p.w_scale + static_cast<long long>(tile.e) * p.N + n_first, 4 * min(COLS_PER_WARP, p.N - n_first), lane);
       if (!mbar_wait_warp(smem_u32(&ss.acc_full[acc]), acc_phase, abort_flag)) { ok = false; break; }
       tc_fence_after();
       const auto release = [&] {
@@ -481,11 +489,10 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         if (n >= p.N) break;
         uint32_t v[32];
         tmem_ld32(t_addr + 32 * c, v);
-        const float w = c < 2 ? c < 1 ? ws[0] : ws[1] : c < 3 ? ws[2] : ws[3];
         const float b = c < 2 ? c < 1 ? bias[0] : bias[1] : c < 3 ? bias[2] : bias[3];
         tmem_ld_wait();
         if (c + 1 == COLS_PER_WARP / 32 || n + 32 >= p.N) release();
-        store_columns<MODE>(p, my_stage, lane, row_base, tile.row_end, n, v, xs, w, b);
+        store_columns<MODE>(p, my_stage, lane, row_base, tile.row_end, tile.e, n, v, xs, b);
       }
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }

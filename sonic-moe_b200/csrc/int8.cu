@@ -80,8 +80,8 @@ __device__ __forceinline__ uint32_t amax_as_float_bits(uint32_t m) {
   return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
 }
 
-template <class T, bool WIDE>
-__global__ void __launch_bounds__(1024) quantize_rows_kernel(const T* x, long long ld, int8_t* q, long long q_ld, float* scale,
+template <class T, bool WIDE, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 1) quantize_rows_kernel(const T* x, long long ld, int8_t* q, long long q_ld, float* scale,
                                                              long long rows, int cols, int tpr) {
   release_next();
   wait_for_previous();
@@ -147,7 +147,7 @@ static cudaError_t launch_quantize(const void* x, long long ld, void* q, long lo
   while (tpr < 1024 && tpr * PIECES < pieces) tpr *= 2;
   const int threads = tpr > 256 ? tpr : 256;
   const long long blocks = (rows + threads / tpr - 1) / (threads / tpr);
-  return launch_chained(quantize_rows_kernel<T, WIDE>, dim3(static_cast<unsigned>(blocks)), threads, 0, st, 1, static_cast<const T*>(x), ld,
+  return launch_chained(threads == 256 ? quantize_rows_kernel<T, WIDE, 256> : quantize_rows_kernel<T, WIDE, 1024>, dim3(static_cast<unsigned>(blocks)), threads, 0, st, 1, static_cast<const T*>(x), ld,
                         static_cast<int8_t*>(q), q_ld, scale, rows, cols, tpr);
 }
 

@@ -115,38 +115,42 @@ __device__ __forceinline__ void zero_other_rows(const Params& p, int warp, int w
 // quantisation of a row: scale = amax / 127 (1 for a row of zeros), q = 127 x / amax rounded half to even
 // ----------------------------------------------------------------------------------------------
 // x times 127 / amax in fp32 is within 127 * 2^-23 = 1.5e-5 of the quotient, which leaves it open on which side of a border it
-// is only where it is that near to one.  There the remainder decides: with values of at most 11 bits 127 x - q amax is exact in
-// fp32 (every fourth piece of 256 bf16 values has a border, most of them ties such as amax / 2, so this has to be cheap: with 64-bit
-// divisions 8192 rows of 4096 took 59 us); with fp32 values the quotient is computed in 64 bits, where 127 x is exact and a quotient
-// of two 24-bit numbers that is no half itself is further than 2^-33 from one.  Rows whose largest value is below 2^-120 or above
-// 2^120, where 127 / amax or 127 x leaves fp32's range, take the 64-bit quotient throughout.
-// Rows that hold an infinity or a NaN get it as their scale, and zeros: every product of theirs is NaN.
+// is only where it is that near to one.  There the remainder 127 x - q amax decides, in exact arithmetic: with values of at most 11
+// bits fp32 holds it, with fp32 values each product is held as the sum of two.  Every fourth piece of 256 bf16 values has a
+// border, most of them ties such as amax / 2, so this has to be cheap: with 64-bit divisions 8192 rows of 4096 took 59 us.
+// Rows whose largest value is below 2^-120 or above 2^120 are multiplied by a power of two first, so that neither 127 / amax nor
+// 127 x leaves fp32's range.  Rows that hold an infinity or a NaN get it as their scale, and zeros: every product of theirs is NaN.
 struct RowScale {
-  float amax, scale, inv;
-  bool fine;     // finite
-  bool extreme;  // every quotient in 64 bits
+  float scale;     // amax / 127
+  float pre;       // power of two for the values
+  float amax;      // times pre
+  float inv;       // 127 / amax
+  uint32_t keep;   // 0: zeros
 };
 // bits: the largest |x| as an integer (a NaN's are above infinity's)
 __device__ __forceinline__ RowScale row_scale(uint32_t bits) {
   RowScale s;
-  s.amax = __uint_as_float(bits);
-  s.fine = bits < 0x7F800000u;
-  s.extreme = (bits < (7u << 23) && bits != 0u) || bits >= (247u << 23);
-  s.scale = bits == 0u ? 1.f : s.fine ? __fdiv_rn(s.amax, 127.f) : s.amax;
-  s.inv = s.extreme || bits == 0u ? 0.f : __fdiv_rn(127.f, s.amax);
+  const float amax = __uint_as_float(bits);
+  const bool some = bits != 0u && bits < 0x7F800000u;
+  s.scale = bits == 0u ? 1.f : some ? __fdiv_rn(amax, 127.f) : amax;
+  s.pre = !some ? 1.f : bits < (7u << 23) ? 18446744073709551616.f : bits >= (247u << 23) ? 1.f / 18446744073709551616.f : 1.f;  // 2^64
+  s.amax = amax * s.pre;
+  s.inv = some ? __fdiv_rn(127.f, s.amax) : 0.f;
+  s.keep = some ? 0xFFFFFFFFu : 0u;
   return s;
 }
 
 constexpr float kRoundMagic = 12582912.f;  // 1.5 * 2^23: adding it leaves the whole number in the low bits
 constexpr float kBorder = 0.5f - 1.f / 32768.f;
 
-static __device__ __noinline__ int quotient64(float x, float amax) {
-  return static_cast<int>(rint(127.0 * static_cast<double>(x) / static_cast<double>(amax)));
-}
-
-// N values -> N bytes in the low bytes of w (four per word).  SHORT: values of at most 11 bits.
+// N values -> N bytes, four per word of w.  SHORT: values of at most 11 bits.
 template <bool SHORT, int N>
-__device__ __forceinline__ void quantize_values(const RowScale& s, const float (&f)[N], uint32_t (&w)[(N + 3) / 4]) {
+__device__ __forceinline__ void quantize_values(const RowScale& s, float (&f)[N], uint32_t (&w)[N / 4]) {
+  static_assert(N % 4 == 0, "whole words");
+  if (s.pre != 1.f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] *= s.pre;
+  }
   float far = 0.f;
   int q[N];
 #pragma unroll
@@ -156,28 +160,26 @@ __device__ __forceinline__ void quantize_values(const RowScale& s, const float (
     q[i] = __float_as_int(m);
     far = fmaxf(far, fabsf(t - (m - kRoundMagic)));
   }
-  if (s.extreme) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) q[i] = s.fine ? quotient64(f[i], s.amax) : 0;
-  } else if (far >= kBorder) {
+  if (far >= kBorder) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
+      const float whole = __int_as_float(q[i]) - kRoundMagic;
+      float rest, over;  // 127 x - q amax;  twice its magnitude - amax
       if constexpr (SHORT) {
-        const float whole = __int_as_float(q[i]) - kRoundMagic;
-        const float rest = fmaf(-whole, s.amax, 127.f * f[i]);
-        const float twice = 2.f * fabsf(rest);
-        if (twice > s.amax || (twice == s.amax && (q[i] & 1))) q[i] += rest > 0.f ? 1 : -1;
+        rest = fmaf(-whole, s.amax, 127.f * f[i]);
+        over = 2.f * fabsf(rest) - s.amax;
       } else {
-        const float t = f[i] * s.inv;
-        if (fabsf(t - (__int_as_float(q[i]) - kRoundMagic)) >= kBorder) q[i] = quotient64(f[i], s.amax);
+        const float x = 127.f * f[i], x_low = fmaf(127.f, f[i], -x);
+        const float p = whole * s.amax, p_low = fmaf(whole, s.amax, -p);
+        rest = x - p;  // exact: the two are within a factor of two of one another, or p is zero
+        over = (2.f * fabsf(rest) - s.amax) + 2.f * (rest >= 0.f ? x_low - p_low : p_low - x_low);
       }
+      if (over > 0.f || (over == 0.f && (q[i] & 1))) q[i] += rest > 0.f ? 1 : -1;
     }
   }
 #pragma unroll
-  for (int j = 0; j < (N + 3) / 4; ++j) {
-    const int b0 = q[4 * j], b1 = 4 * j + 1 < N ? q[4 * j + 1] : 0, b2 = 4 * j + 2 < N ? q[4 * j + 2] : 0, b3 = 4 * j + 3 < N ? q[4 * j + 3] : 0;
-    w[j] = __byte_perm(__byte_perm(b0, b1, 0x0040), __byte_perm(b2, b3, 0x0040), 0x5410);
-  }
+  for (int j = 0; j < N / 4; ++j)
+    w[j] = s.keep & __byte_perm(__byte_perm(q[4 * j], q[4 * j + 1], 0x0040), __byte_perm(q[4 * j + 2], q[4 * j + 3], 0x0040), 0x5410);
 }
 
 // gemm_int8.cu

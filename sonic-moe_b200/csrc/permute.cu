@@ -30,8 +30,7 @@ static inline cudaStream_t S(void* s) { return static_cast<cudaStream_t>(s); }
 // ----------------------------------------------------------------------------------------------
 constexpr int kMaxExperts = 4096;
 constexpr int kMaxBlocks = 128;
-constexpr int kWarps = 8, kSteps = 8;                 // warps of a block, groups of 32 pairs that a warp keeps at a time
-constexpr int kChunk = kWarps * kSteps * 32;          // pairs that a block places at a time
+constexpr int kWarps = 8, kSteps = 8;                 // warps of a block; groups of 32 pairs that a warp has at a time, at most
 constexpr int kOneWarps = 32;                         // the form with one block
 constexpr int kOneMaxPairs = kOneWarps * kSteps * 32, kOneMaxExperts = 1024;
 
@@ -76,13 +75,14 @@ __device__ __forceinline__ int block_scan(int v, int* partial, int* total) {
   return before + incl - v;
 }
 
-// Rank of every pair of this warp's 32 * kSteps among the warp's pairs of the same expert; cnt: the warp's counters.
-__device__ __forceinline__ void rank_pairs(const Plan& a, int first, uint16_t* cnt, int (&expert)[kSteps], int (&rank)[kSteps]) {
+// Rank of every pair of this warp's 32 * steps among the warp's pairs of the same expert; cnt: the warp's counters.
+__device__ __forceinline__ void rank_pairs(const Plan& a, int first, int steps, uint16_t* cnt, int (&expert)[kSteps], int (&rank)[kSteps]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) expert[i] = expert_of(a, first + 32 * i + lane);
+  for (int i = 0; i < kSteps; ++i) expert[i] = i < steps ? expert_of(a, first + 32 * i + lane) : -1;
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
+    if (i >= steps) break;
     const int e = expert[i];
     const unsigned peers = __match_any_sync(0xffffffffu, e);
     const int before = __popc(peers & ((1u << lane) - 1u));
@@ -105,11 +105,12 @@ __device__ __forceinline__ int scan_warps(uint16_t* cnt, int E, int e, int warps
   return run;
 }
 
-__device__ __forceinline__ void place_pairs(const Plan& a, int first, const uint16_t* cnt, const int* base,
+__device__ __forceinline__ void place_pairs(const Plan& a, int first, int steps, const uint16_t* cnt, const int* base,
                                             const int (&expert)[kSteps], const int (&rank)[kSteps]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
+    if (i >= steps) break;
     const int p = first + 32 * i + lane, e = expert[i];
     if (p >= a.n) continue;
     int r = -1;
@@ -151,7 +152,7 @@ __global__ void __launch_bounds__(32 * kOneWarps) permutation_one_block_kernel(c
   const int first = warp * per_warp;
   Plan mine = a;
   mine.n = min(a.n, first + per_warp);
-  rank_pairs(mine, first, cnt + warp * a.E, expert, rank);
+  rank_pairs(mine, first, per_warp / 32, cnt + warp * a.E, expert, rank);
   __syncthreads();
   const int e = threadIdx.x;
   const int c = e < a.E ? scan_warps(cnt, a.E, e, kOneWarps) : 0;
@@ -163,7 +164,7 @@ __global__ void __launch_bounds__(32 * kOneWarps) permutation_one_block_kernel(c
   }
   if (e == 0) base[a.E] = a.offset[a.E] = total;
   __syncthreads();
-  place_pairs(mine, first, cnt + warp * a.E, base, expert, rank);
+  place_pairs(mine, first, per_warp / 32, cnt + warp * a.E, base, expert, rank);
   mark_rest(a, base, 0, 1);
 }
 
@@ -229,7 +230,8 @@ __global__ void __launch_bounds__(1024) permutation_scan_kernel(const Plan a, in
   if (threadIdx.x == 0) a.offset[a.E] = before;
 }
 
-__global__ void __launch_bounds__(32 * kWarps) permutation_place_kernel(const Plan a, int per_block) {
+// steps: groups of 32 pairs of a warp, so that a block has a chunk of 32 * steps * kWarps at a time.
+__global__ void __launch_bounds__(32 * kWarps) permutation_place_kernel(const Plan a, int per_block, int steps) {
   release_next();
   wait_for_previous();
   extern __shared__ int smem[];
@@ -240,12 +242,12 @@ __global__ void __launch_bounds__(32 * kWarps) permutation_place_kernel(const Pl
   Plan mine = a;
   const long long end = static_cast<long long>(blockIdx.x + 1) * per_block;
   mine.n = end < a.n ? static_cast<int>(end) : a.n;
-  for (int first = blockIdx.x * per_block; first < mine.n; first += kChunk) {
+  for (int first = blockIdx.x * per_block; first < mine.n; first += 32 * kWarps * steps) {
     for (int i = threadIdx.x; i < kWarps * a.E; i += blockDim.x) cnt[i] = 0;
     __syncthreads();
     int expert[kSteps], rank[kSteps];
-    const int own = first + warp * (32 * kSteps);
-    rank_pairs(mine, own, cnt + warp * a.E, expert, rank);
+    const int own = first + warp * (32 * steps);
+    rank_pairs(mine, own, steps, cnt + warp * a.E, expert, rank);
     __syncthreads();
     // a chunk's sums are added to the bases only once its pairs have been placed
     int sum[kMaxExperts / (32 * kWarps)];
@@ -255,7 +257,7 @@ __global__ void __launch_bounds__(32 * kWarps) permutation_place_kernel(const Pl
       sum[j] = e < a.E ? scan_warps(cnt, a.E, e, kWarps) : 0;
     }
     __syncthreads();
-    place_pairs(mine, own, cnt + warp * a.E, base, expert, rank);
+    place_pairs(mine, own, steps, cnt + warp * a.E, base, expert, rank);
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kMaxExperts / (32 * kWarps); ++j) {
@@ -509,6 +511,7 @@ __global__ void __launch_bounds__(kThreads, 3) spread_dot_kernel(const Rows a, i
   release_next();
   wait_for_previous();
   if (blockIdx.x < pad_blocks) return zero_rows<VEC>(a, blockIdx.x);
+  constexpr int U = pieces_per_thread(VEC);
   __shared__ float part[kDotChunk][kThreads / 32];
   const int t = blockIdx.x - pad_blocks;
   const int per_row = a.bytes / VEC;
@@ -527,21 +530,32 @@ __global__ void __launch_bounds__(kThreads, 3) spread_dot_kernel(const Rows a, i
         w[j] = r[j] >= 0 ? load_weight(a.weight, a.weight_type, p0 + kc + k0 + j) : 0.f;
         dot[j] = 0.f;
       }
-      for (int c = threadIdx.x; c < per_row; c += blockDim.x) {
-        const long long at = static_cast<long long>(c) * VEC;
-        Piece<VEC> y[kDotRows];
+      for (int c0 = threadIdx.x; c0 < per_row; c0 += U * blockDim.x) {
+        Piece<VEC> y[kDotRows][U], g[U];
 #pragma unroll
-        for (int j = 0; j < kDotRows; ++j)
-          if (r[j] >= 0) y[j] = load_piece<VEC, true>(a.row_src + r[j] * a.row_ld + at);
-        const Piece<VEC> g = load_piece<VEC, false>(src + at);
+        for (int u = 0; u < U; ++u) {
+          const int c = c0 + u * blockDim.x;
+          if (c >= per_row) continue;
+          const long long at = static_cast<long long>(c) * VEC;
+#pragma unroll
+          for (int j = 0; j < kDotRows; ++j)
+            if (r[j] >= 0) y[j][u] = load_piece<VEC, true>(a.row_src + r[j] * a.row_ld + at);
+          g[u] = load_piece<VEC, false>(src + at);
+        }
         // word by word, the row's gradient in the place of its values: four rows of 32 bytes fit into 80 registers, and three
-        // blocks of 256 threads into an SM (with whole rows unpacked, 120 registers, T 24576, H 1536, K 8 took 223 us)
+        // blocks of 256 threads into an SM (with whole rows unpacked, 120 registers, T 24576, H 1536, K 8 took 223 us, now 196)
 #pragma unroll
-        for (int j = 0; j < kDotRows; ++j) {
-          if (r[j] < 0) continue;
+        for (int u = 0; u < U; ++u) {
+          const int c = c0 + u * blockDim.x;
+          if (c >= per_row) continue;
 #pragma unroll
-          for (int i = 0; i < (VEC >= 4 ? VEC / 4 : 1); ++i) y[j].w[i] = dot_word<T, (VEC >= 4)>(y[j].w[i], g.w[i], w[j], dot[j]);
-          store_piece<VEC>(a.out + static_cast<long long>(r[j]) * a.bytes + at, y[j]);
+          for (int j = 0; j < kDotRows; ++j) {
+            if (r[j] < 0) continue;
+#pragma unroll
+            for (int i = 0; i < (VEC >= 4 ? VEC / 4 : 1); ++i)
+              y[j][u].w[i] = dot_word<T, (VEC >= 4)>(y[j][u].w[i], g[u].w[i], w[j], dot[j]);
+            store_piece<VEC>(a.out + static_cast<long long>(r[j]) * a.bytes + static_cast<long long>(c) * VEC, y[j][u]);
+          }
         }
       }
 #pragma unroll
@@ -616,7 +630,7 @@ static int launch_spread_dot(const Rows& a, int vec, cudaStream_t st) {
   return for_piece(vec, sizeof(T), [&](auto v) {
     const unsigned pad = pad_blocks(a.R);
     // as few rounds over the row as 256 threads allow, and no more threads than those rounds need
-    const int pieces = a.bytes / vec, rounds = (pieces + kThreads - 1) / kThreads;
+    const int u = pieces_per_thread(vec), pieces = (a.bytes / vec + u - 1) / u, rounds = (pieces + kThreads - 1) / kThreads;
     const unsigned threads = static_cast<unsigned>(((pieces + rounds - 1) / rounds + 31) / 32 * 32);
     return launched(launch_chained(spread_dot_kernel<T, (v < sizeof(T) ? sizeof(T) : v)>, pad + a.T, threads, 0, st, 1, a,
                                    static_cast<int>(pad)));
@@ -691,16 +705,16 @@ int smoe_token_permutation(const void* expert_idx, int idx_dtype, int T, int K, 
   }
   if (ws == 0)
     return launched(launch_chained(permutation_one_block_kernel, 1, 32 * kOneWarps, one_smem(E), S(stream), 1, a));
-  int blocks = static_cast<int>((n + kChunk - 1) / kChunk);
-  if (blocks > kMaxBlocks) blocks = kMaxBlocks;
-  if (blocks < 1) blocks = 1;
-  const long long chunks = (n + kChunk - 1) / kChunk;
-  const long long per_block = (chunks + blocks - 1) / blocks * kChunk;
-  blocks = n > 0 ? static_cast<int>((n + per_block - 1) / per_block) : 1;
-  const int per = static_cast<int>(per_block > 0 ? per_block : kChunk);
+  // as many blocks as there may be, each with a multiple of 256 pairs: with 2048 of them per block 24594 pairs took 12 blocks
+  const long long group = 32 * kWarps;
+  long long per_block = (n + kMaxBlocks - 1) / kMaxBlocks;
+  per_block = per_block > 0 ? (per_block + group - 1) / group * group : group;
+  const int steps = per_block / group < kSteps ? static_cast<int>(per_block / group) : kSteps;
+  const int blocks = n > 0 ? static_cast<int>((n + per_block - 1) / per_block) : 1;
+  const int per = static_cast<int>(per_block);
   cudaError_t rc = launch_chained(permutation_count_kernel, blocks, 32 * kWarps, E * 4, S(stream), 1, a, per);
   if (rc == cudaSuccess) rc = launch_chained(permutation_scan_kernel, 1, 1024, 0, S(stream), 1, a, blocks);
-  if (rc == cudaSuccess) rc = launch_chained(permutation_place_kernel, blocks, 32 * kWarps, place_smem(E), S(stream), 1, a, per);
+  if (rc == cudaSuccess) rc = launch_chained(permutation_place_kernel, blocks, 32 * kWarps, place_smem(E), S(stream), 1, a, per, steps);
   return launched(rc, 3);
 }
 

@@ -72,6 +72,24 @@ def test_quantize_special_rows(built_library, dtype):
     assert bool(y[8:11].isnan().all()) and not y[fine].isnan().any()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_next_to_borders(built_library, dtype):
+    """The values nearest to every border k + 1/2 of rows with random largest values: a few steps of the type to either side."""
+    from sonicmoe.functional import int8
+
+    g = torch.Generator().manual_seed(1)
+    amax = (torch.rand(400, 1, generator=g, dtype=torch.float64) + 0.5).to(dtype)
+    border = ((torch.arange(254) - 126.5) * amax.double() / 127).to(dtype)
+    bits = border.view(torch.int32 if dtype == torch.float32 else torch.int16)
+    near = torch.cat([(bits + d).view(dtype) for d in (-2, -1, 0, 1, 2)], dim=1)
+    x = torch.cat([amax, near.clamp(-amax, amax)], dim=1)
+    for scale in (1.0, 2.0 ** -130 if dtype == torch.float32 else 1.0, 2.0 ** 125 if dtype != torch.float16 else 1.0):
+        scaled = (x.double() * scale).to(dtype)
+        q, s = int8.quantize_rows(scaled.cuda())
+        want, want_scale = exact_quantize(scaled)
+        assert torch.equal(q.cpu().double(), want) and torch.equal(s.cpu(), want_scale)
+
+
 def test_quantize_leading_dimensions_and_empty(built_library):
     from sonicmoe.functional import int8
 
