@@ -82,14 +82,14 @@ __device__ __forceinline__ uint32_t amax_as_float_bits(uint32_t m) {
 
 template <class T, bool WIDE, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 1) quantize_rows_kernel(const T* x, long long ld, int8_t* q, long long q_ld, float* scale,
-                                                             long long rows, int cols, int tpr) {
+                                                             long long rows, int cols, int tpr_log2) {
   release_next();
   wait_for_previous();
   using L = Loaded<T, WIDE>;
   constexpr int PIECES = 4;
   __shared__ uint32_t part[32];
-  const int per_block = blockDim.x / tpr, sub = threadIdx.x / tpr, tid = threadIdx.x % tpr;
-  const long long row = static_cast<long long>(blockIdx.x) * per_block + sub;
+  const int tpr = 1 << tpr_log2, sub = threadIdx.x >> tpr_log2, tid = threadIdx.x & (tpr - 1);
+  const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x >> tpr_log2) + sub;
   const bool live = row < rows;
   const int pieces = (cols + L::N - 1) / L::N;
   const T* src = x + (live ? row : 0) * ld;
@@ -119,9 +119,9 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 1) quantize_rows
     for (int w = 0; w < of_row; ++w) bits = max(bits, part[sub * of_row + w]);
   }
   if (!live) return;
-  const RowScale s = row_scale(bits);
+  const RowScale s = row_scale<(sizeof(T) == 2)>(bits);
   int8_t* dst = q + row * q_ld;
-  if (tid == 0) scale[row] = s.scale;
+  if (tid == 0) scale[row] = scale_of_row(bits);
   if (kept) {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
@@ -143,12 +143,13 @@ static cudaError_t launch_quantize(const void* x, long long ld, void* q, long lo
                                    cudaStream_t st) {
   constexpr int N = Loaded<T, WIDE>::N, PIECES = 4;
   const int pieces = (cols + N - 1) / N;
-  int tpr = 32;
-  while (tpr < 1024 && tpr * PIECES < pieces) tpr *= 2;
+  int log2 = 5;
+  while (log2 < 10 && (PIECES << log2) < pieces) ++log2;
+  const int tpr = 1 << log2;
   const int threads = tpr > 256 ? tpr : 256;
   const long long blocks = (rows + threads / tpr - 1) / (threads / tpr);
   return launch_chained(threads == 256 ? quantize_rows_kernel<T, WIDE, 256> : quantize_rows_kernel<T, WIDE, 1024>, dim3(static_cast<unsigned>(blocks)), threads, 0, st, 1, static_cast<const T*>(x), ld,
-                        static_cast<int8_t*>(q), q_ld, scale, rows, cols, tpr);
+                        static_cast<int8_t*>(q), q_ld, scale, rows, cols, log2);
 }
 
 template <class T>
@@ -215,6 +216,11 @@ __global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long
   const int e = where[0], row0 = where[1], rows = where[2];
   if (rows > 0) {
     const int8_t* w0 = wq + static_cast<long long>(e) * p.N * w_ld + static_cast<long long>(n0) * w_ld;
+    // the lane's result: row lane / 4, channel lane % 4 of the warp's
+    const int r_out = lane / kDotChannels, n = n0 + lane % kDotChannels;
+    const bool live = r_out < rows && n < p.N;
+    const float ws = live ? p.w_scale[static_cast<long long>(e) * p.N + n] : 0.f;
+    const float bias = live && p.bias != nullptr ? load_typed(p.bias, p.bias_type, static_cast<long long>(e) * p.N + n) : 0.f;
     uint4 w[kDotAhead][kDotChannels];
     const auto fetch = [&](uint4 (&v)[kDotChannels], int c) {
 #pragma unroll
@@ -268,8 +274,8 @@ __global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long
           uint32_t bits = part[r][0];
 #pragma unroll
           for (int i = 1; i < kDotWarps; ++i) bits = max(bits, part[r][i]);
-          const RowScale sc = row_scale(bits);
-          if (threadIdx.x == 0) row_scales[r] = s >= 0 ? sc.scale : 0.f;
+          const RowScale sc = row_scale<(sizeof(TX) == 2)>(bits);
+          if (threadIdx.x == 0) row_scales[r] = s >= 0 ? scale_of_row(bits) : 0.f;
           for (int c = threadIdx.x * L::N; c < kn; c += kDotThreads * L::N) {
             L v;
             v.zero();
@@ -314,26 +320,24 @@ __global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long
         acc[i] = (upper ? acc[i + d] : acc[i]) + other;
       }
     }
-    const int r = lane / kDotChannels, n = n0 + lane % kDotChannels;
-    const bool live = r < rows && n < p.N;
     float y = 0.f;
     if (live) {
       float scale;
       if constexpr (GIVEN) {
-        const int s = source_row(p, row0 + r);
+        const int s = source_row(p, row0 + r_out);
         scale = s >= 0 ? p.x_scale[s] : 0.f;
       } else {
-        scale = row_scales[r];
+        scale = row_scales[r_out];
       }
-      y = scaled(acc[0], scale, p.w_scale[static_cast<long long>(e) * p.N + n]);
-      if (p.bias != nullptr) y += load_typed(p.bias, p.bias_type, static_cast<long long>(e) * p.N + n);
+      y = scaled(acc[0], scale, ws);
+      if (p.bias != nullptr) y += bias;
     }
     const float up = __shfl_down_sync(0xffffffffu, y, 1);
     if (p.activation >= 0 && act_is_gated(p.activation)) {
       if (live && (n & 1) == 0)
-        store_typed(p.out, p.out_type, static_cast<long long>(row0 + r) * (p.N / 2) + n / 2, activate(p.activation, y) * up);
+        store_typed(p.out, p.out_type, static_cast<long long>(row0 + r_out) * (p.N / 2) + n / 2, activate(p.activation, y) * up);
     } else if (live) {
-      store_typed(p.out, p.out_type, static_cast<long long>(row0 + r) * p.N + n, activate(p.activation, y));
+      store_typed(p.out, p.out_type, static_cast<long long>(row0 + r_out) * p.N + n, activate(p.activation, y));
     }
   }
   zero_other_rows(p, (blockIdx.y * gridDim.x + blockIdx.x) * kDotWarps + warp, gridDim.x * gridDim.y * kDotWarps);

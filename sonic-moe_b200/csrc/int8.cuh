@@ -114,36 +114,43 @@ __device__ __forceinline__ void zero_other_rows(const Params& p, int warp, int w
 // ----------------------------------------------------------------------------------------------
 // quantisation of a row: scale = amax / 127 (1 for a row of zeros), q = 127 x / amax rounded half to even
 // ----------------------------------------------------------------------------------------------
-// x times 127 / amax in fp32 is within 127 * 2^-23 = 1.5e-5 of the quotient, which leaves it open on which side of a border it
-// is only where it is that near to one.  There the remainder 127 x - q amax decides, in exact arithmetic: with values of at most 11
-// bits fp32 holds it, with fp32 values each product is held as the sum of two.  Every fourth piece of 256 bf16 values has a
-// border, most of them ties such as amax / 2, so this has to be cheap: with 64-bit divisions 8192 rows of 4096 took 59 us.
+// 16-bit values (at most 11 bits): the quotient t of 127 x and amax by a reciprocal, corrected once by its remainder, which fp32 holds
+// exactly.  That is the quotient to the last bit wherever fp32 has it, at every tie k + 1/2 among others, and any other quotient of
+// such numbers is 2^-12 or more from a tie: rounding it to a whole number is exact.
+// fp32 values: one fused multiply-add is within 127 * 2^-24 + 2^-15 = 3.8e-5 of the quotient, as a fixed-point number with 14 fractional
+// bits; where that is within a step of a border k + 1/2 (seldom), the remainder 127 x - q amax decides, its products held as sums
+// of two.  (The same test for 16-bit values finds a border in every third piece of a warp, most of them ties such as amax / 2: with
+// 64-bit divisions behind it 8192 rows of 4096 took 59 us, with remainders 27.)
 // Rows whose largest value is below 2^-120 or above 2^120 are multiplied by a power of two first, so that neither 127 / amax nor
 // 127 x leaves fp32's range.  Rows that hold an infinity or a NaN get it as their scale, and zeros: every product of theirs is NaN.
 struct RowScale {
-  float scale;     // amax / 127
   float pre;       // power of two for the values
   float amax;      // times pre
-  float inv;       // 127 / amax
+  float inv;       // 1 / amax, of fp32 values 127 / amax; 0: none
   uint32_t keep;   // 0: zeros
 };
 // bits: the largest |x| as an integer (a NaN's are above infinity's)
+__device__ __forceinline__ float scale_of_row(uint32_t bits) {
+  const float amax = __uint_as_float(bits);
+  return bits == 0u ? 1.f : bits < 0x7F800000u ? __fdiv_rn(amax, 127.f) : amax;
+}
+template <bool SHORT>
 __device__ __forceinline__ RowScale row_scale(uint32_t bits) {
   RowScale s;
-  const float amax = __uint_as_float(bits);
   const bool some = bits != 0u && bits < 0x7F800000u;
-  s.scale = bits == 0u ? 1.f : some ? __fdiv_rn(amax, 127.f) : amax;
   s.pre = !some ? 1.f : bits < (7u << 23) ? 18446744073709551616.f : bits >= (247u << 23) ? 1.f / 18446744073709551616.f : 1.f;  // 2^64
-  s.amax = amax * s.pre;
-  s.inv = some ? __fdiv_rn(127.f, s.amax) : 0.f;
+  s.amax = __uint_as_float(bits) * s.pre;
+  s.inv = some ? __fdiv_rn(SHORT ? 1.f : 127.f, s.amax) : 0.f;
   s.keep = some ? 0xFFFFFFFFu : 0u;
   return s;
 }
 
 constexpr float kRoundMagic = 12582912.f;  // 1.5 * 2^23: adding it leaves the whole number in the low bits
-constexpr float kBorder = 0.5f - 1.f / 32768.f;
+// Adding it leaves t + 1/2 + 2^-14 as a fixed-point number in the low 22 bits of the sum, 14 of them behind the point: bits 14 to
+// 21 are t rounded, and the low 14 are at most 2 where t is within a step of a border.
+constexpr float kFixedMagic = 768.f + 0.5f + 1.f / 16384.f;
 
-// N values -> N bytes, four per word of w.  SHORT: values of at most 11 bits.
+// N values -> N bytes, four per word of w.
 template <bool SHORT, int N>
 __device__ __forceinline__ void quantize_values(const RowScale& s, float (&f)[N], uint32_t (&w)[N / 4]) {
   static_assert(N % 4 == 0, "whole words");
@@ -151,30 +158,31 @@ __device__ __forceinline__ void quantize_values(const RowScale& s, float (&f)[N]
 #pragma unroll
     for (int i = 0; i < N; ++i) f[i] *= s.pre;
   }
-  float far = 0.f;
   int q[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float t = f[i] * s.inv;
-    const float m = t + kRoundMagic;
-    q[i] = __float_as_int(m);
-    far = fmaxf(far, fabsf(t - (m - kRoundMagic)));
-  }
-  if (far >= kBorder) {
+  if constexpr (SHORT) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float whole = __int_as_float(q[i]) - kRoundMagic;
-      float rest, over;  // 127 x - q amax;  twice its magnitude - amax
-      if constexpr (SHORT) {
-        rest = fmaf(-whole, s.amax, 127.f * f[i]);
-        over = 2.f * fabsf(rest) - s.amax;
-      } else {
+      const float x = 127.f * f[i], t = x * s.inv;
+      q[i] = __float_as_int(fmaf(fmaf(-t, s.amax, x), s.inv, t) + kRoundMagic);
+    }
+  } else {
+    uint32_t near = 0x3FFFu;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      q[i] = __float_as_int(fmaf(f[i], s.inv, kFixedMagic));
+      near = min(near, static_cast<uint32_t>(q[i]) & 0x3FFFu);
+      q[i] >>= 14;
+    }
+    if (near <= 2u) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float whole = static_cast<float>(static_cast<int8_t>(q[i]));
         const float x = 127.f * f[i], x_low = fmaf(127.f, f[i], -x);
         const float p = whole * s.amax, p_low = fmaf(whole, s.amax, -p);
-        rest = x - p;  // exact: the two are within a factor of two of one another, or p is zero
-        over = (2.f * fabsf(rest) - s.amax) + 2.f * (rest >= 0.f ? x_low - p_low : p_low - x_low);
+        const float rest = x - p;  // exact: the two are within a factor of two of one another, or p is zero
+        const float over = (2.f * fabsf(rest) - s.amax) + 2.f * (rest >= 0.f ? x_low - p_low : p_low - x_low);
+        if (over > 0.f || (over == 0.f && (q[i] & 1))) q[i] += rest > 0.f ? 1 : -1;
       }
-      if (over > 0.f || (over == 0.f && (q[i] & 1))) q[i] += rest > 0.f ? 1 : -1;
     }
   }
 #pragma unroll
