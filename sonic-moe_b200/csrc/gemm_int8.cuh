@@ -2,7 +2,8 @@
 // memory).  A stage holds 128 columns of an operand row, 128 bytes, so staging, swizzle and descriptors are those of the bf16
 // kernels with elements of half the size, and a stage's four MMAs (K 32 each) do twice the work in the same time.
 //
-//   tiles   256 rows x 256 channels per CTA pair: cta_group::2, two accumulators, persistent
+//   tiles   256 rows x 256 channels per CTA pair: cta_group::2, two accumulators, persistent.  An expert's last tile with at most
+//           128 rows has the channels as the MMA's rows and the rows of x, up to the next 32, as its columns.
 //   units   128 channels (the MMA's rows) x up to 128 rows of x per CTA, for experts or batches with few rows, where the weights
 //           are the work: see gemm_skinny.cuh for why the operands trade places.  SPLIT: the reduction of a unit is shared by
 //           the CTAs of a cluster, where there are too few units to keep the memory busy.
@@ -10,6 +11,8 @@
 // Both take their rows from consecutive rows of x or gathered (TMA tile::gather4, a row that is none reads zeros).  The columns
 // past the last are zeros by the tensor maps' extent.  Every wait is bounded (ptx.cuh).
 #pragma once
+#include <type_traits>
+
 #include "int8.cuh"
 #include "ptx.cuh"
 
@@ -154,6 +157,86 @@ __device__ __forceinline__ bool most_rows_in_tiles(const Params& p, int limit, i
   return 2ll * above >= all;
 }
 
+// Scale and bias of channel f + lane; scale of row row0 + lane.  Loaded before the sums are waited for.
+__device__ __forceinline__ void load_channel(const Params& p, int e, int f, int lane, float& ws, float& bias) {
+  const bool mine = f + lane < p.N;
+  const long long at = static_cast<long long>(e) * p.N + f + lane;
+  ws = mine ? p.w_scale[at] : 0.f;
+  bias = mine && p.bias != nullptr ? load_typed(p.bias, p.bias_type, at) : 0.f;
+}
+__device__ __forceinline__ float load_row_scale(const Params& p, int row0, int rows, int lane) {
+  if (lane >= rows) return 0.f;
+  const int s = source_row(p, row0 + lane);
+  return s >= 0 ? p.x_scale[s] : 0.f;
+}
+
+// 32 channels (lane l: channel f + l) of up to 32 rows (word j: row row0 + j), of which `rows` exist.  Neighbouring lanes exchange
+// half of their values: afterwards word j of an even lane has the channels (l, l + 1) of row 2j and that of an odd one (l - 1, l) of
+// row 2j + 1, a gate and its up value, or two values of one 32-bit store.
+template <int MODE>
+__device__ __forceinline__ void store_rows(const Params& p, uint32_t stage, int lane, int f, int row0, int rows,
+                                           const uint32_t (&v)[32], float ws, float bias, float xs) {
+  const bool odd = lane & 1;
+  const bool gated = is_gated<MODE>(p);
+  float lo[16], hi[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    float a = scaled(static_cast<int>(v[2 * j]), __shfl_sync(0xffffffffu, xs, 2 * j), ws);
+    float b = scaled(static_cast<int>(v[2 * j + 1]), __shfl_sync(0xffffffffu, xs, 2 * j + 1), ws);
+    if (p.bias != nullptr) { a += bias; b += bias; }
+    if constexpr (MODE == MODE_ANY) {
+      if (!gated) { a = activation_of<MODE>(p, a); b = activation_of<MODE>(p, b); }
+    }
+    const float other = __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
+    lo[j] = odd ? other : a;
+    hi[j] = odd ? b : other;
+  }
+  const long long cols = gated ? p.N / 2 : p.N;
+  const int size = p.out_type == SMOE_F32 ? 4 : 2;
+  Block b;
+  b.pitch = cols * size;
+  const long long col = gated ? f / 2 : f;
+  b.base = static_cast<char*>(p.out) + row0 * b.pitch + col * size;
+  b.rows = rows;
+  b.valid = (cols - col) * size;
+  b.wide = p.wide_out;
+  b.half = size == 2;
+  const int pair = lane >> 1;
+  const auto at_word = [&](int row, int bytes, int byte) { return stage + row * bytes + byte; };
+  if (gated) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) lo[j] = activation_of<MODE>(p, lo[j]) * hi[j];
+    if (b.half) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const uint32_t h = pack_typed(p.out_type, lo[j], 0.f) & 0xFFFFu;
+        asm volatile("st.shared.b16 [%0], %1;" ::"r"(at_word(2 * j + odd, 32, 2 * pair)), "h"(static_cast<unsigned short>(h)) : "memory");
+      }
+      store_staged<32, 32>(lane, b, [&](int r, int q) { return stage + r * 32 + 16 * q; });
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) st_shared_word(at_word(2 * j + odd, 64, 4 * pair), __float_as_uint(lo[j]));
+      store_staged<32, 64>(lane, b, [&](int r, int q) { return stage + r * 64 + 16 * q; });
+    }
+  } else if (b.half) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) st_shared_word(at_word(2 * j + odd, 64, 4 * pair), pack_typed(p.out_type, lo[j], hi[j]));
+    store_staged<32, 64>(lane, b, [&](int r, int q) { return stage + r * 64 + 16 * q; });
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // 16 rows of 128 bytes at a time
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        st_shared_word(at_word(2 * j + odd, 128, 8 * pair), __float_as_uint(lo[8 * h + j]));
+        st_shared_word(at_word(2 * j + odd, 128, 8 * pair + 4), __float_as_uint(hi[8 * h + j]));
+      }
+      store_staged<16, 128>(lane, b, [&](int r, int q) { return stage + r * 128 + 16 * q; });
+      b.base += 16 * b.pitch;
+      b.rows -= 16;
+    }
+  }
+}
+
 // ----------------------------------------------------------------------------------------------
 // tiles
 // ----------------------------------------------------------------------------------------------
@@ -178,9 +261,16 @@ struct Shared {
 constexpr int SMEM_BYTES = 1024 + STAGES * (A_STAGE_BYTES + B_STAGE_BYTES) + ((sizeof(Shared) + 127) & ~127) + EPI_WARPS * STAGE_ROWS_BYTES;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory per CTA");
 
+// A last tile of at most 128 rows costs half the MMAs and less with the operands in each other's places: 256 channels are the MMA's
+// rows (each CTA its own 128, which it has staged as before), and `few` rows of x, a multiple of 32, its columns, of which
+// each CTA stages half.  The sums then lie one channel to a lane, as in the units.  Without it a 512-row load of 128 experts
+// spends a fifth of its MMAs on rows that do not exist.
 struct Tile {
-  int e, row0, row_end, n0;  // row0: of this CTA's 128 rows
+  int e, row0, row_end, n0;  // row0: of this CTA's staged rows
+  int first;                 // row of the pair's tile
+  int few;                   // 0: rows are the MMA's rows
 };
+__device__ __forceinline__ int few_rows(int rows) { return rows <= BM ? (rows + 31) & ~31 : 0; }
 
 // The tiles of this CTA pair, expert by expert, the channels of a row tile innermost, dealt out round-robin.
 struct Walker {
@@ -192,14 +282,22 @@ struct Walker {
       : p(p_), ss(ss_), lane(lane_), num_n((p_.N + BN - 1) / BN), total(ss_.tiles_before[p_.E] * num_n),
         step_m(static_cast<int>(gridDim.x >> 1) / num_n), step_n(static_cast<int>(gridDim.x >> 1) % num_n),
         t(blockIdx.x >> 1), mi(t / num_n), ni(t % num_n) {}
-  // the MMA issuer counts tiles only
-  __device__ __forceinline__ bool next_uncounted() {
-    const bool more = t < total;
+  __device__ __forceinline__ void advance() {
+    mi += step_m;
+    ni += step_n;
+    if (ni >= num_n) { ni -= num_n; ++mi; }
     t += gridDim.x >> 1;
-    return more;
+  }
+  // for one thread, which wants to know Tile::few only
+  __device__ __forceinline__ bool next_alone(int& few) {
+    if (t >= total) return false;
+    while (ss.tiles_before[e + 1] <= mi) ++e;
+    few = few_rows(ss.end[e] - ss.first[e] - (mi - ss.tiles_before[e]) * (2 * BM));
+    advance();
+    return true;
   }
   __device__ __forceinline__ bool next(uint32_t rank, Tile& tile) {
-    if (!next_uncounted()) return false;
+    if (t >= total) return false;
     while (true) {  // the first expert whose tiles end beyond mi, 32 experts at a time
       const int i = e + 1 + lane;
       const unsigned before = __ballot_sync(0xffffffffu, i <= p.E && ss.tiles_before[i] <= mi);
@@ -207,12 +305,12 @@ struct Walker {
       if (before != 0xffffffffu) break;
     }
     tile.e = e;
-    tile.row0 = ss.first[e] + (mi - ss.tiles_before[e]) * (2 * BM) + static_cast<int>(rank) * BM;
+    tile.first = ss.first[e] + (mi - ss.tiles_before[e]) * (2 * BM);
     tile.row_end = ss.end[e];
+    tile.few = few_rows(tile.row_end - tile.first);
+    tile.row0 = tile.first + static_cast<int>(rank) * (tile.few != 0 ? tile.few / 2 : BM);
     tile.n0 = ni * BN;
-    mi += step_m;
-    ni += step_n;
-    if (ni >= num_n) { ni -= num_n; ++mi; }
+    advance();
     return true;
   }
 };
@@ -363,11 +461,12 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       Tile tile;
       Walker walk(p, ss, lane);
       while (ok && walk.next(rank, tile)) {
+        const uint32_t row_bytes = gathered && tile.few != 0 ? tile.few / 2 * BK : A_STAGE_BYTES;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait_warp(smem_u32(&ss.empty[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
           if (elected) {
             const uint32_t bar = map_to_cta(smem_u32(&ss.full[stage]), 0);
-            if (leader) mbar_arrive_expect_tx(smem_u32(&ss.full[stage]), 2 * (A_STAGE_BYTES + B_STAGE_BYTES));
+            if (leader) mbar_arrive_expect_tx(smem_u32(&ss.full[stage]), 2 * (row_bytes + B_STAGE_BYTES));
             // no rows at all in this CTA's half of the tile: read past the tensor's end, which delivers zeros
             if (!gathered)
               tma_load_2d_pair(&tmA, bar, smem_u32(sA + stage * A_STAGE_BYTES), kb * BK, tile.row0 < tile.row_end ? tile.row0 : p.x_rows);
@@ -382,19 +481,20 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     } else if (warp == 1) {
       // ---- MMA issuer ------------------------------------------------------------------------
       if (leader && elect_one()) {
-        constexpr uint32_t idesc = make_idesc_i8(2 * BM, BN);
-        int stage = 0, acc = 0;
+        int stage = 0, acc = 0, few = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
         Walker walk(p, ss, lane);
-        while (ok && walk.next_uncounted()) {
+        while (ok && walk.next_alone(few)) {
+          const uint32_t idesc = make_idesc_i8(2 * BM, few != 0 ? few : BN);
           if (!mbar_wait(smem_u32(&ss.acc_empty[acc]), acc_phase ^ 1u, abort_flag)) { ok = false; break; }
           tc_fence_after();
           for (int kb = 0; kb < num_kb; ++kb) {
             if (!mbar_wait(smem_u32(&ss.full[stage]), phase, abort_flag)) { ok = false; break; }
             tc_fence_after();
-            const uint64_t a_desc = make_smem_desc(smem_u32(sA + stage * A_STAGE_BYTES), 16, 1024);
-            const uint64_t b_desc = make_smem_desc(smem_u32(sB + stage * B_STAGE_BYTES), 16, 1024);
+            const uint64_t x_desc = make_smem_desc(smem_u32(sA + stage * A_STAGE_BYTES), 16, 1024);
+            const uint64_t w_desc = make_smem_desc(smem_u32(sB + stage * B_STAGE_BYTES), 16, 1024);
+            const uint64_t a_desc = few != 0 ? w_desc : x_desc, b_desc = few != 0 ? x_desc : w_desc;
 #pragma unroll
             for (int k4 = 0; k4 < BK / UMMA_K; ++k4)
               umma_i8<2>(tmem_base + acc * BN, a_desc + ((k4 * UMMA_K) >> 4), b_desc + ((k4 * UMMA_K) >> 4), idesc,
@@ -423,25 +523,35 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       Tile tile;
       Walker walk(p, ss, lane);
       while (ok && walk.next(rank, tile)) {
-        const int r = tile.row0 + 32 * gw + lane;
+        // Every warp has a quarter of the CTA's rows, 4 at least: a stage is not full without it.  A warp that had none would wait for
+        // stages by parity that the others could overtake twice, and take an old phase for the one it waits for.
+        const int ops = (tile.few != 0 ? tile.few / 2 : BM) / 16;
+        const int r = tile.row0 + 4 * ops * gw + lane;
         int mine = p.x_rows;  // rows that do not exist: zeros
-        if (r < tile.row_end) {
+        if (lane < 4 * ops && r < tile.row_end) {
           const int s = source_row(p, r);
           if (s >= 0) mine = s;
         }
         int rows[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) rows[i] = __shfl_sync(0xffffffffu, mine, i);
-        if (elected) {
+        // all eight operations without a test between them, or up to four
+        const auto issue = [&](auto most) {
+          constexpr int MOST = decltype(most)::value;
           for (int kb = 0; kb < num_kb; ++kb) {
             if (!mbar_wait(smem_u32(&ss.empty[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
             const uint32_t bar = map_to_cta(smem_u32(&ss.full[stage]), 0);
-            const uint32_t dst = smem_u32(sA + stage * A_STAGE_BYTES) + gw * 4096;
+            const uint32_t dst = smem_u32(sA + stage * A_STAGE_BYTES) + gw * (MOST == 8 ? 8 : ops) * 512;
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
-              tma_gather4_pair(&tmA, bar, dst + q * 512, kb * BK, rows[4 * q], rows[4 * q + 1], rows[4 * q + 2], rows[4 * q + 3]);
+            for (int q = 0; q < MOST; ++q)
+              if (MOST == 8 || q < ops)
+                tma_gather4_pair(&tmA, bar, dst + q * 512, kb * BK, rows[4 * q], rows[4 * q + 1], rows[4 * q + 2], rows[4 * q + 3]);
             if (++stage == STAGES) { stage = 0; phase ^= 1u; }
           }
+        };
+        if (elected) {
+          if (ops == 8) issue(std::integral_constant<int, 8>());
+          else issue(std::integral_constant<int, 4>());
         }
         ok = __all_sync(0xffffffffu, ok);
       }
@@ -459,6 +569,36 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     Tile tile;
     Walker walk(p, ss, lane);
     while (ok && walk.next(rank, tile)) {
+      const auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&ss.acc_empty[acc]), 0));
+      };
+      if (tile.few != 0) {
+        // lanes are channels: a warp has 32 of them, and every other 32 rows
+        const int f = tile.n0 + static_cast<int>(rank) * BN_CTA + quad * 32, rows = tile.row_end - tile.first;
+        const bool works = f < p.N && 32 * col_half < rows;
+        float ws = 0.f, bias = 0.f, xs0 = 0.f, xs1 = 0.f;
+        if (works) {
+          load_channel(p, tile.e, f, lane, ws, bias);
+          xs0 = load_row_scale(p, tile.first + 32 * col_half, rows - 32 * col_half, lane);
+          xs1 = load_row_scale(p, tile.first + 32 * col_half + 64, rows - 32 * col_half - 64, lane);
+        }
+        if (!mbar_wait_warp(smem_u32(&ss.acc_full[acc]), acc_phase, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        if (!works) release();
+        const uint32_t t_addr = tmem_base + acc * BN + (static_cast<uint32_t>(quad * 32) << 16);
+#pragma unroll 1
+        for (int c = col_half; works && 32 * c < rows; c += 2) {
+          uint32_t v[32];
+          tmem_ld32(t_addr + 32 * c, v);
+          tmem_ld_wait();
+          if (32 * (c + 2) >= rows) release();
+          store_rows<MODE>(p, my_stage, lane, f, tile.first + 32 * c, rows - 32 * c, v, ws, bias, c == col_half ? xs0 : xs1);
+        }
+        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+        continue;
+      }
       const int row_base = tile.row0 + quad * 32, r = row_base + lane;
       const int n_first = tile.n0 + col_half * COLS_PER_WARP;
       float xs = 0.f;
@@ -476,11 +616,6 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       if (works) prefetch_l1(p.w_scale + static_cast<long long>(tile.e) * p.N + n_first, 4 * min(COLS_PER_WARP, p.N - n_first), lane);
       if (!mbar_wait_warp(smem_u32(&ss.acc_full[acc]), acc_phase, abort_flag)) { ok = false; break; }
       tc_fence_after();
-      const auto release = [&] {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&ss.acc_empty[acc]), 0));
-      };
       if (!works) release();
       const uint32_t t_addr = tmem_base + acc * BN + col_half * COLS_PER_WARP + (static_cast<uint32_t>(quad * 32) << 16);
 #pragma unroll 1
@@ -583,86 +718,6 @@ struct Walker {
     return true;
   }
 };
-
-// Scale and bias of channel f + lane; scale of row row0 + lane.  Loaded before the sums are waited for.
-__device__ __forceinline__ void load_channel(const Params& p, int e, int f, int lane, float& ws, float& bias) {
-  const bool mine = f + lane < p.N;
-  const long long at = static_cast<long long>(e) * p.N + f + lane;
-  ws = mine ? p.w_scale[at] : 0.f;
-  bias = mine && p.bias != nullptr ? load_typed(p.bias, p.bias_type, at) : 0.f;
-}
-__device__ __forceinline__ float load_row_scale(const Params& p, int row0, int rows, int lane) {
-  if (lane >= rows) return 0.f;
-  const int s = source_row(p, row0 + lane);
-  return s >= 0 ? p.x_scale[s] : 0.f;
-}
-
-// 32 channels (lane l: channel f + l) of up to 32 rows (word j: row row0 + j), of which `rows` exist.  Neighbouring lanes exchange
-// half of their values: afterwards word j of an even lane has the channels (l, l + 1) of row 2j and that of an odd one (l - 1, l) of
-// row 2j + 1, a gate and its up value, or two values of one 32-bit store.
-template <int MODE>
-__device__ __forceinline__ void store_rows(const Params& p, uint32_t stage, int lane, int f, int row0, int rows,
-                                           const uint32_t (&v)[32], float ws, float bias, float xs) {
-  const bool odd = lane & 1;
-  const bool gated = is_gated<MODE>(p);
-  float lo[16], hi[16];
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    float a = scaled(static_cast<int>(v[2 * j]), __shfl_sync(0xffffffffu, xs, 2 * j), ws);
-    float b = scaled(static_cast<int>(v[2 * j + 1]), __shfl_sync(0xffffffffu, xs, 2 * j + 1), ws);
-    if (p.bias != nullptr) { a += bias; b += bias; }
-    if constexpr (MODE == MODE_ANY) {
-      if (!gated) { a = activation_of<MODE>(p, a); b = activation_of<MODE>(p, b); }
-    }
-    const float other = __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
-    lo[j] = odd ? other : a;
-    hi[j] = odd ? b : other;
-  }
-  const long long cols = gated ? p.N / 2 : p.N;
-  const int size = p.out_type == SMOE_F32 ? 4 : 2;
-  Block b;
-  b.pitch = cols * size;
-  const long long col = gated ? f / 2 : f;
-  b.base = static_cast<char*>(p.out) + row0 * b.pitch + col * size;
-  b.rows = rows;
-  b.valid = (cols - col) * size;
-  b.wide = p.wide_out;
-  b.half = size == 2;
-  const int pair = lane >> 1;
-  const auto at_word = [&](int row, int bytes, int byte) { return stage + row * bytes + byte; };
-  if (gated) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) lo[j] = activation_of<MODE>(p, lo[j]) * hi[j];
-    if (b.half) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const uint32_t h = pack_typed(p.out_type, lo[j], 0.f) & 0xFFFFu;
-        asm volatile("st.shared.b16 [%0], %1;" ::"r"(at_word(2 * j + odd, 32, 2 * pair)), "h"(static_cast<unsigned short>(h)) : "memory");
-      }
-      store_staged<32, 32>(lane, b, [&](int r, int q) { return stage + r * 32 + 16 * q; });
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) st_shared_word(at_word(2 * j + odd, 64, 4 * pair), __float_as_uint(lo[j]));
-      store_staged<32, 64>(lane, b, [&](int r, int q) { return stage + r * 64 + 16 * q; });
-    }
-  } else if (b.half) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) st_shared_word(at_word(2 * j + odd, 64, 4 * pair), pack_typed(p.out_type, lo[j], hi[j]));
-    store_staged<32, 64>(lane, b, [&](int r, int q) { return stage + r * 64 + 16 * q; });
-  } else {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {  // 16 rows of 128 bytes at a time
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        st_shared_word(at_word(2 * j + odd, 128, 8 * pair), __float_as_uint(lo[8 * h + j]));
-        st_shared_word(at_word(2 * j + odd, 128, 8 * pair + 4), __float_as_uint(hi[8 * h + j]));
-      }
-      store_staged<16, 128>(lane, b, [&](int r, int q) { return stage + r * 128 + 16 * q; });
-      b.base += 16 * b.pitch;
-      b.rows -= 16;
-    }
-  }
-}
 
 // most: experts with more rows are the tiles'.  split: CTAs of a cluster that share a unit's reduction (1: none); with SPLIT
 // there are at least as many clusters as units.

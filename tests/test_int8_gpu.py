@@ -211,6 +211,14 @@ def test_columns_behind_the_last_do_not_count(built_library):
         assert torch.equal(y.double(), product(q[:, :K], wq[:, :K]))  # at most 333 * 2^14 < 2^24: exact in fp32
 
 
+@pytest.fixture(autouse=True)
+def no_wait_was_abandoned():
+    yield
+    from sonicmoe import _lib
+
+    _lib.check_status()
+
+
 def grouped_case(T, K, E, align, dropped, seed=0):
     import sonicmoe
 
@@ -279,6 +287,29 @@ def test_grouped_load_in_one_expert(built_library):
         y = int8.int8_grouped_linear(x, wq, ws, off)
         q, xs = int8.quantize_rows(x)
         check(y, product(q, wq[4]), xs[:, None], ws[4], None, None)
+
+
+def test_many_tiles_of_every_kind(built_library):
+    """Loads whose last tiles have 1 to 256 rows, many tiles to a CTA pair, long reductions, again and again: the roles of the
+    tile kernel must not lose one another where a tile's rows are few."""
+    from sonicmoe.functional import int8
+
+    E, N, cols, T, K = 64, 1024, 2048, 2500, 4
+    g = torch.Generator().manual_seed(7)
+    wq = torch.randint(-127, 128, (E, N, cols), generator=g, dtype=torch.int8).cuda()
+    ws = torch.rand(E, N, generator=g).cuda() * 1e-4
+    q = torch.randint(-127, 128, (T, cols), generator=g, dtype=torch.int8).cuda()
+    xs = torch.rand(T, generator=g).cuda()
+    for seed in range(4):
+        p = grouped_case(T, K, E, 1, 0.0, seed)
+        rows, *parts = grouped_reference(p, q, xs, wq, ws, None, E, True, False)
+        for _ in range(5):
+            y = int8.int8_grouped_linear(q, wq, ws, p.expert_frequency_offset, p.x_gather_idx, x_scale=xs, out_dtype=torch.float32)
+        check(y[rows], *parts, None)
+        sorted_x = q[p.x_gather_idx.long()].contiguous()
+        again = int8.int8_grouped_linear(sorted_x, wq, ws, p.expert_frequency_offset, x_scale=xs[p.x_gather_idx.long()].contiguous(),
+                                         out_dtype=torch.float32)
+        assert torch.equal(again, y)
 
 
 def test_offsets_and_gather_indices_out_of_range(built_library):
