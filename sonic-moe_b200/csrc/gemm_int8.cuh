@@ -258,7 +258,7 @@ struct Shared {
   int end[kMaxExpertRows];
   int tiles_before[kMaxExpertRows + 1];
 };
-constexpr int SMEM_BYTES = 1024 + STAGES * (A_STAGE_BYTES + B_STAGE_BYTES) + ((sizeof(Shared) + 127) & ~127) + EPI_WARPS * STAGE_ROWS_BYTES;
+constexpr int SMEM_BYTES = 1024 + STAGES * (A_STAGE_BYTES + B_STAGE_BYTES) + ((sizeof(Shared) + 127) & ~127) + EPI_WARPS * (STAGE_ROWS_BYTES + COLS_PER_WARP * 4);
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory per CTA");
 
 // A last tile of at most 128 rows costs half the MMAs and less with the operands in each other's places: 256 channels are the MMA's
@@ -315,39 +315,22 @@ struct Walker {
   }
 };
 
-// f[j] = v[j] of 32 consecutive values, the same for all lanes: whole words where they start on 16 bytes and all exist.
-__device__ __forceinline__ void load_uniform(const float* v, int exist, float (&f)[32]) {
-  if (exist >= 32 && reinterpret_cast<uintptr_t>(v) % 16 == 0) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float4 q = reinterpret_cast<const float4*>(v)[j];
-      f[4 * j] = q.x; f[4 * j + 1] = q.y; f[4 * j + 2] = q.z; f[4 * j + 3] = q.w;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) f[j] = j < exist ? v[j] : 0.f;
-  }
-}
-
-// Asks the L1 for `bytes` from v on (at most 512): the lines that load_uniform will read.
-__device__ __forceinline__ void prefetch_l1(const void* v, int bytes, int lane) {
-  if (128 * lane < bytes + 127 && lane < 5) {
-    const char* at = static_cast<const char*>(v) + min(128 * lane, bytes - 1);
-    asm volatile("prefetch.global.L1 [%0];" ::"l"(at));
-  }
-}
-
-// 32 channels of the warp's 32 rows: lane l has row l's sums in v, and (with a bias) channel n + l's bias.  The scales come by loads
-// that every lane makes of the same words: they were asked for before the accumulator was waited for (without that a tile of a
-// short reduction waited 2.5 kilocycles for each 32 channels), and cost the shared memory, which feeds the MMAs, less than
-// broadcasts through the staging rows (up projection of 8192 tokens 413 and 431 us).
+// 32 channels of the warp's 32 rows: lane l has row l's sums in v, and (with a bias) channel n + l's bias; scales: those of the 32
+// channels, in shared memory, where they were put before the accumulator was waited for.  With loads of the same words by all
+// lanes from memory, asked for in advance or not, a tile waits up to 2.5 kilocycles for each 32 channels: 8192 x 7168 x 1024 took 72
+// us, 55 without them.
 template <int MODE>
-__device__ __forceinline__ void store_columns(const Params& p, uint32_t stage, int lane, int row_base, int row_end, int e, int n,
-                                              const uint32_t (&v)[32], float xs, float bias) {
+__device__ __forceinline__ void store_columns(const Params& p, uint32_t stage, int lane, int row_base, int row_end, int n,
+                                              const uint32_t (&v)[32], float xs, uint32_t scales, float bias) {
   float f[32];
-  load_uniform(p.w_scale + static_cast<long long>(e) * p.N + n, p.N - n, f);
 #pragma unroll
-  for (int j = 0; j < 32; ++j) f[j] = scaled(static_cast<int>(v[j]), xs, f[j]);
+  for (int j = 0; j < 8; ++j) {
+    const uint4 w = ld_shared_v4(scales + 16 * j);
+    f[4 * j] = scaled(static_cast<int>(v[4 * j]), xs, __uint_as_float(w.x));
+    f[4 * j + 1] = scaled(static_cast<int>(v[4 * j + 1]), xs, __uint_as_float(w.y));
+    f[4 * j + 2] = scaled(static_cast<int>(v[4 * j + 2]), xs, __uint_as_float(w.z));
+    f[4 * j + 3] = scaled(static_cast<int>(v[4 * j + 3]), xs, __uint_as_float(w.w));
+  }
   if (p.bias != nullptr) {
 #pragma unroll
     for (int j = 0; j < 32; ++j) f[j] += __shfl_sync(0xffffffffu, bias, j);
@@ -563,6 +546,7 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     const int quad = warp & 3;
     const int col_half = (warp - FIRST_EPI_WARP) >> 2;
     const uint32_t my_stage = smem_u32(stage_out) + (warp - FIRST_EPI_WARP) * STAGE_ROWS_BYTES;
+    const uint32_t my_scales = smem_u32(stage_out) + EPI_WARPS * STAGE_ROWS_BYTES + (warp - FIRST_EPI_WARP) * (COLS_PER_WARP * 4);
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
@@ -613,7 +597,12 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         const int n = n_first + 32 * c + lane;
         bias[c] = works && n < p.N && p.bias != nullptr ? load_typed(p.bias, p.bias_type, static_cast<long long>(tile.e) * p.N + n) : 0.f;
       }
-      if (works) prefetch_l1(p.w_scale + static_cast<long long>(tile.e) * p.N + n_first, 4 * min(COLS_PER_WARP, p.N - n_first), lane);
+#pragma unroll
+      for (int c = 0; c < COLS_PER_WARP / 32; ++c) {
+        const int n = n_first + 32 * c + lane;
+        st_shared_word(my_scales + 4 * (32 * c + lane), __float_as_uint(works && n < p.N ? p.w_scale[static_cast<long long>(tile.e) * p.N + n] : 0.f));
+      }
+      __syncwarp();
       if (!mbar_wait_warp(smem_u32(&ss.acc_full[acc]), acc_phase, abort_flag)) { ok = false; break; }
       tc_fence_after();
       if (!works) release();
@@ -627,7 +616,7 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         const float b = c < 2 ? c < 1 ? bias[0] : bias[1] : c < 3 ? bias[2] : bias[3];
         tmem_ld_wait();
         if (c + 1 == COLS_PER_WARP / 32 || n + 32 >= p.N) release();
-        store_columns<MODE>(p, my_stage, lane, row_base, tile.row_end, tile.e, n, v, xs, b);
+        store_columns<MODE>(p, my_stage, lane, row_base, tile.row_end, n, v, xs, my_scales + 128 * c, b);
       }
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
