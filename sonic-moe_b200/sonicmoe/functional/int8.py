@@ -3,6 +3,11 @@
     wq, w_scale = quantize_rows(w)                       # once: w (E, N, cols), one scale per expert and channel
     y = int8_grouped_linear(x, wq, w_scale, p.expert_frequency_offset, x_gather_idx=p.x_gather_idx)
 
+or the whole layer, with the router's logits, top-K choice and combine of the bf16 one:
+
+    experts = quantize_experts(moe.c_fc.weight.permute(1, 2, 0), moe.c_fc.bias, moe.c_proj.weight.permute(1, 2, 0), moe.c_proj.bias)
+    o, router_logits, expert_frequency = moe_int8_softmax_topk_layer(x, moe.router.weight, experts, K)
+
 scale = amax / 127 of the row (1 for a row of zeros), values = 127 x / amax rounded half to even; the sum of a product is exact
 in 32-bit integers and rounded once, so results do not depend on how the work is shared out.  Rows that hold an infinity or a NaN
 give NaN.  8-bit rows start on 16-byte boundaries: `quantize_rows` lays them out so, whatever their width.
@@ -13,11 +18,14 @@ are the path for training.  The reference has no 8-bit path.
 
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import torch
+import torch.nn.functional as F
 
 from .. import _lib
 from .._lib import check, lib, ptr, stream_ptr
-from ..enums import ActivationType
+from ..enums import ActivationType, is_glu
 from .permutation import _ROW_TYPES as _FLOAT_TYPES
 
 MAX_COLS = 131071  # sums of that many products of 8-bit integers fit into 32 bits
@@ -157,3 +165,72 @@ def int8_grouped_linear(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor
         raise ValueError("expert_frequency_offset is needed: int8_linear is the product without experts")
     return _linear(x, wq, w_scale, x_scale, bias, out_dtype, _activation_code(activation_type), expert_frequency_offset,
                    expert_frequency, x_gather_idx)
+
+
+@dataclass
+class Int8Experts:
+    """The experts of a layer as `quantize_rows` lays them out: w1q (E, N1, H), w2q (E, H, I), scales and biases like their rows."""
+
+    w1q: torch.Tensor
+    w1_scale: torch.Tensor
+    b1: torch.Tensor | None
+    w2q: torch.Tensor
+    w2_scale: torch.Tensor
+    b2: torch.Tensor | None
+
+
+@torch.no_grad()
+def quantize_experts(w1: torch.Tensor, b1: torch.Tensor | None, w2: torch.Tensor, b2: torch.Tensor | None) -> Int8Experts:
+    """w1 (N1, H, E) and w2 (H, I, E), the ``permute(1, 2, 0)`` views that the other layer functions take; biases (E, N1), (E, H)."""
+    if (b1 is None) != (b2 is None):
+        raise AssertionError("b1 and b2 has to be None or not None at the same time!")
+    if w1.dim() != 3 or w2.dim() != 3 or w1.shape[2] != w2.shape[2] or w1.shape[1] != w2.shape[0]:
+        raise ValueError(f"inconsistent shapes: w1 {tuple(w1.shape)}, w2 {tuple(w2.shape)}")
+    return Int8Experts(*quantize_rows(w1.permute(2, 0, 1)), b1, *quantize_rows(w2.permute(2, 0, 1)), b2)
+
+
+def moe_int8_softmax_topk_layer(
+    x: torch.Tensor,
+    router_w: torch.Tensor,
+    experts: Int8Experts,
+    K: int,
+    activation_type: ActivationType | str = ActivationType.SWIGLU,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Inference forward of the token-choice top-K layer with 8-bit experts: (o (T, H), router_logits (T, E), expert_frequency
+    (E,) int32), as `moe_TC_softmax_topk_layer`.  x (T, H) bf16, quantised per token; the activations between the projections are
+    rounded to bf16 and quantised per row."""
+    from . import _FusedRouter, _route_metadata, fused_router_applies, topk_softmax
+
+    if isinstance(activation_type, str):
+        activation_type = ActivationType(activation_type)
+    _refuse_gradients(x, router_w, experts.w1_scale, experts.b1, experts.w2_scale, experts.b2)
+    _lib.require_cuda(x, "x")
+    if x.dtype != torch.bfloat16 or x.dim() != 2:
+        raise TypeError(f"x has to be (T, H) bf16, got {x.dtype} {tuple(x.shape)}")
+    T, H = x.shape
+    E, n1 = experts.w1q.shape[:2]
+    if router_w.shape != (E, H) or experts.w1q.shape[2] != H or experts.w2q.shape[:2] != (E, H):
+        raise ValueError(f"inconsistent shapes: x {tuple(x.shape)}, router {tuple(router_w.shape)}, w1q {tuple(experts.w1q.shape)}, "
+                         f"w2q {tuple(experts.w2q.shape)}")
+    if experts.w2q.shape[2] * (2 if is_glu(activation_type) else 1) != n1:
+        raise ValueError(f"{n1} rows of the up projection do not fit {experts.w2q.shape[2]} columns of the down projection")
+    if not 1 <= K <= E:
+        raise ValueError(f"1 <= K <= {E} is needed, got {K}")
+    if H % 8:
+        raise ValueError("the hidden size has to be a multiple of 8")  # the combine's accesses
+    with torch.no_grad():
+        if T > 0 and fused_router_applies(x, router_w, K):
+            router_logits, scores, indices = _FusedRouter.apply(x, router_w, K)[:3]
+        else:
+            router_logits = F.linear(x if x.dtype == router_w.dtype else x.to(router_w.dtype), router_w)
+            scores, indices = topk_softmax(router_logits, K)
+        route = _route_metadata(indices.reshape(-1), None, E, K)
+        code = _ACTIVATIONS[activation_type]
+        y1 = _linear(x, experts.w1q, experts.w1_scale, None, experts.b1, None, code, route.expert_frequency_offset, None,
+                     route.x_gather_idx)
+        y2 = _linear(y1, experts.w2q, experts.w2_scale, None, experts.b2, None, -1, route.expert_frequency_offset, None, None)
+        with _lib.on_device(x.device):
+            o = torch.empty_like(x, memory_format=torch.contiguous_format)
+            check(lib.smoe_gather_sum(y2.data_ptr(), o.data_ptr(), scores.data_ptr(), _lib.SMOE_F32,
+                                      route.s_reverse_scatter_idx.data_ptr(), None, T, H, K, stream_ptr(x.device)), "gather_sum")
+    return o, router_logits, route.expert_frequency

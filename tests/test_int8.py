@@ -72,3 +72,20 @@ def test_python_refusals(built_library):
         int8.int8_grouped_linear(x, w[None], s[None], None)
     with pytest.raises(ValueError, match="is not a valid"):
         int8.int8_linear(x, w, s, activation_type="tanh")
+
+
+def test_layer_refusals(built_library):
+    from sonicmoe import SonicMoEError
+    from sonicmoe.functional import int8
+
+    w1, w2 = torch.zeros(8, 4, 16, dtype=torch.int8), torch.zeros(8, 16, 2, dtype=torch.int8)
+    experts = int8.Int8Experts(w1, torch.ones(8, 4), None, w2, torch.ones(8, 16), None)
+    x, router = torch.zeros(3, 16, dtype=torch.bfloat16), torch.zeros(8, 16, dtype=torch.bfloat16)
+    with pytest.raises(SonicMoEError, match="no CPU path"):
+        int8.moe_int8_softmax_topk_layer(x, router, experts, 2)
+    with pytest.raises(NotImplementedError, match="no gradient"):
+        int8.moe_int8_softmax_topk_layer(x.requires_grad_(True), router, experts, 2)
+    with pytest.raises(AssertionError):
+        int8.quantize_experts(torch.zeros(4, 16, 8), None, torch.zeros(16, 2, 8), torch.zeros(8, 16))
+    with pytest.raises(ValueError, match="inconsistent shapes"):
+        int8.quantize_experts(torch.zeros(4, 16, 8), None, torch.zeros(12, 2, 8), None)

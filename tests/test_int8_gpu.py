@@ -389,3 +389,47 @@ def test_sort_quantise_multiply_combine(built_library):
     # one quantised value is off by half a scale, 1 / 254 of its row's largest (about 3.5 of its rms, independent of one
     # another): 0.8 % of the sum of such products per quantised operand, rms; two of them, and the first's goes through SwiGLU
     assert ((o.double() - want).norm() / want.norm()).item() < 3 * 0.008
+
+
+@pytest.mark.parametrize("T,H,I,E,K,activation,biased", [
+    (0, 128, 64, 8, 2, "swiglu", False), (1, 256, 128, 32, 4, "swiglu", False), (77, 192, 64, 8, 1, "gelu", True),
+    (1000, 512, 256, 64, 8, "swiglu", False), (513, 136, 72, 6, 3, "relu_sq", True), (3000, 256, 128, 4, 2, "silu", False)])
+def test_layer(built_library, T, H, I, E, K, activation, biased):
+    """The layer against its steps in 64 bits, with the routing of the logits that it returns."""
+    from sonicmoe.enums import ActivationType
+    from sonicmoe.functional import int8, moe_TC_softmax_topk_layer
+
+    g = torch.Generator().manual_seed(8)
+    n1 = 2 * I if activation in GATED else I
+    x = torch.randn(T, H, generator=g).bfloat16().cuda()
+    router = (torch.randn(E, H, generator=g) * 0.1).bfloat16().cuda()
+    w1 = (torch.randn(E, n1, H, generator=g) * 2 / H ** 0.5).bfloat16().cuda()
+    w2 = (torch.randn(E, H, I, generator=g) / I ** 0.5).bfloat16().cuda()
+    b1, b2 = (torch.randn(E, n, generator=g).bfloat16().cuda() if biased else None for n in (n1, H))
+    experts = int8.quantize_experts(w1.permute(1, 2, 0), b1, w2.permute(1, 2, 0), b2)
+    o, logits, frequency = int8.moe_int8_softmax_topk_layer(x, router, experts, K, ActivationType(activation))
+    assert o.shape == x.shape and o.dtype == torch.bfloat16 and logits.shape == (T, E) and int(frequency.sum()) == T * K
+    if T == 0:
+        return
+    top, idx = torch.sort(logits.float(), dim=1, descending=True, stable=True)
+    scores, idx = torch.softmax(top[:, :K].double(), dim=1), idx[:, :K]
+    assert torch.equal(frequency.long().cpu(), torch.bincount(idx.reshape(-1).cpu(), minlength=E))
+    d1 = experts.w1q.double() * experts.w1_scale.double().unsqueeze(-1)
+    d2 = experts.w2q.double() * experts.w2_scale.double().unsqueeze(-1)
+    q, s = exact_quantize(x)
+    xd = q * s.double().unsqueeze(-1)
+    want = torch.zeros(T, H, dtype=torch.float64, device="cuda")
+    for e in range(E):
+        t, k = torch.nonzero(idx == e, as_tuple=True)
+        z = xd[t] @ d1[e].t() + (0 if b1 is None else b1[e].double())
+        y = act_value(activation, z[:, 0::2])[0] * z[:, 1::2] if activation in GATED else act_value(activation, z)[0]
+        q, s = exact_quantize(y.bfloat16())
+        y = (q * s.double().unsqueeze(-1)) @ d2[e].t() + (0 if b2 is None else b2[e].double())
+        want.index_add_(0, t, y * scores[t, k].unsqueeze(1))
+    # bf16 roundings of the two projections' results and of the sum, at most 2^-8 each, rms a third of that; a value of y1 that
+    # is rounded to the neighbouring bf16 may be quantised to the neighbouring step: 2^-8 of it again
+    assert ((o.double() - want).norm() / want.norm()).item() < 4 * 2.0 ** -8 / 3 ** 0.5
+    bf16 = moe_TC_softmax_topk_layer(x, router, w1.permute(1, 2, 0), b1, w2.permute(1, 2, 0), b2, K, 0, ActivationType(activation),
+                                     True)[0] if H % 64 == 0 and I % 64 == 0 and n1 % 128 == 0 else None
+    if bf16 is not None:  # 8-bit operands: 0.8 % rms each, three of them and the activation's slope
+        assert ((o.double() - bf16.double()).norm() / bf16.double().norm()).item() < 0.06
