@@ -32,7 +32,8 @@ constexpr int kMaxExperts = 4096;
 constexpr int kMaxBlocks = 128;
 constexpr int kWarps = 8, kSteps = 8;                 // warps of a block; groups of 32 pairs that a warp has at a time, at most
 constexpr int kOneWarps = 32;                         // the form with one block
-constexpr int kOneMaxPairs = kOneWarps * kSteps * 32, kOneMaxExperts = 1024;
+constexpr int kOneMaxPairs = 2048, kOneMaxExperts = 1024;
+static_assert(kOneMaxPairs <= kOneWarps * kSteps * 32, "pairs that the block's registers hold");
 
 struct Plan {
   const void* idx;   // (n) int32 or int64
@@ -372,6 +373,61 @@ __device__ __forceinline__ void store_weight(void* w, int dtype, long long i, fl
   else static_cast<__half*>(w)[i] = __float2half_rn(v);
 }
 
+// Rows that start anywhere (on a value), by the 16-byte blocks of the row that is written: one store for each, and two loads from a
+// row that lies otherwise, shifted together.  The first and the last block go value by value.
+template <class T>
+struct Window {
+  static __host__ __device__ __forceinline__ int count(int bytes) { return (bytes + 16 - static_cast<int>(sizeof(T)) + 15) / 16; }
+  // offset of block i in the row at `dst`
+  static __device__ __forceinline__ int offset(int i, const char* dst) { return 16 * i - static_cast<int>(reinterpret_cast<uintptr_t>(dst) & 15); }
+  // 16 bytes of `row` from `at` on, zeros where that is outside of its `bytes`
+  static __device__ __forceinline__ Piece<16> load(const char* row, int at, int bytes) {
+    Piece<16> v;
+    if (at >= 0 && at + 16 <= bytes) {
+      const char* p = row + at;
+      const int s = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);
+      const uint4 a = *reinterpret_cast<const uint4*>(p - s);
+      uint4 b = make_uint4(0u, 0u, 0u, 0u);
+      if (s != 0) b = *reinterpret_cast<const uint4*>(p - s + 16);  // holds the last of the 16 bytes
+      uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      if (s & 8) {
+#pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+      }
+      if (s & 4) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v.w[i] = sizeof(T) == 4 ? w[i] : __funnelshift_r(w[i], w[i + 1], 8 * (s & 2));
+    } else {
+#pragma unroll
+      for (auto& x : v.w) x = 0u;
+#pragma unroll
+      for (int i = 0; i < 16 / static_cast<int>(sizeof(T)); ++i) {
+        const int o = at + i * static_cast<int>(sizeof(T));
+        if (o < 0 || o >= bytes) continue;
+        if constexpr (sizeof(T) == 4) v.w[i] = *reinterpret_cast<const uint32_t*>(row + o);
+        else v.w[i / 2] |= static_cast<uint32_t>(*reinterpret_cast<const unsigned short*>(row + o)) << (16 * (i & 1));
+      }
+    }
+    return v;
+  }
+  static __device__ __forceinline__ void store(char* row, int at, int bytes, const Piece<16>& v) {
+    if (at >= 0 && at + 16 <= bytes) {
+      store_piece<16>(row + at, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16 / static_cast<int>(sizeof(T)); ++i) {
+        const int o = at + i * static_cast<int>(sizeof(T));
+        if (o < 0 || o >= bytes) continue;
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(row + o) = v.w[i];
+        else *reinterpret_cast<unsigned short*>(row + o) = static_cast<unsigned short>(v.w[i / 2] >> (16 * (i & 1)));
+      }
+    }
+  }
+};
+
 struct Rows {
   const char* token_src;  // spread: (T, H) rows of the tokens, token_ld bytes apart
   long long token_ld;
@@ -491,6 +547,71 @@ __global__ void __launch_bounds__(kThreads) collect_kernel(const Rows a) {
 // Four rows of the token are in flight at a time.  A row's dot product is added up piece by piece in a thread, then over the
 // lanes of each warp, then over the warps: always in the same order.
 constexpr int kDotRows = 4, kDotChunk = 32;
+// The two above by windows.  Sides measured (piece by piece / by windows, us): spread, fp32 rows of 1005 values, T 4099, K 6 33 / 23,
+// of 2049, T 8192, K 4 84 / 59, bf16 of 3001, T 16384, K 4 125 / 108, but fp16 of 1030, which have 4-byte pieces of two values, T 5003,
+// K 3 8.6 / 13.5; collect, bf16 of 3001 217 / 171, fp16 of 1030 18.8 / 15.8, but fp32 of 1005 30.3 / 33.  So a spread goes by windows
+// where a piece is one value, and a collect where a value has 16 bits.  (The gradient of the combine, with a window for each of
+// four differently placed rows and their gradients, lost a third.)
+template <class T, bool WEIGHTED>
+__global__ void __launch_bounds__(kThreads) spread_windows_kernel(const Rows a, int pad_blocks) {
+  release_next();
+  wait_for_previous();
+  if (blockIdx.x < pad_blocks) return zero_rows<sizeof(T)>(a, blockIdx.x);
+  using W = Window<T>;
+  const int windows = W::count(a.bytes);
+  const long long g = static_cast<long long>(blockIdx.x - pad_blocks) * kThreads + threadIdx.x;
+  if (g >= static_cast<long long>(a.T) * windows) return;
+  const int t = static_cast<int>(g / windows), c = static_cast<int>(g - static_cast<long long>(t) * windows);
+  const char* src = a.token_src + t * a.token_ld;
+  const long long p0 = static_cast<long long>(t) * a.K;
+#pragma unroll 4
+  for (int k = 0; k < a.K; ++k) {
+    const int r = a.row[p0 + k];
+    if (static_cast<unsigned>(r) >= static_cast<unsigned>(a.R)) continue;
+    char* dst = a.out + static_cast<long long>(r) * a.bytes;
+    const int at = W::offset(c, dst);
+    Piece<16> v = W::load(src, at, a.bytes);
+    if constexpr (WEIGHTED) {
+      const float w = load_weight(a.weight, a.weight_type, p0 + k);
+      float f[kElems<T, 16>];
+      unpack<T, 16>(v, f);
+#pragma unroll
+      for (auto& x : f) x *= w;
+      v = pack<T, 16>(f);
+    }
+    W::store(dst, at, a.bytes, v);
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(kThreads) collect_windows_kernel(const Rows a) {
+  release_next();
+  wait_for_previous();
+  using W = Window<T>;
+  constexpr int N = kElems<T, 16>;
+  const int windows = W::count(a.bytes);
+  const long long g = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x;
+  if (g >= static_cast<long long>(a.T) * windows) return;
+  const int t = static_cast<int>(g / windows), c = static_cast<int>(g - static_cast<long long>(t) * windows);
+  char* dst = a.out + static_cast<long long>(t) * a.bytes;
+  const int at = W::offset(c, dst);
+  float acc[N];
+#pragma unroll
+  for (auto& x : acc) x = 0.f;
+  const long long p0 = static_cast<long long>(t) * a.K;
+#pragma unroll 4
+  for (int k = 0; k < a.K; ++k) {
+    const int r = a.row[p0 + k];
+    if (static_cast<unsigned>(r) >= static_cast<unsigned>(a.R)) continue;
+    const float w = a.weight != nullptr ? load_weight(a.weight, a.weight_type, p0 + k) : 1.f;
+    float f[N];
+    unpack<T, 16>(W::load(a.row_src + r * a.row_ld, at, a.bytes), f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] += w * f[i];
+  }
+  W::store(dst, at, a.bytes, pack<T, 16>(acc));
+}
+
 // dot += <f, g> over the one or two values of a word (FULL: both halves of a 16-bit word); returns w g
 template <class T, bool FULL>
 __device__ __forceinline__ uint32_t dot_word(uint32_t f, uint32_t g, float w, float& dot) {
@@ -591,14 +712,18 @@ static int piece_bytes(std::initializer_list<long long> multiples) {
 }
 static long long address(const void* p) { return static_cast<long long>(reinterpret_cast<uintptr_t>(p)); }
 
-template <class F>
-static int for_piece(int vec, int size, F&& f) {
-  switch (vec) {
-    case 32: return f(std::integral_constant<int, 32>());
-    case 16: return f(std::integral_constant<int, 16>());
-    case 4: return f(std::integral_constant<int, 4>());
-    default: return size == 2 ? f(std::integral_constant<int, 2>()) : SMOE_ERR_ALIGNMENT;
+// LEAST: the narrowest pieces that the kernel has.
+template <int LEAST, class F>
+static int for_piece(int vec, F&& f) {
+  if (vec == 32) return f(std::integral_constant<int, 32>());
+  if (vec == 16) return f(std::integral_constant<int, 16>());
+  if constexpr (LEAST <= 4) {
+    if (vec == 4) return f(std::integral_constant<int, 4>());
   }
+  if constexpr (LEAST <= 2) {
+    if (vec == 2) return f(std::integral_constant<int, 2>());
+  }
+  return SMOE_ERR_ALIGNMENT;
 }
 
 static unsigned pad_blocks(int R) { return static_cast<unsigned>((static_cast<long long>(R) + kPadRows - 1) / kPadRows); }
@@ -609,30 +734,42 @@ static unsigned flat_blocks(const Rows& a, int vec) {
   return static_cast<unsigned>((a.T * stride + kThreads - 1) / kThreads);
 }
 
+template <class T>
+static unsigned window_blocks(const Rows& a) {
+  return static_cast<unsigned>((static_cast<long long>(a.T) * Window<T>::count(a.bytes) + kThreads - 1) / kThreads);
+}
+
 template <class T, bool WEIGHTED>
 static int launch_spread(const Rows& a, int vec, cudaStream_t st) {
-  return for_piece(vec, sizeof(T), [&](auto v) {
+  if (vec == static_cast<int>(sizeof(T))) {
+    const unsigned pad = pad_blocks(a.R);
+    return launched(launch_chained(spread_windows_kernel<T, WEIGHTED>, pad + window_blocks<T>(a), kThreads, 0, st, 1, a, static_cast<int>(pad)));
+  }
+  return for_piece<sizeof(T) == 2 ? 4 : 16>(vec, [&](auto v) {
     const unsigned pad = pad_blocks(a.R), blocks = pad + flat_blocks(a, vec);
-    return launched(launch_chained(spread_kernel<T, (v < sizeof(T) ? sizeof(T) : v), WEIGHTED>, blocks, kThreads, 0, st, 1, a,
+    return launched(launch_chained(spread_kernel<T, v, WEIGHTED>, blocks, kThreads, 0, st, 1, a,
                                    static_cast<int>(pad)));
   });
 }
 
 template <class T>
 static int launch_collect(const Rows& a, int vec, cudaStream_t st) {
-  return for_piece(vec, sizeof(T), [&](auto v) {
-    return launched(launch_chained(collect_kernel<T, (v < sizeof(T) ? sizeof(T) : v)>, flat_blocks(a, vec), kThreads, 0, st, 1, a));
+  if constexpr (sizeof(T) == 2) {
+    if (vec < 16) return launched(launch_chained(collect_windows_kernel<T>, window_blocks<T>(a), kThreads, 0, st, 1, a));
+  }
+  return for_piece<sizeof(T) == 2 ? 16 : 4>(vec, [&](auto v) {
+    return launched(launch_chained(collect_kernel<T, v>, flat_blocks(a, vec), kThreads, 0, st, 1, a));
   });
 }
 
 template <class T>
 static int launch_spread_dot(const Rows& a, int vec, cudaStream_t st) {
-  return for_piece(vec, sizeof(T), [&](auto v) {
+  return for_piece<static_cast<int>(sizeof(T))>(vec, [&](auto v) {
     const unsigned pad = pad_blocks(a.R);
     // as few rounds over the row as 256 threads allow, and no more threads than those rounds need
     const int u = pieces_per_thread(vec), pieces = (a.bytes / vec + u - 1) / u, rounds = (pieces + kThreads - 1) / kThreads;
     const unsigned threads = static_cast<unsigned>(((pieces + rounds - 1) / rounds + 31) / 32 * 32);
-    return launched(launch_chained(spread_dot_kernel<T, (v < sizeof(T) ? sizeof(T) : v)>, pad + a.T, threads, 0, st, 1, a,
+    return launched(launch_chained(spread_dot_kernel<T, v>, pad + a.T, threads, 0, st, 1, a,
                                    static_cast<int>(pad)));
   });
 }
@@ -647,7 +784,7 @@ static int for_type(int dtype, F&& f) {
 
 static bool bad_rows(int T, int K, int H, long long R, int dtype) {
   return T < 0 || K <= 0 || H <= 0 || R < 0 || R > 0x7fffffffll || static_cast<long long>(T) * K > 0x7fffffffll ||
-         static_cast<long long>(H) * type_bytes(dtype) > 0x7fffffffll;
+         static_cast<long long>(H) * type_bytes(dtype) > 0x7fffff00ll;
 }
 
 }  // namespace permute

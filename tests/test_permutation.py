@@ -12,7 +12,7 @@ def test_sizes_of_the_sorted_layout(built_library):
     assert rows(100, 8, 16) == (100 + 8 * 15) // 16 * 16 and rows(3, 8, 16) == 48
     assert rows(-1, 8, 1) == -1 and rows(1, 0, 1) == -1 and rows(1, 8, 0) == -1
     ws = lib.smoe_token_permutation_workspace_bytes
-    assert ws(8192, 1024) == 0 and ws(8193, 8) > 0 and ws(8, 1025) >= 4 * 1025
+    assert ws(2048, 1024) == 0 and ws(2049, 8) > 0 and ws(8, 1025) >= 4 * 1025
 
 
 def test_permutation_refusals(built_library):
@@ -28,7 +28,7 @@ def test_permutation_refusals(built_library):
     assert call(T=2 ** 30, K=2) == -1 and call(T=2 ** 31 - 2 ** 16, K=1) == -1 and call(align=2 ** 29) == -1
     assert call(dtype=0) == call(dtype=4) == -6
     assert call(ws=None) == -7
-    assert call(idx=None) == -1 and call(idx=at + 2) == -2 and call(dtype=3, idx=at + 4) == -2 and call(ws=at + 2) == -2
+    assert call(idx=None) == -1 and call(idx=at + 2) == -2 and call(dtype=3, idx=at + 4) == -2 and call(ws=at + 8) == -2
     for name in ("freq", "off", "gather", "scatter", "reverse"):
         assert call(**{name: None}) == -1 and call(**{name: at + 2}) == -2, name
 

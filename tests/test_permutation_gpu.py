@@ -60,7 +60,9 @@ def check_permutation(p, idx, E, align):
     (0, 2, 4, 1, 0.0), (0, 2, 4, 16, 0.0), (1, 1, 1, 1, 0.0), (1, 8, 128, 1, 0.0), (1, 1, 5, 128, 0.0), (1, 3, 2, 4, 1.0),
     (33, 3, 7, 1, 0.2), (100, 2, 3, 64, 0.3), (1024, 8, 128, 1, 0.0), (1025, 8, 60, 16, 0.1), (8192, 1, 1024, 1, 0.0),
     (8192, 1, 1025, 3, 0.0), (8193, 1, 33, 1, 0.0), (5000, 4, 1, 8, 0.5), (30000, 3, 4096, 1, 0.1), (40000, 8, 256, 128, 0.05),
-    (300, 7, 2000, 2, 1.0)])
+    (300, 7, 2000, 2, 1.0),
+    (2049, 1, 7, 1, 0.0), (4097, 2, 128, 4, 0.2), (16385, 1, 1000, 1, 0.0), (10000, 5, 64, 16, 0.1), (65536, 1, 256, 1, 0.0),
+    (65537, 1, 256, 8, 0.0)])
 def test_permutation(built_library, T, K, E, align, dropped):
     import sonicmoe
 
