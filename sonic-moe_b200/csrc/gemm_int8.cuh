@@ -518,21 +518,21 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         int rows[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) rows[i] = __shfl_sync(0xffffffffu, mine, i);
-        // all eight operations without a test between them, or up to four
-        const auto issue = [&](auto most) {
-          constexpr int MOST = decltype(most)::value;
-          for (int kb = 0; kb < num_kb; ++kb) {
-            if (!mbar_wait(smem_u32(&ss.empty[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
-            const uint32_t bar = map_to_cta(smem_u32(&ss.full[stage]), 0);
-            const uint32_t dst = smem_u32(sA + stage * A_STAGE_BYTES) + gw * (MOST == 8 ? 8 : ops) * 512;
-#pragma unroll
-            for (int q = 0; q < MOST; ++q)
-              if (MOST == 8 || q < ops)
-                tma_gather4_pair(&tmA, bar, dst + q * 512, kb * BK, rows[4 * q], rows[4 * q + 1], rows[4 * q + 2], rows[4 * q + 3]);
-            if (++stage == STAGES) { stage = 0; phase ^= 1u; }
-          }
-        };
         if (elected) {
+          // all eight operations without a test between them, or up to four
+          const auto issue = [&](auto most) {
+            constexpr int MOST = decltype(most)::value;
+            for (int kb = 0; kb < num_kb; ++kb) {
+              if (!mbar_wait(smem_u32(&ss.empty[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
+              const uint32_t bar = map_to_cta(smem_u32(&ss.full[stage]), 0);
+              const uint32_t dst = smem_u32(sA + stage * A_STAGE_BYTES) + gw * (MOST == 8 ? 8 : ops) * 512;
+#pragma unroll
+              for (int q = 0; q < MOST; ++q)
+                if (MOST == 8 || q < ops)
+                  tma_gather4_pair(&tmA, bar, dst + q * 512, kb * BK, rows[4 * q], rows[4 * q + 1], rows[4 * q + 2], rows[4 * q + 3]);
+              if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+            }
+          };
           if (ops == 8) issue(std::integral_constant<int, 8>());
           else issue(std::integral_constant<int, 4>());
         }

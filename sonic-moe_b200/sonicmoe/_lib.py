@@ -171,7 +171,7 @@ _HERE_ALREADY = contextlib.nullcontext()
 
 def on_device(device: torch.device):
     """`torch.cuda.device(device)`, or nothing where it is the current device."""
-    return _HERE_ALREADY if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE_ALREADY if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 _DTYPE_CODES = {torch.float32: SMOE_F32, torch.bfloat16: SMOE_BF16, torch.int32: SMOE_I32, torch.int64: SMOE_I64}

@@ -36,7 +36,12 @@ _ACTIVATIONS = {ActivationType.SWIGLU: 0, ActivationType.GEGLU: 1, ActivationTyp
 
 
 def _refuse_gradients(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                break
+        else:
+            return
         raise NotImplementedError("the 8-bit products have no gradient: call them under torch.no_grad()")
 
 
@@ -79,6 +84,11 @@ def _rows_16(t: torch.Tensor, name: str) -> int:
     return t.stride(-2)
 
 
+def _check_vector(t: torch.Tensor, name: str, dtype: torch.dtype, shape, dev: torch.device) -> None:
+    if t.dtype != dtype or t.shape != shape or t.device != dev or not t.is_contiguous():
+        raise ValueError(f"{name} has to be a contiguous {dtype} tensor {tuple(shape)} on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
 def _linear(x, wq, w_scale, x_scale, bias, out_dtype, activation, offset, frequency, gather):
     grouped = offset is not None
     _refuse_gradients(x, w_scale, x_scale, bias)
@@ -92,13 +102,15 @@ def _linear(x, wq, w_scale, x_scale, bias, out_dtype, activation, offset, freque
         raise ValueError(f"1 to {MAX_COLS} columns, 1 to {MAX_EXPERTS} experts and a channel are needed, got wq {tuple(wq.shape)}")
     dev = x.device
     _lib.require_cuda(x, "x")
-    for name, t, dtype, shape in (("w_scale", w_scale, torch.float32, wq.shape[:-1]), ("x_scale", x_scale, torch.float32, x.shape[:1]),
-                                  ("expert_frequency_offset", offset, torch.int32, (E + 1,)),
-                                  ("expert_frequency", frequency, torch.int32, (E,)), ("x_gather_idx", gather, torch.int32, None)):
-        if t is not None and (t.dtype != dtype or t.device != dev or not t.is_contiguous()
-                              or (t.shape != shape if shape is not None else t.dim() != 1)):
-            raise ValueError(f"{name} has to be a contiguous {dtype} tensor {tuple(shape) if shape is not None else '(rows,)'} on {dev}, got "
-                             f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    _check_vector(w_scale, "w_scale", torch.float32, wq.shape[:-1], dev)
+    if x_scale is not None:
+        _check_vector(x_scale, "x_scale", torch.float32, x.shape[:1], dev)
+    if grouped:
+        _check_vector(offset, "expert_frequency_offset", torch.int32, (E + 1,), dev)
+        if frequency is not None:
+            _check_vector(frequency, "expert_frequency", torch.int32, (E,), dev)
+        if gather is not None:
+            _check_vector(gather, "x_gather_idx", torch.int32, (gather.numel(),), dev)
     if wq.device != dev:
         raise ValueError(f"wq is on {wq.device}, x on {dev}")
     w_ld = _rows_16(wq, "wq")

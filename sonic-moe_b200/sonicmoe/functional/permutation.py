@@ -63,7 +63,7 @@ def token_permutation(topk_indices: torch.Tensor, E: int, align: int = 1) -> Tok
     idx = topk_indices.detach().contiguous()
     dev = idx.device
     with _lib.on_device(dev):
-        freq, off, gather, scatter, reverse = torch.empty(2 * E + 1 + 2 * rows + n, dtype=torch.int32, device=dev).split(
+        freq, off, gather, scatter, reverse = torch.empty(2 * E + 1 + 2 * rows + n, dtype=torch.int32, device=dev).split_with_sizes(
             (E, E + 1, rows, rows, n))
         ws = lib.smoe_token_permutation_workspace_bytes(n, E)
         ws = _lib.workspace(ws, dev) if ws else None
@@ -89,14 +89,14 @@ def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
         raise TypeError(f"{name} has to be fp32, bf16 or fp16, got {t.dtype}")
     if t.shape[1] == 0:
         raise ValueError(f"{name} has rows of no values")
-    return t if t.stride(1) == 1 and t.stride(0) >= 0 else t.contiguous()
+    return t if t.stride(1) == 1 else t.contiguous()
 
 
 def _spread(x, p: TokenPermutation, scores):
     x = _rows(x, "x")
     (T, K), R, H, dev = p.s_reverse_scatter_idx.shape, p.num_rows, x.shape[1], x.device
     with _lib.on_device(dev):
-        rows = torch.empty(R, H, dtype=x.dtype, device=dev)
+        rows = x.new_empty((R, H))
         check(lib.smoe_permute_rows(
             x.data_ptr(), x.stride(0), rows.data_ptr(), _ROW_TYPES[x.dtype], ptr(scores),
             0 if scores is None else _ROW_TYPES[scores.dtype], p.s_reverse_scatter_idx.data_ptr(), p.s_scatter_idx.data_ptr(),
@@ -108,7 +108,7 @@ def _collect(rows, p: TokenPermutation, scores):
     rows = _rows(rows, "rows")
     (T, K), R, H, dev = p.s_reverse_scatter_idx.shape, p.num_rows, rows.shape[1], rows.device
     with _lib.on_device(dev):
-        out = torch.empty(T, H, dtype=rows.dtype, device=dev)
+        out = rows.new_empty((T, H))
         check(lib.smoe_unpermute_rows(
             rows.data_ptr(), rows.stride(0), out.data_ptr(), _ROW_TYPES[rows.dtype], ptr(scores),
             0 if scores is None else _ROW_TYPES[scores.dtype], p.s_reverse_scatter_idx.data_ptr(), T, K, H, R,
@@ -154,7 +154,7 @@ class _Unpermute(torch.autograd.Function):
         dout, rows = _rows(dout, "dout"), _rows(rows, "rows")
         (T, K), R, H, dev = p.s_reverse_scatter_idx.shape, p.num_rows, rows.shape[1], rows.device
         with _lib.on_device(dev):
-            drows = torch.empty(R, H, dtype=rows.dtype, device=dev)
+            drows = rows.new_empty((R, H))
             dscores = torch.empty_like(scores)
             check(lib.smoe_unpermute_rows_backward(
                 dout.data_ptr(), dout.stride(0), rows.data_ptr(), rows.stride(0), drows.data_ptr(), _ROW_TYPES[rows.dtype],
