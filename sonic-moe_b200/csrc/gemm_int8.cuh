@@ -2,14 +2,18 @@
 // memory).  A stage holds 128 columns of an operand row, 128 bytes, so staging, swizzle and descriptors are those of the bf16
 // kernels with elements of half the size, and a stage's four MMAs (K 32 each) do twice the work in the same time.
 //
-//   tiles   256 rows x 256 channels per CTA pair: cta_group::2, two accumulators, persistent.  An expert's last tile with at most
-//           128 rows has the channels as the MMA's rows and the rows of x, up to the next 32, as its columns.
-//   units   128 channels (the MMA's rows) x up to 128 rows of x per CTA, for experts or batches with few rows, where the weights
-//           are the work: see gemm_skinny.cuh for why the operands trade places.  SPLIT: the reduction of a unit is shared by
-//           the CTAs of a cluster, where there are too few units to keep the memory busy.
+// Persistent CTA pairs (cta_group::2), tiles of 256 rows x 256 channels, two accumulators.  An expert's last tile with at most 128
+// rows (every tile of a decode step) has the operands in each other's places: its 256 channels are the MMA's rows, and its rows of
+// x, up to the next 32, the columns, so that neither rows that do not exist are multiplied nor their stages filled.
 //
-// Both take their rows from consecutive rows of x or gathered (TMA tile::gather4, a row that is none reads zeros).  The columns
-// past the last are zeros by the tensor maps' extent.  Every wait is bounded (ptx.cuh).
+// Warps of a CTA (16): 0 TMA producer (weights; x unless gathered), 1 MMA issuer (leader CTA), 2 and 3 zeros for the rows that no
+// expert has, 4..11 epilogue, 12..15 row gather with TMA tile::gather4 (a row that is none reads zeros).  The columns past the
+// last are zeros by the tensor maps' extent.
+//
+// Barriers.  full[s]: leader only; two arrivals, of the two producers, and the bytes of both CTAs.  The other CTA's producer arrives
+// although it may have nothing to load (no channels in its half of the tile): a role that a stage does not need could be overtaken
+// by the ring twice, and would take an old phase for the one it waits for.  empty[s], acc_full[a]: per CTA, by the leader's commits.
+// acc_empty[a]: leader only, one arrival per epilogue warp of both CTAs.  Every wait is bounded (ptx.cuh).
 #pragma once
 #include <type_traits>
 
@@ -117,16 +121,14 @@ __device__ __forceinline__ float activation_of(const Params& p, float x) {
 }
 
 // First rows, ends and the exclusive prefix of the row tiles of all experts, in shared memory.  One warp, all lanes.
-// Experts with rows in (least, most] count.
 template <class Shared>
-__device__ __forceinline__ void list_experts(const Params& p, Shared& ss, int tile_rows, int least, int most, int lane) {
+__device__ __forceinline__ void list_experts(const Params& p, Shared& ss, int tile_rows, int lane) {
   int running = 0;
   for (int base = 0; base < p.E; base += 32) {
     const int e = base + lane;
     int first = 0, end = 0;
     if (e < p.E) { first = first_row(p, e); end = end_row(p, e); }
-    const int rows = end - first;
-    const int v = rows > least && rows <= most ? (rows + tile_rows - 1) / tile_rows : 0;
+    const int v = max(end - first + tile_rows - 1, 0) / tile_rows;
     int incl = v;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -141,20 +143,6 @@ __device__ __forceinline__ void list_experts(const Params& p, Shared& ss, int ti
     running += __shfl_sync(0xffffffffu, incl, 31);
   }
   if (lane == 0) ss.tiles_before[p.E] = running;
-}
-
-// Whether experts with more than `limit` rows have at least half of all rows: then the tiles take every expert, as in
-// tiles_take_all.  One warp, all lanes; the two kernels of a call come to the same answer.
-__device__ __forceinline__ bool most_rows_in_tiles(const Params& p, int limit, int lane) {
-  int above = 0, all = 0;
-  for (int e = lane; e < p.E; e += 32) {
-    const int rows = max(end_row(p, e) - first_row(p, e), 0);
-    all += rows;
-    if (rows > limit) above += rows;
-  }
-  above = __reduce_add_sync(0xffffffffu, above);
-  all = __reduce_add_sync(0xffffffffu, all);
-  return 2ll * above >= all;
 }
 
 // Scale and bias of channel f + lane; scale of row row0 + lane.  Loaded before the sums are waited for.
@@ -237,15 +225,11 @@ __device__ __forceinline__ void store_rows(const Params& p, uint32_t stage, int 
   }
 }
 
-// ----------------------------------------------------------------------------------------------
-// tiles
-// ----------------------------------------------------------------------------------------------
-namespace tiles {
-
 constexpr int BM = 128, BN = 256, BN_CTA = 128, STAGES = 6;
 constexpr int A_STAGE_BYTES = BM * BK, B_STAGE_BYTES = BN_CTA * BK;
 constexpr int THREADS = 512, FIRST_EPI_WARP = 4, EPI_WARPS = 8, FIRST_GATHER_WARP = 12, GATHER_WARPS = 4;
 constexpr int COLS_PER_WARP = BN * 4 / EPI_WARPS;
+constexpr int FEW_BOX = 16;  // rows per TMA box of a tile with few rows
 
 struct Shared {
   uint64_t full[STAGES];
@@ -261,10 +245,10 @@ struct Shared {
 constexpr int SMEM_BYTES = 1024 + STAGES * (A_STAGE_BYTES + B_STAGE_BYTES) + ((sizeof(Shared) + 127) & ~127) + EPI_WARPS * (STAGE_ROWS_BYTES + COLS_PER_WARP * 4);
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory per CTA");
 
-// A last tile of at most 128 rows costs half the MMAs and less with the operands in each other's places: 256 channels are the MMA's
-// rows (each CTA its own 128, which it has staged as before), and `few` rows of x, a multiple of 32, its columns, of which
-// each CTA stages half.  The sums then lie one channel to a lane, as in the units.  Without it a 512-row load of 128 experts
-// spends a fifth of its MMAs on rows that do not exist.
+// With the operands in each other's places each CTA has its own 128 channels, staged as before, and stages half of the `few` rows of
+// x, a multiple of 32.  The sums lie one channel to a lane.  8192 tokens (H 4096, I 1024, E 128, K 8), up projection 450 -> 435 us
+// with its quantisation: without it a fifth of the MMAs works on rows that do not exist.  For experts with few rows it also replaces
+// a kernel of units of 128 channels x 128 rows per CTA (32 rows per expert there 231 -> 184 us).
 struct Tile {
   int e, row0, row_end, n0;  // row0: of this CTA's staged rows
   int first;                 // row of the pair's tile
@@ -276,10 +260,10 @@ __device__ __forceinline__ int few_rows(int rows) { return rows <= BM ? (rows + 
 struct Walker {
   const Params& p;
   const Shared& ss;
-  const int lane, num_n, total, step_m, step_n;
+  const int lane, tile_rows, num_n, total, step_m, step_n;
   int t, mi, ni, e = 0;
-  __device__ __forceinline__ Walker(const Params& p_, const Shared& ss_, int lane_)
-      : p(p_), ss(ss_), lane(lane_), num_n((p_.N + BN - 1) / BN), total(ss_.tiles_before[p_.E] * num_n),
+  __device__ __forceinline__ Walker(const Params& p_, const Shared& ss_, int lane_, int tile_rows_)
+      : p(p_), ss(ss_), lane(lane_), tile_rows(tile_rows_), num_n((p_.N + BN - 1) / BN), total(ss_.tiles_before[p_.E] * num_n),
         step_m(static_cast<int>(gridDim.x >> 1) / num_n), step_n(static_cast<int>(gridDim.x >> 1) % num_n),
         t(blockIdx.x >> 1), mi(t / num_n), ni(t % num_n) {}
   __device__ __forceinline__ void advance() {
@@ -292,7 +276,7 @@ struct Walker {
   __device__ __forceinline__ bool next_alone(int& few) {
     if (t >= total) return false;
     while (ss.tiles_before[e + 1] <= mi) ++e;
-    few = few_rows(ss.end[e] - ss.first[e] - (mi - ss.tiles_before[e]) * (2 * BM));
+    few = few_rows(min(ss.end[e] - ss.first[e] - (mi - ss.tiles_before[e]) * tile_rows, tile_rows));
     advance();
     return true;
   }
@@ -305,8 +289,8 @@ struct Walker {
       if (before != 0xffffffffu) break;
     }
     tile.e = e;
-    tile.first = ss.first[e] + (mi - ss.tiles_before[e]) * (2 * BM);
-    tile.row_end = ss.end[e];
+    tile.first = ss.first[e] + (mi - ss.tiles_before[e]) * tile_rows;
+    tile.row_end = min(ss.end[e], tile.first + tile_rows);
     tile.few = few_rows(tile.row_end - tile.first);
     tile.row0 = tile.first + static_cast<int>(rank) * (tile.few != 0 ? tile.few / 2 : BM);
     tile.n0 = ni * BN;
@@ -384,10 +368,12 @@ __device__ __forceinline__ void store_columns(const Params& p, uint32_t stage, i
   }
 }
 
-// least: experts with at most that many rows are the other kernel's.
+// tmX: rows of x, a box one row high where they are gathered, else BM rows; tmFew: boxes of FEW_BOX rows, unless gathered.
+// tile_rows: 256, or 128 where that leaves fewer CTA pairs idle.
 template <int MODE>
 __global__ void __launch_bounds__(THREADS, 1)
-int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p, const int least) {
+int8_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmFew, const __grid_constant__ CUtensorMap tmW,
+                 const Params p, const int tile_rows) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -404,7 +390,7 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(smem_u32(&ss.full[s]), 1);
+      mbar_init(smem_u32(&ss.full[s]), 2);
       mbar_init(smem_u32(&ss.empty[s]), 1);
     }
     for (int a = 0; a < 2; ++a) {
@@ -415,18 +401,15 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     fence_mbar_init();
   }
   if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmB);
+    tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&tmW);
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(&ss.tmem_base), 2 * BN);
     tmem_relinquish();
   }
   wait_for_previous();
-  if (warp == 2) {
-    const int skip = least > 0 && !most_rows_in_tiles(p, least, lane) ? least : 0;
-    list_experts(p, ss, 2 * BM, skip, p.rows, lane);
-  }
+  if (warp == 2) list_experts(p, ss, tile_rows, lane);
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();
@@ -442,19 +425,25 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       uint32_t phase = 0;
       bool ok = true;
       Tile tile;
-      Walker walk(p, ss, lane);
+      Walker walk(p, ss, lane, tile_rows);
       while (ok && walk.next(rank, tile)) {
-        const uint32_t row_bytes = gathered && tile.few != 0 ? tile.few / 2 * BK : A_STAGE_BYTES;
+        const int staged = tile.few != 0 ? tile.few / 2 : BM;  // rows of x in each CTA
+        // channels behind the last are not loaded: the other half of the tile may have none (what it holds then is never stored)
+        const int n = tile.n0 + static_cast<int>(rank) * BN_CTA;
+        const uint32_t bytes = 2 * staged * BK + (tile.n0 + BN_CTA < p.N ? 2 : 1) * B_STAGE_BYTES;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait_warp(smem_u32(&ss.empty[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
           if (elected) {
             const uint32_t bar = map_to_cta(smem_u32(&ss.full[stage]), 0);
-            if (leader) mbar_arrive_expect_tx(smem_u32(&ss.full[stage]), 2 * (row_bytes + B_STAGE_BYTES));
-            // no rows at all in this CTA's half of the tile: read past the tensor's end, which delivers zeros
-            if (!gathered)
-              tma_load_2d_pair(&tmA, bar, smem_u32(sA + stage * A_STAGE_BYTES), kb * BK, tile.row0 < tile.row_end ? tile.row0 : p.x_rows);
-            tma_load_2d_pair(&tmB, bar, smem_u32(sB + stage * B_STAGE_BYTES), kb * BK,
-                             tile.e * p.N + tile.n0 + static_cast<int>(rank) * BN_CTA);
+            if (leader) mbar_arrive_expect_tx(smem_u32(&ss.full[stage]), bytes);
+            else mbar_arrive_cluster_relaxed(bar);
+            const uint32_t x_dst = smem_u32(sA + stage * A_STAGE_BYTES);
+            if (!gathered && tile.few == 0) {
+              tma_load_2d_pair(&tmX, bar, x_dst, kb * BK, tile.row0);
+            } else if (!gathered) {
+              for (int r = 0; r < staged; r += FEW_BOX) tma_load_2d_pair(&tmFew, bar, x_dst + r * BK, kb * BK, tile.row0 + r);
+            }
+            if (n < p.N) tma_load_2d_pair(&tmW, bar, smem_u32(sB + stage * B_STAGE_BYTES), kb * BK, tile.e * p.N + n);
           }
           __syncwarp();
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
@@ -467,7 +456,7 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         int stage = 0, acc = 0, few = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
-        Walker walk(p, ss, lane);
+        Walker walk(p, ss, lane, tile_rows);
         while (ok && walk.next_alone(few)) {
           const uint32_t idesc = make_idesc_i8(2 * BM, few != 0 ? few : BN);
           if (!mbar_wait(smem_u32(&ss.acc_empty[acc]), acc_phase ^ 1u, abort_flag)) { ok = false; break; }
@@ -492,7 +481,7 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         if (!ok && p.status) atomicCAS(p.status, ST_OK, ST_TIMEOUT_MMA);
       }
     } else {
-      if (p.zero_others) zero_other_rows(p, 2 * blockIdx.x + (warp - 2), 2 * gridDim.x);
+      zero_other_rows(p, 2 * blockIdx.x + (warp - 2), 2 * gridDim.x);
     }
   } else if (warp >= FIRST_GATHER_WARP) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -504,7 +493,7 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       uint32_t phase = 0;
       bool ok = true;
       Tile tile;
-      Walker walk(p, ss, lane);
+      Walker walk(p, ss, lane, tile_rows);
       while (ok && walk.next(rank, tile)) {
         // Every warp has a quarter of the CTA's rows, 4 at least: a stage is not full without it.  A warp that had none would wait for
         // stages by parity that the others could overtake twice, and take an old phase for the one it waits for.
@@ -529,7 +518,7 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 #pragma unroll
               for (int q = 0; q < MOST; ++q)
                 if (MOST == 8 || q < ops)
-                  tma_gather4_pair(&tmA, bar, dst + q * 512, kb * BK, rows[4 * q], rows[4 * q + 1], rows[4 * q + 2], rows[4 * q + 3]);
+                  tma_gather4_pair(&tmX, bar, dst + q * 512, kb * BK, rows[4 * q], rows[4 * q + 1], rows[4 * q + 2], rows[4 * q + 3]);
               if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
           };
@@ -551,7 +540,7 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     uint32_t acc_phase = 0;
     bool ok = true;
     Tile tile;
-    Walker walk(p, ss, lane);
+    Walker walk(p, ss, lane, tile_rows);
     while (ok && walk.next(rank, tile)) {
       const auto release = [&] {
         tc_fence_before();
@@ -638,327 +627,6 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   }
 }
 
-}  // namespace tiles
 
-// ----------------------------------------------------------------------------------------------
-// units
-// ----------------------------------------------------------------------------------------------
-namespace units {
-
-constexpr int BM = 128;  // channels
-constexpr int W_STAGE_BYTES = BM * BK;
-constexpr int MAX_NT = 128, MAX_STAGES = 10, MAX_SPLIT = 8;
-constexpr int EPI_WARPS = 8, FIRST_EPI_WARP = 2, FIRST_GATHER_WARP = FIRST_EPI_WARP + EPI_WARPS, GATHER_WARPS = 4;
-constexpr int THREADS = 32 * (FIRST_GATHER_WARP + GATHER_WARPS);
-constexpr int BOX_ROWS = 32;  // rows per TMA box of a row tile that is not gathered
-
-struct Shared {
-  uint64_t full[MAX_STAGES];
-  uint64_t empty[MAX_STAGES];
-  uint64_t acc_full[2];
-  uint64_t acc_empty[2];
-  uint32_t tmem_base;
-  int abort_flag;
-  int first[kMaxExpertRows];
-  int end[kMaxExpertRows];
-  int tiles_before[kMaxExpertRows + 1];
-};
-__host__ __device__ constexpr int stage_bytes(int nt) { return W_STAGE_BYTES + nt * BK; }
-__host__ __device__ constexpr int smem_bytes(int nt, int stages) {
-  return 1024 + stages * stage_bytes(nt) + EPI_WARPS * STAGE_ROWS_BYTES + static_cast<int>(sizeof(Shared));
-}
-__host__ __device__ constexpr int num_stages(int nt) {
-  const int fit = (227 * 1024 - smem_bytes(nt, 0)) / stage_bytes(nt);
-  return fit < MAX_STAGES ? fit : MAX_STAGES;
-}
-// SPLIT: a CTA's sums of a whole unit, 32-bit integers, take the stages' place
-static_assert(MAX_NT / 2 <= 64, "a share of a unit's rows, by two warps of 32");
-static_assert(num_stages(MAX_NT) * stage_bytes(MAX_NT) >= MAX_NT * BM * 4 && num_stages(32) * stage_bytes(32) >= 32 * BM * 4, "room for the sums");
-
-struct Unit {
-  int e, row0, rows, f0;
-};
-
-// The units of this CTA (SPLIT: of its cluster), expert by expert, row tiles innermost.
-struct Walker {
-  const Params& p;
-  const Shared& ss;
-  const int lane, nt, blocks, total, step;
-  int unit, e = 0;
-  __device__ __forceinline__ Walker(const Params& p_, const Shared& ss_, int lane_, int nt_, int split)
-      : p(p_), ss(ss_), lane(lane_), nt(nt_), blocks((p_.N + BM - 1) / BM), total(ss_.tiles_before[p_.E] * blocks),
-        step(gridDim.x / split), unit(blockIdx.x / split) {}
-  __device__ __forceinline__ bool next(Unit& u) {
-    if (unit >= total) return false;
-    while (true) {
-      const int i = e + 1 + lane;
-      const unsigned before = __ballot_sync(0xffffffffu, i <= p.E && ss.tiles_before[i] * blocks <= unit);
-      e += __popc(before);
-      if (before != 0xffffffffu) break;
-    }
-    const int tiles = ss.tiles_before[e + 1] - ss.tiles_before[e];
-    const int in_expert = unit - ss.tiles_before[e] * blocks;
-    const int b = in_expert / tiles;
-    u.e = e;
-    u.f0 = b * BM;
-    u.row0 = ss.first[e] + (in_expert - b * tiles) * nt;
-    u.rows = min(nt, ss.end[e] - u.row0);
-    unit += step;
-    return true;
-  }
-};
-
-// most: experts with more rows are the tiles'.  split: CTAs of a cluster that share a unit's reduction (1: none); with SPLIT
-// there are at least as many clusters as units.
-template <int MODE, bool SPLIT>
-__global__ void __launch_bounds__(THREADS, 1)
-int8_unit_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Params p, const int8_t* wq,
-                 const long long w_ld, const int most, const int nt, const int stages, const int split) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int stage_size = stage_bytes(nt);
-  uint8_t* stage_out = smem + stages * stage_size;
-  Shared& ss = *reinterpret_cast<Shared*>(stage_out + EPI_WARPS * STAGE_ROWS_BYTES);
-  const int warp = warp_index();
-  const int lane = threadIdx.x & 31;
-  volatile int* abort_flag = &ss.abort_flag;
-  const bool gathered = p.gather != nullptr;
-  const int all_kb = (p.K + BK - 1) / BK;
-  const int slice = SPLIT ? static_cast<int>(cluster_ctarank()) : 0;
-  const int kb_begin = SPLIT ? slice * all_kb / split : 0;
-  const int kb_end = SPLIT ? (slice + 1) * all_kb / split : all_kb;
-
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < stages; ++s) {
-      mbar_init(smem_u32(&ss.full[s]), 1 + (gathered ? GATHER_WARPS : 0));
-      mbar_init(smem_u32(&ss.empty[s]), 1);
-    }
-    for (int a = 0; a < 2; ++a) {
-      mbar_init(smem_u32(&ss.acc_full[a]), 1);
-      mbar_init(smem_u32(&ss.acc_empty[a]), EPI_WARPS);
-    }
-    ss.abort_flag = 0;
-    fence_mbar_init();
-    tma_prefetch_desc(&tmW);
-    tma_prefetch_desc(&tmX);
-  }
-  if (warp == 1) {
-    tmem_alloc(smem_u32(&ss.tmem_base), 2 * MAX_NT);
-    tmem_relinquish();
-  }
-  // One expert: this CTA's weights are known before anything else is.  The L2 fetches them while the previous kernel, as a rule
-  // the one that quantises x, still runs; nothing is read into the block, so nothing can be stale.
-  if (SPLIT && p.off == nullptr && warp >= FIRST_EPI_WARP) {
-    const int tiles = (p.rows + nt - 1) / nt, f0 = static_cast<int>(blockIdx.x) / split / tiles * BM;
-    const int lines = kb_end - kb_begin, all = min(BM, p.N - f0) * lines;
-    for (int i = threadIdx.x - 32 * FIRST_EPI_WARP; i < all; i += THREADS - 32 * FIRST_EPI_WARP)
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(wq + (f0 + i / lines) * w_ld + static_cast<long long>(kb_begin + i % lines) * BK));
-  }
-  wait_for_previous();
-  if (warp == 2) {
-    const int limit = most < p.rows && most_rows_in_tiles(p, most, lane) ? 0 : most;
-    list_experts(p, ss, nt, 0, limit, lane);
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem_base = ss.tmem_base;
-  bool ok = true;
-  Unit u;
-  Walker walk(p, ss, lane, nt, split);
-
-  if (warp == 0) {
-    // ---- TMA producer -------------------------------------------------------------------------
-    const bool elected = elect_one();
-    int stage = 0;
-    uint32_t phase = 0;
-    while (ok && walk.next(u)) {
-      const int boxes = (u.rows + BOX_ROWS - 1) / BOX_ROWS;
-      const uint32_t bytes = W_STAGE_BYTES + (gathered ? (u.rows + 3) / 4 * 512 : boxes * (BOX_ROWS * BK));
-      for (int kb = kb_begin; kb < kb_end; ++kb) {
-        if (!mbar_wait_warp(smem_u32(&ss.empty[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
-        const uint32_t bar = smem_u32(&ss.full[stage]);
-        const uint32_t dst = smem_u32(smem + stage * stage_size);
-        if (elected) {
-          mbar_arrive_expect_tx(bar, bytes);
-          tma_load_2d(&tmW, bar, dst, kb * BK, u.e * p.N + u.f0);
-          if (!gathered) {
-            for (int b = 0; b < boxes; ++b)
-              tma_load_2d(&tmX, bar, dst + W_STAGE_BYTES + b * (BOX_ROWS * BK), kb * BK, u.row0 + b * BOX_ROWS);
-          }
-        }
-        __syncwarp();
-        if (++stage == stages) { stage = 0; phase ^= 1u; }
-      }
-    }
-    if (!ok && lane == 0 && p.status) atomicCAS(p.status, ST_OK, ST_TIMEOUT_PRODUCER);
-  } else if (warp == 1) {
-    // ---- MMA issuer ---------------------------------------------------------------------------
-    const bool elected = elect_one();
-    int stage = 0, acc = 0;
-    uint32_t phase = 0, acc_phase = 0;
-    while (ok && walk.next(u)) {
-      if (elected) {
-        const uint32_t idesc = make_idesc_i8(BM, (u.rows + 15) & ~15);
-        ok = mbar_wait(smem_u32(&ss.acc_empty[acc]), acc_phase ^ 1u, abort_flag);
-        tc_fence_after();
-        for (int kb = kb_begin; ok && kb < kb_end; ++kb) {
-          if (!mbar_wait(smem_u32(&ss.full[stage]), phase, abort_flag)) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t w_addr = smem_u32(smem + stage * stage_size);
-          const uint64_t a_desc = make_smem_desc(w_addr, 16, 1024);
-          const uint64_t b_desc = make_smem_desc(w_addr + W_STAGE_BYTES, 16, 1024);
-#pragma unroll
-          for (int k4 = 0; k4 < BK / UMMA_K; ++k4)
-            umma_i8<1>(tmem_base + acc * MAX_NT, a_desc + ((k4 * UMMA_K) >> 4), b_desc + ((k4 * UMMA_K) >> 4), idesc,
-                       (kb > kb_begin || k4 > 0) ? 1u : 0u);
-          umma_commit(smem_u32(&ss.empty[stage]));
-          if (++stage == stages) { stage = 0; phase ^= 1u; }
-        }
-        if (ok) umma_commit(smem_u32(&ss.acc_full[acc]));
-      }
-      ok = __all_sync(0xffffffffu, ok);
-      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
-    }
-    if (!ok && lane == 0 && p.status) atomicCAS(p.status, ST_OK, ST_TIMEOUT_MMA);
-  } else if (warp >= FIRST_GATHER_WARP) {
-    // ---- row gather; without one, the rows that no expert has ---------------------------------
-    if (gathered) {
-      const int gt = threadIdx.x - 32 * FIRST_GATHER_WARP;
-      const bool issuer = (gt & 3) == 0;
-      const int j = gt >> 2;  // rows 4j .. 4j + 3 of the unit
-      int stage = 0;
-      uint32_t phase = 0;
-      while (ok && walk.next(u)) {
-        const bool mine = issuer && 4 * j < u.rows;
-        int r4[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int s = mine && 4 * j + i < u.rows ? source_row(p, u.row0 + 4 * j + i) : -1;
-          r4[i] = s >= 0 ? s : p.x_rows;  // an index out of range delivers zeros
-        }
-        for (int kb = kb_begin; kb < kb_end; ++kb) {
-          if (!mbar_wait_warp(smem_u32(&ss.empty[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
-          if (mine)
-            tma_gather4(&tmX, smem_u32(&ss.full[stage]), smem_u32(smem + stage * stage_size) + W_STAGE_BYTES + j * 512,
-                        kb * BK, r4[0], r4[1], r4[2], r4[3]);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&ss.full[stage]));  // also where the warp has no rows: see gemm_skinny.cuh
-          if (++stage == stages) { stage = 0; phase ^= 1u; }
-        }
-      }
-      if (!ok && lane == 0 && p.status) atomicCAS(p.status, ST_OK, ST_TIMEOUT_PRODUCER);
-    }
-    if (p.zero_others) zero_other_rows(p, GATHER_WARPS * blockIdx.x + (warp - FIRST_GATHER_WARP), GATHER_WARPS * gridDim.x);
-  } else if constexpr (!SPLIT) {
-    // ---- epilogue -----------------------------------------------------------------------------
-    const int quad = warp & 3;
-    const int half = (warp - FIRST_EPI_WARP) >> 2;
-    const uint32_t my_stage = smem_u32(stage_out) + (warp - FIRST_EPI_WARP) * STAGE_ROWS_BYTES;
-    int acc = 0;
-    uint32_t acc_phase = 0;
-    while (ok && walk.next(u)) {
-      const int f = u.f0 + quad * 32;
-      float ws, bias;
-      load_channel(p, u.e, f, lane, ws, bias);
-      // a warp has the rows 32 half .. and 32 (half + 2) .. of the unit
-      const float xs0 = load_row_scale(p, u.row0 + 32 * half, u.rows - 32 * half, lane);
-      const float xs1 = load_row_scale(p, u.row0 + 32 * half + 64, u.rows - 32 * half - 64, lane);
-      if (!mbar_wait_warp(smem_u32(&ss.acc_full[acc]), acc_phase, abort_flag)) { ok = false; break; }
-      tc_fence_after();
-      const uint32_t t_addr = tmem_base + acc * MAX_NT + (static_cast<uint32_t>(quad * 32) << 16);
-      const auto release = [&] {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&ss.acc_empty[acc]));
-      };
-      const bool works = 32 * half < u.rows && f < p.N;
-      if (!works) release();
-      for (int c = half; works && 32 * c < u.rows; c += 2) {
-        uint32_t v[32];
-        tmem_ld32(t_addr + 32 * c, v);
-        tmem_ld_wait();
-        if (32 * (c + 2) >= u.rows) release();
-        store_rows<MODE>(p, my_stage, lane, f, u.row0 + 32 * c, u.rows - 32 * c, v, ws, bias, c == half ? xs0 : xs1);
-      }
-      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
-    }
-    if (!ok && lane == 0 && p.status) atomicCAS(p.status, ST_OK, ST_TIMEOUT_EPILOGUE);
-  }
-
-  if constexpr (SPLIT) {
-    // The cluster's unit: every CTA lays its sums out in its own shared memory (the stages have been read when they are
-    // complete), row by row; then each adds up an equal share of the rows over all CTAs and stores it.  32-bit integers: the
-    // order does not matter.  All threads of all CTAs meet in both cluster barriers, also after a wait that was abandoned.
-    Walker again(p, ss, lane, nt, split);
-    const bool have = again.next(u);
-    const int quad = warp & 3;
-    const bool epilogue = warp >= FIRST_EPI_WARP && warp < FIRST_GATHER_WARP;
-    const int part = (warp - FIRST_EPI_WARP) >> 2;
-    const int share = (u.rows + split - 1) / split;  // rows of this CTA; half of them, at most 32, for each of a quadrant's two warps
-    const int each = (share + 1) / 2;
-    const int begin = have ? min(slice * share + part * each, u.rows) : 0;
-    const int count = have ? min(min(begin + each, (slice + 1) * share), u.rows) - begin : 0;
-    const int f = u.f0 + quad * 32;
-    const bool works = epilogue && have && count > 0 && f < p.N;
-    float ws = 0.f, bias = 0.f, xs = 0.f;
-    if (works) {
-      load_channel(p, u.e, f, lane, ws, bias);
-      xs = load_row_scale(p, u.row0 + begin, count, lane);
-    }
-    if (epilogue && have) {
-      ok = mbar_wait_warp(smem_u32(&ss.acc_full[0]), 0, abort_flag);
-      if (ok) {
-        tc_fence_after();
-        const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
-        for (int c = part; 32 * c < u.rows; c += 2) {
-          uint32_t v[32];
-          tmem_ld32(t_addr + 32 * c, v);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) st_shared_word(smem_u32(smem) + ((32 * c + j) * BM + quad * 32 + lane) * 4, v[j]);
-        }
-        tc_fence_before();
-      } else if (lane == 0 && p.status) {
-        atomicCAS(p.status, ST_OK, ST_TIMEOUT_EPILOGUE);
-      }
-    }
-    cluster_sync_diverged();
-    if (works && ok) {
-      const uint32_t my_stage = smem_u32(stage_out) + (warp - FIRST_EPI_WARP) * STAGE_ROWS_BYTES;
-      uint32_t v[32];
-#pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = 0u;
-      for (int c = 0; c < split; ++c) {
-        const uint32_t src = map_to_cta(smem_u32(smem), c) + (begin * BM + quad * 32 + lane) * 4;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          if (j < count) {
-            uint32_t w;
-            asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(w) : "r"(src + j * BM * 4) : "memory");
-            v[j] += w;
-          }
-        }
-      }
-      store_rows<MODE>(p, my_stage, lane, f, u.row0 + begin, count, v, ws, bias, xs);
-    }
-    cluster_sync_diverged();  // no CTA leaves while another reads its sums
-  }
-
-  // ---- tear-down ----------------------------------------------------------------------------
-  __syncwarp();
-  if (*abort_flag != 0) {
-    const uint64_t t0 = global_timer_ns();
-    while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
-  }
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem_base, 2 * MAX_NT);
-  }
-}
-
-}  // namespace units
 }  // namespace i8
 }  // namespace smoe

@@ -173,7 +173,7 @@ static int quantize(const void* x, long long ld, int dtype, void* q, long long q
 // For up to 8 rows in all, where the weights are everything.  A block takes the rows of one expert (all of them: 8 at most) and 32
 // channels, a warp four of those, whose weights its lanes load 16 bytes each, straight from memory and eight loads ahead.  The
 // rows lie in shared memory, 4096 columns at a time; rows that are not 8-bit yet are quantised on the way there, by every block
-// for itself, which is a few microseconds less than a launch of its own (one token, 4096 x 4096: 13.8 + 4.1 us -> see below).
+// for itself, which takes less than a launch of its own.
 // Bound by latency: the first loads of the weights are on their way before x is looked at.
 constexpr int kDotRows = 8,  // of an expert, and of a call that takes this kernel
     kDotChannels = 4, kDotWarps = 8, kDotThreads = 32 * kDotWarps, kDotChunk = 4096, kDotAhead = 2;
@@ -358,6 +358,16 @@ static int launch_dot_of(const void* x, long long ld, const void* wq, long long 
   return wide ? launch_dot<TX, true>(x, ld, wq, w_ld, p, st) : launch_dot<TX, false>(x, ld, wq, w_ld, p, st);
 }
 
+// Whether a call goes by dot products, which read the weights at once and need no kernel of their own for x, but the time of another
+// row each.  Dot products / quantiser and tiles, us, for 1, 2, 4, 8 rows of bf16: 4096 x 4096 weights 8.1, 9.7, 13.8, 22.1 / 14.0 to
+// 14.7; 7168 x 2048 6.3, 7.2, 9.6, 14.3 / 12.0; 1024 x 1024 3.7, 4.5, 5.9, 9.0 / 8.3; but 14336 x 4096, four blocks to an SM, 20.1, 23.8,
+// 31.1, 45.1 / 20.5.  Rows of several experts, as a rule one each, are read along with other weights: 8 rows of 128 experts, 2048 x 4096
+// 24.6 / 28.7, of 256, 312 x 1600 10.2 / 21.5.
+static bool by_dots(int rows, int N, int cols, int E) {
+  if (E > 1) return rows <= kDotRows;
+  return rows <= (static_cast<long long>(N) * cols <= (32ll << 20) ? 4 : 1);
+}
+
 static int type_bytes(int dtype) { return dtype == SMOE_F32 ? 4 : dtype == SMOE_BF16 || dtype == SMOE_F16 ? 2 : 0; }
 static bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
 static long long pitch(int cols) { return (static_cast<long long>(cols) + 15) / 16 * 16; }
@@ -381,8 +391,8 @@ int smoe_int8_quantize_rows(const void* x, long long ld, int dtype, void* q, lon
   return quantize(x, ld, dtype, q, q_ld, scale, rows, cols, S(stream));
 }
 
-size_t smoe_int8_linear_workspace_bytes(int x_dtype, int x_rows, int rows, int cols) {
-  if (x_rows <= 0 || rows <= kDotRows || cols <= 0 || x_dtype == SMOE_I8) return 0;
+size_t smoe_int8_linear_workspace_bytes(int x_dtype, int x_rows, int rows, int N, int cols, int E) {
+  if (x_rows <= 0 || rows <= 0 || N <= 0 || cols <= 0 || E <= 0 || x_dtype == SMOE_I8 || by_dots(rows, N, cols, E)) return 0;
   return round256(static_cast<size_t>(x_rows) * pitch(cols)) + round256(static_cast<size_t>(x_rows) * 4);
 }
 
@@ -409,7 +419,7 @@ int smoe_int8_linear(const void* x, long long ld, int x_dtype, const float* x_sc
       (bias != nullptr && misaligned(bias, type_bytes(bias_dtype))) || misaligned(expert_frequency_offset, 4) ||
       misaligned(expert_frequency, 4) || misaligned(x_gather_idx, 4) || misaligned(status, 4))
     return SMOE_ERR_ALIGNMENT;
-  const size_t ws = smoe_int8_linear_workspace_bytes(x_dtype, x_rows, rows, cols);
+  const size_t ws = smoe_int8_linear_workspace_bytes(x_dtype, x_rows, rows, N, cols, E);
   if (ws > 0 && workspace == nullptr) return SMOE_ERR_WORKSPACE;
   if (ws > 0 && misaligned(workspace, 256)) return SMOE_ERR_ALIGNMENT;
   const long long out_cols = activation >= 0 && act_is_gated(activation) ? N / 2 : N;
@@ -420,8 +430,7 @@ int smoe_int8_linear(const void* x, long long ld, int x_dtype, const float* x_sc
   p.out = out; p.out_type = out_dtype; p.activation = activation;
   p.wide_out = !misaligned(out, 16) && out_cols * type_bytes(out_dtype) % 16 == 0;
   p.status = status;
-  if (rows <= kDotRows) {
-    p.zero_others = 1;
+  if (by_dots(rows, N, cols, E)) {
     switch (x_dtype) {
       case SMOE_I8: return launch_dot<int8_t, true>(x, ld, wq, w_ld, p, S(stream));
       case SMOE_F32: return launch_dot_of<float>(x, ld, wq, w_ld, p, S(stream));

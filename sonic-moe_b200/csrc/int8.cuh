@@ -33,7 +33,6 @@ struct Params {
   int out_type;
   int activation;        // kNoActivation or smoe::Activation
   int wide_out;          // rows of the output start on 16-byte boundaries
-  int zero_others;       // this launch zeroes the rows that no expert has
   int* status;
 };
 

@@ -108,7 +108,7 @@ SIGNATURES: dict[str, tuple] = {
     "smoe_unpermute_rows": (I, [P, LL, P, I, P, I, P, I, I, I, LL, P]),
     "smoe_unpermute_rows_backward": (I, [P, LL, P, LL, P, I, P, P, I, P, P, I, I, I, LL, P]),
     "smoe_int8_quantize_rows": (I, [P, LL, I, P, LL, P, LL, I, P]),
-    "smoe_int8_linear_workspace_bytes": (c_size_t, [I, I, I, I]),
+    "smoe_int8_linear_workspace_bytes": (c_size_t, [I, I, I, I, I, I]),
     "smoe_int8_linear": (I, [P, LL, I, P, P, LL, P, P, I, P, I, P, P, P, I, I, I, I, I, I, P, P, P]),
     "smoe_peer_alloc": (I, [c_size_t, P]),
     "smoe_peer_free": (I, [P]),

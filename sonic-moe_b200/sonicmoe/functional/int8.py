@@ -144,7 +144,7 @@ def _linear(x, wq, w_scale, x_scale, bias, out_dtype, activation, offset, freque
         raise ValueError("x has no rows to gather")
     with _lib.on_device(dev):
         out = torch.empty(rows, N // 2 if 0 <= activation <= 2 else N, dtype=out_dtype, device=dev)
-        ws = lib.smoe_int8_linear_workspace_bytes(x_type, T, rows, cols)
+        ws = lib.smoe_int8_linear_workspace_bytes(x_type, T, rows, N, cols, E)
         ws = _lib.workspace(ws, dev) if ws else None
         check(lib.smoe_int8_linear(
             x.data_ptr(), ld, x_type, ptr(x_scale), wq.data_ptr(), w_ld, w_scale.data_ptr(), ptr(bias),

@@ -142,7 +142,7 @@ def product(q, wq):
     return q.double() @ wq.double().transpose(-1, -2)
 
 
-SIZES = [(1, 1, 1), (1, 128, 4096), (3, 7, 17), (8, 34, 130), (9, 64, 16), (16, 96, 128), (33, 100, 520), (64, 2048, 256), (100, 4096, 1000),
+SIZES = [(1, 1, 1), (1, 128, 4096), (3, 7, 17), (4, 34, 130), (5, 34, 130), (9, 64, 16), (128, 700, 264), (256, 520, 400), (16, 96, 128), (33, 100, 520), (64, 2048, 256), (100, 4096, 1000),
          (129, 258, 384), (300, 130, 1000), (257, 512, 131), (1000, 300, 640), (2049, 514, 136), (700, 4096, 2048)]
 
 
@@ -248,7 +248,8 @@ def grouped_reference(p, q, xs, wq, ws, bias, E, gather, frequency):
 @pytest.mark.parametrize("T,K,E,align,dropped,N,cols", [
     (1, 1, 1, 1, 0.0, 64, 64), (1, 8, 64, 1, 0.0, 256, 512), (5, 2, 4, 16, 0.5, 130, 200), (64, 4, 32, 1, 0.0, 512, 256),
     (200, 2, 3, 128, 0.1, 96, 1030), (1000, 3, 5, 1, 0.0, 300, 144), (1027, 4, 60, 64, 0.1, 200, 130), (600, 2, 300, 1, 0.0, 64, 80),
-    (3000, 2, 4, 1, 0.0, 512, 256), (40, 2, 1000, 8, 0.0, 34, 48), (30, 2, 6, 4, 1.0, 64, 64), (2000, 8, 16, 1, 0.3, 256, 384)])
+    (3000, 2, 4, 1, 0.0, 512, 256), (40, 2, 1000, 8, 0.0, 34, 48), (30, 2, 6, 4, 1.0, 64, 64), (2000, 8, 16, 1, 0.3, 256, 384),
+    (512, 8, 64, 1, 0.0, 1536, 256), (700, 8, 64, 1, 0.0, 312, 272), (130, 2, 2, 1, 0.0, 384, 1024)])
 @pytest.mark.parametrize("gather", [False, True])
 @pytest.mark.parametrize("activation,with_bias,dtype", [(None, True, torch.float32), ("swiglu", False, torch.bfloat16),
                                                         ("gelu", True, torch.float16)])
