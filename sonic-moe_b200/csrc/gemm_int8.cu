@@ -46,10 +46,10 @@ static int encode_rows(CUtensorMap* map, const void* base, uint64_t rows, uint64
   return r == CUDA_SUCCESS ? SMOE_OK : SMOE_ERR_TENSORMAP;
 }
 
-template <int MODE>
+template <int ACT>
 static int run(const int8_t* xq, long long ld, const int8_t* wq, long long w_ld, const Params& p, cudaStream_t st) {
   static PerDeviceFlag configured;
-  const auto kernel = int8_tile_kernel<MODE>;
+  const auto kernel = int8_tile_kernel<ACT>;
   const int dev = current_device(), sms = num_sms();
   if (dev < 0 || sms < 2) return SMOE_ERR_DRIVER;
   if (!configured.test(dev)) {
@@ -71,9 +71,16 @@ static int run(const int8_t* xq, long long ld, const int8_t* wq, long long w_ld,
 }
 
 int tensor_core_product(const int8_t* xq, long long ld, const int8_t* wq, long long w_ld, const Params& p, cudaStream_t st) {
-  if (p.activation == kNoActivation) return run<MODE_PLAIN>(xq, ld, wq, w_ld, p, st);
-  if (p.activation == ACT_SWIGLU) return run<MODE_SWIGLU>(xq, ld, wq, w_ld, p, st);
-  return run<MODE_ANY>(xq, ld, wq, w_ld, p, st);
+  switch (p.activation) {
+    case ACT_SWIGLU: return run<ACT_SWIGLU>(xq, ld, wq, w_ld, p, st);
+    case ACT_GEGLU: return run<ACT_GEGLU>(xq, ld, wq, w_ld, p, st);
+    case ACT_REGLU: return run<ACT_REGLU>(xq, ld, wq, w_ld, p, st);
+    case ACT_RELU_SQ: return run<ACT_RELU_SQ>(xq, ld, wq, w_ld, p, st);
+    case ACT_RELU: return run<ACT_RELU>(xq, ld, wq, w_ld, p, st);
+    case ACT_GELU: return run<ACT_GELU>(xq, ld, wq, w_ld, p, st);
+    case ACT_SILU: return run<ACT_SILU>(xq, ld, wq, w_ld, p, st);
+    default: return run<kNoActivation>(xq, ld, wq, w_ld, p, st);
+  }
 }
 
 }  // namespace i8

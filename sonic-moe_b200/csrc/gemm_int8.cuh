@@ -26,9 +26,6 @@ namespace i8 {
 constexpr int BK = 128;  // columns, and bytes, of a stage's row
 constexpr int UMMA_K = 32;
 
-// What the epilogue is compiled for: the switch over the other activations around an element loop slows the common ones.
-enum Mode : int { MODE_PLAIN = 0, MODE_SWIGLU = 1, MODE_ANY = 2 };
-
 __host__ __device__ constexpr uint32_t make_idesc_i8(int M, int N) {
   return (2u << 4)                     // D: 32-bit integers
          | (1u << 7) | (1u << 10)      // A, B: signed bytes, K-major
@@ -108,18 +105,6 @@ __device__ __forceinline__ void store_staged(int lane, const Block& b, Piece&& p
   __syncwarp();
 }
 
-template <int MODE>
-__device__ __forceinline__ bool is_gated(const Params& p) {
-  if constexpr (MODE == MODE_PLAIN) return false;
-  else if constexpr (MODE == MODE_SWIGLU) return true;
-  else return act_is_gated(p.activation);
-}
-template <int MODE>
-__device__ __forceinline__ float activation_of(const Params& p, float x) {
-  if constexpr (MODE == MODE_SWIGLU) return silu(x);
-  else return activate(p.activation, x);
-}
-
 // First rows, ends and the exclusive prefix of the row tiles of all experts, in shared memory.  One warp, all lanes.
 template <class Shared>
 __device__ __forceinline__ void list_experts(const Params& p, Shared& ss, int tile_rows, int lane) {
@@ -161,20 +146,18 @@ __device__ __forceinline__ float load_row_scale(const Params& p, int row0, int r
 // 32 channels (lane l: channel f + l) of up to 32 rows (word j: row row0 + j), of which `rows` exist.  Neighbouring lanes exchange
 // half of their values: afterwards word j of an even lane has the channels (l, l + 1) of row 2j and that of an odd one (l - 1, l) of
 // row 2j + 1, a gate and its up value, or two values of one 32-bit store.
-template <int MODE>
+template <int ACT>
 __device__ __forceinline__ void store_rows(const Params& p, uint32_t stage, int lane, int f, int row0, int rows,
                                            const uint32_t (&v)[32], float ws, float bias, float xs) {
   const bool odd = lane & 1;
-  const bool gated = is_gated<MODE>(p);
+  constexpr bool gated = is_gated(ACT);
   float lo[16], hi[16];
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     float a = scaled(static_cast<int>(v[2 * j]), __shfl_sync(0xffffffffu, xs, 2 * j), ws);
     float b = scaled(static_cast<int>(v[2 * j + 1]), __shfl_sync(0xffffffffu, xs, 2 * j + 1), ws);
     if (p.bias != nullptr) { a += bias; b += bias; }
-    if constexpr (MODE == MODE_ANY) {
-      if (!gated) { a = activation_of<MODE>(p, a); b = activation_of<MODE>(p, b); }
-    }
+    if constexpr (!gated) { a = activate<ACT>(a); b = activate<ACT>(b); }
     const float other = __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
     lo[j] = odd ? other : a;
     hi[j] = odd ? b : other;
@@ -191,9 +174,9 @@ __device__ __forceinline__ void store_rows(const Params& p, uint32_t stage, int 
   b.half = size == 2;
   const int pair = lane >> 1;
   const auto at_word = [&](int row, int bytes, int byte) { return stage + row * bytes + byte; };
-  if (gated) {
+  if constexpr (gated) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) lo[j] = activation_of<MODE>(p, lo[j]) * hi[j];
+    for (int j = 0; j < 16; ++j) lo[j] = activate<ACT>(lo[j]) * hi[j];
     if (b.half) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -303,7 +286,7 @@ struct Walker {
 // channels, in shared memory, where they were put before the accumulator was waited for.  With loads of the same words by all
 // lanes from memory, asked for in advance or not, a tile waits up to 2.5 kilocycles for each 32 channels: 8192 x 7168 x 1024 took 72
 // us, 55 without them.
-template <int MODE>
+template <int ACT>
 __device__ __forceinline__ void store_columns(const Params& p, uint32_t stage, int lane, int row_base, int row_end, int n,
                                               const uint32_t (&v)[32], float xs, uint32_t scales, float bias) {
   float f[32];
@@ -319,7 +302,7 @@ __device__ __forceinline__ void store_columns(const Params& p, uint32_t stage, i
 #pragma unroll
     for (int j = 0; j < 32; ++j) f[j] += __shfl_sync(0xffffffffu, bias, j);
   }
-  const bool gated = is_gated<MODE>(p);
+  constexpr bool gated = is_gated(ACT);
   const long long cols = gated ? p.N / 2 : p.N;
   const int size = p.out_type == SMOE_F32 ? 4 : 2;
   Block b;
@@ -334,9 +317,9 @@ __device__ __forceinline__ void store_columns(const Params& p, uint32_t stage, i
   const auto put = [&](int q, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) { st_shared_v4(piece(lane, q), w0, w1, w2, w3); };
   const auto bits = [&](int j) { return __float_as_uint(f[j]); };
   const auto two = [&](int j) { return pack_typed(p.out_type, f[j], f[j + 1]); };
-  if (gated) {
+  if constexpr (gated) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) f[j] = activation_of<MODE>(p, f[2 * j]) * f[2 * j + 1];
+    for (int j = 0; j < 16; ++j) f[j] = activate<ACT>(f[2 * j]) * f[2 * j + 1];
     if (b.half) {
 #pragma unroll
       for (int q = 0; q < 2; ++q) put(q, two(8 * q), two(8 * q + 2), two(8 * q + 4), two(8 * q + 6));
@@ -348,10 +331,8 @@ __device__ __forceinline__ void store_columns(const Params& p, uint32_t stage, i
     }
     return;
   }
-  if constexpr (MODE == MODE_ANY) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) f[j] = activation_of<MODE>(p, f[j]);
-  }
+  for (int j = 0; j < 32; ++j) f[j] = activate<ACT>(f[j]);
   if (b.half) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) put(q, two(8 * q), two(8 * q + 2), two(8 * q + 4), two(8 * q + 6));
@@ -368,9 +349,10 @@ __device__ __forceinline__ void store_columns(const Params& p, uint32_t stage, i
   }
 }
 
+// ACT: kNoActivation or an Activation (compiled in: with a switch around the element loop's functions GELU took three times as long).
 // tmX: rows of x, a box one row high where they are gathered, else BM rows; tmFew: boxes of FEW_BOX rows, unless gathered.
 // tile_rows: 256, or 128 where that leaves fewer CTA pairs idle.
-template <int MODE>
+template <int ACT>
 __global__ void __launch_bounds__(THREADS, 1)
 int8_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmFew, const __grid_constant__ CUtensorMap tmW,
                  const Params p, const int tile_rows) {
@@ -567,7 +549,7 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
           tmem_ld32(t_addr + 32 * c, v);
           tmem_ld_wait();
           if (32 * (c + 2) >= rows) release();
-          store_rows<MODE>(p, my_stage, lane, f, tile.first + 32 * c, rows - 32 * c, v, ws, bias, c == col_half ? xs0 : xs1);
+          store_rows<ACT>(p, my_stage, lane, f, tile.first + 32 * c, rows - 32 * c, v, ws, bias, c == col_half ? xs0 : xs1);
         }
         if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
         continue;
@@ -605,7 +587,7 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
         const float b = c < 2 ? c < 1 ? bias[0] : bias[1] : c < 3 ? bias[2] : bias[3];
         tmem_ld_wait();
         if (c + 1 == COLS_PER_WARP / 32 || n + 32 >= p.N) release();
-        store_columns<MODE>(p, my_stage, lane, row_base, tile.row_end, n, v, xs, my_scales + 128 * c, b);
+        store_columns<ACT>(p, my_stage, lane, row_base, tile.row_end, n, v, xs, my_scales + 128 * c, b);
       }
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }

@@ -71,22 +71,22 @@ __device__ __forceinline__ float scaled(int acc, float xs, float ws) { return __
 // The activations' values by their definitions.  x sigmoid(x) = x / (1 + exp(-x)) with the fast exponential and division: 2^-21
 // of the value, where the hardware tanh that the bf16 epilogues use is off by 2.5e-4 of x, too much of a small result.
 __device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
-__device__ __forceinline__ float activate(int act, float x) {
-  switch (act) {
-    case ACT_SWIGLU: case ACT_SILU: return silu(x);
-    case ACT_GEGLU: case ACT_GELU: return 0.5f * x * erfcf(x * -0.70710678118654752f);
-    case ACT_RELU_SQ: return x < 0.f ? 0.f : x * x;
-    case ACT_REGLU: case ACT_RELU: return x < 0.f ? 0.f : x;  // NaN stays NaN
-  }
-  return x;
+template <int ACT>
+__device__ __forceinline__ float activate(float x) {
+  if constexpr (ACT == ACT_SWIGLU || ACT == ACT_SILU) return silu(x);
+  else if constexpr (ACT == ACT_GEGLU || ACT == ACT_GELU) return 0.5f * x * erfcf(x * -0.70710678118654752f);
+  else if constexpr (ACT == ACT_RELU_SQ) return x < 0.f ? 0.f : x * x;
+  else if constexpr (ACT == ACT_REGLU || ACT == ACT_RELU) return x < 0.f ? 0.f : x;  // NaN stays NaN
+  else return x;
 }
+__host__ __device__ constexpr bool is_gated(int act) { return act >= 0 && act_is_gated(act); }
 
 // Rows that no expert has (between an expert's rows and the next one's, behind the last) become zeros.  Warp `warp` of `warps`,
 // all its lanes; a row's expert is found by bisection.
 __device__ __forceinline__ void zero_other_rows(const Params& p, int warp, int warps) {
   if (p.off == nullptr) return;
   const int lane = threadIdx.x & 31;
-  const int cols = p.activation >= 0 && act_is_gated(p.activation) ? p.N / 2 : p.N;
+  const int cols = is_gated(p.activation) ? p.N / 2 : p.N;
   const long long bytes = static_cast<long long>(cols) * (p.out_type == SMOE_F32 ? 4 : 2);
   for (long long base = 32ll * warp; base < p.rows; base += 32ll * warps) {
     const int r = static_cast<int>(base) + lane;

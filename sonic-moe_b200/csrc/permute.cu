@@ -19,6 +19,7 @@
 
 #include "../../include/sonicmoe_b200.h"
 #include "launch.cuh"
+#include "rows16.cuh"
 
 namespace smoe {
 namespace permute {
@@ -380,37 +381,9 @@ struct Window {
   static __host__ __device__ __forceinline__ int count(int bytes) { return (bytes + 16 - static_cast<int>(sizeof(T)) + 15) / 16; }
   // offset of block i in the row at `dst`
   static __device__ __forceinline__ int offset(int i, const char* dst) { return 16 * i - static_cast<int>(reinterpret_cast<uintptr_t>(dst) & 15); }
-  // 16 bytes of `row` from `at` on, zeros where that is outside of its `bytes`
   static __device__ __forceinline__ Piece<16> load(const char* row, int at, int bytes) {
     Piece<16> v;
-    if (at >= 0 && at + 16 <= bytes) {
-      const char* p = row + at;
-      const int s = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);
-      const uint4 a = *reinterpret_cast<const uint4*>(p - s);
-      uint4 b = make_uint4(0u, 0u, 0u, 0u);
-      if (s != 0) b = *reinterpret_cast<const uint4*>(p - s + 16);  // holds the last of the 16 bytes
-      uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-      if (s & 8) {
-#pragma unroll
-        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
-      }
-      if (s & 4) {
-#pragma unroll
-        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v.w[i] = sizeof(T) == 4 ? w[i] : __funnelshift_r(w[i], w[i + 1], 8 * (s & 2));
-    } else {
-#pragma unroll
-      for (auto& x : v.w) x = 0u;
-#pragma unroll
-      for (int i = 0; i < 16 / static_cast<int>(sizeof(T)); ++i) {
-        const int o = at + i * static_cast<int>(sizeof(T));
-        if (o < 0 || o >= bytes) continue;
-        if constexpr (sizeof(T) == 4) v.w[i] = *reinterpret_cast<const uint32_t*>(row + o);
-        else v.w[i / 2] |= static_cast<uint32_t>(*reinterpret_cast<const unsigned short*>(row + o)) << (16 * (i & 1));
-      }
-    }
+    load16_of_row<T>(row, at, bytes, v.w);
     return v;
   }
   static __device__ __forceinline__ void store(char* row, int at, int bytes, const Piece<16>& v) {
