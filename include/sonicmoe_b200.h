@@ -484,7 +484,7 @@ int smoe_int8_quantize_rows(const void* x, long long ld, int dtype, void* q, lon
  * rows > 0 needs x_rows > 0.
  * activation: -1 for none, or the codes above; gated ones take the channels 2j and 2j + 1 as gate and up.  out (rows, N), or
  * (rows, N / 2) with a gated activation, packed, SMOE_F32, SMOE_BF16 or SMOE_F16.
- * cols <= 131071, E <= 1024.  workspace: smoe_int8_linear_workspace_bytes bytes, 256-byte aligned (0: may be NULL). */
+ * cols <= 131071, E <= 1024, E * N < 2^31 - 256, rows and x_rows <= 2^31 - 2^16.  workspace: smoe_int8_linear_workspace_bytes bytes, 256-byte aligned (0: may be NULL). */
 size_t smoe_int8_linear_workspace_bytes(int x_dtype, int x_rows, int rows, int N, int cols, int E);
 int smoe_int8_linear(const void* x, long long ld, int x_dtype, const float* x_scale, const void* wq, long long w_ld,
                      const float* w_scale, const void* bias, int bias_dtype, void* out, int out_dtype,

@@ -58,15 +58,18 @@ static int run(const int8_t* xq, long long ld, const int8_t* wq, long long w_ld,
     if (cudaFuncGetAttributes(&fa, kernel) != cudaSuccess || fa.numRegs != 128) return SMOE_ERR_LAUNCH;
     configured.set(dev);
   }
-  CUtensorMap tmX, tmFew, tmW;
-  int rc = encode_rows(&tmX, xq, p.x_rows, p.K, ld, p.gather != nullptr ? 1 : BM);
-  if (rc == SMOE_OK) rc = encode_rows(&tmFew, xq, p.x_rows, p.K, ld, FEW_BOX);
-  if (rc == SMOE_OK) rc = encode_rows(&tmW, wq, static_cast<uint64_t>(p.E) * p.N, p.K, w_ld, BN_CTA);
-  if (rc != SMOE_OK) return rc;
   // Tiles of 128 rows where even so no pair has two of them, whatever the load (4096 x 4096, 256 rows 17.0 -> 14.3 us); a row tile's
   // weights are loaded by each of them.
   const long long row_tiles = p.E == 1 ? (p.rows + BM - 1ll) / BM : p.rows / BM + (p.rows < p.E ? p.rows : p.E);
   const int tile_rows = row_tiles * ((p.N + BN - 1) / BN) <= sms / 2 ? BM : 2 * BM;
+  const bool gathered = p.gather != nullptr;
+  CUtensorMap tmX, tmFew, tmW;
+  int rc = encode_rows(&tmW, wq, static_cast<uint64_t>(p.E) * p.N, p.K, w_ld, BN_CTA);
+  if (rc != SMOE_OK) return rc;
+  tmX = tmFew = tmW;  // a map that no tile reads is not made
+  if (gathered || tile_rows > BM) rc = encode_rows(&tmX, xq, p.x_rows, p.K, ld, gathered ? 1 : BM);
+  if (rc == SMOE_OK && !gathered) rc = encode_rows(&tmFew, xq, p.x_rows, p.K, ld, FEW_BOX);
+  if (rc != SMOE_OK) return rc;
   return launched(launch_chained(kernel, dim3(static_cast<unsigned>(sms & ~1)), THREADS, SMEM_BYTES, st, 2, tmX, tmFew, tmW, p, tile_rows));
 }
 

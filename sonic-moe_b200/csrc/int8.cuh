@@ -15,6 +15,7 @@ namespace smoe {
 namespace i8 {
 
 constexpr int kMaxCols = 131071;     // 131071 * 128 * 128 < 2^31
+constexpr int kMaxRows = 0x7fff0000; // rows of x and of the output: a tile's last row number fits into 32 bits
 constexpr int kMaxExpertRows = 1024; // experts whose offsets the kernels keep in shared memory
 constexpr int kNoActivation = -1;
 

@@ -142,6 +142,8 @@ def _linear(x, wq, w_scale, x_scale, bias, out_dtype, activation, offset, freque
     rows = gather.numel() if gather is not None else T
     if T == 0 and rows > 0:
         raise ValueError("x has no rows to gather")
+    if max(T, rows) > 2 ** 31 - 2 ** 16 or E * N >= 2 ** 31 - 256:
+        raise ValueError(f"{max(T, rows)} rows or {E * N} channels do not fit into 32-bit numbers")
     with _lib.on_device(dev):
         out = torch.empty(rows, N // 2 if 0 <= activation <= 2 else N, dtype=out_dtype, device=dev)
         ws = lib.smoe_int8_linear_workspace_bytes(x_type, T, rows, N, cols, E)

@@ -31,7 +31,7 @@ def test_linear_refusals(built_library):
 
     given = dict(x_type=5, xs=at, work=None)  # 8-bit rows
     assert call(x_type=2) == call(out_type=2) == call(out_type=5) == call(bias=at, bias_type=3) == -6
-    for bad in (dict(T=-1), dict(rows=-1), dict(N=0), dict(cols=0), dict(cols=131072, ld=131072, w_ld=131072), dict(E=0), dict(E=1025),
+    for bad in (dict(T=-1), dict(rows=-1), dict(T=2 ** 31 - 1, rows=2 ** 31 - 1), dict(E=1024, N=2 ** 21), dict(N=0), dict(cols=0), dict(cols=131072, ld=131072, w_ld=131072), dict(E=0), dict(E=1025),
                 dict(w_ld=48), dict(ld=-1), dict(act=-2), dict(act=7), dict(act=0, N=33), dict(off=None), dict(off=None, E=1, freq=at),
                 dict(rows=17), dict(rows=9), dict(gather=at, T=0), dict(given, ld=48), dict(x=None), dict(wq=None), dict(ws=None), dict(out=None), dict(xs=at), dict(x_type=5)):
         assert call(**bad) == -1, bad
