@@ -2,7 +2,7 @@
 // memory).  A stage holds 128 columns of an operand row, 128 bytes, so staging, swizzle and descriptors are those of the bf16
 // kernels with elements of half the size, and a stage's four MMAs (K 32 each) do twice the work in the same time.
 //
-// Persistent CTA pairs (cta_group::2), tiles of 256 rows x 256 channels, two accumulators.  An expert's last tile with at most 128
+// Persistent CTA pairs (cta_group::2), tiles of 256 rows x 256 channels, two accumulators.  An expert's last tile with at most 224
 // rows (every tile of a decode step) has the operands in each other's places: its 256 channels are the MMA's rows, and its rows of
 // x, up to the next 32, the columns, so that neither rows that do not exist are multiplied nor their stages filled.
 //
@@ -237,7 +237,7 @@ struct Tile {
   int first;                 // row of the pair's tile
   int few;                   // 0: rows are the MMA's rows
 };
-__device__ __forceinline__ int few_rows(int rows) { return rows <= BM ? (rows + 31) & ~31 : 0; }
+__device__ __forceinline__ int few_rows(int rows) { return rows <= 2 * BM - 32 ? (rows + 31) & ~31 : 0; }
 
 // The tiles of this CTA pair, expert by expert, the channels of a row tile innermost, dealt out round-robin.
 struct Walker {
@@ -412,7 +412,8 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
         const int staged = tile.few != 0 ? tile.few / 2 : BM;  // rows of x in each CTA
         // channels behind the last are not loaded: the other half of the tile may have none (what it holds then is never stored)
         const int n = tile.n0 + static_cast<int>(rank) * BN_CTA;
-        const uint32_t bytes = 2 * staged * BK + (tile.n0 + BN_CTA < p.N ? 2 : 1) * B_STAGE_BYTES;
+        const bool boxes = !gathered && staged <= BM / 2;  // of FEW_BOX rows, or one of BM
+        const uint32_t bytes = 2 * (gathered || boxes ? staged : BM) * BK + (tile.n0 + BN_CTA < p.N ? 2 : 1) * B_STAGE_BYTES;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait_warp(smem_u32(&ss.empty[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
           if (elected) {
@@ -420,9 +421,9 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
             if (leader) mbar_arrive_expect_tx(smem_u32(&ss.full[stage]), bytes);
             else mbar_arrive_cluster_relaxed(bar);
             const uint32_t x_dst = smem_u32(sA + stage * A_STAGE_BYTES);
-            if (!gathered && tile.few == 0) {
+            if (!gathered && !boxes) {
               tma_load_2d_pair(&tmX, bar, x_dst, kb * BK, tile.row0);
-            } else if (!gathered) {
+            } else if (boxes) {
               for (int r = 0; r < staged; r += FEW_BOX) tma_load_2d_pair(&tmFew, bar, x_dst + r * BK, kb * BK, tile.row0 + r);
             }
             if (n < p.N) tma_load_2d_pair(&tmW, bar, smem_u32(sB + stage * B_STAGE_BYTES), kb * BK, tile.e * p.N + n);
@@ -490,7 +491,7 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
 #pragma unroll
         for (int i = 0; i < 32; ++i) rows[i] = __shfl_sync(0xffffffffu, mine, i);
         if (elected) {
-          // all eight operations without a test between them, or up to four
+          // all eight operations without a test between them, or up to four or seven
           const auto issue = [&](auto most) {
             constexpr int MOST = decltype(most)::value;
             for (int kb = 0; kb < num_kb; ++kb) {
@@ -505,7 +506,8 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
             }
           };
           if (ops == 8) issue(std::integral_constant<int, 8>());
-          else issue(std::integral_constant<int, 4>());
+          else if (ops <= 4) issue(std::integral_constant<int, 4>());
+          else issue(std::integral_constant<int, 7>());
         }
         ok = __all_sync(0xffffffffu, ok);
       }
@@ -533,11 +535,14 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
         // lanes are channels: a warp has 32 of them, and every other 32 rows
         const int f = tile.n0 + static_cast<int>(rank) * BN_CTA + quad * 32, rows = tile.row_end - tile.first;
         const bool works = f < p.N && 32 * col_half < rows;
-        float ws = 0.f, bias = 0.f, xs0 = 0.f, xs1 = 0.f;
+        float ws = 0.f, bias = 0.f, xs[4] = {0.f, 0.f, 0.f, 0.f};
         if (works) {
           load_channel(p, tile.e, f, lane, ws, bias);
-          xs0 = load_row_scale(p, tile.first + 32 * col_half, rows - 32 * col_half, lane);
-          xs1 = load_row_scale(p, tile.first + 32 * col_half + 64, rows - 32 * col_half - 64, lane);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 32 * (col_half + 2 * i);
+            xs[i] = load_row_scale(p, tile.first + r, rows - r, lane);
+          }
         }
         if (!mbar_wait_warp(smem_u32(&ss.acc_full[acc]), acc_phase, abort_flag)) { ok = false; break; }
         tc_fence_after();
@@ -549,7 +554,8 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
           tmem_ld32(t_addr + 32 * c, v);
           tmem_ld_wait();
           if (32 * (c + 2) >= rows) release();
-          store_rows<ACT>(p, my_stage, lane, f, tile.first + 32 * c, rows - 32 * c, v, ws, bias, c == col_half ? xs0 : xs1);
+          store_rows<ACT>(p, my_stage, lane, f, tile.first + 32 * c, rows - 32 * c, v, ws, bias,
+                          c < 4 ? c < 2 ? xs[0] : xs[1] : c < 6 ? xs[2] : xs[3]);
         }
         if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
         continue;
