@@ -32,26 +32,15 @@ __host__ __device__ constexpr uint32_t make_idesc_i8(int M, int N) {
          | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
-template <int CTAS>
-__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
-  if constexpr (CTAS == 2)
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
-        "}\n"
-        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
-        "}\n"
-        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
-        : "memory");
+__device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
+      "}\n"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
 }
 
 __device__ __forceinline__ void st_shared_word(uint32_t addr, uint32_t v) {
@@ -229,9 +218,11 @@ constexpr int SMEM_BYTES = 1024 + STAGES * (A_STAGE_BYTES + B_STAGE_BYTES) + ((s
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory per CTA");
 
 // With the operands in each other's places each CTA has its own 128 channels, staged as before, and stages half of the `few` rows of
-// x, a multiple of 32.  The sums lie one channel to a lane.  8192 tokens (H 4096, I 1024, E 128, K 8), up projection 450 -> 435 us
-// with its quantisation: without it a fifth of the MMAs works on rows that do not exist.  For experts with few rows it also replaces
-// a kernel of units of 128 channels x 128 rows per CTA (32 rows per expert there 231 -> 184 us).
+// x, a multiple of 32.  The sums lie one channel to a lane.  Without it a fifth of the MMAs of 8192 tokens (H 4096, I 1024, E 128, K 8)
+// works on rows that do not exist: up projection with its quantisation 450 -> 412 us.  Experts with few rows need no kernel of their
+// own either: units of 128 channels x 128 rows per CTA took 231 us for 32 rows per expert of that layer, the tiles take 184.
+// Bound by: the weights from memory below some 64 rows per expert (64 tokens of that layer, 1.0 GB in 142 us); above, the MMAs under
+// the power cap (8192 x 7168 x 4096 3.4e15 operations/s alone, tensor pipe 80 % busy at 1.5 GHz in the 8192-token load).
 struct Tile {
   int e, row0, row_end, n0;  // row0: of this CTA's staged rows
   int first;                 // row of the pair's tile
@@ -452,7 +443,7 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
             const uint64_t a_desc = few != 0 ? w_desc : x_desc, b_desc = few != 0 ? x_desc : w_desc;
 #pragma unroll
             for (int k4 = 0; k4 < BK / UMMA_K; ++k4)
-              umma_i8<2>(tmem_base + acc * BN, a_desc + ((k4 * UMMA_K) >> 4), b_desc + ((k4 * UMMA_K) >> 4), idesc,
+              umma_i8_pair(tmem_base + acc * BN, a_desc + ((k4 * UMMA_K) >> 4), b_desc + ((k4 * UMMA_K) >> 4), idesc,
                          (kb > 0 || k4 > 0) ? 1u : 0u);
             umma_commit_pair(smem_u32(&ss.empty[stage]), 3);
             if (++stage == STAGES) { stage = 0; phase ^= 1u; }
