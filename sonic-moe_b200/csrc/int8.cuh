@@ -114,19 +114,23 @@ __device__ __forceinline__ void zero_other_rows(const Params& p, int warp, int w
 // ----------------------------------------------------------------------------------------------
 // quantisation of a row: scale = amax / 127 (1 for a row of zeros), q = 127 x / amax rounded half to even
 // ----------------------------------------------------------------------------------------------
-// 16-bit values (at most 11 bits): the quotient t of 127 x and amax by a reciprocal, corrected once by its remainder, which fp32 holds
-// exactly.  That is the quotient to the last bit wherever fp32 has it, at every tie k + 1/2 among others, and any other quotient of
-// such numbers is 2^-12 or more from a tie: rounding it to a whole number is exact.
+// 16-bit values (at most 11 bits).  With significands mx, ma as whole numbers the quotient is 127 mx 2^s / ma, and it lies on a border
+// k + 1/2 where 254 mx 2^s = (2k + 1) ma.  Both sides are multiples of min(1, 2^s): a quotient off a border is off by at least 1 / (254
+// * 2047) > 2^-19 of its value.  127 divides the left side, so on a border it divides 2k + 1 (which is 127 then, the border 63.5) or ma.
+// Multiplied by 127 / amax made larger by 2^-21, values off a border stay on their side and 63.5 goes to 64, which is even: one
+// multiply-add rounds right, in every row whose ma is no multiple of 127.  In those that are, the quotient by a reciprocal is corrected
+// once by its remainder, which fp32 holds exactly, and so is exact on every border.  (That arithmetic for all rows: 8192 x 4096 bf16 23
+// us; a search for borders with remainders behind it 27, with 64-bit divisions 59.)
 // fp32 values: one fused multiply-add is within 127 * 2^-24 + 2^-15 = 3.8e-5 of the quotient, as a fixed-point number with 14 fractional
 // bits; where that is within a step of a border k + 1/2 (seldom), the remainder 127 x - q amax decides, its products held as sums
-// of two.  (The same test for 16-bit values finds a border in every third piece of a warp, most of them ties such as amax / 2: with
-// 64-bit divisions behind it 8192 rows of 4096 took 59 us, with remainders 27.)
+// of two.
 // Rows whose largest value is below 2^-120 or above 2^120 are multiplied by a power of two first, so that neither 127 / amax nor
 // 127 x leaves fp32's range.  Rows that hold an infinity or a NaN get it as their scale, and zeros: every product of theirs is NaN.
 struct RowScale {
   float pre;       // power of two for the values
   float amax;      // times pre
-  float inv;       // 1 / amax, of fp32 values 127 / amax; 0: none
+  float inv;       // 127 / amax, for 16-bit values times 1 + 2^-21; 0: none
+  bool borders;    // 16-bit values: other borders than 63.5
   uint32_t keep;   // 0: zeros
 };
 // bits: the largest |x| as an integer (a NaN's are above infinity's)
@@ -140,7 +144,9 @@ __device__ __forceinline__ RowScale row_scale(uint32_t bits) {
   const bool some = bits != 0u && bits < 0x7F800000u;
   s.pre = !some ? 1.f : bits < (7u << 23) ? 18446744073709551616.f : bits >= (247u << 23) ? 1.f / 18446744073709551616.f : 1.f;  // 2^64
   s.amax = __uint_as_float(bits) * s.pre;
-  s.inv = some ? __fdiv_rn(SHORT ? 1.f : 127.f, s.amax) : 0.f;
+  s.inv = some ? __fdiv_rn(127.f, s.amax) : 0.f;
+  if (SHORT) s.inv *= 1.f + 1.f / 2097152.f;
+  s.borders = SHORT && some && ((__float_as_uint(s.amax) & 0x7FFFFFu) | 0x800000u) % 127u == 0u;
   s.keep = some ? 0xFFFFFFFFu : 0u;
   return s;
 }
@@ -160,10 +166,16 @@ __device__ __forceinline__ void quantize_values(const RowScale& s, float (&f)[N]
   }
   int q[N];
   if constexpr (SHORT) {
+    if (s.borders) {
+      const float r = __fdiv_rn(1.f, s.amax);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float x = 127.f * f[i], t = x * s.inv;
-      q[i] = __float_as_int(fmaf(fmaf(-t, s.amax, x), s.inv, t) + kRoundMagic);
+      for (int i = 0; i < N; ++i) {
+        const float x = 127.f * f[i], t = x * r;
+        q[i] = __float_as_int(fmaf(fmaf(-t, s.amax, x), r, t) + kRoundMagic);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) q[i] = __float_as_int(fmaf(f[i], s.inv, kRoundMagic));
     }
   } else {
     uint32_t near = 0x3FFFu;
