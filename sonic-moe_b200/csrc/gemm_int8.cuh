@@ -94,26 +94,20 @@ __device__ __forceinline__ void store_staged(int lane, const Block& b, Piece&& p
   __syncwarp();
 }
 
-// First rows, ends and the exclusive prefix of the row tiles of all experts, in shared memory.  One warp, all lanes.
+// The exclusive prefix of the row tiles of all experts, from their first rows and ends in shared memory.  One warp, all lanes.
 template <class Shared>
-__device__ __forceinline__ void list_experts(const Params& p, Shared& ss, int tile_rows, int lane) {
+__device__ __forceinline__ void count_tiles(const Params& p, Shared& ss, int tile_rows, int lane) {
   int running = 0;
   for (int base = 0; base < p.E; base += 32) {
     const int e = base + lane;
-    int first = 0, end = 0;
-    if (e < p.E) { first = first_row(p, e); end = end_row(p, e); }
-    const int v = max(end - first + tile_rows - 1, 0) / tile_rows;
+    const int v = e < p.E ? max(ss.end[e] - ss.first[e] + tile_rows - 1, 0) / tile_rows : 0;
     int incl = v;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int o = __shfl_up_sync(0xffffffffu, incl, d);
       if (lane >= d) incl += o;
     }
-    if (e < p.E) {
-      ss.first[e] = first;
-      ss.end[e] = end;
-      ss.tiles_before[e] = running + incl - v;
-    }
+    if (e < p.E) ss.tiles_before[e] = running + incl - v;
     running += __shfl_sync(0xffffffffu, incl, 31);
   }
   if (lane == 0) ss.tiles_before[p.E] = running;
@@ -382,7 +376,14 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
     tmem_relinquish();
   }
   wait_for_previous();
-  if (warp == 2) list_experts(p, ss, tile_rows, lane);
+  // All experts at once: one warp by itself waits for the offsets of every 32 experts in turn (64 rows of 256 experts, 312 x 1600,
+  // 51.2 -> 50.2 us; of 32 experts, 512 x 1024, 13.3 -> 13.6).
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
+    ss.first[e] = first_row(p, e);
+    ss.end[e] = end_row(p, e);
+  }
+  __syncthreads();
+  if (warp == 2) count_tiles(p, ss, tile_rows, lane);
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();

@@ -197,7 +197,8 @@ __global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long
   __shared__ __align__(16) int8_t xs[kDotRows][kDotChunk];
   __shared__ uint32_t part[kDotRows][kDotWarps];
   __shared__ float row_scales[kDotRows];
-  __shared__ int where[3];  // expert, first row, rows
+  __shared__ int where[3];     // expert, first row, rows
+  __shared__ uint32_t owned;   // rows that an expert has (kDotRows at most in all)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n0 = (blockIdx.x * kDotWarps + warp) * kDotChannels;
   release_next();
@@ -208,21 +209,38 @@ __global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long
       for (int c = 128 * lane; c < p.K; c += 4096) asm volatile("prefetch.global.L2 [%0];" ::"l"(wq + (n0 + j) * w_ld + c));
   }
   wait_for_previous();
-  if (warp == 0) {  // the blockIdx.y-th expert that has rows
-    if (lane == 0) where[2] = 0;
-    __syncwarp();
-    int before = 0;
-    for (int e0 = 0; e0 < p.E; e0 += 32) {
-      const int e = e0 + lane;
-      const int rows = e < p.E ? end_row(p, e) - first_row(p, e) : 0;
-      const unsigned some = __ballot_sync(0xffffffffu, rows > 0);
-      if (rows > 0 && before + __popc(some & ((1u << lane) - 1u)) == static_cast<int>(blockIdx.y)) {
+  // The blockIdx.y-th expert that has rows, and which rows an expert has.  All experts are looked at together (8 rows of 256 experts,
+  // 312 x 1600, 10.2 -> 8.2 us); block (0, 0) then clears the rows that no expert has.
+  if (threadIdx.x == 0) {
+    where[2] = 0;
+    owned = 0u;
+  }
+  int before = 0;  // experts with rows so far
+  for (int e0 = 0; e0 < p.E; e0 += kDotThreads) {
+    const int e = e0 + threadIdx.x;
+    int first = 0, n = 0;
+    if (e < p.E) {
+      first = first_row(p, e);
+      n = min(end_row(p, e) - first, kDotRows);
+    }
+    const unsigned some = __ballot_sync(0xffffffffu, n > 0);
+    __syncthreads();  // the words above, and those of the last round have been read
+    if (lane == 0) part[0][warp] = __popc(some);
+    __syncthreads();
+    int at = before + __popc(some & ((1u << lane) - 1u));
+#pragma unroll
+    for (int w = 0; w < kDotWarps; ++w) {
+      const int c = part[0][w];
+      if (w < warp) at += c;
+      before += c;
+    }
+    if (n > 0) {
+      atomicOr(&owned, ((1u << n) - 1u) << first);
+      if (at == static_cast<int>(blockIdx.y)) {
         where[0] = e;
-        where[1] = first_row(p, e);
-        where[2] = min(rows, kDotRows);
+        where[1] = first;
+        where[2] = n;
       }
-      before += __popc(some);
-      if (before > static_cast<int>(blockIdx.y)) break;
     }
   }
   __syncthreads();
@@ -353,7 +371,13 @@ __global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long
       store_typed(p.out, p.out_type, static_cast<long long>(row0 + r_out) * p.N + n, activate(p.activation, y));
     }
   }
-  zero_other_rows(p, (blockIdx.y * gridDim.x + blockIdx.x) * kDotWarps + warp, gridDim.x * gridDim.y * kDotWarps);
+  if (blockIdx.x == 0 && blockIdx.y == 0) {  // rows that no expert has become zeros
+    const long long bytes = static_cast<long long>(is_gated(p.activation) ? p.N / 2 : p.N) * (p.out_type == SMOE_F32 ? 4 : 2);
+    for (int r = 0; r < p.rows; ++r) {
+      if (owned >> r & 1u) continue;
+      for (long long c = 2 * threadIdx.x; c < bytes; c += 2 * kDotThreads) *reinterpret_cast<uint16_t*>(static_cast<char*>(p.out) + r * bytes + c) = 0;
+    }
+  }
 }
 
 template <class TX, bool WIDE>
