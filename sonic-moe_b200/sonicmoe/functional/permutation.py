@@ -12,7 +12,8 @@ score is not read.  ``align`` starts every expert's rows at a multiple of it; ro
 ignored by `unpermute_tokens` whatever they hold, and get zero gradients.
 
 fp32, bf16 and fp16 rows of any width; sums in fp32 in the order of k, rounded once: the same bits every time.  The number of
-rows follows from the shapes alone, so nothing here waits for the device and all of it can be captured in a graph.
+rows follows from the shapes alone, so nothing here waits for the device and all of it can be captured in a graph.  (For a captured
+backward pass autograd itself asks that no graph recorded outside the capture still holds the same leaves.)
 The reference has no such operators: its GEMMs gather and scatter (sonicmoe/functional/__init__.py:19-82 makes the indices).
 """
 
@@ -92,27 +93,26 @@ def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
     return t if t.stride(1) == 1 else t.contiguous()
 
 
-def _spread(x, p: TokenPermutation, scores):
+def _spread(x, pair, row, scores):
     x = _rows(x, "x")
-    (T, K), R, H, dev = p.s_reverse_scatter_idx.shape, p.num_rows, x.shape[1], x.device
+    (T, K), R, H, dev = pair.shape, row.numel(), x.shape[1], x.device
     with _lib.on_device(dev):
         rows = x.new_empty((R, H))
         check(lib.smoe_permute_rows(
             x.data_ptr(), x.stride(0), rows.data_ptr(), _ROW_TYPES[x.dtype], ptr(scores),
-            0 if scores is None else _ROW_TYPES[scores.dtype], p.s_reverse_scatter_idx.data_ptr(), p.s_scatter_idx.data_ptr(),
-            T, K, H, R, stream_ptr(dev)), "permute_rows")
+            0 if scores is None else _ROW_TYPES[scores.dtype], pair.data_ptr(), row.data_ptr(), T, K, H, R, stream_ptr(dev)),
+            "permute_rows")
     return rows
 
 
-def _collect(rows, p: TokenPermutation, scores):
+def _collect(rows, pair, scores):
     rows = _rows(rows, "rows")
-    (T, K), R, H, dev = p.s_reverse_scatter_idx.shape, p.num_rows, rows.shape[1], rows.device
+    (T, K), (R, H), dev = pair.shape, rows.shape, rows.device
     with _lib.on_device(dev):
         out = rows.new_empty((T, H))
         check(lib.smoe_unpermute_rows(
             rows.data_ptr(), rows.stride(0), out.data_ptr(), _ROW_TYPES[rows.dtype], ptr(scores),
-            0 if scores is None else _ROW_TYPES[scores.dtype], p.s_reverse_scatter_idx.data_ptr(), T, K, H, R,
-            stream_ptr(dev)), "unpermute_rows")
+            0 if scores is None else _ROW_TYPES[scores.dtype], pair.data_ptr(), T, K, H, R, stream_ptr(dev)), "unpermute_rows")
     return out
 
 
@@ -122,45 +122,41 @@ def _refuse_second_derivative():
         raise NotImplementedError("sorted tokens have first derivatives only")
 
 
+# Both keep the index vectors themselves: the fields of a permutation may be replaced before the backward pass.
 class _Permute(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, p):
-        ctx.save_for_backward(p.s_reverse_scatter_idx, p.s_scatter_idx)
-        ctx.p = p
-        return _spread(x, p, None)
+    def forward(ctx, x, pair, row):
+        ctx.save_for_backward(pair)
+        return _spread(x, pair, row, None)
 
     @staticmethod
     def backward(ctx, drows):
         _refuse_second_derivative()
-        ctx.saved_tensors  # raises where an index vector was written to since
-        return _collect(drows, ctx.p, None), None
+        return _collect(drows, *ctx.saved_tensors, None), None, None
 
 
 class _Unpermute(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, rows, p, scores):
-        ctx.save_for_backward(p.s_reverse_scatter_idx, p.s_scatter_idx, scores,
-                              rows if scores is not None and ctx.needs_input_grad[2] else None)
-        ctx.p = p
-        return _collect(rows, p, scores)
+    def forward(ctx, rows, pair, row, scores):
+        ctx.save_for_backward(pair, row, scores, rows if scores is not None and ctx.needs_input_grad[3] else None)
+        return _collect(rows, pair, scores)
 
     @staticmethod
     def backward(ctx, dout):
         _refuse_second_derivative()
-        _, _, scores, rows = ctx.saved_tensors
-        p = ctx.p
+        pair, row, scores, rows = ctx.saved_tensors
         if rows is None:
-            return _spread(dout, p, scores), None, None
+            return _spread(dout, pair, row, scores), None, None, None
         dout, rows = _rows(dout, "dout"), _rows(rows, "rows")
-        (T, K), R, H, dev = p.s_reverse_scatter_idx.shape, p.num_rows, rows.shape[1], rows.device
+        (T, K), (R, H), dev = pair.shape, rows.shape, rows.device
         with _lib.on_device(dev):
             drows = rows.new_empty((R, H))
             dscores = torch.empty_like(scores)
             check(lib.smoe_unpermute_rows_backward(
                 dout.data_ptr(), dout.stride(0), rows.data_ptr(), rows.stride(0), drows.data_ptr(), _ROW_TYPES[rows.dtype],
-                scores.data_ptr(), dscores.data_ptr(), _ROW_TYPES[scores.dtype], p.s_reverse_scatter_idx.data_ptr(),
-                p.s_scatter_idx.data_ptr(), T, K, H, R, stream_ptr(dev)), "unpermute_rows_backward")
-        return drows, None, dscores
+                scores.data_ptr(), dscores.data_ptr(), _ROW_TYPES[scores.dtype], pair.data_ptr(), row.data_ptr(), T, K, H, R,
+                stream_ptr(dev)), "unpermute_rows_backward")
+        return drows, None, None, dscores
 
 
 def permute_tokens(x: torch.Tensor, permutation: TokenPermutation) -> torch.Tensor:
@@ -170,9 +166,10 @@ def permute_tokens(x: torch.Tensor, permutation: TokenPermutation) -> torch.Tens
     _check_permutation(permutation, x.device)
     if x.dim() != 2 or x.shape[0] != permutation.s_reverse_scatter_idx.shape[0]:
         raise ValueError(f"x has to be ({permutation.s_reverse_scatter_idx.shape[0]}, H), got {tuple(x.shape)}")
+    pair, row = permutation.s_reverse_scatter_idx, permutation.s_scatter_idx
     if torch.is_grad_enabled() and x.requires_grad:
-        return _Permute.apply(x, permutation)
-    return _spread(x, permutation, None)
+        return _Permute.apply(x, pair, row)
+    return _spread(x, pair, row, None)
 
 
 def unpermute_tokens(rows: torch.Tensor, permutation: TokenPermutation, scores: torch.Tensor | None = None) -> torch.Tensor:
@@ -182,13 +179,14 @@ def unpermute_tokens(rows: torch.Tensor, permutation: TokenPermutation, scores: 
     _check_permutation(permutation, rows.device)
     if rows.dim() != 2 or rows.shape[0] != permutation.num_rows:
         raise ValueError(f"rows has to be ({permutation.num_rows}, H), got {tuple(rows.shape)}")
+    pair = permutation.s_reverse_scatter_idx
     if scores is not None:
-        if scores.shape != permutation.s_reverse_scatter_idx.shape or scores.device != rows.device:
-            raise ValueError(f"scores has to be {tuple(permutation.s_reverse_scatter_idx.shape)} on {rows.device}, got "
+        if scores.shape != pair.shape or scores.device != rows.device:
+            raise ValueError(f"scores has to be {tuple(pair.shape)} on {rows.device}, got "
                              f"{tuple(scores.shape)} on {scores.device}")
         if scores.dtype not in _ROW_TYPES:
             raise TypeError(f"scores has to be fp32, bf16 or fp16, got {scores.dtype}")
         scores = scores.contiguous()
     if torch.is_grad_enabled() and (rows.requires_grad or (scores is not None and scores.requires_grad)):
-        return _Unpermute.apply(rows, permutation, scores)
-    return _collect(rows, permutation, scores)
+        return _Unpermute.apply(rows, pair, permutation.s_scatter_idx, scores)
+    return _collect(rows, pair, scores)

@@ -237,6 +237,26 @@ def test_broadcast_gradients(built_library):
     assert torch.equal(dy, want.unsqueeze(1).expand(-1, H))
 
 
+def test_fields_replaced_before_the_backward_pass(built_library):
+    """Gradients belong to the permutation of the forward pass, whatever its object holds by then (here: fewer, other rows)."""
+    import sonicmoe
+
+    T, K, E, H = 50, 2, 4, 24
+    p, q = (sonicmoe.token_permutation(indices(t, K, E, 0.2, seed=t).cuda(), E) for t in (T, 20))
+    x = source(T, H, torch.float32, 1).requires_grad_(True)
+    y = source(T * K, H, torch.float32, 2).requires_grad_(True)
+    s = torch.rand(T, K, device="cuda", requires_grad=True)
+    drows, dout = source(T * K, H, torch.float32, 3), source(T, H, torch.float32, 4)
+
+    def outputs():
+        return sonicmoe.permute_tokens(x, p), sonicmoe.unpermute_tokens(y, p), sonicmoe.unpermute_tokens(y, p, s)
+
+    want = torch.autograd.grad(outputs(), (x, y, s), (drows, dout, dout))
+    held = outputs()
+    p.s_reverse_scatter_idx, p.s_scatter_idx = q.s_reverse_scatter_idx, q.s_scatter_idx
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(held, (x, y, s), (drows, dout, dout))))
+
+
 def test_streams_graphs_and_repeats(built_library):
     """On a stream of its own, captured with its backward pass and replayed on new values: the same bits as outside."""
     import sonicmoe
