@@ -30,8 +30,9 @@ static inline cudaStream_t S(void* s) { return static_cast<cudaStream_t>(s); }
 // the permutation
 // ----------------------------------------------------------------------------------------------
 constexpr int kMaxExperts = 4096;
-constexpr int kMaxBlocks = 128;
+constexpr int kMaxBlocks = 256;
 constexpr int kWarps = 8, kSteps = 8;                 // warps of a block; groups of 32 pairs that a warp has at a time, at most
+constexpr int kScanWarps = 4;
 constexpr int kOneWarps = 32;                         // the form with one block
 constexpr int kOneMaxPairs = 2048, kOneMaxExperts = 1024;
 static_assert(kOneMaxPairs <= kOneWarps * kSteps * 32, "pairs that the block's registers hold");
@@ -138,7 +139,8 @@ __device__ __forceinline__ void mark_rest(const Plan& a, const int* offset, int 
 
 __device__ __forceinline__ int round_up(int n, int align) { return (n + align - 1) / align * align; }
 
-// Up to kOneMaxPairs pairs: one block does it all from registers and shared memory, one launch instead of three.
+// Up to kOneMaxPairs pairs: one block does it all from registers and shared memory, one launch instead of three.  512, 1024, 2048
+// pairs 4.5, 5.7, 8.0 us; three launches 6.6 for each, and about 4 us more of the host's time.
 __global__ void __launch_bounds__(32 * kOneWarps) permutation_one_block_kernel(const Plan a) {
   release_next();
   wait_for_previous();
@@ -188,48 +190,39 @@ __global__ void __launch_bounds__(32 * kWarps) permutation_count_kernel(const Pl
   for (int e = threadIdx.x; e < a.E; e += blockDim.x) a.hist[e * kMaxBlocks + blockIdx.x] = smem[e];
 }
 
-// hist[e][b] -> pairs of expert e in the blocks before b; counts and offsets.  A warp has an expert at a time, a lane four of its
-// blocks (the ones that do not exist count nothing).  With the experts' words `blocks` apart and one thread per expert, 128
-// blocks and 128 experts took 34 us.
-__global__ void __launch_bounds__(1024) permutation_scan_kernel(const Plan a, int blocks) {
+// hist[e][b] -> pairs of expert e in the blocks before b; counts.  A warp has an expert, a lane four of its blocks at a time (the
+// ones that do not exist count nothing).
+__global__ void __launch_bounds__(32 * kScanWarps) permutation_scan_kernel(const Plan a, int blocks) {
   release_next();
   wait_for_previous();
-  __shared__ int partial[32];
-  __shared__ int count[kMaxExperts];
-  const int lane = threadIdx.x & 31;
-  static_assert(kMaxBlocks == 128, "a warp's lanes have four blocks each");
-#pragma unroll 4
-  for (int e = threadIdx.x >> 5; e < a.E; e += 32) {
-    int4* words = reinterpret_cast<int4*>(a.hist + e * kMaxBlocks) + lane;
-    int4 v = *words;
-    if (4 * lane >= blocks) v.x = 0;
-    if (4 * lane + 1 >= blocks) v.y = 0;
-    if (4 * lane + 2 >= blocks) v.z = 0;
-    if (4 * lane + 3 >= blocks) v.w = 0;
-    const int own = v.x + v.y + v.z + v.w;
+  constexpr int kQuads = kMaxBlocks / 128;
+  static_assert(kMaxBlocks % 128 == 0, "a warp's lanes have four blocks each at a time");
+  const int lane = threadIdx.x & 31, e = blockIdx.x * kScanWarps + (threadIdx.x >> 5);
+  if (e >= a.E) return;
+  int4* words = reinterpret_cast<int4*>(a.hist + e * kMaxBlocks) + lane;
+  int4 v[kQuads];
+#pragma unroll
+  for (int q = 0; q < kQuads; ++q) v[q] = words[32 * q];
+  int all = 0;
+#pragma unroll
+  for (int q = 0; q < kQuads; ++q) {
+    const int b = 128 * q + 4 * lane;
+    if (b >= blocks) v[q].x = 0;
+    if (b + 1 >= blocks) v[q].y = 0;
+    if (b + 2 >= blocks) v[q].z = 0;
+    if (b + 3 >= blocks) v[q].w = 0;
+    const int own = v[q].x + v[q].y + v[q].z + v[q].w;
     int incl = own;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int o = __shfl_up_sync(0xffffffffu, incl, d);
       if (lane >= d) incl += o;
     }
-    const int before = incl - own;
-    *words = make_int4(before, before + v.x, before + v.x + v.y, before + v.x + v.y + v.z);
-    if (lane == 31) {
-      count[e] = incl;
-      a.count[e] = incl;
-    }
+    const int before = all + incl - own;
+    words[32 * q] = make_int4(before, before + v[q].x, before + v[q].x + v[q].y, before + v[q].x + v[q].y + v[q].z);
+    all += __shfl_sync(0xffffffffu, incl, 31);
   }
-  __syncthreads();
-  int before = 0;
-  for (int e0 = 0; e0 < a.E; e0 += blockDim.x) {
-    const int e = e0 + threadIdx.x;
-    int total;
-    const int at = before + block_scan(e < a.E ? round_up(count[e], a.align) : 0, partial, &total);
-    before += total;
-    if (e < a.E) a.offset[e] = at;
-  }
-  if (threadIdx.x == 0) a.offset[a.E] = before;
+  if (lane == 0) a.count[e] = all;
 }
 
 // steps: groups of 32 pairs of a warp, so that a block has a chunk of 32 * steps * kWarps at a time.
@@ -237,10 +230,28 @@ __global__ void __launch_bounds__(32 * kWarps) permutation_place_kernel(const Pl
   release_next();
   wait_for_previous();
   extern __shared__ int smem[];
-  int* base = smem;                                             // (E) next row of every expert
-  uint16_t* cnt = reinterpret_cast<uint16_t*>(smem + a.E);      // (kWarps, E)
+  __shared__ int partial[kWarps];
+  int* offset = smem;                                                // (E + 1)
+  int* base = smem + a.E + 1;                                        // (E) next row of every expert
+  uint16_t* cnt = reinterpret_cast<uint16_t*>(smem + 2 * a.E + 1);   // (kWarps, E)
   const int warp = threadIdx.x >> 5;
-  for (int e = threadIdx.x; e < a.E; e += blockDim.x) base[e] = a.offset[e] + a.hist[e * kMaxBlocks + blockIdx.x];
+  int before = 0;
+  for (int e0 = 0; e0 < a.E; e0 += blockDim.x) {
+    const int e = e0 + threadIdx.x;
+    const int c = e < a.E ? a.count[e] : 0, in_blocks = e < a.E ? a.hist[e * kMaxBlocks + blockIdx.x] : 0;
+    int total;
+    const int at = before + block_scan(round_up(c, a.align), partial, &total);
+    before += total;
+    if (e < a.E) {
+      offset[e] = at;
+      base[e] = at + in_blocks;
+      if (blockIdx.x == 0) a.offset[e] = at;
+    }
+  }
+  if (threadIdx.x == 0) {
+    offset[a.E] = before;
+    if (blockIdx.x == 0) a.offset[a.E] = before;
+  }
   Plan mine = a;
   const long long end = static_cast<long long>(blockIdx.x + 1) * per_block;
   mine.n = end < a.n ? static_cast<int>(end) : a.n;
@@ -267,7 +278,8 @@ __global__ void __launch_bounds__(32 * kWarps) permutation_place_kernel(const Pl
       if (e < a.E) base[e] += sum[j];
     }
   }
-  mark_rest(a, a.offset, blockIdx.x, gridDim.x);
+  __syncthreads();
+  mark_rest(a, offset, blockIdx.x, gridDim.x);
 }
 
 // ----------------------------------------------------------------------------------------------
@@ -806,7 +818,7 @@ int smoe_token_permutation(const void* expert_idx, int idx_dtype, int T, int K, 
   const int dev = current_device();
   if (dev < 0) return SMOE_ERR_DRIVER;
   const auto one_smem = [](int e) { return (e + 1) * 4 + kOneWarps * e * 2; };
-  const auto place_smem = [](int e) { return e * 4 + kWarps * e * 2; };
+  const auto place_smem = [](int e) { return (2 * e + 1) * 4 + kWarps * e * 2; };
   if (!configured.test(dev)) {
     if (cudaFuncSetAttribute(permutation_one_block_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, one_smem(kOneMaxExperts)) != cudaSuccess ||
         cudaFuncSetAttribute(permutation_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, place_smem(kMaxExperts)) != cudaSuccess)
@@ -815,7 +827,9 @@ int smoe_token_permutation(const void* expert_idx, int idx_dtype, int T, int K, 
   }
   if (ws == 0)
     return launched(launch_chained(permutation_one_block_kernel, 1, 32 * kOneWarps, one_smem(E), S(stream), 1, a));
-  // as many blocks as there may be, each with a multiple of 256 pairs: with 2048 of them per block 24594 pairs took 12 blocks
+  // As many blocks as there may be, each with a multiple of 256 pairs: 24594 pairs would be 12 blocks of 2048.  65536 and 262144
+  // pairs of 128 experts: at most 128 blocks 8.4 and 19.7 us, 256 blocks 7.8 and 13.9, 512 blocks 8.2 and 15.2.  (One block that
+  // scanned all experts made 11.5 and 22.3 of the first.)
   const long long group = 32 * kWarps;
   long long per_block = (n + kMaxBlocks - 1) / kMaxBlocks;
   per_block = per_block > 0 ? (per_block + group - 1) / group * group : group;
@@ -823,7 +837,7 @@ int smoe_token_permutation(const void* expert_idx, int idx_dtype, int T, int K, 
   const int blocks = n > 0 ? static_cast<int>((n + per_block - 1) / per_block) : 1;
   const int per = static_cast<int>(per_block);
   cudaError_t rc = launch_chained(permutation_count_kernel, blocks, 32 * kWarps, E * 4, S(stream), 1, a, per);
-  if (rc == cudaSuccess) rc = launch_chained(permutation_scan_kernel, 1, 1024, 0, S(stream), 1, a, blocks);
+  if (rc == cudaSuccess) rc = launch_chained(permutation_scan_kernel, (E + kScanWarps - 1) / kScanWarps, 32 * kScanWarps, 0, S(stream), 1, a, blocks);
   if (rc == cudaSuccess) rc = launch_chained(permutation_place_kernel, blocks, 32 * kWarps, place_smem(E), S(stream), 1, a, per, steps);
   return launched(rc, 3);
 }

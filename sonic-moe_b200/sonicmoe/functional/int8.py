@@ -65,7 +65,7 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
         check(lib.smoe_int8_quantize_rows(x2.data_ptr(), x2.stride(0), _FLOAT_TYPES[x.dtype], q.data_ptr(), q.shape[-1],
                                           scale.data_ptr(), rows, cols, stream_ptr(dev)), "int8_quantize_rows")
-    return q[..., :cols], scale
+    return q if q.shape[-1] == cols else q[..., :cols], scale
 
 
 def _activation_code(activation_type) -> int:
