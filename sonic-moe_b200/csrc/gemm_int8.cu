@@ -46,31 +46,45 @@ static int encode_rows(CUtensorMap* map, const void* base, uint64_t rows, uint64
   return r == CUDA_SUCCESS ? SMOE_OK : SMOE_ERR_TENSORMAP;
 }
 
-template <int ACT>
-static int run(const int8_t* xq, long long ld, const int8_t* wq, long long w_ld, const Params& p, cudaStream_t st) {
+template <int ACT, bool NARROW>
+static int launch(const CUtensorMap& tmX, const CUtensorMap& tmFew, const CUtensorMap& tmW, const Params& p, int tile_rows, int channels,
+                  int sms, cudaStream_t st) {
   static PerDeviceFlag configured;
-  const auto kernel = int8_tile_kernel<ACT>;
-  const int dev = current_device(), sms = num_sms();
-  if (dev < 0 || sms < 2) return SMOE_ERR_DRIVER;
+  const auto kernel = int8_tile_kernel<ACT, NARROW>;
+  const int dev = current_device();
+  if (dev < 0) return SMOE_ERR_DRIVER;
   if (!configured.test(dev)) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) return SMOE_ERR_LAUNCH;
     cudaFuncAttributes fa;  // setmaxnreg 56 / 200 balances only around 128 registers per thread at launch
     if (cudaFuncGetAttributes(&fa, kernel) != cudaSuccess || fa.numRegs != 128) return SMOE_ERR_LAUNCH;
     configured.set(dev);
   }
-  // Tiles of 128 rows where even so no pair has two of them, whatever the load (4096 x 4096, 256 rows 17.0 -> 14.3 us); a row tile's
-  // weights are loaded by each of them.
-  const long long row_tiles = p.E == 1 ? (p.rows + BM - 1ll) / BM : p.rows / BM + (p.rows < p.E ? p.rows : p.E);
-  const int tile_rows = row_tiles * ((p.N + BN - 1) / BN) <= sms / 2 ? BM : 2 * BM;
+  return launched(launch_chained(kernel, dim3(static_cast<unsigned>(sms & ~1)), THREADS, SMEM_BYTES, st, 2, tmX, tmFew, tmW, p, tile_rows, channels));
+}
+
+template <int ACT>
+static int run(const int8_t* xq, long long ld, const int8_t* wq, long long w_ld, const Params& p, cudaStream_t st) {
+  const int sms = num_sms();
+  if (sms < 2) return SMOE_ERR_DRIVER;
+  // Smaller tiles where even so no pair has two of them, whatever the load, so that pairs which had none load too; a row tile's weights
+  // are loaded by each of them, x by each tile of channels.
   const bool gathered = p.gather != nullptr;
+  const auto one_each = [&](long long rows, int channels) {
+    const long long row_tiles = p.E == 1 ? (p.rows + rows - 1) / rows : p.rows / rows + (p.rows < p.E ? p.rows : p.E);
+    return row_tiles * ((p.N + channels - 1) / channels) <= sms / 2;
+  };
+  int tile_rows = one_each(BM, BN) ? BM : 2 * BM, channels = BN;
+  if (!gathered && one_each(128, 128)) tile_rows = channels = 128;
+  if (!gathered && one_each(64, 64)) tile_rows = channels = 64;
   CUtensorMap tmX, tmFew, tmW;
-  int rc = encode_rows(&tmW, wq, static_cast<uint64_t>(p.E) * p.N, p.K, w_ld, BN_CTA);
+  int rc = encode_rows(&tmW, wq, static_cast<uint64_t>(p.E) * p.N, p.K, w_ld, channels / 2);
   if (rc != SMOE_OK) return rc;
   tmX = tmFew = tmW;  // a map that no tile reads is not made
   if (gathered || tile_rows > BM) rc = encode_rows(&tmX, xq, p.x_rows, p.K, ld, gathered ? 1 : BM);
-  if (rc == SMOE_OK && !gathered) rc = encode_rows(&tmFew, xq, p.x_rows, p.K, ld, FEW_BOX);
+  if (rc == SMOE_OK && !gathered) rc = encode_rows(&tmFew, xq, p.x_rows, p.K, ld, channels < BN ? NARROW_BOX : FEW_BOX);
   if (rc != SMOE_OK) return rc;
-  return launched(launch_chained(kernel, dim3(static_cast<unsigned>(sms & ~1)), THREADS, SMEM_BYTES, st, 2, tmX, tmFew, tmW, p, tile_rows));
+  return channels < BN ? launch<ACT, true>(tmX, tmFew, tmW, p, tile_rows, channels, sms, st)
+                       : launch<ACT, false>(tmX, tmFew, tmW, p, tile_rows, channels, sms, st);
 }
 
 int tensor_core_product(const int8_t* xq, long long ld, const int8_t* wq, long long w_ld, const Params& p, cudaStream_t st) {

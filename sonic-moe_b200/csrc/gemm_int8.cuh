@@ -6,6 +6,12 @@
 // rows (every tile of a decode step) has the operands in each other's places: its 256 channels are the MMA's rows, and its rows of
 // x, up to the next 32, the columns, so that neither rows that do not exist are multiplied nor their stages filled.
 //
+// Narrow tiles, of 64 rows x 64 channels or 128 x 128, where that many tiles are not more than the pairs (dense products of few
+// rows): a stage's bytes hold four or two blocks of 128 columns, so that each of more pairs has as many bytes on their way, which
+// is what a short walk waits for, and an MMA has 128 rows, which takes half the time of one with 256.  Channels are the MMA's rows
+// here too.  33 rows, 8-bit x: 4096 x 4096 13.1 -> 9.9 us, 2048 x 7168 18.2 -> 12.2, 7168 x 2048 10.5 -> 9.5, 1024 x 1024 7.6 -> 6.9.
+// (A block of 64 channels reads 128 bytes each of as many rows again behind its own: sums that no lane takes.)
+//
 // Warps of a CTA (16): 0 TMA producer (weights; x unless gathered), 1 MMA issuer (leader CTA), 2 and 3 zeros for the rows that no
 // expert has, 4..11 epilogue, 12..15 row gather with TMA tile::gather4 (a row that is none reads zeros).  The columns past the
 // last are zeros by the tensor maps' extent.
@@ -195,7 +201,8 @@ constexpr int BM = 128, BN = 256, BN_CTA = 128, STAGES = 6;
 constexpr int A_STAGE_BYTES = BM * BK, B_STAGE_BYTES = BN_CTA * BK;
 constexpr int THREADS = 512, FIRST_EPI_WARP = 4, EPI_WARPS = 8, FIRST_GATHER_WARP = 12, GATHER_WARPS = 4;
 constexpr int COLS_PER_WARP = BN * 4 / EPI_WARPS;
-constexpr int FEW_BOX = 16;  // rows per TMA box of a tile with few rows
+constexpr int FEW_BOX = 16;     // rows per TMA box of a tile with few rows
+constexpr int NARROW_BOX = 32;  // of a narrow tile
 
 struct Shared {
   uint64_t full[STAGES];
@@ -222,16 +229,21 @@ struct Tile {
   int first;                 // row of the pair's tile
   int few;                   // 0: rows are the MMA's rows
 };
-__device__ __forceinline__ int few_rows(int rows) { return rows <= 2 * BM - 32 ? (rows + 31) & ~31 : 0; }
+template <bool NARROW>
+__device__ __forceinline__ int few_rows(int rows) {
+  if (NARROW) return rows <= 64 ? 64 : 128;
+  return rows <= 2 * BM - 32 ? (rows + 31) & ~31 : 0;
+}
 
 // The tiles of this CTA pair, expert by expert, the channels of a row tile innermost, dealt out round-robin.
+template <bool NARROW>
 struct Walker {
   const Params& p;
   const Shared& ss;
-  const int lane, tile_rows, num_n, total, step_m, step_n;
+  const int lane, tile_rows, channels, num_n, total, step_m, step_n;
   int t, mi, ni, e = 0;
-  __device__ __forceinline__ Walker(const Params& p_, const Shared& ss_, int lane_, int tile_rows_)
-      : p(p_), ss(ss_), lane(lane_), tile_rows(tile_rows_), num_n((p_.N + BN - 1) / BN), total(ss_.tiles_before[p_.E] * num_n),
+  __device__ __forceinline__ Walker(const Params& p_, const Shared& ss_, int lane_, int tile_rows_, int channels_)
+      : p(p_), ss(ss_), lane(lane_), tile_rows(tile_rows_), channels(channels_), num_n((p_.N + channels_ - 1) / channels_), total(ss_.tiles_before[p_.E] * num_n),
         step_m(static_cast<int>(gridDim.x >> 1) / num_n), step_n(static_cast<int>(gridDim.x >> 1) % num_n),
         t(blockIdx.x >> 1), mi(t / num_n), ni(t % num_n) {}
   __device__ __forceinline__ void advance() {
@@ -244,7 +256,7 @@ struct Walker {
   __device__ __forceinline__ bool next_alone(int& few) {
     if (t >= total) return false;
     while (ss.tiles_before[e + 1] <= mi) ++e;
-    few = few_rows(min(ss.end[e] - ss.first[e] - (mi - ss.tiles_before[e]) * tile_rows, tile_rows));
+    few = few_rows<NARROW>(min(ss.end[e] - ss.first[e] - (mi - ss.tiles_before[e]) * tile_rows, tile_rows));
     advance();
     return true;
   }
@@ -259,9 +271,9 @@ struct Walker {
     tile.e = e;
     tile.first = ss.first[e] + (mi - ss.tiles_before[e]) * tile_rows;
     tile.row_end = min(ss.end[e], tile.first + tile_rows);
-    tile.few = few_rows(tile.row_end - tile.first);
+    tile.few = few_rows<NARROW>(tile.row_end - tile.first);
     tile.row0 = tile.first + static_cast<int>(rank) * (tile.few != 0 ? tile.few / 2 : BM);
-    tile.n0 = ni * BN;
+    tile.n0 = ni * channels;
     advance();
     return true;
   }
@@ -336,11 +348,11 @@ __device__ __forceinline__ void store_columns(const Params& p, uint32_t stage, i
 
 // ACT: kNoActivation or an Activation (compiled in: with a switch around the element loop's functions GELU took three times as long).
 // tmX: rows of x, a box one row high where they are gathered, else BM rows; tmFew: boxes of FEW_BOX rows, unless gathered.
-// tile_rows: 256, or 128 where that leaves fewer CTA pairs idle.
-template <int ACT>
+// tile_rows: 256, or 128 where that leaves fewer CTA pairs idle.  NARROW: tile_rows = narrow_channels = 64 or 128, not gathered.
+template <int ACT, bool NARROW>
 __global__ void __launch_bounds__(THREADS, 1)
 int8_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmFew, const __grid_constant__ CUtensorMap tmW,
-                 const Params p, const int tile_rows) {
+                 const Params p, const int tile_rows, const int narrow_channels) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -353,7 +365,9 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
   const bool leader = rank == 0;
   volatile int* abort_flag = &ss.abort_flag;
   const int num_kb = (p.K + BK - 1) / BK;
-  const bool gathered = p.gather != nullptr;
+  const bool gathered = !NARROW && p.gather != nullptr;
+  const int channels = NARROW ? narrow_channels : BN, half = channels / 2;
+  const int per_stage = NARROW ? BN / channels : 1;  // blocks of BK columns
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -399,26 +413,31 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
       uint32_t phase = 0;
       bool ok = true;
       Tile tile;
-      Walker walk(p, ss, lane, tile_rows);
+      Walker<NARROW> walk(p, ss, lane, tile_rows, channels);
       while (ok && walk.next(rank, tile)) {
         const int staged = tile.few != 0 ? tile.few / 2 : BM;  // rows of x in each CTA
         // channels behind the last are not loaded: the other half of the tile may have none (what it holds then is never stored)
-        const int n = tile.n0 + static_cast<int>(rank) * BN_CTA;
-        const bool boxes = !gathered && staged <= BM / 2;  // of FEW_BOX rows, or one of BM
-        const uint32_t bytes = 2 * (gathered || boxes ? staged : BM) * BK + (tile.n0 + BN_CTA < p.N ? 2 : 1) * B_STAGE_BYTES;
-        for (int kb = 0; kb < num_kb; ++kb) {
+        const int n = tile.n0 + static_cast<int>(rank) * half;
+        const bool boxes = NARROW || (!gathered && staged <= BM / 2);  // small ones, or one of BM rows
+        constexpr int BOX = NARROW ? NARROW_BOX : FEW_BOX;
+        const uint32_t bytes = (2 * (gathered || boxes ? staged : BM) + (tile.n0 + half < p.N ? channels : half)) * BK;
+        for (int kb = 0; kb < num_kb; kb += per_stage) {
           if (!mbar_wait_warp(smem_u32(&ss.empty[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
           if (elected) {
+            const int blocks = NARROW ? min(per_stage, num_kb - kb) : 1;
             const uint32_t bar = map_to_cta(smem_u32(&ss.full[stage]), 0);
-            if (leader) mbar_arrive_expect_tx(smem_u32(&ss.full[stage]), bytes);
+            if (leader) mbar_arrive_expect_tx(smem_u32(&ss.full[stage]), blocks * bytes);
             else mbar_arrive_cluster_relaxed(bar);
-            const uint32_t x_dst = smem_u32(sA + stage * A_STAGE_BYTES);
-            if (!gathered && !boxes) {
-              tma_load_2d_pair(&tmX, bar, x_dst, kb * BK, tile.row0);
-            } else if (boxes) {
-              for (int r = 0; r < staged; r += FEW_BOX) tma_load_2d_pair(&tmFew, bar, x_dst + r * BK, kb * BK, tile.row0 + r);
+            for (int i = 0; i < blocks; ++i) {
+              const uint32_t at = NARROW ? i * half * BK : 0, x_dst = smem_u32(sA + stage * A_STAGE_BYTES) + at;
+              const int col = (kb + i) * BK;
+              if (!gathered && !boxes) {
+                tma_load_2d_pair(&tmX, bar, x_dst, col, tile.row0);
+              } else if (boxes) {
+                for (int r = 0; r < staged; r += BOX) tma_load_2d_pair(&tmFew, bar, x_dst + r * BK, col, tile.row0 + r);
+              }
+              if (n < p.N) tma_load_2d_pair(&tmW, bar, smem_u32(sB + stage * B_STAGE_BYTES) + at, col, tile.e * p.N + n);
             }
-            if (n < p.N) tma_load_2d_pair(&tmW, bar, smem_u32(sB + stage * B_STAGE_BYTES), kb * BK, tile.e * p.N + n);
           }
           __syncwarp();
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
@@ -431,21 +450,28 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
         int stage = 0, acc = 0, few = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
-        Walker walk(p, ss, lane, tile_rows);
+        Walker<NARROW> walk(p, ss, lane, tile_rows, channels);
         while (ok && walk.next_alone(few)) {
-          const uint32_t idesc = make_idesc_i8(2 * BM, few != 0 ? few : BN);
+          const uint32_t idesc = make_idesc_i8(NARROW ? BM : 2 * BM, few != 0 ? few : BN);
           if (!mbar_wait(smem_u32(&ss.acc_empty[acc]), acc_phase ^ 1u, abort_flag)) { ok = false; break; }
           tc_fence_after();
-          for (int kb = 0; kb < num_kb; ++kb) {
+          for (int kb = 0; kb < num_kb; kb += per_stage) {
             if (!mbar_wait(smem_u32(&ss.full[stage]), phase, abort_flag)) { ok = false; break; }
             tc_fence_after();
             const uint64_t x_desc = make_smem_desc(smem_u32(sA + stage * A_STAGE_BYTES), 16, 1024);
             const uint64_t w_desc = make_smem_desc(smem_u32(sB + stage * B_STAGE_BYTES), 16, 1024);
-            const uint64_t a_desc = few != 0 ? w_desc : x_desc, b_desc = few != 0 ? x_desc : w_desc;
+            uint64_t a_desc = NARROW || few != 0 ? w_desc : x_desc, b_desc = NARROW || few != 0 ? x_desc : w_desc;
+            const int blocks = NARROW ? min(per_stage, num_kb - kb) : 1;
+            for (int i = 0; i < blocks; ++i) {
 #pragma unroll
-            for (int k4 = 0; k4 < BK / UMMA_K; ++k4)
-              umma_i8_pair(tmem_base + acc * BN, a_desc + ((k4 * UMMA_K) >> 4), b_desc + ((k4 * UMMA_K) >> 4), idesc,
-                         (kb > 0 || k4 > 0) ? 1u : 0u);
+              for (int k4 = 0; k4 < BK / UMMA_K; ++k4)
+                umma_i8_pair(tmem_base + acc * BN, a_desc + ((k4 * UMMA_K) >> 4), b_desc + ((k4 * UMMA_K) >> 4), idesc,
+                           (kb > 0 || i > 0 || k4 > 0) ? 1u : 0u);
+              if constexpr (NARROW) {
+                a_desc += (half * BK) >> 4;
+                b_desc += (half * BK) >> 4;
+              }
+            }
             umma_commit_pair(smem_u32(&ss.empty[stage]), 3);
             if (++stage == STAGES) { stage = 0; phase ^= 1u; }
           }
@@ -468,7 +494,7 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
       uint32_t phase = 0;
       bool ok = true;
       Tile tile;
-      Walker walk(p, ss, lane, tile_rows);
+      Walker<NARROW> walk(p, ss, lane, tile_rows, channels);
       while (ok && walk.next(rank, tile)) {
         // Every warp has a quarter of the CTA's rows, 4 at least: a stage is not full without it.  A warp that had none would wait for
         // stages by parity that the others could overtake twice, and take an old phase for the one it waits for.
@@ -516,16 +542,38 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
     uint32_t acc_phase = 0;
     bool ok = true;
     Tile tile;
-    Walker walk(p, ss, lane, tile_rows);
+    Walker<NARROW> walk(p, ss, lane, tile_rows, channels);
     while (ok && walk.next(rank, tile)) {
       const auto release = [&] {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&ss.acc_empty[acc]), 0));
       };
+      if constexpr (NARROW) {
+        // an MMA of 128 rows (64 channels of each CTA): the upper 64 lanes have the second half of the columns
+        const int at = (quad & 1) * 32, f = tile.n0 + static_cast<int>(rank) * half + at;
+        const int col = 32 * col_half, r = (quad >> 1) * (tile.few / 2) + col, rows = tile.row_end - tile.first - r;
+        const bool works = f < p.N && at < half && col < tile.few / 2 && rows > 0;
+        float ws = 0.f, bias = 0.f, xs = 0.f;
+        if (works) {
+          load_channel(p, tile.e, f, lane, ws, bias);
+          xs = load_row_scale(p, tile.first + r, rows, lane);
+        }
+        if (!mbar_wait_warp(smem_u32(&ss.acc_full[acc]), acc_phase, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        uint32_t v[32];
+        if (works) {
+          tmem_ld32(tmem_base + acc * BN + col + (static_cast<uint32_t>(quad * 32) << 16), v);
+          tmem_ld_wait();
+        }
+        release();
+        if (works) store_rows<ACT>(p, my_stage, lane, f, tile.first + r, rows, v, ws, bias, xs);
+        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+        continue;
+      }
       if (tile.few != 0) {
         // lanes are channels: a warp has 32 of them, and every other 32 rows
-        const int f = tile.n0 + static_cast<int>(rank) * BN_CTA + quad * 32, rows = tile.row_end - tile.first;
+        const int f = tile.n0 + static_cast<int>(rank) * half + quad * 32, rows = tile.row_end - tile.first;
         const bool works = f < p.N && 32 * col_half < rows;
         float ws = 0.f, bias = 0.f, xs[4] = {0.f, 0.f, 0.f, 0.f};
         if (works) {

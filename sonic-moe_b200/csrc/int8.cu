@@ -174,7 +174,8 @@ static int quantize(const void* x, long long ld, int dtype, void* q, long long q
 // Bound by latency: the first loads of the weights are on their way before x is looked at.
 constexpr int kDotRows = 8,  // of an expert, and of a call that takes this kernel
     kDotChannels = 4, kDotWarps = 8, kDotThreads = 32 * kDotWarps, kDotChunk = 4096, kDotAhead = 2;
-constexpr long long kDotWeights = 32ll << 20;  // bytes of one expert's weights up to which they are the better choice for a few rows
+constexpr long long kDotWeights = 32ll << 20;  // bytes of one expert's weights up to which they are fetched early
+constexpr int kDotWideN = 2 * 148 * kDotWarps * kDotChannels;  // channels of two blocks on each SM
 
 __device__ __forceinline__ float activate(int act, float x) {
   switch (act) {
@@ -395,14 +396,22 @@ static int launch_dot_of(const void* x, long long ld, const void* wq, long long 
   return wide ? launch_dot<TX, true>(x, ld, wq, w_ld, p, st) : launch_dot<TX, false>(x, ld, wq, w_ld, p, st);
 }
 
-// Whether a call goes by dot products, which read the weights at once and need no kernel of their own for x, but the time of another
-// row each.  Dot products / quantiser and tiles, us, for 1, 2, 4, 8 rows of bf16: 4096 x 4096 weights 8.1, 9.7, 13.8, 22.1 / 14.0 to
-// 14.7; 7168 x 2048 6.3, 7.2, 9.6, 14.3 / 12.0; 1024 x 1024 3.7, 4.5, 5.9, 9.0 / 8.3; but 14336 x 4096, four blocks to an SM, 20.1, 23.8,
-// 31.1, 45.1 / 20.5.  Rows of several experts, as a rule one each, are read along with other weights: 8 rows of 128 experts, 2048 x 4096
-// 24.6 / 28.7, of 256, 312 x 1600 10.2 / 21.5.
+// Whether a product goes by dot products, which read the weights at once but take longer with every row: 8-bit x 0.1 us and 0.12 more
+// for 1024 columns, where 3 us are there to be spent against the tiles.  1, 2, 4, 6, 8 rows / tiles, us: 1024 x 1024 3.5, 3.5, 3.7,
+// 4.2, 4.5 / 6.8; 7168 x 2048 5.5, 5.8, 6.3, 6.8, 7.7 / 9.4; 4096 x 4096 6.5, 7.0, 8.2, 9.9, 11.4 / 10.2; 2048 x 7168 8.7, 9.6, 11.0,
+// 12.9, 14.7 / 12.0; 1024 x 16384 17.4, 19.2, 22.7 / 19.5; and with more than two blocks to an SM, 14336 x 4096 16.0, 17.2, 18.8 / 18.4.
+// Rows of several experts, as a rule one each, are read along with other weights: 8 rows of 128 experts, 2048 x 4096, 24.6 us,
+// quantiser and tiles 28.7; of 256, 312 x 1600, 8.2 and 21.5.
 static bool by_dots(int rows, int N, int cols, int E) {
   if (E > 1) return rows <= kDotRows;
-  return rows <= (static_cast<long long>(N) * cols <= kDotWeights ? 4 : 1);
+  return rows == 1 || (rows <= kDotRows && (N <= kDotWideN ? rows * (cols + 1024) <= 32768 : rows <= 2));
+}
+// Whether they quantise x themselves: a launch less (about 2 us, and 4 of the host's), but every block works on all of x.  1, 2, 3, 4 rows
+// of bf16 inside, then with the quantiser: 1024 x 1024 3.7, 4.5, 5.4, 6.1, then 5 rows 5.9; 7168 x 2048 6.2, 7.2, 8.2, 9.1, then 4 rows
+// 8.4; 4096 x 4096 7.8, 9.4, 11.1, 13.2, then 3 rows 9.9, 4 rows 10.4; 2048 x 7168 10.4, 12.9, 15.5, 18.2, then 2 rows 11.3, 4 rows 13.2.
+static bool quantised_inside(int rows, int N, int cols, int E) {
+  if (E > 1) return by_dots(rows, N, cols, E);
+  return rows == 1 || (N <= kDotWideN && rows <= 4 && rows * (cols + 2048) <= 12288);
 }
 
 static int type_bytes(int dtype) { return dtype == SMOE_F32 ? 4 : dtype == SMOE_BF16 || dtype == SMOE_F16 ? 2 : 0; }
@@ -429,7 +438,7 @@ int smoe_int8_quantize_rows(const void* x, long long ld, int dtype, void* q, lon
 }
 
 size_t smoe_int8_linear_workspace_bytes(int x_dtype, int x_rows, int rows, int N, int cols, int E) {
-  if (x_rows <= 0 || rows <= 0 || N <= 0 || cols <= 0 || E <= 0 || x_dtype == SMOE_I8 || by_dots(rows, N, cols, E)) return 0;
+  if (x_rows <= 0 || rows <= 0 || N <= 0 || cols <= 0 || E <= 0 || x_dtype == SMOE_I8 || quantised_inside(rows, N, cols, E)) return 0;
   return round256(static_cast<size_t>(x_rows) * pitch(cols)) + round256(static_cast<size_t>(x_rows) * 4);
 }
 
@@ -467,9 +476,8 @@ int smoe_int8_linear(const void* x, long long ld, int x_dtype, const float* x_sc
   p.out = out; p.out_type = out_dtype; p.activation = activation;
   p.wide_out = !misaligned(out, 16) && out_cols * type_bytes(out_dtype) % 16 == 0;
   p.status = status;
-  if (by_dots(rows, N, cols, E)) {
+  if (!bytes_given && ws == 0) {
     switch (x_dtype) {
-      case SMOE_I8: return launch_dot<int8_t, true>(x, ld, wq, w_ld, p, S(stream));
       case SMOE_F32: return launch_dot_of<float>(x, ld, wq, w_ld, p, S(stream));
       case SMOE_BF16: return launch_dot_of<__nv_bfloat16>(x, ld, wq, w_ld, p, S(stream));
       default: return launch_dot_of<__half>(x, ld, wq, w_ld, p, S(stream));
@@ -483,6 +491,7 @@ int smoe_int8_linear(const void* x, long long ld, int x_dtype, const float* x_sc
     if (rc != SMOE_OK) return rc;
     xq = q; ld = pitch(cols); p.x_scale = s;
   }
+  if (by_dots(rows, N, cols, E)) return launch_dot<int8_t, true>(xq, ld, wq, w_ld, p, S(stream));
   return tensor_core_product(xq, ld, static_cast<const int8_t*>(wq), w_ld, p, S(stream));
 }
 

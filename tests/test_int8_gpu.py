@@ -291,6 +291,45 @@ def test_grouped_load_in_one_expert(built_library):
         check(y, product(q, wq[4]), xs[:, None], ws[4], None, None)
 
 
+@pytest.mark.parametrize("N,K", [(1, 16), (64, 128), (65, 400), (200, 520), (1030, 2064), (2048, 1152), (4800, 144), (9473, 256)])
+def test_every_number_of_rows(built_library, N, K):
+    """Where the kernel and its tiles change with the rows: scales of one and fp32 results, so that an exact sum has one answer."""
+    from sonicmoe.functional import int8
+
+    g = torch.Generator().manual_seed(N + K)
+    wq = torch.empty(N, (K + 15) // 16 * 16, dtype=torch.int8, device="cuda")[:, :K]
+    wq.copy_(torch.randint(-128, 128, (N, K), generator=g, dtype=torch.int8))
+    q = torch.empty(300, wq.stride(0), dtype=torch.int8, device="cuda")[:, :K]
+    q.copy_(torch.randint(-128, 128, (300, K), generator=g, dtype=torch.int8))
+    want, one = product(q, wq).float(), torch.ones(max(N, 300), device="cuda")
+    for M in (1, 2, 3, 4, 5, 6, 7, 8, 9, 31, 32, 33, 63, 64, 65, 96, 97, 127, 128, 129, 191, 192, 193, 256, 257, 300):
+        first = (300 - M) // 2
+        y = int8.int8_linear(q[first : first + M], wq, one[:N], x_scale=one[:M], out_dtype=torch.float32)
+        assert torch.equal(y, want[first : first + M]), M
+        if N % 2 == 0:
+            z = int8.int8_linear(q[first : first + M], wq, one[:N], x_scale=one[:M], activation_type="reglu", out_dtype=torch.float32)
+            assert torch.equal(z, want[first : first + M, 0::2].clamp_min(0) * want[first : first + M, 1::2]), M
+
+
+@pytest.mark.parametrize("counts", [[9, 0, 3], [1, 60, 3], [0, 0, 64], [40, 50, 30], [128, 0, 0], [1, 1, 90]])
+def test_few_sorted_rows_of_few_experts(built_library, counts):
+    """Small tiles with expert offsets: an expert's last rows next to the following one's first."""
+    from sonicmoe.functional import int8
+
+    R, E, N, K = sum(counts), len(counts), 328, 700
+    g = torch.Generator().manual_seed(R)
+    wq, ws = int8.quantize_rows(torch.randn(E, N, K, generator=g).cuda())
+    x = torch.randn(R + 7, K, generator=g).bfloat16().cuda()
+    off = torch.tensor([0, *torch.tensor(counts).cumsum(0).tolist()], dtype=torch.int32, device="cuda")
+    q, xs = int8.quantize_rows(x)
+    y = int8.int8_grouped_linear(x, wq, ws, off, out_dtype=torch.float32)
+    for e, n in enumerate(counts):
+        rows = slice(int(off[e]), int(off[e]) + n)
+        check(y[rows], product(q[rows], wq[e]), xs[rows, None], ws[e], None, None)
+    assert not y[R:].any()
+    assert torch.equal(y, int8.int8_grouped_linear(q, wq, ws, off, x_scale=xs, out_dtype=torch.float32))
+
+
 def test_many_tiles_of_every_kind(built_library):
     """Loads whose last tiles have 1 to 256 rows, many tiles to a CTA pair, long reductions, again and again: the roles of the
     tile kernel must not lose one another where a tile's rows are few."""
