@@ -168,13 +168,15 @@ static int quantize(const void* x, long long ld, int dtype, void* q, long long q
 // product by 4-way integer dot products
 // ----------------------------------------------------------------------------------------------
 // For up to 8 rows in all, where the weights are everything.  A block takes the rows of one expert (all of them: 8 at most) and 32
-// channels, a warp four of those, whose weights its lanes load 16 bytes each, straight from memory and eight loads ahead.  The
-// rows lie in shared memory, 4096 columns at a time; rows that are not 8-bit yet are quantised on the way there, by every block
-// for itself, which takes less than a launch of its own.
+// channels, a warp four of those, whose weights its lanes load 16 bytes each, straight from memory and eight loads ahead (SPLIT: two
+// or four warps take turns with the columns of four channels, and their sums meet in shared memory).  The rows lie in shared memory,
+// 4096 columns at a time; rows that are not 8-bit yet may be quantised on the way there, by every block for itself.
 // Bound by latency: the first loads of the weights are on their way before x is looked at.
 constexpr int kDotRows = 8,  // of an expert, and of a call that takes this kernel
     kDotChannels = 4, kDotWarps = 8, kDotThreads = 32 * kDotWarps, kDotChunk = 4096, kDotAhead = 2;
 constexpr long long kDotWeights = 32ll << 20;  // bytes of one expert's weights up to which they are fetched early
+constexpr int kDotMostBlocks = 2 * 148;        // two to an SM
+constexpr int kDotMinCols = 2048;              // that warps share
 constexpr int kDotWideN = 2 * 148 * kDotWarps * kDotChannels;  // channels of two blocks on each SM
 
 __device__ __forceinline__ float activate(int act, float x) {
@@ -191,23 +193,27 @@ __device__ __forceinline__ float activate(int act, float x) {
 }
 
 // TX: int8_t, or the type that x is quantised from.
-template <class TX, bool WIDE>
+template <class TX, bool WIDE, bool SPLIT>
 __global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long x_ld, const int8_t* wq, long long w_ld,
-                                                          const Params p) {
+                                                          const Params p, const int shares) {
   constexpr bool GIVEN = std::is_same<TX, int8_t>::value;
   __shared__ __align__(16) int8_t xs[kDotRows][kDotChunk];
   __shared__ uint32_t part[kDotRows][kDotWarps];
   __shared__ float row_scales[kDotRows];
   __shared__ int where[3];     // expert, first row, rows
+  __shared__ int parts[kDotWarps][kDotRows * kDotChannels];
   __shared__ uint32_t owned;   // rows that an expert has (kDotRows at most in all)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int n0 = (blockIdx.x * kDotWarps + warp) * kDotChannels;
+  const int split = SPLIT ? shares : 1;         // warps that share the columns of a channel
+  const int share = SPLIT ? warp % split : 0;
+  const int n0 = (blockIdx.x * (kDotWarps / split) + warp / split) * kDotChannels;
+  const int step = 512 * split;                 // columns that they load at a time
   release_next();
   // One expert: the weights are known.  The L2 fetches them while the previous kernel still runs; nothing is read, so nothing can be
   // stale (4096 x 4096 8.4 -> 7.9 us; but of 14336 x 4096, half of the L2, 18.4 -> 20.1).
   if (p.off == nullptr && static_cast<long long>(p.N) * p.K <= kDotWeights) {
     for (int j = 0; j < kDotChannels && n0 + j < p.N; ++j)
-      for (int c = 128 * lane; c < p.K; c += 4096) asm volatile("prefetch.global.L2 [%0];" ::"l"(wq + (n0 + j) * w_ld + c));
+      for (int c = 4096 * share + 128 * lane; c < p.K; c += 4096 * split) asm volatile("prefetch.global.L2 [%0];" ::"l"(wq + (n0 + j) * w_ld + c));
   }
   wait_for_previous();
   // The blockIdx.y-th expert that has rows, and which rows an expert has.  All experts are looked at together (8 rows of 256 experts,
@@ -250,7 +256,7 @@ __global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long
     const int8_t* w0 = wq + static_cast<long long>(e) * p.N * w_ld + static_cast<long long>(n0) * w_ld;
     // the lane's result: row lane / 4, channel lane % 4 of the warp's
     const int r_out = lane / kDotChannels, n = n0 + lane % kDotChannels;
-    const bool live = r_out < rows && n < p.N;
+    const bool live = share == 0 && r_out < rows && n < p.N;
     const float ws = live ? p.w_scale[static_cast<long long>(e) * p.N + n] : 0.f;
     const float bias = live && p.bias != nullptr ? load_typed(p.bias, p.bias_type, static_cast<long long>(e) * p.N + n) : 0.f;
     uint4 w[kDotAhead][kDotChannels];
@@ -262,7 +268,7 @@ __global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long
       }
     };
 #pragma unroll
-    for (int i = 0; i < kDotAhead; ++i) fetch(w[i], 16 * lane + 512 * i);
+    for (int i = 0; i < kDotAhead; ++i) fetch(w[i], step * i + 512 * share + 16 * lane);
     if constexpr (!GIVEN) {
       using L = Loaded<TX, WIDE>;
       for (int r = 0; r < rows; ++r) {
@@ -317,14 +323,14 @@ __global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long
         }
       }
       __syncthreads();
-      for (int c0 = 0; c0 < kn; c0 += 512 * kDotAhead) {
+      for (int c0 = 512 * share + 16 * lane; c0 - 16 * lane < kn; c0 += step * kDotAhead) {
 #pragma unroll
         for (int i = 0; i < kDotAhead; ++i) {
-          const int c = c0 + 512 * i + 16 * lane;
+          const int c = c0 + step * i;
           uint4 v[kDotChannels];
 #pragma unroll
           for (int j = 0; j < kDotChannels; ++j) v[j] = w[i][j];
-          fetch(w[i], k0 + c + 512 * kDotAhead);
+          fetch(w[i], k0 + c + step * kDotAhead);
           if (c >= kn) continue;
 #pragma unroll
           for (int r = 0; r < kDotRows; ++r) {
@@ -351,6 +357,12 @@ __global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long
         const int other = __shfl_xor_sync(0xffffffffu, upper ? acc[i] : acc[i + d], d);
         acc[i] = (upper ? acc[i + d] : acc[i]) + other;
       }
+    }
+    if constexpr (SPLIT) {
+      parts[warp][lane] = acc[0];
+      __syncthreads();
+      if (share == 0)
+        for (int i = 1; i < split; ++i) acc[0] += parts[warp + i][lane];
     }
     float y = 0.f;
     if (live) {
@@ -383,10 +395,16 @@ __global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long
 
 template <class TX, bool WIDE>
 static int launch_dot(const void* x, long long ld, const void* wq, long long w_ld, const Params& p, cudaStream_t st) {
-  constexpr int channels = kDotWarps * kDotChannels;
-  const dim3 grid((p.N + channels - 1) / channels, p.rows < p.E ? p.rows : p.E);  // experts that can have rows
-  return launched(launch_chained(dot_kernel<TX, WIDE>, grid, kDotThreads, 0, st, 1, static_cast<const TX*>(x), ld,
-                                 static_cast<const int8_t*>(wq), w_ld, p));
+  // Two or four warps share a channel's columns, and a block has fewer channels, while all blocks are on the SMs at once: each warp has
+  // eight loads on their way, and with few channels there are too few warps (1 row of bf16, 2048 x 7168 10.4 -> 7.0 us, 1024 x 16384
+  // 20.6 -> 10.4, 4096 x 4096 7.7 -> 6.8; with four blocks to an SM 9.7; 8 rows, 1024 x 1024 6.0 -> 6.4).
+  const int experts = p.rows < p.E ? p.rows : p.E;  // that can have rows
+  const auto blocks = [&](int split) { return (p.N + kDotWarps * kDotChannels / split - 1) / (kDotWarps * kDotChannels / split); };
+  int split = 1;
+  while (split < 4 && p.K >= kDotMinCols && static_cast<long long>(blocks(2 * split)) * experts <= kDotMostBlocks) split *= 2;
+  const dim3 grid(blocks(split), experts);
+  return launched(launch_chained(split > 1 ? dot_kernel<TX, WIDE, true> : dot_kernel<TX, WIDE, false>, grid, kDotThreads, 0, st, 1,
+                                 static_cast<const TX*>(x), ld, static_cast<const int8_t*>(wq), w_ld, p, split));
 }
 
 template <class TX>
@@ -396,22 +414,22 @@ static int launch_dot_of(const void* x, long long ld, const void* wq, long long 
   return wide ? launch_dot<TX, true>(x, ld, wq, w_ld, p, st) : launch_dot<TX, false>(x, ld, wq, w_ld, p, st);
 }
 
-// Whether a product goes by dot products, which read the weights at once but take longer with every row: 8-bit x 0.1 us and 0.12 more
-// for 1024 columns, where 3 us are there to be spent against the tiles.  1, 2, 4, 6, 8 rows / tiles, us: 1024 x 1024 3.5, 3.5, 3.7,
-// 4.2, 4.5 / 6.8; 7168 x 2048 5.5, 5.8, 6.3, 6.8, 7.7 / 9.4; 4096 x 4096 6.5, 7.0, 8.2, 9.9, 11.4 / 10.2; 2048 x 7168 8.7, 9.6, 11.0,
-// 12.9, 14.7 / 12.0; 1024 x 16384 17.4, 19.2, 22.7 / 19.5; and with more than two blocks to an SM, 14336 x 4096 16.0, 17.2, 18.8 / 18.4.
-// Rows of several experts, as a rule one each, are read along with other weights: 8 rows of 128 experts, 2048 x 4096, 24.6 us,
-// quantiser and tiles 28.7; of 256, 312 x 1600, 8.2 and 21.5.
+// Whether a product goes by dot products, which read the weights at once but take longer with every row.  8-bit x, 1, 2, 4, 6, 8 rows /
+// tiles, us: 1024 x 1024 3.3, 3.5, 3.7, 4.2, 4.4 / 6.8; 7168 x 2048 5.5, 5.8, 6.1, 6.8, 7.7 / 9.4; 4096 x 4096 5.9, 6.3, 7.2, 8.1, 9.0 /
+// 10.2; 2048 x 7168 6.0, 6.7, 7.9, 9.3, 10.6 / 12.0; 1024 x 16384 7.8, 9.1, 12.2, 15.0, 18.2 / 19.5; large weights, 4096 x 14336 15.2,
+// 16.0, 18.4, 20.9, 24.2 / 20.5; more than two blocks to an SM, 12000 x 2512 11.7, 12.3, 13.1, 14.1, 15.0 / 12.6.  Rows of several
+// experts, as a rule one each, are read along with other weights: 8 rows of 128 experts, 2048 x 4096, 24.6 us, quantiser and tiles
+// 28.7; of 256, 312 x 1600, 8.2 and 21.5.
 static bool by_dots(int rows, int N, int cols, int E) {
-  if (E > 1) return rows <= kDotRows;
-  return rows == 1 || (rows <= kDotRows && (N <= kDotWideN ? rows * (cols + 1024) <= 32768 : rows <= 2));
+  return rows <= (E > 1 || (N <= kDotWideN && static_cast<long long>(N) * cols <= kDotWeights) ? kDotRows : 3);
 }
 // Whether they quantise x themselves: a launch less (about 2 us, and 4 of the host's), but every block works on all of x.  1, 2, 3, 4 rows
-// of bf16 inside, then with the quantiser: 1024 x 1024 3.7, 4.5, 5.4, 6.1, then 5 rows 5.9; 7168 x 2048 6.2, 7.2, 8.2, 9.1, then 4 rows
-// 8.4; 4096 x 4096 7.8, 9.4, 11.1, 13.2, then 3 rows 9.9, 4 rows 10.4; 2048 x 7168 10.4, 12.9, 15.5, 18.2, then 2 rows 11.3, 4 rows 13.2.
+// of bf16 inside / with the quantiser: 1024 x 1024 3.7, 4.5, 5.3, 6.1 / 5.2, 5.5, 5.5, 5.6; 7168 x 2048 6.1, 7.2, 8.1, 9.1 / 7.4, 7.7, 8.2,
+// 8.4; 4096 x 4096 6.8, 8.2, 10.0, 11.4 / 8.3, 8.8, 9.3, 9.7; 2048 x 7168 7.0, 9.2, 11.4, 13.7 / 8.7, 9.2, 10.0, 10.8; 1024 x 16384 10.4,
+// 14.5 / 10.5, 11.9; 512 x 65536 39, 61 / 31, 35; 12000 x 2512 13.5, 16.6 / 13.7, 14.5.
 static bool quantised_inside(int rows, int N, int cols, int E) {
-  if (E > 1) return by_dots(rows, N, cols, E);
-  return rows == 1 || (N <= kDotWideN && rows <= 4 && rows * (cols + 2048) <= 12288);
+  const bool inside = E > 1 ? cols <= 18432 : rows <= (N <= kDotWideN ? 4 : 1) && rows * (cols + 4096) <= 22528;
+  return inside && by_dots(rows, N, cols, E);
 }
 
 static int type_bytes(int dtype) { return dtype == SMOE_F32 ? 4 : dtype == SMOE_BF16 || dtype == SMOE_F16 ? 2 : 0; }
