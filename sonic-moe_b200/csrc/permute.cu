@@ -387,7 +387,7 @@ __device__ __forceinline__ void store_weight(void* w, int dtype, long long i, fl
 }
 
 // Rows that start anywhere (on a value), by the 16-byte blocks of the row that is written: one store for each, and two loads from a
-// row that lies otherwise, shifted together.  The first and the last block go value by value.
+// row that lies otherwise, shifted together.  The first and the last block are stored value by value.
 template <class T>
 struct Window {
   static __host__ __device__ __forceinline__ int count(int bytes) { return (bytes + 16 - static_cast<int>(sizeof(T)) + 15) / 16; }
@@ -395,7 +395,7 @@ struct Window {
   static __device__ __forceinline__ int offset(int i, const char* dst) { return 16 * i - static_cast<int>(reinterpret_cast<uintptr_t>(dst) & 15); }
   static __device__ __forceinline__ Piece<16> load(const char* row, int at, int bytes) {
     Piece<16> v;
-    load16_of_row<T>(row, at, bytes, v.w);
+    load16_around_row<T>(row, at, bytes, v.w);
     return v;
   }
   static __device__ __forceinline__ void store(char* row, int at, int bytes, const Piece<16>& v) {
@@ -532,11 +532,12 @@ __global__ void __launch_bounds__(kThreads) collect_kernel(const Rows a) {
 // Four rows of the token are in flight at a time.  A row's dot product is added up piece by piece in a thread, then over the
 // lanes of each warp, then over the warps: always in the same order.
 constexpr int kDotRows = 4, kDotChunk = 32;
-// The two above by windows.  Sides measured (piece by piece / by windows, us): spread, fp32 rows of 1005 values, T 4099, K 6 33 / 23,
-// of 2049, T 8192, K 4 84 / 59, bf16 of 3001, T 16384, K 4 125 / 108, but fp16 of 1030, which have 4-byte pieces of two values, T 5003,
-// K 3 8.6 / 13.5; collect, bf16 of 3001 217 / 171, fp16 of 1030 18.8 / 15.8, but fp32 of 1005 30.3 / 33.  So a spread goes by windows
-// where a piece is one value, and a collect where a value has 16 bits.  (The gradient of the combine, with a window for each of
-// four differently placed rows and their gradients, lost a third.)
+// The two above by windows.  Sides measured (piece by piece / by windows, us): spread, fp32 rows of 1005 values, T 4099, K 6 33 / 22,
+// of 2049, T 8192, K 4 84 / 58, bf16 of 3001, T 16384, K 4 125 / 88, but fp16 of 1030, which have 4-byte pieces of two values, T 5003,
+// K 3 8.6 / 10.2; collect, in the same order 30.7 / 27.7, 87 / 71, 217 / 128, 18.8 / 11.1.  So a spread goes by windows where a piece
+// is one value, a collect where it is less than 16 bytes.  (With the values at the rows' ends loaded one by one a warp with an
+// end takes many times as long: 33, 105, 174, 15.8 for the collect.  The gradient of the combine, with a window for each of four
+// differently placed rows and their gradients, loses: 212 -> 271 us forward and backward for the rows of 2049.)
 template <class T, bool WEIGHTED>
 __global__ void __launch_bounds__(kThreads) spread_windows_kernel(const Rows a, int pad_blocks) {
   release_next();
@@ -739,10 +740,8 @@ static int launch_spread(const Rows& a, int vec, cudaStream_t st) {
 
 template <class T>
 static int launch_collect(const Rows& a, int vec, cudaStream_t st) {
-  if constexpr (sizeof(T) == 2) {
-    if (vec < 16) return launched(launch_chained(collect_windows_kernel<T>, window_blocks<T>(a), kThreads, 0, st, 1, a));
-  }
-  return for_piece<sizeof(T) == 2 ? 16 : 4>(vec, [&](auto v) {
+  if (vec < 16) return launched(launch_chained(collect_windows_kernel<T>, window_blocks<T>(a), kThreads, 0, st, 1, a));
+  return for_piece<16>(vec, [&](auto v) {
     return launched(launch_chained(collect_kernel<T, v>, flat_blocks(a, vec), kThreads, 0, st, 1, a));
   });
 }
