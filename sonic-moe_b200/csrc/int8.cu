@@ -168,12 +168,12 @@ static int quantize(const void* x, long long ld, int dtype, void* q, long long q
 // product by 4-way integer dot products
 // ----------------------------------------------------------------------------------------------
 // For up to 8 rows in all, where the weights are everything.  A block takes the rows of one expert (all of them: 8 at most) and 32
-// channels, a warp four of those, whose weights its lanes load 16 bytes each, straight from memory and eight loads ahead (SPLIT: two
+// channels, a warp four of those, whose weights its lanes load 16 bytes each, straight from memory and eight or four loads ahead (SPLIT: two
 // or four warps take turns with the columns of four channels, and their sums meet in shared memory).  The rows lie in shared memory,
 // 4096 columns at a time; rows that are not 8-bit yet may be quantised on the way there, by every block for itself.
 // Bound by latency: the first loads of the weights are on their way before x is looked at.
 constexpr int kDotRows = 8,  // of an expert, and of a call that takes this kernel
-    kDotChannels = 4, kDotWarps = 8, kDotThreads = 32 * kDotWarps, kDotChunk = 4096, kDotAhead = 2;
+    kDotChannels = 4, kDotWarps = 8, kDotThreads = 32 * kDotWarps, kDotChunk = 4096;
 constexpr long long kDotWeights = 32ll << 20;  // bytes of one expert's weights up to which they are fetched early
 constexpr int kDotMostBlocks = 2 * 148;        // two to an SM
 constexpr int kDotMinCols = 2048;              // that warps share
@@ -193,15 +193,19 @@ __device__ __forceinline__ float activate(int act, float x) {
 }
 
 // TX: int8_t, or the type that x is quantised from.
-template <class TX, bool WIDE, bool SPLIT>
-__global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long x_ld, const int8_t* wq, long long w_ld,
+// ROWS: rows at a time.  Two are for more blocks than two to an SM: with half of the registers, and one round of loads ahead, there are
+// four (14336 x 4096, one row 18.0 -> 15.2 us, 12000 x 2512 13.5 -> 10.7, 8 rows of 64 experts, 1536 x 2048, 16.4 -> 14.3; but with
+// fewer blocks 4096 x 4096 6.8 -> 7.9).  An expert that has more reads its weights again.
+template <class TX, bool WIDE, bool SPLIT, int ROWS>
+__global__ void __launch_bounds__(kDotThreads, ROWS == kDotRows ? 2 : 4) dot_kernel(const TX* x, long long x_ld, const int8_t* wq, long long w_ld,
                                                           const Params p, const int shares) {
   constexpr bool GIVEN = std::is_same<TX, int8_t>::value;
-  __shared__ __align__(16) int8_t xs[kDotRows][kDotChunk];
-  __shared__ uint32_t part[kDotRows][kDotWarps];
-  __shared__ float row_scales[kDotRows];
+  constexpr int AHEAD = ROWS == kDotRows ? 2 : 1;
+  __shared__ __align__(16) int8_t xs[ROWS][kDotChunk];
+  __shared__ uint32_t part[ROWS][kDotWarps];
+  __shared__ float row_scales[ROWS];
   __shared__ int where[3];     // expert, first row, rows
-  __shared__ int parts[kDotWarps][kDotRows * kDotChannels];
+  __shared__ int parts[kDotWarps][32];
   __shared__ uint32_t owned;   // rows that an expert has (kDotRows at most in all)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int split = SPLIT ? shares : 1;         // warps that share the columns of a channel
@@ -228,7 +232,7 @@ __global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long
     int first = 0, n = 0;
     if (e < p.E) {
       first = first_row(p, e);
-      n = min(end_row(p, e) - first, kDotRows);
+      n = end_row(p, e) - first;
     }
     const unsigned some = __ballot_sync(0xffffffffu, n > 0);
     __syncthreads();  // the words above, and those of the last round have been read
@@ -251,15 +255,17 @@ __global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long
     }
   }
   __syncthreads();
-  const int e = where[0], row0 = where[1], rows = where[2];
-  if (rows > 0) {
+  const int e = where[0], last = where[1] + where[2];
+  for (int row0 = where[1]; row0 < last; row0 += ROWS) {
+    const int rows = min(last - row0, ROWS);
     const int8_t* w0 = wq + static_cast<long long>(e) * p.N * w_ld + static_cast<long long>(n0) * w_ld;
-    // the lane's result: row lane / 4, channel lane % 4 of the warp's
-    const int r_out = lane / kDotChannels, n = n0 + lane % kDotChannels;
-    const bool live = share == 0 && r_out < rows && n < p.N;
+    // the lane's result, which COPIES neighbours have
+    constexpr int COPIES = 32 / (ROWS * kDotChannels);
+    const int r_out = lane / COPIES / kDotChannels, n = n0 + lane / COPIES % kDotChannels;
+    const bool live = share == 0 && lane % COPIES == 0 && r_out < rows && n < p.N;
     const float ws = live ? p.w_scale[static_cast<long long>(e) * p.N + n] : 0.f;
     const float bias = live && p.bias != nullptr ? load_typed(p.bias, p.bias_type, static_cast<long long>(e) * p.N + n) : 0.f;
-    uint4 w[kDotAhead][kDotChannels];
+    uint4 w[AHEAD][kDotChannels];
     const auto fetch = [&](uint4 (&v)[kDotChannels], int c) {
 #pragma unroll
       for (int j = 0; j < kDotChannels; ++j) {
@@ -268,7 +274,7 @@ __global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long
       }
     };
 #pragma unroll
-    for (int i = 0; i < kDotAhead; ++i) fetch(w[i], step * i + 512 * share + 16 * lane);
+    for (int i = 0; i < AHEAD; ++i) fetch(w[i], step * i + 512 * share + 16 * lane);
     if constexpr (!GIVEN) {
       using L = Loaded<TX, WIDE>;
       for (int r = 0; r < rows; ++r) {
@@ -285,7 +291,7 @@ __global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long
         if (lane == 0) part[r][warp] = bits;
       }
     }
-    int acc[kDotRows * kDotChannels];
+    int acc[ROWS * kDotChannels];
 #pragma unroll
     for (auto& a : acc) a = 0;
     for (int k0 = 0; k0 < p.K; k0 += kDotChunk) {
@@ -323,17 +329,17 @@ __global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long
         }
       }
       __syncthreads();
-      for (int c0 = 512 * share + 16 * lane; c0 - 16 * lane < kn; c0 += step * kDotAhead) {
+      for (int c0 = 512 * share + 16 * lane; c0 - 16 * lane < kn; c0 += step * AHEAD) {
 #pragma unroll
-        for (int i = 0; i < kDotAhead; ++i) {
+        for (int i = 0; i < AHEAD; ++i) {
           const int c = c0 + step * i;
           uint4 v[kDotChannels];
 #pragma unroll
           for (int j = 0; j < kDotChannels; ++j) v[j] = w[i][j];
-          fetch(w[i], k0 + c + step * kDotAhead);
+          fetch(w[i], k0 + c + step * AHEAD);
           if (c >= kn) continue;
 #pragma unroll
-          for (int r = 0; r < kDotRows; ++r) {
+          for (int r = 0; r < ROWS; ++r) {
             if (r >= rows) break;
             const uint4 q = *reinterpret_cast<const uint4*>(&xs[r][c]);
 #pragma unroll
@@ -348,14 +354,19 @@ __global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long
         }
       }
     }
-    // 32 sums over 32 lanes: afterwards lane l has that of row l / 4, channel l % 4
+    // the sums over the lanes: each step halves the sums that a lane has, as long as there are several
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) {
-      const bool upper = lane & d;
+      const int half = d * (ROWS * kDotChannels) / 32;
+      if (half > 0) {
+        const bool upper = lane & d;
 #pragma unroll
-      for (int i = 0; i < d; ++i) {
-        const int other = __shfl_xor_sync(0xffffffffu, upper ? acc[i] : acc[i + d], d);
-        acc[i] = (upper ? acc[i + d] : acc[i]) + other;
+        for (int i = 0; i < half; ++i) {
+          const int other = __shfl_xor_sync(0xffffffffu, upper ? acc[i] : acc[i + half], d);
+          acc[i] = (upper ? acc[i + half] : acc[i]) + other;
+        }
+      } else {
+        acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], d);
       }
     }
     if constexpr (SPLIT) {
@@ -376,13 +387,14 @@ __global__ void __launch_bounds__(kDotThreads) dot_kernel(const TX* x, long long
       y = scaled(acc[0], scale, ws);
       if (p.bias != nullptr) y += bias;
     }
-    const float up = __shfl_down_sync(0xffffffffu, y, 1);
+    const float up = __shfl_down_sync(0xffffffffu, y, COPIES);
     if (is_gated(p.activation)) {
       if (live && (n & 1) == 0)
         store_typed(p.out, p.out_type, static_cast<long long>(row0 + r_out) * (p.N / 2) + n / 2, activate(p.activation, y) * up);
     } else if (live) {
       store_typed(p.out, p.out_type, static_cast<long long>(row0 + r_out) * p.N + n, activate(p.activation, y));
     }
+    if constexpr (ROWS == kDotRows) break;  // no call has more
   }
   if (blockIdx.x == 0 && blockIdx.y == 0) {  // rows that no expert has become zeros
     const long long bytes = static_cast<long long>(is_gated(p.activation) ? p.N / 2 : p.N) * (p.out_type == SMOE_F32 ? 4 : 2);
@@ -403,8 +415,10 @@ static int launch_dot(const void* x, long long ld, const void* wq, long long w_l
   int split = 1;
   while (split < 4 && p.K >= kDotMinCols && static_cast<long long>(blocks(2 * split)) * experts <= kDotMostBlocks) split *= 2;
   const dim3 grid(blocks(split), experts);
-  return launched(launch_chained(split > 1 ? dot_kernel<TX, WIDE, true> : dot_kernel<TX, WIDE, false>, grid, kDotThreads, 0, st, 1,
-                                 static_cast<const TX*>(x), ld, static_cast<const int8_t*>(wq), w_ld, p, split));
+  const bool many = static_cast<long long>(blocks(1)) * experts > kDotMostBlocks && (p.E > 1 || p.rows <= 2);
+  const auto kernel = many ? dot_kernel<TX, WIDE, false, 2> : split > 1 ? dot_kernel<TX, WIDE, true, kDotRows> : dot_kernel<TX, WIDE, false, kDotRows>;
+  return launched(launch_chained(kernel, grid, kDotThreads, 0, st, 1, static_cast<const TX*>(x), ld, static_cast<const int8_t*>(wq), w_ld,
+                                 p, split));
 }
 
 template <class TX>
@@ -417,18 +431,19 @@ static int launch_dot_of(const void* x, long long ld, const void* wq, long long 
 // Whether a product goes by dot products, which read the weights at once but take longer with every row.  8-bit x, 1, 2, 4, 6, 8 rows /
 // tiles, us: 1024 x 1024 3.3, 3.5, 3.7, 4.2, 4.4 / 6.8; 7168 x 2048 5.5, 5.8, 6.1, 6.8, 7.7 / 9.4; 4096 x 4096 5.9, 6.3, 7.2, 8.1, 9.0 /
 // 10.2; 2048 x 7168 6.0, 6.7, 7.9, 9.3, 10.6 / 12.0; 1024 x 16384 7.8, 9.1, 12.2, 15.0, 18.2 / 19.5; large weights, 4096 x 14336 15.2,
-// 16.0, 18.4, 20.9, 24.2 / 20.5; more than two blocks to an SM, 12000 x 2512 11.7, 12.3, 13.1, 14.1, 15.0 / 12.6.  Rows of several
-// experts, as a rule one each, are read along with other weights: 8 rows of 128 experts, 2048 x 4096, 24.6 us, quantiser and tiles
-// 28.7; of 256, 312 x 1600, 8.2 and 21.5.
+// 16.0, 18.4, 20.9, 24.2 / 20.5.  With more than two blocks to an SM, bf16, 1, 2, 3 rows: 12000 x 2512 10.7, 11.0, 15.0 / 14.3; 14336 x 4096
+// 15.2, 16.0, 19.7 / 20.5.  Rows of several experts, as a rule one each, are read along with other weights: 8 rows of 128 experts,
+// 2048 x 4096, 22.6 us, quantiser and tiles 28.7; of 256, 312 x 1600, 8.2 and 21.5.
 static bool by_dots(int rows, int N, int cols, int E) {
-  return rows <= (E > 1 || (N <= kDotWideN && static_cast<long long>(N) * cols <= kDotWeights) ? kDotRows : 3);
+  if (E > 1) return rows <= kDotRows;
+  return rows <= (static_cast<long long>(N) * cols > kDotWeights ? 3 : N > kDotWideN ? 2 : kDotRows);
 }
 // Whether they quantise x themselves: a launch less (about 2 us, and 4 of the host's), but every block works on all of x.  1, 2, 3, 4 rows
 // of bf16 inside / with the quantiser: 1024 x 1024 3.7, 4.5, 5.3, 6.1 / 5.2, 5.5, 5.5, 5.6; 7168 x 2048 6.1, 7.2, 8.1, 9.1 / 7.4, 7.7, 8.2,
 // 8.4; 4096 x 4096 6.8, 8.2, 10.0, 11.4 / 8.3, 8.8, 9.3, 9.7; 2048 x 7168 7.0, 9.2, 11.4, 13.7 / 8.7, 9.2, 10.0, 10.8; 1024 x 16384 10.4,
-// 14.5 / 10.5, 11.9; 512 x 65536 39, 61 / 31, 35; 12000 x 2512 13.5, 16.6 / 13.7, 14.5.
+// 14.5 / 10.5, 11.9; 512 x 65536 39, 61 / 31, 35.
 static bool quantised_inside(int rows, int N, int cols, int E) {
-  const bool inside = E > 1 ? cols <= 18432 : rows <= (N <= kDotWideN ? 4 : 1) && rows * (cols + 4096) <= 22528;
+  const bool inside = E > 1 ? cols <= 18432 : rows <= 4 && rows * (cols + 4096) <= 22528;
   return inside && by_dots(rows, N, cols, E);
 }
 

@@ -45,7 +45,7 @@ def test_linear_refusals(built_library):
     assert size(5, 100, 100, 64, 64, 4) == 0 and size(1, 0, 100, 64, 64, 4) == 0
     assert size(1, 100, 9, 64, 65, 4) == size(1, 100, 5, 64, 65, 1) == 100 * 80 + 192 + 512
     # few rows are quantised inside the kernel
-    assert size(1, 100, 8, 64, 64, 4) == size(1, 4, 4, 64, 64, 1) == size(1, 1, 1, 14336, 4096, 1) == 0 and size(1, 2, 2, 14336, 4096, 1) > 0
+    assert size(1, 100, 8, 64, 64, 4) == size(1, 4, 4, 64, 64, 1) == size(1, 1, 1, 14336, 4096, 1) == 0 and size(1, 5, 5, 14336, 4096, 1) > 0
 
 
 def test_python_refusals(built_library):
