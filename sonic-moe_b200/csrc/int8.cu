@@ -175,6 +175,7 @@ static int quantize(const void* x, long long ld, int dtype, void* q, long long q
 constexpr int kDotRows = 8,  // of an expert, and of a call that takes this kernel
     kDotChannels = 4, kDotWarps = 8, kDotThreads = 32 * kDotWarps, kDotChunk = 4096;
 constexpr long long kDotWeights = 32ll << 20;  // bytes of one expert's weights up to which they are fetched early
+constexpr int kDotMostRows = 32;               // of several experts
 constexpr int kDotMostBlocks = 2 * 148;        // two to an SM
 constexpr int kDotMinCols = 2048;              // that warps share
 constexpr int kDotWideN = 2 * 148 * kDotWarps * kDotChannels;  // channels of two blocks on each SM
@@ -195,7 +196,8 @@ __device__ __forceinline__ float activate(int act, float x) {
 // TX: int8_t, or the type that x is quantised from.
 // ROWS: rows at a time.  Two are for more blocks than two to an SM: with half of the registers, and one round of loads ahead, there are
 // four (14336 x 4096, one row 18.0 -> 15.2 us, 12000 x 2512 13.5 -> 10.7, 8 rows of 64 experts, 1536 x 2048, 16.4 -> 14.3; but with
-// fewer blocks 4096 x 4096 6.8 -> 7.9).  An expert that has more reads its weights again.
+// fewer blocks 4096 x 4096 6.8 -> 7.9).  An expert that has more has several blocks for
+// a channel.
 template <class TX, bool WIDE, bool SPLIT, int ROWS>
 __global__ void __launch_bounds__(kDotThreads, ROWS == kDotRows ? 2 : 4) dot_kernel(const TX* x, long long x_ld, const int8_t* wq, long long w_ld,
                                                           const Params p, const int shares) {
@@ -206,7 +208,7 @@ __global__ void __launch_bounds__(kDotThreads, ROWS == kDotRows ? 2 : 4) dot_ker
   __shared__ float row_scales[ROWS];
   __shared__ int where[3];     // expert, first row, rows
   __shared__ int parts[kDotWarps][32];
-  __shared__ uint32_t owned;   // rows that an expert has (kDotRows at most in all)
+  __shared__ uint32_t owned;   // rows that an expert has (kDotMostRows at most in all)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int split = SPLIT ? shares : 1;         // warps that share the columns of a channel
   const int share = SPLIT ? warp % split : 0;
@@ -220,25 +222,34 @@ __global__ void __launch_bounds__(kDotThreads, ROWS == kDotRows ? 2 : 4) dot_ker
       for (int c = 4096 * share + 128 * lane; c < p.K; c += 4096 * split) asm volatile("prefetch.global.L2 [%0];" ::"l"(wq + (n0 + j) * w_ld + c));
   }
   wait_for_previous();
-  // The blockIdx.y-th expert that has rows, and which rows an expert has.  All experts are looked at together (8 rows of 256 experts,
+  // The rows of the blockIdx.y-th unit, and which rows an expert has.  All experts are looked at together (8 rows of 256 experts,
   // 312 x 1600, 10.2 -> 8.2 us); block (0, 0) then clears the rows that no expert has.
+  const bool dense = p.off == nullptr;
   if (threadIdx.x == 0) {
-    where[2] = 0;
-    owned = 0u;
+    where[0] = 0;
+    where[1] = blockIdx.y * ROWS;
+    where[2] = dense ? min(p.rows - static_cast<int>(blockIdx.y) * ROWS, ROWS) : 0;
+    owned = dense ? 0xFFFFFFFFu : 0u;
   }
-  int before = 0;  // experts with rows so far
-  for (int e0 = 0; e0 < p.E; e0 += kDotThreads) {
+  int before = 0;  // units, experts' rows ROWS at a time, so far
+  for (int e0 = 0; e0 < p.E && !dense; e0 += kDotThreads) {
     const int e = e0 + threadIdx.x;
     int first = 0, n = 0;
     if (e < p.E) {
       first = first_row(p, e);
       n = end_row(p, e) - first;
     }
-    const unsigned some = __ballot_sync(0xffffffffu, n > 0);
+    const int units = (max(n, 0) + ROWS - 1) / ROWS;
+    int at = units;  // up to this expert, later before it
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, at, d);
+      if (lane >= d) at += o;
+    }
     __syncthreads();  // the words above, and those of the last round have been read
-    if (lane == 0) part[0][warp] = __popc(some);
+    if (lane == 31) part[0][warp] = at;
     __syncthreads();
-    int at = before + __popc(some & ((1u << lane) - 1u));
+    at += before - units;
 #pragma unroll
     for (int w = 0; w < kDotWarps; ++w) {
       const int c = part[0][w];
@@ -246,18 +257,18 @@ __global__ void __launch_bounds__(kDotThreads, ROWS == kDotRows ? 2 : 4) dot_ker
       before += c;
     }
     if (n > 0) {
-      atomicOr(&owned, ((1u << n) - 1u) << first);
-      if (at == static_cast<int>(blockIdx.y)) {
+      atomicOr(&owned, (0xFFFFFFFFu >> (32 - n)) << first);
+      const int mine = static_cast<int>(blockIdx.y) - at;
+      if (mine >= 0 && mine < units) {
         where[0] = e;
-        where[1] = first;
-        where[2] = n;
+        where[1] = first + mine * ROWS;
+        where[2] = min(n - mine * ROWS, ROWS);
       }
     }
   }
   __syncthreads();
-  const int e = where[0], last = where[1] + where[2];
-  for (int row0 = where[1]; row0 < last; row0 += ROWS) {
-    const int rows = min(last - row0, ROWS);
+  const int e = where[0], row0 = where[1], rows = where[2];
+  if (rows > 0) {
     const int8_t* w0 = wq + static_cast<long long>(e) * p.N * w_ld + static_cast<long long>(n0) * w_ld;
     // the lane's result, which COPIES neighbours have
     constexpr int COPIES = 32 / (ROWS * kDotChannels);
@@ -394,7 +405,6 @@ __global__ void __launch_bounds__(kDotThreads, ROWS == kDotRows ? 2 : 4) dot_ker
     } else if (live) {
       store_typed(p.out, p.out_type, static_cast<long long>(row0 + r_out) * p.N + n, activate(p.activation, y));
     }
-    if constexpr (ROWS == kDotRows) break;  // no call has more
   }
   if (blockIdx.x == 0 && blockIdx.y == 0) {  // rows that no expert has become zeros
     const long long bytes = static_cast<long long>(is_gated(p.activation) ? p.N / 2 : p.N) * (p.out_type == SMOE_F32 ? 4 : 2);
@@ -414,8 +424,8 @@ static int launch_dot(const void* x, long long ld, const void* wq, long long w_l
   const auto blocks = [&](int split) { return (p.N + kDotWarps * kDotChannels / split - 1) / (kDotWarps * kDotChannels / split); };
   int split = 1;
   while (split < 4 && p.K >= kDotMinCols && static_cast<long long>(blocks(2 * split)) * experts <= kDotMostBlocks) split *= 2;
-  const dim3 grid(blocks(split), experts);
-  const bool many = static_cast<long long>(blocks(1)) * experts > kDotMostBlocks && (p.E > 1 || p.rows <= 2);
+  const bool many = p.rows > kDotRows || (static_cast<long long>(blocks(1)) * experts > kDotMostBlocks && (p.E > 1 || p.rows <= 2));
+  const dim3 grid(blocks(many ? 1 : split), many ? (p.rows + experts) / 2 : experts);  // as many units as there may be
   const auto kernel = many ? dot_kernel<TX, WIDE, false, 2> : split > 1 ? dot_kernel<TX, WIDE, true, kDotRows> : dot_kernel<TX, WIDE, false, kDotRows>;
   return launched(launch_chained(kernel, grid, kDotThreads, 0, st, 1, static_cast<const TX*>(x), ld, static_cast<const int8_t*>(wq), w_ld,
                                  p, split));
@@ -433,9 +443,11 @@ static int launch_dot_of(const void* x, long long ld, const void* wq, long long 
 // 10.2; 2048 x 7168 6.0, 6.7, 7.9, 9.3, 10.6 / 12.0; 1024 x 16384 7.8, 9.1, 12.2, 15.0, 18.2 / 19.5; large weights, 4096 x 14336 15.2,
 // 16.0, 18.4, 20.9, 24.2 / 20.5.  With more than two blocks to an SM, bf16, 1, 2, 3 rows: 12000 x 2512 10.7, 11.0, 15.0 / 14.3; 14336 x 4096
 // 15.2, 16.0, 19.7 / 20.5.  Rows of several experts, as a rule one each, are read along with other weights: 8 rows of 128 experts,
-// 2048 x 4096, 22.6 us, quantiser and tiles 28.7; of 256, 312 x 1600, 8.2 and 21.5.
+// 2048 x 4096, 22.6 us, quantiser and tiles 28.7; of 256, 312 x 1600, 8.2 and 21.5; 16, 24, 32 rows of 128 experts, 2048 x 4096, 32.8, 45.1,
+// 55.3 and 43.0, 55.3, 67.6; of 32, 512 x 1024, 6.4, 6.9, 8.7 and 10.2, 10.8, 11.0; all 32
+// in one expert 28.7 and 20.5, 7.7 and 9.2.
 static bool by_dots(int rows, int N, int cols, int E) {
-  if (E > 1) return rows <= kDotRows;
+  if (E > 1) return rows <= kDotRows || (rows <= kDotMostRows && rows <= 2 * E);
   return rows <= (static_cast<long long>(N) * cols > kDotWeights ? 3 : N > kDotWideN ? 2 : kDotRows);
 }
 // Whether they quantise x themselves: a launch less (about 2 us, and 4 of the host's), but every block works on all of x.  1, 2, 3, 4 rows

@@ -330,6 +330,36 @@ def test_few_sorted_rows_of_few_experts(built_library, counts):
     assert torch.equal(y, int8.int8_grouped_linear(q, wq, ws, off, x_scale=xs, out_dtype=torch.float32))
 
 
+@pytest.mark.parametrize("rows,E,N", [(32, 16, 200), (32, 128, 72), (31, 300, 64), (9, 5, 640), (8, 64, 1536), (17, 16, 30)])
+@pytest.mark.parametrize("spread", [1, 3, 100])
+def test_few_rows_of_many_experts(built_library, rows, E, N, spread):
+    """Rows shared out in small units: every row in one expert, in three, in as many as there are, and rows that none has between."""
+    from sonicmoe.functional import int8
+
+    g = torch.Generator().manual_seed(rows + E + spread)
+    K = 320
+    wq, ws = int8.quantize_rows(torch.randn(E, N, K, generator=g).cuda())
+    chosen = torch.randperm(E, generator=g)[:spread]
+    owner = chosen[torch.randint(0, len(chosen), (rows,), generator=g)].sort().values
+    count = torch.bincount(owner, minlength=E)
+    gap = (torch.rand(E, generator=g) < 0.02).int()  # a row that no expert has behind some of them
+    off = torch.cat([torch.zeros(1, dtype=torch.long), (count + gap).cumsum(0)])
+    R = int(off[-1])
+    x = torch.randn(5, K, generator=g).bfloat16().cuda()
+    take = torch.randint(-1, 5, (R,), generator=g, dtype=torch.int32).cuda()
+    bias = torch.randn(E, N, generator=g).cuda()
+    out = int8.int8_grouped_linear(x, wq, ws, off.int().cuda(), take, count.int().cuda(), bias=bias, out_dtype=torch.float32)
+    q, xs = int8.quantize_rows(x)
+    for e in range(E):
+        r = torch.arange(int(off[e]), int(off[e] + count[e]), device="cuda")
+        if len(r):
+            src, none = take[r].long().clamp_min(0), take[r] < 0
+            acc = product(q[src], wq[e])
+            acc[none] = 0
+            check(out[r], acc, xs[src, None], ws[e], bias[e], None)
+        assert not out[int(off[e] + count[e]) : int(off[e + 1])].any()
+
+
 def test_many_tiles_of_every_kind(built_library):
     """Loads whose last tiles have 1 to 256 rows, many tiles to a CTA pair, long reductions, again and again: the roles of the
     tile kernel must not lose one another where a tile's rows are few."""
