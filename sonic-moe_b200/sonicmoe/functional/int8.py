@@ -12,7 +12,8 @@ scale = amax / 127 of the row (1 for a row of zeros), values = 127 x / amax roun
 in 32-bit integers and rounded once, so results do not depend on how the work is shared out.  Rows that hold an infinity or a NaN
 give NaN.  8-bit rows start on 16-byte boundaries: `quantize_rows` lays them out so, whatever their width.
 
-There is no gradient: arguments that require one are refused where gradients are recorded.  The FP8 experts (`functional.fp8`)
+There is no gradient: arguments that require one are refused where gradients are recorded, and those with a forward-mode
+tangent everywhere.  The FP8 experts (`functional.fp8`)
 are the path for training.  The reference has no 8-bit path.
 """
 
@@ -22,6 +23,7 @@ from dataclasses import dataclass
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from .. import _lib
 from .._lib import check, lib, ptr, stream_ptr
@@ -39,10 +41,11 @@ def _refuse_gradients(*tensors) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
-                break
-        else:
-            return
-        raise NotImplementedError("the 8-bit products have no gradient: call them under torch.no_grad()")
+                raise NotImplementedError("the 8-bit products have no gradient: call them under torch.no_grad()")
+    if forward_ad._current_level >= 0:  # (torch.no_grad() does not stop these)
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("the 8-bit products have no forward-mode derivative")
 
 
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

@@ -22,6 +22,7 @@ from __future__ import annotations
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from .._lib import check, lib, ptr, stream_ptr
@@ -122,6 +123,14 @@ def _refuse_second_derivative():
         raise NotImplementedError("sorted tokens have first derivatives only")
 
 
+def _recorded(*tensors) -> bool:
+    """Whether a call has to go by its autograd function: gradients are recorded, or forward-mode derivatives may be on their way,
+    which the functions refuse (the kernels alone would lose them)."""
+    if forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 # Both keep the index vectors themselves: the fields of a permutation may be replaced before the backward pass.
 class _Permute(torch.autograd.Function):
     @staticmethod
@@ -167,7 +176,7 @@ def permute_tokens(x: torch.Tensor, permutation: TokenPermutation) -> torch.Tens
     if x.dim() != 2 or x.shape[0] != permutation.s_reverse_scatter_idx.shape[0]:
         raise ValueError(f"x has to be ({permutation.s_reverse_scatter_idx.shape[0]}, H), got {tuple(x.shape)}")
     pair, row = permutation.s_reverse_scatter_idx, permutation.s_scatter_idx
-    if torch.is_grad_enabled() and x.requires_grad:
+    if _recorded(x):
         return _Permute.apply(x, pair, row)
     return _spread(x, pair, row, None)
 
@@ -187,6 +196,6 @@ def unpermute_tokens(rows: torch.Tensor, permutation: TokenPermutation, scores: 
         if scores.dtype not in _ROW_TYPES:
             raise TypeError(f"scores has to be fp32, bf16 or fp16, got {scores.dtype}")
         scores = scores.contiguous()
-    if torch.is_grad_enabled() and (rows.requires_grad or (scores is not None and scores.requires_grad)):
+    if _recorded(rows, scores):
         return _Unpermute.apply(rows, pair, permutation.s_scatter_idx, scores)
     return _collect(rows, pair, scores)

@@ -91,3 +91,27 @@ def test_layer_refusals(built_library):
         int8.quantize_experts(torch.zeros(4, 16, 8), None, torch.zeros(16, 2, 8), torch.zeros(8, 16))
     with pytest.raises(ValueError, match="inconsistent shapes"):
         int8.quantize_experts(torch.zeros(4, 16, 8), None, torch.zeros(12, 2, 8), None)
+
+
+def test_forward_mode_derivatives_are_refused(built_library):
+    """A dual tensor does not require a gradient, and torch.no_grad() leaves its tangent alone."""
+    from torch.autograd import forward_ad
+
+    from sonicmoe.functional import int8
+
+    x, w = torch.zeros(4, 32), torch.zeros(8, 32, dtype=torch.int8)
+    s, xs, bias = torch.ones(8), torch.ones(4), torch.zeros(8)
+    experts = int8.Int8Experts(torch.zeros(8, 4, 16, dtype=torch.int8), torch.ones(8, 4), None,
+                               torch.zeros(8, 16, 2, dtype=torch.int8), torch.ones(8, 16), None)
+    t, router = torch.zeros(3, 16, dtype=torch.bfloat16), torch.zeros(8, 16, dtype=torch.bfloat16)
+    with forward_ad.dual_level(), torch.no_grad():
+        dual = lambda v: forward_ad.make_dual(v, torch.ones_like(v))
+        off = torch.zeros(2, dtype=torch.int32)
+        for call in (lambda: int8.int8_linear(dual(x), w, s), lambda: int8.int8_linear(x, w, dual(s)),
+                     lambda: int8.int8_linear(x.to(torch.int8), w, s, x_scale=dual(xs)),
+                     lambda: int8.int8_linear(x, w, s, bias=dual(bias)),
+                     lambda: int8.int8_grouped_linear(dual(x), w[None], s[None], off),
+                     lambda: int8.moe_int8_softmax_topk_layer(dual(t), router, experts, 2),
+                     lambda: int8.moe_int8_softmax_topk_layer(t, dual(router), experts, 2)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()

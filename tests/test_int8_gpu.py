@@ -504,3 +504,16 @@ def test_layer(built_library, T, H, I, E, K, activation, biased):
                                      True)[0] if H % 64 == 0 and I % 64 == 0 and n1 % 128 == 0 else None
     if bf16 is not None:  # 8-bit operands: 0.8 % rms each, three of them and the activation's slope
         assert ((o.double() - bf16.double()).norm() / bf16.double().norm()).item() < 0.06
+
+
+def test_quantising_a_dual_tensor_is_refused(built_library):
+    from torch.autograd import forward_ad
+
+    from sonicmoe.functional import int8
+
+    w = torch.randn(2, 6, 16, device="cuda")
+    with forward_ad.dual_level():
+        for call in (int8.quantize_rows, lambda v: int8.quantize_experts(v.permute(1, 2, 0), None, v.permute(2, 1, 0), None)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(forward_ad.make_dual(w, torch.ones_like(w)))
+        assert int8.quantize_rows(w)[0].shape == w.shape

@@ -320,3 +320,24 @@ def test_row_numbers_out_of_range_count_as_none(built_library):
     ok = (broken >= 0) & (broken < p.num_rows)
     want = torch.where(ok.unsqueeze(2), y[torch.where(ok, broken, 0).long()], torch.zeros(1, 1, 1, device="cuda")).sum(1)
     assert torch.allclose(sonicmoe.unpermute_tokens(y, q), want, rtol=0, atol=2.0 ** -20)
+
+
+def test_forward_mode_derivatives_are_refused(built_library):
+    """A dual tensor does not require a gradient: its tangent must not be lost without a word, under torch.no_grad() either."""
+    from torch.autograd import forward_ad
+
+    import sonicmoe
+
+    T, K, E, H = 20, 2, 3, 16
+    p = sonicmoe.token_permutation(indices(T, K, E).cuda(), E)
+    x, y, s = source(T, H, torch.float32, 1), source(T * K, H, torch.float32, 2), torch.rand(T, K, device="cuda")
+    plain = sonicmoe.permute_tokens(x, p), sonicmoe.unpermute_tokens(y, p, s)
+    for enabled in (True, False):
+        with forward_ad.dual_level(), torch.set_grad_enabled(enabled):
+            dual = lambda v: forward_ad.make_dual(v, torch.ones_like(v))
+            for call in (lambda: sonicmoe.permute_tokens(dual(x), p), lambda: sonicmoe.unpermute_tokens(dual(y), p),
+                         lambda: sonicmoe.unpermute_tokens(dual(y), p, s), lambda: sonicmoe.unpermute_tokens(y, p, dual(s))):
+                with pytest.raises(NotImplementedError, match="jvp"):
+                    call()
+            again = sonicmoe.permute_tokens(x, p), sonicmoe.unpermute_tokens(y, p, s)
+            assert all(torch.equal(a, b) and not b.requires_grad for a, b in zip(plain, again))
