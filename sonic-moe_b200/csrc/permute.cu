@@ -6,7 +6,8 @@
 //                 and with it dw[t, k] = <dout[t], rows[row(t, k)]>
 //   collect       out[t] = sum over k of w[t, k] rows[row(t, k)]; also the gradient of the sort by x (w = 1)
 //
-// A pair whose expert is not in [0, E) is dropped: it has no row (-1), adds nothing and its weight is not read.  Everything here
+// A pair whose expert is not in [0, E) is dropped: it has no row (-1), adds nothing and its weight is not read.  So is one whose
+// row number is taken out of `row` later on: a row has a pair where `slot` and `row` name one another.  Everything here
 // is bound by memory.  The row movers go token by token, not row by row: a token's row is read once for its K places (expert
 // by expert the whole of x would be read up to K times), and the sum over k stays in registers, in fp32, in the order of k.
 #include <cuda_bf16.h>
@@ -423,14 +424,20 @@ struct Rows {
   void* dweight;          // (T, K), the type of weight
   int weight_type;
   const int* row;         // (T, K) sorted row of every pair, or -1
-  const int* slot;        // (R) pair of every row, or -1
+  const int* slot;        // (R) pair of every row, or none (outside of [0, T K))
   int T, K, R, bytes;     // bytes: of one row of H values
 };
 
 constexpr int kThreads = 256;
 constexpr int kPadRows = 64;  // rows that a block looks through for ones without a pair, eight a warp at a time
 
-// The last blocks of a spread: zeros for the rows without a pair.
+// Whether no pair writes row r: none is named, or the one that is has no row or another (a pair dropped after the sort, in `row` alone).
+__device__ __forceinline__ bool is_empty(const Rows& a, int r) {
+  const int p = a.slot[r];
+  return static_cast<unsigned>(p) >= static_cast<unsigned>(a.T * a.K) || a.row[p] != r;
+}
+
+// The first blocks of a spread: zeros for the rows without a pair.
 template <int VEC>
 __device__ __forceinline__ void zero_rows(const Rows& a, int block) {
   const int lane = threadIdx.x & 31;
@@ -439,7 +446,7 @@ __device__ __forceinline__ void zero_rows(const Rows& a, int block) {
   for (auto& w : zero.w) w = 0u;
   for (int i = 8 * (threadIdx.x >> 5); i < kPadRows; i += 8 * (blockDim.x >> 5)) {
     const long long first = static_cast<long long>(block) * kPadRows + i;
-    const bool empty = lane < 8 && first + lane < a.R && a.slot[first + lane] < 0;
+    const bool empty = lane < 8 && first + lane < a.R && is_empty(a, static_cast<int>(first) + lane);
     unsigned todo = __ballot_sync(0xffffffffu, empty);
     for (; todo != 0u; todo &= todo - 1u) {
       char* dst = a.out + (first + __ffs(todo) - 1) * a.bytes;

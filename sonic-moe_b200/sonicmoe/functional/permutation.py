@@ -8,8 +8,9 @@ products), which take their rows expert by expert.
 
 Both directions have gradients (the sums over a token's rows, the rows' dot products for the scores).  A pair whose expert is
 outside [0, E) (-1, say: a token beyond an expert's capacity, a padding token) is dropped: it has no row, adds nothing, and its
-score is not read.  ``align`` starts every expert's rows at a multiple of it; rows without a pair are zeros in `permute_tokens`,
-ignored by `unpermute_tokens` whatever they hold, and get zero gradients.
+score is not read.  A pair may also be dropped after the sort, by -1 in ``s_reverse_scatter_idx``.  ``align`` starts every
+expert's rows at a multiple of it; rows without a pair are zeros in `permute_tokens`, ignored by `unpermute_tokens` whatever they
+hold, and get zero gradients.
 
 fp32, bf16 and fp16 rows of any width; sums in fp32 in the order of k, rounded once: the same bits every time.  The number of
 rows follows from the shapes alone, so nothing here waits for the device and all of it can be captured in a graph.  (For a captured

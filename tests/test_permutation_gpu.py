@@ -341,3 +341,45 @@ def test_forward_mode_derivatives_are_refused(built_library):
                     call()
             again = sonicmoe.permute_tokens(x, p), sonicmoe.unpermute_tokens(y, p, s)
             assert all(torch.equal(a, b) and not b.requires_grad for a, b in zip(plain, again))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,pitch,offset", LAYOUTS)
+def test_pairs_dropped_after_the_sort(built_library, dtype, H, pitch, offset):
+    """A pair taken out of s_reverse_scatter_idx alone (a capacity applied later): its row is zeros, in the gradients too, whatever
+    the memory held before.  Every number here is a value of the inputs or a product of two: one rounding each."""
+    import sonicmoe
+
+    T, K, E, align = 37, 3, 6, 8
+    p = sonicmoe.token_permutation(indices(T, K, E, 0.1).cuda(), E, align)
+    kept = p.s_reverse_scatter_idx.clone()
+    g = torch.Generator().manual_seed(9)
+    lost = (torch.rand(T, K, generator=g) < 0.4).cuda()
+    kept[lost] = torch.where(torch.rand(T, K, generator=g) < 0.5, -1, p.num_rows).int().cuda()[lost]
+    q = sonicmoe.TokenPermutation(p.expert_frequency, p.expert_frequency_offset, p.x_gather_idx, p.s_scatter_idx, kept, align)
+    has_row = (kept >= 0) & (kept < p.num_rows)
+    rows = kept[has_row].long()
+    token = torch.arange(T, device="cuda").unsqueeze(1).expand(T, K)[has_row]
+    x, y, dout = source(T, H, dtype, 1, pitch, offset), source(p.num_rows, H, dtype, 2, pitch, offset), source(T, H, dtype, 3, pitch, offset)
+    s = torch.rand(T, K, generator=g).cuda()
+
+    def poisoned(call):
+        junk = torch.full((p.num_rows, H), float("nan"), dtype=dtype, device="cuda")  # the block that the rows get
+        del junk
+        return call()
+
+    def expected(values, weights=None):
+        want = torch.zeros(p.num_rows, H, dtype=torch.float64, device="cuda")
+        want[rows] = values.double()[token] * (1 if weights is None else weights.double()[has_row].unsqueeze(1))
+        return want
+
+    assert torch.equal(poisoned(lambda: sonicmoe.permute_tokens(x, q)).double(), expected(x))
+    for scores, leaves in ((None, 1), (s, 1), (s, 2)):  # by the rows, by the rows with constant scores, by both
+        rows_in = y.detach().requires_grad_(True)
+        weights = None if scores is None else scores.clone().requires_grad_(leaves == 2)
+        out = sonicmoe.unpermute_tokens(rows_in, q, weights)
+        grads = poisoned(lambda: torch.autograd.grad(out, (rows_in, weights)[:leaves], dout))
+        want = expected(dout, scores)
+        assert bool(((grads[0].double() - want).abs() <= half_step(dtype, want) + 2.0 ** -24 * want.abs()).all())
+        if leaves == 2:
+            assert not grads[1][~has_row].any()
