@@ -127,14 +127,15 @@ __device__ __forceinline__ void place_pairs(const Plan& a, int first, int steps,
   }
 }
 
-// Rows behind an expert's pairs (warp by warp) and behind the last expert hold no pair.
+// Rows behind an expert's pairs (warp by warp) and behind the last expert hold no pair.  Unsigned row numbers: a step behind the last
+// row may pass 2^31.
 __device__ __forceinline__ void mark_rest(const Plan& a, const int* offset, int block, int blocks) {
-  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const unsigned lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   if (a.align > 1) {
     for (int e = block * warps + (threadIdx.x >> 5); e < a.E; e += blocks * warps)
-      for (int r = offset[e] + a.count[e] + lane; r < offset[e + 1]; r += 32) a.slot[r] = a.token[r] = -1;
+      for (unsigned r = offset[e] + a.count[e] + lane, end = offset[e + 1]; r < end; r += 32) a.slot[r] = a.token[r] = -1;
   }
-  for (int r = offset[a.E] + block * blockDim.x + threadIdx.x; r < a.rows; r += blocks * blockDim.x)
+  for (unsigned r = offset[a.E] + block * blockDim.x + threadIdx.x, end = a.rows; r < end; r += blocks * blockDim.x)
     a.slot[r] = a.token[r] = -1;
 }
 

@@ -383,3 +383,25 @@ def test_pairs_dropped_after_the_sort(built_library, dtype, H, pitch, offset):
         assert bool(((grads[0].double() - want).abs() <= half_step(dtype, want) + 2.0 ** -24 * want.abs()).all())
         if leaves == 2:
             assert not grads[1][~has_row].any()
+
+
+def test_the_largest_permutation(built_library):
+    """As many pairs as there may be, and row numbers within a block's step of 2^31: rows behind the last pair are marked, and
+    nothing else is written."""
+    import sonicmoe
+
+    n, E, align = 2 ** 31 - 2 ** 16 - 1, 512, 64
+    if torch.cuda.mem_get_info()[0] < 6 * 4 * n:
+        pytest.skip("needs 52 GB")
+    for expert in (3, -1):
+        p = sonicmoe.token_permutation(torch.full((n, 1), expert, dtype=torch.int32, device="cuda"), E, align)
+        kept = n if expert >= 0 else 0
+        assert p.num_rows > 2 ** 31 - 2 ** 15 - 1024 and int(p.expert_frequency.sum()) == kept
+        assert p.expert_frequency_offset.tolist() == [0] * 4 + [-(-kept // align) * align] * (E - 3)
+        for got in (p.s_scatter_idx, p.x_gather_idx):
+            assert bool((got[kept:] == -1).all())
+        count = torch.arange(n, dtype=torch.int32, device="cuda")
+        for got in (p.s_scatter_idx[:kept], p.x_gather_idx[:kept], p.s_reverse_scatter_idx[:kept, 0]):
+            assert torch.equal(got, count[:kept])
+        assert bool((p.s_reverse_scatter_idx[kept:] == -1).all())
+        del p, got, count
