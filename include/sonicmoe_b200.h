@@ -449,6 +449,8 @@ int smoe_token_permutation(const void* expert_idx, int idx_dtype, int T, int K, 
  * one row of the input to the next (0: the same row for all); outputs are packed.  weights (T,K): SMOE_F32, SMOE_BF16, SMOE_F16
  * or NULL = 1.  Where s_reverse_scatter_idx names a row, s_scatter_idx names that pair, as the sort leaves them.  A pair may be
  * dropped afterwards by a row index outside [0,R) (-1, say) in s_reverse_scatter_idx alone.
+ * Sizes whose blocks (one per token in unpermute_rows_backward, 256 threads for 16 bytes of a row or more elsewhere, and one per
+ * 64 rows) are more than 2^31 - 1 are refused.
  *   permute_rows:            rows[s_reverse_scatter_idx[t,k]] = weights[t,k] * x[t]; zeros in rows of no pair, or a dropped one
  *   unpermute_rows:          out[t] = sum over k of weights[t,k] * rows[s_reverse_scatter_idx[t,k]], in the order of k
  *   unpermute_rows_backward: drows as permute_rows of dout, dweights[t,k] = <dout[t], rows[s_reverse_scatter_idx[t,k]]> (0 for

@@ -720,49 +720,48 @@ static int for_piece(int vec, F&& f) {
   return SMOE_ERR_ALIGNMENT;
 }
 
-static unsigned pad_blocks(int R) { return static_cast<unsigned>((static_cast<long long>(R) + kPadRows - 1) / kPadRows); }
+static long long pad_blocks(int R) { return (static_cast<long long>(R) + kPadRows - 1) / kPadRows; }
 
-static unsigned flat_blocks(const Rows& a, int vec) {
+static long long flat_blocks(const Rows& a, int vec) {
   const int u = pieces_per_thread(vec);
   const long long stride = (a.bytes / vec + u - 1) / u;
-  return static_cast<unsigned>((a.T * stride + kThreads - 1) / kThreads);
+  return (a.T * stride + kThreads - 1) / kThreads;
 }
 
 template <class T>
-static unsigned window_blocks(const Rows& a) {
-  return static_cast<unsigned>((static_cast<long long>(a.T) * Window<T>::count(a.bytes) + kThreads - 1) / kThreads);
+static long long window_blocks(const Rows& a) {
+  return (static_cast<long long>(a.T) * Window<T>::count(a.bytes) + kThreads - 1) / kThreads;
+}
+
+template <class Kernel, class... Args>
+static int launch_blocks(Kernel kernel, long long blocks, unsigned threads, cudaStream_t st, Args... args) {
+  if (blocks > 0x7fffffffll) return SMOE_ERR_SHAPE;  // of a grid; less by far than the rows that memory holds, but rows may be broadcast
+  return launched(launch_chained(kernel, static_cast<unsigned>(blocks), threads, 0, st, 1, args...));
 }
 
 template <class T, bool WEIGHTED>
 static int launch_spread(const Rows& a, int vec, cudaStream_t st) {
-  if (vec == static_cast<int>(sizeof(T))) {
-    const unsigned pad = pad_blocks(a.R);
-    return launched(launch_chained(spread_windows_kernel<T, WEIGHTED>, pad + window_blocks<T>(a), kThreads, 0, st, 1, a, static_cast<int>(pad)));
-  }
-  return for_piece<sizeof(T) == 2 ? 4 : 16>(vec, [&](auto v) {
-    const unsigned pad = pad_blocks(a.R), blocks = pad + flat_blocks(a, vec);
-    return launched(launch_chained(spread_kernel<T, v, WEIGHTED>, blocks, kThreads, 0, st, 1, a,
-                                   static_cast<int>(pad)));
-  });
+  const long long pad = pad_blocks(a.R);
+  if (vec == static_cast<int>(sizeof(T)))
+    return launch_blocks(spread_windows_kernel<T, WEIGHTED>, pad + window_blocks<T>(a), kThreads, st, a, static_cast<int>(pad));
+  return for_piece<sizeof(T) == 2 ? 4 : 16>(
+      vec, [&](auto v) { return launch_blocks(spread_kernel<T, v, WEIGHTED>, pad + flat_blocks(a, vec), kThreads, st, a, static_cast<int>(pad)); });
 }
 
 template <class T>
 static int launch_collect(const Rows& a, int vec, cudaStream_t st) {
-  if (vec < 16) return launched(launch_chained(collect_windows_kernel<T>, window_blocks<T>(a), kThreads, 0, st, 1, a));
-  return for_piece<16>(vec, [&](auto v) {
-    return launched(launch_chained(collect_kernel<T, v>, flat_blocks(a, vec), kThreads, 0, st, 1, a));
-  });
+  if (vec < 16) return launch_blocks(collect_windows_kernel<T>, window_blocks<T>(a), kThreads, st, a);
+  return for_piece<16>(vec, [&](auto v) { return launch_blocks(collect_kernel<T, v>, flat_blocks(a, vec), kThreads, st, a); });
 }
 
 template <class T>
 static int launch_spread_dot(const Rows& a, int vec, cudaStream_t st) {
   return for_piece<static_cast<int>(sizeof(T))>(vec, [&](auto v) {
-    const unsigned pad = pad_blocks(a.R);
+    const long long pad = pad_blocks(a.R);
     // as few rounds over the row as 256 threads allow, and no more threads than those rounds need
     const int u = pieces_per_thread(vec), pieces = (a.bytes / vec + u - 1) / u, rounds = (pieces + kThreads - 1) / kThreads;
     const unsigned threads = static_cast<unsigned>(((pieces + rounds - 1) / rounds + 31) / 32 * 32);
-    return launched(launch_chained(spread_dot_kernel<T, v>, pad + a.T, threads, 0, st, 1, a,
-                                   static_cast<int>(pad)));
+    return launch_blocks(spread_dot_kernel<T, v>, pad + a.T, threads, st, a, static_cast<int>(pad));
   });
 }
 

@@ -80,3 +80,18 @@ def test_python_refusals(built_library):
         sonicmoe.permute_tokens(torch.zeros(4, 16), p)
     with pytest.raises(SonicMoEError, match="no CPU path"):
         sonicmoe.unpermute_tokens(torch.zeros(8, 16), p)
+
+
+def test_grids_past_the_limit_are_refused(built_library):
+    """Broadcast rows (ld 0) and rows of one value allow for more blocks than a grid has, although all of it fits into memory."""
+    from sonicmoe._lib import lib
+
+    at, T, H = 4096, 2 ** 31 - 1, 2 ** 20
+    # 2^31 rows of 2^18 pieces of 16 bytes are 2^41 blocks: zero in 32 bits
+    assert lib.smoe_permute_rows(at, 0, at, 0, None, 0, at, at, T, 1, H, 64, None) == -1
+    assert lib.smoe_permute_rows(at + 4, 0, at, 0, None, 0, at, at, T, 1, H + 1, 64, None) == -1
+    assert lib.smoe_unpermute_rows(at, 0, at, 0, None, 0, at, T, 1, H, 64, None) == -1
+    assert lib.smoe_unpermute_rows(at + 2, 0, at, 1, None, 0, at, T, 1, H + 1, 64, None) == -1
+    # a block per token and one per 64 rows
+    n = 2 ** 31 - 2 ** 16 - 1
+    assert lib.smoe_unpermute_rows_backward(at, 1, at, 1, at, 1, at, at, 0, at, at, n, 1, 1, n, None) == -1
