@@ -73,7 +73,8 @@ def token_permutation(topk_indices: torch.Tensor, E: int, align: int = 1) -> Tok
         check(lib.smoe_token_permutation(
             idx.data_ptr(), _lib.dtype_code(idx.dtype), T, K, E, align, freq.data_ptr(), off.data_ptr(), gather.data_ptr(),
             scatter.data_ptr(), reverse.data_ptr(), ptr(ws), stream_ptr(dev)), "token_permutation")
-    return TokenPermutation(freq, off, gather, scatter, reverse.view(T, K), align)
+    # tensors in their own right: as views of one buffer they would share the count of in-place changes that autograd looks at
+    return TokenPermutation(freq.data, off.data, gather.data, scatter.data, reverse.view(T, K).data, align)
 
 
 def _check_permutation(p: TokenPermutation, dev: torch.device) -> None:

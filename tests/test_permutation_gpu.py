@@ -405,3 +405,32 @@ def test_the_largest_permutation(built_library):
             assert torch.equal(got, count[:kept])
         assert bool((p.s_reverse_scatter_idx[kept:] == -1).all())
         del p, got, count
+
+
+def test_fields_changed_in_place_before_the_backward_pass(built_library):
+    """The counts and the other index vectors are the caller's to change; a change of those that the gradient takes is noticed."""
+    import sonicmoe
+
+    T, K, E, H = 30, 2, 4, 16
+    x, drows = source(T, H, torch.float32, 1).requires_grad_(True), source(T * K, H, torch.float32, 2)
+    s = torch.rand(T, K, device="cuda", requires_grad=True)
+    dout = source(T, H, torch.float32, 3)
+    for inference in (False, True):
+        with torch.inference_mode(inference):
+            p = sonicmoe.token_permutation(indices(T, K, E).cuda(), E)
+        if inference:  # still what it was
+            assert all(t.is_inference() for t in (p.expert_frequency, p.s_reverse_scatter_idx))
+            continue
+        want = torch.autograd.grad(sonicmoe.permute_tokens(x, p), x, drows)[0]
+        rows = sonicmoe.permute_tokens(x, p)
+        out = sonicmoe.unpermute_tokens(rows.detach(), p, s)
+        first = p.expert_frequency_offset.clone()
+        p.expert_frequency.add_(7)
+        p.expert_frequency_offset.zero_()
+        p.x_gather_idx.fill_(-1)
+        assert torch.equal(torch.autograd.grad(rows, x, drows)[0], want) and bool(first.any())
+        torch.autograd.grad(out, s, dout)
+        rows = sonicmoe.permute_tokens(x, p)
+        p.s_reverse_scatter_idx.copy_(p.s_reverse_scatter_idx.flip(0))
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(rows, x, drows)
