@@ -12,6 +12,8 @@ score is not read.  A pair may also be dropped after the sort, by -1 in ``s_reve
 expert's rows at a multiple of it; rows without a pair are zeros in `permute_tokens`, ignored by `unpermute_tokens` whatever they
 hold, and get zero gradients.
 
+The gradients have gradients of their own, any number of times, where there are no scores; with scores that is refused.
+
 fp32, bf16 and fp16 rows of any width; sums in fp32 in the order of k, rounded once: the same bits every time.  The number of
 rows follows from the shapes alone, so nothing here waits for the device and all of it can be captured in a graph.  (For a captured
 backward pass autograd itself asks that no graph recorded outside the capture still holds the same leaves.)
@@ -119,10 +121,16 @@ def _collect(rows, pair, scores):
     return out
 
 
-def _refuse_second_derivative():
-    # (the decorator for it costs more than the launch)
-    if torch.is_grad_enabled():
-        raise NotImplementedError("sorted tokens have first derivatives only")
+class _FirstDerivative(torch.autograd.Function):
+    """A gradient as it is; its own derivative, by what it was computed from, is refused where one is asked for."""
+
+    @staticmethod
+    def forward(ctx, grad, *of):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise NotImplementedError("unpermute_tokens has first derivatives only where there are scores")
 
 
 def _recorded(*tensors) -> bool:
@@ -133,17 +141,18 @@ def _recorded(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
-# Both keep the index vectors themselves: the fields of a permutation may be replaced before the backward pass.
+# Both keep the index vectors themselves: the fields of a permutation may be replaced before the backward pass.  Gradients are recorded
+# there where the caller wants to differentiate them again: without scores each function's gradient is the other one.
 class _Permute(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, pair, row):
-        ctx.save_for_backward(pair)
+        ctx.save_for_backward(pair, row)
         return _spread(x, pair, row, None)
 
     @staticmethod
     def backward(ctx, drows):
-        _refuse_second_derivative()
-        return _collect(drows, *ctx.saved_tensors, None), None, None
+        pair, row = ctx.saved_tensors
+        return _Unpermute.apply(drows, pair, row, None) if torch.is_grad_enabled() else _collect(drows, pair, None), None, None
 
 
 class _Unpermute(torch.autograd.Function):
@@ -154,19 +163,24 @@ class _Unpermute(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout):
-        _refuse_second_derivative()
         pair, row, scores, rows = ctx.saved_tensors
+        again = torch.is_grad_enabled()
+        if scores is None:
+            return _Permute.apply(dout, pair, row) if again else _spread(dout, pair, row, None), None, None, None
         if rows is None:
-            return _spread(dout, pair, row, scores), None, None, None
-        dout, rows = _rows(dout, "dout"), _rows(rows, "rows")
-        (T, K), (R, H), dev = pair.shape, rows.shape, rows.device
+            drows = _spread(dout, pair, row, scores)
+            return _FirstDerivative.apply(drows, dout, scores) if again else drows, None, None, None
+        g, y = _rows(dout, "dout"), _rows(rows, "rows")
+        (T, K), (R, H), dev = pair.shape, y.shape, y.device
         with _lib.on_device(dev):
-            drows = rows.new_empty((R, H))
+            drows = y.new_empty((R, H))
             dscores = torch.empty_like(scores)
             check(lib.smoe_unpermute_rows_backward(
-                dout.data_ptr(), dout.stride(0), rows.data_ptr(), rows.stride(0), drows.data_ptr(), _ROW_TYPES[rows.dtype],
+                g.data_ptr(), g.stride(0), y.data_ptr(), y.stride(0), drows.data_ptr(), _ROW_TYPES[y.dtype],
                 scores.data_ptr(), dscores.data_ptr(), _ROW_TYPES[scores.dtype], pair.data_ptr(), row.data_ptr(), T, K, H, R,
                 stream_ptr(dev)), "unpermute_rows_backward")
+        if again:
+            drows, dscores = _FirstDerivative.apply(drows, dout, scores), _FirstDerivative.apply(dscores, dout, rows)
         return drows, None, None, dscores
 
 

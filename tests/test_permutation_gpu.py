@@ -434,3 +434,43 @@ def test_fields_changed_in_place_before_the_backward_pass(built_library):
         p.s_reverse_scatter_idx.copy_(p.s_reverse_scatter_idx.flip(0))
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             torch.autograd.grad(rows, x, drows)
+
+
+def test_gradients_of_gradients(built_library):
+    """create_graph alone asks for nothing; without scores every order follows, with scores the second one is refused."""
+    import sonicmoe
+
+    T, K, E, H = 30, 3, 4, 16
+    p = sonicmoe.token_permutation(indices(T, K, E, 0.2).cuda(), E, 4)
+    token = p.x_gather_idx.long()
+    live = token >= 0
+    x, y = source(T, H, torch.float32, 1).requires_grad_(True), source(p.num_rows, H, torch.float32, 2).requires_grad_(True)
+    s = torch.rand(T, K, device="cuda", requires_grad=True)
+
+    def penalty(leaf, call):  # |d sum(out^3) / d leaf|^2 and its gradient
+        first, = torch.autograd.grad(call(leaf).pow(3).sum(), leaf, create_graph=True)
+        return torch.autograd.grad(first.pow(2).sum(), leaf)[0]
+
+    def plain_permute(v):
+        return torch.where(live.unsqueeze(1), v[token.clamp_min(0)], 0.0)
+
+    def plain_unpermute(v):
+        return torch.zeros(T, H, dtype=v.dtype, device="cuda").index_add(0, token[live], v[live])
+
+    for leaf, own, plain in ((x, sonicmoe.permute_tokens, plain_permute), (y, sonicmoe.unpermute_tokens, plain_unpermute)):
+        got, want = penalty(leaf, lambda v: own(v, p)), penalty(leaf.detach().double().requires_grad_(True), plain)
+        # powers and sums of K values of up to 5: a few roundings of each, relative to the largest
+        assert bool(((got.double() - want).abs() <= 64 * 2.0 ** -24 * want.abs().max()).all())
+
+    dout = source(T, H, torch.float32, 3)
+    for leaves in ((y, s), (y,)):
+        out = sonicmoe.unpermute_tokens(y, p, s if len(leaves) == 2 else s.detach())
+        want = torch.autograd.grad(out, leaves, dout, retain_graph=True)
+        first = torch.autograd.grad(out, leaves, dout, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(first, want))
+    out = sonicmoe.unpermute_tokens(y, p, s)
+    d = dout.clone().requires_grad_(True)
+    for i, by in ((0, s), (1, y), (0, d), (1, d)):  # the score is in the rows' gradient, the rows in the score's
+        first = torch.autograd.grad(out, (y, s), d, create_graph=True)
+        with pytest.raises(NotImplementedError, match="first derivatives only"):
+            torch.autograd.grad(first[i].sum(), by)
