@@ -141,8 +141,13 @@ def _recorded(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _again() -> bool:
+    return torch.is_grad_enabled() or forward_ad._current_level >= 0
+
+
 # Both keep the index vectors themselves: the fields of a permutation may be replaced before the backward pass.  Gradients are recorded
-# there where the caller wants to differentiate them again: without scores each function's gradient is the other one.
+# there where the caller wants to differentiate them again: without scores each function's gradient is the other one.  An upstream
+# gradient with a forward-mode tangent goes the same way, and is refused.
 class _Permute(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, pair, row):
@@ -152,7 +157,7 @@ class _Permute(torch.autograd.Function):
     @staticmethod
     def backward(ctx, drows):
         pair, row = ctx.saved_tensors
-        return _Unpermute.apply(drows, pair, row, None) if torch.is_grad_enabled() else _collect(drows, pair, None), None, None
+        return _Unpermute.apply(drows, pair, row, None) if _again() else _collect(drows, pair, None), None, None
 
 
 class _Unpermute(torch.autograd.Function):
@@ -164,7 +169,7 @@ class _Unpermute(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         pair, row, scores, rows = ctx.saved_tensors
-        again = torch.is_grad_enabled()
+        again = _again()
         if scores is None:
             return _Permute.apply(dout, pair, row) if again else _spread(dout, pair, row, None), None, None, None
         if rows is None:

@@ -474,3 +474,23 @@ def test_gradients_of_gradients(built_library):
         first = torch.autograd.grad(out, (y, s), d, create_graph=True)
         with pytest.raises(NotImplementedError, match="first derivatives only"):
             torch.autograd.grad(first[i].sum(), by)
+
+
+def test_forward_mode_tangents_of_upstream_gradients_are_refused(built_library):
+    from torch.autograd import forward_ad
+
+    import sonicmoe
+
+    T, K, E, H = 20, 2, 3, 16
+    p = sonicmoe.token_permutation(indices(T, K, E).cuda(), E)
+    x, y = source(T, H, torch.float32, 1).requires_grad_(True), source(T * K, H, torch.float32, 2).requires_grad_(True)
+    s = torch.rand(T, K, device="cuda", requires_grad=True)
+    for call, leaves in ((lambda: sonicmoe.permute_tokens(x, p), x), (lambda: sonicmoe.unpermute_tokens(y, p), y),
+                         (lambda: sonicmoe.unpermute_tokens(y, p, s), (y, s)), (lambda: sonicmoe.unpermute_tokens(y, p, s.detach()), y)):
+        out = call()
+        g = torch.ones_like(out)
+        want = torch.autograd.grad(out, leaves, g, retain_graph=True)
+        with forward_ad.dual_level():
+            assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, g, retain_graph=True), want))
+            with pytest.raises(NotImplementedError, match="jvp"):
+                torch.autograd.grad(out, leaves, forward_ad.make_dual(g, torch.ones_like(g)))
