@@ -145,7 +145,7 @@ __device__ __forceinline__ void store_rows(const Params& p, uint32_t stage, int 
   for (int j = 0; j < 16; ++j) {
     float a = scaled(static_cast<int>(v[2 * j]), __shfl_sync(0xffffffffu, xs, 2 * j), ws);
     float b = scaled(static_cast<int>(v[2 * j + 1]), __shfl_sync(0xffffffffu, xs, 2 * j + 1), ws);
-    if (p.bias != nullptr) { a += bias; b += bias; }
+    if (p.bias != nullptr) { a = biased(a, bias); b = biased(b, bias); }
     if constexpr (!gated) { a = activate<ACT>(a); b = activate<ACT>(b); }
     const float other = __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
     lo[j] = odd ? other : a;
@@ -297,7 +297,7 @@ __device__ __forceinline__ void store_columns(const Params& p, uint32_t stage, i
   }
   if (p.bias != nullptr) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) f[j] += __shfl_sync(0xffffffffu, bias, j);
+    for (int j = 0; j < 32; ++j) f[j] = biased(f[j], __shfl_sync(0xffffffffu, bias, j));
   }
   constexpr bool gated = is_gated(ACT);
   const long long cols = gated ? p.N / 2 : p.N;

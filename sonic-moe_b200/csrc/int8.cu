@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(kDotThreads, ROWS == kDotRows ? 2 : 4) dot_ker
         scale = row_scales[r_out];
       }
       y = scaled(acc[0], scale, ws);
-      if (p.bias != nullptr) y += bias;
+      if (p.bias != nullptr) y = biased(y, bias);
     }
     const float up = __shfl_down_sync(0xffffffffu, y, COPIES);
     if (is_gated(p.activation)) {

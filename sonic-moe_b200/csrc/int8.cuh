@@ -67,7 +67,10 @@ __device__ __forceinline__ uint32_t pack_typed(int dtype, float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-__device__ __forceinline__ float scaled(int acc, float xs, float ws) { return __int2float_rn(acc) * xs * ws; }
+// (sum x_scale) w_scale, and + bias, each step rounded by itself: a compiler that fused the last two in one kernel and not in another
+// would give other bits.
+__device__ __forceinline__ float scaled(int acc, float xs, float ws) { return __fmul_rn(__fmul_rn(__int2float_rn(acc), xs), ws); }
+__device__ __forceinline__ float biased(float y, float bias) { return __fadd_rn(y, bias); }
 
 // The activations' values by their definitions.  x sigmoid(x) = x / (1 + exp(-x)) with the fast exponential and division: 2^-21
 // of the value, where the hardware tanh that the bf16 epilogues use is off by 2.5e-4 of x, too much of a small result.

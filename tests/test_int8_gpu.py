@@ -517,3 +517,40 @@ def test_quantising_a_dual_tensor_is_refused(built_library):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call(forward_ad.make_dual(w, torch.ones_like(w)))
         assert int8.quantize_rows(w)[0].shape == w.shape
+
+
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+@pytest.mark.parametrize("N,K", [(200, 520), (1030, 144), (9602, 256)])
+def test_the_same_bits_from_every_kernel(built_library, activation, N, K):
+    """A row's result does not depend on the rows beside it, on x being quantised before, on the way there or inside, or on an expert's
+    other rows: dot products of eight and of two rows, tiles of every kind, with scales and biases of any value."""
+    from sonicmoe.functional import int8
+
+    g = torch.Generator().manual_seed(N + K)
+    R = 600
+    x = torch.randn(R, K, generator=g).bfloat16().cuda()
+    wq, ws = int8.quantize_rows((torch.randn(N, K, generator=g) * torch.rand(N, 1, generator=g)).cuda())
+    bias = torch.randn(N, generator=g).cuda()
+    q, xs = int8.quantize_rows(x)
+    for b in (bias, None):
+        call = dict(bias=b, activation_type=activation, out_dtype=torch.float32)
+        want = int8.int8_linear(q, wq, ws, x_scale=xs, **call)
+        for M in (1, 2, 3, 4, 8, 9, 31, 33, 64, 65, 100, 128, 129, 200, 224, 225, 300, 512):
+            for first in (0, R - M):
+                rows = slice(first, first + M)
+                assert torch.equal(int8.int8_linear(q[rows], wq, ws, x_scale=xs[rows], **call), want[rows]), M
+                assert torch.equal(int8.int8_linear(x[rows], wq, ws, **call), want[rows]), M
+        many = wq.unsqueeze(0).expand(6, N, K).contiguous() if K % 16 == 0 else int8_copies(wq, 6)
+        scales, biases = ws.expand(6, N).contiguous(), None if b is None else b.expand(6, N).contiguous()
+        for off in ([0, 0, 3, 5, 9, 20, 31], [0, 5, 45, 190, 420, 599, 600], [0, 0, 0, 600, 600, 600, 600]):
+            take = torch.arange(R, dtype=torch.int32, device="cuda")[: off[-1]]
+            y = int8.int8_grouped_linear(q, many, scales, torch.tensor(off, dtype=torch.int32, device="cuda"), take, x_scale=xs,
+                                         bias=biases, activation_type=activation, out_dtype=torch.float32)
+            assert torch.equal(y, want[: off[-1]]), off
+
+
+def int8_copies(wq, n):
+    """n experts with the same 8-bit rows, laid out as quantize_rows does."""
+    N, K = wq.shape
+    out = torch.zeros(n, N, (K + 15) // 16 * 16, dtype=torch.int8, device=wq.device)[..., :K]
+    return out.copy_(wq)
