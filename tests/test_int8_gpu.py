@@ -554,3 +554,61 @@ def int8_copies(wq, n):
     N, K = wq.shape
     out = torch.zeros(n, N, (K + 15) // 16 * 16, dtype=torch.int8, device=wq.device)[..., :K]
     return out.copy_(wq)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(1, 40, 8192), (1, 33, 18001), (1, 24, 18432), (2, 72, 4097), (2, 40, 7168), (3, 40, 3400), (1, 200, 4112)])
+def test_few_long_rows_quantised_on_the_way(built_library, dtype, M, N, K):
+    """More columns than the kernel has in shared memory at a time: the same bits as from rows quantised before."""
+    from sonicmoe.functional import int8
+
+    g = torch.Generator().manual_seed(K)
+    x = (torch.randn(M, K, generator=g) * torch.rand(M, 1, generator=g)).to(dtype).cuda()
+    x[0, -1] = 9  # the largest value is one of the last
+    wq, ws = int8.quantize_rows(torch.randn(N, K, generator=g).cuda())
+    bias = torch.randn(N, generator=g).cuda()
+    q, xs = int8.quantize_rows(x)
+    y = int8.int8_linear(x, wq, ws, bias=bias, out_dtype=torch.float32)
+    assert torch.equal(y, int8.int8_linear(q, wq, ws, x_scale=xs, bias=bias, out_dtype=torch.float32))
+    check(y, product(q, wq), xs[:, None], ws, bias, None)
+    shifted = torch.zeros(M, K + 3, dtype=dtype, device="cuda")[:, 1 : K + 1].copy_(x)  # rows that start anywhere
+    assert torch.equal(int8.int8_linear(shifted, wq, ws, bias=bias, out_dtype=torch.float32), y)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,E,N,K", [(8, 5, 64, 9001), (24, 13, 40, 9001), (16, 40, 32, 18432), (5, 3, 32, 18433)])
+def test_few_long_rows_of_experts(built_library, dtype, rows, E, N, K):
+    from sonicmoe.functional import int8
+
+    g = torch.Generator().manual_seed(rows)
+    wq, ws = int8.quantize_rows(torch.randn(E, N, K, generator=g).cuda())
+    x = torch.randn(7, K, generator=g).to(dtype).cuda()
+    take = torch.randint(-1, 7, (rows,), generator=g, dtype=torch.int32).cuda()
+    first = torch.randint(0, rows + 1, (E - 1,), generator=g).sort().values.tolist()
+    off = torch.tensor([0, *first, rows], dtype=torch.int32, device="cuda")
+    q, xs = int8.quantize_rows(x)
+    y = int8.int8_grouped_linear(x, wq, ws, off, take, out_dtype=torch.float32)
+    assert torch.equal(y, int8.int8_grouped_linear(q, wq, ws, off, take, x_scale=xs, out_dtype=torch.float32))
+    for e in range(E):
+        r = torch.arange(int(off[e]), int(off[e + 1]), device="cuda")
+        if len(r):
+            src, none = take[r].long().clamp_min(0), take[r] < 0
+            acc = product(q[src], wq[e])
+            acc[none] = 0
+            check(y[r], acc, xs[src, None], ws[e], None, None)
+
+
+@pytest.mark.parametrize("N,K", [(8448, 4096), (4096, 8200)])
+def test_few_rows_of_large_weights(built_library, N, K):
+    """Above 32 MB of weights the kernels change at other numbers of rows."""
+    from sonicmoe.functional import int8
+
+    g = torch.Generator().manual_seed(N)
+    wq, ws = int8.quantize_rows(torch.randn(N, K, generator=g).cuda())
+    x = torch.randn(9, K, generator=g).bfloat16().cuda()
+    q, xs = int8.quantize_rows(x)
+    want = int8.int8_linear(q, wq, ws, x_scale=xs, out_dtype=torch.float32)
+    check(want, product(q, wq), xs[:, None], ws, None, None)
+    for M in range(1, 9):
+        assert torch.equal(int8.int8_linear(x[:M], wq, ws, out_dtype=torch.float32), want[:M]), M
+        assert torch.equal(int8.int8_linear(q[:M], wq, ws, x_scale=xs[:M], out_dtype=torch.float32), want[:M]), M

@@ -494,3 +494,41 @@ def test_forward_mode_tangents_of_upstream_gradients_are_refused(built_library):
             assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, g, retain_graph=True), want))
             with pytest.raises(NotImplementedError, match="jvp"):
                 torch.autograd.grad(out, leaves, forward_ad.make_dual(g, torch.ones_like(g)))
+
+
+@pytest.mark.parametrize("T,K,E,align,dropped", [
+    (2048, 1, 1024, 1, 0.0), (2047, 1, 1023, 3, 0.0), (1025, 1, 7, 1, 0.0), (256, 8, 128, 1, 0.2), (1024, 2, 8, 128, 0.0),
+    (2048, 1, 1025, 1, 0.0), (2049, 1, 1024, 1, 0.1), (683, 3, 1000, 2, 1.0)])
+def test_permutation_by_one_block_and_next_to_it(built_library, T, K, E, align, dropped):
+    """Up to 2048 pairs of 1024 experts one block sorts, 32 pairs of a warp or up to 64 in turn; one pair or expert more is another form."""
+    import sonicmoe
+
+    for dtype in (torch.int32, torch.int64):
+        idx = indices(T, K, E, dropped, dtype)
+        check_permutation(sonicmoe.token_permutation(idx.cuda(), E, align), idx, E, align)
+    idx = torch.full((T, K), E - 1, dtype=torch.int32)
+    check_permutation(sonicmoe.token_permutation(idx.cuda(), E, align), idx, E, align)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,pitch,offset", LAYOUTS)
+@pytest.mark.parametrize("score_type", TYPES)
+def test_gradients_of_one_argument(built_library, dtype, H, pitch, offset, score_type):
+    """By the rows where the scores are constant, a product with one rounding, and by the scores where the rows are."""
+    import sonicmoe
+
+    T, K, E, align = 21, 3, 6, 4
+    p = sonicmoe.token_permutation(indices(T, K, E, 0.25).cuda(), E, align)
+    slot, token = p.s_scatter_idx.long(), p.x_gather_idx.long()
+    live = slot >= 0
+    g = torch.Generator().manual_seed(11)
+    y, dout = source(p.num_rows, H, dtype, 3, pitch, offset), source(T, H, dtype, 5, pitch, offset)
+    scores = torch.rand(T, K, generator=g).to(score_type).cuda()
+    rows = y.detach().requires_grad_(True)
+    got, = torch.autograd.grad(sonicmoe.unpermute_tokens(rows, p, scores), rows, dout)
+    want = torch.where(live.unsqueeze(1), dout.double()[token.clamp_min(0)] * scores.double().reshape(-1)[slot.clamp_min(0)].unsqueeze(1), 0.0)
+    assert got.dtype == dtype and bool(((got.double() - want).abs() <= half_step(dtype, want) + 2.0 ** -24 * want.abs()).all())
+    leaf = scores.detach().requires_grad_(True)
+    got, = torch.autograd.grad(sonicmoe.unpermute_tokens(y, p, leaf), leaf, dout)
+    both, = torch.autograd.grad(sonicmoe.unpermute_tokens(rows, p, leaf), leaf, dout)
+    assert torch.equal(got, both) and got.dtype == score_type
