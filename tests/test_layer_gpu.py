@@ -632,3 +632,48 @@ def test_backward_pass_under_autocast(built_library, K, dtype):
     for p, c in zip(plain, cast):
         assert p.dtype == c.dtype == torch.bfloat16
         assert (p.double() - c.double()).norm() <= 2.0 ** -6 * p.double().norm()
+
+
+@pytest.mark.parametrize("seed", [204, 1544, 1884, 2156])
+def test_relu_gradient_beside_its_kink(built_library, seed):
+    """Draws in which one pre-activation is a few 1e-8, less than the rounding of its 256 products' sum (2^-24 of their magnitudes is
+    4e-7): on which side of zero it comes out is up to the order of the sum, and either derivative is right.  The other one
+    moves its token's dx by |dy score| |w1 row|, up to 0.0068 of all of dx here and more than the bound of 0.01 once in some 10^4
+    draws; that much is allowed for, in those tokens, and nothing else."""
+    import sonicmoe
+    from sonicmoe import _lib
+    from sonicmoe.enums import ActivationType
+    from sonicmoe.functional import layer_router_logits
+
+    T, H, I, E, K = 700, 256, 128, 8, 2
+    g = torch.Generator().manual_seed(seed)
+    weights = [(torch.randn(shape, generator=g) * 0.05).bfloat16() for shape in ((E, H), (E, I, H), (E, H, I))]
+    x, dout = (torch.randn(T, H, generator=g).bfloat16() for _ in range(2))
+    m = sonicmoe.MoE(E, K, H, I, ActivationType.RELU, False, 0.05).cuda().to(torch.bfloat16)
+    with torch.no_grad():
+        for p, w in zip((m.router.weight, m.c_fc.weight, m.c_proj.weight), weights):
+            p.copy_(w)
+    leaf = x.cuda().requires_grad_(True)
+    o, _ = m(leaf)
+    dx, = torch.autograd.grad(o, leaf, dout.cuda())
+    logits = layer_router_logits(leaf.detach(), m.router.weight.detach(), K).float().cpu()
+    _lib.check_status()
+    scores, idx = orc.topk_softmax(logits, K)
+    rw, w1, w2 = (w.double() for w in weights)
+    xd, d = x.double(), dout.double()
+    want_o, want, ds, jump = torch.zeros(T, H).double(), torch.zeros(T, H).double(), torch.zeros(T, K).double(), torch.zeros(T).double()
+    for e in range(E):
+        t, k = torch.nonzero(idx == e, as_tuple=True)
+        s = scores[t, k].double().unsqueeze(1)
+        z, dy = xd[t] @ w1[e].t(), d[t] @ w2[e]
+        y = z.clamp_min(0) @ w2[e].t()
+        want_o.index_add_(0, t, y * s)
+        ds[t, k] = (d[t] * y).sum(1)
+        want.index_add_(0, t, (dy * (z > 0) * s) @ w1[e])
+        either = z.abs() <= H * 2.0 ** -24 * (xd[t].abs() @ w1[e].abs().t())
+        jump.index_add_(0, t, ((dy * s).abs() * either) @ w1[e].norm(dim=1))
+    want += orc.softmax_topk_backward(scores, idx, ds.float(), E).double() @ rw
+    assert rel(o, want_o) < TOL
+    off = ((dx.double().cpu() - want).norm(dim=1) - jump).clamp_min(0)
+    assert (off.norm() / want.norm()).item() < TOL
+    assert 0 < int((jump > 0).sum()) < T // 4
