@@ -21,6 +21,18 @@ inline int current_device() {
   return dev;
 }
 
+// Tensor maps are made by a driver call, which needs the device's primary context current on the calling thread, and a thread that
+// has made no runtime call yet (an autograd worker) has none.  Setting the device that is current anyway binds it, and is allowed
+// while a stream is captured; a cudaFree(nullptr) there ends the capture with an error.
+inline bool bind_context() {
+  static thread_local bool bound = false;
+  if (!bound) {
+    const int dev = current_device();
+    bound = dev >= 0 && cudaSetDevice(dev) == cudaSuccess;
+  }
+  return bound;
+}
+
 // One flag per device: "this kernel's launch attributes have been set on that device".  Two threads racing on
 // the first call both set the attribute, which is harmless.
 struct PerDeviceFlag {

@@ -35,12 +35,7 @@ static EncodeTiledFn get_encode_fn() {
 static int encode_u8(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows,
                      uint32_t box_cols) {
   EncodeTiledFn fn = get_encode_fn();
-  if (fn == nullptr) return SMOE_ERR_DRIVER;
-  static thread_local bool context_bound = false;
-  if (!context_bound) {
-    if (cudaFree(nullptr) != cudaSuccess) return SMOE_ERR_DRIVER;
-    context_bound = true;
-  }
+  if (fn == nullptr || !bind_context()) return SMOE_ERR_DRIVER;
   if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || cols % 16 != 0) return SMOE_ERR_ALIGNMENT;
   const cuuint64_t dims[2] = {cols, rows};
   const cuuint64_t strides[1] = {cols};

@@ -30,12 +30,7 @@ static EncodeTiledFn get_encode_fn() {
 // Rows of `cols` bytes, `pitch` bytes apart; boxes of box_rows x 128 bytes, 128-byte swizzle, zeros outside.
 static int encode_rows(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t box_rows) {
   const EncodeTiledFn fn = get_encode_fn();
-  if (fn == nullptr) return SMOE_ERR_DRIVER;
-  static thread_local bool context_bound = false;  // a thread without any runtime call so far has no current context
-  if (!context_bound) {
-    if (cudaFree(nullptr) != cudaSuccess) return SMOE_ERR_DRIVER;
-    context_bound = true;
-  }
+  if (fn == nullptr || !bind_context()) return SMOE_ERR_DRIVER;
   const cuuint64_t dims[2] = {cols, rows};
   const cuuint64_t strides[1] = {pitch};
   const cuuint32_t box[2] = {BK, box_rows};

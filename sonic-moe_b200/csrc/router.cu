@@ -731,12 +731,7 @@ static EncodeTiledFn encode_fn() {
 
 static int encode_rows(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
   EncodeTiledFn fn = encode_fn();
-  if (fn == nullptr) return SMOE_ERR_DRIVER;
-  static thread_local bool context_bound = false;
-  if (!context_bound) {
-    if (cudaFree(nullptr) != cudaSuccess) return SMOE_ERR_DRIVER;
-    context_bound = true;
-  }
+  if (fn == nullptr || !bind_context()) return SMOE_ERR_DRIVER;
   if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0) return SMOE_ERR_ALIGNMENT;
   const cuuint64_t dims[2] = {cols, rows};
   const cuuint64_t strides[1] = {cols * 2};

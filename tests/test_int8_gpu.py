@@ -612,3 +612,36 @@ def test_few_rows_of_large_weights(built_library, N, K):
     for M in range(1, 9):
         assert torch.equal(int8.int8_linear(x[:M], wq, ws, out_dtype=torch.float32), want[:M]), M
         assert torch.equal(int8.int8_linear(q[:M], wq, ws, x_scale=xs[:M], out_dtype=torch.float32), want[:M]), M
+
+
+def test_captured_by_a_thread_of_its_own(built_library):
+    """The first call of a thread is part of a capture there; so is the first one of the bf16 layer."""
+    import threading
+
+    import sonicmoe
+    from sonicmoe.functional import int8
+
+    x = torch.randn(100, 256, device="cuda")
+    wq, ws = int8.quantize_rows(torch.randn(64, 256, device="cuda"))
+    m = sonicmoe.MoE(32, 2, 128, 64, sonicmoe.ActivationType.SWIGLU, False, 0.05).cuda().bfloat16()
+    t = torch.randn(3000, 128, device="cuda").bfloat16()
+
+    def calls():
+        with torch.no_grad():
+            return int8.int8_linear(x, wq, ws), m(t, is_inference_mode=True)[0]
+
+    want, got = calls(), []  # (kernels are loaded and workspaces of the library exist)
+    torch.cuda.synchronize()
+
+    def run():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+            out = calls()
+        graph.replay()
+        torch.cuda.synchronize()
+        got.extend(v.clone() for v in out)
+
+    thread = threading.Thread(target=run)
+    thread.start()
+    thread.join()
+    assert len(got) == 2 and all(torch.equal(a, b) for a, b in zip(got, want))
