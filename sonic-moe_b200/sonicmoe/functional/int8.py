@@ -149,6 +149,8 @@ def _linear(x, wq, w_scale, x_scale, bias, out_dtype, activation, offset, freque
         raise ValueError(f"{max(T, rows)} rows or {E * N} channels do not fit into 32-bit numbers")
     with _lib.on_device(dev):
         out = torch.empty(rows, N // 2 if 0 <= activation <= 2 else N, dtype=out_dtype, device=dev)
+        if rows == 0:  # (an empty gather index has no address, which would stand for no gathering)
+            return out
         ws = lib.smoe_int8_linear_workspace_bytes(x_type, T, rows, N, cols, E)
         ws = _lib.workspace(ws, dev) if ws else None
         check(lib.smoe_int8_linear(

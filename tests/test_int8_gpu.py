@@ -645,3 +645,25 @@ def test_captured_by_a_thread_of_its_own(built_library):
     thread.start()
     thread.join()
     assert len(got) == 2 and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_no_rows(built_library):
+    """No tokens, and tokens none of which is gathered."""
+    from sonicmoe.functional import int8
+
+    E, N, K = 3, 40, 64
+    wq, ws = int8.quantize_rows(torch.randn(E, N, K, device="cuda"))
+    off = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    for dtype in TYPES:
+        x = torch.randn(30, K, device="cuda").to(dtype)
+        q, xs = int8.quantize_rows(x)
+        for activation, width in ((None, N), ("swiglu", N // 2)):
+            call = dict(activation_type=activation)
+            for y in (int8.int8_grouped_linear(x, wq, ws, off, none, **call), int8.int8_grouped_linear(x[:0], wq, ws, off, none, **call),
+                      int8.int8_grouped_linear(x[:0], wq, ws, off, **call), int8.int8_linear(x[:0], wq[0], ws[0], **call),
+                      int8.int8_grouped_linear(q, wq, ws, off, none, x_scale=xs, out_dtype=dtype, **call),
+                      int8.int8_linear(q[:0], wq[0], ws[0], x_scale=xs[:0], out_dtype=dtype, **call)):
+                assert y.shape == (0, width) and y.dtype == dtype and y.is_cuda
+    with pytest.raises(ValueError, match="no rows to gather"):
+        int8.int8_grouped_linear(x[:0], wq, ws, off, torch.zeros(2, dtype=torch.int32, device="cuda"))
