@@ -68,19 +68,18 @@ def token_permutation(topk_indices: torch.Tensor, E: int, align: int = 1) -> Tok
     idx = topk_indices.detach().contiguous()
     dev = idx.device
     with _lib.on_device(dev):
-        freq, off, gather, scatter, reverse = torch.empty(2 * E + 1 + 2 * rows + n, dtype=torch.int32, device=dev).split_with_sizes(
-            (E, E + 1, rows, rows, n))
+        # tensors in their own right: views of one buffer would share the count of in-place changes that autograd looks at
+        freq, off, gather, scatter, reverse = torch.empty(
+            2 * E + 1 + 2 * rows + n, dtype=torch.int32, device=dev).unsafe_split_with_sizes((E, E + 1, rows, rows, n))
         ws = lib.smoe_token_permutation_workspace_bytes(n, E)
         ws = _lib.workspace(ws, dev) if ws else None
         check(lib.smoe_token_permutation(
             idx.data_ptr(), _lib.dtype_code(idx.dtype), T, K, E, align, freq.data_ptr(), off.data_ptr(), gather.data_ptr(),
             scatter.data_ptr(), reverse.data_ptr(), ptr(ws), stream_ptr(dev)), "token_permutation")
-    # tensors in their own right: as views of one buffer they would share the count of in-place changes that autograd looks at
-    return TokenPermutation(freq.data, off.data, gather.data, scatter.data, reverse.view(T, K).data, align)
+    return TokenPermutation(freq, off, gather, scatter, reverse.view(T, K), align)
 
 
-def _check_permutation(p: TokenPermutation, dev: torch.device) -> None:
-    pair, row = p.s_reverse_scatter_idx, p.s_scatter_idx
+def _check_permutation(pair: torch.Tensor, row: torch.Tensor, dev: torch.device) -> None:
     if pair.dim() != 2 or row.dim() != 1 or pair.shape[1] == 0:
         raise ValueError("a permutation's s_reverse_scatter_idx is (T, K) and its s_scatter_idx (rows,)")
     if not (pair.dtype == row.dtype == torch.int32 and pair.device == row.device == dev and pair.is_contiguous() and row.is_contiguous()):
@@ -133,21 +132,9 @@ class _FirstDerivative(torch.autograd.Function):
         raise NotImplementedError("unpermute_tokens has first derivatives only where there are scores")
 
 
-def _recorded(*tensors) -> bool:
-    """Whether a call has to go by its autograd function: gradients are recorded, or forward-mode derivatives may be on their way,
-    which the functions refuse (the kernels alone would lose them)."""
-    if forward_ad._current_level >= 0:
-        return True
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _again() -> bool:
-    return torch.is_grad_enabled() or forward_ad._current_level >= 0
-
-
 # Both keep the index vectors themselves: the fields of a permutation may be replaced before the backward pass.  Gradients are recorded
-# there where the caller wants to differentiate them again: without scores each function's gradient is the other one.  An upstream
-# gradient with a forward-mode tangent goes the same way, and is refused.
+# there where the caller wants to differentiate them again: without scores each function's gradient is the other one.  What may have
+# a forward-mode tangent goes by the functions too, here and below, which refuse it; the kernels alone would lose it.
 class _Permute(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, pair, row):
@@ -157,7 +144,8 @@ class _Permute(torch.autograd.Function):
     @staticmethod
     def backward(ctx, drows):
         pair, row = ctx.saved_tensors
-        return _Unpermute.apply(drows, pair, row, None) if _again() else _collect(drows, pair, None), None, None
+        again = torch.is_grad_enabled() or forward_ad._current_level >= 0
+        return _Unpermute.apply(drows, pair, row, None) if again else _collect(drows, pair, None), None, None
 
 
 class _Unpermute(torch.autograd.Function):
@@ -169,7 +157,7 @@ class _Unpermute(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         pair, row, scores, rows = ctx.saved_tensors
-        again = _again()
+        again = torch.is_grad_enabled() or forward_ad._current_level >= 0
         if scores is None:
             return _Permute.apply(dout, pair, row) if again else _spread(dout, pair, row, None), None, None, None
         if rows is None:
@@ -193,11 +181,11 @@ def permute_tokens(x: torch.Tensor, permutation: TokenPermutation) -> torch.Tens
     """rows (permutation.num_rows, H): x[token] of every row's pair, zeros in rows without one.  x (T, H); the gradient of x is
     the sum of its tokens' rows."""
     _lib.require_cuda(x, "x")
-    _check_permutation(permutation, x.device)
-    if x.dim() != 2 or x.shape[0] != permutation.s_reverse_scatter_idx.shape[0]:
-        raise ValueError(f"x has to be ({permutation.s_reverse_scatter_idx.shape[0]}, H), got {tuple(x.shape)}")
     pair, row = permutation.s_reverse_scatter_idx, permutation.s_scatter_idx
-    if _recorded(x):
+    _check_permutation(pair, row, x.device)
+    if x.dim() != 2 or x.shape[0] != pair.shape[0]:
+        raise ValueError(f"x has to be ({pair.shape[0]}, H), got {tuple(x.shape)}")
+    if torch.is_grad_enabled() and x.requires_grad or forward_ad._current_level >= 0:
         return _Permute.apply(x, pair, row)
     return _spread(x, pair, row, None)
 
@@ -206,10 +194,10 @@ def unpermute_tokens(rows: torch.Tensor, permutation: TokenPermutation, scores: 
     """out (T, H): the sum over each token's pairs of score * row (``scores`` (T, K) fp32, bf16 or fp16; None: 1).  Gradients flow
     to rows and scores."""
     _lib.require_cuda(rows, "rows")
-    _check_permutation(permutation, rows.device)
-    if rows.dim() != 2 or rows.shape[0] != permutation.num_rows:
-        raise ValueError(f"rows has to be ({permutation.num_rows}, H), got {tuple(rows.shape)}")
-    pair = permutation.s_reverse_scatter_idx
+    pair, row = permutation.s_reverse_scatter_idx, permutation.s_scatter_idx
+    _check_permutation(pair, row, rows.device)
+    if rows.dim() != 2 or rows.shape[0] != row.shape[0]:
+        raise ValueError(f"rows has to be ({row.shape[0]}, H), got {tuple(rows.shape)}")
     if scores is not None:
         if scores.shape != pair.shape or scores.device != rows.device:
             raise ValueError(f"scores has to be {tuple(pair.shape)} on {rows.device}, got "
@@ -217,6 +205,6 @@ def unpermute_tokens(rows: torch.Tensor, permutation: TokenPermutation, scores: 
         if scores.dtype not in _ROW_TYPES:
             raise TypeError(f"scores has to be fp32, bf16 or fp16, got {scores.dtype}")
         scores = scores.contiguous()
-    if _recorded(rows, scores):
-        return _Unpermute.apply(rows, pair, permutation.s_scatter_idx, scores)
+    if torch.is_grad_enabled() and (rows.requires_grad or scores is not None and scores.requires_grad) or forward_ad._current_level >= 0:
+        return _Unpermute.apply(rows, pair, row, scores)
     return _collect(rows, pair, scores)
