@@ -479,9 +479,11 @@ int smoe_int8_quantize_rows(const void* x, long long ld, int dtype, void* q, lon
 /* y[r, n] = act(x_scale[s] * w_scale[e, n] * sum_k xq[s, k] wq[e, n, k] + bias[e, n]) for the rows r of every expert e.  The sum
  * is exact; it is rounded to fp32, and the result to out_dtype.
  * x (x_rows, cols): SMOE_I8 with x_scale (x_rows), rows starting on 16-byte boundaries (ld bytes apart), or SMOE_F32, SMOE_BF16,
- * SMOE_F16 (ld values apart, x_scale NULL), which is quantised into the workspace first.  wq (E, N, cols) int8, rows w_ld
+ * SMOE_F16 (ld values apart, x_scale NULL), which is quantised into the workspace first, or, with few rows, inside the product's kernel
+ * (the workspace's size is 0 then).  Products of two scales and a sum are formed in fp32, the sum times x_scale first: with the
+ * largest |x| of a row from 2^-119 to 2^103 (or 0) that cannot leave its range before the result does.  wq (E, N, cols) int8, rows w_ld
  * bytes apart (a multiple of 16, 16-byte aligned base), w_scale (E, N).  bias (E, N) SMOE_F32, SMOE_BF16, SMOE_F16 or NULL.
- * expert_frequency_offset (E+1): first row of every expert; NULL: E is 1 and has all rows.  expert_frequency (E) or NULL: rows
+ * expert_frequency_offset (E+1): first row of every expert, ascending; NULL: E is 1 and has all rows.  expert_frequency (E) or NULL: rows
  * of every expert where they do not reach up to the next one's.  Rows of the output that no expert has become zeros.
  * x_gather_idx (rows): the row s of x that r takes (outside [0, x_rows): a row of zeros), or NULL: s = r and x_rows = rows.
  * rows > 0 needs x_rows > 0.

@@ -72,8 +72,10 @@ __device__ __forceinline__ uint32_t pack_typed(int dtype, float lo, float hi) {
 __device__ __forceinline__ float scaled(int acc, float xs, float ws) { return __fmul_rn(__fmul_rn(__int2float_rn(acc), xs), ws); }
 __device__ __forceinline__ float biased(float y, float bias) { return __fadd_rn(y, bias); }
 
-// The activations' values by their definitions.  x sigmoid(x) = x / (1 + exp(-x)) with the fast exponential and division: 2^-21
-// of the value, where the hardware tanh that the bf16 epilogues use is off by 2.5e-4 of x, too much of a small result.
+// The activations' values by their definitions.  x sigmoid(x) = x / (1 + exp(-x)) with the fast exponential, off by up to 2 + 1.2 |x|
+// units in the last place of its value, and division, 2 units: within (5 + 1.2 |x|) 2^-23 of the value, 2^-20 at x = -2 and 2^-17 at -60;
+// below -87, where the value is under 1.5e-36, the division gives zero.  (The hardware tanh that the bf16 epilogues use is off by 2.5e-4
+// of x, too much of a small result.)
 __device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
 template <int ACT>
 __device__ __forceinline__ float activate(float x) {

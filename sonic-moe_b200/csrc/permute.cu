@@ -536,10 +536,6 @@ __global__ void __launch_bounds__(kThreads) collect_kernel(const Rows a) {
     if (c + u * stride < per_row) store_piece<VEC>(dst + static_cast<long long>(c + u * stride) * VEC, pack<T, VEC>(acc[u]));
 }
 
-// The combine's backward pass, one block per token: drows[row(t, k)] = w[t, k] dout[t] and dw[t, k] = <dout[t], rows[row(t, k)]>.
-// Four rows of the token are in flight at a time.  A row's dot product is added up piece by piece in a thread, then over the
-// lanes of each warp, then over the warps: always in the same order.
-constexpr int kDotRows = 4, kDotChunk = 32;
 // The two above by windows.  Sides measured (piece by piece / by windows, us): spread, fp32 rows of 1005 values, T 4099, K 6 33 / 22,
 // of 2049, T 8192, K 4 84 / 58, bf16 of 3001, T 16384, K 4 125 / 88, but fp16 of 1030, which have 4-byte pieces of two values, T 5003,
 // K 3 8.6 / 10.2; collect, in the same order 30.7 / 27.7, 87 / 71, 217 / 128, 18.8 / 11.1.  So a spread goes by windows where a piece
@@ -606,6 +602,10 @@ __global__ void __launch_bounds__(kThreads) collect_windows_kernel(const Rows a)
   W::store(dst, at, a.bytes, pack<T, 16>(acc));
 }
 
+// The combine's backward pass, one block per token: drows[row(t, k)] = w[t, k] dout[t] and dw[t, k] = <dout[t], rows[row(t, k)]>.
+// Four rows of the token are in flight at a time.  A row's dot product is added up piece by piece in a thread, then over the
+// lanes of each warp, then over the warps: always in the same order.
+constexpr int kDotRows = 4, kDotChunk = 32;
 // dot += <f, g> over the one or two values of a word (FULL: both halves of a 16-bit word); returns w g
 template <class T, bool FULL>
 __device__ __forceinline__ uint32_t dot_word(uint32_t f, uint32_t g, float w, float& dot) {

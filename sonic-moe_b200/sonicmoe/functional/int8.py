@@ -3,18 +3,18 @@
     wq, w_scale = quantize_rows(w)                       # once: w (E, N, cols), one scale per expert and channel
     y = int8_grouped_linear(x, wq, w_scale, p.expert_frequency_offset, x_gather_idx=p.x_gather_idx)
 
-or the whole layer, with the router's logits, top-K choice and combine of the bf16 one:
+or the whole layer, with the router's logits, top-K choice and combine of the bf16 one (under torch.no_grad()):
 
     experts = quantize_experts(moe.c_fc.weight.permute(1, 2, 0), moe.c_fc.bias, moe.c_proj.weight.permute(1, 2, 0), moe.c_proj.bias)
     o, router_logits, expert_frequency = moe_int8_softmax_topk_layer(x, moe.router.weight, experts, K)
 
 scale = amax / 127 of the row (1 for a row of zeros), values = 127 x / amax rounded half to even; the sum of a product is exact
-in 32-bit integers and rounded once, so results do not depend on how the work is shared out.  Rows that hold an infinity or a NaN
-give NaN.  8-bit rows start on 16-byte boundaries: `quantize_rows` lays them out so, whatever their width.
+in 32-bit integers and rounded once, so results do not depend on how the work is shared out.  It is multiplied by the row's scale
+and then by the channel's in fp32: rows whose largest value is 0 or from 2^-119 to 2^103 leave its range only where the result does.
+Rows that hold an infinity or a NaN give NaN.  8-bit rows start on 16-byte boundaries: `quantize_rows` lays them out so, whatever their width.
 
 There is no gradient: arguments that require one are refused where gradients are recorded, and those with a forward-mode
-tangent everywhere.  The FP8 experts (`functional.fp8`)
-are the path for training.  The reference has no 8-bit path.
+tangent everywhere.  The FP8 experts (`functional.fp8`) are the path for training.  The reference has no 8-bit path.
 """
 
 from __future__ import annotations
