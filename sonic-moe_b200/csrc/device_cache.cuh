@@ -4,6 +4,7 @@
 // process may drive several devices through this library (threads, one module per GPU), so nothing here is
 // cached per process.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -21,14 +22,21 @@ inline int current_device() {
   return dev;
 }
 
-// Tensor maps are made by a driver call, which needs the device's primary context current on the calling thread, and a thread that
-// has made no runtime call yet (an autograd worker) has none.  Setting the device that is current anyway binds it, and is allowed
-// while a stream is captured; a cudaFree(nullptr) there ends the capture with an error.
+// Tensor maps are made by a driver call, which needs a context current on the calling thread, and a thread that has made no runtime
+// call yet (an autograd worker) has none.  Setting the device that is current anyway binds its primary one, and is allowed while a
+// stream is captured; a cudaFree(nullptr) there ends the capture with an error.  A context that the caller has made current stays.
 inline bool bind_context() {
   static thread_local bool bound = false;
   if (!bound) {
+    using GetCurrentFn = CUresult (*)(CUcontext*);
+    void* get_current = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuCtxGetCurrent", &get_current, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+      return false;
+    CUcontext context = nullptr;
+    if (reinterpret_cast<GetCurrentFn>(get_current)(&context) != CUDA_SUCCESS) return false;
     const int dev = current_device();
-    bound = dev >= 0 && cudaSetDevice(dev) == cudaSuccess;
+    bound = context != nullptr || (dev >= 0 && cudaSetDevice(dev) == cudaSuccess);
   }
   return bound;
 }
