@@ -442,8 +442,8 @@ static int launch_dot_of(const void* x, long long ld, const void* wq, long long 
 // tiles, us: 1024 x 1024 3.3, 3.5, 3.7, 4.2, 4.4 / 6.8; 7168 x 2048 5.5, 5.8, 6.1, 6.8, 7.7 / 9.4; 4096 x 4096 5.9, 6.3, 7.2, 8.1, 9.0 /
 // 10.2; 2048 x 7168 6.0, 6.7, 7.9, 9.3, 10.6 / 12.0; 1024 x 16384 7.8, 9.1, 12.2, 15.0, 18.2 / 19.5; large weights, 4096 x 14336 15.2,
 // 16.0, 18.4, 20.9, 24.2 / 20.5.  Four rows of large weights, 8-bit x: 4096 x 14336 16.5 / 18.5, 8448 x 4096 9.9 / 11.4, 7168 x 8192 15.7 /
-// 15.6, 14336 x 4096 16.9 / 14.4, 28672 x 4096 29.1 / 24.6: by tiles, which lose less than they gain.  With more than two blocks to an SM, bf16, 1, 2, 3 rows: 12000 x 2512 10.7, 11.0, 15.0 / 14.3; 14336 x 4096
-// 15.2, 16.0, 19.7 / 20.5.  Rows of several experts, as a rule one each, are read along with other weights: 8 rows of 128 experts,
+// 15.6, 14336 x 4096 16.9 / 14.4, 28672 x 4096 29.1 / 24.6: by tiles, which gain more than they lose.  With more than two blocks to an
+// SM, bf16, 1, 2, 3 rows: 12000 x 2512 10.7, 11.0, 15.0 / 14.3; 14336 x 4096 15.2, 16.0, 19.7 / 20.5.  Rows of several experts, as a rule one each, are read along with other weights: 8 rows of 128 experts,
 // 2048 x 4096, 22.6 us, quantiser and tiles 28.7; of 256, 312 x 1600, 8.2 and 21.5; 16, 24, 32 rows of 128 experts, 2048 x 4096, 32.8, 45.1,
 // 55.3 and 43.0, 55.3, 67.6; of 32, 512 x 1024, 6.4, 6.9, 8.7 and 10.2, 10.8, 11.0; all 32
 // in one expert 28.7 and 20.5, 7.7 and 9.2.

@@ -606,6 +606,7 @@ __global__ void __launch_bounds__(kThreads) collect_windows_kernel(const Rows a)
 // Four rows of the token are in flight at a time.  A row's dot product is added up piece by piece in a thread, then over the
 // lanes of each warp, then over the warps: always in the same order.
 constexpr int kDotRows = 4, kDotChunk = 32;
+
 // dot += <f, g> over the one or two values of a word (FULL: both halves of a 16-bit word); returns w g
 template <class T, bool FULL>
 __device__ __forceinline__ uint32_t dot_word(uint32_t f, uint32_t g, float w, float& dot) {
