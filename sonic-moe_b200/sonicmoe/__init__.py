@@ -6,6 +6,7 @@ Exports match the reference package (sonicmoe/__init__.py:5-8).
 from .count_cumsum import count_cumsum
 from .enums import ActivationType, KernelBackendMoE
 from .functional import enable_quack_gemm, moe_general_routing_inputs, moe_TC_softmax_topk_layer
+from .functional.norm import NormedRows, rms_norm, rms_norm_quantize
 from .functional.permutation import TokenPermutation, permute_tokens, token_permutation, unpermute_tokens
 from .moe import MoE
 from ._lib import SonicMoEError, check_status
@@ -26,4 +27,8 @@ __all__ = [
     "token_permutation",
     "permute_tokens",
     "unpermute_tokens",
+    # the norm in front of the layer, in the activations' type or as 8-bit rows
+    "NormedRows",
+    "rms_norm",
+    "rms_norm_quantize",
 ]

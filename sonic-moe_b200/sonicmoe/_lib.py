@@ -9,7 +9,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
-from ctypes import c_int, c_longlong, c_size_t, c_uint, c_void_p
+from ctypes import c_float, c_int, c_longlong, c_size_t, c_uint, c_void_p
 
 import torch
 
@@ -29,7 +29,7 @@ _ERRORS = {
     -8: "size exceeds the built-in scratch of the allocation-free entry point",
 }
 
-P, I, LL = c_void_p, c_int, c_longlong
+P, I, LL, F = c_void_p, c_int, c_longlong, c_float
 
 # name -> (restype, argtypes); must list every function the header declares.
 SIGNATURES: dict[str, tuple] = {
@@ -110,6 +110,9 @@ SIGNATURES: dict[str, tuple] = {
     "smoe_int8_quantize_rows": (I, [P, LL, I, P, LL, P, LL, I, P]),
     "smoe_int8_linear_workspace_bytes": (c_size_t, [I, I, I, I, I, I]),
     "smoe_int8_linear": (I, [P, LL, I, P, P, LL, P, P, I, P, I, P, P, P, I, I, I, I, I, I, P, P, P]),
+    "smoe_rms_norm": (I, [P, LL, P, LL, P, I, P, P, P, P, LL, P, I, LL, I, F, P]),
+    "smoe_rms_norm_backward_workspace_bytes": (c_size_t, [LL, I]),
+    "smoe_rms_norm_backward": (I, [P, LL, P, LL, P, LL, P, I, P, P, P, I, LL, I, P, P]),
     "smoe_peer_alloc": (I, [c_size_t, P]),
     "smoe_peer_free": (I, [P]),
     "smoe_peer_export": (I, [P, P]),
