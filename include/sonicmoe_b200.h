@@ -502,16 +502,16 @@ int smoe_int8_linear(const void* x, long long ld, int x_dtype, const float* x_sc
 
 /* h = x + residual, rounded to dtype (residual NULL: h = x); r = 1 / sqrt(mean(h^2) + eps); y = h r weight.
  * x, residual, y, h (rows, H): SMOE_F32, SMOE_BF16 or SMOE_F16; ld, residual_ld: values from row to row of the inputs; y and h are
- * packed.  weight (H): of the same type, or SMOE_F32.  Everything between h and the results is fp32, rounded once.
+ * packed and 16-byte aligned.  weight (H): of the same type, or SMOE_F32.  Everything between h and the results is fp32, rounded once.
  * h (NULL: not kept) needs a residual.  rstd (rows) fp32 or NULL: r, as the backward call takes it.
  * q (rows, H) int8, q_ld bytes from row to row (a multiple of 16; columns up to the next multiple of 16 become zeros) with scale (rows), or
  * both NULL: the unrounded y as smoe_int8_quantize_rows quantises fp32 rows; H <= 131071.  y may be NULL where q is given.
- * eps >= 0, rows < 2^31, H <= 2^30.  No output overlaps an input. */
+ * eps >= 0, rows < 2^31, H <= 2^28.  No output overlaps an input. */
 int smoe_rms_norm(const void* x, long long ld, const void* residual, long long residual_ld, const void* weight,
                   int weight_dtype, void* y, void* h, float* rstd, void* q, long long q_ld, float* scale, int dtype,
                   long long rows, int H, float eps, void* stream);
 /* With u = h rstd and g = dy weight: dx = dh + rstd (g - u mean(g u)) (the residual's gradient too), dweight = sum over the rows of
- * dy u.  dh (the upstream gradient of h): NULL for none.  dx packed, dweight of the weight's type; either may be NULL.  With dweight,
+ * dy u.  dh (the upstream gradient of h): NULL for none.  dx packed and 16-byte aligned, dweight of the weight's type; either may be NULL.  With dweight,
  * workspace: smoe_rms_norm_backward_workspace_bytes bytes, 16-byte aligned.  The same bits every time. */
 size_t smoe_rms_norm_backward_workspace_bytes(long long rows, int H);
 int smoe_rms_norm_backward(const void* dy, long long dy_ld, const void* dh, long long dh_ld, const void* h, long long h_ld,

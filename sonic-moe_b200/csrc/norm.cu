@@ -7,140 +7,239 @@ namespace norm {
 struct Forward {
   const void* x; long long x_ld;            // values from row to row
   const void* res; long long res_ld;        // or nullptr
-  const void* w; int w_wide;                // weights of the columns start on 16-byte boundaries
+  const void* w; int w_wide;                // starts on a 16-byte boundary
   void* y;                                  // packed rows, or nullptr
   void* h;                                  // packed rows, or nullptr
   float* rstd;                              // (rows), or nullptr
   int8_t* q; long long q_ld; float* scale;  // or nullptr
   long long rows;
   int H;
-  float eps;
+  float eps, per_value;                     // 1 / H
 };
 
-// VE 8-bit values of b, the `i`-th VE of them.
-template <int VE, int N>
-__device__ __forceinline__ void store_bytes(int8_t* q, const uint32_t (&b)[N], int i) {
-  if constexpr (VE == 8) *reinterpret_cast<uint2*>(q) = make_uint2(b[2 * i], b[2 * i + 1]);
-  else if constexpr (VE == 4) *reinterpret_cast<uint32_t*>(q) = b[i];
-  else if constexpr (VE == 2) *reinterpret_cast<uint16_t*>(q) = static_cast<uint16_t>(b[i / 2] >> (16 * (i & 1)));
-  else *q = static_cast<int8_t>(b[i / 4] >> (8 * (i & 3)));
+template <class T, class W, int EP, bool ALIGNED, bool MASKED>
+__device__ __forceinline__ void take_weights(const Forward& a, const Columns<T, ALIGNED>& columns, int c0, int step, Values<W, EP, kValues<T>>& w) {
+  if (ALIGNED && a.w_wide) w.template load<true, false>(static_cast<const W*>(a.w), columns, c0, step);
+  else w.template load<false, false>(static_cast<const W*>(a.w), columns, c0, step);
+  if (MASKED) w.template mask<ALIGNED>(columns, c0, step);
+}
+// h, on its way out the first time
+template <class T, int EP, bool ALIGNED>
+__device__ __forceinline__ void take_rows(const Forward& a, long long row, const Columns<T, ALIGNED>& columns, int c0, int step, bool keep, Values<T, EP, kValues<T>>& h) {
+  h.template load<ALIGNED, true>(static_cast<const T*>(a.x) + row * a.x_ld, columns, c0, step);
+  if (a.res == nullptr) {
+    h.template mask<ALIGNED>(columns, c0, step);
+    return;
+  }
+  Values<T, EP, kValues<T>> r;
+  r.template load<ALIGNED, true>(static_cast<const T*>(a.res) + row * a.res_ld, columns, c0, step);
+#pragma unroll
+  for (int k = 0; k < EP / 2; ++k) h.add(k, r);
+  h.template mask<ALIGNED>(columns, c0, step);
+  if (keep && a.h != nullptr) h.template store<ALIGNED>(static_cast<T*>(a.h) + row * a.H, columns, c0, step);
 }
 
-// A row is read once and stays in registers, EP values in each of its 2^log2 threads.  Bound by memory.  y = (h w) r: the maximum of |h w|
-// times r is that of |y|, whatever is rounded on the way, so that one reduction serves both.  LONG: rows that a block's threads
-// do not hold are read twice, EP values of each thread at a time.
-template <class T, class W, int VE, int EP, bool Q, bool LONG>
-__global__ void __launch_bounds__(kThreads) forward_kernel(const Forward a, int log2) {
+template <class T, class W, int EP, bool Q>
+__device__ __forceinline__ void measure(const Values<T, EP, kValues<T>>& h, const Values<W, EP, kValues<T>>& w, F2& sum, float& most) {
+#pragma unroll
+  for (int k = 0; k < EP / 2; ++k) {
+    const F2 f = h.get(k);
+    sum = fma2(f, f, sum);
+    if (Q) {
+      float x, y;
+      (f * w.get(k)).split(x, y);
+      most = max_abs(most, x, y);
+    }
+  }
+}
+
+// 8-bit values of fp32 rows are rounded exactly, as quantize_rows rounds them.  Those of 16-bit rows: y, off by some units itself, times 127 /
+// max |y| in one fused multiply-add: within 127 * 2^-23 = 1.6e-5 of a step of the half to even of that product (exactly as above 8192 x 4096
+// with a residual takes 199 / 55 us).
+template <bool EXACT>
+__device__ __forceinline__ void quantise(const i8::RowScale& s, float (&f)[8], uint32_t (&b)[2]) {
+  if constexpr (EXACT) {
+    i8::quantize_values<false>(s, f, b);
+  } else {
+    if (s.pre != 1.f) {
+#pragma unroll
+      for (auto& x : f) x *= s.pre;
+    }
+    int q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = __float_as_int(fmaf(f[i], s.inv, i8::kRoundMagic));
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      b[j] = s.keep & __byte_perm(__byte_perm(q[4 * j], q[4 * j + 1], 0x0040), __byte_perm(q[4 * j + 2], q[4 * j + 3], 0x0040), 0x5410);
+  }
+}
+
+// What follows the sum of a row's squares and the largest |h w|: r, y = (h w) r, the 8-bit values, the row's scale.  The maximum of |h w|
+// times r is that of |y|, whatever is rounded on the way, so that one reduction serves both.
+template <class T, class W, int EP, bool ALIGNED, bool Q>
+struct Finish {
+  static constexpr int VE = kValues<T>, P = EP / VE;
+  float r;
+  i8::RowScale s;
+  __device__ __forceinline__ Finish(const Forward& a, long long row, float sum, float most, bool writes) {
+    r = inverse_root(fmaf(sum, a.per_value, a.eps));
+    if (writes && a.rstd != nullptr) a.rstd[row] = r;
+    if (Q) {
+      const uint32_t bits = __float_as_uint(most * r) & 0x7FFFFFFFu;
+      s = i8::row_scale<false>(bits);
+      if (writes) a.scale[row] = i8::scale_of_row(bits);
+    }
+  }
+  __device__ __forceinline__ void put(const Forward& a, long long row, const Columns<T, ALIGNED>& columns, int c0, int step,
+                                      const Values<T, EP, VE>& h, const Values<W, EP, VE>& w) const {
+    if (Q && a.y == nullptr) return;
+    const F2 rr(r, r);
+    Values<T, EP, VE> y;
+#pragma unroll
+    for (int k = 0; k < EP / 2; ++k) y.set(k, h.get(k) * w.get(k) * rr);
+    y.template store<ALIGNED>(static_cast<T*>(a.y) + row * a.H, columns, c0, step);
+  }
+  // the 8-bit values, in the order of h's
+  __device__ __forceinline__ void quantised(const Values<T, EP, VE>& h, const Values<W, EP, VE>& w, uint32_t (&b)[EP / 4]) const {
+    const F2 rr(r, r);
+#pragma unroll
+    for (int g = 0; g < EP; g += 8) {
+      float f[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) (h.get(g / 2 + k) * w.get(g / 2 + k) * rr).split(f[2 * k], f[2 * k + 1]);
+      uint32_t two[2];
+      quantise<(sizeof(T) == 4)>(s, f, two);
+      b[g / 4] = two[0];
+      b[g / 4 + 1] = two[1];
+    }
+  }
+};
+
+// A row is read once and stays in registers, EP values in each of its threads.  Bound by memory.
+template <class T, class W, int EP, bool ALIGNED, bool Q>
+__global__ void __launch_bounds__(kThreads, EP <= 16 ? 2 : 1) forward_kernel(const Forward a, int tpr) {
   release_next();
   wait_for_previous();
-  constexpr int P = EP / VE;
-  __shared__ float part[kThreads / 32];
-  __shared__ uint32_t part_bits[kThreads / 32];
-  const int tpr = 1 << log2, sub = threadIdx.x >> log2, tid = threadIdx.x & (tpr - 1);
-  const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x >> log2) + sub;
+  __shared__ Parts part;
+  const Share at(tpr);
+  const long long row = static_cast<long long>(blockIdx.x) * at.subs + at.sub;
   const bool live = row < a.rows;
-  const int pieces = live ? a.H / VE : 0;
-  const T* x = static_cast<const T*>(a.x) + row * a.x_ld;
-  const T* res = static_cast<const T*>(a.res) + row * a.res_ld;
-  const W* weight = static_cast<const W*>(a.w);
-  Piece<T, VE> h[P];
-  Piece<W, VE> w[P];
-  // pieces c0, c0 + tpr, ..: h on its way out the first time
-  const auto take = [&](int c0, bool first) {
-    Piece<T, VE> r[P];
+  Columns<T, ALIGNED> columns(row, a.H);
+  if (!live) columns.pieces = 0;
+  Values<T, EP, kValues<T>> h;
+  Values<W, EP, kValues<T>> w;
+  take_rows<T, EP, ALIGNED>(a, row, columns, at.tid, tpr, true, h);
+  take_weights<T, W, EP, ALIGNED, Q>(a, columns, at.tid, tpr, w);
+  F2 sums(0.f, 0.f);
+  float most = 0.f;
+  measure<T, W, EP, Q>(h, w, sums, most);
+  float sum = sums.sum();
+  row_reduce<Q>(sum, most, at, part);
+  h.forget();
+  w.forget();
+  const Finish<T, W, EP, ALIGNED, Q> finish(a, row, sum, most, live && at.tid == 0);
+  finish.put(a, row, columns, at.tid, tpr, h, w);
+  if constexpr (Q) {
+    // A row of 8-bit values starts on a 16-byte boundary.  Where the pieces do not, the end of a piece and the beginning of the next one
+    // make a store; what follows the row are zeros, and so are its columns up to the next multiple of 16.
+    constexpr int VE = kValues<T>, P = EP / VE;
+    using Bytes = typename std::conditional<VE == 8, uint64_t, uint32_t>::type;
+    uint32_t b[EP / 4];
+    finish.quantised(h, w, b);
+    Bytes v[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      const int c = c0 + i * tpr;
-      if (c < pieces) h[i].load(x + static_cast<long long>(c) * VE); else h[i].zero();
+      if constexpr (VE == 8) v[i] = b[2 * i] | static_cast<uint64_t>(b[2 * i + 1]) << 32;
+      else v[i] = b[i];
     }
-    if (a.res != nullptr) {
+    if constexpr (!ALIGNED) {
+      __shared__ Bytes bytes[EP / VE * kThreads];
 #pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const int c = c0 + i * tpr;
-        if (c < pieces) r[i].load(res + static_cast<long long>(c) * VE); else r[i].zero();
+      for (int i = 0; i < P; ++i) bytes[i * blockDim.x + threadIdx.x] = v[i];
+      __syncthreads();
+      if (columns.shift > 0) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          const bool last = at.tid == tpr - 1;
+          const Bytes next = !last ? bytes[i * blockDim.x + threadIdx.x + 1] : i + 1 < P ? bytes[(i + 1) * blockDim.x + threadIdx.x - at.tid] : 0;
+          v[i] = (v[i] >> (8 * columns.shift)) | (next << (8 * (VE - columns.shift)));
+        }
       }
     }
+    const int end = live ? (a.H + 15) / 16 * 16 : 0;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      const int c = c0 + i * tpr;
-      if (c < pieces) w[i].load_shared(weight + static_cast<long long>(c) * VE, a.w_wide); else w[i].zero();
+      const int c = at.tid + i * tpr;
+      if (VE * c < end) *reinterpret_cast<Bytes*>(a.q + row * a.q_ld + VE * c) = v[i];
     }
-    if (a.res != nullptr) {
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const int c = c0 + i * tpr;
-#pragma unroll
-        for (int j = 0; j < VE; ++j) h[i].set(j, h[i][j] + r[i][j]);
-        if (first && a.h != nullptr && c < pieces) h[i].store(static_cast<T*>(a.h) + row * a.H + static_cast<long long>(c) * VE);
-      }
-    }
-  };
-  float sum = 0.f;
-  uint32_t bits = 0u;
-  for (int c0 = tid; c0 < (LONG ? pieces : tid + 1); c0 += P * tpr) {
-    take(c0, true);
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-#pragma unroll
-      for (int j = 0; j < VE; ++j) {
-        sum = fmaf(h[i][j], h[i][j], sum);
-        if (Q) bits = max(bits, __float_as_uint(h[i][j] * w[i][j]) & 0x7FFFFFFFu);
-      }
-    }
-  }
-  row_reduce<Q>(sum, bits, log2, part, part_bits);
-  if (!live) return;
-  const float r = __frsqrt_rn(sum / static_cast<float>(a.H) + a.eps);
-  if (tid == 0 && a.rstd != nullptr) a.rstd[row] = r;
-  i8::RowScale s;
-  if (Q) {
-    bits = __float_as_uint(__uint_as_float(bits) * r) & 0x7FFFFFFFu;
-    s = i8::row_scale<false>(bits);
-    if (tid == 0) a.scale[row] = i8::scale_of_row(bits);
-  }
-  for (int c0 = tid; c0 < (LONG ? pieces : tid + 1); c0 += P * tpr) {
-    if (LONG) take(c0, false);
-    float f[EP];
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-#pragma unroll
-      for (int j = 0; j < VE; ++j) f[i * VE + j] = h[i][j] * w[i][j] * r;
-    }
-    if (!Q || a.y != nullptr) {
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const int c = c0 + i * tpr;
-        Piece<T, VE> o;
-#pragma unroll
-        for (int j = 0; j < VE; ++j) o.set(j, f[i * VE + j]);
-        if (c < pieces) o.store(static_cast<T*>(a.y) + row * a.H + static_cast<long long>(c) * VE);
-      }
-    }
-    if constexpr (Q) {
-      uint32_t b[EP / 4];
-      i8::quantize_values<false>(s, f, b);
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const int c = c0 + i * tpr;
-        if (c < pieces) store_bytes<VE>(a.q + row * a.q_ld + static_cast<long long>(c) * VE, b, i);
-      }
-    }
-  }
-  if (Q) {  // columns up to the next multiple of 16 are zeros
-    for (int c = a.H + tid; c < (a.H + 15) / 16 * 16; c += tpr) a.q[row * a.q_ld + c] = 0;
+    for (int c = at.tid + P * tpr; VE * c < end; c += tpr) *reinterpret_cast<Bytes*>(a.q + row * a.q_ld + VE * c) = 0;
   }
 }
 
-template <class T, class W, int VE, int EP, bool Q, bool LONG>
-static cudaError_t launch_forward(const Forward& a, int log2, cudaStream_t st) {
-  const int threads = log2 > 8 ? 1 << log2 : 256;
-  const long long per = threads >> log2, blocks = (a.rows + per - 1) / per;
-  return launch_chained(forward_kernel<T, W, VE, EP, Q, LONG>, dim3(static_cast<unsigned>(blocks)), threads, 0, st, 1, a, log2);
+// Rows that a block's threads do not hold: read twice, EP values of each thread at a time, a row to a block.
+template <class T, class W, int EP, bool ALIGNED, bool Q>
+__global__ void __launch_bounds__(kThreads) forward_long_kernel(const Forward a) {
+  release_next();
+  wait_for_previous();
+  __shared__ Parts part;
+  const Share at(kThreads);
+  const long long row = blockIdx.x;
+  const Columns<T, ALIGNED> columns(row, a.H);
+  const int round = EP / kValues<T> * kThreads;
+  Values<T, EP, kValues<T>> h;
+  Values<W, EP, kValues<T>> w;
+  F2 sums(0.f, 0.f);
+  float most = 0.f;
+  for (int c = 0; c < columns.pieces; c += round) {
+    take_rows<T, EP, ALIGNED>(a, row, columns, c + at.tid, kThreads, true, h);
+    take_weights<T, W, EP, ALIGNED, Q>(a, columns, c + at.tid, kThreads, w);
+    measure<T, W, EP, Q>(h, w, sums, most);
+  }
+  float sum = sums.sum();
+  row_reduce<Q>(sum, most, at, part);
+  const Finish<T, W, EP, ALIGNED, Q> finish(a, row, sum, most, at.tid == 0);
+  for (int c = 0; c < columns.pieces; c += round) {
+    take_rows<T, EP, ALIGNED>(a, row, columns, c + at.tid, kThreads, false, h);
+    take_weights<T, W, EP, ALIGNED, Q>(a, columns, c + at.tid, kThreads, w);
+    finish.put(a, row, columns, c + at.tid, kThreads, h, w);
+    if constexpr (Q) {
+      uint32_t b[EP / 4];
+      finish.quantised(h, w, b);
+#pragma unroll
+      for (int i = 0; i < EP; ++i) {
+        const int col = columns.first(c + at.tid + i / kValues<T> * kThreads) + i % kValues<T>;
+        if (col >= 0 && col < (a.H + 15) / 16 * 16) a.q[row * a.q_ld + col] = static_cast<int8_t>(b[i / 4] >> (8 * (i % 4)));
+      }
+    }
+  }
 }
-template <class T, class W, int VE, bool Q>
+
+template <class T, class W, int EP, bool ALIGNED, bool Q>
+static cudaError_t launch_rows(const Forward& a, const Shape& s, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>((a.rows + s.subs - 1) / s.subs));
+  return launch_chained(forward_kernel<T, W, EP, ALIGNED, Q>, grid, s.threads, 0, st, 1, a, s.tpr);
+}
+// Values of a thread.  Whole pieces: 16 with a residual, 32 without one, so that as many loads are on their way (bf16, us: 16384 x 5000 66.5 / 50.1,
+// 100000 x 256 18.2 / 17.5; with a residual 32768 x 4096 157.9 / 158.8, as 8-bit rows 163 / 174).  Other rows: whichever of 16, 24 and 32 leaves
+// the fewest threads idle (100000 x 257 57.9 / 39.6 / 48.4, 20000 x 2049 with a residual 65.5 / 60.4 / 71.2); of two that leave as many, the
+// smaller up to 256 threads a row (5003 x 1030 10.0 / 11.0), the larger above (16384 x 7169 192 / 161).
+template <class T, class W, bool ALIGNED, bool Q>
 static cudaError_t launch_forward(const Forward& a, cudaStream_t st) {
-  if (a.H <= 16 * kThreads) return launch_forward<T, W, VE, 16, Q, false>(a, row_threads_log2(a.H, 16), st);
-  return launch_forward<T, W, VE, 16, Q, true>(a, 9, st);
+  const long long values = a.H + (ALIGNED ? 0 : kValues<T> - 1);
+  if (values > 32 * kThreads)
+    return launch_chained(forward_long_kernel<T, W, 16, ALIGNED, Q>, dim3(static_cast<unsigned>(a.rows)), kThreads, 0, st, 1, a);
+  const Shape s16 = shape_of(values, 16), s32 = shape_of(values, 32);
+  if constexpr (ALIGNED) {
+    if (values <= 16 * kThreads && (a.res != nullptr || values < 64)) return launch_rows<T, W, 16, ALIGNED, Q>(a, s16, st);
+    return launch_rows<T, W, 32, ALIGNED, Q>(a, s32, st);
+  } else {
+    const Shape s24 = shape_of(values, 24);
+    const int w16 = 16 * s16.tpr, w24 = 24 * s24.tpr, w32 = 32 * s32.tpr;
+    const bool wide = s16.tpr > 256;
+    if (s16.tpr <= kThreads && (wide ? w16 < w24 && w16 < w32 : w16 <= w24 && w16 <= w32)) return launch_rows<T, W, 16, ALIGNED, Q>(a, s16, st);
+    if (s24.tpr <= kThreads && (wide ? w24 < w32 : w24 <= w32)) return launch_rows<T, W, 24, ALIGNED, Q>(a, s24, st);
+    return launch_rows<T, W, 32, ALIGNED, Q>(a, s32, st);
+  }
 }
 
 }  // namespace norm
@@ -159,21 +258,19 @@ extern "C" int smoe_rms_norm(const void* x, long long ld, const void* residual, 
   if (rows == 0) return SMOE_OK;
   if (x == nullptr || weight == nullptr || (y == nullptr && q == nullptr) || (q == nullptr) != (scale == nullptr)) return SMOE_ERR_SHAPE;
   if (h != nullptr && residual == nullptr) return SMOE_ERR_SHAPE;
-  if ((address(x) | address(residual) | address(y) | address(h)) % size != 0 || address(weight) % wsize != 0 ||
-      (address(rstd) | address(scale)) % 4 != 0 || address(q) % 16 != 0 || (q != nullptr && q_ld % 16 != 0))
+  if ((address(x) | address(residual)) % size != 0 || address(weight) % wsize != 0 || (address(y) | address(h) | address(q)) % 16 != 0 ||
+      (address(rstd) | address(scale)) % 4 != 0 || (q != nullptr && q_ld % 16 != 0))
     return SMOE_ERR_ALIGNMENT;
   Forward a = {};
   a.x = x; a.x_ld = ld; a.res = residual; a.res_ld = residual != nullptr ? residual_ld : 0;
   a.w = weight; a.w_wide = address(weight) % 16 == 0;
   a.y = y; a.h = h; a.rstd = rstd; a.q = static_cast<int8_t*>(q); a.q_ld = q_ld; a.scale = scale;
-  a.rows = rows; a.H = H; a.eps = eps;
-  const int bytes = access_bytes({address(x) | address(residual) | address(y) | address(h), ld * size, a.res_ld * size,
-                                  static_cast<long long>(H) * size});
+  a.rows = rows; a.H = H; a.eps = eps; a.per_value = 1.f / static_cast<float>(H);
+  const bool aligned = (address(x) | address(residual) | ld * size | a.res_ld * size | static_cast<long long>(H) * size) % 16 == 0;
   return for_types(dtype, weight_dtype, [&](auto t, auto v) {
     using T = decltype(t);
     using W = decltype(v);
-    return launched(for_access<T>(bytes, [&](auto ve) {
-      return q != nullptr ? launch_forward<T, W, ve, true>(a, S(stream)) : launch_forward<T, W, ve, false>(a, S(stream));
-    }));
+    if (q != nullptr) return launched(aligned ? launch_forward<T, W, true, true>(a, S(stream)) : launch_forward<T, W, false, true>(a, S(stream)));
+    return launched(aligned ? launch_forward<T, W, true, false>(a, S(stream)) : launch_forward<T, W, false, false>(a, S(stream)));
   });
 }

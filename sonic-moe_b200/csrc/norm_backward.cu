@@ -8,122 +8,159 @@ struct Backward {
   const void* dy; long long dy_ld;  // values from row to row
   const void* dh; long long dh_ld;  // or nullptr
   const void* h; long long h_ld;
-  const void* w; int w_wide;        // weights of the columns start on 16-byte boundaries
+  const void* w; int w_wide;        // starts on a 16-byte boundary
   const float* rstd;
   void* dx;                         // packed rows, or nullptr
   float* partial;                   // (blocks, H): each block's part of the weight's gradient, or nullptr
   long long rows;
   int H;
+  float per_value;                  // 1 / H
 };
 
 constexpr int kMostBlocks = 4 * 148;  // four to each of a B200's SMs
 
-// Blocks take rows in turn and keep their part of the weight's gradient in registers, EP columns in each thread, until the end.  A row is
-// read once.  Bound by memory.  LONG: rows that a block's threads do not hold are read twice, and the part lies in the block's row of
-// `partial`, where the same thread adds to the same columns each time.
-template <class T, class W, int VE, int EP, bool LONG>
-__global__ void __launch_bounds__(kThreads) backward_kernel(const Backward a, int log2) {
-  release_next();
+template <class T, class W, int EP, bool ALIGNED>
+__device__ __forceinline__ void take_weights(const Backward& a, const Columns<T, ALIGNED>& columns, int c0, int step, Values<W, EP, kValues<T>>& w) {
+  if (ALIGNED && a.w_wide) w.template load<true, false>(static_cast<const W*>(a.w), columns, c0, step);
+  else w.template load<false, false>(static_cast<const W*>(a.w), columns, c0, step);
+  w.template mask<ALIGNED>(columns, c0, step);
+}
+
+// With p = dy w: dx = dh + r p - h (r^2 mean(p h r)), the sum over a row being r times that of (dy h) w; dw sums (dy h) r.
+template <class T, class W, int EP, int VE>
+__device__ __forceinline__ void row_gradient(const Values<T, EP, VE>& dy, const Values<T, EP, VE>& h, const Values<W, EP, VE>& w,
+                                             const Values<T, EP, VE>& dh, float r, float mean, Values<T, EP, VE>& dx) {
+  const F2 rr(r, r), along(-r * r * mean, -r * r * mean);
+#pragma unroll
+  for (int k = 0; k < EP / 2; ++k) dx.set(k, fma2(h.get(k), along, fma2(dy.get(k) * w.get(k), rr, dh.get(k))));
+}
+
+// Blocks take rows in turn and keep the weights and their part of the weights' gradient in registers, EP columns in each thread, until the end: so
+// the rows of a thread all have the same shift (Columns), `step` rows apart.  A row is read once.  Bound by memory.
+template <class T, class W, int EP, bool ALIGNED, int REGISTERS>
+__global__ void __maxnreg__(REGISTERS) backward_kernel(const Backward a, int tpr) {
   wait_for_previous();
-  constexpr int P = EP / VE;
-  __shared__ float part[2][kThreads / 32];
-  extern __shared__ float sums[];
-  const int tpr = 1 << log2, sub = threadIdx.x >> log2, tid = threadIdx.x & (tpr - 1), subs = blockDim.x >> log2;
-  const float per_value = 1.f / static_cast<float>(a.H);
-  const int all = a.H / VE;
-  const W* weight = static_cast<const W*>(a.w);
-  float* mine = a.partial + static_cast<long long>(blockIdx.x) * a.H;
-  Piece<W, VE> w[P];
-  Piece<T, VE> dy[P], h[P], dh[P];
-  float acc[EP];
+  constexpr int VE = kValues<T>;
+  __shared__ Parts part[2];
+  extern __shared__ float sums[];  // (subs, H) where a block has several rows at a time
+  const Share at(tpr);
+  const long long step = static_cast<long long>(gridDim.x) * at.subs;
+  const long long first = static_cast<long long>(blockIdx.x) * at.subs + at.sub;
+  const Columns<T, ALIGNED> columns(first, a.H);
+  Values<W, EP, VE> w;
+  take_weights<T, W, EP, ALIGNED>(a, columns, at.tid, tpr, w);
+  F2 acc[EP / 2];
 #pragma unroll
-  for (int i = 0; i < EP; ++i) acc[i] = 0.f;
-  const auto take_weights = [&](int c0) {
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const int c = c0 + i * tpr;
-      if (c < all) w[i].load_shared(weight + static_cast<long long>(c) * VE, a.w_wide); else w[i].zero();
-    }
-  };
-  const auto take = [&](long long row, int c0) {
-    const bool live = row < a.rows;
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const long long c = c0 + i * tpr;
-      if (live && c < all) {
-        dy[i].load(static_cast<const T*>(a.dy) + row * a.dy_ld + c * VE);
-        h[i].load(static_cast<const T*>(a.h) + row * a.h_ld + c * VE);
-        if (a.dh != nullptr) dh[i].load(static_cast<const T*>(a.dh) + row * a.dh_ld + c * VE);
-      } else {
-        dy[i].zero();
-        h[i].zero();
-      }
-    }
-  };
-  if (!LONG) take_weights(tid);
+  for (int k = 0; k < EP / 2; ++k) acc[k] = F2(0.f, 0.f);
   int turn = 0;
-  for (long long base = static_cast<long long>(blockIdx.x) * subs; base < a.rows; base += static_cast<long long>(gridDim.x) * subs) {
-    const long long row = base + sub;
-    const bool live = row < a.rows;
-    const float r = live ? a.rstd[row] : 0.f;
-    float sum = 0.f;
-    for (int c0 = tid; c0 < (LONG ? all : tid + 1); c0 += P * tpr) {
-      take(row, c0);
-      if (LONG) take_weights(c0);
+  for (long long row = first; row - at.sub < a.rows; row += step) {
+    Columns<T, ALIGNED> mine = columns;
+    if (row >= a.rows) mine.pieces = 0;
+    const float r = row < a.rows ? a.rstd[row] : 0.f;
+    Values<T, EP, VE> dy, h, dh;
+    dy.template load<ALIGNED, true>(static_cast<const T*>(a.dy) + row * a.dy_ld, mine, at.tid, tpr);
+    h.template load<ALIGNED, true>(static_cast<const T*>(a.h) + row * a.h_ld, mine, at.tid, tpr);
+    dy.template mask<ALIGNED>(mine, at.tid, tpr);
+    h.template mask<ALIGNED>(mine, at.tid, tpr);
+    Columns<T, ALIGNED> upstream = mine;
+    if (a.dh == nullptr) upstream.pieces = 0;
+    dh.template load<ALIGNED, true>(static_cast<const T*>(a.dh) + row * a.dh_ld, upstream, at.tid, tpr);
+    F2 total(0.f, 0.f);
+    const F2 rr(r, r);
 #pragma unroll
-      for (int i = 0; i < P; ++i) {
+    for (int k = 0; k < EP / 2; ++k) {
+      const F2 t = dy.get(k) * h.get(k);
+      total = fma2(t, w.get(k), total);
+      acc[k] = fma2(t, rr, acc[k]);
+    }
+    w.forget();
+    if (a.dx == nullptr) continue;
+    float sum = total.sum(), none = 0.f;
+    row_reduce<false>(sum, none, at, part[turn]);
+    turn ^= 1;  // the next row's sums lie elsewhere: one barrier a row is enough
+    dy.forget();
+    h.forget();
+    Values<T, EP, VE> dx;
+    row_gradient(dy, h, w, dh, r, sum * r * a.per_value, dx);
+    dx.template store<ALIGNED>(static_cast<T*>(a.dx) + row * a.H, mine, at.tid, tpr);
+    w.forget();
+  }
+  if (a.partial == nullptr) return;
+  float* part_of_block = a.partial + static_cast<long long>(blockIdx.x) * a.H;
+  float* to = at.subs > 1 ? sums + at.sub * a.H : part_of_block;
 #pragma unroll
-        for (int j = 0; j < VE; ++j) {
-          const float t = dy[i][j] * (h[i][j] * r);
-          sum = fmaf(t, w[i][j], sum);
-          if (!LONG) {
-            acc[i * VE + j] += t;
-          } else if (a.partial != nullptr && c0 + i * tpr < all) {
-            float* d = mine + static_cast<long long>(c0 + i * tpr) * VE + j;
-            *d = base == blockIdx.x ? t : *d + t;  // (LONG: a block has a row at a time)
+  for (int k = 0; k < EP / 2; ++k) {
+    float f[2];
+    acc[k].split(f[0], f[1]);
+#pragma unroll
+    for (int i = 2 * k; i < 2 * k + 2; ++i) {
+      const int col = columns.first(at.tid + i / VE * tpr) + i % VE;
+      if (col >= 0 && col < a.H) to[col] = f[i & 1];
+    }
+  }
+  if (at.subs == 1) return;
+  __syncthreads();
+  for (int c = threadIdx.x; c < a.H; c += blockDim.x) {
+    float s = 0.f;
+    for (int k = 0; k < at.subs; ++k) s += sums[k * a.H + c];
+    part_of_block[c] = s;
+  }
+}
+
+// Rows that a block's threads do not hold: read twice, EP values of each thread at a time, a row to a block at a time; the block's part of the
+// weights' gradient lies in its row of `partial`, where the same thread adds to the same columns each time (equal shifts here too).
+template <class T, class W, int EP, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads) backward_long_kernel(const Backward a) {
+  wait_for_previous();
+  constexpr int VE = kValues<T>;
+  __shared__ Parts part[2];
+  const Share at(kThreads);
+  const Columns<T, ALIGNED> columns(blockIdx.x, a.H);
+  const int round = EP / VE * kThreads;
+  float* mine = a.partial + static_cast<long long>(blockIdx.x) * a.H;
+  Values<W, EP, VE> w;
+  Values<T, EP, VE> dy, h;
+  int turn = 0;
+  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const float r = a.rstd[row];
+    const auto take = [&](int c0) {
+      dy.template load<ALIGNED, true>(static_cast<const T*>(a.dy) + row * a.dy_ld, columns, c0, kThreads);
+      h.template load<ALIGNED, true>(static_cast<const T*>(a.h) + row * a.h_ld, columns, c0, kThreads);
+      dy.template mask<ALIGNED>(columns, c0, kThreads);
+      h.template mask<ALIGNED>(columns, c0, kThreads);
+      take_weights<T, W, EP, ALIGNED>(a, columns, c0, kThreads, w);
+    };
+    F2 total(0.f, 0.f);
+    for (int c0 = at.tid; c0 < columns.pieces; c0 += round) {
+      take(c0);
+#pragma unroll
+      for (int k = 0; k < EP / 2; ++k) {
+        const F2 t = dy.get(k) * h.get(k);
+        total = fma2(t, w.get(k), total);
+        if (a.partial != nullptr) {
+          float f[2];
+          t.split(f[0], f[1]);
+#pragma unroll
+          for (int i = 2 * k; i < 2 * k + 2; ++i) {
+            const int col = columns.first(c0 + i / VE * kThreads) + i % VE;
+            if (col >= 0 && col < a.H) mine[col] = fmaf(f[i & 1], r, row == blockIdx.x ? 0.f : mine[col]);
           }
         }
       }
     }
     if (a.dx == nullptr) continue;
-    uint32_t none = 0u;
-    row_reduce<false>(sum, none, log2, part[turn], nullptr);
-    turn ^= 1;  // the next row's sums lie elsewhere: one barrier a row is enough
-    const float mean = sum * per_value;
-    for (int c0 = tid; c0 < (LONG ? all : tid + 1); c0 += P * tpr) {
-      if (LONG) {
-        take(row, c0);
-        take_weights(c0);
-      }
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const long long c = c0 + i * tpr;
-        Piece<T, VE> o;
-#pragma unroll
-        for (int j = 0; j < VE; ++j) {
-          const float g = r * (dy[i][j] * w[i][j] - (h[i][j] * r) * mean);
-          o.set(j, a.dh != nullptr ? dh[i][j] + g : g);
-        }
-        if (live && c < all) o.store(static_cast<T*>(a.dx) + row * a.H + c * VE);
-      }
+    float sum = total.sum(), none = 0.f;
+    row_reduce<false>(sum, none, at, part[turn]);
+    turn ^= 1;
+    for (int c0 = at.tid; c0 < columns.pieces; c0 += round) {
+      take(c0);
+      Values<T, EP, VE> dh, dx;
+      Columns<T, ALIGNED> upstream = columns;
+      if (a.dh == nullptr) upstream.pieces = 0;
+      dh.template load<ALIGNED, true>(static_cast<const T*>(a.dh) + row * a.dh_ld, upstream, c0, kThreads);
+      row_gradient(dy, h, w, dh, r, sum * r * a.per_value, dx);
+      dx.template store<ALIGNED>(static_cast<T*>(a.dx) + row * a.H, columns, c0, kThreads);
     }
-  }
-  if (a.partial == nullptr || LONG) return;
-  float* to = subs == 1 ? mine : sums + sub * a.H;
-#pragma unroll
-  for (int i = 0; i < P; ++i) {
-    const int c = tid + i * tpr;
-    if (c < all) {
-#pragma unroll
-      for (int j = 0; j < VE; ++j) to[c * VE + j] = acc[i * VE + j];
-    }
-  }
-  if (subs == 1) return;
-  __syncthreads();
-  for (int c = threadIdx.x; c < a.H; c += blockDim.x) {
-    float s = 0.f;
-    for (int k = 0; k < subs; ++k) s += sums[k * a.H + c];
-    mine[c] = s;
   }
 }
 
@@ -150,18 +187,44 @@ __global__ void __launch_bounds__(32 * kShares) weight_grad_kernel(const float* 
   }
 }
 
-template <class T, class W, int VE, int EP, bool LONG>
-static cudaError_t launch_backward(const Backward& a, int log2, int& blocks, cudaStream_t st) {
-  const int threads = log2 > 8 ? 1 << log2 : 256, subs = threads >> log2;
-  const long long need = (a.rows + subs - 1) / subs;
-  blocks = static_cast<int>(need < kMostBlocks ? need : kMostBlocks);
-  const size_t smem = subs > 1 ? static_cast<size_t>(subs) * a.H * sizeof(float) : 0;  // subs H <= 256 EP
-  return launch_chained(backward_kernel<T, W, VE, EP, LONG>, dim3(static_cast<unsigned>(blocks)), threads, smem, st, 1, a, log2);
+// Blocks of `kernel`: as many as the device holds at a time, at most one for each `subs` rows, and where rows have different shifts a multiple of
+// their number (8 or 4), unless no block has a second row; 0 on failure.
+template <class T, bool ALIGNED, class... Params>
+static int blocks_of(void (*kernel)(Params...), int threads, size_t smem, long long rows, int subs) {
+  const long long need = (rows + subs - 1) / subs;
+  const int sms = num_sms();
+  if (need <= sms) return static_cast<int>(need);
+  int per = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, threads, smem) != cudaSuccess || per <= 0 || sms <= 0) return 0;
+  long long all = static_cast<long long>(per) * sms;
+  if (all > kMostBlocks) all = kMostBlocks;
+  if (need <= all) return static_cast<int>(need);
+  return static_cast<int>(ALIGNED ? all : all / kValues<T> * kValues<T>);
 }
-template <class T, class W, int VE>
+
+template <class T, class W, int EP, bool ALIGNED, int REGISTERS>
+static cudaError_t launch_rows(const Backward& a, const Shape& s, int& blocks, cudaStream_t st) {
+  const size_t smem = s.subs > 1 ? static_cast<size_t>(s.subs) * a.H * sizeof(float) : 0;  // subs H <= 256 EP
+  blocks = blocks_of<T, ALIGNED>(backward_kernel<T, W, EP, ALIGNED, REGISTERS>, s.threads, smem, a.rows, s.subs);
+  if (blocks == 0) return cudaErrorInvalidConfiguration;
+  return launch_chained(backward_kernel<T, W, EP, ALIGNED, REGISTERS>, dim3(static_cast<unsigned>(blocks)), s.threads, smem, st, 1, a, s.tpr);
+}
+// Values of a thread, and its registers: fp32 rows 16 and 128 (with 80, 8192 x 4096 85.5 / 108 us); 16-bit rows of whole pieces 32 and 128, which
+// halves what every thread does for a row (32768 x 4096 with a residual, 32 / 16 values 171 / 179 us, 16384 x 7168 157 / 177, 16384 x 5000 98 / 116),
+// but short ones 16 and 80, three blocks to an SM (262144 x 128 40.0 / 36.5; 64 registers 39.8); other rows, whose pieces cost more registers, 16
+// up to 256 threads a row (20000 x 2049 126 / 96.5), 32 above (16384 x 7169 245 / 278).
+template <class T, class W, bool ALIGNED>
 static cudaError_t launch_backward(const Backward& a, int& blocks, cudaStream_t st) {
-  if (a.H <= 16 * kThreads) return launch_backward<T, W, VE, 16, false>(a, row_threads_log2(a.H, 16), blocks, st);
-  return launch_backward<T, W, VE, 16, true>(a, 9, blocks, st);
+  const long long values = a.H + (ALIGNED ? 0 : kValues<T> - 1);
+  if constexpr (sizeof(T) == 4) {
+    if (values <= 16 * kThreads) return launch_rows<T, W, 16, ALIGNED, 128>(a, shape_of(values, 16), blocks, st);
+  } else {
+    if (ALIGNED ? values < 256 : values <= 16 * 256) return launch_rows<T, W, 16, ALIGNED, 80>(a, shape_of(values, 16), blocks, st);
+    if (values <= 32 * kThreads) return launch_rows<T, W, 32, ALIGNED, 128>(a, shape_of(values, 32), blocks, st);
+  }
+  blocks = blocks_of<T, ALIGNED>(backward_long_kernel<T, W, 16, ALIGNED>, kThreads, 0, a.rows, 1);
+  if (blocks == 0) return cudaErrorInvalidConfiguration;
+  return launch_chained(backward_long_kernel<T, W, 16, ALIGNED>, dim3(static_cast<unsigned>(blocks)), kThreads, 0, st, 1, a);
 }
 
 }  // namespace norm
@@ -185,7 +248,7 @@ int smoe_rms_norm_backward(const void* dy, long long dy_ld, const void* dh, long
   if (rows < 0 || rows > 0x7fffffffll || H <= 0 || H > kMaxWidth || dy_ld < 0 || dh_ld < 0 || h_ld < 0) return SMOE_ERR_SHAPE;
   if (dx == nullptr && dweight == nullptr) return SMOE_ERR_SHAPE;
   if (rows > 0 && (dy == nullptr || h == nullptr || weight == nullptr || rstd == nullptr)) return SMOE_ERR_SHAPE;
-  if ((address(dy) | address(dh) | address(h) | address(dx)) % size != 0 || (address(weight) | address(dweight)) % wsize != 0 ||
+  if ((address(dy) | address(dh) | address(h)) % size != 0 || address(dx) % 16 != 0 || (address(weight) | address(dweight)) % wsize != 0 ||
       address(rstd) % 4 != 0 || address(workspace) % 16 != 0)
     return SMOE_ERR_ALIGNMENT;
   if (dweight != nullptr && rows > 0 && workspace == nullptr) return SMOE_ERR_WORKSPACE;
@@ -193,13 +256,14 @@ int smoe_rms_norm_backward(const void* dy, long long dy_ld, const void* dh, long
   a.dy = dy; a.dy_ld = dy_ld; a.dh = dh; a.dh_ld = dh != nullptr ? dh_ld : 0; a.h = h; a.h_ld = h_ld;
   a.w = weight; a.w_wide = address(weight) % 16 == 0;
   a.rstd = rstd; a.dx = dx; a.partial = dweight != nullptr ? static_cast<float*>(workspace) : nullptr;
-  a.rows = rows; a.H = H;
+  a.rows = rows; a.H = H; a.per_value = 1.f / static_cast<float>(H);
   int blocks = 0, kernels = 0;
   if (rows > 0) {
-    const int bytes = access_bytes({address(dy) | address(dh) | address(h) | address(dx), dy_ld * size, h_ld * size, a.dh_ld * size,
-                                    static_cast<long long>(H) * size});
+    const bool aligned = (address(dy) | address(dh) | address(h) | dy_ld * size | a.dh_ld * size | h_ld * size | static_cast<long long>(H) * size) % 16 == 0;
     const int rc = for_types(dtype, weight_dtype, [&](auto t, auto v) {
-      return launched(for_access<decltype(t)>(bytes, [&](auto ve) { return launch_backward<decltype(t), decltype(v), ve>(a, blocks, S(stream)); }), 0);
+      using T = decltype(t);
+      using W = decltype(v);
+      return launched(aligned ? launch_backward<T, W, true>(a, blocks, S(stream)) : launch_backward<T, W, false>(a, blocks, S(stream)), 0);
     });
     if (rc != SMOE_OK) return rc;
     ++kernels;

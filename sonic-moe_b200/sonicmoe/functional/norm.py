@@ -29,7 +29,7 @@ from .._lib import check, lib, ptr, stream_ptr
 from .int8 import MAX_COLS
 from .permutation import _ROW_TYPES
 
-_MAX_WIDTH = 2 ** 30
+_MAX_WIDTH = 2 ** 28
 
 
 def _as_rows(t: torch.Tensor) -> torch.Tensor:
