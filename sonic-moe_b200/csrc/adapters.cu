@@ -1,0 +1,759 @@
+// Low-rank adapters of many requests beside a shared projection: with e the adapter of token t,
+//   out[t] = base[t] + scale[e] b[e] (a[e] x[t]),   a (n, r, H), b (n, N, r);   out[t] = base[t] where t has none
+// (base NULL: zeros).  Tokens are sorted by adapter, e's rows starting at a multiple of `align` (smoe_token_permutation), so that a tile of 16
+// to `align` rows has one adapter.  x, base and out are met once each: between 20 and 200 operations for a byte of them, so that the products
+// go by mma.sync from registers and shared memory, whose rate they stay below, and memory bounds all of this.
+//
+// The inner product is fp32: every warp's part by the tensor core's fp32 sums, the parts added in the same order every time.  s = scale[e] (a x) goes on
+// as two 16-bit numbers, its leading bits and the rest (16 bits of s for bf16; 22 for fp16, after a row of s was multiplied by a power of two,
+// which keeps it in range), and the second product takes both: rounding s to 16 bits alone would make the error of out half as large
+// again where base is small.  out is rounded once.
+//
+// Two ways, of which `in_one_kernel` chooses:
+//   one kernel   a cluster of eight blocks has 16 rows; each block reads an eighth of the columns of x and a, the blocks add their parts over
+//                distributed shared memory, and each computes an eighth of the columns of out.  Weights go straight from memory to
+//                registers: this is for few tokens, or few to an adapter, where weights are everything and latency counts.
+//   two kernels  tiles of up to 128 rows, a warp for 16 of them, that share the weights in shared memory; s lies in memory in between.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "../../include/sonicmoe_b200.h"
+#include "launch.cuh"
+#include "ptx.cuh"
+
+namespace smoe {
+namespace adapters {
+
+constexpr int kMaxAdapters = 4096, kMaxRank = 128, kMaxRows = 0x7fff0000;
+constexpr int kCluster = 8, kWarps = 8;   // of the one kernel
+constexpr int kGroup = 32;                // columns of out that a warp has at a time
+
+struct Params {
+  const char* x; long long x_ld;          // distances in bytes
+  const char* a;
+  const char* b;
+  const float* scale;                     // (n) or nullptr
+  const char* base; long long base_ld;    // or nullptr
+  char* out; long long out_ld;
+  const int* off;                         // (n + 1) first row of each adapter, ascending
+  const int* gather;                      // (rows) token of each row
+  const int* reverse;                     // (T) row of each token
+  char* s;                                // two kernels: leading bits (rows, RP), the rest (rows, RP), factors (rows)
+  int T, rows, H, N, n, r;
+  int tiles;                              // of 16 rows, or of a block's
+  int splits;                             // two kernels: blocks that share the columns of x
+  int in_place;                           // out is base
+};
+
+// ----------------------------------------------------------------------------------------------
+// what the kernels share
+// ----------------------------------------------------------------------------------------------
+// c += a b: 16 rows of a, 8 columns of b, 16 products each.  Lane 4 g + t holds a[g][2t, 2t+1], a[g+8][..], a[g][2t+8, ..], a[g+8][..], b[2t, ..][g],
+// b[2t+8, ..][g] and c[g][2t, 2t+1], c[g+8][..].
+template <class T>
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Eight 16-bit values of a row from column `col` on (a multiple of 8), zeros behind its last column.  ALIGNED: rows start on 16-byte boundaries and
+// have whole eights.  Otherwise the one or two 16-byte blocks that hold them are loaded, none that holds nothing of the row.
+template <bool ALIGNED>
+__device__ __forceinline__ uint4 load8(const char* row, int col, int cols) {
+  if (col >= cols) return make_uint4(0u, 0u, 0u, 0u);
+  if (ALIGNED) return *reinterpret_cast<const uint4*>(row + 2ll * col);
+  const int o = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15);
+  const char* p = row + 2ll * col - o;
+  const uint4 q = *reinterpret_cast<const uint4*>(p);
+  uint4 r = make_uint4(0u, 0u, 0u, 0u);
+  if (o != 0 && 2 * (cols - col) + o > 16) r = *reinterpret_cast<const uint4*>(p + 16);
+  uint32_t v[8] = {q.x, q.y, q.z, q.w, r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 6; ++i) v[i] = o & 8 ? v[i + 2] : v[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) v[i] = o & 4 ? v[i + 1] : v[i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __funnelshift_r(v[i], v[i + 1], 8 * (o & 2));
+  const int left = cols - col;
+  if (left < 8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = left <= 2 * i ? 0u : left == 2 * i + 1 ? v[i] & 0xFFFFu : v[i];
+  }
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// The adapter of row `row` (all lanes of the warp): the last whose first row is not behind it.
+__device__ __forceinline__ int adapter_of(const Params& p, int row) {
+  const int lane = threadIdx.x & 31;
+  int count = 0;
+  for (int i = lane; i < p.n; i += 32) count += p.off[i] <= row;
+  count = static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(count)));
+  return min(max(count - 1, 0), p.n - 1);
+}
+// Whether rows from `row` on may have tokens.
+__device__ __forceinline__ bool within(const Params& p, int row) { return row < min(p.off[p.n], p.rows); }
+// The token of a row, or -1: a pair may have been dropped after the sort, in `reverse` alone.
+__device__ __forceinline__ int token_of(const Params& p, int row) {
+  if (row >= p.rows) return -1;
+  const int t = p.gather[row];
+  return static_cast<unsigned>(t) < static_cast<unsigned>(p.T) && p.reverse[t] == row ? t : -1;
+}
+
+// Rows of tokens that no tile writes (`tile` rows each): base, or zeros.  Warp `warp` of `warps`, all its lanes.
+__device__ __forceinline__ void copy_others(const Params& p, int tile, long long warp, long long warps) {
+  const int lane = threadIdx.x & 31;
+  const int end = min(p.off[p.n], p.rows);
+  for (long long t = warp; t < p.T; t += warps) {
+    const int row = p.reverse[t];
+    if (row >= 0 && row < p.rows && row / tile * tile < end && p.gather[row] == t) continue;
+    char* out = p.out + t * p.out_ld;
+    const char* base = p.base != nullptr ? p.base + t * p.base_ld : nullptr;
+    if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(base) | 2ull * p.N) % 16 == 0) {
+      for (int c = lane; c < p.N / 8; c += 32)
+        reinterpret_cast<uint4*>(out)[c] = base != nullptr ? reinterpret_cast<const uint4*>(base)[c] : make_uint4(0u, 0u, 0u, 0u);
+    } else {
+      for (int c = lane; c < p.N; c += 32)
+        reinterpret_cast<uint16_t*>(out)[c] = base != nullptr ? reinterpret_cast<const uint16_t*>(base)[c] : static_cast<uint16_t>(0);
+    }
+  }
+}
+
+// s as leading bits and the rest.  fp16: `factor` is a power of two that takes the row's largest |s| to 2^14; the product is multiplied by its inverse.
+template <class T>
+__device__ __forceinline__ float factor_of(float most) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return 1.f;
+  const int e = static_cast<int>(__float_as_uint(most) >> 23);  // exponent + 127; 255: infinity, NaN
+  if (e == 255 || most == 0.f) return 1.f;
+  return __int_as_float(min(127 + 14 + 127 - e, 253) << 23);
+}
+template <class T>
+__device__ __forceinline__ float inverse_of(float factor) {  // of a power of two
+  return __int_as_float((254 << 23) - __float_as_int(factor));
+}
+template <class T>
+__device__ __forceinline__ void split(float s, uint32_t& lead, uint32_t& rest) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const uint32_t bits = __float_as_uint(s);
+    lead = bits >> 16;  // cut, so that it stays finite
+    if ((bits & 0x7F800000u) == 0x7F800000u) {
+      if ((bits & 0x7FFFFFu) != 0u) lead |= 0x40u;  // NaN stays NaN
+      rest = 0u;
+    } else {
+      rest = __bfloat16_as_ushort(__float2bfloat16_rn(s - __uint_as_float(bits & 0xFFFF0000u)));
+    }
+  } else {
+    const __half h = __float2half_rn(s);
+    lead = __half_as_ushort(h);
+    rest = (lead & 0x7C00u) == 0x7C00u ? 0u : __half_as_ushort(__float2half_rn(s - __half2float(h)));
+  }
+}
+template <class T>
+__device__ __forceinline__ void split2(float x, float y, uint32_t& lead, uint32_t& rest) {
+  uint32_t l0, r0, l1, r1;
+  split<T>(x, l0, r0);
+  split<T>(y, l1, r1);
+  lead = l0 | l1 << 16;
+  rest = r0 | r1 << 16;
+}
+
+template <class T>
+__device__ __forceinline__ float2 unpack(uint32_t w) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <class T>
+__device__ __forceinline__ uint32_t pack(float x, float y) {
+  uint32_t w;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y), "f"(x));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y), "f"(x));
+  return w;
+}
+template <class T>
+__device__ __forceinline__ float value(uint16_t w) { return unpack<T>(w).x; }
+
+// The second product: 16 rows of s by columns n0 .. n0 + 31 of out.  Products are taken in an order that lets a lane load what lies together: of
+// RP = 16 columns of s, lane t of a quad has 4t .. 4t + 3 (one step), of 32 it has 8t .. 8t + 7 (two steps).  And column 8 (g / 2) + 2 j + g % 2 of out
+// is column g of product j, so that the four products give a lane the eight columns 8t .. 8t + 7 of out.
+template <int RP>
+struct Steps {
+  static constexpr int K = RP / 16;                     // steps of 16
+  static constexpr int L = RP == 16 ? 1 : RP / 32;      // loads of a lane for a row
+};
+// steps 2 l and 2 l + 1 (RP 16: step 0) of a product by one load `w` of a row of b
+template <class T, int RP>
+__device__ __forceinline__ void step(float (&c)[4], const uint32_t (&lead)[Steps<RP>::K][4], const uint32_t (&rest)[Steps<RP>::K][4], int l, uint4 w) {
+  constexpr int two = RP == 16 ? 1 : 2;
+#pragma unroll
+  for (int k = 0; k < two; ++k) {
+    const int i = two * l + k;
+    const uint32_t b0 = k == 0 ? w.x : w.z, b1 = k == 0 ? w.y : w.w;
+    mma<T>(c, lead[i][0], lead[i][1], lead[i][2], lead[i][3], b0, b1);
+    mma<T>(c, rest[i][0], rest[i][1], rest[i][2], rest[i][3], b0, b1);
+  }
+}
+__device__ __forceinline__ int out_column(int g, int j) { return 8 * (g >> 1) + 2 * j + (g & 1); }
+
+// base + c inverse for the rows of tokens t0 (g) and t1 (g + 8), columns n0 + 8 t ..; nothing for a token of -1.  ALIGNED: eight columns at a time,
+// else a warp's 16 rows one by one through `stage` (16 x 34 floats).
+template <class T>
+struct BaseRows {
+  uint4 v[2];
+  __device__ __forceinline__ void load(const Params& p, int n, int t0, int t1) {
+    v[0] = v[1] = make_uint4(0u, 0u, 0u, 0u);
+    if (p.base == nullptr || n >= p.N) return;
+    if (t0 >= 0) v[0] = __ldcs(reinterpret_cast<const uint4*>(p.base + t0 * p.base_ld + 2ll * n));
+    if (t1 >= 0) v[1] = __ldcs(reinterpret_cast<const uint4*>(p.base + t1 * p.base_ld + 2ll * n));
+  }
+};
+template <class T>
+__device__ __forceinline__ void put_row(const Params& p, int n, int t, const uint4& base, const float (&c)[4][4], int half, float inverse) {
+  if (t < 0 || n >= p.N) return;
+  const uint32_t b[4] = {base.x, base.y, base.z, base.w};
+  uint32_t o[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = unpack<T>(b[j]);
+    o[j] = pack<T>(fmaf(c[j][2 * half], inverse, f.x), fmaf(c[j][2 * half + 1], inverse, f.y));
+  }
+  __stcs(reinterpret_cast<uint4*>(p.out + t * p.out_ld + 2ll * n), make_uint4(o[0], o[1], o[2], o[3]));
+}
+constexpr int kStagePitch = 34;
+template <class T>
+__device__ __forceinline__ void put_staged(const Params& p, int n0, int tokens /* of row `lane` % 16 */, const float (&c)[4][4], float inverse0, float inverse1, float* stage) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    *reinterpret_cast<float2*>(stage + g * kStagePitch + 8 * t + 2 * j) = make_float2(c[j][0] * inverse0, c[j][1] * inverse0);
+    *reinterpret_cast<float2*>(stage + (g + 8) * kStagePitch + 8 * t + 2 * j) = make_float2(c[j][2] * inverse1, c[j][3] * inverse1);
+  }
+  __syncwarp();
+  const int n = n0 + lane;
+#pragma unroll 4
+  for (int row = 0; row < 16; ++row) {
+    const int token = __shfl_sync(0xffffffffu, tokens, row);
+    if (token < 0 || n >= p.N) continue;
+    float f = stage[row * kStagePitch + lane];
+    if (p.base != nullptr) f += value<T>(*reinterpret_cast<const uint16_t*>(p.base + token * p.base_ld + 2ll * n));
+    *reinterpret_cast<uint16_t*>(p.out + token * p.out_ld + 2ll * n) = static_cast<uint16_t>(pack<T>(f, 0.f));
+  }
+}
+
+// ----------------------------------------------------------------------------------------------
+// one kernel
+// ----------------------------------------------------------------------------------------------
+__device__ __forceinline__ float load_cluster(uint32_t addr) {
+  float f;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(addr) : "memory");
+  return f;
+}
+
+template <int RP>
+constexpr size_t one_smem() {  // warps' parts or staged rows, the block's part, s
+  return sizeof(float) * (kWarps * 16 * (RP > kStagePitch ? RP : kStagePitch) + 2 * 16 * RP);
+}
+
+template <class T, int RP, bool ALIGNED>
+__global__ void __launch_bounds__(32 * kWarps) one_kernel(const Params p) {
+  release_next();
+  wait_for_previous();
+  extern __shared__ __align__(16) float smem[];
+  float* parts = smem;                                                       // [warp][16][RP]
+  float* part = smem + kWarps * 16 * (RP > kStagePitch ? RP : kStagePitch);  // [16][RP]
+  float* s_all = part + 16 * RP;                                             // [16][RP]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int rank = static_cast<int>(cluster_ctarank()), tile = blockIdx.x / kCluster;
+  if (tile >= p.tiles) {
+    const long long first = static_cast<long long>(p.tiles) * kCluster;
+    copy_others(p, 16, (blockIdx.x - first) * kWarps + warp, (gridDim.x - first) * kWarps);
+    return;
+  }
+  const int row0 = 16 * tile;
+  if (!within(p, row0)) return;
+  const int tokens = token_of(p, row0 + (lane & 15));
+  if (__all_sync(0xffffffffu, tokens < 0)) return;  // (the cluster's blocks all see the same)
+  const int e = adapter_of(p, row0);
+  const int t0 = __shfl_sync(0xffffffffu, tokens, g), t1 = __shfl_sync(0xffffffffu, tokens, g + 8);
+  // this block's columns of out, and the L2 fetches the weights for them meanwhile
+  const int groups = (p.N + kGroup - 1) / kGroup;
+  const int n_first = static_cast<int>(static_cast<long long>(groups) * rank / kCluster), n_end = static_cast<int>(static_cast<long long>(groups) * (rank + 1) / kCluster);
+  const char* b = p.b + static_cast<long long>(e) * p.N * p.r * 2;
+  {
+    const long long first = static_cast<long long>(n_first) * kGroup * p.r * 2, end = min(static_cast<long long>(n_end) * kGroup, static_cast<long long>(p.N)) * p.r * 2;
+    for (long long o = first + 128ll * threadIdx.x; o < end; o += 128ll * blockDim.x) asm volatile("prefetch.global.L2 [%0];" ::"l"(b + o));
+  }
+  // a x over this warp's columns
+  constexpr int NT = RP / 8;
+  float acc[NT][4];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+  {
+    const int chunks = (p.H + 31) / 32, parts_of = kCluster * kWarps, mine = rank * kWarps + warp;
+    const int first = static_cast<int>(static_cast<long long>(chunks) * mine / parts_of), end = static_cast<int>(static_cast<long long>(chunks) * (mine + 1) / parts_of);
+    const char* x0 = p.x + t0 * p.x_ld;
+    const char* x1 = p.x + t1 * p.x_ld;
+    const char* a = p.a + static_cast<long long>(e) * p.r * p.H * 2;
+    constexpr int U = RP <= 32 ? 2 : 1;  // chunks whose loads are on their way together
+    for (int c = first; c < end; c += U) {
+      uint4 xa[U][2], w[U][NT];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int col = c + u < end ? 32 * (c + u) + 8 * t : p.H;
+        xa[u][0] = load8<ALIGNED>(x0, t0 >= 0 ? col : p.H, p.H);
+        xa[u][1] = load8<ALIGNED>(x1, t1 >= 0 ? col : p.H, p.H);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) w[u][j] = load8<ALIGNED>(a + (8ll * j + g) * p.H * 2, 8 * j + g < p.r ? col : p.H, p.H);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          mma<T>(acc[j], xa[u][0].x, xa[u][1].x, xa[u][0].y, xa[u][1].y, w[u][j].x, w[u][j].y);
+          mma<T>(acc[j], xa[u][0].z, xa[u][1].z, xa[u][0].w, xa[u][1].w, w[u][j].z, w[u][j].w);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    float* to = parts + (warp * 16 + g) * RP + 8 * j + 2 * t;
+    *reinterpret_cast<float2*>(to) = make_float2(acc[j][0], acc[j][1]);
+    *reinterpret_cast<float2*>(to + 8 * RP) = make_float2(acc[j][2], acc[j][3]);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * RP; i += 32 * kWarps) {
+    float f = parts[i];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) f += parts[w * 16 * RP + i];
+    part[i] = f;
+  }
+  cluster_sync_all();
+  const float scale = p.scale != nullptr ? p.scale[e] : 1.f;
+  for (int i = threadIdx.x; i < 16 * RP; i += 32 * kWarps) {
+    const uint32_t at = smem_u32(part + i);
+    float f[kCluster];
+#pragma unroll
+    for (int k = 0; k < kCluster; ++k) f[k] = load_cluster(map_to_cta(at, k));
+#pragma unroll
+    for (int k = 1; k < kCluster; ++k) f[0] += f[k];
+    s_all[i] = f[0] * scale;
+  }
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this block has read the others' parts
+  __syncthreads();
+  // s in this warp's registers
+  constexpr int K = Steps<RP>::K, L = Steps<RP>::L, V = RP == 16 ? 4 : 8;
+  uint32_t lead[K][4], rest[K][4];
+  float most0 = 0.f, most1 = 0.f;
+#pragma unroll
+  for (int l = 0; l < L; ++l) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      most0 = fmaxf(most0, fabsf(s_all[g * RP + 32 * l + V * t + i]));
+      most1 = fmaxf(most1, fabsf(s_all[(g + 8) * RP + 32 * l + V * t + i]));
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 4; o *= 2) {
+    most0 = fmaxf(most0, __shfl_xor_sync(0xffffffffu, most0, o));
+    most1 = fmaxf(most1, __shfl_xor_sync(0xffffffffu, most1, o));
+  }
+  const float f0 = factor_of<T>(most0), f1 = factor_of<T>(most1);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int col = RP == 16 ? 4 * t : 32 * (k / 2) + 8 * t + 4 * (k & 1);
+    const float4 u = *reinterpret_cast<const float4*>(s_all + g * RP + col), v = *reinterpret_cast<const float4*>(s_all + (g + 8) * RP + col);
+    split2<T>(u.x * f0, u.y * f0, lead[k][0], rest[k][0]);
+    split2<T>(v.x * f1, v.y * f1, lead[k][1], rest[k][1]);
+    split2<T>(u.z * f0, u.w * f0, lead[k][2], rest[k][2]);
+    split2<T>(v.z * f1, v.w * f1, lead[k][3], rest[k][3]);
+  }
+  const float i0 = inverse_of<T>(f0), i1 = inverse_of<T>(f1);
+  for (int group = n_first + warp; group < n_end; group += kWarps) {
+    const int n0 = kGroup * group;
+    BaseRows<T> base;
+    if (ALIGNED) base.load(p, n0 + 8 * t, t0, t1);
+    float c[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
+      const int n = n0 + out_column(g, j);
+      const char* row = b + static_cast<long long>(n) * p.r * 2;
+#pragma unroll
+      for (int l = 0; l < L; ++l) {
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (n < p.N) {
+          if constexpr (RP == 16) {
+            if (ALIGNED) {
+              if (4 * t < p.r) {
+                const uint2 h = *reinterpret_cast<const uint2*>(row + 8 * t);
+                w.x = h.x;
+                w.y = h.y;
+              }
+            } else {
+              const uint4 q = load8<false>(row, 8 * (t >> 1), p.r);
+              w.x = t & 1 ? q.z : q.x;
+              w.y = t & 1 ? q.w : q.y;
+            }
+          } else {
+            w = load8<ALIGNED>(row, 32 * l + 8 * t, p.r);
+          }
+        }
+        step<T, RP>(c[j], lead, rest, l, w);
+      }
+    }
+    if (ALIGNED) {
+      put_row<T>(p, n0 + 8 * t, t0, base.v[0], c, 0, i0);
+      put_row<T>(p, n0 + 8 * t, t1, base.v[1], c, 1, i1);
+    } else {
+      put_staged<T>(p, n0, tokens, c, i0, i1, parts + warp * 16 * kStagePitch);
+    }
+  }
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// ----------------------------------------------------------------------------------------------
+// two kernels
+// ----------------------------------------------------------------------------------------------
+// The first: s of a tile's rows.  A block has a share of the columns of x, its warps 16 rows each; x goes from memory to registers, a stage of
+// columns ahead, a through shared memory.  The blocks of a cluster add their parts, each for a share of the rows.
+template <int RP>
+struct First {
+  static constexpr int kCols = RP <= 64 ? 128 : 64;    // of a stage
+  static constexpr int kPitch = 2 * kCols + 64;        // of its rows: eight lanes of a load meet all banks
+  static constexpr int kStage = RP * kPitch;
+};
+template <int RP>
+static size_t first_smem(int tile) {
+  const size_t stages = 2 * First<RP>::kStage, part = sizeof(float) * tile * RP;
+  return stages > part ? stages : part;
+}
+
+template <class T, int RP, bool ALIGNED>
+__global__ void __launch_bounds__(256, RP <= 64 ? 2 : 1) first_kernel(const Params p) {
+  release_next();
+  wait_for_previous();
+  extern __shared__ __align__(16) char stages[];
+  constexpr int COLS = First<RP>::kCols, PITCH = First<RP>::kPitch, NT = RP / 8, C = COLS / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, tile_rows = blockDim.x / 2;
+  const int tile = blockIdx.x / p.splits, share = blockIdx.x - tile * p.splits;
+  const int row0 = tile * tile_rows;
+  if (!within(p, row0)) return;  // (the cluster's blocks all see the same)
+  const int e = adapter_of(p, row0);
+  const int tokens = token_of(p, row0 + 16 * warp + (lane & 15));
+  const int t0 = __shfl_sync(0xffffffffu, tokens, g), t1 = __shfl_sync(0xffffffffu, tokens, g + 8);
+  const bool any = __any_sync(0xffffffffu, tokens >= 0);
+  const char* x0 = p.x + t0 * p.x_ld;
+  const char* x1 = p.x + t1 * p.x_ld;
+  const char* a = p.a + static_cast<long long>(e) * p.r * p.H * 2;
+  const int all = (p.H + COLS - 1) / COLS;
+  const int first = static_cast<int>(static_cast<long long>(all) * share / p.splits), end = static_cast<int>(static_cast<long long>(all) * (share + 1) / p.splits);
+  const auto fetch_a = [&](int stage) {
+    if (stage >= end) return;
+    char* to = stages + (stage & 1) * First<RP>::kStage;
+    for (int i = threadIdx.x; i < RP * (COLS / 8); i += blockDim.x) {
+      const int row = i / (COLS / 8), k = i % (COLS / 8), col = COLS * stage + 8 * k;
+      const char* from = a + static_cast<long long>(row) * p.H * 2;
+      if (ALIGNED) cp_async16(smem_u32(to + row * PITCH + 16 * k), row < p.r && col < p.H ? from + 2ll * col : a, row < p.r && col < p.H ? 16 : 0);
+      else *reinterpret_cast<uint4*>(to + row * PITCH + 16 * k) = load8<false>(from, row < p.r ? col : p.H, p.H);
+    }
+  };
+  uint4 xa[C][2];
+  const auto fetch_x = [&](int stage, uint4 (&v)[C][2]) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int col = stage < end ? COLS * stage + 32 * c + 8 * t : p.H;
+      v[c][0] = load8<ALIGNED>(x0, t0 >= 0 ? col : p.H, p.H);
+      v[c][1] = load8<ALIGNED>(x1, t1 >= 0 ? col : p.H, p.H);
+    }
+  };
+  float acc[NT][4];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+  fetch_a(first);
+  fetch_x(first, xa);
+  for (int stage = first; stage < end; ++stage) {
+    cp_async_wait_all();
+    __syncthreads();  // the stage is there, and the other one has been read
+    fetch_a(stage + 1);
+    uint4 next[C][2];
+    fetch_x(stage + 1, next);
+    if (any) {
+      const char* from = stages + (stage & 1) * First<RP>::kStage + g * PITCH + 16 * t;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const uint4 w = *reinterpret_cast<const uint4*>(from + 8 * j * PITCH + 64 * c);
+          mma<T>(acc[j], xa[c][0].x, xa[c][1].x, xa[c][0].y, xa[c][1].y, w.x, w.y);
+          mma<T>(acc[j], xa[c][0].z, xa[c][1].z, xa[c][0].w, xa[c][1].w, w.z, w.w);
+        }
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      xa[c][0] = next[c][0];
+      xa[c][1] = next[c][1];
+    }
+  }
+  __syncthreads();
+  float* part = reinterpret_cast<float*>(stages);  // [tile_rows][RP]
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    float* to = part + (16 * warp + g) * RP + 8 * j + 2 * t;
+    *reinterpret_cast<float2*>(to) = make_float2(acc[j][0], acc[j][1]);
+    *reinterpret_cast<float2*>(to + 8 * RP) = make_float2(acc[j][2], acc[j][3]);
+  }
+  if (p.splits > 1) cluster_sync_all(); else __syncthreads();
+  // rows share * tile_rows / splits and on, four columns to a thread
+  const float scale = p.scale != nullptr ? p.scale[e] : 1.f;
+  constexpr int Q = RP / 4;
+  const int mine = tile_rows / p.splits, begin = share * mine;
+  uint2* lead = reinterpret_cast<uint2*>(p.s);
+  uint2* rest = lead + static_cast<long long>(p.rows) * Q;
+  float* factors = reinterpret_cast<float*>(rest + static_cast<long long>(p.rows) * Q);
+  for (int first_of = 0; first_of < mine * Q; first_of += blockDim.x) {  // (all threads, for the shuffles)
+    const int i = first_of + threadIdx.x;
+    const bool live = i < mine * Q;
+    const int row = begin + (live ? i / Q : 0), q = i % Q;
+    float f[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < p.splits; ++k) {
+      const uint32_t at = smem_u32(part + row * RP + 4 * q), from = p.splits > 1 ? map_to_cta(at, k) : at;
+      float v[4];
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(from) : "memory");
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] += v[j];
+    }
+    float most = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f[j] *= scale;
+      most = fmaxf(most, fabsf(f[j]));
+    }
+#pragma unroll
+    for (int o = 1; o < Q; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const float factor = factor_of<T>(most);
+    uint2 l, r;
+    split2<T>(f[0] * factor, f[1] * factor, l.x, r.x);
+    split2<T>(f[2] * factor, f[3] * factor, l.y, r.y);
+    const long long at = static_cast<long long>(row0 + row) * Q + q;
+    if (live && row0 + row < p.rows) {
+      lead[at] = l;
+      rest[at] = r;
+      if (q == 0) factors[row0 + row] = inverse_of<T>(factor);
+    }
+  }
+  if (p.splits > 1) cluster_sync_all();  // the others have read this block's part
+}
+
+// The second: a tile's rows by a share of the columns of out, whose weights the warps share in shared memory.
+constexpr int kShareCols = 256;
+template <int RP>
+struct Second {
+  static constexpr int kPitch = RP <= 32 ? 2 * RP : 2 * RP + 64;  // 64 bytes beyond a multiple of 128: as above
+  static constexpr size_t kSmem = kShareCols * kPitch;
+};
+
+template <class T, int RP, bool ALIGNED>
+__global__ void __launch_bounds__(256, RP <= 64 ? 2 : 1) second_kernel(const Params p) {
+  release_next();
+  wait_for_previous();
+  extern __shared__ __align__(16) char weights[];
+  constexpr int PITCH = Second<RP>::kPitch, K = Steps<RP>::K, L = Steps<RP>::L;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, tile_rows = blockDim.x / 2;
+  const int shares = (p.N + kShareCols - 1) / kShareCols;
+  const int tile = blockIdx.x / shares, n_first = (blockIdx.x - tile * shares) * kShareCols;
+  if (tile >= p.tiles) {
+    const long long first = static_cast<long long>(p.tiles) * shares, warps = blockDim.x / 32;
+    copy_others(p, tile_rows, (blockIdx.x - first) * warps + warp, (gridDim.x - first) * warps);
+    return;
+  }
+  const int row0 = tile * tile_rows;
+  if (!within(p, row0)) return;
+  const int e = adapter_of(p, row0);
+  const char* b = p.b + static_cast<long long>(e) * p.N * p.r * 2;
+  for (int i = threadIdx.x; i < kShareCols * (RP / 8); i += blockDim.x) {
+    const int row = i / (RP / 8), k = i % (RP / 8), n = n_first + row;
+    const bool in = n < p.N && 8 * k < p.r;
+    const char* from = b + static_cast<long long>(n) * p.r * 2;
+    if (ALIGNED) cp_async16(smem_u32(weights + row * PITCH + 16 * k), in ? from + 16 * k : b, in ? 16 : 0);
+    else *reinterpret_cast<uint4*>(weights + row * PITCH + 16 * k) = load8<false>(from, in ? 8 * k : p.r, p.r);
+  }
+  const int my_row = row0 + 16 * warp;
+  const int tokens = token_of(p, my_row + (lane & 15));
+  const int t0 = __shfl_sync(0xffffffffu, tokens, g), t1 = __shfl_sync(0xffffffffu, tokens, g + 8);
+  const bool any = __any_sync(0xffffffffu, tokens >= 0);
+  uint32_t lead[K][4], rest[K][4];
+  float i0 = 1.f, i1 = 1.f;
+  if (any) {  // (so the tile's rows are all there)
+    const uint2* sl = reinterpret_cast<const uint2*>(p.s);
+    const uint2* sr = sl + static_cast<long long>(p.rows) * (RP / 4);
+    const float* factors = reinterpret_cast<const float*>(sr + static_cast<long long>(p.rows) * (RP / 4));
+    const long long at0 = static_cast<long long>(my_row + g) * (RP / 4), at1 = at0 + 8ll * (RP / 4);
+    const bool both = my_row + g + 8 < p.rows, one = my_row + g < p.rows;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int q = RP == 16 ? t : 8 * (k / 2) + 2 * t + (k & 1);  // four columns each
+      const uint2 z = make_uint2(0u, 0u);
+      const uint2 u = one ? sl[at0 + q] : z, v = both ? sl[at1 + q] : z, ur = one ? sr[at0 + q] : z, vr = both ? sr[at1 + q] : z;
+      lead[k][0] = u.x; lead[k][1] = v.x; lead[k][2] = u.y; lead[k][3] = v.y;
+      rest[k][0] = ur.x; rest[k][1] = vr.x; rest[k][2] = ur.y; rest[k][3] = vr.y;
+    }
+    if (std::is_same<T, __half>::value) {
+      i0 = one ? factors[my_row + g] : 1.f;
+      i1 = both ? factors[my_row + g + 8] : 1.f;
+    }
+  }
+  const int groups = min(kShareCols, p.N - n_first + kGroup - 1) / kGroup;
+  BaseRows<T> base;
+  if (ALIGNED) base.load(p, n_first + 8 * t, t0, t1);
+  cp_async_wait_all();
+  __syncthreads();
+  if (!any) return;
+  __shared__ float staged[ALIGNED ? 1 : kWarps * 16 * kStagePitch];
+  for (int group = 0; group < groups; ++group) {
+    const int n0 = n_first + kGroup * group;
+    BaseRows<T> next;
+    if (ALIGNED) next.load(p, group + 1 < groups ? n0 + kGroup + 8 * t : p.N, t0, t1);
+    float c[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
+      const char* row = weights + (kGroup * group + out_column(g, j)) * PITCH;
+#pragma unroll
+      for (int l = 0; l < L; ++l) {
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (RP == 16) {
+          const uint2 h = *reinterpret_cast<const uint2*>(row + 8 * t);
+          w.x = h.x;
+          w.y = h.y;
+        } else {
+          w = *reinterpret_cast<const uint4*>(row + 64 * l + 16 * t);
+        }
+        step<T, RP>(c[j], lead, rest, l, w);
+      }
+    }
+    if (ALIGNED) {
+      put_row<T>(p, n0 + 8 * t, t0, base.v[0], c, 0, i0);
+      put_row<T>(p, n0 + 8 * t, t1, base.v[1], c, 1, i1);
+      base = next;
+    } else {
+      put_staged<T>(p, n0, tokens, c, i0, i1, staged + warp * 16 * kStagePitch);
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------------------------
+// launches
+// ----------------------------------------------------------------------------------------------
+static int padded_rank(int r) { return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : 128; }
+// Rows of a tile of the two kernels: 32, 64 or 128, or 0 where the sort aligns to less.
+static int tile_of(int align) { return align % 128 == 0 ? 128 : align % 64 == 0 ? 64 : align % 32 == 0 ? 32 : 0; }
+static bool in_one_kernel(int T, int align) { return T <= 256 || tile_of(align) == 0; }
+static size_t round256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+template <class T, int RP, bool ALIGNED>
+static int launch(Params p, int align, cudaStream_t st) {
+  static PerDeviceFlag configured;
+  const int dev = current_device();
+  if (dev < 0) return SMOE_ERR_DRIVER;
+  if (!configured.test(dev)) {
+    if (cudaFuncSetAttribute(one_kernel<T, RP, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(one_smem<RP>())) != cudaSuccess ||
+        cudaFuncSetAttribute(first_kernel<T, RP, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(first_smem<RP>(128))) != cudaSuccess ||
+        cudaFuncSetAttribute(second_kernel<T, RP, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Second<RP>::kSmem)) != cudaSuccess)
+      return SMOE_ERR_LAUNCH;
+    configured.set(dev);
+  }
+  if (in_one_kernel(p.T, align)) {
+    p.tiles = (p.rows + 15) / 16;
+    const long long others = p.in_place ? 0 : (p.T + 8ll * kCluster * kWarps - 1) / (8 * kCluster * kWarps);  // clusters, eight tokens to a warp
+    const long long blocks = (p.tiles + others) * kCluster;
+    if (blocks == 0) return SMOE_OK;
+    return launched(launch_chained(one_kernel<T, RP, ALIGNED>, dim3(static_cast<unsigned>(blocks)), 32 * kWarps, one_smem<RP>(), st, kCluster, p));
+  }
+  const int rows = tile_of(align), threads = 2 * rows;
+  p.tiles = (p.rows + rows - 1) / rows;
+  const int full = (p.T + rows - 1) / rows;
+  p.splits = full >= 148 ? 1 : full >= 74 ? 2 : full >= 37 ? 4 : 8;
+  int kernels = 0;
+  if (p.tiles > 0) {
+    const cudaError_t rc = launch_chained(first_kernel<T, RP, ALIGNED>, dim3(static_cast<unsigned>(p.tiles * p.splits)), threads, first_smem<RP>(rows), st, p.splits, p);
+    if (rc != cudaSuccess) return SMOE_ERR_LAUNCH;
+    ++kernels;
+  }
+  const int shares = (p.N + kShareCols - 1) / kShareCols, warps = threads / 32;
+  const long long others = p.in_place ? 0 : (p.T + 8ll * warps - 1) / (8 * warps);
+  const long long blocks = static_cast<long long>(p.tiles) * shares + others;
+  if (blocks == 0) return launched(cudaSuccess, kernels);
+  return launched(launch_chained(second_kernel<T, RP, ALIGNED>, dim3(static_cast<unsigned>(blocks)), threads, Second<RP>::kSmem, st, 1, p), kernels + 1);
+}
+template <class T, bool ALIGNED>
+static int launch(const Params& p, int align, cudaStream_t st) {
+  switch (padded_rank(p.r)) {
+    case 16: return launch<T, 16, ALIGNED>(p, align, st);
+    case 32: return launch<T, 32, ALIGNED>(p, align, st);
+    case 64: return launch<T, 64, ALIGNED>(p, align, st);
+    default: return launch<T, 128, ALIGNED>(p, align, st);
+  }
+}
+
+static long long address(const void* p) { return static_cast<long long>(reinterpret_cast<uintptr_t>(p)); }
+
+}  // namespace adapters
+}  // namespace smoe
+
+using namespace smoe;
+using namespace smoe::adapters;
+
+extern "C" {
+
+size_t smoe_adapter_linear_workspace_bytes(int T, long long rows, int r, int align) {
+  if (T <= 0 || rows <= 0 || r <= 0 || r > kMaxRank || align <= 0 || in_one_kernel(T, align)) return 0;
+  return round256(static_cast<size_t>(rows) * (4 * padded_rank(r) + 4));
+}
+
+int smoe_adapter_linear(const void* x, long long ld, const void* a, const void* b, const float* scale, const void* base, long long base_ld,
+                        void* out, long long out_ld, int dtype, const int* expert_frequency_offset, const int* x_gather_idx,
+                        const int* s_reverse_scatter_idx, int T, long long rows, int H, int N, int n, int r, int align, void* workspace,
+                        void* stream) {
+  if (dtype != SMOE_BF16 && dtype != SMOE_F16) return SMOE_ERR_DTYPE;
+  if (T < 0 || T > kMaxRows || rows < 0 || rows > kMaxRows || H <= 0 || N <= 0 || n <= 0 || n > kMaxAdapters || r <= 0 || r > kMaxRank || align <= 0 ||
+      align % 16 != 0 || ld < 0 || base_ld < 0 || out_ld < N)
+    return SMOE_ERR_SHAPE;
+  if (H > 1 << 28 || N > 1 << 28) return SMOE_ERR_SHAPE;
+  const int tile = in_one_kernel(T, align) ? 16 : tile_of(align);
+  // blocks: eight to 16 rows of one kernel, up to eight and one to 256 columns of two; and those of the other tokens
+  if (((rows + tile - 1) / tile + T / 8 + 1) * (8ll + (N + kShareCols - 1) / kShareCols) > 0x7fffffffll) return SMOE_ERR_SHAPE;
+  if (T == 0) return SMOE_OK;
+  if (x == nullptr || a == nullptr || b == nullptr || out == nullptr || expert_frequency_offset == nullptr || s_reverse_scatter_idx == nullptr ||
+      (rows > 0 && x_gather_idx == nullptr))
+    return SMOE_ERR_SHAPE;
+  const size_t ws = smoe_adapter_linear_workspace_bytes(T, rows, r, align);
+  if (ws > 0 && workspace == nullptr) return SMOE_ERR_WORKSPACE;
+  if ((address(x) | address(a) | address(b) | address(base) | address(out)) % 2 != 0 ||
+      (address(scale) | address(expert_frequency_offset) | address(x_gather_idx) | address(s_reverse_scatter_idx)) % 4 != 0 || address(workspace) % 256 != 0)
+    return SMOE_ERR_ALIGNMENT;
+  Params p = {};
+  p.x = static_cast<const char*>(x); p.x_ld = 2 * ld;
+  p.a = static_cast<const char*>(a); p.b = static_cast<const char*>(b); p.scale = scale;
+  p.base = static_cast<const char*>(base); p.base_ld = base != nullptr ? 2 * base_ld : 0;
+  p.out = static_cast<char*>(out); p.out_ld = 2 * out_ld;
+  p.off = expert_frequency_offset; p.gather = x_gather_idx; p.reverse = s_reverse_scatter_idx;
+  p.s = static_cast<char*>(workspace);
+  p.T = T; p.rows = static_cast<int>(rows); p.H = H; p.N = N; p.n = n; p.r = r;
+  p.in_place = base == out && base_ld == out_ld;
+  const bool aligned = (address(x) | address(a) | address(b) | address(base) | address(out) | p.x_ld | p.base_ld | p.out_ld) % 16 == 0 && H % 8 == 0 &&
+                       N % 8 == 0 && r % 8 == 0;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == SMOE_BF16) return aligned ? launch<__nv_bfloat16, true>(p, align, st) : launch<__nv_bfloat16, false>(p, align, st);
+  return aligned ? launch<__half, true>(p, align, st) : launch<__half, false>(p, align, st);
+}
+
+}  // extern "C"

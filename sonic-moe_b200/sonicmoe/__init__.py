@@ -6,6 +6,7 @@ Exports match the reference package (sonicmoe/__init__.py:5-8).
 from .count_cumsum import count_cumsum
 from .enums import ActivationType, KernelBackendMoE
 from .functional import enable_quack_gemm, moe_general_routing_inputs, moe_TC_softmax_topk_layer
+from .functional.adapters import adapter_linear, adapter_permutation
 from .functional.norm import NormedRows, rms_norm, rms_norm_quantize
 from .functional.permutation import TokenPermutation, permute_tokens, token_permutation, unpermute_tokens
 from .moe import MoE
@@ -31,4 +32,7 @@ __all__ = [
     "NormedRows",
     "rms_norm",
     "rms_norm_quantize",
+    # low-rank adapters of many requests beside a shared projection
+    "adapter_linear",
+    "adapter_permutation",
 ]

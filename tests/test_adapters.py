@@ -1,0 +1,68 @@
+"""The adapters' argument checks, which come before anything is launched (no GPU; the addresses here belong to nothing)."""
+
+import pytest
+import torch
+
+
+def test_refusals(built_library):
+    from sonicmoe._lib import lib
+
+    at = 4096
+
+    def call(x=at, ld=64, a=at, b=at, scale=None, base=None, base_ld=0, out=at, out_ld=32, dtype=1, off=at, gather=at, reverse=at, T=300,
+             rows=512, H=64, N=32, n=4, r=8, align=32, ws=at):
+        return lib.smoe_adapter_linear(x, ld, a, b, scale, base, base_ld, out, out_ld, dtype, off, gather, reverse, T, rows, H, N, n, r, align, ws, None)
+
+    assert call(dtype=0) == call(dtype=2) == -6
+    assert call(T=-1) == call(rows=-1) == call(H=0) == call(N=0) == call(n=0) == call(n=4097) == call(r=0) == call(r=129) == -1
+    assert call(align=0) == call(align=8) == call(align=-16) == call(align=40) == call(ld=-1) == call(out_ld=31) == call(base=at, base_ld=-1) == -1
+    assert call(H=2 ** 28 + 1) == call(N=2 ** 28 + 1, out_ld=2 ** 30) == call(rows=2 ** 31 - 2 ** 15) == call(T=2 ** 31 - 2 ** 15) == -1
+    assert call(x=None) == call(a=None) == call(b=None) == call(out=None) == call(off=None) == call(gather=None) == call(reverse=None) == -1
+    assert call(ws=None) == -7
+    assert call(x=at + 1) == call(a=at + 1) == call(b=at + 1) == call(out=at + 1) == call(base=at + 1) == -2
+    assert call(scale=at + 2) == call(off=at + 2) == call(gather=at + 2) == call(reverse=at + 2) == call(ws=at + 128) == -2
+    assert call(T=0) == 0
+    # more blocks than a grid has: 2^26 tiles of 32 rows by 2^20 shares of the columns
+    assert call(T=2 ** 30, rows=2 ** 31 - 2 ** 17, N=2 ** 28, out_ld=2 ** 28) == -1
+
+
+def test_workspace_bytes(built_library):
+    from sonicmoe._lib import lib
+
+    ws = lib.smoe_adapter_linear_workspace_bytes
+    assert ws(256, 4096, 16, 128) == 0 and ws(10000, 20000, 16, 16) == 0 and ws(10000, 20000, 16, 48) == 0  # one kernel
+    assert ws(0, 0, 16, 128) == 0 and ws(1000, 0, 16, 128) == 0
+    assert ws(257, 512, 16, 32) >= 512 * 68 and ws(257, 512, 100, 64) >= 512 * 516
+
+
+def test_python_refusals(built_library):
+    import sonicmoe
+    from sonicmoe import SonicMoEError
+
+    x, a, b = (torch.zeros(s, dtype=torch.bfloat16) for s in ((4, 64), (3, 8, 64), (3, 32, 8)))
+    p = sonicmoe.TokenPermutation(*[torch.zeros(n, dtype=torch.int32) for n in (3, 4, 64, 64)], torch.zeros(4, 1, dtype=torch.int32), 16)
+    with pytest.raises(SonicMoEError, match="no CPU path"):
+        sonicmoe.adapter_linear(x, a, b, p)
+    for bad in ((x[0], a, b), (x, a[0], b), (x, a, b[0])):
+        with pytest.raises(ValueError, match="has to be"):
+            sonicmoe.adapter_linear(*bad, p)
+    for bad in ((x[:, :32], a, b), (x, a[:2], b), (x, a[:, :4], b)):
+        with pytest.raises(ValueError, match="inconsistent"):
+            sonicmoe.adapter_linear(*bad, p)
+    for bad in ((x.float(), a.float(), b.float()), (x.half(), a, b), (x, a, b.half())):
+        with pytest.raises(TypeError, match="bf16 or fp16"):
+            sonicmoe.adapter_linear(*bad, p)
+    wide = torch.zeros(3, 129, 64, dtype=torch.bfloat16), torch.zeros(3, 32, 129, dtype=torch.bfloat16)
+    for bad in (wide, (a[:, :0], b[:, :, :0]), (a[:0], b[:0]), (a, b[:, :0])):
+        with pytest.raises(ValueError, match="are needed"):
+            sonicmoe.adapter_linear(x, *bad, p)
+    idx = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="has to be"):
+        sonicmoe.adapter_permutation(idx[None], 3)
+    for n in (0, 4097):
+        with pytest.raises(ValueError, match="are needed"):
+            sonicmoe.adapter_permutation(idx, n)
+    with pytest.raises(TypeError, match="int32 or int64"):
+        sonicmoe.adapter_permutation(idx.float(), 3)
+    with pytest.raises(SonicMoEError, match="no CPU path"):
+        sonicmoe.adapter_permutation(idx, 3)
