@@ -42,9 +42,9 @@ struct Params {
   const int* off;                         // (n + 1) first row of each adapter, ascending
   const int* gather;                      // (rows) token of each row
   const int* reverse;                     // (T) row of each token
-  char* s;                                // two kernels: leading bits (rows, RP), the rest (rows, RP), factors (rows)
+  char* s;                                // two kernels: `Between`
   int T, rows, H, N, n, r;
-  int tiles;                              // of 16 rows, or of a block's
+  int tiles;                              // of 16 rows, or of 128
   int splits;                             // two kernels: blocks that share the columns of x
   int in_place;                           // out is base
 };
@@ -64,6 +64,20 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// Eight 16-bit values that begin `o` bytes into v, at its beginning; those from the `left`-th on are zeros.
+__device__ __forceinline__ void shift_down(uint32_t (&v)[8], int o, int left) {
+#pragma unroll
+  for (int i = 0; i < 6; ++i) v[i] = o & 8 ? v[i + 2] : v[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) v[i] = o & 4 ? v[i + 1] : v[i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __funnelshift_r(v[i], v[i + 1], 8 * (o & 2));
+  if (left < 8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = left <= 2 * i ? 0u : left == 2 * i + 1 ? v[i] & 0xFFFFu : v[i];
+  }
+}
+
 // Eight 16-bit values of a row from column `col` on (a multiple of 8), zeros behind its last column.  ALIGNED: rows start on 16-byte boundaries and
 // have whole eights.  Otherwise the one or two 16-byte blocks that hold them are loaded, none that holds nothing of the row.
 template <bool ALIGNED>
@@ -76,17 +90,15 @@ __device__ __forceinline__ uint4 load8(const char* row, int col, int cols) {
   uint4 r = make_uint4(0u, 0u, 0u, 0u);
   if (o != 0 && 2 * (cols - col) + o > 16) r = *reinterpret_cast<const uint4*>(p + 16);
   uint32_t v[8] = {q.x, q.y, q.z, q.w, r.x, r.y, r.z, r.w};
-#pragma unroll
-  for (int i = 0; i < 6; ++i) v[i] = o & 8 ? v[i + 2] : v[i];
-#pragma unroll
-  for (int i = 0; i < 5; ++i) v[i] = o & 4 ? v[i + 1] : v[i];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = __funnelshift_r(v[i], v[i + 1], 8 * (o & 2));
-  const int left = cols - col;
-  if (left < 8) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = left <= 2 * i ? 0u : left == 2 * i + 1 ? v[i] & 0xFFFFu : v[i];
-  }
+  shift_down(v, o, cols - col);
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// The same from a copy of the row's 16-byte blocks: eight values `o` bytes behind `p`, of which `left` belong to the row.
+__device__ __forceinline__ uint4 in_place8(const char* p, int o, int left) {
+  const uint4 q = *reinterpret_cast<const uint4*>(p), r = *reinterpret_cast<const uint4*>(p + 16);
+  uint32_t v[8] = {q.x, q.y, q.z, q.w, r.x, r.y, r.z, r.w};
+  shift_down(v, o, left);
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
@@ -100,11 +112,15 @@ __device__ __forceinline__ int adapter_of(const Params& p, int row) {
 }
 // Whether rows from `row` on may have tokens.
 __device__ __forceinline__ bool within(const Params& p, int row) { return row < min(p.off[p.n], p.rows); }
-// The token of a row, or -1: a pair may have been dropped after the sort, in `reverse` alone.
-__device__ __forceinline__ int token_of(const Params& p, int row) {
+// The token of a row, or -1.  It is the row's if `reverse` says so too: a pair may have been dropped after the sort, in `reverse` alone.
+__device__ __forceinline__ int gathered_of(const Params& p, int row) {
   if (row >= p.rows) return -1;
   const int t = p.gather[row];
-  return static_cast<unsigned>(t) < static_cast<unsigned>(p.T) && p.reverse[t] == row ? t : -1;
+  return static_cast<unsigned>(t) < static_cast<unsigned>(p.T) ? t : -1;
+}
+__device__ __forceinline__ int token_of(const Params& p, int row) {
+  const int t = gathered_of(p, row);
+  return t >= 0 && p.reverse[t] == row ? t : -1;
 }
 
 // Rows of tokens that no tile writes (`tile` rows each): base, or zeros.  Warp `warp` of `warps`, all its lanes.
@@ -225,9 +241,20 @@ __device__ __forceinline__ void put_row(const Params& p, int n, int t, const uin
   }
   __stcs(reinterpret_cast<uint4*>(p.out + t * p.out_ld + 2ll * n), make_uint4(o[0], o[1], o[2], o[3]));
 }
+// Without whole pieces: a warp's 16 rows one by one, a column to a lane, by way of `stage` (16 x 34 floats).  Their base is fetched at once.
 constexpr int kStagePitch = 34;
+struct BaseColumn {
+  uint16_t v[16];
+  __device__ __forceinline__ void load(const Params& p, int n, int tokens /* of row `lane` % 16 */) {
+#pragma unroll
+    for (int row = 0; row < 16; ++row) {
+      const int token = __shfl_sync(0xffffffffu, tokens, row);
+      v[row] = p.base != nullptr && token >= 0 && n < p.N ? *reinterpret_cast<const uint16_t*>(p.base + token * p.base_ld + 2ll * n) : static_cast<uint16_t>(0);
+    }
+  }
+};
 template <class T>
-__device__ __forceinline__ void put_staged(const Params& p, int n0, int tokens /* of row `lane` % 16 */, const float (&c)[4][4], float inverse0, float inverse1, float* stage) {
+__device__ __forceinline__ void put_staged(const Params& p, int n0, int tokens, const BaseColumn& base, const float (&c)[4][4], float inverse0, float inverse1, float* stage) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   __syncwarp();
 #pragma unroll
@@ -237,13 +264,43 @@ __device__ __forceinline__ void put_staged(const Params& p, int n0, int tokens /
   }
   __syncwarp();
   const int n = n0 + lane;
-#pragma unroll 4
+#pragma unroll
   for (int row = 0; row < 16; ++row) {
     const int token = __shfl_sync(0xffffffffu, tokens, row);
-    if (token < 0 || n >= p.N) continue;
-    float f = stage[row * kStagePitch + lane];
-    if (p.base != nullptr) f += value<T>(*reinterpret_cast<const uint16_t*>(p.base + token * p.base_ld + 2ll * n));
-    *reinterpret_cast<uint16_t*>(p.out + token * p.out_ld + 2ll * n) = static_cast<uint16_t>(pack<T>(f, 0.f));
+    const float f = stage[row * kStagePitch + lane] + value<T>(base.v[row]);
+    if (token >= 0 && n < p.N) *reinterpret_cast<uint16_t*>(p.out + token * p.out_ld + 2ll * n) = static_cast<uint16_t>(pack<T>(f, 0.f));
+  }
+}
+
+// Four products with a row of b each, straight from memory: columns n0 .. n0 + 31 of out.
+template <class T, int RP, bool ALIGNED>
+__device__ __forceinline__ void direct_columns(const Params& p, const char* b, int n0, const uint32_t (&lead)[Steps<RP>::K][4], const uint32_t (&rest)[Steps<RP>::K][4], float (&c)[4][4]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
+    const int n = n0 + out_column(g, j);
+    const char* row = b + static_cast<long long>(n) * p.r * 2;
+#pragma unroll
+    for (int l = 0; l < Steps<RP>::L; ++l) {
+      uint4 w = make_uint4(0u, 0u, 0u, 0u);
+      if (n < p.N) {
+        if constexpr (RP > 16) {
+          w = load8<ALIGNED>(row, 32 * l + 8 * t, p.r);
+        } else if (ALIGNED) {
+          if (4 * t < p.r) {
+            const uint2 h = *reinterpret_cast<const uint2*>(row + 8 * t);
+            w.x = h.x;
+            w.y = h.y;
+          }
+        } else {
+          const uint4 q = load8<false>(row, 8 * (t >> 1), p.r);
+          w.x = t & 1 ? q.z : q.x;
+          w.y = t & 1 ? q.w : q.y;
+        }
+      }
+      step<T, RP>(c[j], lead, rest, l, w);
+    }
   }
 }
 
@@ -278,10 +335,12 @@ __global__ void __launch_bounds__(32 * kWarps) one_kernel(const Params p) {
   }
   const int row0 = 16 * tile;
   if (!within(p, row0)) return;
-  const int tokens = token_of(p, row0 + (lane & 15));
-  if (__all_sync(0xffffffffu, tokens < 0)) return;  // (the cluster's blocks all see the same)
+  // what is read of a token does not wait for the check that the row is still its own
+  const int gathered = gathered_of(p, row0 + (lane & 15));
+  if (__all_sync(0xffffffffu, gathered < 0)) return;  // (the cluster's blocks all see the same)
+  const int row_of = gathered >= 0 ? p.reverse[gathered] : -1;
   const int e = adapter_of(p, row0);
-  const int t0 = __shfl_sync(0xffffffffu, tokens, g), t1 = __shfl_sync(0xffffffffu, tokens, g + 8);
+  const int x_t0 = __shfl_sync(0xffffffffu, gathered, g), x_t1 = __shfl_sync(0xffffffffu, gathered, g + 8);
   // this block's columns of out, and the L2 fetches the weights for them meanwhile
   const int groups = (p.N + kGroup - 1) / kGroup;
   const int n_first = static_cast<int>(static_cast<long long>(groups) * rank / kCluster), n_end = static_cast<int>(static_cast<long long>(groups) * (rank + 1) / kCluster);
@@ -298,8 +357,8 @@ __global__ void __launch_bounds__(32 * kWarps) one_kernel(const Params p) {
   {
     const int chunks = (p.H + 31) / 32, parts_of = kCluster * kWarps, mine = rank * kWarps + warp;
     const int first = static_cast<int>(static_cast<long long>(chunks) * mine / parts_of), end = static_cast<int>(static_cast<long long>(chunks) * (mine + 1) / parts_of);
-    const char* x0 = p.x + t0 * p.x_ld;
-    const char* x1 = p.x + t1 * p.x_ld;
+    const char* x0 = p.x + x_t0 * p.x_ld;
+    const char* x1 = p.x + x_t1 * p.x_ld;
     const char* a = p.a + static_cast<long long>(e) * p.r * p.H * 2;
     constexpr int U = RP <= 32 ? 2 : 1;  // chunks whose loads are on their way together
     for (int c = first; c < end; c += U) {
@@ -307,8 +366,8 @@ __global__ void __launch_bounds__(32 * kWarps) one_kernel(const Params p) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int col = c + u < end ? 32 * (c + u) + 8 * t : p.H;
-        xa[u][0] = load8<ALIGNED>(x0, t0 >= 0 ? col : p.H, p.H);
-        xa[u][1] = load8<ALIGNED>(x1, t1 >= 0 ? col : p.H, p.H);
+        xa[u][0] = load8<ALIGNED>(x0, x_t0 >= 0 ? col : p.H, p.H);
+        xa[u][1] = load8<ALIGNED>(x1, x_t1 >= 0 ? col : p.H, p.H);
 #pragma unroll
         for (int j = 0; j < NT; ++j) w[u][j] = load8<ALIGNED>(a + (8ll * j + g) * p.H * 2, 8 * j + g < p.r ? col : p.H, p.H);
       }
@@ -376,44 +435,22 @@ __global__ void __launch_bounds__(32 * kWarps) one_kernel(const Params p) {
     split2<T>(v.z * f1, v.w * f1, lead[k][3], rest[k][3]);
   }
   const float i0 = inverse_of<T>(f0), i1 = inverse_of<T>(f1);
+  const int tokens = row_of == row0 + (lane & 15) ? gathered : -1;
+  const int t0 = __shfl_sync(0xffffffffu, tokens, g), t1 = __shfl_sync(0xffffffffu, tokens, g + 8);
   for (int group = n_first + warp; group < n_end; group += kWarps) {
     const int n0 = kGroup * group;
-    BaseRows<T> base;
-    if (ALIGNED) base.load(p, n0 + 8 * t, t0, t1);
     float c[4][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
-      const int n = n0 + out_column(g, j);
-      const char* row = b + static_cast<long long>(n) * p.r * 2;
-#pragma unroll
-      for (int l = 0; l < L; ++l) {
-        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (n < p.N) {
-          if constexpr (RP == 16) {
-            if (ALIGNED) {
-              if (4 * t < p.r) {
-                const uint2 h = *reinterpret_cast<const uint2*>(row + 8 * t);
-                w.x = h.x;
-                w.y = h.y;
-              }
-            } else {
-              const uint4 q = load8<false>(row, 8 * (t >> 1), p.r);
-              w.x = t & 1 ? q.z : q.x;
-              w.y = t & 1 ? q.w : q.y;
-            }
-          } else {
-            w = load8<ALIGNED>(row, 32 * l + 8 * t, p.r);
-          }
-        }
-        step<T, RP>(c[j], lead, rest, l, w);
-      }
-    }
     if (ALIGNED) {
+      BaseRows<T> base;
+      base.load(p, n0 + 8 * t, t0, t1);
+      direct_columns<T, RP, ALIGNED>(p, b, n0, lead, rest, c);
       put_row<T>(p, n0 + 8 * t, t0, base.v[0], c, 0, i0);
       put_row<T>(p, n0 + 8 * t, t1, base.v[1], c, 1, i1);
     } else {
-      put_staged<T>(p, n0, tokens, c, i0, i1, parts + warp * 16 * kStagePitch);
+      BaseColumn base;
+      base.load(p, n0 + lane, tokens);
+      direct_columns<T, RP, ALIGNED>(p, b, n0, lead, rest, c);
+      put_staged<T>(p, n0, tokens, base, c, i0, i1, parts + warp * 16 * kStagePitch);
     }
   }
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -422,89 +459,173 @@ __global__ void __launch_bounds__(32 * kWarps) one_kernel(const Params p) {
 // ----------------------------------------------------------------------------------------------
 // two kernels
 // ----------------------------------------------------------------------------------------------
-// The first: s of a tile's rows.  A block has a share of the columns of x, its warps 16 rows each; x goes from memory to registers, a stage of
-// columns ahead, a through shared memory.  The blocks of a cluster add their parts, each for a share of the rows.
+// A block has 128 rows, each of its eight warps 16 of them, which have one adapter.  As the rows are sorted most blocks have one adapter too, whose
+// weights the warps share in shared memory; in the others each warp reads its own.
+constexpr int kTileRows = 16 * kWarps;
+
+// What the first kernel leaves to the second one in the workspace.
 template <int RP>
-struct First {
-  static constexpr int kCols = RP <= 64 ? 128 : 64;    // of a stage
-  static constexpr int kPitch = 2 * kCols + 64;        // of its rows: eight lanes of a load meet all banks
-  static constexpr int kStage = RP * kPitch;
+struct Between {
+  char* lead;      // (rows, RP) 16-bit
+  char* rest;      // (rows, RP)
+  float* inverse;  // (rows)
+  int* token;      // (rows), -1: none
+  int* adapter;    // (rows / 16), -1: no tokens
+  __device__ __forceinline__ explicit Between(const Params& p) {
+    const long long rows = p.tiles * static_cast<long long>(kTileRows);
+    lead = p.s;
+    rest = lead + rows * 2 * RP;
+    inverse = reinterpret_cast<float*>(rest + rows * 2 * RP);
+    token = reinterpret_cast<int*>(inverse + rows);
+    adapter = token + rows;
+  }
 };
-template <int RP>
-static size_t first_smem(int tile) {
-  const size_t stages = 2 * First<RP>::kStage, part = sizeof(float) * tile * RP;
-  return stages > part ? stages : part;
+static size_t between_bytes(long long rows, int rp) {
+  const long long padded = (rows + kTileRows - 1) / kTileRows * kTileRows;
+  return static_cast<size_t>(padded) * (4 * rp + 8) + static_cast<size_t>(padded / 16) * 4;
 }
 
+// The first: s of a block's rows over a share of the columns of x.  Every warp brings in its own rows of x, the block a, 64 columns in a stage and
+// kAhead stages ahead.  The blocks of a cluster add their parts, each for a share of the rows.  Rows of x that start anywhere come in by the
+// 16-byte blocks that hold them, and are put in place on the way out of shared memory; a is on the way in.
+template <int RP, bool ALIGNED>
+struct First {
+  static constexpr int kCols = 64, kStages = 3;
+  static constexpr int kPitch = ALIGNED ? 128 : 192;  // of a row of x; 128: the odd rows' halves trade places, so that eight lanes meet all banks
+  static constexpr int kWarpBytes = 16 * kPitch, kXBytes = kWarps * kWarpBytes, kABytes = RP * 128;
+  static constexpr size_t kStaging = kStages * static_cast<size_t>(kXBytes + kABytes), kPart = sizeof(float) * kTileRows * RP;
+  static constexpr size_t kSmem = kStaging > kPart ? kStaging : kPart;
+};
+// place of the 16-byte block `k` of row `row` in a row of 128 bytes
+__device__ __forceinline__ int swizzled(int row, int k) { return 16 * (k ^ ((row & 1) << 2)); }
+
 template <class T, int RP, bool ALIGNED>
-__global__ void __launch_bounds__(256, RP <= 64 ? 2 : 1) first_kernel(const Params p) {
+__global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) first_kernel(const Params p) {
   release_next();
   wait_for_previous();
-  extern __shared__ __align__(16) char stages[];
-  constexpr int COLS = First<RP>::kCols, PITCH = First<RP>::kPitch, NT = RP / 8, C = COLS / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, tile_rows = blockDim.x / 2;
+  using F = First<RP, ALIGNED>;
+  extern __shared__ __align__(128) char staging[];
+  constexpr int COLS = F::kCols, STAGES = F::kStages, NT = RP / 8, C = COLS / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int tile = blockIdx.x / p.splits, share = blockIdx.x - tile * p.splits;
-  const int row0 = tile * tile_rows;
-  if (!within(p, row0)) return;  // (the cluster's blocks all see the same)
-  const int e = adapter_of(p, row0);
-  const int tokens = token_of(p, row0 + 16 * warp + (lane & 15));
-  const int t0 = __shfl_sync(0xffffffffu, tokens, g), t1 = __shfl_sync(0xffffffffu, tokens, g + 8);
-  const bool any = __any_sync(0xffffffffu, tokens >= 0);
-  const char* x0 = p.x + t0 * p.x_ld;
-  const char* x1 = p.x + t1 * p.x_ld;
-  const char* a = p.a + static_cast<long long>(e) * p.r * p.H * 2;
+  const int row0 = tile * kTileRows, my_row = row0 + 16 * warp;
+  __shared__ int adapters[kWarps];
+  const bool in = within(p, my_row);
+  const int gathered = in ? gathered_of(p, my_row + (lane & 15)) : -1;
+  const bool any = __any_sync(0xffffffffu, gathered >= 0);
+  const int row_of = gathered >= 0 ? p.reverse[gathered] : -1;
+  const int e = any ? adapter_of(p, my_row) : -1;
+  if (lane == 0) adapters[warp] = e;
+  __syncthreads();
+  int shared_e = -1;
+  bool mixed = false;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const int other = adapters[w];
+    mixed |= other >= 0 && shared_e >= 0 && other != shared_e;
+    shared_e = other >= 0 ? other : shared_e;
+  }
+  const Between<RP> between(p);
+  if (share == 0) {
+    if (lane < 16) between.token[my_row + lane] = row_of == my_row + lane ? gathered : -1;
+    if (lane == 0) between.adapter[my_row / 16] = e;
+  }
+  if (shared_e < 0) return;  // (the cluster's blocks all see the same)
+  const int t0 = __shfl_sync(0xffffffffu, gathered, g), t1 = __shfl_sync(0xffffffffu, gathered, g + 8);
+  const char* a = p.a + static_cast<long long>(mixed ? e : shared_e) * p.r * p.H * 2;
   const int all = (p.H + COLS - 1) / COLS;
   const int first = static_cast<int>(static_cast<long long>(all) * share / p.splits), end = static_cast<int>(static_cast<long long>(all) * (share + 1) / p.splits);
-  const auto fetch_a = [&](int stage) {
-    if (stage >= end) return;
-    char* to = stages + (stage & 1) * First<RP>::kStage;
-    for (int i = threadIdx.x; i < RP * (COLS / 8); i += blockDim.x) {
-      const int row = i / (COLS / 8), k = i % (COLS / 8), col = COLS * stage + 8 * k;
-      const char* from = a + static_cast<long long>(row) * p.H * 2;
-      if (ALIGNED) cp_async16(smem_u32(to + row * PITCH + 16 * k), row < p.r && col < p.H ? from + 2ll * col : a, row < p.r && col < p.H ? 16 : 0);
-      else *reinterpret_cast<uint4*>(to + row * PITCH + 16 * k) = load8<false>(from, row < p.r ? col : p.H, p.H);
+  const auto x_stage = [&](int stage) { return staging + stage % STAGES * (F::kXBytes + F::kABytes) + warp * F::kWarpBytes; };
+  const auto a_stage = [&](int stage) { return staging + stage % STAGES * (F::kXBytes + F::kABytes) + F::kXBytes; };
+  // rows lane / 8, + 4, + 8, + 12 of this warp, block lane % 8 of each
+  const char* x_row[4];
+  int x_off[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int token = __shfl_sync(0xffffffffu, gathered, (lane >> 3) + 4 * i);
+    const char* row = token >= 0 ? p.x + token * p.x_ld : nullptr;
+    x_off[i] = ALIGNED ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15);
+    x_row[i] = token >= 0 ? row - x_off[i] : nullptr;
+  }
+  const auto fetch_x = [&](int stage) {
+    char* to = x_stage(stage);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = (lane >> 3) + 4 * i, k = lane & 7;
+      const long long at = 2ll * COLS * stage + 16 * k;  // behind x_row
+      const long long bytes = x_off[i] + 2ll * p.H;      // of the row, from x_row on
+      const bool has = x_row[i] != nullptr && at < bytes;
+      if (ALIGNED) {
+        cp_async16(smem_u32(to + row * F::kPitch + swizzled(row, k)), has ? x_row[i] + at : p.x, has ? 16 : 0);
+      } else {
+        cp_async16(smem_u32(to + row * F::kPitch + 16 * k), has ? x_row[i] + at : p.a - (reinterpret_cast<uintptr_t>(p.a) & 15), has ? 16 : 0);
+        if (k == 0) {  // the ninth block
+          const bool more = x_row[i] != nullptr && at + 128 < bytes;
+          cp_async16(smem_u32(to + row * F::kPitch + 128), more ? x_row[i] + at + 128 : p.a - (reinterpret_cast<uintptr_t>(p.a) & 15), more ? 16 : 0);
+        }
+      }
     }
   };
-  uint4 xa[C][2];
-  const auto fetch_x = [&](int stage, uint4 (&v)[C][2]) {
+  constexpr int A_LOADS = RP * 8 / (32 * kWarps) > 0 ? RP * 8 / (32 * kWarps) : 1;
+  const auto fetch_a = [&](int stage) {
+    if (mixed || stage >= end) return;
+    char* to = a_stage(stage);
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const int col = stage < end ? COLS * stage + 32 * c + 8 * t : p.H;
-      v[c][0] = load8<ALIGNED>(x0, t0 >= 0 ? col : p.H, p.H);
-      v[c][1] = load8<ALIGNED>(x1, t1 >= 0 ? col : p.H, p.H);
+    for (int i = 0; i < A_LOADS; ++i) {
+      const int at = threadIdx.x + 32 * kWarps * i, row = at >> 3, k = at & 7, col = COLS * stage + 8 * k;
+      if (row >= RP) continue;
+      const char* from = a + static_cast<long long>(row) * p.H * 2;
+      const bool has = row < p.r && col < p.H;
+      if (ALIGNED) cp_async16(smem_u32(to + 128 * row + swizzled(row, k)), has ? from + 2ll * col : p.a, has ? 16 : 0);
+      else *reinterpret_cast<uint4*>(to + 128 * row + swizzled(row, k)) = load8<false>(from, has ? col : p.H, p.H);
     }
   };
   float acc[NT][4];
 #pragma unroll
   for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-  fetch_a(first);
-  fetch_x(first, xa);
+  const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) {
+    if (any && first + i < end) fetch_x(first + i);
+    fetch_a(first + i);
+    commit();
+  }
+  // where this lane's rows of x begin in their blocks
+  const int o0 = ALIGNED || t0 < 0 ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(p.x + t0 * p.x_ld) & 15);
+  const int o1 = ALIGNED || t1 < 0 ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(p.x + t1 * p.x_ld) & 15);
   for (int stage = first; stage < end; ++stage) {
-    cp_async_wait_all();
-    __syncthreads();  // the stage is there, and the other one has been read
-    fetch_a(stage + 1);
-    uint4 next[C][2];
-    fetch_x(stage + 1, next);
-    if (any) {
-      const char* from = stages + (stage & 1) * First<RP>::kStage + g * PITCH + 16 * t;
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const uint4 w = *reinterpret_cast<const uint4*>(from + 8 * j * PITCH + 64 * c);
-          mma<T>(acc[j], xa[c][0].x, xa[c][1].x, xa[c][0].y, xa[c][1].y, w.x, w.y);
-          mma<T>(acc[j], xa[c][0].z, xa[c][1].z, xa[c][0].w, xa[c][1].w, w.z, w.w);
-        }
-      }
-    }
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    __syncthreads();  // the stage is there for all, and the one that comes next into its place has been read
+    if (any && stage + STAGES - 1 < end) fetch_x(stage + STAGES - 1);
+    fetch_a(stage + STAGES - 1);
+    commit();
+    if (!any) continue;
+    const char* x = x_stage(stage);
+    const char* w_from = a_stage(stage);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      xa[c][0] = next[c][0];
-      xa[c][1] = next[c][1];
+      uint4 x0, x1;
+      if (ALIGNED) {
+        x0 = *reinterpret_cast<const uint4*>(x + g * F::kPitch + swizzled(g, 4 * c + t));
+        x1 = *reinterpret_cast<const uint4*>(x + (g + 8) * F::kPitch + swizzled(g, 4 * c + t));
+      } else {
+        const int left = p.H - (COLS * stage + 32 * c + 8 * t);
+        x0 = in_place8(x + g * F::kPitch + 16 * (4 * c + t), o0, left);
+        x1 = in_place8(x + (g + 8) * F::kPitch + 16 * (4 * c + t), o1, left);
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        uint4 w;
+        if (mixed) w = load8<ALIGNED>(a + (8ll * j + g) * p.H * 2, 8 * j + g < p.r ? COLS * stage + 32 * c + 8 * t : p.H, p.H);
+        else w = *reinterpret_cast<const uint4*>(w_from + 128 * (8 * j + g) + swizzled(g, 4 * c + t));
+        mma<T>(acc[j], x0.x, x1.x, x0.y, x1.y, w.x, w.y);
+        mma<T>(acc[j], x0.z, x1.z, x0.w, x1.w, w.z, w.w);
+      }
     }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
-  float* part = reinterpret_cast<float*>(stages);  // [tile_rows][RP]
+  float* part = reinterpret_cast<float*>(staging);  // [kTileRows][RP]
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     float* to = part + (16 * warp + g) * RP + 8 * j + 2 * t;
@@ -512,17 +633,14 @@ __global__ void __launch_bounds__(256, RP <= 64 ? 2 : 1) first_kernel(const Para
     *reinterpret_cast<float2*>(to + 8 * RP) = make_float2(acc[j][2], acc[j][3]);
   }
   if (p.splits > 1) cluster_sync_all(); else __syncthreads();
-  // rows share * tile_rows / splits and on, four columns to a thread
-  const float scale = p.scale != nullptr ? p.scale[e] : 1.f;
+  // rows share * kTileRows / splits and on, four columns to a thread
   constexpr int Q = RP / 4;
-  const int mine = tile_rows / p.splits, begin = share * mine;
-  uint2* lead = reinterpret_cast<uint2*>(p.s);
-  uint2* rest = lead + static_cast<long long>(p.rows) * Q;
-  float* factors = reinterpret_cast<float*>(rest + static_cast<long long>(p.rows) * Q);
-  for (int first_of = 0; first_of < mine * Q; first_of += blockDim.x) {  // (all threads, for the shuffles)
-    const int i = first_of + threadIdx.x;
-    const bool live = i < mine * Q;
-    const int row = begin + (live ? i / Q : 0), q = i % Q;
+  const int mine = kTileRows / p.splits, begin = share * mine;
+  uint2* lead = reinterpret_cast<uint2*>(between.lead);
+  uint2* rest = reinterpret_cast<uint2*>(between.rest);
+  for (int i = threadIdx.x; i < mine * Q; i += blockDim.x) {  // (16 rows of at least four columns' threads for a warp: all lanes of it)
+    const int row = begin + i / Q, q = i % Q, of = adapters[row / 16];
+    const float scale = p.scale != nullptr && of >= 0 ? p.scale[of] : 1.f;
     float f[4] = {0.f, 0.f, 0.f, 0.f};
     for (int k = 0; k < p.splits; ++k) {
       const uint32_t at = smem_u32(part + row * RP + 4 * q), from = p.splits > 1 ? map_to_cta(at, k) : at;
@@ -544,108 +662,118 @@ __global__ void __launch_bounds__(256, RP <= 64 ? 2 : 1) first_kernel(const Para
     split2<T>(f[0] * factor, f[1] * factor, l.x, r.x);
     split2<T>(f[2] * factor, f[3] * factor, l.y, r.y);
     const long long at = static_cast<long long>(row0 + row) * Q + q;
-    if (live && row0 + row < p.rows) {
-      lead[at] = l;
-      rest[at] = r;
-      if (q == 0) factors[row0 + row] = inverse_of<T>(factor);
-    }
+    lead[at] = l;
+    rest[at] = r;
+    if (q == 0) between.inverse[row0 + row] = inverse_of<T>(factor);
   }
   if (p.splits > 1) cluster_sync_all();  // the others have read this block's part
 }
 
-// The second: a tile's rows by a share of the columns of out, whose weights the warps share in shared memory.
+// The second: a block's rows by a share of the columns of out.
 constexpr int kShareCols = 256;
 template <int RP>
 struct Second {
-  static constexpr int kPitch = RP <= 32 ? 2 * RP : 2 * RP + 64;  // 64 bytes beyond a multiple of 128: as above
+  static constexpr int kPitch = RP <= 32 ? 2 * RP : 2 * RP + 64;  // 64 bytes beyond a multiple of 128, so that eight lanes of a load meet all banks
   static constexpr size_t kSmem = kShareCols * kPitch;
 };
 
 template <class T, int RP, bool ALIGNED>
-__global__ void __launch_bounds__(256, RP <= 64 ? 2 : 1) second_kernel(const Params p) {
+__global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) second_kernel(const Params p) {
   release_next();
   wait_for_previous();
   extern __shared__ __align__(16) char weights[];
   constexpr int PITCH = Second<RP>::kPitch, K = Steps<RP>::K, L = Steps<RP>::L;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, tile_rows = blockDim.x / 2;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int shares = (p.N + kShareCols - 1) / kShareCols;
   const int tile = blockIdx.x / shares, n_first = (blockIdx.x - tile * shares) * kShareCols;
   if (tile >= p.tiles) {
-    const long long first = static_cast<long long>(p.tiles) * shares, warps = blockDim.x / 32;
-    copy_others(p, tile_rows, (blockIdx.x - first) * warps + warp, (gridDim.x - first) * warps);
+    const long long first = static_cast<long long>(p.tiles) * shares;
+    copy_others(p, 16, (blockIdx.x - first) * kWarps + warp, (gridDim.x - first) * kWarps);
     return;
   }
-  const int row0 = tile * tile_rows;
-  if (!within(p, row0)) return;
-  const int e = adapter_of(p, row0);
-  const char* b = p.b + static_cast<long long>(e) * p.N * p.r * 2;
-  for (int i = threadIdx.x; i < kShareCols * (RP / 8); i += blockDim.x) {
-    const int row = i / (RP / 8), k = i % (RP / 8), n = n_first + row;
-    const bool in = n < p.N && 8 * k < p.r;
-    const char* from = b + static_cast<long long>(n) * p.r * 2;
-    if (ALIGNED) cp_async16(smem_u32(weights + row * PITCH + 16 * k), in ? from + 16 * k : b, in ? 16 : 0);
-    else *reinterpret_cast<uint4*>(weights + row * PITCH + 16 * k) = load8<false>(from, in ? 8 * k : p.r, p.r);
-  }
-  const int my_row = row0 + 16 * warp;
-  const int tokens = token_of(p, my_row + (lane & 15));
+  const int row0 = tile * kTileRows, my_row = row0 + 16 * warp;
+  const Between<RP> between(p);
+  int adapters = between.adapter[row0 / 16 + (lane & (kWarps - 1))];
+  const int tokens = between.token[my_row + (lane & 15)];
+  const int shared_e = static_cast<int>(__reduce_max_sync(0xffffffffu, adapters));
+  if (shared_e < 0) return;
+  const bool mixed = !__all_sync(0xffffffffu, adapters < 0 || adapters == shared_e);
+  const int e = __shfl_sync(0xffffffffu, adapters, warp);
   const int t0 = __shfl_sync(0xffffffffu, tokens, g), t1 = __shfl_sync(0xffffffffu, tokens, g + 8);
   const bool any = __any_sync(0xffffffffu, tokens >= 0);
+  const char* b = p.b + static_cast<long long>(mixed ? max(e, 0) : shared_e) * p.N * p.r * 2;
+  if (!mixed) {
+    for (int i = threadIdx.x; i < kShareCols * (RP / 8); i += 32 * kWarps) {
+      const int row = i / (RP / 8), k = i % (RP / 8), n = n_first + row;
+      const bool has = n < p.N && 8 * k < p.r;
+      const char* from = b + static_cast<long long>(n) * p.r * 2;
+      if (ALIGNED) cp_async16(smem_u32(weights + row * PITCH + 16 * k), has ? from + 16 * k : p.b, has ? 16 : 0);
+      else *reinterpret_cast<uint4*>(weights + row * PITCH + 16 * k) = load8<false>(from, has ? 8 * k : p.r, p.r);
+    }
+  }
   uint32_t lead[K][4], rest[K][4];
   float i0 = 1.f, i1 = 1.f;
-  if (any) {  // (so the tile's rows are all there)
-    const uint2* sl = reinterpret_cast<const uint2*>(p.s);
-    const uint2* sr = sl + static_cast<long long>(p.rows) * (RP / 4);
-    const float* factors = reinterpret_cast<const float*>(sr + static_cast<long long>(p.rows) * (RP / 4));
-    const long long at0 = static_cast<long long>(my_row + g) * (RP / 4), at1 = at0 + 8ll * (RP / 4);
-    const bool both = my_row + g + 8 < p.rows, one = my_row + g < p.rows;
+  constexpr int AHEAD = 2;  // groups whose base is on its way
+  BaseRows<T> base[AHEAD];
+  const int groups = min(kShareCols, p.N - n_first + kGroup - 1) / kGroup;
+  if (any) {
+    const uint2* lead0 = reinterpret_cast<const uint2*>(between.lead) + static_cast<long long>(my_row + g) * (RP / 4);
+    const uint2* rest0 = reinterpret_cast<const uint2*>(between.rest) + static_cast<long long>(my_row + g) * (RP / 4);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int q = RP == 16 ? t : 8 * (k / 2) + 2 * t + (k & 1);  // four columns each
-      const uint2 z = make_uint2(0u, 0u);
-      const uint2 u = one ? sl[at0 + q] : z, v = both ? sl[at1 + q] : z, ur = one ? sr[at0 + q] : z, vr = both ? sr[at1 + q] : z;
+      const uint2 u = lead0[q], v = lead0[8 * (RP / 4) + q], ur = rest0[q], vr = rest0[8 * (RP / 4) + q];
       lead[k][0] = u.x; lead[k][1] = v.x; lead[k][2] = u.y; lead[k][3] = v.y;
       rest[k][0] = ur.x; rest[k][1] = vr.x; rest[k][2] = ur.y; rest[k][3] = vr.y;
     }
     if (std::is_same<T, __half>::value) {
-      i0 = one ? factors[my_row + g] : 1.f;
-      i1 = both ? factors[my_row + g + 8] : 1.f;
+      i0 = between.inverse[my_row + g];
+      i1 = between.inverse[my_row + g + 8];
+    }
+    if (ALIGNED) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) base[i].load(p, i < groups ? n_first + kGroup * i + 8 * t : p.N, t0, t1);
     }
   }
-  const int groups = min(kShareCols, p.N - n_first + kGroup - 1) / kGroup;
-  BaseRows<T> base;
-  if (ALIGNED) base.load(p, n_first + 8 * t, t0, t1);
   cp_async_wait_all();
   __syncthreads();
   if (!any) return;
   __shared__ float staged[ALIGNED ? 1 : kWarps * 16 * kStagePitch];
+#pragma unroll 2
   for (int group = 0; group < groups; ++group) {
     const int n0 = n_first + kGroup * group;
-    BaseRows<T> next;
-    if (ALIGNED) next.load(p, group + 1 < groups ? n0 + kGroup + 8 * t : p.N, t0, t1);
+    BaseColumn column;
+    if (!ALIGNED) column.load(p, n0 + lane, tokens);
     float c[4][4];
+    if (mixed) {
+      direct_columns<T, RP, ALIGNED>(p, b, n0, lead, rest, c);
+    } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
-      const char* row = weights + (kGroup * group + out_column(g, j)) * PITCH;
+      for (int j = 0; j < 4; ++j) {
+        c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
+        const char* row = weights + (kGroup * group + out_column(g, j)) * PITCH;
 #pragma unroll
-      for (int l = 0; l < L; ++l) {
-        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if constexpr (RP == 16) {
-          const uint2 h = *reinterpret_cast<const uint2*>(row + 8 * t);
-          w.x = h.x;
-          w.y = h.y;
-        } else {
-          w = *reinterpret_cast<const uint4*>(row + 64 * l + 16 * t);
+        for (int l = 0; l < L; ++l) {
+          uint4 w = make_uint4(0u, 0u, 0u, 0u);
+          if constexpr (RP == 16) {
+            const uint2 h = *reinterpret_cast<const uint2*>(row + 8 * t);
+            w.x = h.x;
+            w.y = h.y;
+          } else {
+            w = *reinterpret_cast<const uint4*>(row + 64 * l + 16 * t);
+          }
+          step<T, RP>(c[j], lead, rest, l, w);
         }
-        step<T, RP>(c[j], lead, rest, l, w);
       }
     }
     if (ALIGNED) {
-      put_row<T>(p, n0 + 8 * t, t0, base.v[0], c, 0, i0);
-      put_row<T>(p, n0 + 8 * t, t1, base.v[1], c, 1, i1);
-      base = next;
+      put_row<T>(p, n0 + 8 * t, t0, base[0].v[0], c, 0, i0);
+      put_row<T>(p, n0 + 8 * t, t1, base[0].v[1], c, 1, i1);
+#pragma unroll
+      for (int i = 0; i + 1 < AHEAD; ++i) base[i] = base[i + 1];
+      base[AHEAD - 1].load(p, group + AHEAD < groups ? n0 + kGroup * AHEAD + 8 * t : p.N, t0, t1);
     } else {
-      put_staged<T>(p, n0, tokens, c, i0, i1, staged + warp * 16 * kStagePitch);
+      put_staged<T>(p, n0, tokens, column, c, i0, i1, staged + warp * 16 * kStagePitch);
     }
   }
 }
@@ -654,53 +782,53 @@ __global__ void __launch_bounds__(256, RP <= 64 ? 2 : 1) second_kernel(const Par
 // launches
 // ----------------------------------------------------------------------------------------------
 static int padded_rank(int r) { return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : 128; }
-// Rows of a tile of the two kernels: 32, 64 or 128, or 0 where the sort aligns to less.
-static int tile_of(int align) { return align % 128 == 0 ? 128 : align % 64 == 0 ? 64 : align % 32 == 0 ? 32 : 0; }
-static bool in_one_kernel(int T, int align) { return T <= 256 || tile_of(align) == 0; }
+static bool in_one_kernel(int T, int n) {
+  const long long tiles = T / 16 + static_cast<long long>(n < T ? n : T);  // of 16 rows, at most (or as many as there are tokens)
+  return (tiles < T ? tiles : T) <= 256;
+}
 static size_t round256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 template <class T, int RP, bool ALIGNED>
-static int launch(Params p, int align, cudaStream_t st) {
+static int launch(Params p, cudaStream_t st) {
   static PerDeviceFlag configured;
   const int dev = current_device();
   if (dev < 0) return SMOE_ERR_DRIVER;
   if (!configured.test(dev)) {
     if (cudaFuncSetAttribute(one_kernel<T, RP, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(one_smem<RP>())) != cudaSuccess ||
-        cudaFuncSetAttribute(first_kernel<T, RP, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(first_smem<RP>(128))) != cudaSuccess ||
+        cudaFuncSetAttribute(first_kernel<T, RP, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(First<RP, ALIGNED>::kSmem)) != cudaSuccess ||
         cudaFuncSetAttribute(second_kernel<T, RP, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Second<RP>::kSmem)) != cudaSuccess)
       return SMOE_ERR_LAUNCH;
     configured.set(dev);
   }
-  if (in_one_kernel(p.T, align)) {
+  if (in_one_kernel(p.T, p.n)) {
     p.tiles = (p.rows + 15) / 16;
     const long long others = p.in_place ? 0 : (p.T + 8ll * kCluster * kWarps - 1) / (8 * kCluster * kWarps);  // clusters, eight tokens to a warp
     const long long blocks = (p.tiles + others) * kCluster;
     if (blocks == 0) return SMOE_OK;
     return launched(launch_chained(one_kernel<T, RP, ALIGNED>, dim3(static_cast<unsigned>(blocks)), 32 * kWarps, one_smem<RP>(), st, kCluster, p));
   }
-  const int rows = tile_of(align), threads = 2 * rows;
-  p.tiles = (p.rows + rows - 1) / rows;
-  const int full = (p.T + rows - 1) / rows;
+  p.tiles = (p.rows + kTileRows - 1) / kTileRows;
+  const int full = (p.T + kTileRows - 1) / kTileRows;
   p.splits = full >= 148 ? 1 : full >= 74 ? 2 : full >= 37 ? 4 : 8;
   int kernels = 0;
   if (p.tiles > 0) {
-    const cudaError_t rc = launch_chained(first_kernel<T, RP, ALIGNED>, dim3(static_cast<unsigned>(p.tiles * p.splits)), threads, first_smem<RP>(rows), st, p.splits, p);
+    const cudaError_t rc = launch_chained(first_kernel<T, RP, ALIGNED>, dim3(static_cast<unsigned>(p.tiles * p.splits)), 32 * kWarps, First<RP, ALIGNED>::kSmem, st, p.splits, p);
     if (rc != cudaSuccess) return SMOE_ERR_LAUNCH;
     ++kernels;
   }
-  const int shares = (p.N + kShareCols - 1) / kShareCols, warps = threads / 32;
-  const long long others = p.in_place ? 0 : (p.T + 8ll * warps - 1) / (8 * warps);
+  const int shares = (p.N + kShareCols - 1) / kShareCols;
+  const long long others = p.in_place ? 0 : (p.T + 8ll * kWarps - 1) / (8 * kWarps);
   const long long blocks = static_cast<long long>(p.tiles) * shares + others;
   if (blocks == 0) return launched(cudaSuccess, kernels);
-  return launched(launch_chained(second_kernel<T, RP, ALIGNED>, dim3(static_cast<unsigned>(blocks)), threads, Second<RP>::kSmem, st, 1, p), kernels + 1);
+  return launched(launch_chained(second_kernel<T, RP, ALIGNED>, dim3(static_cast<unsigned>(blocks)), 32 * kWarps, Second<RP>::kSmem, st, 1, p), kernels + 1);
 }
 template <class T, bool ALIGNED>
-static int launch(const Params& p, int align, cudaStream_t st) {
+static int launch(const Params& p, cudaStream_t st) {
   switch (padded_rank(p.r)) {
-    case 16: return launch<T, 16, ALIGNED>(p, align, st);
-    case 32: return launch<T, 32, ALIGNED>(p, align, st);
-    case 64: return launch<T, 64, ALIGNED>(p, align, st);
-    default: return launch<T, 128, ALIGNED>(p, align, st);
+    case 16: return launch<T, 16, ALIGNED>(p, st);
+    case 32: return launch<T, 32, ALIGNED>(p, st);
+    case 64: return launch<T, 64, ALIGNED>(p, st);
+    default: return launch<T, 128, ALIGNED>(p, st);
   }
 }
 
@@ -714,9 +842,9 @@ using namespace smoe::adapters;
 
 extern "C" {
 
-size_t smoe_adapter_linear_workspace_bytes(int T, long long rows, int r, int align) {
-  if (T <= 0 || rows <= 0 || r <= 0 || r > kMaxRank || align <= 0 || in_one_kernel(T, align)) return 0;
-  return round256(static_cast<size_t>(rows) * (4 * padded_rank(r) + 4));
+size_t smoe_adapter_linear_workspace_bytes(int T, long long rows, int n, int r) {
+  if (T <= 0 || rows <= 0 || n <= 0 || r <= 0 || r > kMaxRank || in_one_kernel(T, n)) return 0;
+  return round256(between_bytes(rows, padded_rank(r)));
 }
 
 int smoe_adapter_linear(const void* x, long long ld, const void* a, const void* b, const float* scale, const void* base, long long base_ld,
@@ -728,14 +856,14 @@ int smoe_adapter_linear(const void* x, long long ld, const void* a, const void* 
       align % 16 != 0 || ld < 0 || base_ld < 0 || out_ld < N)
     return SMOE_ERR_SHAPE;
   if (H > 1 << 28 || N > 1 << 28) return SMOE_ERR_SHAPE;
-  const int tile = in_one_kernel(T, align) ? 16 : tile_of(align);
-  // blocks: eight to 16 rows of one kernel, up to eight and one to 256 columns of two; and those of the other tokens
-  if (((rows + tile - 1) / tile + T / 8 + 1) * (8ll + (N + kShareCols - 1) / kShareCols) > 0x7fffffffll) return SMOE_ERR_SHAPE;
+  // blocks: eight to 16 rows of one kernel, up to eight and one to 256 columns for 128 rows of two; and those of the other tokens
+  if ((in_one_kernel(T, n) ? (rows + 15) / 16 * kCluster : (rows + kTileRows - 1) / kTileRows * (8ll + (N + kShareCols - 1) / kShareCols)) + T / 8 + kCluster > 0x7fffffffll)
+    return SMOE_ERR_SHAPE;
   if (T == 0) return SMOE_OK;
   if (x == nullptr || a == nullptr || b == nullptr || out == nullptr || expert_frequency_offset == nullptr || s_reverse_scatter_idx == nullptr ||
       (rows > 0 && x_gather_idx == nullptr))
     return SMOE_ERR_SHAPE;
-  const size_t ws = smoe_adapter_linear_workspace_bytes(T, rows, r, align);
+  const size_t ws = smoe_adapter_linear_workspace_bytes(T, rows, n, r);
   if (ws > 0 && workspace == nullptr) return SMOE_ERR_WORKSPACE;
   if ((address(x) | address(a) | address(b) | address(base) | address(out)) % 2 != 0 ||
       (address(scale) | address(expert_frequency_offset) | address(x_gather_idx) | address(s_reverse_scatter_idx)) % 4 != 0 || address(workspace) % 256 != 0)
@@ -752,8 +880,8 @@ int smoe_adapter_linear(const void* x, long long ld, const void* a, const void* 
   const bool aligned = (address(x) | address(a) | address(b) | address(base) | address(out) | p.x_ld | p.base_ld | p.out_ld) % 16 == 0 && H % 8 == 0 &&
                        N % 8 == 0 && r % 8 == 0;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == SMOE_BF16) return aligned ? launch<__nv_bfloat16, true>(p, align, st) : launch<__nv_bfloat16, false>(p, align, st);
-  return aligned ? launch<__half, true>(p, align, st) : launch<__half, false>(p, align, st);
+  if (dtype == SMOE_BF16) return aligned ? launch<__nv_bfloat16, true>(p, st) : launch<__nv_bfloat16, false>(p, st);
+  return aligned ? launch<__half, true>(p, st) : launch<__half, false>(p, st);
 }
 
 }  // extern "C"

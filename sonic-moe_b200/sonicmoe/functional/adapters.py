@@ -29,13 +29,12 @@ _TYPES = {torch.bfloat16: _lib.SMOE_BF16, torch.float16: _lib.SMOE_F16}
 
 def adapter_permutation(adapter_idx: torch.Tensor, num_adapters: int) -> TokenPermutation:
     """The tokens sorted by adapter.  adapter_idx (T,) int32 or int64; a token whose index is outside [0, num_adapters) (-1, say) has
-    no adapter.  An adapter's rows start at a multiple of 16, or of as many as its tokens are likely to fill, 128 at most."""
+    no adapter."""
     if adapter_idx.dim() != 1:
         raise ValueError(f"adapter_idx has to be (T,), got {tuple(adapter_idx.shape)}")
     if not 0 < num_adapters <= MAX_ADAPTERS:
         raise ValueError(f"1 to {MAX_ADAPTERS} adapters are needed, got {num_adapters}")
-    each = adapter_idx.numel() // num_adapters
-    return token_permutation(adapter_idx.unsqueeze(1), num_adapters, align=128 if each >= 96 else 64 if each >= 48 else 32 if each >= 24 else 16)
+    return token_permutation(adapter_idx.unsqueeze(1), num_adapters, align=16)
 
 
 def _refuse_gradients(*tensors) -> None:
@@ -101,7 +100,7 @@ def adapter_linear(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, permutatio
         # (the distance of a single row means nothing)
         base_ld = 0 if base is None else base.stride(0) if T > 1 else max(N, base.stride(0))
         out = base if inplace else torch.empty(T, N, dtype=x.dtype, device=dev)
-        ws = lib.smoe_adapter_linear_workspace_bytes(T, rows, r, align)
+        ws = lib.smoe_adapter_linear_workspace_bytes(T, rows, n, r)
         ws = _lib.workspace(ws, dev) if ws else None
         check(lib.smoe_adapter_linear(
             x.data_ptr(), x.stride(0), a.data_ptr(), b.data_ptr(), ptr(scale), ptr(base), base_ld, out.data_ptr(),

@@ -9,8 +9,8 @@ def test_refusals(built_library):
 
     at = 4096
 
-    def call(x=at, ld=64, a=at, b=at, scale=None, base=None, base_ld=0, out=at, out_ld=32, dtype=1, off=at, gather=at, reverse=at, T=300,
-             rows=512, H=64, N=32, n=4, r=8, align=32, ws=at):
+    def call(x=at, ld=64, a=at, b=at, scale=None, base=None, base_ld=0, out=at, out_ld=32, dtype=1, off=at, gather=at, reverse=at, T=5000,
+             rows=5120, H=64, N=32, n=4, r=8, align=32, ws=at):
         return lib.smoe_adapter_linear(x, ld, a, b, scale, base, base_ld, out, out_ld, dtype, off, gather, reverse, T, rows, H, N, n, r, align, ws, None)
 
     assert call(dtype=0) == call(dtype=2) == -6
@@ -30,9 +30,9 @@ def test_workspace_bytes(built_library):
     from sonicmoe._lib import lib
 
     ws = lib.smoe_adapter_linear_workspace_bytes
-    assert ws(256, 4096, 16, 128) == 0 and ws(10000, 20000, 16, 16) == 0 and ws(10000, 20000, 16, 48) == 0  # one kernel
-    assert ws(0, 0, 16, 128) == 0 and ws(1000, 0, 16, 128) == 0
-    assert ws(257, 512, 16, 32) >= 512 * 68 and ws(257, 512, 100, 64) >= 512 * 516
+    assert ws(256, 4096, 1000, 16) == 0 and ws(2048, 4096, 100, 128) == 0  # few tiles of 16 rows: one kernel
+    assert ws(0, 0, 4, 16) == 0 and ws(10000, 0, 4, 16) == 0
+    assert ws(5000, 5120, 4, 16) >= 5120 * 72 and ws(5000, 5120, 4, 100) >= 5120 * 520 and ws(1000, 2000, 1000, 8) > 0
 
 
 def test_python_refusals(built_library):
