@@ -44,7 +44,7 @@ struct Params {
   const int* reverse;                     // (T) row of each token
   char* s;                                // two kernels: `Between`
   int T, rows, H, N, n, r;
-  int tiles;                              // of 16 rows, or of 128
+  int tiles;                              // of 16 rows, or of a block's of two kernels, at most
   int splits;                             // two kernels: blocks that share the columns of x
   int in_place;                           // out is base
 };
@@ -459,30 +459,74 @@ __global__ void __launch_bounds__(32 * kWarps) one_kernel(const Params p) {
 // ----------------------------------------------------------------------------------------------
 // two kernels
 // ----------------------------------------------------------------------------------------------
-// A block has 128 rows, each of its eight warps 16 of them, which have one adapter.  As the rows are sorted most blocks have one adapter too, whose
-// weights the warps share in shared memory; in the others each warp reads its own.
-constexpr int kTileRows = 16 * kWarps;
+// A block has 32, 64 or 128 rows of one adapter (the last block of an adapter what is left), a warp 16 of them; the warps share the weights in
+// shared memory.
 
 // What the first kernel leaves to the second one in the workspace.
 template <int RP>
 struct Between {
-  char* lead;      // (rows, RP) 16-bit
+  char* lead;      // (rows, RP) 16-bit, 128 rows more than there are
   char* rest;      // (rows, RP)
   float* inverse;  // (rows)
   int* token;      // (rows), -1: none
-  int* adapter;    // (rows / 16), -1: no tokens
+  int4* tile;      // (tiles) adapter (-1: no tile), first row, end
   __device__ __forceinline__ explicit Between(const Params& p) {
-    const long long rows = p.tiles * static_cast<long long>(kTileRows);
+    const long long rows = (p.rows + 127ll) / 128 * 128 + 128;
     lead = p.s;
     rest = lead + rows * 2 * RP;
     inverse = reinterpret_cast<float*>(rest + rows * 2 * RP);
     token = reinterpret_cast<int*>(inverse + rows);
-    adapter = token + rows;
+    tile = reinterpret_cast<int4*>(token + rows);
   }
 };
-static size_t between_bytes(long long rows, int rp) {
-  const long long padded = (rows + kTileRows - 1) / kTileRows * kTileRows;
-  return static_cast<size_t>(padded) * (4 * rp + 8) + static_cast<size_t>(padded / 16) * 4;
+static size_t between_bytes(long long rows, long long tiles, int rp) {
+  return static_cast<size_t>((rows + 127) / 128 * 128 + 128) * (4 * rp + 8) + static_cast<size_t>(tiles) * 16;
+}
+
+// The `tile`-th block's adapter, first row and end, adapters in their order (all lanes of the warp); adapter -1 behind the last.  Each lane counts
+// the tiles of a run of adapters; then the lanes look at the run that holds the tile.
+__device__ __forceinline__ int4 tile_of(const Params& p, int tile, int tile_rows) {
+  const int lane = threadIdx.x & 31;
+  const auto row_at = [&](int e) { return min(max(p.off[e], 0), p.rows); };
+  const auto tiles_between = [&](int first, int end) { return end > first ? (end - first + tile_rows - 1) / tile_rows : 0; };
+  const auto scan = [&](int v) {  // sum over the lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int other = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += other;
+    }
+    return v;
+  };
+  const int run = (p.n + 31) / 32;
+  int mine = 0;
+  {
+    const int end = min(p.n, (lane + 1) * run);
+    int last = lane * run < p.n ? row_at(lane * run) : 0;
+#pragma unroll 4
+    for (int e = lane * run; e < end; ++e) {
+      const int next = row_at(e + 1);
+      mine += tiles_between(last, next);
+      last = next;
+    }
+  }
+  int sum = scan(mine);
+  unsigned found = __ballot_sync(0xffffffffu, tile < sum);
+  if (found == 0u) return make_int4(-1, 0, 0, 0);
+  const int who = __ffs(found) - 1;
+  int before = __shfl_sync(0xffffffffu, sum - mine, who);
+  for (int e0 = who * run;; e0 += 32) {  // (it is in one of them)
+    const int e = e0 + lane;
+    const bool in = e < min(p.n, (who + 1) * run);
+    const int first = in ? row_at(e) : 0, end = in ? row_at(e + 1) : 0, tiles = tiles_between(first, end);
+    sum = before + scan(tiles);
+    found = __ballot_sync(0xffffffffu, tile < sum);
+    if (found != 0u || e0 >= p.n) {
+      const int at = found != 0u ? __ffs(found) - 1 : 0;
+      const int row = __shfl_sync(0xffffffffu, first, at) + (tile - __shfl_sync(0xffffffffu, sum - tiles, at)) * tile_rows;
+      return make_int4(found != 0u ? e0 + at : -1, row, min(row + tile_rows, __shfl_sync(0xffffffffu, end, at)), 0);
+    }
+    before = __shfl_sync(0xffffffffu, sum, 31);
+  }
 }
 
 // The first: s of a block's rows over a share of the columns of x.  Every warp brings in its own rows of x, the block a, 64 columns in a stage and
@@ -492,9 +536,11 @@ template <int RP, bool ALIGNED>
 struct First {
   static constexpr int kCols = 64, kStages = 3;
   static constexpr int kPitch = ALIGNED ? 128 : 192;  // of a row of x; 128: the odd rows' halves trade places, so that eight lanes meet all banks
-  static constexpr int kWarpBytes = 16 * kPitch, kXBytes = kWarps * kWarpBytes, kABytes = RP * 128;
-  static constexpr size_t kStaging = kStages * static_cast<size_t>(kXBytes + kABytes), kPart = sizeof(float) * kTileRows * RP;
-  static constexpr size_t kSmem = kStaging > kPart ? kStaging : kPart;
+  static constexpr int kWarpBytes = 16 * kPitch, kABytes = RP * 128;
+  static size_t smem(int warps) {
+    const size_t staging = kStages * static_cast<size_t>(warps * kWarpBytes + kABytes), part = sizeof(float) * 16 * warps * RP;
+    return staging > part ? staging : part;
+  }
 };
 // place of the 16-byte block `k` of row `row` in a row of 128 bytes
 __device__ __forceinline__ int swizzled(int row, int k) { return 16 * (k ^ ((row & 1) << 2)); }
@@ -507,36 +553,23 @@ __global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) first_kernel(co
   extern __shared__ __align__(128) char staging[];
   constexpr int COLS = F::kCols, STAGES = F::kStages, NT = RP / 8, C = COLS / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int warps = blockDim.x / 32, tile_rows = 16 * warps;
   const int tile = blockIdx.x / p.splits, share = blockIdx.x - tile * p.splits;
-  const int row0 = tile * kTileRows, my_row = row0 + 16 * warp;
-  __shared__ int adapters[kWarps];
-  const bool in = within(p, my_row);
-  const int gathered = in ? gathered_of(p, my_row + (lane & 15)) : -1;
-  const bool any = __any_sync(0xffffffffu, gathered >= 0);
-  const int row_of = gathered >= 0 ? p.reverse[gathered] : -1;
-  const int e = any ? adapter_of(p, my_row) : -1;
-  if (lane == 0) adapters[warp] = e;
-  __syncthreads();
-  int shared_e = -1;
-  bool mixed = false;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    const int other = adapters[w];
-    mixed |= other >= 0 && shared_e >= 0 && other != shared_e;
-    shared_e = other >= 0 ? other : shared_e;
-  }
+  const int4 what = tile_of(p, tile, tile_rows);
   const Between<RP> between(p);
-  if (share == 0) {
-    if (lane < 16) between.token[my_row + lane] = row_of == my_row + lane ? gathered : -1;
-    if (lane == 0) between.adapter[my_row / 16] = e;
-  }
-  if (shared_e < 0) return;  // (the cluster's blocks all see the same)
+  if (share == 0 && threadIdx.x == 0) between.tile[tile] = what;
+  if (what.x < 0) return;  // (the cluster's blocks all see the same)
+  const int e = what.x, row0 = what.y, my_row = row0 + 16 * warp;
+  const int gathered = my_row + (lane & 15) < what.z ? gathered_of(p, my_row + (lane & 15)) : -1;
+  const bool any = __any_sync(0xffffffffu, gathered >= 0);
+  if (share == 0 && lane < 16 && my_row + lane < what.z) between.token[my_row + lane] = gathered >= 0 && p.reverse[gathered] == my_row + lane ? gathered : -1;
   const int t0 = __shfl_sync(0xffffffffu, gathered, g), t1 = __shfl_sync(0xffffffffu, gathered, g + 8);
-  const char* a = p.a + static_cast<long long>(mixed ? e : shared_e) * p.r * p.H * 2;
+  const char* a = p.a + static_cast<long long>(e) * p.r * p.H * 2;
   const int all = (p.H + COLS - 1) / COLS;
   const int first = static_cast<int>(static_cast<long long>(all) * share / p.splits), end = static_cast<int>(static_cast<long long>(all) * (share + 1) / p.splits);
-  const auto x_stage = [&](int stage) { return staging + stage % STAGES * (F::kXBytes + F::kABytes) + warp * F::kWarpBytes; };
-  const auto a_stage = [&](int stage) { return staging + stage % STAGES * (F::kXBytes + F::kABytes) + F::kXBytes; };
+  const int stage_bytes = F::kABytes + warps * F::kWarpBytes;
+  const auto a_stage = [&](int stage) { return staging + stage % STAGES * stage_bytes; };
+  const auto x_stage = [&](int stage) { return a_stage(stage) + F::kABytes + warp * F::kWarpBytes; };
   // rows lane / 8, + 4, + 8, + 12 of this warp, block lane % 8 of each
   const char* x_row[4];
   int x_off[4];
@@ -566,14 +599,11 @@ __global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) first_kernel(co
       }
     }
   };
-  constexpr int A_LOADS = RP * 8 / (32 * kWarps) > 0 ? RP * 8 / (32 * kWarps) : 1;
   const auto fetch_a = [&](int stage) {
-    if (mixed || stage >= end) return;
+    if (stage >= end) return;
     char* to = a_stage(stage);
-#pragma unroll
-    for (int i = 0; i < A_LOADS; ++i) {
-      const int at = threadIdx.x + 32 * kWarps * i, row = at >> 3, k = at & 7, col = COLS * stage + 8 * k;
-      if (row >= RP) continue;
+    for (int at = threadIdx.x; at < RP * 8; at += blockDim.x) {
+      const int row = at >> 3, k = at & 7, col = COLS * stage + 8 * k;
       const char* from = a + static_cast<long long>(row) * p.H * 2;
       const bool has = row < p.r && col < p.H;
       if (ALIGNED) cp_async16(smem_u32(to + 128 * row + swizzled(row, k)), has ? from + 2ll * col : p.a, has ? 16 : 0);
@@ -615,9 +645,7 @@ __global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) first_kernel(co
       }
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        uint4 w;
-        if (mixed) w = load8<ALIGNED>(a + (8ll * j + g) * p.H * 2, 8 * j + g < p.r ? COLS * stage + 32 * c + 8 * t : p.H, p.H);
-        else w = *reinterpret_cast<const uint4*>(w_from + 128 * (8 * j + g) + swizzled(g, 4 * c + t));
+        const uint4 w = *reinterpret_cast<const uint4*>(w_from + 128 * (8 * j + g) + swizzled(g, 4 * c + t));
         mma<T>(acc[j], x0.x, x1.x, x0.y, x1.y, w.x, w.y);
         mma<T>(acc[j], x0.z, x1.z, x0.w, x1.w, w.z, w.w);
       }
@@ -625,7 +653,7 @@ __global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) first_kernel(co
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
-  float* part = reinterpret_cast<float*>(staging);  // [kTileRows][RP]
+  float* part = reinterpret_cast<float*>(staging);  // [tile_rows][RP]
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     float* to = part + (16 * warp + g) * RP + 8 * j + 2 * t;
@@ -633,14 +661,16 @@ __global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) first_kernel(co
     *reinterpret_cast<float2*>(to + 8 * RP) = make_float2(acc[j][2], acc[j][3]);
   }
   if (p.splits > 1) cluster_sync_all(); else __syncthreads();
-  // rows share * kTileRows / splits and on, four columns to a thread
+  // rows share * tile_rows / splits and on, four columns to a thread
   constexpr int Q = RP / 4;
-  const int mine = kTileRows / p.splits, begin = share * mine;
+  const int mine = tile_rows / p.splits, begin = share * mine;
+  const float scale = p.scale != nullptr ? p.scale[e] : 1.f;
   uint2* lead = reinterpret_cast<uint2*>(between.lead);
   uint2* rest = reinterpret_cast<uint2*>(between.rest);
-  for (int i = threadIdx.x; i < mine * Q; i += blockDim.x) {  // (16 rows of at least four columns' threads for a warp: all lanes of it)
-    const int row = begin + i / Q, q = i % Q, of = adapters[row / 16];
-    const float scale = p.scale != nullptr && of >= 0 ? p.scale[of] : 1.f;
+  for (int first_of = 0; first_of < mine * Q; first_of += blockDim.x) {  // (all threads, for the shuffles)
+    const int i = first_of + threadIdx.x;
+    const bool live = i < mine * Q;
+    const int row = begin + (live ? i / Q : 0), q = i % Q;
     float f[4] = {0.f, 0.f, 0.f, 0.f};
     for (int k = 0; k < p.splits; ++k) {
       const uint32_t at = smem_u32(part + row * RP + 4 * q), from = p.splits > 1 ? map_to_cta(at, k) : at;
@@ -662,9 +692,11 @@ __global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) first_kernel(co
     split2<T>(f[0] * factor, f[1] * factor, l.x, r.x);
     split2<T>(f[2] * factor, f[3] * factor, l.y, r.y);
     const long long at = static_cast<long long>(row0 + row) * Q + q;
-    lead[at] = l;
-    rest[at] = r;
-    if (q == 0) between.inverse[row0 + row] = inverse_of<T>(factor);
+    if (live && row0 + row < what.z) {
+      lead[at] = l;
+      rest[at] = r;
+      if (q == 0) between.inverse[row0 + row] = inverse_of<T>(factor);
+    }
   }
   if (p.splits > 1) cluster_sync_all();  // the others have read this block's part
 }
@@ -688,32 +720,27 @@ __global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) second_kernel(c
   const int tile = blockIdx.x / shares, n_first = (blockIdx.x - tile * shares) * kShareCols;
   if (tile >= p.tiles) {
     const long long first = static_cast<long long>(p.tiles) * shares;
-    copy_others(p, 16, (blockIdx.x - first) * kWarps + warp, (gridDim.x - first) * kWarps);
+    copy_others(p, 16, (blockIdx.x - first) * (blockDim.x / 32) + warp, (gridDim.x - first) * (blockDim.x / 32));
     return;
   }
-  const int row0 = tile * kTileRows, my_row = row0 + 16 * warp;
   const Between<RP> between(p);
-  int adapters = between.adapter[row0 / 16 + (lane & (kWarps - 1))];
-  const int tokens = between.token[my_row + (lane & 15)];
-  const int shared_e = static_cast<int>(__reduce_max_sync(0xffffffffu, adapters));
-  if (shared_e < 0) return;
-  const bool mixed = !__all_sync(0xffffffffu, adapters < 0 || adapters == shared_e);
-  const int e = __shfl_sync(0xffffffffu, adapters, warp);
+  const int4 what = between.tile[tile];
+  if (what.x < 0) return;
+  const int my_row = what.y + 16 * warp;
+  const int tokens = my_row + (lane & 15) < what.z ? between.token[my_row + (lane & 15)] : -1;
+  const char* b = p.b + static_cast<long long>(what.x) * p.N * p.r * 2;
+  for (int i = threadIdx.x; i < kShareCols * (RP / 8); i += blockDim.x) {
+    const int row = i / (RP / 8), k = i % (RP / 8), n = n_first + row;
+    const bool has = n < p.N && 8 * k < p.r;
+    const char* from = b + static_cast<long long>(n) * p.r * 2;
+    if (ALIGNED) cp_async16(smem_u32(weights + row * PITCH + 16 * k), has ? from + 16 * k : p.b, has ? 16 : 0);
+    else *reinterpret_cast<uint4*>(weights + row * PITCH + 16 * k) = load8<false>(from, has ? 8 * k : p.r, p.r);
+  }
   const int t0 = __shfl_sync(0xffffffffu, tokens, g), t1 = __shfl_sync(0xffffffffu, tokens, g + 8);
   const bool any = __any_sync(0xffffffffu, tokens >= 0);
-  const char* b = p.b + static_cast<long long>(mixed ? max(e, 0) : shared_e) * p.N * p.r * 2;
-  if (!mixed) {
-    for (int i = threadIdx.x; i < kShareCols * (RP / 8); i += 32 * kWarps) {
-      const int row = i / (RP / 8), k = i % (RP / 8), n = n_first + row;
-      const bool has = n < p.N && 8 * k < p.r;
-      const char* from = b + static_cast<long long>(n) * p.r * 2;
-      if (ALIGNED) cp_async16(smem_u32(weights + row * PITCH + 16 * k), has ? from + 16 * k : p.b, has ? 16 : 0);
-      else *reinterpret_cast<uint4*>(weights + row * PITCH + 16 * k) = load8<false>(from, has ? 8 * k : p.r, p.r);
-    }
-  }
   uint32_t lead[K][4], rest[K][4];
   float i0 = 1.f, i1 = 1.f;
-  constexpr int AHEAD = 2;  // groups whose base is on its way
+  constexpr int AHEAD = 2;  // groups whose base is fetched together: 128 bytes of a row
   BaseRows<T> base[AHEAD];
   const int groups = min(kShareCols, p.N - n_first + kGroup - 1) / kGroup;
   if (any) {
@@ -739,19 +766,23 @@ __global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) second_kernel(c
   __syncthreads();
   if (!any) return;
   __shared__ float staged[ALIGNED ? 1 : kWarps * 16 * kStagePitch];
-#pragma unroll 2
-  for (int group = 0; group < groups; ++group) {
-    const int n0 = n_first + kGroup * group;
-    BaseColumn column;
-    if (!ALIGNED) column.load(p, n0 + lane, tokens);
-    float c[4][4];
-    if (mixed) {
-      direct_columns<T, RP, ALIGNED>(p, b, n0, lead, rest, c);
-    } else {
+  for (int group = 0; group < groups; group += AHEAD) {
+    BaseRows<T> next[AHEAD];
+    BaseColumn column[ALIGNED ? 1 : AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (ALIGNED) next[i].load(p, group + AHEAD + i < groups ? n_first + kGroup * (group + AHEAD + i) + 8 * t : p.N, t0, t1);
+      else column[i].load(p, group + i < groups ? n_first + kGroup * (group + i) + lane : p.N, tokens);
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (group + i >= groups) break;
+      const int n0 = n_first + kGroup * (group + i);
+      float c[4][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
-        const char* row = weights + (kGroup * group + out_column(g, j)) * PITCH;
+        const char* row = weights + (kGroup * (group + i) + out_column(g, j)) * PITCH;
 #pragma unroll
         for (int l = 0; l < L; ++l) {
           uint4 w = make_uint4(0u, 0u, 0u, 0u);
@@ -765,16 +796,15 @@ __global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) second_kernel(c
           step<T, RP>(c[j], lead, rest, l, w);
         }
       }
+      if (ALIGNED) {
+        put_row<T>(p, n0 + 8 * t, t0, base[i].v[0], c, 0, i0);
+        put_row<T>(p, n0 + 8 * t, t1, base[i].v[1], c, 1, i1);
+      } else {
+        put_staged<T>(p, n0, tokens, column[ALIGNED ? 0 : i], c, i0, i1, staged + warp * 16 * kStagePitch);
+      }
     }
-    if (ALIGNED) {
-      put_row<T>(p, n0 + 8 * t, t0, base[0].v[0], c, 0, i0);
-      put_row<T>(p, n0 + 8 * t, t1, base[0].v[1], c, 1, i1);
 #pragma unroll
-      for (int i = 0; i + 1 < AHEAD; ++i) base[i] = base[i + 1];
-      base[AHEAD - 1].load(p, group + AHEAD < groups ? n0 + kGroup * AHEAD + 8 * t : p.N, t0, t1);
-    } else {
-      put_staged<T>(p, n0, tokens, column, c, i0, i1, staged + warp * 16 * kStagePitch);
-    }
+    for (int i = 0; i < AHEAD; ++i) base[i] = next[i];
   }
 }
 
@@ -786,6 +816,12 @@ static bool in_one_kernel(int T, int n) {
   const long long tiles = T / 16 + static_cast<long long>(n < T ? n : T);  // of 16 rows, at most (or as many as there are tokens)
   return (tiles < T ? tiles : T) <= 256;
 }
+// Warps of a block of the two kernels, by the tokens that an adapter has on average.
+static int warps_of(int T, int n) { return T / n <= 32 ? 2 : T / n <= 64 ? 4 : 8; }
+// Blocks' tiles, at most: every adapter's last one may be part of a tile.
+static long long tiles_of(int T, long long rows, int n) {
+  return rows / (16 * warps_of(T, n)) + (n < T ? n : T);
+}
 static size_t round256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 template <class T, int RP, bool ALIGNED>
@@ -795,7 +831,7 @@ static int launch(Params p, cudaStream_t st) {
   if (dev < 0) return SMOE_ERR_DRIVER;
   if (!configured.test(dev)) {
     if (cudaFuncSetAttribute(one_kernel<T, RP, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(one_smem<RP>())) != cudaSuccess ||
-        cudaFuncSetAttribute(first_kernel<T, RP, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(First<RP, ALIGNED>::kSmem)) != cudaSuccess ||
+        cudaFuncSetAttribute(first_kernel<T, RP, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(First<RP, ALIGNED>::smem(kWarps))) != cudaSuccess ||
         cudaFuncSetAttribute(second_kernel<T, RP, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Second<RP>::kSmem)) != cudaSuccess)
       return SMOE_ERR_LAUNCH;
     configured.set(dev);
@@ -807,20 +843,21 @@ static int launch(Params p, cudaStream_t st) {
     if (blocks == 0) return SMOE_OK;
     return launched(launch_chained(one_kernel<T, RP, ALIGNED>, dim3(static_cast<unsigned>(blocks)), 32 * kWarps, one_smem<RP>(), st, kCluster, p));
   }
-  p.tiles = (p.rows + kTileRows - 1) / kTileRows;
-  const int full = (p.T + kTileRows - 1) / kTileRows;
+  const int warps = warps_of(p.T, p.n);
+  p.tiles = static_cast<int>(tiles_of(p.T, p.rows, p.n));
+  const int full = (p.T + 16 * warps - 1) / (16 * warps);
   p.splits = full >= 148 ? 1 : full >= 74 ? 2 : full >= 37 ? 4 : 8;
   int kernels = 0;
   if (p.tiles > 0) {
-    const cudaError_t rc = launch_chained(first_kernel<T, RP, ALIGNED>, dim3(static_cast<unsigned>(p.tiles * p.splits)), 32 * kWarps, First<RP, ALIGNED>::kSmem, st, p.splits, p);
+    const cudaError_t rc = launch_chained(first_kernel<T, RP, ALIGNED>, dim3(static_cast<unsigned>(p.tiles * p.splits)), 32 * warps, First<RP, ALIGNED>::smem(warps), st, p.splits, p);
     if (rc != cudaSuccess) return SMOE_ERR_LAUNCH;
     ++kernels;
   }
   const int shares = (p.N + kShareCols - 1) / kShareCols;
-  const long long others = p.in_place ? 0 : (p.T + 8ll * kWarps - 1) / (8 * kWarps);
+  const long long others = p.in_place ? 0 : (p.T + 8ll * warps - 1) / (8 * warps);
   const long long blocks = static_cast<long long>(p.tiles) * shares + others;
   if (blocks == 0) return launched(cudaSuccess, kernels);
-  return launched(launch_chained(second_kernel<T, RP, ALIGNED>, dim3(static_cast<unsigned>(blocks)), 32 * kWarps, Second<RP>::kSmem, st, 1, p), kernels + 1);
+  return launched(launch_chained(second_kernel<T, RP, ALIGNED>, dim3(static_cast<unsigned>(blocks)), 32 * warps, Second<RP>::kSmem, st, 1, p), kernels + 1);
 }
 template <class T, bool ALIGNED>
 static int launch(const Params& p, cudaStream_t st) {
@@ -844,7 +881,7 @@ extern "C" {
 
 size_t smoe_adapter_linear_workspace_bytes(int T, long long rows, int n, int r) {
   if (T <= 0 || rows <= 0 || n <= 0 || r <= 0 || r > kMaxRank || in_one_kernel(T, n)) return 0;
-  return round256(between_bytes(rows, padded_rank(r)));
+  return round256(between_bytes(rows, tiles_of(T, rows, n), padded_rank(r)));
 }
 
 int smoe_adapter_linear(const void* x, long long ld, const void* a, const void* b, const float* scale, const void* base, long long base_ld,
@@ -857,7 +894,7 @@ int smoe_adapter_linear(const void* x, long long ld, const void* a, const void* 
     return SMOE_ERR_SHAPE;
   if (H > 1 << 28 || N > 1 << 28) return SMOE_ERR_SHAPE;
   // blocks: eight to 16 rows of one kernel, up to eight and one to 256 columns for 128 rows of two; and those of the other tokens
-  if ((in_one_kernel(T, n) ? (rows + 15) / 16 * kCluster : (rows + kTileRows - 1) / kTileRows * (8ll + (N + kShareCols - 1) / kShareCols)) + T / 8 + kCluster > 0x7fffffffll)
+  if ((in_one_kernel(T, n) ? (rows + 15) / 16 * kCluster : tiles_of(T, rows, n) * (8ll + (N + kShareCols - 1) / kShareCols)) + T / 8 + kCluster > 0x7fffffffll)
     return SMOE_ERR_SHAPE;
   if (T == 0) return SMOE_OK;
   if (x == nullptr || a == nullptr || b == nullptr || out == nullptr || expert_frequency_offset == nullptr || s_reverse_scatter_idx == nullptr ||
