@@ -529,13 +529,11 @@ int smoe_rms_norm_backward(const void* dy, long long dy_ld, const void* dh, long
  * The tokens sorted by adapter, as smoe_token_permutation sorts T pairs (K = 1) of n experts: expert_frequency_offset (n+1), first rows,
  * multiples of `align`, which is a multiple of 16; x_gather_idx (rows): token of each row, -1 for none; s_reverse_scatter_idx (T): row
  * of each token, outside [0, rows) where it has no adapter.  A token is a row's where each names the other.
- * n <= 4096, r <= 128, H and N <= 2^28.  Sizes whose blocks are more than 2^31 - 1 are refused.  workspace:
- * smoe_adapter_linear_workspace_bytes bytes, 256-byte aligned (0: may be NULL). */
-size_t smoe_adapter_linear_workspace_bytes(int T, long long rows, int n, int r);
+ * n <= 4096, r <= 128, H and N <= 2^28, T and rows <= 2^31 - 2^16. */
 int smoe_adapter_linear(const void* x, long long ld, const void* a, const void* b, const float* scale, const void* base,
                         long long base_ld, void* out, long long out_ld, int dtype, const int* expert_frequency_offset,
                         const int* x_gather_idx, const int* s_reverse_scatter_idx, int T, long long rows, int H, int N, int n,
-                        int r, int align, void* workspace, void* stream);
+                        int r, int align, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Expert parallelism over peer memory (one node, NVLink / NVSwitch).  The reference has no distributed

@@ -9,11 +9,11 @@
 // which keeps it in range), and the second product takes both: rounding s to 16 bits alone would make the error of out half as large
 // again where base is small.  out is rounded once.
 //
-// Two ways, of which `in_one_kernel` chooses:
-//   one kernel   a cluster of eight blocks has 16 rows; each block reads an eighth of the columns of x and a, the blocks add their parts over
-//                distributed shared memory, and each computes an eighth of the columns of out.  Weights go straight from memory to
-//                registers: this is for few tokens, or few to an adapter, where weights are everything and latency counts.
-//   two kernels  tiles of up to 128 rows, a warp for 16 of them, that share the weights in shared memory; s lies in memory in between.
+// In both kernels the blocks of a cluster share a tile of rows: each has a part of the columns of x and a, they add their products over distributed
+// shared memory, and each computes a part of the columns of out.
+//   few_kernel   tiles of 16 rows, clusters of eight; the warps of a block share the columns, and weights go straight from memory to registers: for few
+//                tokens, or few to an adapter, where weights are everything and latency counts
+//   tile_kernel  tiles of 32 to 128 rows of one adapter, a warp for 16 of them; the warps share the weights in shared memory
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -29,7 +29,7 @@ namespace smoe {
 namespace adapters {
 
 constexpr int kMaxAdapters = 4096, kMaxRank = 128, kMaxRows = 0x7fff0000;
-constexpr int kCluster = 8, kWarps = 8;   // of the one kernel
+constexpr int kCluster = 8, kWarps = 8;   // of few_kernel; warps of tile_kernel at most
 constexpr int kGroup = 32;                // columns of out that a warp has at a time
 
 struct Params {
@@ -42,10 +42,9 @@ struct Params {
   const int* off;                         // (n + 1) first row of each adapter, ascending
   const int* gather;                      // (rows) token of each row
   const int* reverse;                     // (T) row of each token
-  char* s;                                // two kernels: `Between`
   int T, rows, H, N, n, r;
-  int tiles;                              // of 16 rows, or of a block's of two kernels, at most
-  int splits;                             // two kernels: blocks that share the columns of x
+  int tiles;                              // few_kernel: of 16 rows; tile_kernel: at most
+  int cluster;                            // tile_kernel: blocks that share a tile
   int in_place;                           // out is base
 };
 
@@ -229,9 +228,9 @@ struct BaseRows {
     if (t1 >= 0) v[1] = __ldcs(reinterpret_cast<const uint4*>(p.base + t1 * p.base_ld + 2ll * n));
   }
 };
+// base + c inverse: eight columns of row g (half 0) or g + 8 (half 1)
 template <class T>
-__device__ __forceinline__ void put_row(const Params& p, int n, int t, const uint4& base, const float (&c)[4][4], int half, float inverse) {
-  if (t < 0 || n >= p.N) return;
+__device__ __forceinline__ uint4 sum_row(const uint4& base, const float (&c)[4][4], int half, float inverse) {
   const uint32_t b[4] = {base.x, base.y, base.z, base.w};
   uint32_t o[4];
 #pragma unroll
@@ -239,7 +238,40 @@ __device__ __forceinline__ void put_row(const Params& p, int n, int t, const uin
     const float2 f = unpack<T>(b[j]);
     o[j] = pack<T>(fmaf(c[j][2 * half], inverse, f.x), fmaf(c[j][2 * half + 1], inverse, f.y));
   }
-  __stcs(reinterpret_cast<uint4*>(p.out + t * p.out_ld + 2ll * n), make_uint4(o[0], o[1], o[2], o[3]));
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+template <class T>
+__device__ __forceinline__ void put_row(const Params& p, int n, int t, const uint4& base, const float (&c)[4][4], int half, float inverse) {
+  if (t < 0 || n >= p.N) return;
+  __stcs(reinterpret_cast<uint4*>(p.out + t * p.out_ld + 2ll * n), sum_row<T>(base, c, half, inverse));
+}
+// A warp's 16 rows of results, columns n0 - 8 .. n0 + 63, to rows of out that start anywhere: the 16-byte blocks of out that end at n0 + 64 or before, what
+// is left waits for the next columns.  Columns from `first` on, where others have those before; `end`: of the last columns, whose rest goes
+// out too.
+__device__ __forceinline__ void put_shifted(const Params& p, const char* results, int pitch, int tokens /* of row `lane` % 16 */, int n0, int first, int end) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = (lane >> 3) + 4 * i, token = __shfl_sync(0xffffffffu, tokens, row);
+    if (token < 0) continue;
+    char* out = p.out + token * p.out_ld;
+    const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(out) & 15) / 2;  // values of out's first block in front of the row
+    for (int k = lane & 7; k < (end != 0x7fffffff ? 9 : 8); k += 8) {
+      const int col = n0 + 8 * k - shift, from = 2 * (8 + 8 * k - shift);
+      if (k == 8 && shift == 0) continue;  // nothing is left
+      const uint4 v = in_place8(results + row * pitch + (from & ~15), from & 15, 8);
+      if (col >= first && col + 8 <= min(end, p.N)) {
+        __stcs(reinterpret_cast<uint4*>(out + 2ll * col), v);
+      } else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (col + j >= first && col + j < min(end, p.N) && 8 * k - shift + j < 64)
+            reinterpret_cast<uint16_t*>(out)[col + j] = static_cast<uint16_t>(w[j / 2] >> (16 * (j & 1)));
+        }
+      }
+    }
+  }
 }
 // Without whole pieces: a warp's 16 rows one by one, a column to a lane, by way of `stage` (16 x 34 floats).  Their base is fetched at once.
 constexpr int kStagePitch = 34;
@@ -305,7 +337,7 @@ __device__ __forceinline__ void direct_columns(const Params& p, const char* b, i
 }
 
 // ----------------------------------------------------------------------------------------------
-// one kernel
+// few rows
 // ----------------------------------------------------------------------------------------------
 __device__ __forceinline__ float load_cluster(uint32_t addr) {
   float f;
@@ -314,12 +346,12 @@ __device__ __forceinline__ float load_cluster(uint32_t addr) {
 }
 
 template <int RP>
-constexpr size_t one_smem() {  // warps' parts or staged rows, the block's part, s
+constexpr size_t few_smem() {  // warps' parts or staged rows, the block's part, s
   return sizeof(float) * (kWarps * 16 * (RP > kStagePitch ? RP : kStagePitch) + 2 * 16 * RP);
 }
 
 template <class T, int RP, bool ALIGNED>
-__global__ void __launch_bounds__(32 * kWarps) one_kernel(const Params p) {
+__global__ void __launch_bounds__(32 * kWarps) few_kernel(const Params p) {
   release_next();
   wait_for_previous();
   extern __shared__ __align__(16) float smem[];
@@ -457,33 +489,9 @@ __global__ void __launch_bounds__(32 * kWarps) one_kernel(const Params p) {
 }
 
 // ----------------------------------------------------------------------------------------------
-// two kernels
+// tiles
 // ----------------------------------------------------------------------------------------------
-// A block has 32, 64 or 128 rows of one adapter (the last block of an adapter what is left), a warp 16 of them; the warps share the weights in
-// shared memory.
-
-// What the first kernel leaves to the second one in the workspace.
-template <int RP>
-struct Between {
-  char* lead;      // (rows, RP) 16-bit, 128 rows more than there are
-  char* rest;      // (rows, RP)
-  float* inverse;  // (rows)
-  int* token;      // (rows), -1: none
-  int4* tile;      // (tiles) adapter (-1: no tile), first row, end
-  __device__ __forceinline__ explicit Between(const Params& p) {
-    const long long rows = (p.rows + 127ll) / 128 * 128 + 128;
-    lead = p.s;
-    rest = lead + rows * 2 * RP;
-    inverse = reinterpret_cast<float*>(rest + rows * 2 * RP);
-    token = reinterpret_cast<int*>(inverse + rows);
-    tile = reinterpret_cast<int4*>(token + rows);
-  }
-};
-static size_t between_bytes(long long rows, long long tiles, int rp) {
-  return static_cast<size_t>((rows + 127) / 128 * 128 + 128) * (4 * rp + 8) + static_cast<size_t>(tiles) * 16;
-}
-
-// The `tile`-th block's adapter, first row and end, adapters in their order (all lanes of the warp); adapter -1 behind the last.  Each lane counts
+// The `tile`-th tile's adapter, first row and end, adapters in their order (all lanes of the warp); adapter -1 behind the last.  Each lane counts
 // the tiles of a run of adapters; then the lanes look at the run that holds the tile.
 __device__ __forceinline__ int4 tile_of(const Params& p, int tile, int tile_rows) {
   const int lane = threadIdx.x & 31;
@@ -529,335 +537,343 @@ __device__ __forceinline__ int4 tile_of(const Params& p, int tile, int tile_rows
   }
 }
 
-// The first: s of a block's rows over a share of the columns of x.  Every warp brings in its own rows of x, the block a, 64 columns in a stage and
-// kAhead stages ahead.  The blocks of a cluster add their parts, each for a share of the rows.  Rows of x that start anywhere come in by the
-// 16-byte blocks that hold them, and are put in place on the way out of shared memory; a is on the way in.
+// Stages of 64 columns, `kStages` of them in turn: RP rows of a (or 64 of b) for the block, and each warp's 16 rows of x (or base), which it brings in
+// itself.  ALIGNED: rows of 128 bytes by asynchronous copies; the halves of odd ones trade places, so that eight lanes of a load meet all
+// banks.  Otherwise rows of x and base come in by the nine 16-byte blocks that hold them and are put in place on the way out of shared
+// memory, weights on the way in.
 template <int RP, bool ALIGNED>
-struct First {
+struct Tile {
   static constexpr int kCols = 64, kStages = 3;
-  static constexpr int kPitch = ALIGNED ? 128 : 192;  // of a row of x; 128: the odd rows' halves trade places, so that eight lanes meet all banks
-  static constexpr int kWarpBytes = 16 * kPitch, kABytes = RP * 128;
+  static constexpr int kPitch = ALIGNED ? 128 : 144, kWarpBytes = 16 * kPitch, kWeightBytes = RP * 128;
+  static constexpr int kOutPitch = 160;  // of a row of results on its way out: eight columns of the stage before, 64, and what a shifted load may touch
+  // of a warp: s (leading bits, the rest), later its results
+  static constexpr int kOwnBytes = 64 * RP > 16 * kOutPitch || ALIGNED ? 64 * RP : 16 * kOutPitch;
   static size_t smem(int warps) {
-    const size_t staging = kStages * static_cast<size_t>(warps * kWarpBytes + kABytes), part = sizeof(float) * 16 * warps * RP;
-    return staging > part ? staging : part;
+    const size_t stages = kStages * static_cast<size_t>(kWeightBytes + warps * kWarpBytes), part = sizeof(float) * 16 * warps * RP;
+    return (stages > part ? stages : part) + static_cast<size_t>(warps) * kOwnBytes + sizeof(float) * 16 * warps;
   }
 };
-// place of the 16-byte block `k` of row `row` in a row of 128 bytes
+// place of the 16-byte block `k` of row `row`
 __device__ __forceinline__ int swizzled(int row, int k) { return 16 * (k ^ ((row & 1) << 2)); }
+// place of block `k` of row `row` among rows of RP 16-bit values
+template <int RP>
+__device__ __forceinline__ int weight_place(int row, int k) { return 2 * RP * row + (RP >= 64 ? swizzled(row, k) : 16 * k); }
 
-template <class T, int RP, bool ALIGNED>
-__global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) first_kernel(const Params p) {
-  release_next();
-  wait_for_previous();
-  using F = First<RP, ALIGNED>;
-  extern __shared__ __align__(128) char staging[];
-  constexpr int COLS = F::kCols, STAGES = F::kStages, NT = RP / 8, C = COLS / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int warps = blockDim.x / 32, tile_rows = 16 * warps;
-  const int tile = blockIdx.x / p.splits, share = blockIdx.x - tile * p.splits;
-  const int4 what = tile_of(p, tile, tile_rows);
-  const Between<RP> between(p);
-  if (share == 0 && threadIdx.x == 0) between.tile[tile] = what;
-  if (what.x < 0) return;  // (the cluster's blocks all see the same)
-  const int e = what.x, row0 = what.y, my_row = row0 + 16 * warp;
-  const int gathered = my_row + (lane & 15) < what.z ? gathered_of(p, my_row + (lane & 15)) : -1;
-  const bool any = __any_sync(0xffffffffu, gathered >= 0);
-  if (share == 0 && lane < 16 && my_row + lane < what.z) between.token[my_row + lane] = gathered >= 0 && p.reverse[gathered] == my_row + lane ? gathered : -1;
-  const int t0 = __shfl_sync(0xffffffffu, gathered, g), t1 = __shfl_sync(0xffffffffu, gathered, g + 8);
-  const char* a = p.a + static_cast<long long>(e) * p.r * p.H * 2;
-  const int all = (p.H + COLS - 1) / COLS;
-  const int first = static_cast<int>(static_cast<long long>(all) * share / p.splits), end = static_cast<int>(static_cast<long long>(all) * (share + 1) / p.splits);
-  const int stage_bytes = F::kABytes + warps * F::kWarpBytes;
-  const auto a_stage = [&](int stage) { return staging + stage % STAGES * stage_bytes; };
-  const auto x_stage = [&](int stage) { return a_stage(stage) + F::kABytes + warp * F::kWarpBytes; };
-  // rows lane / 8, + 4, + 8, + 12 of this warp, block lane % 8 of each
-  const char* x_row[4];
-  int x_off[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int token = __shfl_sync(0xffffffffu, gathered, (lane >> 3) + 4 * i);
-    const char* row = token >= 0 ? p.x + token * p.x_ld : nullptr;
-    x_off[i] = ALIGNED ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15);
-    x_row[i] = token >= 0 ? row - x_off[i] : nullptr;
-  }
-  const auto fetch_x = [&](int stage) {
-    char* to = x_stage(stage);
+__device__ __forceinline__ void store_cluster(uint32_t addr, uint2 v) {
+  asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(v.x), "r"(v.y) : "memory");
+}
+
+// A warp's 16 rows on their way into shared memory: lane l has block l % 8 (and l % 8 = 0 the ninth) of the rows l / 8, + 4, + 8, + 12.
+template <bool ALIGNED, int PITCH>
+struct RowCopy {
+  const char* row[4];  // the row's first block, or nullptr
+  long long bytes[4];  // up to the row's end
+  __device__ __forceinline__ void set(const char* rows, long long ld, int width, int tokens /* of row `lane` % 16 */) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = (lane >> 3) + 4 * i, k = lane & 7;
-      const long long at = 2ll * COLS * stage + 16 * k;  // behind x_row
-      const long long bytes = x_off[i] + 2ll * p.H;      // of the row, from x_row on
-      const bool has = x_row[i] != nullptr && at < bytes;
-      if (ALIGNED) {
-        cp_async16(smem_u32(to + row * F::kPitch + swizzled(row, k)), has ? x_row[i] + at : p.x, has ? 16 : 0);
-      } else {
-        cp_async16(smem_u32(to + row * F::kPitch + 16 * k), has ? x_row[i] + at : p.a - (reinterpret_cast<uintptr_t>(p.a) & 15), has ? 16 : 0);
-        if (k == 0) {  // the ninth block
-          const bool more = x_row[i] != nullptr && at + 128 < bytes;
-          cp_async16(smem_u32(to + row * F::kPitch + 128), more ? x_row[i] + at + 128 : p.a - (reinterpret_cast<uintptr_t>(p.a) & 15), more ? 16 : 0);
-        }
+      const int token = __shfl_sync(0xffffffffu, tokens, (lane >> 3) + 4 * i);
+      const char* p = rows + token * ld;
+      const int off = ALIGNED ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);
+      row[i] = token >= 0 && rows != nullptr ? p - off : nullptr;
+      bytes[i] = off + 2ll * width;
+    }
+  }
+  // columns 64 stage and on; zeros behind the row's end
+  __device__ __forceinline__ void fetch(char* to, int stage, const void* some /* an address for copies of nothing */) const {
+    const int lane = threadIdx.x & 31, k = lane & 7;
+    const char* none = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(some) & ~static_cast<uintptr_t>(15));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = (lane >> 3) + 4 * i;
+      const long long at = 128ll * stage + 16 * k;
+      const bool has = row[i] != nullptr && at < bytes[i];
+      cp_async16(smem_u32(to + r * PITCH + (ALIGNED ? swizzled(r, k) : 16 * k)), has ? row[i] + at : none, has ? 16 : 0);
+      if (!ALIGNED && k == 0) {
+        const bool more = row[i] != nullptr && at + 128 < bytes[i];
+        cp_async16(smem_u32(to + r * PITCH + 128), more ? row[i] + at + 128 : none, more ? 16 : 0);
       }
     }
+  }
+};
+// eight columns from 8 k of a stage on, of row `r`, which begins `off` bytes into its first block; `left`: columns of the row from there on
+template <bool ALIGNED, int PITCH>
+__device__ __forceinline__ uint4 staged_row(const char* from, int r, int k, int off, int left) {
+  if (ALIGNED) return *reinterpret_cast<const uint4*>(from + r * PITCH + swizzled(r, k));
+  return in_place8(from + r * PITCH + 16 * k, off, left);
+}
+
+// One block of rows of weights, RP or 64 of them, 64 or RP columns each, into shared memory by all threads.
+template <bool ALIGNED, class Place>
+__device__ __forceinline__ void fetch_weights(char* to, const char* from, int width /* of a row in memory */, int rows, int rows_left, int col, int cols, Place place) {
+  const int per = cols / 8;
+  for (int i = threadIdx.x; i < rows * per; i += blockDim.x) {
+    const int row = i / per, k = i % per, c = col + 8 * k;
+    const char* p = from + 2ll * width * row;
+    const bool has = row < rows_left && c < width;
+    if (ALIGNED) cp_async16(smem_u32(to + place(row, k)), has ? p + 2ll * c : from, has ? 16 : 0);
+    else *reinterpret_cast<uint4*>(to + place(row, k)) = load8<false>(p, has ? c : width, width);
+  }
+}
+
+template <class T, int RP, bool ALIGNED>
+__global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) tile_kernel(const Params p) {
+  release_next();
+  wait_for_previous();
+  using Ti = Tile<RP, ALIGNED>;
+  extern __shared__ __align__(128) char smem_tile[];
+  constexpr int COLS = Ti::kCols, STAGES = Ti::kStages, PITCH = Ti::kPitch, NT = RP / 8, C = COLS / 32, K = Steps<RP>::K, L = Steps<RP>::L;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, warps = blockDim.x / 32, tile_rows = 16 * warps;
+  const int tile = blockIdx.x / p.cluster, share = blockIdx.x - tile * p.cluster;
+  if (tile >= p.tiles) {
+    const long long first = static_cast<long long>(p.tiles) * p.cluster;
+    copy_others(p, 16, (blockIdx.x - first) * warps + warp, (gridDim.x - first) * warps);
+    return;
+  }
+  const int4 what = tile_of(p, tile, tile_rows);
+  if (what.x < 0) return;  // (the cluster's blocks all see the same)
+  const int e = what.x, my_row = what.y + 16 * warp + (lane & 15);
+  const int gathered = my_row < what.z ? gathered_of(p, my_row) : -1;
+  const bool any = __any_sync(0xffffffffu, gathered >= 0);
+  const int row_of = gathered >= 0 ? p.reverse[gathered] : -1;  // what is read of a token does not wait for the check that the row is still its own
+  const int stage_bytes = Ti::kWeightBytes + warps * Ti::kWarpBytes;
+  const auto weights_in = [&](int stage) { return smem_tile + stage % STAGES * stage_bytes; };
+  const auto rows_in = [&](int stage) { return weights_in(stage) + Ti::kWeightBytes + warp * Ti::kWarpBytes; };
+  const size_t ring = max(static_cast<size_t>(STAGES) * stage_bytes, sizeof(float) * tile_rows * RP);
+  char* own = smem_tile + ring;                                                // [warp][lead: 16 x RP, rest: 16 x RP]
+  float* inverses = reinterpret_cast<float*>(own + warps * Ti::kOwnBytes);     // [tile_rows]
+  const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+  const auto range = [&](int all, int& first, int& end) {
+    first = static_cast<int>(static_cast<long long>(all) * share / p.cluster);
+    end = static_cast<int>(static_cast<long long>(all) * (share + 1) / p.cluster);
   };
-  const auto fetch_a = [&](int stage) {
-    if (stage >= end) return;
-    char* to = a_stage(stage);
-    for (int at = threadIdx.x; at < RP * 8; at += blockDim.x) {
-      const int row = at >> 3, k = at & 7, col = COLS * stage + 8 * k;
-      const char* from = a + static_cast<long long>(row) * p.H * 2;
-      const bool has = row < p.r && col < p.H;
-      if (ALIGNED) cp_async16(smem_u32(to + 128 * row + swizzled(row, k)), has ? from + 2ll * col : p.a, has ? 16 : 0);
-      else *reinterpret_cast<uint4*>(to + 128 * row + swizzled(row, k)) = load8<false>(from, has ? col : p.H, p.H);
-    }
-  };
+
+  // s, of this block's columns of x
   float acc[NT][4];
 #pragma unroll
   for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-  const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) {
-    if (any && first + i < end) fetch_x(first + i);
-    fetch_a(first + i);
-    commit();
-  }
-  // where this lane's rows of x begin in their blocks
-  const int o0 = ALIGNED || t0 < 0 ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(p.x + t0 * p.x_ld) & 15);
-  const int o1 = ALIGNED || t1 < 0 ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(p.x + t1 * p.x_ld) & 15);
-  for (int stage = first; stage < end; ++stage) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-    __syncthreads();  // the stage is there for all, and the one that comes next into its place has been read
-    if (any && stage + STAGES - 1 < end) fetch_x(stage + STAGES - 1);
-    fetch_a(stage + STAGES - 1);
-    commit();
-    if (!any) continue;
-    const char* x = x_stage(stage);
-    const char* w_from = a_stage(stage);
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      uint4 x0, x1;
-      if (ALIGNED) {
-        x0 = *reinterpret_cast<const uint4*>(x + g * F::kPitch + swizzled(g, 4 * c + t));
-        x1 = *reinterpret_cast<const uint4*>(x + (g + 8) * F::kPitch + swizzled(g, 4 * c + t));
-      } else {
-        const int left = p.H - (COLS * stage + 32 * c + 8 * t);
-        x0 = in_place8(x + g * F::kPitch + 16 * (4 * c + t), o0, left);
-        x1 = in_place8(x + (g + 8) * F::kPitch + 16 * (4 * c + t), o1, left);
+  {
+    int first, end;
+    range((p.H + COLS - 1) / COLS, first, end);
+    const char* a = p.a + static_cast<long long>(e) * p.r * p.H * 2;
+    RowCopy<ALIGNED, PITCH> x;
+    x.set(p.x, p.x_ld, p.H, gathered);
+    const auto fetch = [&](int stage) {
+      if (stage < end) {
+        if (any) x.fetch(rows_in(stage), stage, p.x);
+        fetch_weights<ALIGNED>(weights_in(stage), a, p.H, RP, p.r, COLS * stage, COLS, [](int row, int k) { return 128 * row + swizzled(row, k); });
       }
+      commit();
+    };
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const uint4 w = *reinterpret_cast<const uint4*>(w_from + 128 * (8 * j + g) + swizzled(g, 4 * c + t));
-        mma<T>(acc[j], x0.x, x1.x, x0.y, x1.y, w.x, w.y);
-        mma<T>(acc[j], x0.z, x1.z, x0.w, x1.w, w.z, w.w);
+    for (int i = 0; i < STAGES - 1; ++i) fetch(first + i);
+    const int t0 = __shfl_sync(0xffffffffu, gathered, g), t1 = __shfl_sync(0xffffffffu, gathered, g + 8);
+    const int o0 = ALIGNED ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(p.x + t0 * p.x_ld) & 15), o1 = ALIGNED ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(p.x + t1 * p.x_ld) & 15);
+    for (int stage = first; stage < end; ++stage) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+      __syncthreads();  // the stage is there for all, and the one whose place the next takes has been read
+      fetch(stage + STAGES - 1);
+      if (!any) continue;
+      const char* xs = rows_in(stage);
+      const char* ws = weights_in(stage);
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int left = p.H - (COLS * stage + 32 * c + 8 * t);
+        const uint4 x0 = staged_row<ALIGNED, PITCH>(xs, g, 4 * c + t, o0, left), x1 = staged_row<ALIGNED, PITCH>(xs, g + 8, 4 * c + t, o1, left);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const uint4 w = *reinterpret_cast<const uint4*>(ws + 128 * (8 * j + g) + swizzled(g, 4 * c + t));
+          mma<T>(acc[j], x0.x, x1.x, x0.y, x1.y, w.x, w.y);
+          mma<T>(acc[j], x0.z, x1.z, x0.w, x1.w, w.z, w.w);
+        }
       }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  __syncthreads();
-  float* part = reinterpret_cast<float*>(staging);  // [tile_rows][RP]
+
+  // the blocks add their parts, each for a share of the rows, and give all of them the sums
+  float* part = reinterpret_cast<float*>(smem_tile);  // [tile_rows][RP]
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     float* to = part + (16 * warp + g) * RP + 8 * j + 2 * t;
     *reinterpret_cast<float2*>(to) = make_float2(acc[j][0], acc[j][1]);
     *reinterpret_cast<float2*>(to + 8 * RP) = make_float2(acc[j][2], acc[j][3]);
   }
-  if (p.splits > 1) cluster_sync_all(); else __syncthreads();
-  // rows share * tile_rows / splits and on, four columns to a thread
-  constexpr int Q = RP / 4;
-  const int mine = tile_rows / p.splits, begin = share * mine;
-  const float scale = p.scale != nullptr ? p.scale[e] : 1.f;
-  uint2* lead = reinterpret_cast<uint2*>(between.lead);
-  uint2* rest = reinterpret_cast<uint2*>(between.rest);
-  for (int first_of = 0; first_of < mine * Q; first_of += blockDim.x) {  // (all threads, for the shuffles)
-    const int i = first_of + threadIdx.x;
-    const bool live = i < mine * Q;
-    const int row = begin + (live ? i / Q : 0), q = i % Q;
-    float f[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < p.splits; ++k) {
-      const uint32_t at = smem_u32(part + row * RP + 4 * q), from = p.splits > 1 ? map_to_cta(at, k) : at;
-      float v[4];
-      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(from) : "memory");
+  cluster_sync_all();
+  {
+    const float scale = p.scale != nullptr ? p.scale[e] : 1.f;
+    constexpr int Q = RP / 4;  // threads of a row, four columns each
+    const int mine = tile_rows / p.cluster;
+    for (int first_of = 0; first_of < mine * Q; first_of += blockDim.x) {  // (all threads, for the shuffles)
+      const int i = first_of + threadIdx.x;
+      const bool live = i < mine * Q;
+      const int row = share * mine + (live ? i / Q : 0), q = i % Q;
+      float f[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < p.cluster; ++k) {
+        float v[4];
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(map_to_cta(smem_u32(part + row * RP + 4 * q), k)) : "memory");
 #pragma unroll
-      for (int j = 0; j < 4; ++j) f[j] += v[j];
-    }
-    float most = 0.f;
+        for (int j = 0; j < 4; ++j) f[j] += v[j];
+      }
+      float most = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f[j] *= scale;
-      most = fmaxf(most, fabsf(f[j]));
-    }
+      for (int j = 0; j < 4; ++j) {
+        f[j] *= scale;
+        most = fmaxf(most, fabsf(f[j]));
+      }
 #pragma unroll
-    for (int o = 1; o < Q; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    const float factor = factor_of<T>(most);
-    uint2 l, r;
-    split2<T>(f[0] * factor, f[1] * factor, l.x, r.x);
-    split2<T>(f[2] * factor, f[3] * factor, l.y, r.y);
-    const long long at = static_cast<long long>(row0 + row) * Q + q;
-    if (live && row0 + row < what.z) {
-      lead[at] = l;
-      rest[at] = r;
-      if (q == 0) between.inverse[row0 + row] = inverse_of<T>(factor);
+      for (int o = 1; o < Q; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      const float factor = factor_of<T>(most);
+      uint2 lead, rest;
+      split2<T>(f[0] * factor, f[1] * factor, lead.x, rest.x);
+      split2<T>(f[2] * factor, f[3] * factor, lead.y, rest.y);
+      if (live) {
+        const uint32_t to = smem_u32(own + row / 16 * Ti::kOwnBytes) + weight_place<RP>(row % 16, q / 2) + 8 * (q & 1);
+        for (int k = 0; k < p.cluster; ++k) {
+          store_cluster(map_to_cta(to, k), lead);
+          store_cluster(map_to_cta(to + 32 * RP, k), rest);
+          if (std::is_same<T, __half>::value && q == 0)
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_cta(smem_u32(inverses + row), k)), "f"(inverse_of<T>(factor)) : "memory");
+        }
+      }
     }
   }
-  if (p.splits > 1) cluster_sync_all();  // the others have read this block's part
-}
+  cluster_sync_all();
 
-// The second: a block's rows by a share of the columns of out.
-constexpr int kShareCols = 256;
-template <int RP>
-struct Second {
-  static constexpr int kPitch = RP <= 32 ? 2 * RP : 2 * RP + 64;  // 64 bytes beyond a multiple of 128, so that eight lanes of a load meet all banks
-  static constexpr size_t kSmem = kShareCols * kPitch;
-};
-
-template <class T, int RP, bool ALIGNED>
-__global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) second_kernel(const Params p) {
-  release_next();
-  wait_for_previous();
-  extern __shared__ __align__(16) char weights[];
-  constexpr int PITCH = Second<RP>::kPitch, K = Steps<RP>::K, L = Steps<RP>::L;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int shares = (p.N + kShareCols - 1) / kShareCols;
-  const int tile = blockIdx.x / shares, n_first = (blockIdx.x - tile * shares) * kShareCols;
-  if (tile >= p.tiles) {
-    const long long first = static_cast<long long>(p.tiles) * shares;
-    copy_others(p, 16, (blockIdx.x - first) * (blockDim.x / 32) + warp, (gridDim.x - first) * (blockDim.x / 32));
-    return;
-  }
-  const Between<RP> between(p);
-  const int4 what = between.tile[tile];
-  if (what.x < 0) return;
-  const int my_row = what.y + 16 * warp;
-  const int tokens = my_row + (lane & 15) < what.z ? between.token[my_row + (lane & 15)] : -1;
-  const char* b = p.b + static_cast<long long>(what.x) * p.N * p.r * 2;
-  for (int i = threadIdx.x; i < kShareCols * (RP / 8); i += blockDim.x) {
-    const int row = i / (RP / 8), k = i % (RP / 8), n = n_first + row;
-    const bool has = n < p.N && 8 * k < p.r;
-    const char* from = b + static_cast<long long>(n) * p.r * 2;
-    if (ALIGNED) cp_async16(smem_u32(weights + row * PITCH + 16 * k), has ? from + 16 * k : p.b, has ? 16 : 0);
-    else *reinterpret_cast<uint4*>(weights + row * PITCH + 16 * k) = load8<false>(from, has ? 8 * k : p.r, p.r);
-  }
+  // this block's columns of out
+  int first, end;
+  range((p.N + COLS - 1) / COLS, first, end);
+  const char* b = p.b + static_cast<long long>(e) * p.N * p.r * 2;
+  const int tokens = row_of == my_row ? gathered : -1;
+  const bool writes = __any_sync(0xffffffffu, tokens >= 0);
   const int t0 = __shfl_sync(0xffffffffu, tokens, g), t1 = __shfl_sync(0xffffffffu, tokens, g + 8);
-  const bool any = __any_sync(0xffffffffu, tokens >= 0);
+  RowCopy<ALIGNED, PITCH> base;
+  base.set(p.base, p.base_ld, p.N, tokens);
+  const auto fetch = [&](int stage) {
+    if (stage < end) {
+      if (writes && p.base != nullptr) base.fetch(rows_in(stage), stage, p.x);
+      fetch_weights<ALIGNED>(weights_in(stage), b + 2ll * COLS * stage * p.r, p.r, COLS, p.N - COLS * stage, 0, RP, weight_place<RP>);
+    }
+    commit();
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) fetch(first + i);
   uint32_t lead[K][4], rest[K][4];
-  float i0 = 1.f, i1 = 1.f;
-  constexpr int AHEAD = 2;  // groups whose base is fetched together: 128 bytes of a row
-  BaseRows<T> base[AHEAD];
-  const int groups = min(kShareCols, p.N - n_first + kGroup - 1) / kGroup;
-  if (any) {
-    const uint2* lead0 = reinterpret_cast<const uint2*>(between.lead) + static_cast<long long>(my_row + g) * (RP / 4);
-    const uint2* rest0 = reinterpret_cast<const uint2*>(between.rest) + static_cast<long long>(my_row + g) * (RP / 4);
+  {
+    const char* mine = own + warp * Ti::kOwnBytes;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int q = RP == 16 ? t : 8 * (k / 2) + 2 * t + (k & 1);  // four columns each
-      const uint2 u = lead0[q], v = lead0[8 * (RP / 4) + q], ur = rest0[q], vr = rest0[8 * (RP / 4) + q];
-      lead[k][0] = u.x; lead[k][1] = v.x; lead[k][2] = u.y; lead[k][3] = v.y;
-      rest[k][0] = ur.x; rest[k][1] = vr.x; rest[k][2] = ur.y; rest[k][3] = vr.y;
-    }
-    if (std::is_same<T, __half>::value) {
-      i0 = between.inverse[my_row + g];
-      i1 = between.inverse[my_row + g + 8];
-    }
-    if (ALIGNED) {
+    for (int l = 0; l < L; ++l) {
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) base[i].load(p, i < groups ? n_first + kGroup * i + 8 * t : p.N, t0, t1);
+      for (int h = 0; h < 2; ++h) {  // rows g and g + 8
+        if constexpr (RP == 16) {
+          const uint2 u = *reinterpret_cast<const uint2*>(mine + weight_place<RP>(g + 8 * h, 0) + 8 * t), v = *reinterpret_cast<const uint2*>(mine + 32 * RP + weight_place<RP>(g + 8 * h, 0) + 8 * t);
+          lead[0][h] = u.x; lead[0][2 + h] = u.y;
+          rest[0][h] = v.x; rest[0][2 + h] = v.y;
+        } else {
+          const uint4 u = *reinterpret_cast<const uint4*>(mine + weight_place<RP>(g + 8 * h, 4 * l + t)), v = *reinterpret_cast<const uint4*>(mine + 32 * RP + weight_place<RP>(g + 8 * h, 4 * l + t));
+          lead[2 * l][h] = u.x; lead[2 * l][2 + h] = u.y; lead[2 * l + 1][h] = u.z; lead[2 * l + 1][2 + h] = u.w;
+          rest[2 * l][h] = v.x; rest[2 * l][2 + h] = v.y; rest[2 * l + 1][h] = v.z; rest[2 * l + 1][2 + h] = v.w;
+        }
+      }
     }
   }
-  cp_async_wait_all();
-  __syncthreads();
-  if (!any) return;
-  __shared__ float staged[ALIGNED ? 1 : kWarps * 16 * kStagePitch];
-  for (int group = 0; group < groups; group += AHEAD) {
-    BaseRows<T> next[AHEAD];
-    BaseColumn column[ALIGNED ? 1 : AHEAD];
+  const float i0 = std::is_same<T, __half>::value ? inverses[16 * warp + g] : 1.f, i1 = std::is_same<T, __half>::value ? inverses[16 * warp + g + 8] : 1.f;
+  const int o0 = ALIGNED ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(p.base + t0 * p.base_ld) & 15), o1 = ALIGNED ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(p.base + t1 * p.base_ld) & 15);
+  __syncwarp();  // s has been read: the results may lie there
+  char* results = own + warp * Ti::kOwnBytes;
+  for (int stage = first; stage < end; ++stage) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    __syncthreads();
+    fetch(stage + STAGES - 1);
+    if (!writes) continue;
+    const char* bs = rows_in(stage);
+    const char* ws = weights_in(stage);
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      if (ALIGNED) next[i].load(p, group + AHEAD + i < groups ? n_first + kGroup * (group + AHEAD + i) + 8 * t : p.N, t0, t1);
-      else column[i].load(p, group + i < groups ? n_first + kGroup * (group + i) + lane : p.N, tokens);
-    }
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      if (group + i >= groups) break;
-      const int n0 = n_first + kGroup * (group + i);
+    for (int i = 0; i < C; ++i) {
+      const int n0 = COLS * stage + kGroup * i;
       float c[4][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
-        const char* row = weights + (kGroup * (group + i) + out_column(g, j)) * PITCH;
+        const int row = kGroup * i + out_column(g, j);
 #pragma unroll
         for (int l = 0; l < L; ++l) {
           uint4 w = make_uint4(0u, 0u, 0u, 0u);
           if constexpr (RP == 16) {
-            const uint2 h = *reinterpret_cast<const uint2*>(row + 8 * t);
+            const uint2 h = *reinterpret_cast<const uint2*>(ws + weight_place<RP>(row, 0) + 8 * t);
             w.x = h.x;
             w.y = h.y;
           } else {
-            w = *reinterpret_cast<const uint4*>(row + 64 * l + 16 * t);
+            w = *reinterpret_cast<const uint4*>(ws + weight_place<RP>(row, 4 * l + t));
           }
           step<T, RP>(c[j], lead, rest, l, w);
         }
       }
+      uint4 b0 = make_uint4(0u, 0u, 0u, 0u), b1 = b0;
+      if (p.base != nullptr) {
+        const int left = p.N - (n0 + 8 * t);
+        b0 = staged_row<ALIGNED, PITCH>(bs, g, 4 * i + t, o0, left);
+        b1 = staged_row<ALIGNED, PITCH>(bs, g + 8, 4 * i + t, o1, left);
+      }
+      const uint4 r0 = sum_row<T>(b0, c, 0, i0), r1 = sum_row<T>(b1, c, 1, i1);
       if (ALIGNED) {
-        put_row<T>(p, n0 + 8 * t, t0, base[i].v[0], c, 0, i0);
-        put_row<T>(p, n0 + 8 * t, t1, base[i].v[1], c, 1, i1);
+        const int n = n0 + 8 * t;
+        if (t0 >= 0 && n < p.N) __stcs(reinterpret_cast<uint4*>(p.out + t0 * p.out_ld + 2ll * n), r0);
+        if (t1 >= 0 && n < p.N) __stcs(reinterpret_cast<uint4*>(p.out + t1 * p.out_ld + 2ll * n), r1);
       } else {
-        put_staged<T>(p, n0, tokens, column[ALIGNED ? 0 : i], c, i0, i1, staged + warp * 16 * kStagePitch);
+        *reinterpret_cast<uint4*>(results + g * Ti::kOutPitch + 16 + 64 * i + 16 * t) = r0;
+        *reinterpret_cast<uint4*>(results + (g + 8) * Ti::kOutPitch + 16 + 64 * i + 16 * t) = r1;
       }
     }
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) base[i] = next[i];
+    if (!ALIGNED) {
+      __syncwarp();
+      put_shifted(p, results, Ti::kOutPitch, tokens, COLS * stage, COLS * first, stage + 1 == end ? min(COLS * end, p.N) : 0x7fffffff);
+      __syncwarp();
+      if (lane < 16) *reinterpret_cast<uint4*>(results + lane * Ti::kOutPitch) = *reinterpret_cast<const uint4*>(results + lane * Ti::kOutPitch + 128);
+      __syncwarp();
+    }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // ----------------------------------------------------------------------------------------------
 // launches
 // ----------------------------------------------------------------------------------------------
 static int padded_rank(int r) { return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : 128; }
-static bool in_one_kernel(int T, int n) {
+static bool by_few_rows(int T, int n) {
   const long long tiles = T / 16 + static_cast<long long>(n < T ? n : T);  // of 16 rows, at most (or as many as there are tokens)
   return (tiles < T ? tiles : T) <= 256;
 }
-// Warps of a block of the two kernels, by the tokens that an adapter has on average.
+// Warps of tile_kernel's blocks, by the tokens that an adapter has on average.
 static int warps_of(int T, int n) { return T / n <= 32 ? 2 : T / n <= 64 ? 4 : 8; }
-// Blocks' tiles, at most: every adapter's last one may be part of a tile.
+// Its tiles, at most: every adapter's last one may be a part of one.
 static long long tiles_of(int T, long long rows, int n) {
   return rows / (16 * warps_of(T, n)) + (n < T ? n : T);
 }
-static size_t round256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
-
 template <class T, int RP, bool ALIGNED>
 static int launch(Params p, cudaStream_t st) {
   static PerDeviceFlag configured;
   const int dev = current_device();
   if (dev < 0) return SMOE_ERR_DRIVER;
   if (!configured.test(dev)) {
-    if (cudaFuncSetAttribute(one_kernel<T, RP, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(one_smem<RP>())) != cudaSuccess ||
-        cudaFuncSetAttribute(first_kernel<T, RP, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(First<RP, ALIGNED>::smem(kWarps))) != cudaSuccess ||
-        cudaFuncSetAttribute(second_kernel<T, RP, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Second<RP>::kSmem)) != cudaSuccess)
+    if (cudaFuncSetAttribute(few_kernel<T, RP, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(few_smem<RP>())) != cudaSuccess ||
+        cudaFuncSetAttribute(tile_kernel<T, RP, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Tile<RP, ALIGNED>::smem(kWarps))) != cudaSuccess)
       return SMOE_ERR_LAUNCH;
     configured.set(dev);
   }
-  if (in_one_kernel(p.T, p.n)) {
-    p.tiles = (p.rows + 15) / 16;
-    const long long others = p.in_place ? 0 : (p.T + 8ll * kCluster * kWarps - 1) / (8 * kCluster * kWarps);  // clusters, eight tokens to a warp
-    const long long blocks = (p.tiles + others) * kCluster;
-    if (blocks == 0) return SMOE_OK;
-    return launched(launch_chained(one_kernel<T, RP, ALIGNED>, dim3(static_cast<unsigned>(blocks)), 32 * kWarps, one_smem<RP>(), st, kCluster, p));
-  }
-  const int warps = warps_of(p.T, p.n);
-  p.tiles = static_cast<int>(tiles_of(p.T, p.rows, p.n));
-  const int full = (p.T + 16 * warps - 1) / (16 * warps);
-  p.splits = full >= 148 ? 1 : full >= 74 ? 2 : full >= 37 ? 4 : 8;
-  int kernels = 0;
-  if (p.tiles > 0) {
-    const cudaError_t rc = launch_chained(first_kernel<T, RP, ALIGNED>, dim3(static_cast<unsigned>(p.tiles * p.splits)), 32 * warps, First<RP, ALIGNED>::smem(warps), st, p.splits, p);
-    if (rc != cudaSuccess) return SMOE_ERR_LAUNCH;
-    ++kernels;
-  }
-  const int shares = (p.N + kShareCols - 1) / kShareCols;
-  const long long others = p.in_place ? 0 : (p.T + 8ll * warps - 1) / (8 * warps);
-  const long long blocks = static_cast<long long>(p.tiles) * shares + others;
-  if (blocks == 0) return launched(cudaSuccess, kernels);
-  return launched(launch_chained(second_kernel<T, RP, ALIGNED>, dim3(static_cast<unsigned>(blocks)), 32 * warps, Second<RP>::kSmem, st, 1, p), kernels + 1);
+  const bool few = by_few_rows(p.T, p.n);
+  const int warps = few ? kWarps : warps_of(p.T, p.n);
+  // (eight blocks to 16 rows at most, and less than one to eight of the other tokens: less than 2^31)
+  p.tiles = static_cast<int>(few ? (p.rows + 15) / 16 : tiles_of(p.T, p.rows, p.n));
+  const int full = (p.T + 16 * warps - 1) / (16 * warps);  // tiles, if they were all full
+  p.cluster = few ? kCluster : full > 148 ? 1 : full > 74 ? 2 : full > 37 ? 4 : 8;
+  const long long to_a_cluster = 8ll * warps * p.cluster;  // eight tokens to a warp
+  const long long others = p.in_place ? 0 : (p.T + to_a_cluster - 1) / to_a_cluster, blocks = (p.tiles + others) * p.cluster;
+  if (blocks == 0) return SMOE_OK;
+  return launched(few ? launch_chained(few_kernel<T, RP, ALIGNED>, dim3(static_cast<unsigned>(blocks)), 32 * warps, few_smem<RP>(), st, p.cluster, p)
+                      : launch_chained(tile_kernel<T, RP, ALIGNED>, dim3(static_cast<unsigned>(blocks)), 32 * warps, Tile<RP, ALIGNED>::smem(warps), st, p.cluster, p));
 }
 template <class T, bool ALIGNED>
 static int launch(const Params& p, cudaStream_t st) {
@@ -879,31 +895,20 @@ using namespace smoe::adapters;
 
 extern "C" {
 
-size_t smoe_adapter_linear_workspace_bytes(int T, long long rows, int n, int r) {
-  if (T <= 0 || rows <= 0 || n <= 0 || r <= 0 || r > kMaxRank || in_one_kernel(T, n)) return 0;
-  return round256(between_bytes(rows, tiles_of(T, rows, n), padded_rank(r)));
-}
-
 int smoe_adapter_linear(const void* x, long long ld, const void* a, const void* b, const float* scale, const void* base, long long base_ld,
                         void* out, long long out_ld, int dtype, const int* expert_frequency_offset, const int* x_gather_idx,
-                        const int* s_reverse_scatter_idx, int T, long long rows, int H, int N, int n, int r, int align, void* workspace,
-                        void* stream) {
+                        const int* s_reverse_scatter_idx, int T, long long rows, int H, int N, int n, int r, int align, void* stream) {
   if (dtype != SMOE_BF16 && dtype != SMOE_F16) return SMOE_ERR_DTYPE;
   if (T < 0 || T > kMaxRows || rows < 0 || rows > kMaxRows || H <= 0 || N <= 0 || n <= 0 || n > kMaxAdapters || r <= 0 || r > kMaxRank || align <= 0 ||
       align % 16 != 0 || ld < 0 || base_ld < 0 || out_ld < N)
     return SMOE_ERR_SHAPE;
   if (H > 1 << 28 || N > 1 << 28) return SMOE_ERR_SHAPE;
-  // blocks: eight to 16 rows of one kernel, up to eight and one to 256 columns for 128 rows of two; and those of the other tokens
-  if ((in_one_kernel(T, n) ? (rows + 15) / 16 * kCluster : tiles_of(T, rows, n) * (8ll + (N + kShareCols - 1) / kShareCols)) + T / 8 + kCluster > 0x7fffffffll)
-    return SMOE_ERR_SHAPE;
   if (T == 0) return SMOE_OK;
   if (x == nullptr || a == nullptr || b == nullptr || out == nullptr || expert_frequency_offset == nullptr || s_reverse_scatter_idx == nullptr ||
       (rows > 0 && x_gather_idx == nullptr))
     return SMOE_ERR_SHAPE;
-  const size_t ws = smoe_adapter_linear_workspace_bytes(T, rows, n, r);
-  if (ws > 0 && workspace == nullptr) return SMOE_ERR_WORKSPACE;
   if ((address(x) | address(a) | address(b) | address(base) | address(out)) % 2 != 0 ||
-      (address(scale) | address(expert_frequency_offset) | address(x_gather_idx) | address(s_reverse_scatter_idx)) % 4 != 0 || address(workspace) % 256 != 0)
+      (address(scale) | address(expert_frequency_offset) | address(x_gather_idx) | address(s_reverse_scatter_idx)) % 4 != 0)
     return SMOE_ERR_ALIGNMENT;
   Params p = {};
   p.x = static_cast<const char*>(x); p.x_ld = 2 * ld;
@@ -911,7 +916,6 @@ int smoe_adapter_linear(const void* x, long long ld, const void* a, const void* 
   p.base = static_cast<const char*>(base); p.base_ld = base != nullptr ? 2 * base_ld : 0;
   p.out = static_cast<char*>(out); p.out_ld = 2 * out_ld;
   p.off = expert_frequency_offset; p.gather = x_gather_idx; p.reverse = s_reverse_scatter_idx;
-  p.s = static_cast<char*>(workspace);
   p.T = T; p.rows = static_cast<int>(rows); p.H = H; p.N = N; p.n = n; p.r = r;
   p.in_place = base == out && base_ld == out_ld;
   const bool aligned = (address(x) | address(a) | address(b) | address(base) | address(out) | p.x_ld | p.base_ld | p.out_ld) % 16 == 0 && H % 8 == 0 &&

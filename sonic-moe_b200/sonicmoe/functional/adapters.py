@@ -100,10 +100,8 @@ def adapter_linear(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, permutatio
         # (the distance of a single row means nothing)
         base_ld = 0 if base is None else base.stride(0) if T > 1 else max(N, base.stride(0))
         out = base if inplace else torch.empty(T, N, dtype=x.dtype, device=dev)
-        ws = lib.smoe_adapter_linear_workspace_bytes(T, rows, n, r)
-        ws = _lib.workspace(ws, dev) if ws else None
         check(lib.smoe_adapter_linear(
             x.data_ptr(), x.stride(0), a.data_ptr(), b.data_ptr(), ptr(scale), ptr(base), base_ld, out.data_ptr(),
             base_ld if inplace else N, _TYPES[x.dtype], offset.data_ptr(), row.data_ptr(), pair.data_ptr(), T, rows, H, N, n, r, align,
-            ptr(ws), stream_ptr(dev)), "adapter_linear")
+            stream_ptr(dev)), "adapter_linear")
     return out
