@@ -1,6 +1,8 @@
 // Root-mean-square norm, gradients (the formulas are in norm.cuh).
 #include "norm.cuh"
 
+#include <atomic>
+
 namespace smoe {
 namespace norm {
 
@@ -188,14 +190,23 @@ __global__ void __launch_bounds__(32 * kShares) weight_grad_kernel(const float* 
 }
 
 // Blocks of `kernel`: as many as the device holds at a time, at most one for each `subs` rows, and where rows have different shifts a multiple of
-// their number (8 or 4), unless no block has a second row; 0 on failure.
+// their number (8 or 4), unless no block has a second row; 0 on failure.  `known`: the last answer of the runtime for this kernel and device.
+struct Residency {
+  std::atomic<unsigned long long> last[kMaxDevices] = {};  // threads, shared memory, blocks on an SM
+};
 template <class T, bool ALIGNED, class... Params>
-static int blocks_of(void (*kernel)(Params...), int threads, size_t smem, long long rows, int subs) {
+static int blocks_of(void (*kernel)(Params...), int threads, size_t smem, long long rows, int subs, Residency& known) {
   const long long need = (rows + subs - 1) / subs;
-  const int sms = num_sms();
+  const int sms = num_sms(), dev = current_device();
+  if (sms <= 0 || dev < 0) return 0;
   if (need <= sms) return static_cast<int>(need);
-  int per = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, threads, smem) != cudaSuccess || per <= 0 || sms <= 0) return 0;
+  const unsigned long long key = static_cast<unsigned long long>(threads) << 48 | static_cast<unsigned long long>(smem) << 16;
+  const unsigned long long last = known.last[dev].load(std::memory_order_relaxed);
+  int per = static_cast<int>(last & 0xFFFF);
+  if (last >> 16 != key >> 16) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, threads, smem) != cudaSuccess || per <= 0) return 0;
+    known.last[dev].store(key | static_cast<unsigned long long>(per), std::memory_order_relaxed);
+  }
   long long all = static_cast<long long>(per) * sms;
   if (all > kMostBlocks) all = kMostBlocks;
   if (need <= all) return static_cast<int>(need);
@@ -205,7 +216,8 @@ static int blocks_of(void (*kernel)(Params...), int threads, size_t smem, long l
 template <class T, class W, int EP, bool ALIGNED, int REGISTERS>
 static cudaError_t launch_rows(const Backward& a, const Shape& s, int& blocks, cudaStream_t st) {
   const size_t smem = s.subs > 1 ? static_cast<size_t>(s.subs) * a.H * sizeof(float) : 0;  // subs H <= 256 EP
-  blocks = blocks_of<T, ALIGNED>(backward_kernel<T, W, EP, ALIGNED, REGISTERS>, s.threads, smem, a.rows, s.subs);
+  static Residency known;
+  blocks = blocks_of<T, ALIGNED>(backward_kernel<T, W, EP, ALIGNED, REGISTERS>, s.threads, smem, a.rows, s.subs, known);
   if (blocks == 0) return cudaErrorInvalidConfiguration;
   return launch_chained(backward_kernel<T, W, EP, ALIGNED, REGISTERS>, dim3(static_cast<unsigned>(blocks)), s.threads, smem, st, 1, a, s.tpr);
 }
@@ -222,7 +234,8 @@ static cudaError_t launch_backward(const Backward& a, int& blocks, cudaStream_t 
     if (ALIGNED ? values < 256 : values <= 16 * 256) return launch_rows<T, W, 16, ALIGNED, 80>(a, shape_of(values, 16), blocks, st);
     if (values <= 32 * kThreads) return launch_rows<T, W, 32, ALIGNED, 128>(a, shape_of(values, 32), blocks, st);
   }
-  blocks = blocks_of<T, ALIGNED>(backward_long_kernel<T, W, 16, ALIGNED>, kThreads, 0, a.rows, 1);
+  static Residency known;
+  blocks = blocks_of<T, ALIGNED>(backward_long_kernel<T, W, 16, ALIGNED>, kThreads, 0, a.rows, 1, known);
   if (blocks == 0) return cudaErrorInvalidConfiguration;
   return launch_chained(backward_long_kernel<T, W, 16, ALIGNED>, dim3(static_cast<unsigned>(blocks)), kThreads, 0, st, 1, a);
 }

@@ -99,7 +99,7 @@ def adapter_linear(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, permutatio
             base = base.contiguous()
         # (the distance of a single row means nothing)
         base_ld = 0 if base is None else base.stride(0) if T > 1 else max(N, base.stride(0))
-        out = base if inplace else torch.empty(T, N, dtype=x.dtype, device=dev)
+        out = base if inplace else torch.empty_like(base) if base is not None and base.is_contiguous() else x.new_empty((T, N))
         check(lib.smoe_adapter_linear(
             x.data_ptr(), x.stride(0), a.data_ptr(), b.data_ptr(), ptr(scale), ptr(base), base_ld, out.data_ptr(),
             base_ld if inplace else N, _TYPES[x.dtype], offset.data_ptr(), row.data_ptr(), pair.data_ptr(), T, rows, H, N, n, r, align,

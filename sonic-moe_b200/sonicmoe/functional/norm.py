@@ -63,26 +63,33 @@ def _check(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.Te
         raise ValueError(f"{x.numel() // H} rows do not fit into 32-bit numbers")
 
 
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor of the shape and type of x (a copy of its layout is the cheapest way to one)."""
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+
+
 def _norm(x, weight, eps, residual, keep_rstd=False, keep_y=True, quantise=False):
     """(y, h, rstd, q, scale), each None where it is not asked for; h is None without a residual."""
-    rows, H, dev, dtype = x.numel() // x.shape[-1], x.shape[-1], x.device, x.dtype
+    shape, dev, code = x.shape, x.device, _ROW_TYPES[x.dtype]
+    H = shape[-1]
+    rows = x.numel() // H
     with _lib.on_device(dev):
         x2 = _as_rows(x)
-        r2 = None if residual is None else _as_rows(residual)
-        y = torch.empty(x.shape, dtype=dtype, device=dev) if keep_y else None
-        h = None if residual is None else torch.empty(x.shape, dtype=dtype, device=dev)
-        rstd = torch.empty(rows, dtype=torch.float32, device=dev) if keep_rstd else None
-        q = scale = None
+        y = _like(x) if keep_y else None
+        h = q = scale = rstd = res = None
+        res_ld = q_ld = 0
+        if residual is not None:
+            r2 = _as_rows(residual)
+            res, res_ld, h = r2.data_ptr(), r2.stride(0), _like(x)
+        if keep_rstd:
+            rstd = x.new_empty(rows, dtype=torch.float32)
         if quantise:
-            q = torch.empty(*x.shape[:-1], -(-H // 16) * 16, dtype=torch.int8, device=dev)
-            scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-        check(lib.smoe_rms_norm(
-            x2.data_ptr(), x2.stride(0), ptr(r2), 0 if r2 is None else r2.stride(0), weight.data_ptr(), _ROW_TYPES[weight.dtype],
-            ptr(y), ptr(h), ptr(rstd), ptr(q), 0 if q is None else q.shape[-1], ptr(scale), _ROW_TYPES[dtype], rows, H, eps,
-            stream_ptr(dev)), "rms_norm")
-    if q is not None and q.shape[-1] != H:
-        q = q[..., :H]
-    return y, h, rstd, q, scale
+            q_ld = -(-H // 16) * 16
+            q = x.new_empty((*shape[:-1], q_ld), dtype=torch.int8)
+            scale = x.new_empty(shape[:-1], dtype=torch.float32)
+        check(lib.smoe_rms_norm(x2.data_ptr(), x2.stride(0), res, res_ld, weight.data_ptr(), _ROW_TYPES[weight.dtype], ptr(y), ptr(h),
+                                ptr(rstd), ptr(q), q_ld, ptr(scale), code, rows, H, eps, stream_ptr(dev)), "rms_norm")
+    return y, h, rstd, q if q_ld in (0, H) else q[..., :H], scale
 
 
 class _FirstDerivative(torch.autograd.Function):
@@ -115,10 +122,10 @@ class _RmsNorm(torch.autograd.Function):
         with _lib.on_device(dev):
             dy2, h2 = _as_rows(dy), _as_rows(h)
             dh2 = None if dh is None or not need_dx else _as_rows(dh)
-            dx = torch.empty(h.shape, dtype=h.dtype, device=dev) if need_dx else None
+            dx = _like(h) if need_dx else None
             dw = torch.empty_like(weight) if need_dw else None
             ws = lib.smoe_rms_norm_backward_workspace_bytes(rows, H) if need_dw else 0
-            ws = _lib.workspace(ws, dev) if ws else None
+            ws = weight.new_empty(ws, dtype=torch.uint8) if ws else None
             check(lib.smoe_rms_norm_backward(
                 dy2.data_ptr(), dy2.stride(0), ptr(dh2), 0 if dh2 is None else dh2.stride(0), h2.data_ptr(), h2.stride(0),
                 weight.data_ptr(), _ROW_TYPES[weight.dtype], rstd.data_ptr(), ptr(dx), ptr(dw), _ROW_TYPES[h.dtype], rows, H,
