@@ -527,12 +527,12 @@ int smoe_rms_norm_backward(const void* dy, long long dy_ld, const void* dh, long
  * same type, packed; scale (n) fp32 or NULL = 1.  fp32 sums, one rounding of out.  out may be base (of the same distances): tokens
  * without an adapter are left as they are then.  No other overlap.
  * The tokens sorted by adapter, as smoe_token_permutation sorts T pairs (K = 1) of n experts: expert_frequency_offset (n+1), first rows,
- * multiples of `align`, which is a multiple of 16; x_gather_idx (rows): token of each row, -1 for none; s_reverse_scatter_idx (T): row
+ * multiples of `align`, which is a multiple of 16; expert_frequency (n): tokens of each; x_gather_idx (rows): token of each row, -1 for none; s_reverse_scatter_idx (T): row
  * of each token, outside [0, rows) where it has no adapter.  A token is a row's where each names the other.
  * n <= 4096, r <= 128, H and N <= 2^28, T and rows <= 2^31 - 2^16. */
 int smoe_adapter_linear(const void* x, long long ld, const void* a, const void* b, const float* scale, const void* base,
                         long long base_ld, void* out, long long out_ld, int dtype, const int* expert_frequency_offset,
-                        const int* x_gather_idx, const int* s_reverse_scatter_idx, int T, long long rows, int H, int N, int n,
+                        const int* expert_frequency, const int* x_gather_idx, const int* s_reverse_scatter_idx, int T, long long rows, int H, int N, int n,
                         int r, int align, void* stream);
 
 /* ---------------------------------------------------------------------------------------------

@@ -40,11 +40,14 @@ struct Params {
   const char* base; long long base_ld;    // or nullptr
   char* out; long long out_ld;
   const int* off;                         // (n + 1) first row of each adapter, ascending
+  const int* count;                       // (n) its rows that have tokens
   const int* gather;                      // (rows) token of each row
   const int* reverse;                     // (T) row of each token
   int T, rows, H, N, n, r;
   int tiles;                              // few_kernel: of 16 rows; tile_kernel: at most
   int cluster;                            // tile_kernel: blocks that share a tile
+  int copies;                             // pieces of other tokens' rows for a warp
+  int sparse;                             // few_kernel: most tiles of 16 rows may be empty, its tiles are the others
   int in_place;                           // out is base
 };
 
@@ -93,6 +96,28 @@ __device__ __forceinline__ uint4 load8(const char* row, int col, int cols) {
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
+// load8 in two steps, so that many loads are on their way before the first is looked at.
+template <bool ALIGNED>
+struct Raw8 {
+  uint4 q, r;
+  __device__ __forceinline__ void load(const char* row, int col, int cols) {
+    const int o = ALIGNED ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15);
+    const char* p = row + 2ll * col - o;
+    q = make_uint4(0u, 0u, 0u, 0u);
+    if (col < cols) q = *reinterpret_cast<const uint4*>(p);
+    if (!ALIGNED) {
+      r = make_uint4(0u, 0u, 0u, 0u);
+      if (o != 0 && 2ll * (cols - col) + o > 16) r = *reinterpret_cast<const uint4*>(p + 16);
+    }
+  }
+  __device__ __forceinline__ uint4 get(const char* row, int col, int cols) const {
+    if (ALIGNED) return q;
+    uint32_t v[8] = {q.x, q.y, q.z, q.w, r.x, r.y, r.z, r.w};
+    shift_down(v, static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15), cols - col);
+    return make_uint4(v[0], v[1], v[2], v[3]);
+  }
+};
+
 // The same from a copy of the row's 16-byte blocks: eight values `o` bytes behind `p`, of which `left` belong to the row.
 __device__ __forceinline__ uint4 in_place8(const char* p, int o, int left) {
   const uint4 q = *reinterpret_cast<const uint4*>(p), r = *reinterpret_cast<const uint4*>(p + 16);
@@ -122,22 +147,74 @@ __device__ __forceinline__ int token_of(const Params& p, int row) {
   return t >= 0 && p.reverse[t] == row ? t : -1;
 }
 
-// Rows of tokens that no tile writes (`tile` rows each): base, or zeros.  Warp `warp` of `warps`, all its lanes.
-__device__ __forceinline__ void copy_others(const Params& p, int tile, long long warp, long long warps) {
+// The `tile`-th tile's adapter, first row and end, adapters in their order (all lanes of the warp); adapter -1 behind the last.  Each lane counts
+// the tiles of a run of adapters; then the lanes look at the run that holds the tile.
+__device__ __forceinline__ int4 tile_of(const Params& p, int tile, int tile_rows) {
   const int lane = threadIdx.x & 31;
-  const int end = min(p.off[p.n], p.rows);
-  for (long long t = warp; t < p.T; t += warps) {
+  const auto tiles = [&](int e) { return (max(p.count[e], 0) + tile_rows - 1) / tile_rows; };
+  const auto scan = [&](int v) {  // sum over the lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int other = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += other;
+    }
+    return v;
+  };
+  const int run = (p.n + 31) / 32;
+  int mine = 0;
+  const int run_end = min(p.n, (lane + 1) * run);
+#pragma unroll 4
+  for (int e = lane * run; e < run_end; ++e) mine += tiles(e);
+  int sum = scan(mine);
+  unsigned found = __ballot_sync(0xffffffffu, tile < sum);
+  if (found == 0u) return make_int4(-1, 0, 0, 0);
+  const int who = __ffs(found) - 1;
+  int before = __shfl_sync(0xffffffffu, sum - mine, who);
+  const int end = min(p.n, (who + 1) * run);
+  for (int e0 = who * run; e0 < end; e0 += 32) {
+    const int here = e0 + lane < end ? tiles(e0 + lane) : 0;
+    sum = before + scan(here);
+    found = __ballot_sync(0xffffffffu, tile < sum);
+    if (found != 0u) {
+      const int at = __ffs(found) - 1, e = e0 + at, first = min(max(p.off[e], 0), p.rows);
+      const int row = first + (tile - __shfl_sync(0xffffffffu, sum - here, at)) * tile_rows;
+      return make_int4(e, row, min(min(row + tile_rows, first + max(p.count[e], 0)), p.rows), 0);
+    }
+    before = __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return make_int4(-1, 0, 0, 0);
+}
+
+// Rows of tokens that no tile writes: base, or zeros.  A piece of work is 1024 columns of a token, `pieces` of them to each of `warps` warps, of which
+// this is warp `warp` (all its lanes); 16-byte blocks of out, four of a lane on their way together.
+constexpr int kCopyCols = 1024;
+static long long copy_pieces(int T, int N) { return static_cast<long long>(T) * ((N + kCopyCols - 1) / kCopyCols); }
+__device__ __forceinline__ void copy_others(const Params& p, long long warp) {
+  const int lane = threadIdx.x & 31;
+  const int end = min(p.off[p.n], p.rows), parts = (p.N + kCopyCols - 1) / kCopyCols;
+  const long long all = static_cast<long long>(p.T) * parts;
+  for (long long piece = warp * p.copies; piece < min((warp + 1) * p.copies, all); ++piece) {
+    const int t = static_cast<int>(piece / parts), c0 = static_cast<int>(piece - static_cast<long long>(t) * parts) * kCopyCols, c1 = min(c0 + kCopyCols, p.N);
     const int row = p.reverse[t];
-    if (row >= 0 && row < p.rows && row / tile * tile < end && p.gather[row] == t) continue;
+    if (row >= 0 && row < p.rows && row / 16 * 16 < end && p.gather[row] == t) continue;
     char* out = p.out + t * p.out_ld;
     const char* base = p.base != nullptr ? p.base + t * p.base_ld : nullptr;
-    if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(base) | 2ull * p.N) % 16 == 0) {
-      for (int c = lane; c < p.N / 8; c += 32)
-        reinterpret_cast<uint4*>(out)[c] = base != nullptr ? reinterpret_cast<const uint4*>(base)[c] : make_uint4(0u, 0u, 0u, 0u);
-    } else {
-      for (int c = lane; c < p.N; c += 32)
-        reinterpret_cast<uint16_t*>(out)[c] = base != nullptr ? reinterpret_cast<const uint16_t*>(base)[c] : static_cast<uint16_t>(0);
+    // columns of the piece in front of out's next 16-byte boundary, and behind its last one, one by one
+    const int head = min(static_cast<int>((16 - (reinterpret_cast<uintptr_t>(out + 2ll * c0) & 15)) & 15) / 2, c1 - c0), blocks = (c1 - c0 - head) / 8;
+    const int edge = lane < 8 ? (lane < head ? c0 + lane : -1) : lane < 16 && c0 + head + 8 * blocks + lane - 8 < c1 ? c0 + head + 8 * blocks + lane - 8 : -1;
+    Raw8<false> v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = lane + 32 * i, c = c0 + head + 8 * k;
+      v[i].load(base + 2ll * c, 0, base != nullptr && k < blocks ? 8 : 0);
     }
+    const uint16_t one = base != nullptr && edge >= 0 ? reinterpret_cast<const uint16_t*>(base)[edge] : static_cast<uint16_t>(0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = lane + 32 * i, c = c0 + head + 8 * k;
+      if (k < blocks) *reinterpret_cast<uint4*>(out + 2ll * c) = v[i].get(base + 2ll * c, 0, base != nullptr ? 8 : 0);
+    }
+    if (edge >= 0) reinterpret_cast<uint16_t*>(out)[edge] = one;
   }
 }
 
@@ -304,80 +381,107 @@ __device__ __forceinline__ void put_staged(const Params& p, int n0, int tokens, 
   }
 }
 
-// Four products with a row of b each, straight from memory: columns n0 .. n0 + 31 of out.
-template <class T, int RP, bool ALIGNED>
-__device__ __forceinline__ void direct_columns(const Params& p, const char* b, int n0, const uint32_t (&lead)[Steps<RP>::K][4], const uint32_t (&rest)[Steps<RP>::K][4], float (&c)[4][4]) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+// What a lane needs of b for columns n0 .. n0 + 31 of out, straight from memory.
+template <int RP, bool ALIGNED>
+struct ColumnWeights {
+  static constexpr int L = Steps<RP>::L;
+  Raw8<ALIGNED> w[4][L];
+  // (a row ends where b has no more)
+  static __device__ __forceinline__ void place(const Params& p, const char* b, int n0, int j, int l, const char*& row, int& col, int& cols) {
+    const int lane = threadIdx.x & 31, n = n0 + out_column(lane >> 2, j);
+    row = b + static_cast<long long>(n) * p.r * 2;
+    col = RP == 16 ? 8 * ((lane & 3) >> 1) : 32 * l + 8 * (lane & 3);
+    cols = n < p.N ? p.r : 0;
+  }
+  __device__ __forceinline__ void load(const Params& p, const char* b, int n0) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
-    const int n = n0 + out_column(g, j);
-    const char* row = b + static_cast<long long>(n) * p.r * 2;
+    for (int j = 0; j < 4; ++j) {
 #pragma unroll
-    for (int l = 0; l < Steps<RP>::L; ++l) {
-      uint4 w = make_uint4(0u, 0u, 0u, 0u);
-      if (n < p.N) {
-        if constexpr (RP > 16) {
-          w = load8<ALIGNED>(row, 32 * l + 8 * t, p.r);
-        } else if (ALIGNED) {
-          if (4 * t < p.r) {
-            const uint2 h = *reinterpret_cast<const uint2*>(row + 8 * t);
-            w.x = h.x;
-            w.y = h.y;
-          }
-        } else {
-          const uint4 q = load8<false>(row, 8 * (t >> 1), p.r);
-          w.x = t & 1 ? q.z : q.x;
-          w.y = t & 1 ? q.w : q.y;
-        }
+      for (int l = 0; l < L; ++l) {
+        const char* row;
+        int col, cols;
+        place(p, b, n0, j, l, row, col, cols);
+        w[j][l].load(row, col, cols);
       }
-      step<T, RP>(c[j], lead, rest, l, w);
     }
   }
-}
+  template <class T>
+  __device__ __forceinline__ void multiply(const Params& p, const char* b, int n0, const uint32_t (&lead)[Steps<RP>::K][4], const uint32_t (&rest)[Steps<RP>::K][4], float (&c)[4][4]) const {
+    const bool odd = threadIdx.x & 1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
+#pragma unroll
+      for (int l = 0; l < L; ++l) {
+        const char* row;
+        int col, cols;
+        place(p, b, n0, j, l, row, col, cols);
+        uint4 v = w[j][l].get(row, col, cols);
+        if (RP == 16 && odd) v = make_uint4(v.z, v.w, 0u, 0u);  // four of the eight are this lane's
+        step<T, RP>(c[j], lead, rest, l, v);
+      }
+    }
+  }
+};
 
 // ----------------------------------------------------------------------------------------------
 // few rows
 // ----------------------------------------------------------------------------------------------
-__device__ __forceinline__ float load_cluster(uint32_t addr) {
-  float f;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 load_cluster(uint32_t addr) {
+  float4 f;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(addr) : "memory");
   return f;
 }
 
+// Pitches in shared memory, in floats: of parts, which lanes write two at a time in eight rows, and of s, which they read four at a time.
 template <int RP>
-constexpr size_t few_smem() {  // warps' parts or staged rows, the block's part, s
-  return sizeof(float) * (kWarps * 16 * (RP > kStagePitch ? RP : kStagePitch) + 2 * 16 * RP);
-}
+struct Few {
+  static constexpr int kPart = RP + 8, kS = RP + 4;
+  static constexpr int kWarp = 16 * (kPart > kStagePitch ? kPart : kStagePitch);  // a warp's part, later its staged rows
+  static constexpr size_t kSmem = sizeof(float) * (kWarps * kWarp + 16 * kPart + 16 * kS);
+};
 
-template <class T, int RP, bool ALIGNED>
-__global__ void __launch_bounds__(32 * kWarps) few_kernel(const Params p) {
+// AHEAD: a warp's weights and base for its first columns of out are on their way before the blocks add their parts, those of the next ones before the
+// last are done, and more of x and a at a time.  That takes registers, so it is for as many blocks as there is room for at once.
+template <class T, int RP, bool ALIGNED, bool AHEAD>
+__global__ void __launch_bounds__(32 * kWarps, AHEAD ? 1 : RP == 16 ? (ALIGNED ? 4 : 2) : RP == 32 ? (ALIGNED ? 3 : 2) : RP == 64 && ALIGNED ? 2 : 1) few_kernel(const Params p) {
   release_next();
   wait_for_previous();
+  using F = Few<RP>;
   extern __shared__ __align__(16) float smem[];
-  float* parts = smem;                                                       // [warp][16][RP]
-  float* part = smem + kWarps * 16 * (RP > kStagePitch ? RP : kStagePitch);  // [16][RP]
-  float* s_all = part + 16 * RP;                                             // [16][RP]
+  float* parts = smem;                       // [warp][16][kPart]
+  float* part = smem + kWarps * F::kWarp;    // [16][kPart]
+  float* s_all = part + 16 * F::kPart;       // [16][kS]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int rank = static_cast<int>(cluster_ctarank()), tile = blockIdx.x / kCluster;
   if (tile >= p.tiles) {
     const long long first = static_cast<long long>(p.tiles) * kCluster;
-    copy_others(p, 16, (blockIdx.x - first) * kWarps + warp, (gridDim.x - first) * kWarps);
+    copy_others(p, (blockIdx.x - first) * kWarps + warp);
     return;
   }
-  const int row0 = 16 * tile;
-  if (!within(p, row0)) return;
-  // what is read of a token does not wait for the check that the row is still its own
-  const int gathered = gathered_of(p, row0 + (lane & 15));
+  // Loads of the row's tokens, of the adapters' rows, and then of all that hangs on them are on their way together; whether a row is still its token's
+  // is looked at in the end.
+  int row0 = 16 * tile, e;
+  bool rows_here = true;
+  if (p.sparse) {
+    const int4 what = tile_of(p, tile, 16);
+    e = max(what.x, 0);
+    row0 = what.y;
+    rows_here = what.x >= 0;
+  } else {
+    e = adapter_of(p, row0);
+  }
+  const int my_row = row0 + (lane & 15);
+  const int candidate = gathered_of(p, my_row);
+  if (!p.sparse) rows_here = within(p, row0);
+  const int gathered = rows_here ? candidate : -1;
   if (__all_sync(0xffffffffu, gathered < 0)) return;  // (the cluster's blocks all see the same)
   const int row_of = gathered >= 0 ? p.reverse[gathered] : -1;
-  const int e = adapter_of(p, row0);
   const int x_t0 = __shfl_sync(0xffffffffu, gathered, g), x_t1 = __shfl_sync(0xffffffffu, gathered, g + 8);
-  // this block's columns of out, and the L2 fetches the weights for them meanwhile
   const int groups = (p.N + kGroup - 1) / kGroup;
   const int n_first = static_cast<int>(static_cast<long long>(groups) * rank / kCluster), n_end = static_cast<int>(static_cast<long long>(groups) * (rank + 1) / kCluster);
   const char* b = p.b + static_cast<long long>(e) * p.N * p.r * 2;
-  {
+  {  // the L2 fetches the weights of this block's columns of out meanwhile
     const long long first = static_cast<long long>(n_first) * kGroup * p.r * 2, end = min(static_cast<long long>(n_end) * kGroup, static_cast<long long>(p.N)) * p.r * 2;
     for (long long o = first + 128ll * threadIdx.x; o < end; o += 128ll * blockDim.x) asm volatile("prefetch.global.L2 [%0];" ::"l"(b + o));
   }
@@ -391,99 +495,131 @@ __global__ void __launch_bounds__(32 * kWarps) few_kernel(const Params p) {
     const int first = static_cast<int>(static_cast<long long>(chunks) * mine / parts_of), end = static_cast<int>(static_cast<long long>(chunks) * (mine + 1) / parts_of);
     const char* x0 = p.x + x_t0 * p.x_ld;
     const char* x1 = p.x + x_t1 * p.x_ld;
-    const char* a = p.a + static_cast<long long>(e) * p.r * p.H * 2;
-    constexpr int U = RP <= 32 ? 2 : 1;  // chunks whose loads are on their way together
+    const char* a = p.a + (static_cast<long long>(e) * p.r + g) * p.H * 2;
+    const int width0 = x_t0 >= 0 ? p.H : 0, width1 = x_t1 >= 0 ? p.H : 0;
+    constexpr int U = RP <= 32 || (RP == 64 && ALIGNED && AHEAD) ? 2 : 1;  // chunks whose loads are on their way together
     for (int c = first; c < end; c += U) {
-      uint4 xa[U][2], w[U][NT];
+      Raw8<ALIGNED> xa[U][2], w[U][NT];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int col = c + u < end ? 32 * (c + u) + 8 * t : p.H;
-        xa[u][0] = load8<ALIGNED>(x0, x_t0 >= 0 ? col : p.H, p.H);
-        xa[u][1] = load8<ALIGNED>(x1, x_t1 >= 0 ? col : p.H, p.H);
+        xa[u][0].load(x0, col, width0);
+        xa[u][1].load(x1, col, width1);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) w[u][j] = load8<ALIGNED>(a + (8ll * j + g) * p.H * 2, 8 * j + g < p.r ? col : p.H, p.H);
+        for (int j = 0; j < NT; ++j) w[u][j].load(a + 16ll * j * p.H, col, 8 * j + g < p.r ? p.H : 0);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
+        const int col = c + u < end ? 32 * (c + u) + 8 * t : p.H;
+        const uint4 v0 = xa[u][0].get(x0, col, width0), v1 = xa[u][1].get(x1, col, width1);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          mma<T>(acc[j], xa[u][0].x, xa[u][1].x, xa[u][0].y, xa[u][1].y, w[u][j].x, w[u][j].y);
-          mma<T>(acc[j], xa[u][0].z, xa[u][1].z, xa[u][0].w, xa[u][1].w, w[u][j].z, w[u][j].w);
+          const uint4 v = w[u][j].get(a + 16ll * j * p.H, col, 8 * j + g < p.r ? p.H : 0);
+          mma<T>(acc[j], v0.x, v1.x, v0.y, v1.y, v.x, v.y);
+          mma<T>(acc[j], v0.z, v1.z, v0.w, v1.w, v.z, v.w);
         }
       }
     }
   }
+  int group = n_first + warp;
+  ColumnWeights<RP, ALIGNED> weights;
+  BaseRows<T> base;
+  BaseColumn column;
+  const auto fetch = [&] {
+    if (group >= n_end) return;
+    weights.load(p, b, kGroup * group);
+    if (ALIGNED) base.load(p, kGroup * group + 8 * t, x_t0, x_t1);
+    else column.load(p, kGroup * group + lane, gathered);
+  };
+  if (AHEAD && RP <= 64) fetch();
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
-    float* to = parts + (warp * 16 + g) * RP + 8 * j + 2 * t;
+    float* to = parts + warp * F::kWarp + g * F::kPart + 8 * j + 2 * t;
     *reinterpret_cast<float2*>(to) = make_float2(acc[j][0], acc[j][1]);
-    *reinterpret_cast<float2*>(to + 8 * RP) = make_float2(acc[j][2], acc[j][3]);
+    *reinterpret_cast<float2*>(to + 8 * F::kPart) = make_float2(acc[j][2], acc[j][3]);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * RP; i += 32 * kWarps) {
-    float f = parts[i];
+  constexpr int Q = RP / 4;  // fours of a row
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) f += parts[w * 16 * RP + i];
-    part[i] = f;
+  for (int i0 = 0; i0 < 16 * Q; i0 += 32 * kWarps) {
+    const int i = i0 + threadIdx.x, at = i / Q * F::kPart + 4 * (i % Q);
+    if (i >= 16 * Q) continue;
+    float4 f = *reinterpret_cast<const float4*>(parts + at);
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) {
+      const float4 v = *reinterpret_cast<const float4*>(parts + w * F::kWarp + at);
+      f.x += v.x; f.y += v.y; f.z += v.z; f.w += v.w;
+    }
+    *reinterpret_cast<float4*>(part + at) = f;
   }
   cluster_sync_all();
   const float scale = p.scale != nullptr ? p.scale[e] : 1.f;
-  for (int i = threadIdx.x; i < 16 * RP; i += 32 * kWarps) {
-    const uint32_t at = smem_u32(part + i);
-    float f[kCluster];
+#pragma unroll
+  for (int i0 = 0; i0 < 16 * Q; i0 += 32 * kWarps) {
+    const int i = i0 + threadIdx.x;
+    if (i >= 16 * Q) continue;
+    const uint32_t at = smem_u32(part + i / Q * F::kPart + 4 * (i % Q));
+    float4 f[kCluster];
 #pragma unroll
     for (int k = 0; k < kCluster; ++k) f[k] = load_cluster(map_to_cta(at, k));
 #pragma unroll
-    for (int k = 1; k < kCluster; ++k) f[0] += f[k];
-    s_all[i] = f[0] * scale;
+    for (int k = 1; k < kCluster; ++k) {
+      f[0].x += f[k].x; f[0].y += f[k].y; f[0].z += f[k].z; f[0].w += f[k].w;
+    }
+    *reinterpret_cast<float4*>(s_all + i / Q * F::kS + 4 * (i % Q)) = make_float4(f[0].x * scale, f[0].y * scale, f[0].z * scale, f[0].w * scale);
   }
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this block has read the others' parts
   __syncthreads();
   // s in this warp's registers
-  constexpr int K = Steps<RP>::K, L = Steps<RP>::L, V = RP == 16 ? 4 : 8;
+  constexpr int K = Steps<RP>::K;
   uint32_t lead[K][4], rest[K][4];
-  float most0 = 0.f, most1 = 0.f;
+  const auto fours = [&](int row, int k) {
+    return *reinterpret_cast<const float4*>(s_all + row * F::kS + (RP == 16 ? 4 * t : 32 * (k / 2) + 8 * t + 4 * (k & 1)));
+  };
+  float f0 = 1.f, f1 = 1.f;
+  if (std::is_same<T, __half>::value) {
+    float most0 = 0.f, most1 = 0.f;
 #pragma unroll
-  for (int l = 0; l < L; ++l) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      most0 = fmaxf(most0, fabsf(s_all[g * RP + 32 * l + V * t + i]));
-      most1 = fmaxf(most1, fabsf(s_all[(g + 8) * RP + 32 * l + V * t + i]));
+    for (int k = 0; k < K; ++k) {
+      const float4 u = fours(g, k), v = fours(g + 8, k);
+      most0 = fmaxf(fmaxf(most0, fmaxf(fabsf(u.x), fabsf(u.y))), fmaxf(fabsf(u.z), fabsf(u.w)));
+      most1 = fmaxf(fmaxf(most1, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
     }
-  }
 #pragma unroll
-  for (int o = 1; o < 4; o *= 2) {
-    most0 = fmaxf(most0, __shfl_xor_sync(0xffffffffu, most0, o));
-    most1 = fmaxf(most1, __shfl_xor_sync(0xffffffffu, most1, o));
+    for (int o = 1; o < 4; o *= 2) {
+      most0 = fmaxf(most0, __shfl_xor_sync(0xffffffffu, most0, o));
+      most1 = fmaxf(most1, __shfl_xor_sync(0xffffffffu, most1, o));
+    }
+    f0 = factor_of<T>(most0);
+    f1 = factor_of<T>(most1);
   }
-  const float f0 = factor_of<T>(most0), f1 = factor_of<T>(most1);
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int col = RP == 16 ? 4 * t : 32 * (k / 2) + 8 * t + 4 * (k & 1);
-    const float4 u = *reinterpret_cast<const float4*>(s_all + g * RP + col), v = *reinterpret_cast<const float4*>(s_all + (g + 8) * RP + col);
+    const float4 u = fours(g, k), v = fours(g + 8, k);
     split2<T>(u.x * f0, u.y * f0, lead[k][0], rest[k][0]);
     split2<T>(v.x * f1, v.y * f1, lead[k][1], rest[k][1]);
     split2<T>(u.z * f0, u.w * f0, lead[k][2], rest[k][2]);
     split2<T>(v.z * f1, v.w * f1, lead[k][3], rest[k][3]);
   }
   const float i0 = inverse_of<T>(f0), i1 = inverse_of<T>(f1);
-  const int tokens = row_of == row0 + (lane & 15) ? gathered : -1;
+  const int tokens = row_of == my_row ? gathered : -1;
   const int t0 = __shfl_sync(0xffffffffu, tokens, g), t1 = __shfl_sync(0xffffffffu, tokens, g + 8);
-  for (int group = n_first + warp; group < n_end; group += kWarps) {
+  if (!AHEAD || RP > 64) fetch();
+  while (group < n_end) {
     const int n0 = kGroup * group;
     float c[4][4];
+    weights.template multiply<T>(p, b, n0, lead, rest, c);
+    const BaseRows<T> base_now = base;
+    const BaseColumn column_now = column;
+    group += kWarps;
+    if (AHEAD) fetch();
     if (ALIGNED) {
-      BaseRows<T> base;
-      base.load(p, n0 + 8 * t, t0, t1);
-      direct_columns<T, RP, ALIGNED>(p, b, n0, lead, rest, c);
-      put_row<T>(p, n0 + 8 * t, t0, base.v[0], c, 0, i0);
-      put_row<T>(p, n0 + 8 * t, t1, base.v[1], c, 1, i1);
+      put_row<T>(p, n0 + 8 * t, t0, base_now.v[0], c, 0, i0);
+      put_row<T>(p, n0 + 8 * t, t1, base_now.v[1], c, 1, i1);
     } else {
-      BaseColumn base;
-      base.load(p, n0 + lane, tokens);
-      direct_columns<T, RP, ALIGNED>(p, b, n0, lead, rest, c);
-      put_staged<T>(p, n0, tokens, base, c, i0, i1, parts + warp * 16 * kStagePitch);
+      put_staged<T>(p, n0, tokens, column_now, c, i0, i1, parts + warp * F::kWarp);
     }
+    if (!AHEAD) fetch();
   }
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -491,52 +627,6 @@ __global__ void __launch_bounds__(32 * kWarps) few_kernel(const Params p) {
 // ----------------------------------------------------------------------------------------------
 // tiles
 // ----------------------------------------------------------------------------------------------
-// The `tile`-th tile's adapter, first row and end, adapters in their order (all lanes of the warp); adapter -1 behind the last.  Each lane counts
-// the tiles of a run of adapters; then the lanes look at the run that holds the tile.
-__device__ __forceinline__ int4 tile_of(const Params& p, int tile, int tile_rows) {
-  const int lane = threadIdx.x & 31;
-  const auto row_at = [&](int e) { return min(max(p.off[e], 0), p.rows); };
-  const auto tiles_between = [&](int first, int end) { return end > first ? (end - first + tile_rows - 1) / tile_rows : 0; };
-  const auto scan = [&](int v) {  // sum over the lanes up to this one
-#pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-      const int other = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += other;
-    }
-    return v;
-  };
-  const int run = (p.n + 31) / 32;
-  int mine = 0;
-  {
-    const int end = min(p.n, (lane + 1) * run);
-    int last = lane * run < p.n ? row_at(lane * run) : 0;
-#pragma unroll 4
-    for (int e = lane * run; e < end; ++e) {
-      const int next = row_at(e + 1);
-      mine += tiles_between(last, next);
-      last = next;
-    }
-  }
-  int sum = scan(mine);
-  unsigned found = __ballot_sync(0xffffffffu, tile < sum);
-  if (found == 0u) return make_int4(-1, 0, 0, 0);
-  const int who = __ffs(found) - 1;
-  int before = __shfl_sync(0xffffffffu, sum - mine, who);
-  for (int e0 = who * run;; e0 += 32) {  // (it is in one of them)
-    const int e = e0 + lane;
-    const bool in = e < min(p.n, (who + 1) * run);
-    const int first = in ? row_at(e) : 0, end = in ? row_at(e + 1) : 0, tiles = tiles_between(first, end);
-    sum = before + scan(tiles);
-    found = __ballot_sync(0xffffffffu, tile < sum);
-    if (found != 0u || e0 >= p.n) {
-      const int at = found != 0u ? __ffs(found) - 1 : 0;
-      const int row = __shfl_sync(0xffffffffu, first, at) + (tile - __shfl_sync(0xffffffffu, sum - tiles, at)) * tile_rows;
-      return make_int4(found != 0u ? e0 + at : -1, row, min(row + tile_rows, __shfl_sync(0xffffffffu, end, at)), 0);
-    }
-    before = __shfl_sync(0xffffffffu, sum, 31);
-  }
-}
-
 // Stages of 64 columns, `kStages` of them in turn: RP rows of a (or 64 of b) for the block, and each warp's 16 rows of x (or base), which it brings in
 // itself.  ALIGNED: rows of 128 bytes by asynchronous copies; the halves of odd ones trade places, so that eight lanes of a load meet all
 // banks.  Otherwise rows of x and base come in by the nine 16-byte blocks that hold them and are put in place on the way out of shared
@@ -549,7 +639,7 @@ struct Tile {
   // of a warp: s (leading bits, the rest), later its results
   static constexpr int kOwnBytes = 64 * RP > 16 * kOutPitch || ALIGNED ? 64 * RP : 16 * kOutPitch;
   static size_t smem(int warps) {
-    const size_t stages = kStages * static_cast<size_t>(kWeightBytes + warps * kWarpBytes), part = sizeof(float) * 16 * warps * RP;
+    const size_t stages = kStages * static_cast<size_t>(kWeightBytes + warps * kWarpBytes), part = sizeof(float) * 16 * warps * Few<RP>::kPart;
     return (stages > part ? stages : part) + static_cast<size_t>(warps) * kOwnBytes + sizeof(float) * 16 * warps;
   }
 };
@@ -627,7 +717,7 @@ __global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) tile_kernel(con
   const int tile = blockIdx.x / p.cluster, share = blockIdx.x - tile * p.cluster;
   if (tile >= p.tiles) {
     const long long first = static_cast<long long>(p.tiles) * p.cluster;
-    copy_others(p, 16, (blockIdx.x - first) * warps + warp, (gridDim.x - first) * warps);
+    copy_others(p, (blockIdx.x - first) * warps + warp);
     return;
   }
   const int4 what = tile_of(p, tile, tile_rows);
@@ -639,7 +729,7 @@ __global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) tile_kernel(con
   const int stage_bytes = Ti::kWeightBytes + warps * Ti::kWarpBytes;
   const auto weights_in = [&](int stage) { return smem_tile + stage % STAGES * stage_bytes; };
   const auto rows_in = [&](int stage) { return weights_in(stage) + Ti::kWeightBytes + warp * Ti::kWarpBytes; };
-  const size_t ring = max(static_cast<size_t>(STAGES) * stage_bytes, sizeof(float) * tile_rows * RP);
+  const size_t ring = max(static_cast<size_t>(STAGES) * stage_bytes, sizeof(float) * tile_rows * Few<RP>::kPart);
   char* own = smem_tile + ring;                                                // [warp][lead: 16 x RP, rest: 16 x RP]
   float* inverses = reinterpret_cast<float*>(own + warps * Ti::kOwnBytes);     // [tile_rows]
   const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
@@ -693,12 +783,13 @@ __global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) tile_kernel(con
   }
 
   // the blocks add their parts, each for a share of the rows, and give all of them the sums
-  float* part = reinterpret_cast<float*>(smem_tile);  // [tile_rows][RP]
+  constexpr int PART = Few<RP>::kPart;
+  float* part = reinterpret_cast<float*>(smem_tile);  // [tile_rows][PART]
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
-    float* to = part + (16 * warp + g) * RP + 8 * j + 2 * t;
+    float* to = part + (16 * warp + g) * PART + 8 * j + 2 * t;
     *reinterpret_cast<float2*>(to) = make_float2(acc[j][0], acc[j][1]);
-    *reinterpret_cast<float2*>(to + 8 * RP) = make_float2(acc[j][2], acc[j][3]);
+    *reinterpret_cast<float2*>(to + 8 * PART) = make_float2(acc[j][2], acc[j][3]);
   }
   cluster_sync_all();
   {
@@ -710,12 +801,10 @@ __global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) tile_kernel(con
       const bool live = i < mine * Q;
       const int row = share * mine + (live ? i / Q : 0), q = i % Q;
       float f[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
       for (int k = 0; k < p.cluster; ++k) {
-        float v[4];
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(map_to_cta(smem_u32(part + row * RP + 4 * q), k)) : "memory");
-#pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] += v[j];
+        const float4 v = load_cluster(map_to_cta(smem_u32(part + row * PART + 4 * q), k));
+        f[0] += v.x; f[1] += v.y; f[2] += v.z; f[3] += v.w;
       }
       float most = 0.f;
 #pragma unroll
@@ -842,37 +931,45 @@ __global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) tile_kernel(con
 // launches
 // ----------------------------------------------------------------------------------------------
 static int padded_rank(int r) { return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : 128; }
-static bool by_few_rows(int T, int n) {
-  const long long tiles = T / 16 + static_cast<long long>(n < T ? n : T);  // of 16 rows, at most (or as many as there are tokens)
-  return (tiles < T ? tiles : T) <= 256;
+// Tiles of `rows` rows, at most: what the adapters' tokens fill, and a part of one more each.
+static long long tiles_of(int T, int n, int rows) {
+  const long long tiles = T / rows + static_cast<long long>(n < T ? n : T);
+  return tiles < T ? tiles : T;
 }
+static bool by_few_rows(int T, int n, int r) { return tiles_of(T, n, 16) * padded_rank(r) <= 4096; }
 // Warps of tile_kernel's blocks, by the tokens that an adapter has on average.
 static int warps_of(int T, int n) { return T / n <= 32 ? 2 : T / n <= 64 ? 4 : 8; }
-// Its tiles, at most: every adapter's last one may be a part of one.
-static long long tiles_of(int T, long long rows, int n) {
-  return rows / (16 * warps_of(T, n)) + (n < T ? n : T);
-}
+// Blocks of few_kernel with AHEAD that an SM has room for.
+template <int RP, bool ALIGNED>
+constexpr int kAheadBlocks = RP == 16 ? (ALIGNED ? 3 : 2) : RP == 32 && ALIGNED ? 2 : 1;
+
 template <class T, int RP, bool ALIGNED>
 static int launch(Params p, cudaStream_t st) {
   static PerDeviceFlag configured;
   const int dev = current_device();
   if (dev < 0) return SMOE_ERR_DRIVER;
   if (!configured.test(dev)) {
-    if (cudaFuncSetAttribute(few_kernel<T, RP, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(few_smem<RP>())) != cudaSuccess ||
+    if (cudaFuncSetAttribute(few_kernel<T, RP, ALIGNED, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Few<RP>::kSmem)) != cudaSuccess ||
+        cudaFuncSetAttribute(few_kernel<T, RP, ALIGNED, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Few<RP>::kSmem)) != cudaSuccess ||
         cudaFuncSetAttribute(tile_kernel<T, RP, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Tile<RP, ALIGNED>::smem(kWarps))) != cudaSuccess)
       return SMOE_ERR_LAUNCH;
     configured.set(dev);
   }
-  const bool few = by_few_rows(p.T, p.n);
+  const bool few = by_few_rows(p.T, p.n, p.r);
   const int warps = few ? kWarps : warps_of(p.T, p.n);
-  // (eight blocks to 16 rows at most, and less than one to eight of the other tokens: less than 2^31)
-  p.tiles = static_cast<int>(few ? (p.rows + 15) / 16 : tiles_of(p.T, p.rows, p.n));
+  p.sparse = (p.rows + 15) / 16 > tiles_of(p.T, p.n, 16);
+  p.tiles = static_cast<int>(!few ? tiles_of(p.T, p.n, 16 * warps) : p.sparse ? tiles_of(p.T, p.n, 16) : (p.rows + 15) / 16);
   const int full = (p.T + 16 * warps - 1) / (16 * warps);  // tiles, if they were all full
   p.cluster = few ? kCluster : full > 148 ? 1 : full > 74 ? 2 : full > 37 ? 4 : 8;
-  const long long to_a_cluster = 8ll * warps * p.cluster;  // eight tokens to a warp
-  const long long others = p.in_place ? 0 : (p.T + to_a_cluster - 1) / to_a_cluster, blocks = (p.tiles + others) * p.cluster;
+  // the other tokens: a piece to a warp, or up to eight where that makes more blocks than the device takes at a time
+  const long long pieces = p.in_place ? 0 : copy_pieces(p.T, p.N), room = 148 * 4 * kWarps;
+  p.copies = static_cast<int>(pieces <= room ? 1 : pieces >= 8 * room ? 8 : pieces / room);
+  const long long to_a_cluster = static_cast<long long>(p.copies) * warps * p.cluster;
+  const long long blocks = (p.tiles + (pieces + to_a_cluster - 1) / to_a_cluster) * p.cluster;
+  if (blocks > 0x7fffffffll) return SMOE_ERR_SHAPE;
   if (blocks == 0) return SMOE_OK;
-  return launched(few ? launch_chained(few_kernel<T, RP, ALIGNED>, dim3(static_cast<unsigned>(blocks)), 32 * warps, few_smem<RP>(), st, p.cluster, p)
+  const bool ahead = tiles_of(p.T, p.n, 16) * kCluster <= 148 * kAheadBlocks<RP, ALIGNED>;
+  return launched(few ? launch_chained(ahead ? few_kernel<T, RP, ALIGNED, true> : few_kernel<T, RP, ALIGNED, false>, dim3(static_cast<unsigned>(blocks)), 32 * warps, Few<RP>::kSmem, st, p.cluster, p)
                       : launch_chained(tile_kernel<T, RP, ALIGNED>, dim3(static_cast<unsigned>(blocks)), 32 * warps, Tile<RP, ALIGNED>::smem(warps), st, p.cluster, p));
 }
 template <class T, bool ALIGNED>
@@ -896,26 +993,26 @@ using namespace smoe::adapters;
 extern "C" {
 
 int smoe_adapter_linear(const void* x, long long ld, const void* a, const void* b, const float* scale, const void* base, long long base_ld,
-                        void* out, long long out_ld, int dtype, const int* expert_frequency_offset, const int* x_gather_idx,
-                        const int* s_reverse_scatter_idx, int T, long long rows, int H, int N, int n, int r, int align, void* stream) {
+                        void* out, long long out_ld, int dtype, const int* expert_frequency_offset, const int* expert_frequency,
+                        const int* x_gather_idx, const int* s_reverse_scatter_idx, int T, long long rows, int H, int N, int n, int r, int align, void* stream) {
   if (dtype != SMOE_BF16 && dtype != SMOE_F16) return SMOE_ERR_DTYPE;
   if (T < 0 || T > kMaxRows || rows < 0 || rows > kMaxRows || H <= 0 || N <= 0 || n <= 0 || n > kMaxAdapters || r <= 0 || r > kMaxRank || align <= 0 ||
       align % 16 != 0 || ld < 0 || base_ld < 0 || out_ld < N)
     return SMOE_ERR_SHAPE;
   if (H > 1 << 28 || N > 1 << 28) return SMOE_ERR_SHAPE;
   if (T == 0) return SMOE_OK;
-  if (x == nullptr || a == nullptr || b == nullptr || out == nullptr || expert_frequency_offset == nullptr || s_reverse_scatter_idx == nullptr ||
+  if (x == nullptr || a == nullptr || b == nullptr || out == nullptr || expert_frequency_offset == nullptr || expert_frequency == nullptr || s_reverse_scatter_idx == nullptr ||
       (rows > 0 && x_gather_idx == nullptr))
     return SMOE_ERR_SHAPE;
   if ((address(x) | address(a) | address(b) | address(base) | address(out)) % 2 != 0 ||
-      (address(scale) | address(expert_frequency_offset) | address(x_gather_idx) | address(s_reverse_scatter_idx)) % 4 != 0)
+      (address(scale) | address(expert_frequency_offset) | address(expert_frequency) | address(x_gather_idx) | address(s_reverse_scatter_idx)) % 4 != 0)
     return SMOE_ERR_ALIGNMENT;
   Params p = {};
   p.x = static_cast<const char*>(x); p.x_ld = 2 * ld;
   p.a = static_cast<const char*>(a); p.b = static_cast<const char*>(b); p.scale = scale;
   p.base = static_cast<const char*>(base); p.base_ld = base != nullptr ? 2 * base_ld : 0;
   p.out = static_cast<char*>(out); p.out_ld = 2 * out_ld;
-  p.off = expert_frequency_offset; p.gather = x_gather_idx; p.reverse = s_reverse_scatter_idx;
+  p.off = expert_frequency_offset; p.count = expert_frequency; p.gather = x_gather_idx; p.reverse = s_reverse_scatter_idx;
   p.T = T; p.rows = static_cast<int>(rows); p.H = H; p.N = N; p.n = n; p.r = r;
   p.in_place = base == out && base_ld == out_ld;
   const bool aligned = (address(x) | address(a) | address(b) | address(base) | address(out) | p.x_ld | p.base_ld | p.out_ld) % 16 == 0 && H % 8 == 0 &&

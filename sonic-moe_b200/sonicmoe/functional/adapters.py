@@ -71,13 +71,15 @@ def adapter_linear(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, permutatio
     for t, name in ((a, "a"), (b, "b")):
         if t.device != dev or not t.is_contiguous():
             raise ValueError(f"{name} has to be a contiguous tensor on {dev}, got strides {t.stride()} on {t.device}")
-    pair, row, offset = permutation.s_reverse_scatter_idx, permutation.x_gather_idx, permutation.expert_frequency_offset
+    pair, row = permutation.s_reverse_scatter_idx, permutation.x_gather_idx
+    offset, count = permutation.expert_frequency_offset, permutation.expert_frequency
     _check_permutation(pair, row, dev)
     if pair.shape != (T, 1):
         raise ValueError(f"the permutation has to be of ({T}, 1) pairs, got {tuple(pair.shape)}")
-    if offset.dtype != torch.int32 or offset.shape != (n + 1,) or offset.device != dev or not offset.is_contiguous():
-        raise ValueError(f"the permutation has to be by {n} adapters, a contiguous int32 offset tensor on {dev}, got {offset.dtype} "
-                         f"{tuple(offset.shape)} on {offset.device}")
+    for t, size in ((offset, n + 1), (count, n)):
+        if t.dtype != torch.int32 or t.shape != (size,) or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"the permutation has to be by {n} adapters, contiguous int32 tensors on {dev}, got {t.dtype} "
+                             f"{tuple(t.shape)} on {t.device}")
     align = permutation.align
     if align <= 0 or align % 16:
         raise ValueError(f"the permutation's align has to be a multiple of 16, got {align} (adapter_permutation chooses one)")
@@ -102,6 +104,6 @@ def adapter_linear(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, permutatio
         out = base if inplace else torch.empty_like(base) if base is not None and base.is_contiguous() else x.new_empty((T, N))
         check(lib.smoe_adapter_linear(
             x.data_ptr(), x.stride(0), a.data_ptr(), b.data_ptr(), ptr(scale), ptr(base), base_ld, out.data_ptr(),
-            base_ld if inplace else N, _TYPES[x.dtype], offset.data_ptr(), row.data_ptr(), pair.data_ptr(), T, rows, H, N, n, r, align,
+            base_ld if inplace else N, _TYPES[x.dtype], offset.data_ptr(), count.data_ptr(), row.data_ptr(), pair.data_ptr(), T, rows, H, N, n, r, align,
             stream_ptr(dev)), "adapter_linear")
     return out
