@@ -533,7 +533,7 @@ int smoe_rms_norm_backward(const void* dy, long long dy_ld, const void* dh, long
 int smoe_adapter_linear(const void* x, long long ld, const void* a, const void* b, const float* scale, const void* base,
                         long long base_ld, void* out, long long out_ld, int dtype, const int* expert_frequency_offset,
                         const int* expert_frequency, const int* x_gather_idx, const int* s_reverse_scatter_idx, int T, long long rows, int H, int N, int n,
-                        int r, int align, void* stream);
+                        int r, int align, int* status, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Expert parallelism over peer memory (one node, NVLink / NVSwitch).  The reference has no distributed

@@ -113,7 +113,7 @@ SIGNATURES: dict[str, tuple] = {
     "smoe_rms_norm": (I, [P, LL, P, LL, P, I, P, P, P, P, LL, P, I, LL, I, F, P]),
     "smoe_rms_norm_backward_workspace_bytes": (c_size_t, [LL, I]),
     "smoe_rms_norm_backward": (I, [P, LL, P, LL, P, LL, P, I, P, P, P, I, LL, I, P, P]),
-    "smoe_adapter_linear": (I, [P, LL, P, P, P, P, LL, P, LL, I, P, P, P, P, I, LL, I, I, I, I, I, P]),
+    "smoe_adapter_linear": (I, [P, LL, P, P, P, P, LL, P, LL, I, P, P, P, P, I, LL, I, I, I, I, I, P, P]),
     "smoe_peer_alloc": (I, [c_size_t, P]),
     "smoe_peer_free": (I, [P]),
     "smoe_peer_export": (I, [P, P]),

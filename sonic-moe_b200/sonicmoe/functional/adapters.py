@@ -105,5 +105,5 @@ def adapter_linear(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, permutatio
         check(lib.smoe_adapter_linear(
             x.data_ptr(), x.stride(0), a.data_ptr(), b.data_ptr(), ptr(scale), ptr(base), base_ld, out.data_ptr(),
             base_ld if inplace else N, _TYPES[x.dtype], offset.data_ptr(), count.data_ptr(), row.data_ptr(), pair.data_ptr(), T, rows, H, N, n, r, align,
-            stream_ptr(dev)), "adapter_linear")
+            _lib.device_state(dev).status.data_ptr(), stream_ptr(dev)), "adapter_linear")
     return out

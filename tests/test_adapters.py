@@ -10,8 +10,8 @@ def test_refusals(built_library):
     at = 4096
 
     def call(x=at, ld=64, a=at, b=at, scale=None, base=None, base_ld=0, out=at, out_ld=32, dtype=1, off=at, count=at, gather=at, reverse=at, T=5000,
-             rows=5120, H=64, N=32, n=4, r=8, align=32):
-        return lib.smoe_adapter_linear(x, ld, a, b, scale, base, base_ld, out, out_ld, dtype, off, count, gather, reverse, T, rows, H, N, n, r, align, None)
+             rows=5120, H=64, N=32, n=4, r=8, align=32, status=None):
+        return lib.smoe_adapter_linear(x, ld, a, b, scale, base, base_ld, out, out_ld, dtype, off, count, gather, reverse, T, rows, H, N, n, r, align, status, None)
 
     assert call(dtype=0) == call(dtype=2) == -6
     assert call(T=-1) == call(rows=-1) == call(H=0) == call(N=0) == call(n=0) == call(n=4097) == call(r=0) == call(r=129) == -1
@@ -19,7 +19,7 @@ def test_refusals(built_library):
     assert call(H=2 ** 28 + 1) == call(N=2 ** 28 + 1, out_ld=2 ** 30) == call(rows=2 ** 31 - 2 ** 15) == call(T=2 ** 31 - 2 ** 15) == -1
     assert call(x=None) == call(a=None) == call(b=None) == call(out=None) == call(off=None) == call(count=None) == call(gather=None) == call(reverse=None) == -1
     assert call(x=at + 1) == call(a=at + 1) == call(b=at + 1) == call(out=at + 1) == call(base=at + 1) == -2
-    assert call(scale=at + 2) == call(off=at + 2) == call(count=at + 2) == call(gather=at + 2) == call(reverse=at + 2) == -2
+    assert call(scale=at + 2) == call(off=at + 2) == call(count=at + 2) == call(gather=at + 2) == call(reverse=at + 2) == call(status=at + 2) == -2
     assert call(T=0) == 0
 
 
