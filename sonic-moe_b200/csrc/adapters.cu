@@ -279,9 +279,11 @@ int smoe_adapter_linear(const void* x, long long ld, const void* a, const void* 
   const int warps = few ? kWarps : warps_of(T, n);
   p.sparse = (rows + 15) / 16 > tiles_of(T, n, 16);
   p.tiles = static_cast<int>(few && !p.sparse && rows > 0 ? (rows + 15) / 16 : tiles_of(T, n, few ? 16 : 16 * warps));  // (one at least: its blocks see to the other tokens)
-  // tiles that there may be, half of the adapters having one that is not full: as many blocks as run at a time, two to an SM, share them
-  const int likely = (T + 16 * warps - 1) / (16 * warps) + (n < T ? n : T) / 2;
-  p.cluster = few ? kCluster : likely > 148 ? 1 : likely > 74 ? 2 : likely > 37 ? 4 : 8;
+  // Warps of the tiles that there may be, half of the adapters having one that is not full: as many blocks share a tile as let 1200 to 2400 warps, eight
+  // to sixteen to an SM, run at a time.  2048 tokens of 100 adapters, 4096 x 1024, rank 32, take 50 / 31 / 23 / 18 us with 1 / 2 / 4 / 8 blocks to a tile
+  // of 32 rows; 8192 of 400 110 / 84 / 84 / 85; 8192 of 8, 4096 x 4096, rank 64, 56 us with four to a tile of 128; 32768 of them 183 / 194 / 209 / 244.
+  const long long likely = warps * ((T + 16ll * warps - 1) / (16 * warps) + (n < T ? n : T) / 2);
+  p.cluster = few ? kCluster : likely > 8 * 148 ? 1 : likely > 4 * 148 ? 2 : likely > 2 * 148 ? 4 : 8;
   // The tokens without an adapter: a warp of clusters behind the tiles' for each, or, with many tokens, some of them for every warp of the tiles (blocks
   // of their own made 8192 tokens that all have adapters wait 13 us for blocks that found nothing).
   long long blocks = static_cast<long long>(p.tiles) * p.cluster;
