@@ -207,7 +207,14 @@ static long long tiles_of(int T, int n, int rows) {
   const long long tiles = T / rows + static_cast<long long>(n < T ? n : T);
   return tiles < T ? tiles : T;
 }
-static bool by_few_rows(int T, int n, int r) { return tiles_of(T, n, 16) * padded_rank(r) <= 4096; }
+// Tiles of 16 rows and eight blocks each: while few of them are needed, more for wide rows, and where it is the weights of adapters with a few tokens each that take the
+// time, which come straight from memory there.  us by few_kernel / by tiles, 4096 x 4096 unless said: 256 tokens of 2 adapters, rank 16, 7 / 14; 512 of
+// 4, rank 64, 14 / 21, 1024 x 1024 10 / 11; 2048 of 4, rank 16, 22 / 21, 1024 x 1024 14 / 10; 64 of 64, rank 128, 41 / 54, 4097 x 4095 68 / 310; 512 of 100, rank 64, 27 / 31, rank 128, 64 / 56, 4097 x 4095
+// 118 / 346; 4096 of 500, rank 64, 132 / 107, 4097 x 4095, rank 128, 524 / 1219; 448 of 160, 342 x 187, rank 16, 31 / 16.
+static bool by_few_rows(int T, int n, int r, int H, int N, bool aligned) {
+  const long long size = tiles_of(T, n, 16) * padded_rank(r);
+  return size <= (H + N > 8000 ? 2304 : 1024) || (T / n < 16 && H + N > 3000 && (!aligned || size <= 8192));
+}
 // Warps of a tile's blocks otherwise, by the tokens that an adapter has on average.
 static int warps_of(int T, int n) { return T / n <= 32 ? 2 : T / n <= 64 ? 4 : 8; }
 
@@ -275,7 +282,9 @@ int smoe_adapter_linear(const void* x, long long ld, const void* a, const void* 
   p.off = expert_frequency_offset; p.count = expert_frequency; p.gather = x_gather_idx; p.reverse = s_reverse_scatter_idx;
   p.T = T; p.rows = static_cast<int>(rows); p.H = H; p.N = N; p.n = n; p.r = r;
   p.status = status;
-  const bool few = by_few_rows(T, n, r);
+  const bool wide_in = (address(x) | address(a) | address(b) | p.x_ld) % 16 == 0 && H % 8 == 0 && r % 8 == 0;
+  const bool wide_out = (address(base) | address(out) | p.base_ld | p.out_ld) % 16 == 0 && N % 8 == 0;
+  const bool few = by_few_rows(T, n, r, H, N, wide_in && wide_out);
   const int warps = few ? kWarps : warps_of(T, n);
   p.sparse = (rows + 15) / 16 > tiles_of(T, n, 16);
   p.tiles = static_cast<int>(few && !p.sparse && rows > 0 ? (rows + 15) / 16 : tiles_of(T, n, few ? 16 : 16 * warps));  // (one at least: its blocks see to the other tokens)
@@ -292,8 +301,6 @@ int smoe_adapter_linear(const void* x, long long ld, const void* a, const void* 
     if (few) blocks += (T + kCluster * kWarps - 1ll) / (kCluster * kWarps) * kCluster;
   }
   if (blocks > 0x7fffffffll) return SMOE_ERR_SHAPE;
-  const bool wide_in = (address(x) | address(a) | address(b) | p.x_ld) % 16 == 0 && H % 8 == 0 && r % 8 == 0;
-  const bool wide_out = (address(base) | address(out) | p.base_ld | p.out_ld) % 16 == 0 && N % 8 == 0;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (!few) return launch_tiles(p, dtype, wide_in, wide_out, warps, blocks, st);
   if (dtype == SMOE_BF16) return wide_in && wide_out ? launch_few<__nv_bfloat16, true>(p, blocks, st) : launch_few<__nv_bfloat16, false>(p, blocks, st);
