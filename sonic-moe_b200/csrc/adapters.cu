@@ -211,12 +211,24 @@ static long long tiles_of(int T, int n, int rows) {
 // time, which come straight from memory there.  us by few_kernel / by tiles, 4096 x 4096 unless said: 256 tokens of 2 adapters, rank 16, 7 / 14; 512 of
 // 4, rank 64, 14 / 21, 1024 x 1024 10 / 11; 2048 of 4, rank 16, 22 / 21, 1024 x 1024 14 / 10; 64 of 64, rank 128, 41 / 54, 4097 x 4095 68 / 310; 512 of 100, rank 64, 27 / 31, rank 128, 64 / 56, 4097 x 4095
 // 118 / 346; 4096 of 500, rank 64, 132 / 107, 4097 x 4095, rank 128, 524 / 1219; 448 of 160, 342 x 187, rank 16, 31 / 16.
-static bool by_few_rows(int T, int n, int r, int H, int N, bool aligned) {
-  const long long size = tiles_of(T, n, 16) * padded_rank(r);
-  return size <= (H + N > 8000 ? 2304 : 1024) || (T / n < 16 && H + N > 3000 && (!aligned || size <= 8192));
+// Of those, the ones with tcgen05.mma need fewer (wide_in, rows of out that start anywhere: 2048 of 100, rank 128, 247 / 121, 512 of 100, rank 64, 65 / 57,
+// rank 32, 34 / 49).  Twelve tiles would leave most of the card idle as tiles of more rows: 130 tokens of 2, 1920 x 5917, rank 124, 25 / 55.
+static bool by_few_rows(int T, int n, int r, int H, int N, bool wide_in, bool wide_out) {
+  const int rank = padded_rank(r);
+  const bool tensor = wide_in && !wide_out && rank >= 64;
+  const long long tiles = tiles_of(T, n, 16), size = tiles * rank;
+  return tiles <= 12 || size <= (H + N > 8000 && !tensor ? 2304 : 1024) || (T / n < 16 && H + N > 3000 && !tensor && (!wide_out || !wide_in || size <= 8192));
 }
-// Warps of a tile's blocks otherwise, by the tokens that an adapter has on average.
-static int warps_of(int T, int n) { return T / n <= 32 ? 2 : T / n <= 64 ? 4 : 8; }
+// Warps of a tile's blocks otherwise, by the tokens that an adapter has on average: eight where that brings in tcgen05.mma, more for wide weights, which the
+// warps fetch together.  us with 2 / 4 / 8: 2048 tokens of 100, 4096 x 4096, rank 32, 27 / 36 / 38, rank 128, 86 / 63 / 82, 4097 x 4095, rank 32, 66 / 89 /
+// 85, rank 64, 194 / 133 / 112, rank 128, 533 / 222 / 283, 4096 x 4095, rank 32, 66 / 87 / 65, rank 64, 193 / 133 / 71; 512 of 100, 342 x 187, rank 64, 15 / 19
+// / 15; 1024 of 16, 4096 x 4096, rank 128, 56 / 37 / 49.
+static int warps_of(int T, int n, int r, bool wide_in, bool wide_out) {
+  const int rank = padded_rank(r), tokens = T / n;
+  if (wide_in && !wide_out && (rank >= 64 || (rank == 32 && tokens >= 16))) return 8;
+  const int two = rank == 128 ? (wide_in ? 16 : 0) : rank == 64 && !wide_in ? 16 : 32;
+  return tokens <= two && two > 0 ? 2 : tokens <= 64 ? 4 : 8;
+}
 
 // Blocks of few_kernel with AHEAD that an SM has room for.
 template <int RP, bool ALIGNED>
@@ -284,8 +296,8 @@ int smoe_adapter_linear(const void* x, long long ld, const void* a, const void* 
   p.status = status;
   const bool wide_in = (address(x) | address(a) | address(b) | p.x_ld) % 16 == 0 && H % 8 == 0 && r % 8 == 0;
   const bool wide_out = (address(base) | address(out) | p.base_ld | p.out_ld) % 16 == 0 && N % 8 == 0;
-  const bool few = by_few_rows(T, n, r, H, N, wide_in && wide_out);
-  const int warps = few ? kWarps : warps_of(T, n);
+  const bool few = by_few_rows(T, n, r, H, N, wide_in, wide_out);
+  const int warps = few ? kWarps : warps_of(T, n, r, wide_in, wide_out);
   p.sparse = (rows + 15) / 16 > tiles_of(T, n, 16);
   p.tiles = static_cast<int>(few && !p.sparse && rows > 0 ? (rows + 15) / 16 : tiles_of(T, n, few ? 16 : 16 * warps));  // (one at least: its blocks see to the other tokens)
   // Warps of the tiles that there may be, half of the adapters having one that is not full: as many blocks share a tile as let 1200 to 2400 warps, eight
