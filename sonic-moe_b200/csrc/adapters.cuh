@@ -180,9 +180,12 @@ __device__ __forceinline__ int4 tile_of(const Params& p, int tile, int tile_rows
     sum = before + scan(here);
     found = __ballot_sync(0xffffffffu, tile < sum);
     if (found != 0u) {
-      const int at = __ffs(found) - 1, e = e0 + at, first = min(max(p.off[e], 0), p.rows);
-      const int row = first + (tile - __shfl_sync(0xffffffffu, sum - here, at)) * tile_rows;
-      return make_int4(e, row, min(min(row + tile_rows, first + max(p.count[e], 0)), p.rows), 0);
+      const int at = __ffs(found) - 1, e = e0 + at;
+      const int first = min(max(p.off[e], 0), p.rows);
+      const long long row = first + static_cast<long long>(tile - __shfl_sync(0xffffffffu, sum - here, at)) * tile_rows;
+      if (row < 0 || row >= p.rows) return make_int4(-1, 0, 0, 0);  // (counts that no sort gave)
+      const long long end = min(row + tile_rows, static_cast<long long>(first) + max(p.count[e], 0));
+      return make_int4(e, static_cast<int>(row), static_cast<int>(min(end, static_cast<long long>(p.rows))), 0);
     }
     before = __shfl_sync(0xffffffffu, sum, 31);
   }

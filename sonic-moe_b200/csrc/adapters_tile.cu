@@ -349,7 +349,6 @@ __device__ __forceinline__ constexpr uint32_t instruction(int N) {  // 128 rows,
 
 template <class T, int RP, bool WIDE>
 __global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) tensor_kernel(const Params p) {
-  release_next();
   wait_for_previous();
   using Te = Tensor<RP, WIDE>;
   extern __shared__ char smem_any[];
@@ -391,6 +390,7 @@ __global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) tensor_kernel(c
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  release_next();  // not before: a next kernel that waits for this one with all of the tensor memory in hand would leave this block none
   const uint32_t tmem = tmem_slot;
   volatile int* abort_flag = &gave_up;
 

@@ -48,13 +48,25 @@ def _refuse_gradients(*tensors) -> None:
                 raise NotImplementedError("the adapters have no forward-mode derivative")
 
 
+def _meets_other_rows(x: torch.Tensor, out: torch.Tensor) -> bool:
+    """Whether rows of out, at the distance of out.stride(0), share memory with rows of x of other tokens."""
+    (T, H), N = x.shape, out.shape[1]
+    if T <= 1:
+        return False
+    ahead, ld = (out.data_ptr() - x.data_ptr()) // x.element_size(), x.stride(0)
+    if ahead >= (T - 1) * ld + H or -ahead >= (T - 1) * out.stride(0) + N:
+        return False
+    return ld != out.stride(0) or ahead + N > ld or H - ahead > ld
+
+
 def adapter_linear(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, permutation: TokenPermutation,
                    base: torch.Tensor | None = None, scale: torch.Tensor | None = None, inplace: bool = False) -> torch.Tensor:
     """out (T, N) = base + scale[e] b[e] (a[e] x), and base where a token has no adapter (None: zeros).
 
     x (T, H), base (T, N), a (n, r, H) and b (n, N, r), all bf16 or all fp16; scale (n,) fp32, None: 1.  ``permutation``: of the T tokens by
     n adapters, K = 1, an ``align`` that is a multiple of 16 (`adapter_permutation`).  ``inplace`` adds to base, which is returned, and
-    leaves the rows of tokens without an adapter as they are; base may be a slice of columns."""
+    leaves the rows of tokens without an adapter as they are; base may be a slice of columns, and share memory with the same tokens' rows of x
+    (not with those of others)."""
     if x.dim() != 2 or a.dim() != 3 or b.dim() != 3:
         raise ValueError(f"x has to be (T, H), a (n, r, H) and b (n, N, r), got {tuple(x.shape)}, {tuple(a.shape)} and {tuple(b.shape)}")
     (T, H), (n, r), N = x.shape, a.shape[:2], b.shape[1]
@@ -97,6 +109,8 @@ def adapter_linear(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, permutatio
         raise ValueError(f"{max(T, rows)} rows do not fit into 32-bit numbers")
     with _lib.on_device(dev):
         x = x if x.stride(1) == 1 or H == 1 else x.contiguous()
+        if inplace and _meets_other_rows(x, base):
+            raise ValueError("a base that is added to in place shares memory with other tokens' rows of x")
         if base is not None and base.stride(1) != 1 and N > 1:
             base = base.contiguous()
         # (the distance of a single row means nothing)

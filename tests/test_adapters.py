@@ -54,3 +54,26 @@ def test_python_refusals(built_library):
         sonicmoe.adapter_permutation(idx.float(), 3)
     with pytest.raises(SonicMoEError, match="no CPU path"):
         sonicmoe.adapter_permutation(idx, 3)
+
+
+def test_rows_that_share_memory(built_library):
+    from sonicmoe.functional.adapters import _meets_other_rows
+
+    flat = torch.zeros(4000, dtype=torch.bfloat16)
+    wide = flat.view(40, 100)
+
+    def brute(x, out):
+        at = lambda t: (t.data_ptr() - flat.data_ptr()) // 2
+        rows = lambda t: [set(range(at(t[i]), at(t[i]) + t.shape[1])) for i in range(t.shape[0])]
+        xs, outs = rows(x), rows(out)
+        return any(xs[i] & outs[j] for i in range(len(xs)) for j in range(len(outs)) if i != j)
+
+    for x, out in ((wide[:10, :60], wide[:10, 60:]), (wide[:10, 60:], wide[:10, :60]), (wide[:10, :60], wide[:10, 20:90]), (wide[:10], wide[:10]),
+                   (wide[:10], wide[10:20]), (wide[:10], wide[9:19]), (wide[1:11, :30], wide[:10, 40:]), (wide[:1], wide[:1, :7]),
+                   (wide[0].expand(10, 100), wide[:10]), (wide[0].expand(10, 100), wide[1:11]), (flat[5:1005].view(10, 100), wide[:10]),
+                   (wide[5:15], wide[:5]), (flat[:500].view(5, 100), flat[500:1500].view(5, 200)), (flat[:500].view(5, 100), flat[400:1400].view(5, 200))):
+        # (rows at different distances that only share their range are taken to meet)
+        assert _meets_other_rows(x[:out.shape[0]], out) >= brute(x[:out.shape[0]], out)
+        if x.stride(0) == out.stride(0):
+            assert _meets_other_rows(x[:out.shape[0]], out) == brute(x[:out.shape[0]], out)
+    assert not _meets_other_rows(wide[:10, :60], wide[:10, 60:]) and not _meets_other_rows(wide[1:11, :30], wide[:10, 40:])

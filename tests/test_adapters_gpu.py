@@ -138,6 +138,21 @@ def test_in_place_into_a_slice(built_library, T, align, N):
     assert torch.equal(qkv, before) and got.data_ptr() == qkv[:, N:].data_ptr()
 
 
+@pytest.mark.parametrize("T,n,r", [(30, 4, 16), (900, 40, 16), (4400, 5, 16), (4400, 5, 64)])
+def test_in_place_into_the_rows_that_are_read(built_library, T, n, r):
+    import sonicmoe
+
+    for H in (256, 251):
+        x, a, b, idx, _, scale = make(T, H, H, n, r, torch.bfloat16)
+        p = sonicmoe.adapter_permutation(idx, n)
+        want = sonicmoe.adapter_linear(x, a, b, p, base=x, scale=scale)
+        check(want, x, a, b, idx, x, scale)
+        assert torch.equal(sonicmoe.adapter_linear(x, a, b, p, base=x, scale=scale, inplace=True), want)
+    flat = torch.zeros((T + 1) * 256, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="other tokens' rows"):
+        sonicmoe.adapter_linear(flat[:-256].view(T, 256), a.new_zeros(n, r, 256), b.new_zeros(n, 256, r), p, base=flat[256:].view(T, 256), inplace=True)
+
+
 @pytest.mark.parametrize("T,align", [(30, 16), (600, 32), (4400, 16), (4400, 128)])
 def test_loads(built_library, T, align):
     """All tokens with one adapter, none with any, every token with its own, the first or the last one alone."""
@@ -215,6 +230,37 @@ def test_the_same_bits_every_time_and_in_a_graph(built_library):
         graph.replay()
         check(got, x, a, b, live, base, scale)
         torch.cuda.synchronize()
+
+
+def test_between_other_kernels_with_tensor_memory(built_library):
+    """Tiles by tensor memory with products that want all of it right behind them, on two streams."""
+    import sonicmoe
+    from sonicmoe.functional import int8
+
+    x, a, b, idx, base, scale = make(9000, 512, 512, 3, 64, torch.bfloat16)
+    p = sonicmoe.adapter_permutation(idx, 3)
+    g = torch.Generator().manual_seed(4)
+    wq, w_scale = int8.quantize_rows((torch.randn(512, 512, generator=g) * 0.05).cuda())
+
+    def chain():
+        out = x
+        for _ in range(6):
+            out = sonicmoe.adapter_linear(out, a, b, p, base=int8.int8_linear(out, wq, w_scale, out_dtype=torch.bfloat16), scale=scale)
+            out = out / 4
+        return out
+
+    want = chain()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            got.append(chain())
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in got)
+    sonicmoe.check_status()
 
 
 def test_adapter_permutation(built_library):
