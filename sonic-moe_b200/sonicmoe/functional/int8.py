@@ -214,16 +214,23 @@ def moe_int8_softmax_topk_layer(
     experts: Int8Experts,
     K: int,
     activation_type: ActivationType | str = ActivationType.SWIGLU,
+    x_q: torch.Tensor | None = None,
+    x_scale: torch.Tensor | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Inference forward of the token-choice top-K layer with 8-bit experts: (o (T, H), router_logits (T, E), expert_frequency
     (E,) int32), as `moe_TC_softmax_topk_layer`.  x (T, H) bf16, quantised per token; the activations between the projections are
-    rounded to bf16 and quantised per row."""
+    rounded to bf16 and quantised per row.  ``x_q`` (T, H) int8 with ``x_scale`` (T,): x's rows in 8 bits where the norm in front has made
+    them already (`rms_norm_quantize` with ``keep_y``); x then serves the router alone."""
     from . import _FusedRouter, _route_metadata, fused_router_applies, topk_softmax
 
     if isinstance(activation_type, str):
         activation_type = ActivationType(activation_type)
-    _refuse_gradients(x, router_w, experts.w1_scale, experts.b1, experts.w2_scale, experts.b2)
+    _refuse_gradients(x, router_w, experts.w1_scale, experts.b1, experts.w2_scale, experts.b2, x_scale)
+    if (x_q is None) != (x_scale is None):
+        raise ValueError("x_q and x_scale belong together")
     _lib.require_cuda(x, "x")
+    if x_q is not None and (x_q.dtype != torch.int8 or x_q.shape != x.shape or x_q.device != x.device):
+        raise ValueError(f"x_q has to be int8 {tuple(x.shape)} on {x.device}, got {x_q.dtype} {tuple(x_q.shape)} on {x_q.device}")
     if x.dtype != torch.bfloat16 or x.dim() != 2:
         raise TypeError(f"x has to be (T, H) bf16, got {x.dtype} {tuple(x.shape)}")
     T, H = x.shape
@@ -245,7 +252,7 @@ def moe_int8_softmax_topk_layer(
             scores, indices = topk_softmax(router_logits, K)
         route = _route_metadata(indices.reshape(-1), None, E, K)
         code = _ACTIVATIONS[activation_type]
-        y1 = _linear(x, experts.w1q, experts.w1_scale, None, experts.b1, None, code, route.expert_frequency_offset, None,
+        y1 = _linear(x if x_q is None else x_q, experts.w1q, experts.w1_scale, x_scale, experts.b1, None, code, route.expert_frequency_offset, None,
                      route.x_gather_idx)
         y2 = _linear(y1, experts.w2q, experts.w2_scale, None, experts.b2, None, -1, route.expert_frequency_offset, None, None)
         with _lib.on_device(x.device):

@@ -355,3 +355,58 @@ def test_on_another_stream_and_in_a_graph(built_library):
         ye, he = sonicmoe.rms_norm(xe, ws.detach(), EPS, residual=rs.detach())
         assert torch.equal(y, ye) and torch.equal(h, he)
         assert torch.equal(grads[0], torch.autograd.grad((ye, he), xe, (dy, dh))[0])
+
+
+@pytest.mark.parametrize("T", [1, 40, 3000])
+@pytest.mark.parametrize("residual", [False, True])
+def test_the_8_bit_layer_takes_the_rows(built_library, T, residual):
+    """The layer on a norm's 8-bit rows against the layer on those of quantize_rows, which differ where a value is next to a border, and the layer's
+    own quantising against rows that are given: the same bits."""
+    import sonicmoe
+    from sonicmoe.functional import int8
+
+    g = torch.Generator().manual_seed(12)
+    H, I, E, K = 256, 64, 8, 2
+    x = torch.randn(T, H, generator=g).bfloat16().cuda()
+    h0 = torch.randn(T, H, generator=g).bfloat16().cuda() if residual else None
+    weight = (1 + 0.1 * torch.randn(H, generator=g)).bfloat16().cuda()
+    router = (torch.randn(E, H, generator=g) * 0.1).bfloat16().cuda()
+    w1 = (torch.randn(E, 2 * I, H, generator=g) * 2 / H ** 0.5).bfloat16().cuda()
+    w2 = (torch.randn(E, H, I, generator=g) / I ** 0.5).bfloat16().cuda()
+    experts = int8.quantize_experts(w1.permute(1, 2, 0), None, w2.permute(1, 2, 0), None)
+    r = sonicmoe.rms_norm_quantize(x, weight, residual=h0, keep_y=True)
+    o, logits, frequency = int8.moe_int8_softmax_topk_layer(r.y, router, experts, K, x_q=r.q, x_scale=r.scale)
+    h = (x if h0 is None else r.h).double()
+    y = h * torch.rsqrt(h.square().mean(1, keepdim=True) + 1e-6) * weight.double()
+    q, scale = int8.quantize_rows(y.float())
+    # fp32 sums of 256 squares, a root and three products: under 2^-19 of y and of the scale, so that a value within 127 2^-19 of a step of a border may
+    # go to the other side: 127 2^-18 of all values, evenly spread, and 8 for the spread of a small number
+    assert (r.q != q).sum() <= 8 + T * H * 127 * 2.0 ** -18 and (r.q.int() - q.int()).abs().max() <= 1
+    assert ((r.scale - scale).abs() <= 2.0 ** -19 * scale).all()
+    same = int8.moe_int8_softmax_topk_layer(r.y, router, experts, K, x_q=q, x_scale=scale)
+    assert torch.equal(same[1], logits) and torch.equal(same[2], frequency)
+    # a value by a step changes its row by under 1 / 127 (its largest value, 1/16 of the row's norm at least, over 127), and what follows is rounded twice
+    # to bf16 (2^-8) and once to 8 bits (1 / 127) where it changes
+    assert ((o.double() - same[0].double()).norm() / o.double().norm()).item() < 4 / 127
+    own = int8.moe_int8_softmax_topk_layer(r.y, router, experts, K)
+    q, scale = int8.quantize_rows(r.y)
+    given = int8.moe_int8_softmax_topk_layer(r.y, router, experts, K, x_q=q, x_scale=scale)
+    assert all(torch.equal(a, b) for a, b in zip(own, given))
+
+
+def test_rows_that_the_8_bit_layer_refuses(built_library):
+    from sonicmoe.functional import int8
+
+    x = torch.randn(4, 256, device="cuda").bfloat16()
+    router = torch.randn(8, 256, device="cuda").bfloat16()
+    experts = int8.quantize_experts(torch.randn(128, 256, 8, device="cuda").bfloat16(), None, torch.randn(256, 64, 8, device="cuda").bfloat16(), None)
+    q, scale = int8.quantize_rows(x)
+    for bad in ({"x_q": q}, {"x_scale": scale}):
+        with pytest.raises(ValueError, match="belong together"):
+            int8.moe_int8_softmax_topk_layer(x, router, experts, 2, **bad)
+    for bad in (q[:3], q[:, :128], q.short(), q.cpu()):
+        with pytest.raises(ValueError, match="x_q has to be"):
+            int8.moe_int8_softmax_topk_layer(x, router, experts, 2, x_q=bad, x_scale=scale)
+    for bad in (scale[:3], scale.double(), scale.cpu()):
+        with pytest.raises(ValueError, match="x_scale has to be"):
+            int8.moe_int8_softmax_topk_layer(x, router, experts, 2, x_q=q, x_scale=bad)
