@@ -17,6 +17,9 @@ struct Few {
 
 // AHEAD: a warp's weights and base for its first columns of out are on their way before the blocks add their parts, those of the next ones before the
 // last are done, and more of x and a at a time.  That takes registers, so it is for as many blocks as there is room for at once.
+// Latency bounds it (bf16, us): one token, 4096 x 4096, rank 16 4.8 (5.5 without AHEAD); 64 tokens of 64 adapters, 4096 x 2048, rank 16 8.3, rank 64 18
+// (1.75 TB/s of weights, x, base and out); 128 tokens of 2, 4096 x 4096, rank 64 8.8 (13 without); 256 of 4, rank 16 6.9.  Clusters: its rows are too
+// few to fill the card, so eight blocks share the columns of each 16.
 template <class T, int RP, bool ALIGNED, bool AHEAD>
 __global__ void __launch_bounds__(32 * kWarps, AHEAD ? 1 : RP == 16 ? (ALIGNED ? 4 : 2) : RP == 32 ? (ALIGNED ? 3 : 2) : RP == 64 && ALIGNED ? 2 : 1) few_kernel(const Params p) {
   release_next();

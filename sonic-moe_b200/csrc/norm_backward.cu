@@ -38,7 +38,8 @@ __device__ __forceinline__ void row_gradient(const Values<T, EP, VE>& dy, const 
 }
 
 // Blocks take rows in turn and keep the weights and their part of the weights' gradient in registers, EP columns in each thread, until the end: so
-// the rows of a thread all have the same shift (Columns), `step` rows apart.  A row is read once.  Bound by memory.
+// the rows of a thread all have the same shift (Columns), `step` rows apart.  A row is read once.  Bound by memory: bf16 32768 x 4096
+// with a residual 171 us, 6.3 TB/s, 8192 x 4096 51; 262144 x 128 36.5, 5.5 TB/s; fp32 4099 x 1005 16.5 us.
 template <class T, class W, int EP, bool ALIGNED, int REGISTERS>
 __global__ void __maxnreg__(REGISTERS) backward_kernel(const Backward a, int tpr) {
   wait_for_previous();

@@ -8,7 +8,9 @@
 
 y = h / sqrt(mean(h^2) + eps) * weight over the last dimension.  h is rounded to the type of x once, and y is the norm of that h; the
 sum of squares and everything up to y's one rounding is fp32 (squares past its range, of values above 1.8e19, make a row zeros).  The 8-bit
-rows are those of the unrounded y: scale = amax / 127, values rounded half to even, as `int8.quantize_rows` makes them of fp32 rows.
+rows are those of the unrounded y: scale = amax / 127, values rounded half to even, as `int8.quantize_rows` makes them of fp32 rows (of bf16
+and fp16 x by one multiply-add: a value within 1.6e-5 of a step of a border may go to the other side).  They are what `int8.int8_linear` and
+`int8.moe_int8_softmax_topk_layer` take as x and x_q.
 
 fp32, bf16 and fp16 rows of any width; weights of the same type or fp32.  `rms_norm` has gradients for x, the residual and the
 weight (its sum over the rows is fp32, in the same order every time; the residual's gradient is that of x); second derivatives and forward-mode
