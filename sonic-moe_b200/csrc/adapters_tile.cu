@@ -504,12 +504,12 @@ __global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) tensor_kernel(c
         umma_commit(smem_u32(&done_first[i % Te::kFirst]));
       }
       // the stage before has been read: its place is the next one's
-      if (i > 0) mbar_wait(smem_u32(&done_first[(i - 1) % Te::kFirst]), (i - 1) / Te::kFirst & 1, abort_flag);
+      if (i > 0) mbar_wait_warp(smem_u32(&done_first[(i - 1) % Te::kFirst]), (i - 1) / Te::kFirst & 1, abort_flag);
       fetch(stage + Te::kFirst - 1);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     const int last = end - first - 1;
-    if (last >= 0) mbar_wait(smem_u32(&done_first[last % Te::kFirst]), last / Te::kFirst & 1, abort_flag);
+    if (last >= 0) mbar_wait_warp(smem_u32(&done_first[last % Te::kFirst]), last / Te::kFirst & 1, abort_flag);
     tc_fence_after();
     __syncthreads();
     for (int i = 0; i < Te::kEarly; ++i) fetch_second(i);  // on their way while the blocks add their parts
@@ -550,7 +550,7 @@ __global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) tensor_kernel(c
   uint4 left_over = make_uint4(0u, 0u, 0u, 0u);  // (not WIDE) the row's last eight results
   // the results of stage i, out
   const auto put = [&](int i) {
-    mbar_wait(smem_u32(&done_second[i & 1]), i >> 1 & 1, abort_flag);
+    mbar_wait_warp(smem_u32(&done_second[i & 1]), i >> 1 & 1, abort_flag);
     tc_fence_after();
     uint32_t v[32];
     tmem_ld32(tmem + 64 * (i & 1) + 32 * half + (static_cast<uint32_t>(quad * 32) << 16), v);
