@@ -210,17 +210,19 @@ static long long tiles_of(int T, int n, int rows) {
   const long long tiles = T / rows + static_cast<long long>(n < T ? n : T);
   return tiles < T ? tiles : T;
 }
-// Tiles of 16 rows and eight blocks each: while few of them are needed, more for wide rows, and where it is the weights of adapters with a few tokens each that take the
-// time, which come straight from memory there.  us by few_kernel / by tiles, 4096 x 4096 unless said: 256 tokens of 2 adapters, rank 16, 7 / 14; 512 of
-// 4, rank 64, 14 / 21, 1024 x 1024 10 / 11; 2048 of 4, rank 16, 22 / 21, 1024 x 1024 14 / 10; 64 of 64, rank 128, 41 / 54, 4097 x 4095 68 / 310; 512 of 100, rank 64, 27 / 31, rank 128, 64 / 56, 4097 x 4095
-// 118 / 346; 4096 of 500, rank 64, 132 / 107, 4097 x 4095, rank 128, 524 / 1219; 448 of 160, 342 x 187, rank 16, 31 / 16.
+// Tiles of 16 rows and eight blocks each: while few of them are needed, more for wide rows, and where it is the weights of adapters with a few tokens each
+// that take the time, which come straight from memory there.  us by few_kernel / by tiles, 4096 x 4096 unless said: 256 tokens of 2 adapters, rank 16,
+// 7 / 14; 512 of 8, rank 64, 13 / 20; 512 of 4, rank 64, 14 / 21, 1024 x 1024 13 / 12; 2048 of 4, rank 16, 21 / 21, 1024 x 1024 14 / 10; 64 of 64, rank
+// 128, 41 / 54, 4097 x 4095 68 / 310; 512 of 100, rank 64, 27 / 31, rank 128, 64 / 56, 4097 x 4095 118 / 346; 4096 of 500, rank 64, 132 / 107, 4097 x
+// 4095, rank 128, 524 / 1219; 448 of 160, 342 x 187, rank 16, 31 / 16.
 // Of those, the ones with tcgen05.mma need fewer (wide_in, rows of out that start anywhere: 2048 of 100, rank 128, 247 / 121, 512 of 100, rank 64, 65 / 57,
 // rank 32, 34 / 49).  Twelve tiles would leave most of the card idle as tiles of more rows: 130 tokens of 2, 1920 x 5917, rank 124, 25 / 55.
 static bool by_few_rows(int T, int n, int r, int H, int N, bool wide_in, bool wide_out) {
   const int rank = padded_rank(r);
   const bool tensor = wide_in && !wide_out && rank >= 64;
   const long long tiles = tiles_of(T, n, 16), size = tiles * rank;
-  return tiles <= 12 || size <= (H + N > 8000 && !tensor ? 2304 : 1024) || (T / n < 16 && H + N > 3000 && !tensor && (!wide_out || !wide_in || size <= 8192));
+  const int most = H + N <= 8000 || tensor ? 1024 : wide_in && wide_out ? 2600 : 2304;
+  return tiles <= 12 || size <= most || (T / n < 16 && H + N > 3000 && !tensor && (!wide_out || !wide_in || size <= 8192));
 }
 // Warps of a tile's blocks otherwise, by the tokens that an adapter has on average: eight where that brings in tcgen05.mma, more for wide weights, which the
 // warps fetch together.  us with 2 / 4 / 8: 2048 tokens of 100, 4096 x 4096, rank 32, 27 / 36 / 38, rank 128, 86 / 63 / 82, 4097 x 4095, rank 32, 66 / 89 /
