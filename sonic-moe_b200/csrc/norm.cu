@@ -214,6 +214,10 @@ __global__ void __launch_bounds__(kThreads) forward_long_kernel(const Forward a)
       }
     }
   }
+  if constexpr (Q) {  // zeros up to the next multiple of 16 columns where the rounds' pieces, `shift` columns ahead of them, end before it
+    const int covered = columns.first((columns.pieces + round - 1) / round * round);
+    if (covered + at.tid < (a.H + 15) / 16 * 16) a.q[row * a.q_ld + covered + at.tid] = 0;
+  }
 }
 
 template <class T, class W, int EP, bool ALIGNED, bool Q>

@@ -161,6 +161,25 @@ def test_fp32_rows_are_quantised_as_quantize_rows_does(built_library):
         assert torch.equal(r.q, q) and torch.equal(r.scale, scale)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H", [17, 1005, 16376, 16378, 16381, 16383, 16387, 24570, 24573, 24575, 32761, 131071])
+def test_columns_behind_8_bit_rows(built_library, dtype, H):
+    """Zeros up to the next multiple of 16, whatever was there, for rows of every shift; nothing behind that is written."""
+    import sonicmoe
+    from sonicmoe import _lib
+
+    T, width = 17, -(-H // 16) * 16
+    x, w = source(T, H, dtype, 1), weights(H, dtype, 2)
+    want = sonicmoe.rms_norm_quantize(x, w, EPS)
+    q = torch.full((T, width + 16), 85, dtype=torch.int8, device="cuda")
+    scale = torch.empty(T, dtype=torch.float32, device="cuda")
+    code = {torch.float32: _lib.SMOE_F32, torch.bfloat16: _lib.SMOE_BF16, torch.float16: _lib.SMOE_F16}[dtype]
+    _lib.check(_lib.lib.smoe_rms_norm(x.data_ptr(), H, None, 0, w.data_ptr(), code, None, None, None, q.data_ptr(), width + 16, scale.data_ptr(),
+                                      code, T, H, EPS, _lib.stream_ptr(x.device)), "rms_norm")
+    assert torch.equal(q[:, :H], want.q) and torch.equal(scale, want.scale)
+    assert (q[:, H:width] == 0).all() and (q[:, width:] == 85).all()
+
+
 def plain_gradients(x, w, eps, residual, dy, dh):
     _, h, r = plain(x, w, eps, residual)
     u = h.double() * r
