@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from .. import _lib
 from .._lib import check, lib, ptr, stream_ptr
@@ -66,7 +67,7 @@ def adapter_linear(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, permutatio
     x (T, H), base (T, N), a (n, r, H) and b (n, N, r), all bf16 or all fp16; scale (n,) fp32, None: 1.  ``permutation``: of the T tokens by
     n adapters, K = 1, an ``align`` that is a multiple of 16 (`adapter_permutation`).  ``inplace`` adds to base, which is returned, and
     leaves the rows of tokens without an adapter as they are; base may be a slice of columns, and share memory with the same tokens' rows of x
-    (not with those of others)."""
+    (not with those of others).  Autograd counts it as a change of base, as it does base.add_()."""
     if x.dim() != 2 or a.dim() != 3 or b.dim() != 3:
         raise ValueError(f"x has to be (T, H), a (n, r, H) and b (n, N, r), got {tuple(x.shape)}, {tuple(a.shape)} and {tuple(b.shape)}")
     (T, H), (n, r), N = x.shape, a.shape[:2], b.shape[1]
@@ -120,4 +121,6 @@ def adapter_linear(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, permutatio
             x.data_ptr(), x.stride(0), a.data_ptr(), b.data_ptr(), ptr(scale), ptr(base), base_ld, out.data_ptr(),
             base_ld if inplace else N, _TYPES[x.dtype], offset.data_ptr(), count.data_ptr(), row.data_ptr(), pair.data_ptr(), T, rows, H, N, n, r, align,
             _lib.device_state(dev).status.data_ptr(), stream_ptr(dev)), "adapter_linear")
+    if inplace:  # (the library writes through an address, which autograd does not see; tensors of inference mode have no count, and that is no error)
+        increment_version(base)
     return out

@@ -138,6 +138,34 @@ def test_in_place_into_a_slice(built_library, T, align, N):
     assert torch.equal(qkv, before) and got.data_ptr() == qkv[:, N:].data_ptr()
 
 
+def test_in_place_counts_as_a_change(built_library):
+    """What autograd has saved of a base that is added to in place is no longer what a backward pass needs: it refuses, as after base.add_()."""
+    import sonicmoe
+
+    x, a, b, idx, base, scale = make(40, 64, 48, 5, 16, torch.bfloat16)
+    p = sonicmoe.adapter_permutation(idx, 5)
+    y = base.clone().requires_grad_().sigmoid()
+    version = y._version
+    sonicmoe.adapter_linear(x, a, b, p, base=y.detach(), scale=scale)
+    assert y._version == version
+    y.sum().backward(retain_graph=True)
+    sonicmoe.adapter_linear(x, a, b, p, base=y.detach(), scale=scale, inplace=True)
+    assert y._version == version + 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    leaf = base.clone().requires_grad_()
+    w = torch.ones(48, dtype=base.dtype, device="cuda")
+    z, h = sonicmoe.rms_norm(leaf, w, residual=base)
+    with torch.no_grad():  # the first half of the columns alone
+        sonicmoe.adapter_linear(x, a, b[:, :24].contiguous(), p, base=h[:, :24], scale=scale, inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
+    with torch.inference_mode():  # tensors without a count, and those of outside
+        for own in (base.clone(), base):
+            want = sonicmoe.adapter_linear(x, a, b, p, base=own, scale=scale)
+            assert torch.equal(sonicmoe.adapter_linear(x, a, b, p, base=own, scale=scale, inplace=True), want)
+
+
 @pytest.mark.parametrize("T,n,r", [(30, 4, 16), (900, 40, 16), (4400, 5, 16), (4400, 5, 64)])
 def test_in_place_into_the_rows_that_are_read(built_library, T, n, r):
     import sonicmoe
