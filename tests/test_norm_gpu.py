@@ -240,6 +240,29 @@ def test_gradients_over_many_rows(built_library):
         assert torch.equal(again[0], dx) and torch.equal(again[1], dw)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,pitch,offset", [(64, 0, 0), (64, 3, 1), (4096, 0, 0), (32768, 0, 0), (32768, 3, 1)])
+def test_gradients_of_rows_whose_root_squared_leaves_the_range(built_library, dtype, H, pitch, offset):
+    """eps 0 and rows of 1 to 3 times 2^-66: r is some 2^65 and r^2 past fp32's range, dx some 2^65.  The squares are whole multiples of 2^-132, their
+    mean one of 2^-147, at most 9 H of them, which fp32 holds: sums and mean are exact, and the bounds of other rows hold."""
+    import sonicmoe
+
+    T = 5
+    g = torch.Generator().manual_seed(1)
+    x = source(T, H, dtype, 1, pitch, offset)
+    x.copy_(torch.randint(1, 4, (T, H), generator=g) * (2 * torch.randint(0, 2, (T, H), generator=g) - 1) * 2.0 ** -66)
+    x.requires_grad_()
+    w, dy = weights(H, dtype, 2).requires_grad_(), source(T, H, dtype, 3)
+    y = sonicmoe.rms_norm(x, w, 0.0)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    check_y(y.detach(), plain(x.detach(), w.detach(), 0.0)[0], H)
+    want, size, want_dw, size_dw = plain_gradients(x.detach(), w.detach(), 0.0, None, dy, None)
+    bound = (3 * chain(H) + 10 * U) * size
+    assert ((dx.double() - want).abs() <= bound + half_step(dtype, want.abs() + bound)).all()
+    bound = ((T + 34) * U + chain(H) + 3 * U) * size_dw
+    assert ((dw.double() - want_dw).abs() <= bound + half_step(dtype, want_dw.abs() + bound)).all()
+
+
 def test_gradients_against_differences(built_library):
     """fp32 differences of the loss <y, a> + <h, b> along random directions, by 64-bit evaluations of the formula."""
     import sonicmoe
