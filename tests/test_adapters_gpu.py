@@ -196,6 +196,63 @@ def test_loads(built_library, T, align):
         check(sonicmoe.adapter_linear(x, a, b, p, base=base, scale=scale), x, a, b, idx, base, scale)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,H,N,n,r", [(2048, 136, 264, 512, 64), (8192, 264, 136, 256, 32), (4400, 72, 96, 4096, 16), (4200, 131, 257, 300, 128),
+                                       (6000, 264, 201, 700, 128), (3000, 520, 264, 2000, 8)])
+def test_few_adapters_of_many_in_use(built_library, dtype, T, H, N, n, r):
+    """Long prompts of eight requests, one without an adapter, with hundreds of adapters to choose from."""
+    import sonicmoe
+
+    x, a, b, _, base, scale = make(T, H, N, n, r, dtype)
+    g = torch.Generator().manual_seed(6)
+    request = torch.randint(0, 8, (T,), generator=g).sort().values
+    idx = torch.randperm(n, generator=g)[:8].index_fill_(0, torch.tensor([5]), -1)[request].to(torch.int32).cuda()
+    p = sonicmoe.adapter_permutation(idx, n)
+    check(sonicmoe.adapter_linear(x, a, b, p, base=base, scale=scale), x, a, b, idx, base, scale)
+    check(sonicmoe.adapter_linear(x, a, b, p), x, a, b, idx, None, None)
+
+
+def test_two_threads(built_library):
+    """Calls of two host threads, each on a stream of its own."""
+    import threading
+
+    import sonicmoe
+
+    inputs = [make(T, 200, 136, 6, r, torch.float16, seed=T) for T, r in ((50, 16), (4400, 64))]
+    x = [i[0] for i in inputs]
+    w = torch.ones(200, dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(k):
+        try:
+            xk, a, b, idx, base, scale = inputs[k]
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    leaf = xk.detach().clone().requires_grad_()
+                    y = sonicmoe.rms_norm(leaf, w)
+                    g, = torch.autograd.grad(y, leaf, xk)
+                    out = sonicmoe.adapter_linear(xk, a, b, sonicmoe.adapter_permutation(idx, 6), base=base, scale=scale)
+            stream.synchronize()
+            got[k] = (y.detach(), g, out)
+        except Exception as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for k, (xk, a, b, idx, base, scale) in enumerate(inputs):
+        leaf = x[k].detach().clone().requires_grad_()
+        y = sonicmoe.rms_norm(leaf, w)
+        g, = torch.autograd.grad(y, leaf, x[k])
+        assert torch.equal(got[k][0], y) and torch.equal(got[k][1], g)
+        check(got[k][2], xk, a, b, idx, base, scale)
+
+
 @pytest.mark.parametrize("T,align", [(30, 16), (4400, 64)])
 def test_tokens_dropped_after_the_sort(built_library, T, align):
     import sonicmoe

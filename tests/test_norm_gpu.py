@@ -240,6 +240,25 @@ def test_gradients_over_many_rows(built_library):
         assert torch.equal(again[0], dx) and torch.equal(again[1], dw)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,H", [(3000, 2049), (3000, 1005), (200000, 10), (1500, 7169), (1300, 8197), (1300, 16389), (3000, 2056), (150000, 24), (1300, 16400)])
+def test_gradients_of_many_rows_of_every_type(built_library, dtype, T, H):
+    """Several rows of a thread, which start anywhere or on 16-byte boundaries, with a residual and an upstream gradient of h."""
+    import sonicmoe
+
+    x, res, w = source(T, H, dtype, 1).requires_grad_(), source(T, H, dtype, 2).requires_grad_(), weights(H, dtype, 3).requires_grad_()
+    dy, dh = source(T, H, dtype, 4), source(T, H, dtype, 5)
+    dx, dres, dw = torch.autograd.grad(sonicmoe.rms_norm(x, w, EPS, residual=res), (x, res, w), (dy, dh))
+    want, size, want_dw, size_dw = plain_gradients(x.detach(), w.detach(), EPS, res.detach(), dy, dh)
+    bound = (3 * chain(H) + 10 * U) * size
+    assert ((dx.double() - want).abs() <= bound + half_step(dtype, want.abs() + bound)).all() and torch.equal(dx, dres)
+    # as in test_gradients_over_many_rows, and the weight's own type
+    bound = ((min(T, T / 148 + 400) + 34) * U + chain(H) + 3 * U) * size_dw
+    assert ((dw.double() - want_dw).abs() <= bound + half_step(dtype, want_dw.abs() + bound)).all()
+    again = torch.autograd.grad(sonicmoe.rms_norm(x, w, EPS, residual=res), (x, res, w), (dy, dh))
+    assert torch.equal(again[0], dx) and torch.equal(again[2], dw)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("H,pitch,offset", [(64, 0, 0), (64, 3, 1), (4096, 0, 0), (32768, 0, 0), (32768, 3, 1)])
 def test_gradients_of_rows_whose_root_squared_leaves_the_range(built_library, dtype, H, pitch, offset):
