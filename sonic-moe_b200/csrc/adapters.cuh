@@ -146,10 +146,6 @@ __device__ __forceinline__ int gathered_of(const Params& p, int row) {
   const int t = p.gather[row];
   return static_cast<unsigned>(t) < static_cast<unsigned>(p.T) ? t : -1;
 }
-__device__ __forceinline__ int token_of(const Params& p, int row) {
-  const int t = gathered_of(p, row);
-  return t >= 0 && p.reverse[t] == row ? t : -1;
-}
 
 // The `tile`-th tile's adapter, first row and end, adapters in their order (all lanes of the warp); adapter -1 behind the last.  Each lane counts
 // the tiles of a run of adapters; then the lanes look at the run that holds the tile.

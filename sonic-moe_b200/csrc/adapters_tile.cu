@@ -669,7 +669,10 @@ template <class T, int RP>
 static int launch_rank(const Params& p, bool wide_in, bool wide_out, int warps, long long blocks, cudaStream_t st) {
   // (tcgen05 / mma.sync, us, 8192 tokens, 4096 x 4096, 8 adapters, rank 16: 59 / 46, 32: 60 / 50, 64: 63.5 / 64, 128: 121 / 129; 4095 columns of out, rank 16:
   // 84 / 86, 64: 88 / 123, 128: 184 / 390; 2048 tokens of one adapter, rank 64: 30 / 36)
-  if (wide_in && warps == kWarps && (RP >= 64 || !wide_out)) return wide_out ? launch_tensor<T, RP, true>(p, blocks, st) : launch_tensor<T, RP, false>(p, blocks, st);
+  if (wide_in && warps == kWarps) {
+    if (!wide_out) return launch_tensor<T, RP, false>(p, blocks, st);
+    if constexpr (RP >= 64) return launch_tensor<T, RP, true>(p, blocks, st);
+  }
   return wide_in && wide_out ? launch_tile<T, RP, true>(p, warps, blocks, st) : launch_tile<T, RP, false>(p, warps, blocks, st);
 }
 template <class T>

@@ -78,7 +78,7 @@ __device__ __forceinline__ void quantise(const i8::RowScale& s, float (&f)[8], u
 // times r is that of |y|, whatever is rounded on the way, so that one reduction serves both.
 template <class T, class W, int EP, bool ALIGNED, bool Q>
 struct Finish {
-  static constexpr int VE = kValues<T>, P = EP / VE;
+  static constexpr int VE = kValues<T>;
   float r;
   i8::RowScale s;
   __device__ __forceinline__ Finish(const Forward& a, long long row, float sum, float most, bool writes) {
