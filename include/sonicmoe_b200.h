@@ -513,7 +513,7 @@ int smoe_rms_norm(const void* x, long long ld, const void* residual, long long r
                   long long rows, int H, float eps, void* stream);
 /* With u = h rstd and g = dy weight: dx = dh + rstd (g - u mean(g u)) (the residual's gradient too), dweight = sum over the rows of
  * dy u.  dh (the upstream gradient of h): NULL for none.  dx packed and 16-byte aligned, dweight of the weight's type; either may be NULL.  With dweight,
- * workspace: smoe_rms_norm_backward_workspace_bytes bytes, 16-byte aligned.  The same bits every time. */
+ * workspace: smoe_rms_norm_backward_workspace_bytes bytes, 16-byte aligned.  The same bits every time.  No output overlaps an input. */
 size_t smoe_rms_norm_backward_workspace_bytes(long long rows, int H);
 int smoe_rms_norm_backward(const void* dy, long long dy_ld, const void* dh, long long dh_ld, const void* h, long long h_ld,
                            const void* weight, int weight_dtype, const float* rstd, void* dx, void* dweight, int dtype,

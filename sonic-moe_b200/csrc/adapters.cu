@@ -210,9 +210,13 @@ static long long tiles_of(int T, int n, int rows) {
   const long long tiles = T / rows + static_cast<long long>(n < T ? n : T);
   return tiles < T ? tiles : T;
 }
+// The rules below go by the adapters that there are, since the host does not know how many of them the tokens use: where that is a few of many, they take tiles
+// for fewer rows than there are.  8192 tokens of 8 requests, 4096 x 4096, rank 64, 56 / 71 / 109 us with 8 / 64 / 512 adapters to choose from, 2048 tokens
+// 30 / 33 / 94; of 12, rank 16, 42 with 8, 63 with 512.
 // Tiles of 16 rows and eight blocks each: while few of them are needed, more for wide rows, and where it is the weights of adapters with a few tokens each
 // that take the time, which come straight from memory there.  us by few_kernel / by tiles, 4096 x 4096 unless said: 256 tokens of 2 adapters, rank 16,
-// 7 / 14; 512 of 8, rank 64, 13 / 20; 512 of 4, rank 64, 14 / 21, 1024 x 1024 13 / 12; 2048 of 4, rank 16, 21 / 21, 1024 x 1024 14 / 10; 64 of 64, rank
+// 7 / 14; 512 of 8, rank 64, 13 / 20 with 64 tokens each, 20 / 20 drawn at random (37 tiles of eight blocks are what 148 SMs hold at a time at rank 64; the
+// tokens then fill 36 to 39); 512 of 4, rank 64, 14 / 21, 1024 x 1024 13 / 12; 2048 of 4, rank 16, 21 / 21, 1024 x 1024 14 / 10; 64 of 64, rank
 // 128, 41 / 54, 4097 x 4095 68 / 310; 512 of 100, rank 64, 27 / 31, rank 128, 64 / 56, 4097 x 4095 118 / 346; 4096 of 500, rank 64, 132 / 107, 4097 x
 // 4095, rank 128, 524 / 1219; 448 of 160, 342 x 187, rank 16, 31 / 16.
 // Of those, the ones with tcgen05.mma need fewer (wide_in, rows of out that start anywhere: 2048 of 100, rank 128, 247 / 121, 512 of 100, rank 64, 65 / 57,

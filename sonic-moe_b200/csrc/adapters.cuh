@@ -2,7 +2,7 @@
 //   out[t] = base[t] + scale[e] b[e] (a[e] x[t]),   a (n, r, H), b (n, N, r);   out[t] = base[t] where t has none
 // (base NULL: zeros).  Tokens are sorted by adapter, e's rows starting at a multiple of `align` (smoe_token_permutation), so that a tile of 16
 // to `align` rows has one adapter.  x, base and out are met once each: between 20 and 200 operations for a byte of them, so that
-// memory bounds all of this.
+// memory is the floor of all of this.  The kernels do not reach it: what holds each of them up is written there.
 //
 // The inner product is fp32: every warp's part by the tensor core's fp32 sums, the parts added in the same order every time.  s = scale[e] (a x) goes on
 // as two 16-bit numbers, its leading bits and the rest (16 bits of s for bf16; 22 for fp16, after a row of s was multiplied by a power of two,

@@ -129,9 +129,10 @@ __device__ __forceinline__ void share_sums(const Params& p, const float* part, i
   }
 }
 
-// Bound by memory, in rows of 128 bytes at a time: 8192 tokens, 4096 x 4096, 8 adapters, bf16 with a base 41 us at rank 16 (4.9 TB/s), 47 at rank 32; a
-// kernel that only reads and writes rows in this order (three stages of 128 bytes of each, clusters of four) takes 17 + 27 us for the two halves.  Rows that
-// start anywhere: 2048 tokens of 100 adapters, 4097 x 4095, rank 32 66 us, of 27 on 4096 x 4096.
+// Bound by how a block's rows come and go, 128 bytes at a time in two phases one after the other: 8192 tokens, 4096 x 4096, 8 adapters, bf16 with a base 41 us
+// at rank 16 (4.9 TB/s; DRAM 46 % busy in a single cold launch), 47 at rank 32; a kernel that only reads and writes rows in this order (three
+// stages of 128 bytes of each, clusters of four) takes 17 + 27 us for the two halves.  Rows that start anywhere: 2048 tokens of 100 adapters, 4097 x 4095, rank 32 66
+// us, of 27 on 4096 x 4096: weights go through registers, without the ring's lead.
 template <class T, int RP, bool ALIGNED>
 __global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) tile_kernel(const Params p) {
   release_next();
@@ -328,7 +329,8 @@ __global__ void __launch_bounds__(32 * kWarps, RP <= 64 ? 2 : 1) tile_kernel(con
 // product is on the tensor core while the last one's 32 rows by 32 columns of each warp are added to base and go out.
 // WIDE: rows of base and out are whole 16-byte pieces.  Otherwise each half of the warps has a run of columns of its own, so that what of a row's results
 // does not fill a 16-byte block of out waits in the row's thread for the next ones; base comes in by the blocks that hold it.
-// Bound by memory up to rank 64: 8192 tokens, 4096 x 4096, 8 adapters 56 us (3.7 TB/s, 153 TFLOP/s), 4095 columns of out 83; 32768 tokens 182 us, 4.5 TB/s.
+// 8192 tokens, 4096 x 4096, 8 adapters, rank 64 56 us (3.7 TB/s, 153 TFLOP/s; DRAM 34 % and the tensor pipe 14 % busy: it is the phases one after the other
+// that take the time), 4095 columns of out 83; 32768 tokens 182 us, 4.5 TB/s.
 // Of a block's time 30 and 45 thousand cycles are the two products, at the rate at which their rows come and go, 9 the sums' way over the cluster, 5 the
 // start.  Rank 128, one block to an SM for its s: 119 us.
 template <int RP, bool WIDE>

@@ -7,7 +7,9 @@
     z = int8.int8_linear(r.q, wq, w_scale, x_scale=r.scale)
 
 y = h / sqrt(mean(h^2) + eps) * weight over the last dimension.  h is rounded to the type of x once, and y is the norm of that h; the
-sum of squares and everything up to y's one rounding is fp32 (squares past its range, of values above 1.8e19, make a row zeros).  The 8-bit
+sum of squares and everything up to y's one rounding is fp32.  So are products of two of h, weight and the gradients: h weight is formed before
+it is multiplied by the root.  Squares past fp32's range, of values above 1.8e19, make a row zeros; where eps is 0, or below 1e-38 (it is taken as
+fp32 too), squares of values below 1e-19 lose bits, and rows of values below 1e-23 have none left: their root is infinite, and so are they.  The 8-bit
 rows are those of the unrounded y: scale = amax / 127, values rounded half to even, as `int8.quantize_rows` makes them of fp32 rows (of bf16
 and fp16 x by one multiply-add: a value within 1.6e-5 of a step of a border may go to the other side).  They are what `int8.int8_linear` and
 `int8.moe_int8_softmax_topk_layer` take as x and x_q.
